@@ -250,11 +250,105 @@ LLMX_API llmx_status llmx_ipc_free(void *ptr);
 LLMX_API llmx_status llmx_convert(const void *src, int32_t src_dtype, void *dst, int32_t dst_dtype, size_t n,
                                   void *stream);
 
+/* ------------------------------------------------------------------------
+ * Key/value cache held in 4 bits.  No counterpart in the reference (it has
+ * no cache).  K and V (fp16 / bf16, head_dim 64, 128 or 256) are quantised
+ * in groups of LLMX_KV4_GROUP channels of one (token, kv head), each with a
+ * step s and a minimum m held in the type T of K and V:
+ *   m = min x,  r = fl32(fl32(max x - m) / 15),  s = the smallest T >= r,
+ *   n = min(15, rint(fl32(fl32(x - m) / s)))  (0 where s = 0),
+ *   value = n s + m.
+ * A group with a NaN or an infinity in it (or, for bf16, a range max x - m
+ * past fp32) reads back as NaN.  4.5 bits a value: 18 * head_dim bytes per
+ * 16 tokens of K and V of one kv head.
+ *
+ * The cache is made of pages of page_size tokens (a multiple of 16).  Page p,
+ * kv head h starts at data + p * page_stride + h * head_stride and holds
+ * page_size / 16 tiles of 18 * head_dim bytes, one after the other.  A tile is
+ * [K codes, 8 * head_dim][V codes, 8 * head_dim][parameters, 2 * head_dim].
+ * Codes are 32-bit words of 8 consecutive channels, channel c of the word in
+ * bits 4c .. 4c + 3.  Word x of lane (g, t) (g < 8, t < 4) lies at byte
+ * (x / 4) * 512 + (4 g + t) * 16 + (x % 4) * 4 of its section, where with
+ * G = head_dim / 64
+ *   K: x = (r * G + h) * 2 + w     token 8 r + g, channels 64 h + 16 t + 8 w ..
+ *   V: x = (2 a + c) * G + h       token 8 a + 2 t + c, channels 64 h + 8 g ..
+ * which is the order of the matrix fragments that the attention kernel feeds
+ * to the tensor cores, so a tile is read with whole 16-byte loads.  The
+ * parameters are [16 tokens][K, V][G][s, m] in T.
+ *
+ * Token j of sequence b lies in page block_table[b * table_stride + j /
+ * page_size] (NULL: page b * max_pages + j / page_size).  Entries that hold
+ * no token of the sequence are not read.  An entry outside [0, n_pages), or a
+ * position outside [0, max_pages * page_size), is skipped, never followed: a
+ * store drops those rows, a load writes 0 for them, the attention does not
+ * see them, and llmx_attn_device_status then returns
+ * LLMX_ERR_INVALID_ARGUMENT.  Two rows stored to the same place by one call
+ * leave an undefined mix of both there. */
+#define LLMX_KV4_GROUP 64
+#define LLMX_KV4_TILE_TOKENS 16
+typedef struct llmx_kv4_cache {
+  int32_t dtype;      /* llmx_dtype of K and V: fp16 or bf16              */
+  int32_t n_kv_heads; /* >= 1                                             */
+  int32_t head_dim;   /* 64, 128 or 256                                   */
+  int32_t page_size;  /* tokens, a multiple of 16                         */
+  int32_t n_pages;    /* >= 1                                             */
+  int32_t max_pages;  /* pages of one sequence (columns of block_table);
+                         max_pages * page_size <= 2^30                    */
+  void *data;         /* device, 16-byte aligned                          */
+  int64_t page_stride; /* bytes, multiples of 16                          */
+  int64_t head_stride;
+  const int32_t *block_table; /* device [batch, max_pages] or NULL        */
+  int64_t table_stride;       /* elements between its rows                */
+} llmx_kv4_cache;
+
+/* Rows of K and V outside the cache: [batch, max_rows, n_kv_heads, head_dim]
+ * by element strides {batch, row, head}, unit stride on head_dim.  Row i <
+ * lens[b] (NULL: max_rows; clamped to [0, max_rows]) is token start[b] + i
+ * (NULL: i) of sequence b. */
+typedef struct llmx_kv4_rows {
+  int32_t batch;
+  int32_t max_rows;
+  void *k;
+  void *v;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  const int32_t *start; /* device [batch] or NULL                         */
+  const int32_t *lens;  /* device [batch] or NULL                         */
+} llmx_kv4_rows;
+
+/* Bytes of one page of one kv head (the least head_stride). */
+LLMX_API llmx_status llmx_kv4_page_bytes(int32_t head_dim, int32_t page_size, int64_t *bytes);
+
+/* Quantises the rows of K and V into the cache (a prompt's, or one new token's
+ * per sequence).  Nothing else of the cache changes. */
+LLMX_API llmx_status llmx_kv4_store(const llmx_kv4_cache *c, const llmx_kv4_rows *rows, void *stream);
+
+/* Reads rows of the cache back (n s + m in fp32, rounded to T) into k and v;
+ * rows at or past lens[b] are written as 0. */
+LLMX_API llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_rows *rows, void *stream);
+
+/* llmx_attn_fwd over the cache instead of dense K / V: same request, masks
+ * and results (p->k, p->v and their strides are ignored; p->dtype, n_kv_heads
+ * and head_dim must match the cache; p->max_kv_len <= max_pages * page_size
+ * bounds kv_lens; kv_offset / kv_total must be 0).  p->algo:
+ *   DECODE  reads the 4-bit tiles directly, in one pass per 8 to 32 (head,
+ *           query row) pairs of a kv head; any max_q_len, any q / o alignment.
+ *           The values n s + m are used unrounded.
+ *   TCGEN05 expands the sequences into the workspace (values rounded to T)
+ *           and runs the tensor-core prefill on them; needs its workspace.
+ *   AUTO    DECODE, or for long query blocks TCGEN05 where it can run.
+ * A call on the DECODE path given too little workspace runs without
+ * splitting the keys. */
+LLMX_API llmx_status llmx_kv4_attn_workspace_size(const llmx_attn_params *p, const llmx_kv4_cache *c, size_t *bytes);
+LLMX_API llmx_status llmx_kv4_attn_fwd(const llmx_attn_params *p, const llmx_kv4_cache *c, void *stream);
+
 /* Which kernel family llmx_attn_fwd would run for *p (an llmx_attn_algo). */
 LLMX_API llmx_status llmx_attn_select_algo(const llmx_attn_params *p, int32_t *algo);
 
 /* Synchronises `device` and reads (and optionally clears) its device-side
- * error word: LLMX_ERR_TIMEOUT if any kernel gave up on a bounded wait. */
+ * error word: LLMX_ERR_TIMEOUT if any kernel gave up on a bounded wait,
+ * LLMX_ERR_INVALID_ARGUMENT if a 4-bit cache was given a page or position
+ * outside it. */
 LLMX_API llmx_status llmx_attn_device_status(int32_t device, int32_t clear);
 
 LLMX_API const char *llmx_status_string(llmx_status s);

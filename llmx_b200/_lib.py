@@ -91,6 +91,39 @@ class RowScatter(ctypes.Structure):
     ]
 
 
+class Kv4Cache(ctypes.Structure):
+    """Mirror of ``llmx_kv4_cache``."""
+
+    _fields_ = [
+        ("dtype", _i32),
+        ("n_kv_heads", _i32),
+        ("head_dim", _i32),
+        ("page_size", _i32),
+        ("n_pages", _i32),
+        ("max_pages", _i32),
+        ("data", _vp),
+        ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("block_table", _vp),
+        ("table_stride", ctypes.c_int64),
+    ]
+
+
+class Kv4Rows(ctypes.Structure):
+    """Mirror of ``llmx_kv4_rows``."""
+
+    _fields_ = [
+        ("batch", _i32),
+        ("max_rows", _i32),
+        ("k", _vp),
+        ("v", _vp),
+        ("k_stride", _i64x3),
+        ("v_stride", _i64x3),
+        ("start", _vp),
+        ("lens", _vp),
+    ]
+
+
 IPC_HANDLE_BYTES = 64
 
 # Every function include/llmx_attn.h declares: name -> (restype, argtypes).
@@ -115,6 +148,14 @@ SIGNATURES = {
     "llmx_ipc_open": (_i32, [_vp, ctypes.POINTER(_vp)]),
     "llmx_ipc_close": (_i32, [_vp]),
     "llmx_ipc_free": (_i32, [_vp]),
+    "llmx_kv4_page_bytes": (_i32, [_i32, _i32, ctypes.POINTER(ctypes.c_int64)]),
+    "llmx_kv4_store": (_i32, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Rows), _vp]),
+    "llmx_kv4_load": (_i32, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Rows), _vp]),
+    "llmx_kv4_attn_workspace_size": (
+        _i32,
+        [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache), ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "llmx_kv4_attn_fwd": (_i32, [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache), _vp]),
     "llmx_convert": (_i32, [_vp, _i32, _vp, _i32, ctypes.c_size_t, _vp]),
     "llmx_attn_device_status": (_i32, [_i32, _i32]),
     "llmx_status_string": (ctypes.c_char_p, [_i32]),

@@ -30,7 +30,8 @@ NVCC_FLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
 # Kernel and C-ABI units export only what include/llmx_attn.h marks LLMX_API;
 # the C++ Tensor / attention API units export their whole public surface.
 HIDDEN = ["-Xcompiler", "-fvisibility=hidden"]
-SOURCES = ["attn_api.cu", "attn_simt.cu", "attn_decode.cu", "attn_sm100.cu", "attn_merge.cu", "llmx_convert.cu",
+SOURCES = ["attn_api.cu", "attn_simt.cu", "attn_decode.cu", "attn_sm100.cu", "attn_merge.cu", "attn_kv4.cu",
+           "kv4_cache.cu", "llmx_convert.cu",
            "llmx_tensor.cu", "attention_api.cu", "llmx_ops.cu"]
 # The C++ Tensor / attention / registry units; every other unit is compiled hidden.
 CXX_API_UNITS = ("llmx_tensor.cu", "attention_api.cu", "llmx_ops.cu")

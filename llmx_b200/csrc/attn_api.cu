@@ -208,6 +208,24 @@ llmx_status prepare_decode_request(const llmx_attn_params *p, AttnArgs *a) {
 
 llmx_status record_error(llmx_status s, const char *msg) { return fail(s, msg); }
 
+llmx_status validate_without_kv(const llmx_attn_params *p, AttnArgs *a) {
+  if (p == nullptr) return fail(LLMX_ERR_INVALID_ARGUMENT, "params is NULL");
+  llmx_attn_params q = *p;
+  q.k = q.v = q.q;
+  for (int i = 0; i < 3; ++i) q.k_stride[i] = q.v_stride[i] = 0;
+  return validate(&q, a);
+}
+
+llmx_status current_device_info(unsigned int **err, int *num_sms) {
+  int dev = 0;
+  const DeviceInfo *info = nullptr;
+  const llmx_status s = current_device(&dev, &info);
+  if (s != LLMX_OK) return s;
+  *err = info->err;
+  *num_sms = info->num_sms;
+  return LLMX_OK;
+}
+
 }  // namespace llmx_b200
 
 using namespace llmx_b200;
@@ -421,6 +439,8 @@ llmx_status llmx_attn_device_status(int32_t device, int32_t clear) {
   if (e != cudaSuccess) return fail(LLMX_ERR_CUDA, cudaGetErrorString(e));
   if (word & kDevErrTimeout) return fail(LLMX_ERR_TIMEOUT, "a device-side bounded wait expired");
   if (word & kDevErrTmemAlloc) return fail(LLMX_ERR_TIMEOUT, "tensor-memory allocation timed out");
+  if (word & kDevErrBadPage)
+    return fail(LLMX_ERR_INVALID_ARGUMENT, "a 4-bit cache was given a page or position outside it");
   return LLMX_OK;
 }
 
