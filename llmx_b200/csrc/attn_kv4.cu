@@ -36,6 +36,7 @@
 #include <string>
 
 #include "kv4.cuh"
+#include "sm100_ptx.cuh"
 
 namespace llmx_b200 {
 namespace {
@@ -47,8 +48,14 @@ constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum of a row moves only when a score passes it by this
 // much (log2): p reaches 2^6 at most, and p s at most 2^14 in fp16.
 constexpr float kLazyMax = 6.f;
-constexpr int kStepExp = 7;      // the largest s is scaled to [2^7, 2^8)
-constexpr int kMinStepExp = -100;
+// The largest weight times the largest step stays in [2^7, 2^8) (times 2^6
+// under a lazy maximum): fp16 then keeps 11 bits of weights down to 2^-21 of
+// the largest.  Steps count from 2^-40 on (smaller ones lose bits from 2^-61
+// on), which keeps the sums of scaled weights inside fp32.
+constexpr int kStepExp = 7;
+constexpr int kMinStepExp = -40;
+constexpr int kMaxStepExp = 125;
+constexpr uint64_t kWaitNs = 1000000000ull;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -117,54 +124,57 @@ __device__ __forceinline__ int first_token(const AttnArgs &a, int ql, int kl) {
   return lo & ~15;
 }
 
-// One lane's share of a tile of 16 tokens.
-template <int G>
-struct Tile {
-  uint4 k[G], v[G];
-  uint32_t par[2][2 * G];  // [token g, g + 8][K groups, V groups]
-};
-
-template <int G>
-__device__ __forceinline__ void load_tile(Tile<G> &t, const unsigned char *p, int lane) {
-#pragma unroll
-  for (int i = 0; i < G; ++i) t.k[i] = ld_stream16(p + i * 512 + lane * 16);
-#pragma unroll
-  for (int i = 0; i < G; ++i) t.v[i] = ld_stream16(p + G * 512 + i * 512 + lane * 16);
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const unsigned char *q = p + G * 1024 + ((lane >> 2) + 8 * r) * (8 * G);
-    if constexpr (G == 1) {
-      const uint2 u = *reinterpret_cast<const uint2 *>(q);
-      t.par[r][0] = u.x;
-      t.par[r][1] = u.y;
-    } else {
-#pragma unroll
-      for (int i = 0; i < G / 2; ++i) {
-        const uint4 u = ld_stream16(q + i * 16);
-        t.par[r][4 * i] = u.x;
-        t.par[r][4 * i + 1] = u.y;
-        t.par[r][4 * i + 2] = u.z;
-        t.par[r][4 * i + 3] = u.w;
-      }
-    }
-  }
-}
-
 __device__ __forceinline__ uint32_t word_of(const uint4 &u, int i) {
   return i == 0 ? u.x : (i == 1 ? u.y : (i == 2 ? u.z : u.w));
 }
 
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
+  return r;
+}
+
+// One contiguous tile, global -> this CTA's shared memory, counted on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+               : "memory");
+}
+
+// Sizes of one variant: 8 * NT pairs of head_dim D.
+template <int D, int NT>
+struct Shape {
+  static constexpr int G = D / kKv4Group;
+  static constexpr int R = 8 * NT;
+  static constexpr int LDO = D + 4;  // padded row of the merge buffer
+  static constexpr int kTile = 18 * D;
+  static constexpr int kStages = D == 64 ? 6 : (D == 128 ? 4 : 3);
+  // q fragments and row factors stay in registers where they are few.
+  static constexpr bool kQRegs = NT * G <= 2;
+  static constexpr int kMinCtas = NT * G <= 2 ? 4 : (NT * G <= 4 ? 3 : 2);
+  static constexpr size_t kRing = (size_t)kWarps * kStages * kTile;
+  static constexpr size_t kMerge = (size_t)kWarps * R * LDO * sizeof(float);
+  static constexpr size_t kRingOrMerge = kRing > kMerge ? kRing : kMerge;
+  static constexpr size_t kQFrag = (size_t)NT * G * 2 * 32 * 16;
+  static constexpr size_t kSmem = kRingOrMerge + kQFrag;
+};
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args c, int chunk, int n_splits, int row_blocks,
-                                                            float *part_o, float *part_lse) {
-  constexpr int G = D / kKv4Group;
-  constexpr int R = 8 * NT;
-  constexpr int LDO = D + 4;
-  extern __shared__ __align__(16) unsigned char smem[];
-  __half *sm_q = reinterpret_cast<__half *>(smem);            // [R][D]
-  float *sm_o = reinterpret_cast<float *>(smem);              // [kWarps][R][LDO], after the loop
-  __shared__ float sm_f[R], sm_qs[R][G];
+__global__ void __launch_bounds__(kThreads, Shape<D, NT>::kMinCtas)
+    kv4_attn_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Kv4Args c, int chunk, int n_splits,
+                    int row_blocks, float *part_o, float *part_lse) {
+  using Sh = Shape<D, NT>;
+  constexpr int G = Sh::G, R = Sh::R, LDO = Sh::LDO, kStages = Sh::kStages;
+  extern __shared__ __align__(128) unsigned char smem[];
+  float *sm_o = reinterpret_cast<float *>(smem);                              // [kWarps][R][LDO], after the loop
+  __half *sm_q = reinterpret_cast<__half *>(smem + Sh::kRingOrMerge);         // fragments of q
+  __shared__ float sm_f[R], sm_qs[G][R], sm_slope[R];
+  __shared__ int sm_lo[R], sm_hi[R];
   __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];
+  __shared__ uint64_t sm_full[kWarps][kStages];
+
+  // The combine kernel may be set up while this one runs.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int split = blockIdx.x;
   const int kvh = blockIdx.y / row_blocks;
@@ -177,14 +187,16 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args 
   const int ql = clamp_len(a.q_lens, b, a.Sq);
   const int kl = clamp_len(a.kv_lens, b, a.Skv);
 
-  // Tokens of this split that some row of the block sees.
-  int t_lo = 0, t_hi = 0;
+  // Tokens of this split that some row of the block sees, and the ones
+  // [lo_in, hi_in) that all of its rows see (the rows' ranges move one way:
+  // the last row's begin, the first row's end).
+  int t_lo = 0, t_hi = 0, lo_in = 0, hi_in = 0;
   {
     const int i0 = r0 / a.group, i1 = min(min(r0 + R, rows) - 1, ql * a.group - 1) / a.group;
     if (i0 < ql && kl > 0) {
-      int lo0, hi0, lo1, hi1;
-      row_range(a, i0, ql, kl, lo0, hi0);
-      row_range(a, i1, ql, kl, lo1, hi1);
+      int lo0, hi1;
+      row_range(a, i0, ql, kl, lo0, hi_in);
+      row_range(a, i1, ql, kl, lo_in, hi1);
       const int s0 = first_token(a, ql, kl) + split * chunk;
       t_lo = max(lo0, s0);
       t_hi = min(hi1, s0 + chunk);
@@ -200,8 +212,11 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args 
     return;
   }
 
+  // Weights are kept as 2^(S - ref) with one reference per row: the running
+  // maximum less a power of two that brings the largest step times the
+  // largest weight into fp16's upper range (kRoom below).
   float o[NT][G][4][4];
-  float l[NT][2], aff[NT][2][G], mx[NT][2];
+  float l[NT][2], aff[NT][2][G], ref[NT][2];
   int step_exp = kMinStepExp;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -214,26 +229,69 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args 
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       l[n][q] = 0.f;
-      mx[n][q] = -CUDART_INF_F;
+      ref[n][q] = -CUDART_INF_F;
 #pragma unroll
       for (int h = 0; h < G; ++h) aff[n][q][h] = 0.f;
     }
   }
 
   if (t_lo < t_hi) {
-    // Query rows to fp16, scaled by a power of two, with the factor that
-    // undoes it and the sums of their groups.  Lane l holds D / 32
-    // consecutive channels.
+    const int tile0 = t_lo >> 4, tile1 = (t_hi + 15) >> 4;
+    const int tpp = c.page_size >> 4;
+    const unsigned char *base = c.data + kvh * c.head_stride;
+    const int mine = tile1 - tile0 > warp ? (tile1 - tile0 - warp + kWarps - 1) / kWarps : 0;  // tiles of this warp
+    const uint32_t ring = sm100::smem_u32(smem) + warp * kStages * Sh::kTile;
+
+    // Lane i of the warp keeps where its tile (32 n + i) lies, and issues
+    // its copy.  Bit i of `bad`: that tile's page is outside the cache.
+    long long where = -1;
+    uint32_t bad_now = 0, bad_issue = 0;
+    auto locate = [&](int first) {
+      const int idx = first + lane;
+      where = -1;
+      if (idx < mine) {
+        const int tile = tile0 + warp + idx * kWarps;
+        const int page = tile / tpp;
+        where = kv4_page_offset(c, b, page);
+        if (where >= 0) where += (long long)(tile - page * tpp) * Sh::kTile;
+      }
+      bad_issue = __ballot_sync(0xffffffffu, idx < mine && where < 0);
+    };
+    auto issue = [&](int i, int stage) {
+      if (lane == i % 32 && where >= 0) {
+        sm100::mbar_arrive_expect_tx(&sm_full[warp][stage], Sh::kTile);
+        bulk_load(ring + stage * Sh::kTile, base + where, Sh::kTile, &sm_full[warp][stage]);
+      }
+    };
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) sm100::mbar_init(&sm_full[warp][i], 1);
+      sm100::fence_mbar_init();
+    }
+    locate(0);
+    bad_now = bad_issue;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kStages; ++i)
+      if (i < mine) issue(i, i);
+
+    // Query rows to fp16, scaled by a power of two, in the order of the
+    // operand fragments, with the factor that undoes the scale and the sums
+    // of their groups.  Lane l holds D / 32 consecutive channels.
     constexpr int E = D / 32;
     for (int r = warp; r < R; r += kWarps) {
       const bool live = r0 + r < rows && (r0 + r) / a.group < ql;
       float x[E];
       float top = 0.f, sum = 0.f;
+      int lo = 0, hi = 0;
+      float slope = 0.f;
       if (live) {
         const int i = (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
         const T *p = static_cast<const T *>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2] + lane * E;
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = Elem<T>::to_f(p[e]);
+        row_range(a, i, ql, kl, lo, hi);
+        if (a.alibi != nullptr) slope = a.alibi[h] * kLog2e;
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -250,74 +308,61 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args 
       const float up = pow2i(min(126, 14 - ex));
       const float scale = a.softcap > 0.f ? a.sm_scale / a.softcap : a.sm_scale * kLog2e;
 #pragma unroll
-      for (int e = 0; e < E; ++e) sm_q[r * D + lane * E + e] = __float2half_rn(x[e] * up);
-      // 2^24 for the subnormals, 2^(ex - 14) for the scaling.
-      if (lane == 0) sm_f[r] = scale * 0x1p24f * pow2i(max(-126, ex - 14));
-      if (lane % (32 / G) == 0) sm_qs[r][lane / (32 / G)] = sum * scale;
+      for (int e = 0; e < E; ++e) {
+        const int d = lane * E + e, p = d & 7;
+        // Channels 0..7 of a word go to halves 0, 2, 4, 6, 1, 3, 5, 7 of the
+        // fragment; the odd ones meet nibbles that are 16 times too large.
+        const int at = ((((r >> 3) * G + (d >> 6)) * 2 + ((d >> 3) & 1)) * 32 + 4 * (r & 7) + ((d >> 4) & 3)) * 8 +
+                       (p & 3) * 2 + (p >> 2);
+        sm_q[at] = __float2half_rn(x[e] * (p & 1 ? up * 0.0625f : up));
+      }
+      if (lane == 0) {
+        // 2^24 for the subnormals, 2^(ex - 14) for the scaling.
+        sm_f[r] = scale * 0x1p24f * pow2i(max(-126, ex - 14));
+        sm_lo[r] = lo;
+        sm_hi[r] = hi;
+        sm_slope[r] = slope;
+      }
+      if (lane % (32 / G) == 0) sm_qs[lane / (32 / G)][r] = sum * scale;
     }
     __syncthreads();
 
-    // Operand fragments of q: 4 registers per 16 channels and column block.
-    uint32_t qf[NT][G][2][4];
-    float fac[NT][2], qs[NT][2][G], slope[NT][2];
-    int lo[NT][2], hi[NT][2];
-    int lo_in = 0, hi_in = 0x7fffffff;  // tokens in [lo_in, hi_in) are seen by every row
+    uint4 qf[Sh::kQRegs ? NT * G * 2 : 1];
+    float2 fac_r[Sh::kQRegs ? NT : 1], qs_r[Sh::kQRegs ? NT * G : 1];
+    const uint32_t q_at = sm100::smem_u32(sm_q) + lane * 16;
+    if constexpr (Sh::kQRegs) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const __half *qr = sm_q + (n * 8 + g) * D;
+      for (int i = 0; i < NT * G * 2; ++i) qf[i] = lds16(q_at + i * 512);
 #pragma unroll
-      for (int h = 0; h < G; ++h)
+      for (int n = 0; n < NT; ++n) {
+        fac_r[n] = *reinterpret_cast<const float2 *>(&sm_f[n * 8 + 2 * t]);
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint4 u = *reinterpret_cast<const uint4 *>(qr + 64 * h + 16 * t + 8 * w);
-          const uint32_t sixteenth = 0x2c002c00u;  // 2^-4, twice
-          const __half2 s16 = *reinterpret_cast<const __half2 *>(&sixteenth);
-          qf[n][h][w][0] = __byte_perm(u.x, u.z, 0x5410);  // channels 0, 4
-          uint32_t x1 = __byte_perm(u.x, u.z, 0x7632);     // channels 1, 5
-          qf[n][h][w][2] = __byte_perm(u.y, u.w, 0x5410);  // channels 2, 6
-          uint32_t x3 = __byte_perm(u.y, u.w, 0x7632);     // channels 3, 7
-          const __half2 y1 = __hmul2(*reinterpret_cast<const __half2 *>(&x1), s16);
-          const __half2 y3 = __hmul2(*reinterpret_cast<const __half2 *>(&x3), s16);
-          qf[n][h][w][1] = *reinterpret_cast<const uint32_t *>(&y1);
-          qf[n][h][w][3] = *reinterpret_cast<const uint32_t *>(&y3);
-        }
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int r = n * 8 + 2 * t + q;
-        fac[n][q] = sm_f[r];
-#pragma unroll
-        for (int h = 0; h < G; ++h) qs[n][q][h] = sm_qs[r][h];
-        const bool live = r0 + r < rows && (r0 + r) / a.group < ql;
-        lo[n][q] = hi[n][q] = 0;
-        if (live) row_range(a, (r0 + r) / a.group, ql, kl, lo[n][q], hi[n][q]);
-        slope[n][q] = a.alibi != nullptr && live ? a.alibi[kvh * a.group + (r0 + r) % a.group] * kLog2e : 0.f;
+        for (int h = 0; h < G; ++h) qs_r[n * G + h] = *reinterpret_cast<const float2 *>(&sm_qs[h][n * 8 + 2 * t]);
       }
     }
-    {
-      // Rows of the block in order: the last one's lo and the first one's hi.
-      const int i0 = r0 / a.group, i1 = min(min(r0 + R, rows) - 1, ql * a.group - 1) / a.group;
-      int x;
-      row_range(a, i1, ql, kl, lo_in, x);
-      row_range(a, i0, ql, kl, x, hi_in);
-    }
 
-    const int tile0 = t_lo >> 4, tile1 = (t_hi + 15) >> 4;
-    const int tpp = c.page_size >> 4;
-    const unsigned char *base = c.data + kvh * c.head_stride;
-    const int mine = tile1 - tile0 > warp ? (tile1 - tile0 - warp + kWarps - 1) / kWarps : 0;  // tiles of this warp
-
-    // Lane i of the warp keeps where its tile (32 n + i) lies.
-    auto locate = [&](int first) -> long long {
-      const int idx = first + lane;
-      if (idx >= mine) return -1;
-      const int tile = tile0 + warp + idx * kWarps;
-      const int page = tile / tpp;
-      const long long off = kv4_page_offset(c, b, page);
-      return off < 0 ? -1 : off + (long long)(tile - page * tpp) * kv4_tile_bytes(D);
-    };
-
-    auto compute = [&](const Tile<G> &tl, int tok0) {
-      // Scores.
+    // One tile at shared address `at`, tokens tok0 ..  PART: some row does
+    // not see all of its tokens.
+    auto compute = [&](uint32_t at, int tok0, auto part_tag) {
+      constexpr bool PART = decltype(part_tag)::value;
+      uint32_t par[2][2 * G];  // parameters of tokens g, g + 8: [K groups, V groups]
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t q = at + G * 1024 + (g + 8 * r) * (8 * G);
+        if constexpr (G == 1) {
+          asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(par[r][0]), "=r"(par[r][1]) : "r"(q));
+        } else {
+#pragma unroll
+          for (int i = 0; i < G / 2; ++i) {
+            const uint4 u = lds16(q + i * 16);
+            par[r][4 * i] = u.x;
+            par[r][4 * i + 1] = u.y;
+            par[r][4 * i + 2] = u.z;
+            par[r][4 * i + 3] = u.w;
+          }
+        }
+      }
+      // Scores, less the rows' references.
       float s[NT][4];
       {
         float acc[NT][G][4];
@@ -327,129 +372,173 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args 
           for (int h = 0; h < G; ++h)
 #pragma unroll
             for (int x = 0; x < 4; ++x) acc[n][h][x] = 0.f;
+        uint4 kw[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) kw[i] = lds16(at + i * 512 + lane * 16);
 #pragma unroll
         for (int h = 0; h < G; ++h)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const int x0 = h * 2 + w, x1 = (G + h) * 2 + w;
-            uint32_t k0 = word_of(tl.k[x0 / 4], x0 % 4), k1 = word_of(tl.k[x1 / 4], x1 % 4);
+            uint32_t k0 = word_of(kw[x0 / 4], x0 % 4), k1 = word_of(kw[x1 / 4], x1 % 4);
+            uint32_t af[2][4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-                mma16816(acc[n][h], k0 & 0x000f000fu, k1 & 0x000f000fu, k0 & 0x00f000f0u, k1 & 0x00f000f0u,
-                         qf[n][h][w][2 * half], qf[n][h][w][2 * half + 1]);
+              af[half][0] = k0 & 0x000f000fu;
+              af[half][1] = k1 & 0x000f000fu;
+              af[half][2] = k0 & 0x00f000f0u;
+              af[half][3] = k1 & 0x00f000f0u;
               k0 >>= 8;
               k1 >>= 8;
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              uint4 qw;
+              if constexpr (Sh::kQRegs) qw = qf[(n * G + h) * 2 + w];
+              else qw = lds16(q_at + ((n * G + h) * 2 + w) * 512);
+              mma16816(acc[n][h], af[0][0], af[0][1], af[0][2], af[0][3], qw.x, qw.y);
+              mma16816(acc[n][h], af[1][0], af[1][1], af[1][2], af[1][3], qw.z, qw.w);
+            }
+          }
+        float2 kp[2][G];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int h = 0; h < G; ++h) kp[r][h] = kv4_unpack_param<T>(par[r][h]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float2 fac, qs[G];
+          if constexpr (Sh::kQRegs) {
+            fac = fac_r[n];
+#pragma unroll
+            for (int h = 0; h < G; ++h) qs[h] = qs_r[n * G + h];
+          } else {
+            fac = *reinterpret_cast<const float2 *>(&sm_f[n * 8 + 2 * t]);
+#pragma unroll
+            for (int h = 0; h < G; ++h) qs[h] = *reinterpret_cast<const float2 *>(&sm_qs[h][n * 8 + 2 * t]);
           }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float2 p[G];
-#pragma unroll
-          for (int h = 0; h < G; ++h) p[h] = kv4_unpack_param<T>(tl.par[r][h]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-              float dot = 0.f, off = 0.f;
+              // With a soft-cap the reference comes off behind the tanh.
+              float off = a.softcap > 0.f || ref[n][q] == -CUDART_INF_F ? 0.f : -ref[n][q];
+              float dot = kp[r][0].x * acc[n][0][2 * r + q];
+              off = fmaf(kp[r][0].y, q ? qs[0].y : qs[0].x, off);
 #pragma unroll
-              for (int h = 0; h < G; ++h) {
-                dot = fmaf(p[h].x, acc[n][h][2 * r + q], dot);
-                off = fmaf(p[h].y, qs[n][q][h], off);
+              for (int h = 1; h < G; ++h) {
+                dot = fmaf(kp[r][h].x, acc[n][h][2 * r + q], dot);
+                off = fmaf(kp[r][h].y, q ? qs[h].y : qs[h].x, off);
               }
-              s[n][2 * r + q] = fmaf(dot, fac[n][q], off);
+              s[n][2 * r + q] = fmaf(dot, q ? fac.y : fac.x, off);
             }
         }
       }
       if (a.softcap > 0.f) {
+        const float cap2 = a.softcap * kLog2e;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[n][x] = tanhf(s[n][x]) * (a.softcap * kLog2e);
+          for (int x = 0; x < 4; ++x)
+            s[n][x] = fmaf(tanhf(s[n][x]), cap2, ref[n][x & 1] == -CUDART_INF_F ? 0.f : -ref[n][x & 1]);
       }
       if (a.alibi != nullptr) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          const float2 sl = *reinterpret_cast<const float2 *>(&sm_slope[n * 8 + 2 * t]);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[n][x] = fmaf(slope[n][x & 1], (float)(tok0 + g + 8 * (x >> 1)), s[n][x]);
+          for (int x = 0; x < 4; ++x)
+            s[n][x] = fmaf(x & 1 ? sl.y : sl.x, (float)(tok0 + g + 8 * (x >> 1)), s[n][x]);
+        }
       }
-      // Masks, only where the tile is not seen whole by every row.
-      const bool part = tok0 < max(lo_in, t_lo) || tok0 + 16 > min(hi_in, t_hi);
       uint32_t vis = 0xffffffffu;
-      if (part) {
+      if constexpr (PART) {
         vis = 0;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          const int2 lo = *reinterpret_cast<const int2 *>(&sm_lo[n * 8 + 2 * t]);
+          const int2 hi = *reinterpret_cast<const int2 *>(&sm_hi[n * 8 + 2 * t]);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int j = tok0 + g + 8 * (x >> 1);
-            const bool ok = j >= max(lo[n][x & 1], t_lo) && j < min(hi[n][x & 1], t_hi);
-            if (ok) vis |= 1u << (n * 4 + x);
+            if (j >= max(x & 1 ? lo.y : lo.x, t_lo) && j < min(x & 1 ? hi.y : hi.x, t_hi)) vis |= 1u << (n * 4 + x);
             else s[n][x] = -CUDART_INF_F;
           }
-      }
-      // V's parameters; a token that no row sees may hold anything.
-      float sv[2][G], cv[2][G];
-      uint32_t sbits = 0;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const bool dead = part && (vis & (0x33333333u << (2 * r))) == 0;
-#pragma unroll
-        for (int h = 0; h < G; ++h) {
-          float2 p = kv4_unpack_param<T>(tl.par[r][G + h]);
-          if (dead) p = make_float2(0.f, 0.f);
-          sv[r][h] = p.x;
-          cv[r][h] = fmaf(8.f, p.x, p.y);
-          const uint32_t u = __float_as_uint(p.x);
-          sbits = max(sbits, u < 0x7f800000u ? u : 0u);
         }
       }
-      // Running maxima: moved, with everything accumulated, when a score
-      // passes one by kLazyMax or a larger step turns up.
-      bool move = false;
+      // V's steps and centres; a token that no row sees may hold anything.
+      float sv[2][G], cv[2][G];
+      float smax = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int r = 0; r < 2; ++r) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) move |= fmaxf(s[n][q], s[n][2 + q]) > mx[n][q] + kLazyMax;
-      move |= (int)(sbits >> 23) - 127 > step_exp;
-      if (__any_sync(0xffffffffu, move)) {
-        const int top = (int)(__reduce_max_sync(0xffffffffu, sbits) >> 23) - 127;
-        const int new_exp = max(step_exp, top);
-        const float down = step_exp - new_exp < -126 ? 0.f : pow2i(step_exp - new_exp);
+        for (int h = 0; h < G; ++h) {
+          float2 p = kv4_unpack_param<T>(par[r][G + h]);
+          if (PART && (vis & (0x33333333u << (2 * r))) == 0) p = make_float2(0.f, 0.f);
+          sv[r][h] = p.x;
+          cv[r][h] = fmaf(8.f, p.x, p.y);
+          smax = fmaxf(smax, p.x);
+        }
+      }
+      // The references move, with everything accumulated, when a score
+      // passes its row's maximum by kLazyMax or a larger step turns up.
+      const float limit = kLazyMax + (float)(kStepExp - step_exp);
+      float most = s[0][0];
+      bool first = false;  // a row without a reference so far
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) most = fmaxf(most, s[n][x]);
+        first |= ref[n][0] == -CUDART_INF_F || ref[n][1] == -CUDART_INF_F;
+      }
+      if (__any_sync(0xffffffffu, first || most > limit || smax >= pow2i(step_exp + 1))) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int h = 0; h < G; ++h) {
+            const uint32_t u = __float_as_uint(sv[r][h]);
+            bits = max(bits, u < 0x7f800000u ? u : 0u);
+          }
+        const int new_exp = max(step_exp, min(kMaxStepExp, (int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 127));
+        const float old_room = (float)(kStepExp - step_exp), new_room = (float)(kStepExp - new_exp);
         step_exp = new_exp;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            float v = fmaxf(s[n][q], s[n][2 + q]);
+            const bool none = ref[n][q] == -CUDART_INF_F;
+            const float shift = none ? 0.f : ref[n][q];
+            float v = fmaxf(s[n][q], s[n][2 + q]) + shift;
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-            const float m = fmaxf(mx[n][q], v);
-            const float al = m == -CUDART_INF_F ? 1.f : exp2_fast(mx[n][q] - m);
-            mx[n][q] = m;
+            const float m = none ? v : fmaxf(ref[n][q] + old_room, v);
+            const float now = m == -CUDART_INF_F ? m : m - new_room;
+            const float al = none ? 1.f : exp2_fast(ref[n][q] - now);
+            const float back = now == -CUDART_INF_F ? 0.f : shift - now;
+            ref[n][q] = now;
+            s[n][q] += back;
+            s[n][2 + q] += back;
             l[n][q] *= al;
 #pragma unroll
             for (int h = 0; h < G; ++h) {
               aff[n][q][h] *= al;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                o[n][h][i][q] *= al * down;
-                o[n][h][i][2 + q] *= al * down;
+                o[n][h][i][q] *= al;
+                o[n][h][i][2 + q] *= al;
               }
             }
           }
       }
       // Weights.
-      const float vs = pow2i(kStepExp - step_exp);
       uint32_t pf[NT][G][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float p[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const float m = mx[n][x & 1];
-          p[x] = exp2_fast(s[n][x] - (m == -CUDART_INF_F ? 0.f : m));
+          p[x] = exp2_fast(s[n][x]);
           l[n][x & 1] += p[x];
         }
 #pragma unroll
@@ -459,19 +548,29 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args 
             float w[2];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-              const bool ok = !part || (vis >> (n * 4 + 2 * r + q) & 1u);
-              w[q] = ok ? p[2 * r + q] * (sv[r][h] * vs) : 0.f;
-              aff[n][q][h] += ok ? p[2 * r + q] * cv[r][h] : 0.f;
+              w[q] = p[2 * r + q] * sv[r][h];
+              float f = p[2 * r + q] * cv[r][h];
+              if constexpr (PART) {
+                const bool ok = vis >> (n * 4 + 2 * r + q) & 1u;
+                w[q] = ok ? w[q] : 0.f;
+                f = ok ? f : 0.f;
+                aff[n][q][h] += f;
+              } else {
+                aff[n][q][h] = fmaf(p[2 * r + q], cv[r][h], aff[n][q][h]);
+              }
             }
             pf[n][h][r] = transpose8x8(pack_half2(w[0], w[1]));
           }
       }
       // O^T += V^T P^T.
+      uint4 vw[G];
+#pragma unroll
+      for (int i = 0; i < G; ++i) vw[i] = lds16(at + G * 512 + i * 512 + lane * 16);
 #pragma unroll
       for (int h = 0; h < G; ++h) {
         uint32_t w[4];
 #pragma unroll
-        for (int sl = 0; sl < 4; ++sl) w[sl] = word_of(tl.v[(sl * G + h) / 4], (sl * G + h) % 4);
+        for (int sl = 0; sl < 4; ++sl) w[sl] = word_of(vw[(sl * G + h) / 4], (sl * G + h) % 4);
 #pragma unroll
         for (int part16 = 0; part16 < 2; ++part16) {
           uint32_t z0 = __byte_perm(w[0], w[1], part16 ? 0x7632 : 0x5410);
@@ -488,23 +587,33 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args 
       }
     };
 
-    long long where = locate(0);
-    Tile<G> cur, nxt;
-    bool have = false, have_next = false;
-    auto fetch = [&](int i, Tile<G> &dst) -> bool {
-      if (i >= mine) return false;
-      if (i > 0 && i % 32 == 0) where = locate(i);
-      const long long off = __shfl_sync(0xffffffffu, where, i % 32);
-      if (off < 0) return false;
-      load_tile<G>(dst, base + off, lane);
-      return true;
-    };
-    have = fetch(0, cur);
+    const int full_lo = max(lo_in, t_lo), full_hi = min(hi_in, t_hi);
+    int stage = 0;
+    uint32_t parity = 0;  // bit s: parity of stage s's next phase
     for (int i = 0; i < mine; ++i) {
-      have_next = fetch(i + 1, nxt);
-      if (have) compute(cur, (tile0 + warp + i * kWarps) << 4);
-      cur = nxt;
-      have = have_next;
+      if (i % 32 == 0) bad_now = bad_issue;
+      if (!(bad_now >> (i % 32) & 1u)) {
+        const bool ok = sm100::mbar_wait(&sm_full[warp][stage], parity >> stage & 1u, kWaitNs);
+        if (!__all_sync(0xffffffffu, ok)) {
+          // Never seen to happen: the copy did not arrive in a second.  The
+          // copies in flight get as long again before the CTA goes on.
+          raise_error(a.err, kDevErrTimeout);
+          for (int k = 0; k < kStages && i + k < mine; ++k) {
+            const int st = (stage + k) % kStages;
+            if (!(bad_now >> ((i + k) % 32) & 1u)) sm100::mbar_wait(&sm_full[warp][st], parity >> st & 1u, kWaitNs);
+          }
+          break;
+        }
+        parity ^= 1u << stage;
+        const int tok0 = (tile0 + warp + i * kWarps) << 4;
+        if (tok0 >= full_lo && tok0 + 16 <= full_hi) compute(ring + stage * Sh::kTile, tok0, std::false_type{});
+        else compute(ring + stage * Sh::kTile, tok0, std::true_type{});
+      }
+      const int next = i + kStages;
+      if (next % 32 == 0) locate(next);
+      __syncwarp();  // the warp has read the stage
+      if (next < mine) issue(next, stage);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
   }
 
@@ -520,33 +629,30 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args 
         for (int h = 0; h < G; ++h) aff[n][q][h] += __shfl_xor_sync(0xffffffffu, aff[n][q][h], off);
       }
     }
-  __syncthreads();  // q in shared memory has been read
-  {
-    const float unscale = pow2i(step_exp - kStepExp);
+  __syncthreads();  // every warp is through with its ring
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int r = n * 8 + 2 * t + q;
-        if (g == 0) {
-          sm_m[warp][r] = mx[n][q];
-          sm_l[warp][r] = l[n][q];
-        }
-        float *dst = sm_o + (warp * R + r) * LDO;
-#pragma unroll
-        for (int h = 0; h < G; ++h) {
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[2 * i] = fmaf(o[n][h][i][q], unscale, aff[n][q][h]);
-            v[2 * i + 1] = fmaf(o[n][h][i][2 + q], unscale * 0.0625f, aff[n][q][h]);
-          }
-          float4 *d4 = reinterpret_cast<float4 *>(dst + 64 * h + 8 * g);
-          d4[0] = make_float4(v[0], v[1], v[2], v[3]);
-          d4[1] = make_float4(v[4], v[5], v[6], v[7]);
-        }
+    for (int q = 0; q < 2; ++q) {
+      const int r = n * 8 + 2 * t + q;
+      if (g == 0) {
+        sm_m[warp][r] = ref[n][q];
+        sm_l[warp][r] = l[n][q];
       }
-  }
+      float *dst = sm_o + (warp * R + r) * LDO;
+#pragma unroll
+      for (int h = 0; h < G; ++h) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = o[n][h][i][q] + aff[n][q][h];
+          v[2 * i + 1] = fmaf(o[n][h][i][2 + q], 0.0625f, aff[n][q][h]);
+        }
+        float4 *d4 = reinterpret_cast<float4 *>(dst + 64 * h + 8 * g);
+        d4[0] = make_float4(v[0], v[1], v[2], v[3]);
+        d4[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    }
   __syncthreads();
 
   // Merge the warps.
@@ -560,7 +666,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a, Kv4Args 
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float wt = sm_m[w][r] == -CUDART_INF_F ? 0.f : exp2f(sm_m[w][r] - top);
-      // A warp that saw no finite maximum adds nothing, unless its sum is a NaN.
+      // A warp that saw no finite score adds nothing, unless its sum is a NaN.
       lsum += wt == 0.f ? (sm_l[w][r] == sm_l[w][r] ? 0.f : sm_l[w][r]) : sm_l[w][r] * wt;
       ov += wt == 0.f ? 0.f : sm_o[(w * R + r) * LDO + d] * wt;
     }
@@ -584,6 +690,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) kv4_combine_kernel(AttnArgs a, int chunk, int n_splits, const float *part_o,
                                                           const float *part_lse) {
   constexpr int E = D / 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits are written
   const int lane = threadIdx.x % 32;
   const long long n_rows = (long long)a.B * a.Sq * a.H;
   const long long row = (long long)blockIdx.x * 4 + threadIdx.x / 32;
@@ -624,22 +731,29 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(AttnArgs a, int chunk,
 
 template <int D>
 constexpr int max_nt() {
-  return D == 64 ? 4 : (D == 128 ? 2 : 1);
+  return D == 64 ? 4 : (D == 128 ? 4 : 2);
 }
 
 SplitPlan plan_kv4(const AttnArgs &a, size_t ws_available) {
   SplitPlan p;
   p.rows = a.group * a.Sq;
-  const int most = a.D == 64 ? 4 : (a.D == 128 ? 2 : 1);
-  p.nt = p.rows <= 8 || most == 1 ? 1 : (p.rows <= 16 || most == 2 ? 2 : 4);
+  const int G = a.D / kKv4Group;
+  const int most = a.D == 256 ? 2 : 4;
+  p.nt = p.rows <= 8 ? 1 : (p.rows <= 16 || most == 2 ? 2 : 4);
   p.row_blocks = (p.rows + 8 * p.nt - 1) / (8 * p.nt);
   const long long units = (long long)a.B * a.Hkv * p.row_blocks;
+  const long long slots = (long long)a.num_sms * (p.nt * G <= 2 ? 4 : (p.nt * G <= 4 ? 3 : 2));
   // Tokens that a sequence's rows can see between them.
   long long span = a.Skv;
   if (a.window >= 0) span = std::min<long long>(span, (long long)a.window + a.Sq + 16);
-  int chunk = 1024;
-  while (chunk > 64 && units * ((span + chunk - 1) / chunk) < 4LL * a.num_sms) chunk /= 2;
-  p.chunk = chunk;
+  // One wave of CTAs where that leaves each 128 tokens at least; splits of
+  // 1024 tokens where there is more than a wave of work anyway (sequences
+  // differ in length, so equal shares cannot be dealt from here).
+  long long n = std::max<long long>(1, slots / units);
+  n = std::min(n, (span + 127) / 128);
+  if (units > slots / 2) n = std::max(n, (span + 1023) / 1024);
+  long long chunk = ((span + n - 1) / n + 63) / 64 * 64;
+  p.chunk = (int)chunk;
   p.n_splits = (int)((span + chunk - 1) / chunk);
   p.ws_bytes = p.n_splits > 1 ? (size_t)p.n_splits * a.B * a.Sq * a.H * (a.D + 1) * sizeof(float) : 0;
   if (p.n_splits > 1 && ws_available < p.ws_bytes) {
@@ -651,9 +765,7 @@ SplitPlan plan_kv4(const AttnArgs &a, size_t ws_available) {
 
 template <typename T, int D, int NT>
 cudaError_t launch_nt(const AttnArgs &a, const Kv4Args &c, const SplitPlan &p, void *ws, cudaStream_t s) {
-  constexpr size_t o_bytes = (size_t)kWarps * 8 * NT * (D + 4) * sizeof(float);
-  constexpr size_t q_bytes = (size_t)8 * NT * D * sizeof(__half);
-  constexpr size_t smem = o_bytes > q_bytes ? o_bytes : q_bytes;
+  constexpr size_t smem = Shape<D, NT>::kSmem;
   if (smem > 48 * 1024) {
     const cudaError_t e =
         cudaFuncSetAttribute(kv4_attn_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -669,8 +781,18 @@ cudaError_t launch_nt(const AttnArgs &a, const Kv4Args &c, const SplitPlan &p, v
   kv4_attn_kernel<T, D, NT><<<grid, kThreads, smem, s>>>(a, c, p.chunk, p.n_splits, p.row_blocks, part_o, part_lse);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.n_splits == 1) return e;
-  kv4_combine_kernel<T, D><<<(unsigned)((n_rows + 3) / 4), 128, 0, s>>>(a, p.chunk, p.n_splits, part_o, part_lse);
-  return cudaGetLastError();
+  // The combine's launch overlaps the splits; it waits for them itself.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((n_rows + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D>, a, p.chunk, p.n_splits, (const float *)part_o,
+                            (const float *)part_lse);
 }
 
 template <typename T, int D>
