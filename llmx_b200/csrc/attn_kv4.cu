@@ -7,31 +7,38 @@
 //   sum_j p_j V_j = sum_j (p_j s_jh) (n_jh - 8) + sum_j p_j (m_jh + 8 s_jh)
 // so the matrix products run on the integers themselves, which fp16 holds
 // exactly, and the affine part is a few fp32 operations per token and group.
-//   * K: a nibble masked in place is the fp16 subnormal n 2^-24 (bits 0-3) or
-//     16 n 2^-24 (bits 4-7; q carries the 1/16), one AND per two values.
-//     q is scaled by a power of two per row to fit fp16: 11 bits of it are
-//     kept, all that fp16 and bf16 have.
+//   * K: the nibbles of a word are 4 + 4 bytes after two ANDs and a shift, and
+//     go as they are into the integer tensor product (m16n8k32, u8 x s8, exact
+//     in 32 bits).  q is a 16-bit integer of its row's largest value (steps of
+//     1/32512), its high and low byte two products.
 //   * V: a nibble OR-ed into 1024 (0x6400) and 1032 (or 1152 = 1024 + 128 for
 //     bits 4-7) subtracted is n - 8 (16 (n - 8)), two operations per two
 //     values.  Centred, because the tensor core's fp32 accumulation would
 //     otherwise carry a mean of 7.5 through the whole sequence that cancels
 //     only at the end.
-//   * p s is rounded to fp16 (2^-12 relative), after a scale by a power of two
-//     that brings the largest s seen so far to [2^7, 2^8).  Scores, p, the
-//     softmax sums and the affine part stay fp32.
+//   * p s is rounded to fp16 (2^-11 relative at most), after a scale by a power
+//     of two that brings the largest s seen so far to [2^7, 2^8).  Scores, p,
+//     the softmax sums and the affine part stay fp32.
 //
-// Shape.  S^T = K q^T as mma m16n8k16 with 16 tokens as rows and 8 (head,
-// query row) pairs of one kv head as columns; O^T += V^T P^T with channels as
-// rows.  The cache's tile layout is the order of these fragments, so K and V
-// go from 16-byte global loads to registers to the tensor core, without
-// shared memory; P^T changes from the accumulator's layout to the operand's
-// with one 8x8 transpose (movmatrix) per 8 tokens and group.  mma.sync and not
-// tcgen05: the operands are made in registers, 8 columns are all there are in
-// a decode, and the pass is bound by the cache's bytes, not by the products.
+// Shape.  S^T = K q^T with 16 tokens as rows and 8 columns of (head, query row)
+// pairs of one kv head; O^T += V^T P^T (m16n8k16, fp16) with channels as rows.
+// The cache's tile layout is the order of these fragments, so K and V go from
+// linear copies in shared memory to registers to the tensor core; P^T changes
+// from the accumulator's layout to the operand's with one 8x8 transpose
+// (movmatrix) per 8 tokens and group.  mma.sync and not tcgen05: the operands
+// are made in registers, 8 columns are all there are in a decode, and what
+// bounds the pass is the integer unit that unpacks the nibbles (two cycles an
+// operation and warp, 88 operations a 16-token tile of 128 channels) next to
+// the cache's bytes, not the products.
 //
-// A CTA takes a range of tokens of one (sequence, kv head, block of 8 * NT
-// pairs); its warps take every fourth tile and are merged at the end, and the
-// ranges (splits) by a second kernel as in attn_decode.cu.
+// Work.  A unit is one (sequence, kv head, block of pairs); its tokens are cut
+// into steps of one or two tiles, and the steps of all units, end to end, are
+// dealt to the resident warps in equal shares.  A warp works alone: it copies
+// its tiles into its own ring in shared memory (one bulk copy a tile, issued
+// ahead across unit boundaries), and writes the result of a unit that it has
+// whole.  Of a unit that several warps share each writes a partial result (at
+// most two a warp, so the workspace does not grow with the sequences), and a
+// second kernel merges them as in attn_decode.cu.
 #include <algorithm>
 #include <string>
 
@@ -52,6 +59,7 @@ constexpr float kLazyMax = 6.f;
 // under a lazy maximum): fp16 then keeps 11 bits of weights down to 2^-21 of
 // the largest.  Steps count from 2^-40 on (smaller ones lose bits from 2^-61
 // on), which keeps the sums of scaled weights inside fp32.
+constexpr float kQTop = 32512.f;  // 127 * 256: q's largest value as an integer
 constexpr int kStepExp = 7;
 constexpr int kMinStepExp = -40;
 constexpr int kMaxStepExp = 125;
@@ -63,6 +71,22 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 4-bit integers (one a byte) times the bytes of q, exact in 32 bits.
+__device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void imma16832_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
 // 8x8 transpose of 16-bit elements across the warp: lane (g, t) gives row g,
@@ -78,14 +102,21 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// (x & mask) | bits in one operation.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
+  return r;
+}
+
 // (n - 8) of the nibbles in bits 0-3 of both halves; 16 (n - 8) of bits 4-7.
 __device__ __forceinline__ uint32_t centred_lo(uint32_t z) {
-  const uint32_t u = (z & 0x000f000fu) | 0x64006400u, c = 0x64086408u;
+  const uint32_t u = and_or(z, 0x000f000fu, 0x64006400u), c = 0x64086408u;
   const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&u), *reinterpret_cast<const __half2 *>(&c));
   return *reinterpret_cast<const uint32_t *>(&r);
 }
 __device__ __forceinline__ uint32_t centred_hi(uint32_t z) {
-  const uint32_t u = (z & 0x00f000f0u) | 0x64006400u, c = 0x64806480u;
+  const uint32_t u = and_or(z, 0x00f000f0u, 0x64006400u), c = 0x64806480u;
   const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&u), *reinterpret_cast<const __half2 *>(&c));
   return *reinterpret_cast<const uint32_t *>(&r);
 }
@@ -100,15 +131,6 @@ __device__ __forceinline__ float pow2i(int e) {  // 2^e for e in [-126, 127]
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-struct SplitPlan {
-  int rows;       // (head, query row) pairs of one kv head
-  int nt;         // columns of 8 pairs a CTA takes
-  int row_blocks;
-  int chunk;      // tokens per split, a multiple of 64
-  int n_splits;
-  size_t ws_bytes;
-};
-
 // Tokens that row i sees: [lo, hi).
 __device__ __forceinline__ void row_range(const AttnArgs &a, int i, int ql, int kl, int &lo, int &hi) {
   const int diag = i + kl - ql;
@@ -116,12 +138,110 @@ __device__ __forceinline__ void row_range(const AttnArgs &a, int i, int ql, int 
   lo = a.window >= 0 ? max(0, diag - a.window) : 0;
 }
 
-// First token of split 0 of a sequence: the first one that its row 0 sees,
-// on a 16-token tile.  Later rows see none before it.
-__device__ __forceinline__ int first_token(const AttnArgs &a, int ql, int kl) {
-  int lo, hi;
-  row_range(a, 0, ql, kl, lo, hi);
-  return lo & ~15;
+// The tokens of sequence b that its rows see between them, as steps of W
+// tiles from a 16-token boundary (rows' ranges move one way: the first row's
+// begin to the last row's end).
+struct Span {
+  int first, steps;
+  int blocks;  // of R pairs
+};
+template <int W>
+__device__ __forceinline__ Span span_of(const AttnArgs &a, int R, int ql, int kl) {
+  Span s = {0, 0, 0};
+  if (ql > 0 && kl > 0) {
+    int lo, hi, x;
+    row_range(a, 0, ql, kl, lo, x);
+    row_range(a, ql - 1, ql, kl, x, hi);
+    s.first = lo & ~15;
+    if (hi > lo) {
+      s.steps = (hi - s.first + 16 * W - 1) / (16 * W);
+      s.blocks = (ql * a.group + R - 1) / R;
+    }
+  }
+  return s;
+}
+
+// A launch's part of the batch and its shares.
+struct Work {
+  int b0, nb;      // sequences
+  int R;           // pairs of a block
+  int workers;     // warps (CTAs, where a CTA's warps work together) that take a share, at most
+  int min_steps;   // a share is at least this long
+  int split;       // 0: shares end where units end
+};
+constexpr int kMaxSlice = 512;
+
+// Shares: worker w of `n` has the steps [begin(w), begin(w + 1)) of `total`
+// (below 2^31, which the host sees to).
+__device__ __forceinline__ uint32_t share_begin(uint32_t total, int w, int n) {
+  return (uint32_t)((unsigned long long)total * w / n);
+}
+__device__ __forceinline__ int share_of(uint32_t total, uint32_t step, int n) {
+  return (int)((((unsigned long long)step + 1) * n - 1) / total);
+}
+__device__ __forceinline__ int share_count(const Work &wk, uint32_t total) {
+  const uint32_t n = total / wk.min_steps;
+  return n < 1 ? 1 : (n < (uint32_t)wk.workers ? (int)n : wk.workers);
+}
+
+// Steps of all units before each sequence of the slice, prefix[nb] their sum,
+// and the sequences' query and key lengths.
+// Called by all of the CTA's kThreads threads; ends with a barrier.
+template <int W>
+__device__ __forceinline__ void scan_steps(const AttnArgs &a, const Work &wk, uint32_t *prefix, int2 *lens, uint32_t *tmp) {
+  const int tid = threadIdx.x, lane = tid % 32;
+  const int per = (wk.nb + kThreads - 1) / kThreads;
+  uint32_t sum = 0;
+  for (int i = tid * per; i < min(wk.nb, (tid + 1) * per); ++i) {
+    const int b = wk.b0 + i;
+    prefix[i] = sum;
+    lens[i] = make_int2(clamp_len(a.q_lens, b, a.Sq), clamp_len(a.kv_lens, b, a.Skv));
+    const Span sp = span_of<W>(a, wk.R, lens[i].x, lens[i].y);
+    sum += (uint32_t)sp.steps * sp.blocks * a.Hkv;
+  }
+  uint32_t up = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xffffffffu, up, off);
+    if (lane >= off) up += x;
+  }
+  if (lane == 31) tmp[tid / 32] = up;
+  __syncthreads();
+  uint32_t before = up - sum;
+  for (int w = 0; w < tid / 32; ++w) before += tmp[w];
+  for (int i = tid * per; i < min(wk.nb, (tid + 1) * per); ++i) prefix[i] += before;
+  if (tid == kThreads - 1) prefix[wk.nb] = before + sum;
+  __syncthreads();
+}
+
+// Where a step of the slice lies.
+struct Place {
+  int b, ql, kl;   // sequence
+  int kvh, block;  // unit
+  int first;       // first token of the unit's steps
+  int at, steps;   // step in its unit, and the unit's steps
+};
+template <int W>
+__device__ __forceinline__ Place place_of(const AttnArgs &a, const Work &wk, const uint32_t *prefix, const int2 *lens, uint32_t step) {
+  int lo = 0, hi = wk.nb - 1;  // the last sequence that begins at or before the step
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (prefix[mid] <= step) lo = mid;
+    else hi = mid - 1;
+  }
+  Place p;
+  p.b = wk.b0 + lo;
+  p.ql = lens[lo].x;
+  p.kl = lens[lo].y;
+  const Span sp = span_of<W>(a, wk.R, p.ql, p.kl);
+  const uint32_t rest = step - prefix[lo];
+  const int unit = (int)(rest / (uint32_t)sp.steps);
+  p.first = sp.first;
+  p.steps = sp.steps;
+  p.at = (int)(rest - (uint32_t)unit * sp.steps);
+  p.kvh = unit / sp.blocks;
+  p.block = unit - p.kvh * sp.blocks;
+  return p;
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4 &u, int i) {
@@ -134,6 +254,48 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   return r;
 }
 
+// The K words of group h: [token g, g + 8][8-channel word] from this lane's
+// place in a tile (layout: word x = (r G + h) 2 + w).
+template <int G>
+__device__ __forceinline__ void lds_k(uint32_t (&k)[2][2], uint32_t addr, int h) {
+  if constexpr (G == 1) {
+    const uint4 u = lds16(addr);
+    k[0][0] = u.x;
+    k[0][1] = u.y;
+    k[1][0] = u.z;
+    k[1][1] = u.w;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int x = (r * G + h) * 2;
+      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
+                   : "=r"(k[r][0]), "=r"(k[r][1])
+                   : "r"(addr + x / 4 * 512 + x % 4 * 4));
+    }
+  }
+}
+
+// The parameter words of one token's K or V.
+template <int G>
+__device__ __forceinline__ void lds_params(uint32_t (&w)[G], uint32_t addr) {
+  if constexpr (G == 1) {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+  } else if constexpr (G == 2) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  } else {
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T *p, const float (&f)[4]) {
+  const float x[8] = {f[0], f[1], f[2], f[3], 0.f, 0.f, 0.f, 0.f};
+  const uint4 u = pack8<T>(x);
+  *reinterpret_cast<uint2 *>(p) = make_uint2(u.x, u.y);
+}
+
 // One contiguous tile, global -> this CTA's shared memory, counted on `bar`.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -141,584 +303,808 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                : "memory");
 }
 
-// Sizes of one variant: 8 * NT pairs of head_dim D.
-template <int D, int NT>
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Sizes of one variant: 8 columns, SLOTS tiles side by side in them.  With few
+// pairs (8 / SLOTS or less) the columns hold the pairs SLOTS times, once per
+// tile: q is 0 in the columns of the other tiles, so the
+// products of all tiles add up in one accumulator without mixing, and the
+// whole softmax part runs once for SLOTS tiles.
+//
+// NQ = 2: a thread works on columns 2t and 2t + 1, two pairs.  NQ = 1, for
+// fewer pairs still: one pair has both, with the low byte of q in the odd one.
+template <int D, int NQ, int SLOTS, bool COOP>
 struct Shape {
   static constexpr int G = D / kKv4Group;
-  static constexpr int R = 8 * NT;
-  static constexpr int LDO = D + 4;  // padded row of the merge buffer
+  static constexpr int kCols = 8;
+  static constexpr int kTileCols = kCols / SLOTS;          // columns of one tile
+  static constexpr int R = kTileCols / (NQ == 1 ? 2 : 1);  // pairs a warp takes
   static constexpr int kTile = 18 * D;
-  static constexpr int kStages = D == 64 ? 6 : (D == 128 ? 4 : 3);
-  // q fragments and row factors stay in registers where they are few.
-  static constexpr bool kQRegs = NT * G <= 2;
-  static constexpr int kMinCtas = NT * G <= 2 ? 4 : (NT * G <= 4 ? 3 : 2);
-  static constexpr size_t kRing = (size_t)kWarps * kStages * kTile;
-  static constexpr size_t kMerge = (size_t)kWarps * R * LDO * sizeof(float);
-  static constexpr size_t kRingOrMerge = kRing > kMerge ? kRing : kMerge;
-  static constexpr size_t kQFrag = (size_t)NT * G * 2 * 32 * 16;
-  static constexpr size_t kSmem = kRingOrMerge + kQFrag;
+  static constexpr int W = D == 256 ? 1 : 2;  // tiles of a step: copied and waited for together
+  static constexpr int kStages = D == 64 ? 4 : (D == 128 ? 2 : 3);
+  static constexpr int kMinCtas = G <= 2 ? 4 : 3;
+  static constexpr int kRing = kStages * W * kTile;
+  static constexpr int kQFrag = G * 2 * 32 * 16;
+  static constexpr int kRows = kCols * (4 + G) * 4;  // factor, slope, lo, hi and group sums of each column
+  // Each warp's ring; q and its columns, of each warp or of all; as many
+  // zeros as q for the other tiles' columns; lengths and prefix sums.
+  static constexpr int kZeros = SLOTS > 1 ? kQFrag : 0;
+  static constexpr int kSmem = kWarps * kRing + (COOP ? 1 : kWarps) * (kQFrag + kRows) + kZeros;
+  static constexpr int kMergeRow = D + 4;  // floats of a row in the ring when warps are merged
+  static_assert(W % SLOTS == 0, "a step holds whole groups of tiles");
+  static_assert(R * kMergeRow * 4 <= kRing, "a warp's result fits its ring");
 };
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, Shape<D, NT>::kMinCtas)
-    kv4_attn_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Kv4Args c, int chunk, int n_splits,
-                    int row_blocks, float *part_o, float *part_lse) {
-  using Sh = Shape<D, NT>;
-  constexpr int G = Sh::G, R = Sh::R, LDO = Sh::LDO, kStages = Sh::kStages;
+template <typename T, int D, int NQ, int SLOTS, bool COOP>
+__global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
+    kv4_attn_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Kv4Args c, const __grid_constant__ Work wk,
+                    float *part_o, float *part_lse) {
+  using Sh = Shape<D, NQ, SLOTS, COOP>;
+  constexpr int G = Sh::G, R = Sh::R, kStages = Sh::kStages, W = Sh::W, kCols = Sh::kCols;
+  constexpr int kTileCols = Sh::kTileCols, kColStep = NQ == 1 ? 2 : 1;  // pair r of a tile has column r * kColStep
   extern __shared__ __align__(128) unsigned char smem[];
-  float *sm_o = reinterpret_cast<float *>(smem);                              // [kWarps][R][LDO], after the loop
-  __half *sm_q = reinterpret_cast<__half *>(smem + Sh::kRingOrMerge);         // fragments of q
-  __shared__ float sm_f[R], sm_qs[G][R], sm_slope[R];
-  __shared__ int sm_lo[R], sm_hi[R];
-  __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];
   __shared__ uint64_t sm_full[kWarps][kStages];
-
-  // The combine kernel may be set up while this one runs.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  const int split = blockIdx.x;
-  const int kvh = blockIdx.y / row_blocks;
-  const int r0 = blockIdx.y % row_blocks * R;
-  const int b = blockIdx.z;
+  __shared__ uint32_t sm_tmp[kWarps];
+  __shared__ float sm_m[kWarps][R], sm_l[kWarps][R];  // with COOP: each warp's references and sums
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int g = lane >> 2, t = lane & 3;
-  const int rows = a.group * a.Sq;  // pair r: query row r / group, head r % group of the kv head
+  unsigned char *own = smem + warp * Sh::kRing;
+  unsigned char *q_at0 = smem + kWarps * Sh::kRing + (COOP ? 0 : warp) * (Sh::kQFrag + Sh::kRows);
+  uint4 *q_own = reinterpret_cast<uint4 *>(q_at0);
+  float *row_f = reinterpret_cast<float *>(q_at0 + Sh::kQFrag);
+  float *row_slope = row_f + kCols, *row_qs = row_f + 2 * kCols;  // row_qs [G][kCols]
+  int *row_lo = reinterpret_cast<int *>(row_qs + G * kCols), *row_hi = row_lo + kCols;
+  unsigned char *zeros = smem + Sh::kSmem - Sh::kZeros;
+  int2 *lens = reinterpret_cast<int2 *>(smem + Sh::kSmem);               // [nb]
+  uint32_t *prefix = reinterpret_cast<uint32_t *>(lens + wk.nb);  // [nb + 1]
 
-  const int ql = clamp_len(a.q_lens, b, a.Sq);
-  const int kl = clamp_len(a.kv_lens, b, a.Skv);
+  // The merge kernel may be set up while this one runs.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // Tokens of this split that some row of the block sees, and the ones
-  // [lo_in, hi_in) that all of its rows see (the rows' ranges move one way:
-  // the last row's begin, the first row's end).
-  int t_lo = 0, t_hi = 0, lo_in = 0, hi_in = 0;
-  {
-    const int i0 = r0 / a.group, i1 = min(min(r0 + R, rows) - 1, ql * a.group - 1) / a.group;
-    if (i0 < ql && kl > 0) {
-      int lo0, hi1;
-      row_range(a, i0, ql, kl, lo0, hi_in);
-      row_range(a, i1, ql, kl, lo_in, hi1);
-      const int s0 = first_token(a, ql, kl) + split * chunk;
-      t_lo = max(lo0, s0);
-      t_hi = min(hi1, s0 + chunk);
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) sm100::mbar_init(&sm_full[warp][i], W);
+    sm100::fence_mbar_init();
+  }
+  for (int i = tid; i < Sh::kZeros / 16; i += kThreads) reinterpret_cast<uint4 *>(zeros)[i] = make_uint4(0u, 0u, 0u, 0u);
+  scan_steps<W>(a, wk, prefix, lens, sm_tmp);
+
+  // Neighbouring shares go to different CTAs, so that few of them spread over the SMs.
+  const int worker = COOP ? blockIdx.x : warp * gridDim.x + blockIdx.x;
+  const uint32_t total = prefix[wk.nb];
+
+  // Rows that see nothing, past their sequence's or in one without a visible
+  // key, are 0.
+  for (int i = warp * gridDim.x + blockIdx.x; i < wk.nb; i += kWarps * gridDim.x) {
+    const int b = wk.b0 + i;
+    const int r0 = prefix[i + 1] == prefix[i] ? 0 : lens[i].x;
+    for (long long e = lane; e < (long long)(a.Sq - r0) * a.H * (D / 8); e += 32) {
+      const int d = (int)(e % (D / 8)) * 8, h = (int)(e / (D / 8) % a.H), r = r0 + (int)(e / (D / 8) / a.H);
+      T *op = static_cast<T *>(a.o) + b * a.os[0] + r * a.os[1] + h * a.os[2] + d;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) op[x] = Elem<T>::from_f(0.f);
+      if (a.lse != nullptr && d == 0) a.lse[((long long)b * a.H + h) * a.Sq + r] = -CUDART_INF_F;
     }
   }
+  if (total == 0) return;
 
-  if (t_lo >= t_hi && n_splits > 1) {
-    // Nothing here; a row whose range of splits holds this one skips it.
-    for (int r = tid; r < R && r0 + r < rows; r += kThreads) {
-      const int i = (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
-      part_lse[(((long long)split * a.B + b) * a.Sq + i) * a.H + h] = -CUDART_INF_F;
-    }
-    return;
+  uint32_t begin, end;
+  if (wk.split) {
+    const int n = share_count(wk, total);
+    if (worker >= n) return;
+    begin = share_begin(total, worker, n);
+    end = share_begin(total, worker + 1, n);
+  } else {
+    // Whole units: a share ends with the unit that holds its last step.
+    auto snap = [&](uint32_t step) {
+      if (step >= total) return total;
+      const Place pl = place_of<W>(a, wk, prefix, lens, step);
+      return pl.at == 0 ? step : step - pl.at + pl.steps;
+    };
+    begin = snap(share_begin(total, worker, wk.workers));
+    end = snap(share_begin(total, worker + 1, wk.workers));
   }
+  // Steps of the share; this warp takes those with index k0 + kEvery i.
+  const int mine = (int)(end - begin);
+  constexpr int kEvery = COOP ? kWarps : 1;
+  const int k0 = COOP ? warp : 0;
 
-  // Weights are kept as 2^(S - ref) with one reference per row: the running
-  // maximum less a power of two that brings the largest step times the
-  // largest weight into fp16's upper range (kRoom below).
-  float o[NT][G][4][4];
-  float l[NT][2], aff[NT][2][G], ref[NT][2];
-  int step_exp = kMinStepExp;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int h = 0; h < G; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) o[n][h][i][x] = 0.f;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      l[n][q] = 0.f;
-      ref[n][q] = -CUDART_INF_F;
-#pragma unroll
-      for (int h = 0; h < G; ++h) aff[n][q][h] = 0.f;
-    }
-  }
+  // Steps in the order of the shares; with ALiBi a unit's last tokens come
+  // first: the bias grows with the token, so the maxima are there from the
+  // start and rarely move.
+  const bool reverse = a.alibi != nullptr;
+  const int tpp = c.page_size >> 4;
+  const uint32_t ring = sm100::smem_u32(own);
+  uint64_t *bar = &sm_full[warp][0];
 
-  if (t_lo < t_hi) {
-    const int tile0 = t_lo >> 4, tile1 = (t_hi + 15) >> 4;
-    const int tpp = c.page_size >> 4;
-    const unsigned char *base = c.data + kvh * c.head_stride;
-    const int mine = tile1 - tile0 > warp ? (tile1 - tile0 - warp + kWarps - 1) / kWarps : 0;  // tiles of this warp
-    const uint32_t ring = sm100::smem_u32(smem) + warp * kStages * Sh::kTile;
-
-    // Lane i of the warp keeps where its tile (32 n + i) lies, and issues
-    // its copy.  Bit i of `bad`: that tile's page is outside the cache.
-    long long where = -1;
-    uint32_t bad_now = 0, bad_issue = 0;
-    auto locate = [&](int first) {
-      const int idx = first + lane;
-      where = -1;
-      if (idx < mine) {
-        const int tile = tile0 + warp + idx * kWarps;
+  // Lane W j + u of the warp keeps where tile u of its step (n 32 / W + j)
+  // lies, and issues its copy.  Bit W j + u of `bad`: the page of that tile is
+  // outside the cache.
+  constexpr int kBatch = 32 / W;
+  // A warp on its own runs ahead into the next unit; warps together stop at
+  // the unit's end, `last`, where the rings serve the merge.
+  const unsigned char *where = nullptr;
+  uint32_t bad_now = 0, bad_issue = 0;
+  int last = mine, locate_from = 0;
+  auto locate = [&](int first) {
+    const int i = first + lane / W;
+    where = nullptr;
+    bool bad = false;
+    if (k0 + kEvery * i < last) {
+      const Place pl = place_of<W>(a, wk, prefix, lens, begin + k0 + kEvery * i);
+      const int tile = (pl.first >> 4) + W * (reverse ? pl.steps - 1 - pl.at : pl.at) + lane % W;
+      if (tile * 16 < pl.kl) {
         const int page = tile / tpp;
-        where = kv4_page_offset(c, b, page);
-        if (where >= 0) where += (long long)(tile - page * tpp) * Sh::kTile;
+        const long long off = kv4_page_offset(c, pl.b, page);
+        bad = off < 0;
+        if (!bad) where = c.data + pl.kvh * c.head_stride + off + (tile - page * tpp) * Sh::kTile;
       }
-      bad_issue = __ballot_sync(0xffffffffu, idx < mine && where < 0);
-    };
-    auto issue = [&](int i, int stage) {
-      if (lane == i % 32 && where >= 0) {
-        sm100::mbar_arrive_expect_tx(&sm_full[warp][stage], Sh::kTile);
-        bulk_load(ring + stage * Sh::kTile, base + where, Sh::kTile, &sm_full[warp][stage]);
-      }
-    };
-    if (lane == 0) {
-#pragma unroll
-      for (int i = 0; i < kStages; ++i) sm100::mbar_init(&sm_full[warp][i], 1);
-      sm100::fence_mbar_init();
     }
+    bad_issue = __ballot_sync(0xffffffffu, bad);
+  };
+  auto issue = [&](int i, int stage) {
+    if (lane / W == (i - locate_from) % kBatch) {
+      if (where != nullptr) {
+        sm100::mbar_arrive_expect_tx(bar + stage, Sh::kTile);
+        bulk_load(ring + (W * stage + lane % W) * Sh::kTile, where, Sh::kTile, bar + stage);
+      } else {
+        sm100::mbar_arrive(bar + stage);
+      }
+    }
+  };
+  if constexpr (!COOP) {
     locate(0);
-    bad_now = bad_issue;
-    __syncwarp();
 #pragma unroll
     for (int i = 0; i < kStages; ++i)
       if (i < mine) issue(i, i);
+  }
 
-    // Query rows to fp16, scaled by a power of two, in the order of the
-    // operand fragments, with the factor that undoes the scale and the sums
-    // of their groups.  Lane l holds D / 32 consecutive channels.
-    constexpr int E = D / 32;
-    for (int r = warp; r < R; r += kWarps) {
-      const bool live = r0 + r < rows && (r0 + r) / a.group < ql;
-      float x[E];
-      float top = 0.f, sum = 0.f;
-      int lo = 0, hi = 0;
-      float slope = 0.f;
+  // Where this lane's column finds q for tile `sl`: in its own tile's columns,
+  // elsewhere zeros.
+  const int my_slot = SLOTS > 1 ? 2 * t / kTileCols : 0;  // tile of this lane's accumulator columns 2t, 2t + 1
+  uint32_t q_at[SLOTS];
+#pragma unroll
+  for (int sl = 0; sl < SLOTS; ++sl)
+    q_at[sl] = (SLOTS > 1 && g / kTileCols != sl ? sm100::smem_u32(zeros) : sm100::smem_u32(q_own)) + lane * 16;
+
+  uint32_t at = ring, phase = 0;
+  uint64_t wait_ns = kWaitNs;
+  int stage = 0;
+  int mine_done = 0;  // steps that this warp has taken
+  for (int done = 0, n_steps; done < mine; done += n_steps) {
+    // ---- the next unit, or the share's part of it
+    const Place pl = place_of<W>(a, wk, prefix, lens, begin + done);
+    const int b = pl.b, kvh = pl.kvh, r0 = pl.block * R, ql = pl.ql, kl = pl.kl, first = pl.first;
+    const int rows = ql * a.group;  // pair r: query row r / group, head r % group of the kv head
+    n_steps = min(mine - done, pl.steps - pl.at);
+    const int before = mine_done;
+    if constexpr (COOP) {
+      // The warp's steps of this unit: indexes i from `before` on with k0 + kEvery i < last.
+      last = done + n_steps;
+      locate_from = before;
+      locate(before);
+#pragma unroll
+      for (int i = 0; i < kStages; ++i)
+        if (k0 + kEvery * (before + i) < last) issue(before + i, (stage + i) % kStages);
+    }
+    // Tokens [lo_in, hi_in) are seen by all rows of the block.
+    int lo_in = 0, hi_in = 0;
+    {
+      int x;
+      row_range(a, r0 / a.group, ql, kl, x, hi_in);
+      row_range(a, (min(r0 + R, rows) - 1) / a.group, ql, kl, lo_in, x);
+    }
+
+    // q as 16-bit integers of its row's largest value, high and low byte, in
+    // the order of the operand fragments; with the factor that undoes the
+    // scale and the sums of the groups.  A lane takes 16 channels of a pair.
+    // An infinity makes the factor one, and so the scores NaN (0 inf).
+    __syncwarp();
+    constexpr int kLanes = D / 16, kPass = 32 / kLanes;  // lanes of a pair, pairs side by side
+#pragma unroll
+    for (int p0 = COOP ? warp * kPass : 0; p0 < R; p0 += COOP ? kWarps * kPass : kPass) {
+      const int pr = p0 + lane / kLanes, sub = lane % kLanes, r = r0 + pr;
+      const bool here = R % kPass == 0 || pr < R, live = here && r < rows;
+      const int i = r / a.group, h0 = kvh * a.group + r % a.group;
+      uint4 raw[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
       if (live) {
-        const int i = (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
-        const T *p = static_cast<const T *>(a.q) + b * a.qs[0] + i * a.qs[1] + h * a.qs[2] + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = Elem<T>::to_f(p[e]);
-        row_range(a, i, ql, kl, lo, hi);
-        if (a.alibi != nullptr) slope = a.alibi[h] * kLog2e;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (!live) x[e] = 0.f;
-        top = fmaxf(top, fabsf(x[e]));
-        sum += x[e];
-      }
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-#pragma unroll
-      for (int off = 1; off < 32 / G; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      // top in [2^ex, 2^(ex + 1)) goes to [2^14, 2^15).
-      const int ex = max(-112, (int)(__float_as_uint(top) >> 23) - 127);
-      const float up = pow2i(min(126, 14 - ex));
-      const float scale = a.softcap > 0.f ? a.sm_scale / a.softcap : a.sm_scale * kLog2e;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int d = lane * E + e, p = d & 7;
-        // Channels 0..7 of a word go to halves 0, 2, 4, 6, 1, 3, 5, 7 of the
-        // fragment; the odd ones meet nibbles that are 16 times too large.
-        const int at = ((((r >> 3) * G + (d >> 6)) * 2 + ((d >> 3) & 1)) * 32 + 4 * (r & 7) + ((d >> 4) & 3)) * 8 +
-                       (p & 3) * 2 + (p >> 2);
-        sm_q[at] = __float2half_rn(x[e] * (p & 1 ? up * 0.0625f : up));
-      }
-      if (lane == 0) {
-        // 2^24 for the subnormals, 2^(ex - 14) for the scaling.
-        sm_f[r] = scale * 0x1p24f * pow2i(max(-126, ex - 14));
-        sm_lo[r] = lo;
-        sm_hi[r] = hi;
-        sm_slope[r] = slope;
-      }
-      if (lane % (32 / G) == 0) sm_qs[lane / (32 / G)][r] = sum * scale;
-    }
-    __syncthreads();
-
-    uint4 qf[Sh::kQRegs ? NT * G * 2 : 1];
-    float2 fac_r[Sh::kQRegs ? NT : 1], qs_r[Sh::kQRegs ? NT * G : 1];
-    const uint32_t q_at = sm100::smem_u32(sm_q) + lane * 16;
-    if constexpr (Sh::kQRegs) {
-#pragma unroll
-      for (int i = 0; i < NT * G * 2; ++i) qf[i] = lds16(q_at + i * 512);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        fac_r[n] = *reinterpret_cast<const float2 *>(&sm_f[n * 8 + 2 * t]);
-#pragma unroll
-        for (int h = 0; h < G; ++h) qs_r[n * G + h] = *reinterpret_cast<const float2 *>(&sm_qs[h][n * 8 + 2 * t]);
-      }
-    }
-
-    // One tile at shared address `at`, tokens tok0 ..  PART: some row does
-    // not see all of its tokens.
-    auto compute = [&](uint32_t at, int tok0, auto part_tag) {
-      constexpr bool PART = decltype(part_tag)::value;
-      uint32_t par[2][2 * G];  // parameters of tokens g, g + 8: [K groups, V groups]
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t q = at + G * 1024 + (g + 8 * r) * (8 * G);
-        if constexpr (G == 1) {
-          asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(par[r][0]), "=r"(par[r][1]) : "r"(q));
+        const T *p = static_cast<const T *>(a.q) + b * a.qs[0] + i * a.qs[1] + h0 * a.qs[2] + 16 * sub;
+        if (c.vec) {
+          raw[0] = reinterpret_cast<const uint4 *>(p)[0];
+          raw[1] = reinterpret_cast<const uint4 *>(p)[1];
         } else {
+          const unsigned short *e = reinterpret_cast<const unsigned short *>(p);
+          uint32_t u[8];
 #pragma unroll
-          for (int i = 0; i < G / 2; ++i) {
-            const uint4 u = lds16(q + i * 16);
-            par[r][4 * i] = u.x;
-            par[r][4 * i + 1] = u.y;
-            par[r][4 * i + 2] = u.z;
-            par[r][4 * i + 3] = u.w;
+          for (int x = 0; x < 8; ++x) u[x] = (uint32_t)e[2 * x] | ((uint32_t)e[2 * x + 1] << 16);
+          raw[0] = make_uint4(u[0], u[1], u[2], u[3]);
+          raw[1] = make_uint4(u[4], u[5], u[6], u[7]);
+        }
+      }
+      float f[2][8], top = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        unpack8<T>(raw[w], f[w]);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          top = fmaxf(top, fabsf(f[w][x]));
+          sum += f[w][x];
+        }
+      }
+#pragma unroll
+      for (int off = 1; off < kLanes; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const float up = top > 0.f ? fminf(kQTop / top, 0x1p126f) : 0.f;
+      const float scale = a.softcap > 0.f ? a.sm_scale / a.softcap : a.sm_scale * kLog2e;
+      const int h = sub >> 2, tt = sub & 3;
+      if (here) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint32_t hi8[2] = {0u, 0u}, lo8[2] = {0u, 0u};
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            // A word's even channels are the low nibbles of its bytes (the
+            // first half of the 32 the product sums over), the odd ones the high.
+            const int v = __float2int_rn(f[w][x] * up);
+            hi8[x & 1] |= (uint32_t)((v + 128) >> 8 & 255) << (8 * (x >> 1));
+            lo8[x & 1] |= (uint32_t)(v & 255) << (8 * (x >> 1));
+          }
+#pragma unroll
+          for (int sl = 0; sl < SLOTS; ++sl) {
+            const int col = sl * kTileCols + pr * kColStep;
+            uint4 *dst = q_own + (((col >> 3) * G + h) * 2 + w) * 32 + 4 * (col & 7) + tt;
+            dst[0] = make_uint4(hi8[0], hi8[1], lo8[0], lo8[1]);
+            if constexpr (NQ == 1) dst[4] = make_uint4(lo8[0], lo8[1], 0u, 0u);
+          }
+        }
+#pragma unroll
+        for (int sl = 0; sl < SLOTS; ++sl) {
+          const int col = sl * kTileCols + pr * kColStep;
+          if (tt == 0) row_qs[h * kCols + col] = sum * scale;
+          if (sub == 0) {
+            int lo, hi;
+            row_range(a, live ? i : ql - 1, ql, kl, lo, hi);  // a column without a row goes with the last one
+            row_f[col] = up > 0.f ? scale / up : 0.f;
+            row_slope[col] = live && a.alibi != nullptr ? a.alibi[h0] * kLog2e : 0.f;
+            row_lo[col] = lo;
+            row_hi[col] = hi;
           }
         }
       }
-      // Scores, less the rows' references.
-      float s[NT][4];
+    }
+    if constexpr (COOP) __syncthreads();
+    else __syncwarp();
+
+    // Weights are kept as 2^(S - ref) with one reference per row: the running
+    // maximum less a power of two that brings the largest step times the
+    // largest weight into fp16's upper range (kStepExp).
+    float o[G][4][4];
+    float l[NQ], aff[NQ][G], ref[NQ];
+    // What a score starts from: minus its row's reference, which with a
+    // soft-cap comes off behind the tanh.  0 while there is none.
+    float start[NQ], after[NQ];
+    int step_exp = kMinStepExp;
+    bool fresh = true;                   // some row has no reference yet (the same in all lanes)
+    float limit = 0.f, next_step = 0.f;  // a score above `limit` or a step from `next_step` on moves the references
+    {
+#pragma unroll
+      for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[h][i][x] = 0.f;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        l[q] = start[q] = after[q] = 0.f;
+        ref[q] = -CUDART_INF_F;
+#pragma unroll
+        for (int h = 0; h < G; ++h) aff[q][h] = 0.f;
+      }
+    }
+
+    // SLOTS tiles at shared address `at`, tokens tok0 ..  PART: some row does
+    // not see all of their tokens; bit u of `lost`: tile u has no page.
+    auto compute = [&](uint32_t at, int tok0, uint32_t lost, auto part_tag) {
+      constexpr bool PART = decltype(part_tag)::value;
+      const uint32_t mine_at = at + my_slot * Sh::kTile;  // the tile of this lane's columns
+      const int tok = tok0 + 16 * my_slot + g;
+      // ---- scores, less the rows' references
+      float s[2][NQ];
       {
-        float acc[NT][G][4];
+        // High and low byte of q; with NQ = 1 columns 2t and 2t + 1 of one.
+        constexpr int B = NQ == 1 ? 1 : 2;
+        int acc[G][B][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int sl = 0; sl < SLOTS; ++sl)
 #pragma unroll
-          for (int h = 0; h < G; ++h)
+          for (int h = 0; h < G; ++h) {
+            uint32_t kw[2][2];  // [token g, g + 8][word]
+            lds_k<G>(kw, at + sl * Sh::kTile + lane * 16, h);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) acc[n][h][x] = 0.f;
-        uint4 kw[G];
-#pragma unroll
-        for (int i = 0; i < G; ++i) kw[i] = lds16(at + i * 512 + lane * 16);
-#pragma unroll
-        for (int h = 0; h < G; ++h)
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const int x0 = h * 2 + w, x1 = (G + h) * 2 + w;
-            uint32_t k0 = word_of(kw[x0 / 4], x0 % 4), k1 = word_of(kw[x1 / 4], x1 % 4);
-            uint32_t af[2][4];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              af[half][0] = k0 & 0x000f000fu;
-              af[half][1] = k1 & 0x000f000fu;
-              af[half][2] = k0 & 0x00f000f0u;
-              af[half][3] = k1 & 0x00f000f0u;
-              k0 >>= 8;
-              k1 >>= 8;
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              uint4 qw;
-              if constexpr (Sh::kQRegs) qw = qf[(n * G + h) * 2 + w];
-              else qw = lds16(q_at + ((n * G + h) * 2 + w) * 512);
-              mma16816(acc[n][h], af[0][0], af[0][1], af[0][2], af[0][3], qw.x, qw.y);
-              mma16816(acc[n][h], af[1][0], af[1][1], af[1][2], af[1][3], qw.z, qw.w);
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t a0 = kw[0][w] & 0x0f0f0f0fu, a2 = (kw[0][w] >> 4) & 0x0f0f0f0fu;
+              const uint32_t a1 = kw[1][w] & 0x0f0f0f0fu, a3 = (kw[1][w] >> 4) & 0x0f0f0f0fu;
+              {
+                const uint4 qw = lds16(q_at[sl] + (h * 2 + w) * 512);
+                if (w == 0 && sl == 0) {
+                  imma16832_first(acc[h][0], a0, a1, a2, a3, qw.x, qw.y);
+                  if constexpr (B == 2) imma16832_first(acc[h][B - 1], a0, a1, a2, a3, qw.z, qw.w);
+                } else {
+                  imma16832(acc[h][0], a0, a1, a2, a3, qw.x, qw.y);
+                  if constexpr (B == 2) imma16832(acc[h][B - 1], a0, a1, a2, a3, qw.z, qw.w);
+                }
+              }
             }
           }
         float2 kp[2][G];
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2; ++r) {
+          uint32_t par[G];
+          lds_params<G>(par, mine_at + G * 1024 + (g + 8 * r) * (8 * G));
 #pragma unroll
-          for (int h = 0; h < G; ++h) kp[r][h] = kv4_unpack_param<T>(par[r][h]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float2 fac, qs[G];
-          if constexpr (Sh::kQRegs) {
-            fac = fac_r[n];
-#pragma unroll
-            for (int h = 0; h < G; ++h) qs[h] = qs_r[n * G + h];
-          } else {
-            fac = *reinterpret_cast<const float2 *>(&sm_f[n * 8 + 2 * t]);
-#pragma unroll
-            for (int h = 0; h < G; ++h) qs[h] = *reinterpret_cast<const float2 *>(&sm_qs[h][n * 8 + 2 * t]);
-          }
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              // With a soft-cap the reference comes off behind the tanh.
-              float off = a.softcap > 0.f || ref[n][q] == -CUDART_INF_F ? 0.f : -ref[n][q];
-              float dot = kp[r][0].x * acc[n][0][2 * r + q];
-              off = fmaf(kp[r][0].y, q ? qs[0].y : qs[0].x, off);
-#pragma unroll
-              for (int h = 1; h < G; ++h) {
-                dot = fmaf(kp[r][h].x, acc[n][h][2 * r + q], dot);
-                off = fmaf(kp[r][h].y, q ? qs[h].y : qs[h].x, off);
-              }
-              s[n][2 * r + q] = fmaf(dot, q ? fac.y : fac.x, off);
-            }
+          for (int h = 0; h < G; ++h) kp[r][h] = kv4_unpack_param<T>(par[h]);
         }
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            const float fac = row_f[2 * t + q];
+            float qs[G];
+#pragma unroll
+            for (int h = 0; h < G; ++h) qs[h] = row_qs[h * kCols + 2 * t + q];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float dot = 0.f, off = start[q];
+#pragma unroll
+              for (int h = 0; h < G; ++h) {
+                const int sum = NQ == 1 ? acc[h][0][2 * r] * 256 + acc[h][0][2 * r + 1]
+                                        : acc[h][0][2 * r + q] * 256 + acc[h][B - 1][2 * r + q];
+                dot = h == 0 ? kp[r][h].x * (float)sum : fmaf(kp[r][h].x, (float)sum, dot);
+                off = fmaf(kp[r][h].y, qs[h], off);
+              }
+              s[r][q] = fmaf(dot, fac, off);
+            }
+          }
       }
       if (a.softcap > 0.f) {
         const float cap2 = a.softcap * kLog2e;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            s[n][x] = fmaf(tanhf(s[n][x]), cap2, ref[n][x & 1] == -CUDART_INF_F ? 0.f : -ref[n][x & 1]);
+            for (int q = 0; q < NQ; ++q) s[r][q] = fmaf(tanhf(s[r][q]), cap2, after[q]);
       }
       if (a.alibi != nullptr) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float2 sl = *reinterpret_cast<const float2 *>(&sm_slope[n * 8 + 2 * t]);
+          for (int q = 0; q < NQ; ++q) {
+            const float slope = row_slope[2 * t + q];
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            s[n][x] = fmaf(x & 1 ? sl.y : sl.x, (float)(tok0 + g + 8 * (x >> 1)), s[n][x]);
-        }
-      }
-      uint32_t vis = 0xffffffffu;
-      if constexpr (PART) {
-        vis = 0;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int2 lo = *reinterpret_cast<const int2 *>(&sm_lo[n * 8 + 2 * t]);
-          const int2 hi = *reinterpret_cast<const int2 *>(&sm_hi[n * 8 + 2 * t]);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int j = tok0 + g + 8 * (x >> 1);
-            if (j >= max(x & 1 ? lo.y : lo.x, t_lo) && j < min(x & 1 ? hi.y : hi.x, t_hi)) vis |= 1u << (n * 4 + x);
-            else s[n][x] = -CUDART_INF_F;
+            for (int r = 0; r < 2; ++r) s[r][q] = fmaf(slope, (float)(tok + 8 * r), s[r][q]);
           }
-        }
       }
-      // V's steps and centres; a token that no row sees may hold anything.
+      uint32_t vis = 0;  // bit r NQ + q; only with PART
+      if constexpr (PART) {
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            const int lo = row_lo[2 * t + q], hi = row_hi[2 * t + q];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int j = tok + 8 * r;
+              if (j >= lo && j < hi && !(lost >> my_slot & 1u)) vis |= 1u << r * NQ + q;
+              else s[r][q] = -CUDART_INF_F;
+            }
+          }
+      }
+      // ---- V's steps and centres; a token that no row sees may hold anything
       float sv[2][G], cv[2][G];
-      float smax = 0.f;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
+        uint32_t par[G];
+        lds_params<G>(par, mine_at + G * 1024 + (g + 8 * r) * (8 * G) + 4 * G);
+        bool dead = false;
+        if constexpr (PART) {
+          dead = true;
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) dead = dead && !(vis >> r * NQ + q & 1u);
+        }
 #pragma unroll
         for (int h = 0; h < G; ++h) {
-          float2 p = kv4_unpack_param<T>(par[r][G + h]);
-          if (PART && (vis & (0x33333333u << (2 * r))) == 0) p = make_float2(0.f, 0.f);
+          float2 p = kv4_unpack_param<T>(par[h]);
+          if (dead) p = make_float2(0.f, 0.f);
           sv[r][h] = p.x;
           cv[r][h] = fmaf(8.f, p.x, p.y);
-          smax = fmaxf(smax, p.x);
         }
       }
-      // The references move, with everything accumulated, when a score
-      // passes its row's maximum by kLazyMax or a larger step turns up.
-      const float limit = kLazyMax + (float)(kStepExp - step_exp);
-      float most = s[0][0];
-      bool first = false;  // a row without a reference so far
+      // ---- the references move, with everything accumulated, when a score
+      // passes its row's maximum by kLazyMax or a larger step turns up
+      float most = -CUDART_INF_F, smax = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+        for (int q = 0; q < NQ; ++q) most = max3(most, s[0][q], s[1][q]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) most = fmaxf(most, s[n][x]);
-        first |= ref[n][0] == -CUDART_INF_F || ref[n][1] == -CUDART_INF_F;
-      }
-      if (__any_sync(0xffffffffu, first || most > limit || smax >= pow2i(step_exp + 1))) {
+      for (int h = 0; h < G; ++h) smax = max3(smax, sv[0][h], sv[1][h]);
+      if (__any_sync(0xffffffffu, fresh || most > limit || smax >= next_step)) {
         uint32_t bits = 0;
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
           for (int h = 0; h < G; ++h) {
-            const uint32_t u = __float_as_uint(sv[r][h]);
-            bits = max(bits, u < 0x7f800000u ? u : 0u);
+            const uint32_t x = __float_as_uint(sv[r][h]);
+            bits = max(bits, x < 0x7f800000u ? x : 0u);
           }
         const int new_exp = max(step_exp, min(kMaxStepExp, (int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 127));
         const float old_room = (float)(kStepExp - step_exp), new_room = (float)(kStepExp - new_exp);
         step_exp = new_exp;
+        limit = kLazyMax + new_room;
+        next_step = pow2i(new_exp + 1);
+        bool missing = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const bool none = ref[n][q] == -CUDART_INF_F;
-            const float shift = none ? 0.f : ref[n][q];
-            float v = fmaxf(s[n][q], s[n][2 + q]) + shift;
+          for (int q = 0; q < NQ; ++q) {
+            const bool none = ref[q] == -CUDART_INF_F;
+            const float shift = none ? 0.f : ref[q];
+            float v = fmaxf(s[0][q], s[1][q]) + shift;
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-            const float m = none ? v : fmaxf(ref[n][q] + old_room, v);
+            const float m = none ? v : fmaxf(ref[q] + old_room, v);
             const float now = m == -CUDART_INF_F ? m : m - new_room;
-            const float al = none ? 1.f : exp2_fast(ref[n][q] - now);
+            const float al = none ? 1.f : exp2_fast(ref[q] - now);
             const float back = now == -CUDART_INF_F ? 0.f : shift - now;
-            ref[n][q] = now;
-            s[n][q] += back;
-            s[n][2 + q] += back;
-            l[n][q] *= al;
+            ref[q] = now;
+            missing |= now == -CUDART_INF_F;
+            const float minus = now == -CUDART_INF_F ? 0.f : -now;
+            start[q] = a.softcap > 0.f ? 0.f : minus;
+            after[q] = minus;
+            s[0][q] += back;
+            s[1][q] += back;
+            l[q] *= al;
 #pragma unroll
             for (int h = 0; h < G; ++h) {
-              aff[n][q][h] *= al;
+              aff[q][h] *= al;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                o[n][h][i][q] *= al;
-                o[n][h][i][2 + q] *= al;
+                o[h][i][q] *= al;
+                o[h][i][2 + q] *= al;
               }
             }
           }
+        fresh = __any_sync(0xffffffffu, missing);
       }
-      // Weights.
-      uint32_t pf[NT][G][2];
+      // ---- weights
+      uint32_t pf[G][2];
+      {
+        float p[2][NQ];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float p[4];
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          p[x] = exp2_fast(s[n][x]);
-          l[n][x & 1] += p[x];
-        }
+          for (int q = 0; q < NQ; ++q) {
+            p[r][q] = exp2_fast(s[r][q]);
+            l[q] += p[r][q];
+          }
 #pragma unroll
         for (int h = 0; h < G; ++h)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float w[2];
+            float w[2] = {0.f, 0.f};
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              w[q] = p[2 * r + q] * sv[r][h];
-              float f = p[2 * r + q] * cv[r][h];
+            for (int q = 0; q < NQ; ++q) {
+              w[q] = p[r][q] * sv[r][h];
               if constexpr (PART) {
-                const bool ok = vis >> (n * 4 + 2 * r + q) & 1u;
-                w[q] = ok ? w[q] : 0.f;
-                f = ok ? f : 0.f;
-                aff[n][q][h] += f;
+                const bool ok = vis >> r * NQ + q & 1u;
+                if (!ok) w[q] = 0.f;
+                aff[q][h] += ok ? p[r][q] * cv[r][h] : 0.f;
               } else {
-                aff[n][q][h] = fmaf(p[2 * r + q], cv[r][h], aff[n][q][h]);
+                aff[q][h] = fmaf(p[r][q], cv[r][h], aff[q][h]);
               }
             }
-            pf[n][h][r] = transpose8x8(pack_half2(w[0], w[1]));
+            pf[h][r] = transpose8x8(pack_half2(w[0], w[1]));
           }
       }
-      // O^T += V^T P^T.
-      uint4 vw[G];
+      // ---- O^T += V^T P^T, each tile with its own columns
 #pragma unroll
-      for (int i = 0; i < G; ++i) vw[i] = lds16(at + G * 512 + i * 512 + lane * 16);
+      for (int sl = 0; sl < SLOTS; ++sl) {
+        const uint32_t tile = at + sl * Sh::kTile + G * 512;
+        uint4 vw[G];
 #pragma unroll
-      for (int h = 0; h < G; ++h) {
-        uint32_t w[4];
+        for (int i = 0; i < G; ++i) vw[i] = lds16(tile + i * 512 + lane * 16);
 #pragma unroll
-        for (int sl = 0; sl < 4; ++sl) w[sl] = word_of(vw[(sl * G + h) / 4], (sl * G + h) % 4);
+        for (int h = 0; h < G; ++h) {
+          uint32_t w[4], pb[2];
 #pragma unroll
-        for (int part16 = 0; part16 < 2; ++part16) {
-          uint32_t z0 = __byte_perm(w[0], w[1], part16 ? 0x7632 : 0x5410);
-          uint32_t z1 = __byte_perm(w[2], w[3], part16 ? 0x7632 : 0x5410);
+          for (int k = 0; k < 4; ++k) w[k] = word_of(vw[(k * G + h) / 4], (k * G + h) % 4);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t a0 = centred_lo(z0), a1 = centred_hi(z0), a2 = centred_lo(z1), a3 = centred_hi(z1);
+            for (int r = 0; r < 2; ++r) pb[r] = SLOTS == 1 || g / kTileCols == sl ? pf[h][r] : 0u;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816(o[n][h][2 * part16 + half], a0, a1, a2, a3, pf[n][h][0], pf[n][h][1]);
-            z0 >>= 8;
-            z1 >>= 8;
+          for (int part16 = 0; part16 < 2; ++part16) {
+            uint32_t z0 = __byte_perm(w[0], w[1], part16 ? 0x7632 : 0x5410);
+            uint32_t z1 = __byte_perm(w[2], w[3], part16 ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t a0 = centred_lo(z0), a1 = centred_hi(z0), a2 = centred_lo(z1), a3 = centred_hi(z1);
+              mma16816(o[h][2 * part16 + half], a0, a1, a2, a3, pb[0], pb[1]);
+              z0 >>= 8;
+              z1 >>= 8;
+            }
           }
         }
       }
     };
 
-    const int full_lo = max(lo_in, t_lo), full_hi = min(hi_in, t_hi);
-    int stage = 0;
-    uint32_t parity = 0;  // bit s: parity of stage s's next phase
-    for (int i = 0; i < mine; ++i) {
-      if (i % 32 == 0) bad_now = bad_issue;
-      if (!(bad_now >> (i % 32) & 1u)) {
-        const bool ok = sm100::mbar_wait(&sm_full[warp][stage], parity >> stage & 1u, kWaitNs);
-        if (!__all_sync(0xffffffffu, ok)) {
-          // Never seen to happen: the copy did not arrive in a second.  The
-          // copies in flight get as long again before the CTA goes on.
-          raise_error(a.err, kDevErrTimeout);
-          for (int k = 0; k < kStages && i + k < mine; ++k) {
-            const int st = (stage + k) % kStages;
-            if (!(bad_now >> ((i + k) % 32) & 1u)) sm100::mbar_wait(&sm_full[warp][st], parity >> st & 1u, kWaitNs);
-          }
-          break;
-        }
-        parity ^= 1u << stage;
-        const int tok0 = (tile0 + warp + i * kWarps) << 4;
-        if (tok0 >= full_lo && tok0 + 16 <= full_hi) compute(ring + stage * Sh::kTile, tok0, std::false_type{});
-        else compute(ring + stage * Sh::kTile, tok0, std::true_type{});
+    // Steps [whole_lo, whole_lo + whole) of the unit lie inside what every row sees.
+    const int whole_lo = max(0, (lo_in - first + 16 * W - 1) / (16 * W));
+    const int whole = max(0, (hi_in - first) / (16 * W) - whole_lo);
+    for (int k; (k = k0 + kEvery * mine_done) < done + n_steps; ++mine_done) {
+      // A copy that does not arrive in a second (never seen to happen) sets
+      // the error word; the warp goes on without waiting again.
+      if (!sm100::mbar_wait(bar + stage, phase, wait_ns)) {
+        raise_error(a.err, kDevErrTimeout);
+        wait_ns = 0;
       }
-      const int next = i + kStages;
-      if (next % 32 == 0) locate(next);
+      const int in_batch = (mine_done - locate_from) % kBatch;
+      if (in_batch == 0) bad_now = bad_issue;
+      const int order = pl.at + k - done;
+      const int st = reverse ? pl.steps - 1 - order : order;
+      const int tok0 = first + 16 * W * st;
+      const uint32_t lost = bad_now >> (in_batch * W) & ((1u << W) - 1u);
+#pragma unroll
+      for (int u = 0; u < W; u += SLOTS) {
+        if ((unsigned)(st - whole_lo) < (unsigned)whole && lost == 0)
+          compute(at + u * Sh::kTile, tok0 + 16 * u, 0u, std::false_type{});
+        else
+          compute(at + u * Sh::kTile, tok0 + 16 * u, lost >> u, std::true_type{});
+      }
+      const int next = mine_done + kStages;
+      if ((next - locate_from) % kBatch == 0) locate(next);
       __syncwarp();  // the warp has read the stage
-      if (next < mine) issue(next, stage);
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      if (k0 + kEvery * next < last) issue(next, stage);
+      at += W * Sh::kTile;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
+        at = ring;
+      }
+    }
+
+    // ---- the unit's result: sums over the tokens (lanes with the same t hold
+    // the same rows), then over the tiles' columns
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          l[q] += __shfl_xor_sync(0xffffffffu, l[q], off);
+#pragma unroll
+          for (int h = 0; h < G; ++h) aff[q][h] += __shfl_xor_sync(0xffffffffu, aff[q][h], off);
+        }
+        float out[G][8];
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            out[h][2 * i] = o[h][i][q] + aff[q][h];
+            out[h][2 * i + 1] = fmaf(o[h][i][2 + q], 0.0625f, aff[q][h]);
+          }
+        float m = ref[q], sum = l[q];
+        if constexpr (SLOTS == 2) {
+          const float other = __shfl_xor_sync(0xffffffffu, m, 2);
+          const float both = fmaxf(m, other);
+          // Columns that saw no finite score add nothing, unless their sum is a NaN.
+          const float wt = m == -CUDART_INF_F ? (sum == sum ? 0.f : 1.f) : exp2_fast(m - both);
+          m = both;
+          sum *= wt;
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+          for (int h = 0; h < G; ++h)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              out[h][x] = wt == 0.f ? 0.f : out[h][x] * wt;
+              out[h][x] += __shfl_xor_sync(0xffffffffu, out[h][x], 2);
+            }
+        }
+        const int pr = (2 * t + q) % kTileCols / kColStep, r = r0 + pr;
+        if constexpr (COOP) {
+          if (my_slot == 0 && r < rows) {
+            float *dst = reinterpret_cast<float *>(own) + pr * Sh::kMergeRow + 8 * g;
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+              *reinterpret_cast<float4 *>(dst + 64 * h) = make_float4(out[h][0], out[h][1], out[h][2], out[h][3]);
+              *reinterpret_cast<float4 *>(dst + 64 * h + 4) = make_float4(out[h][4], out[h][5], out[h][6], out[h][7]);
+            }
+            if (g == 0) {
+              sm_m[warp][pr] = m;
+              sm_l[warp][pr] = sum;
+            }
+          }
+        } else if (my_slot == 0 && r < rows) {
+          const bool none = sum == 0.f;
+          const float inv = 1.f / sum;
+          const float lse = none ? -CUDART_INF_F : (m == -CUDART_INF_F ? sum : (m + log2f(sum)) * kLn2);
+#pragma unroll
+          for (int h = 0; h < G; ++h)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) out[h][x] = none ? 0.f : out[h][x] * inv;
+          const int i = r / a.group, h0 = kvh * a.group + r % a.group;
+          if (n_steps == pl.steps) {
+            T *op = static_cast<T *>(a.o) + b * a.os[0] + i * a.os[1] + h0 * a.os[2] + 8 * g;
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+              if (c.vec) {
+                *reinterpret_cast<uint4 *>(op + 64 * h) = pack8<T>(out[h]);
+              } else {
+#pragma unroll
+                for (int x = 0; x < 8; ++x) op[64 * h + x] = Elem<T>::from_f(out[h][x]);
+              }
+            }
+            if (a.lse != nullptr && g == 0) a.lse[((long long)b * a.H + h0) * a.Sq + i] = lse;
+          } else {
+            // Slot 1 for the unit that begins in this share, slot 0 for the
+            // one that began before it.
+            const long long row = ((long long)worker * 2 + (pl.at == 0 ? 1 : 0)) * R + pr;
+            float *dst = part_o + row * D + 8 * g;
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+              *reinterpret_cast<float4 *>(dst + 64 * h) = make_float4(out[h][0], out[h][1], out[h][2], out[h][3]);
+              *reinterpret_cast<float4 *>(dst + 64 * h + 4) = make_float4(out[h][4], out[h][5], out[h][6], out[h][7]);
+            }
+            if (g == 0) part_lse[row] = lse;
+          }
+        }
+      }
+    if constexpr (COOP) {
+      // The warps' sums, four channels a thread.
+      __syncthreads();
+      const int live = min(R, rows - r0);
+      for (int e = tid; e < live * (D / 4); e += kThreads) {
+        const int pr = e / (D / 4), d = e % (D / 4) * 4;
+        float mw[kWarps], top = -CUDART_INF_F;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          mw[w] = sm_m[w][pr];
+          top = fmaxf(top, mw[w]);
+        }
+        float sum = 0.f;
+        float4 ov = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float lw = sm_l[w][pr];
+          // A warp that saw no finite score adds nothing, unless its sum is a NaN.
+          if (mw[w] == -CUDART_INF_F && lw == lw) continue;
+          const float wt = mw[w] == -CUDART_INF_F ? 1.f : exp2_fast(mw[w] - top);
+          const float4 x = *reinterpret_cast<const float4 *>(smem + w * Sh::kRing + (pr * Sh::kMergeRow + d) * 4);
+          sum = fmaf(lw, wt, sum);
+          ov.x = fmaf(x.x, wt, ov.x);
+          ov.y = fmaf(x.y, wt, ov.y);
+          ov.z = fmaf(x.z, wt, ov.z);
+          ov.w = fmaf(x.w, wt, ov.w);
+        }
+        const bool none = sum == 0.f;
+        const float inv = none ? 0.f : 1.f / sum;
+        const float lse = none ? -CUDART_INF_F : (top == -CUDART_INF_F ? sum : (top + log2f(sum)) * kLn2);
+        ov = make_float4(ov.x * inv, ov.y * inv, ov.z * inv, ov.w * inv);
+        const int r = r0 + pr, i = r / a.group, h0 = kvh * a.group + r % a.group;
+        if (n_steps == pl.steps) {
+          T *op = static_cast<T *>(a.o) + b * a.os[0] + i * a.os[1] + h0 * a.os[2] + d;
+          if (c.vec) {
+            const float f[4] = {ov.x, ov.y, ov.z, ov.w};
+            store4<T>(op, f);
+          } else {
+            op[0] = Elem<T>::from_f(ov.x);
+            op[1] = Elem<T>::from_f(ov.y);
+            op[2] = Elem<T>::from_f(ov.z);
+            op[3] = Elem<T>::from_f(ov.w);
+          }
+          if (a.lse != nullptr && d == 0) a.lse[((long long)b * a.H + h0) * a.Sq + i] = lse;
+        } else {
+          const long long row = ((long long)worker * 2 + (pl.at == 0 ? 1 : 0)) * R + pr;
+          *reinterpret_cast<float4 *>(part_o + row * D + d) = ov;
+          if (d == 0) part_lse[row] = lse;
+        }
+      }
+      // The next unit's copies come after these reads and writes.
+      sm100::fence_proxy_async_smem();
+      __syncthreads();
     }
   }
-
-  // Sums over the tokens of the warp (lanes with the same t hold the same rows).
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        l[n][q] += __shfl_xor_sync(0xffffffffu, l[n][q], off);
-#pragma unroll
-        for (int h = 0; h < G; ++h) aff[n][q][h] += __shfl_xor_sync(0xffffffffu, aff[n][q][h], off);
-      }
-    }
-  __syncthreads();  // every warp is through with its ring
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int r = n * 8 + 2 * t + q;
-      if (g == 0) {
-        sm_m[warp][r] = ref[n][q];
-        sm_l[warp][r] = l[n][q];
-      }
-      float *dst = sm_o + (warp * R + r) * LDO;
-#pragma unroll
-      for (int h = 0; h < G; ++h) {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[2 * i] = o[n][h][i][q] + aff[n][q][h];
-          v[2 * i + 1] = fmaf(o[n][h][i][2 + q], 0.0625f, aff[n][q][h]);
-        }
-        float4 *d4 = reinterpret_cast<float4 *>(dst + 64 * h + 8 * g);
-        d4[0] = make_float4(v[0], v[1], v[2], v[3]);
-        d4[1] = make_float4(v[4], v[5], v[6], v[7]);
-      }
-    }
-  __syncthreads();
-
-  // Merge the warps.
-  for (int e = tid; e < R * D; e += kThreads) {
-    const int r = e / D, d = e % D;
-    if (r0 + r >= rows) break;
-    float top = -CUDART_INF_F;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
-    float lsum = 0.f, ov = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float wt = sm_m[w][r] == -CUDART_INF_F ? 0.f : exp2f(sm_m[w][r] - top);
-      // A warp that saw no finite score adds nothing, unless its sum is a NaN.
-      lsum += wt == 0.f ? (sm_l[w][r] == sm_l[w][r] ? 0.f : sm_l[w][r]) : sm_l[w][r] * wt;
-      ov += wt == 0.f ? 0.f : sm_o[(w * R + r) * LDO + d] * wt;
-    }
-    const bool none = lsum == 0.f;
-    const float inv = none ? 0.f : 1.f / lsum;
-    const float lse = none ? -CUDART_INF_F : (top == -CUDART_INF_F ? lsum : (top + log2f(lsum)) * kLn2);
-    const int i = (r0 + r) / a.group, h = kvh * a.group + (r0 + r) % a.group;
-    if (n_splits == 1) {
-      static_cast<T *>(a.o)[b * a.os[0] + i * a.os[1] + h * a.os[2] + d] = Elem<T>::from_f(ov * inv);
-      if (a.lse != nullptr && d == 0) a.lse[((long long)b * a.H + h) * a.Sq + i] = lse;
-    } else {
-      const long long row = (((long long)split * a.B + b) * a.Sq + i) * a.H + h;
-      part_o[row * D + d] = ov * inv;
-      if (d == 0) part_lse[row] = lse;
-    }
+  if (wait_ns == 0) {
+    // Copies may still be in flight: they get a last second each before the
+    // shared memory goes to another CTA.  (Both parities: which one is due
+    // differs from stage to stage.)
+    for (int st = 0; st < kStages; ++st)
+      for (uint32_t ph = 0; ph < 2; ++ph) sm100::mbar_wait(bar + st, ph, kWaitNs);
   }
 }
 
-// O = sum_s exp(lse_s - lse) O_s over the splits; a warp per output row.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_combine_kernel(AttnArgs a, int chunk, int n_splits, const float *part_o,
-                                                          const float *part_lse) {
+// O = sum_s exp(lse_s - lse) O_s over the shares of a unit that several workers
+// have.  A warp per output row, or with many shares (WIDE) a CTA, whose warps
+// take every fourth one.  A lane has D / 32 channels; four shares are read at
+// a time, before their weights are known.
+template <typename T, int D, int W, bool WIDE>
+__global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Work wk,
+                                                             const float *part_o, const float *part_lse) {
   constexpr int E = D / 32;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits are written
-  const int lane = threadIdx.x % 32;
-  const long long n_rows = (long long)a.B * a.Sq * a.H;
-  const long long row = (long long)blockIdx.x * 4 + threadIdx.x / 32;
-  if (row >= n_rows) return;
-  const int h = (int)(row % a.H), i = (int)(row / a.H % a.Sq), b = (int)(row / a.H / a.Sq);
-  const int ql = clamp_len(a.q_lens, b, a.Sq), kl = clamp_len(a.kv_lens, b, a.Skv);
-  int used = 0;
-  if (i < ql && kl > 0) {
-    int lo, hi;
-    row_range(a, i, ql, kl, lo, hi);
-    const int s0 = first_token(a, ql, kl);
-    if (hi > lo) used = min(n_splits, (hi - s0 + chunk - 1) / chunk);
+  __shared__ float sm_m[kWarps], sm_l[kWarps], sm_o[WIDE ? kWarps : 1][WIDE ? D : 1];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const long long out_row = WIDE ? blockIdx.x : (long long)blockIdx.x * kWarps + warp;
+  if (out_row >= (long long)wk.nb * a.Sq * a.H) return;
+  const int h = (int)(out_row % a.H), i = (int)(out_row / a.H % a.Sq), n = (int)(out_row / a.H / a.Sq), b = wk.b0 + n;
+  const int ql = clamp_len(a.q_lens, b, a.Sq);
+  if (i >= ql) return;  // 0 already
+  // Steps before this sequence, and of all.
+  uint32_t before = 0, all = 0;
+  for (int x = lane; x < wk.nb; x += 32) {
+    const Span sp = span_of<W>(a, wk.R, clamp_len(a.q_lens, wk.b0 + x, a.Sq), clamp_len(a.kv_lens, wk.b0 + x, a.Skv));
+    const uint32_t s = (uint32_t)sp.steps * sp.blocks * a.Hkv;
+    all += s;
+    if (x < n) before += s;
   }
-  float top = -CUDART_INF_F;
-  for (int s = lane; s < used; s += 32) top = fmaxf(top, part_lse[s * n_rows + row]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  float sum = 0.f, o[E];
+  before = __reduce_add_sync(0xffffffffu, before);
+  all = __reduce_add_sync(0xffffffffu, all);
+  const Span sp = span_of<W>(a, wk.R, ql, clamp_len(a.kv_lens, b, a.Skv));
+  if (sp.steps == 0) return;
+  const int shares = share_count(wk, all), R = wk.R;
+  const int r = i * a.group + h % a.group;
+  const uint32_t first = before + (uint32_t)(h / a.group * sp.blocks + r / R) * sp.steps;
+  const int w0 = share_of(all, first, shares), w1 = share_of(all, first + sp.steps - 1, shares);
+  if (w0 == w1) return;  // one worker had the unit whole
+  const int used = w1 - w0 + 1;
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the shares are written
+  constexpr int kStride = WIDE ? kWarps : 1;
+  float m = -CUDART_INF_F, sum = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s = 0; s < used; ++s) {
-    const float ls = part_lse[s * n_rows + row];
-    if (ls == -CUDART_INF_F) continue;
-    const float w = expf(ls - top);  // a NaN goes on into the sum
-    sum += w;
-    const float *p = part_o + (s * n_rows + row) * D + lane * E;
+  for (int s0 = WIDE ? warp : 0; s0 < used; s0 += 4 * kStride) {
+    float l[4], x[4][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(w, p[e], o[e]);
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u * kStride;
+      l[u] = -CUDART_INF_F;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[u][e] = 0.f;
+      if (s < used) {
+        const long long row = ((long long)(w0 + s) * 2 + (s == 0 ? 1 : 0)) * R + r % R;
+        l[u] = part_lse[row];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 v = *reinterpret_cast<const float2 *>(part_o + row * D + lane * E + e);
+          x[u][e] = v.x;
+          x[u][e + 1] = v.y;
+        }
+      }
+    }
+    const float top = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), m);
+    const float al = m == -CUDART_INF_F ? 0.f : expf(m - top);
+    m = top;
+    sum *= al;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= al;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float w = l[u] == -CUDART_INF_F ? 0.f : expf(l[u] - top);  // a NaN goes on into the sum
+      sum += w;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(w, x[u][e], o[e]);
+    }
+  }
+  if constexpr (WIDE) {
+    if (lane == 0) {
+      sm_m[warp] = m;
+      sm_l[warp] = sum;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sm_o[warp][lane * E + e] = o[e];
+    __syncthreads();
+    if (warp != 0) return;
+    m = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+    sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float wt = sm_m[w] == -CUDART_INF_F ? (sm_l[w] == sm_l[w] ? 0.f : 1.f) : expf(sm_m[w] - m);
+      sum = fmaf(sm_l[w], wt, sum);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(sm_o[w][lane * E + e], wt, o[e]);
+    }
   }
   const bool none = sum == 0.f;
   const float inv = none ? 0.f : 1.f / sum;
@@ -726,93 +1112,108 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(AttnArgs a, int chunk,
 #pragma unroll
   for (int e = 0; e < E; ++e) op[e] = Elem<T>::from_f(o[e] * inv);
   if (a.lse != nullptr && lane == 0)
-    a.lse[((long long)b * a.H + h) * a.Sq + i] = none ? -CUDART_INF_F : top + logf(sum);
+    a.lse[((long long)b * a.H + h) * a.Sq + i] = none ? -CUDART_INF_F : m + logf(sum);
 }
 
-template <int D>
-constexpr int max_nt() {
-  return D == 64 ? 4 : (D == 128 ? 4 : 2);
-}
+struct Plan {
+  int rows;        // (head, query row) pairs of one kv head
+  int variant;     // 0: 2 pairs, 1: 4 pairs, 2: 8 pairs a worker
+  int R, tiles;    // pairs of a block, tiles of a step
+  bool coop;       // a CTA's warps share units
+  int ctas;        // of one launch
+  int nb;          // sequences of one launch
+  bool shared;     // several workers may have to share a unit
+  int per_unit;    // about so many
+  size_t ws_bytes;
+};
 
-SplitPlan plan_kv4(const AttnArgs &a, size_t ws_available) {
-  SplitPlan p;
+Plan plan_kv4(const AttnArgs &a) {
+  Plan p;
   p.rows = a.group * a.Sq;
-  const int G = a.D / kKv4Group;
-  const int most = a.D == 256 ? 2 : 4;
-  p.nt = p.rows <= 8 ? 1 : (p.rows <= 16 || most == 2 ? 2 : 4);
-  p.row_blocks = (p.rows + 8 * p.nt - 1) / (8 * p.nt);
-  const long long units = (long long)a.B * a.Hkv * p.row_blocks;
-  const long long slots = (long long)a.num_sms * (p.nt * G <= 2 ? 4 : (p.nt * G <= 4 ? 3 : 2));
+  p.variant = a.D == 256 ? 2 : (p.rows <= 2 ? 0 : (p.rows <= 4 ? 1 : 2));
+  p.R = 2 << p.variant;
+  p.tiles = a.D == 256 ? 1 : 2;
   // Tokens that a sequence's rows can see between them.
   long long span = a.Skv;
-  if (a.window >= 0) span = std::min<long long>(span, (long long)a.window + a.Sq + 16);
-  // One wave of CTAs where that leaves each 128 tokens at least; splits of
-  // 1024 tokens where there is more than a wave of work anyway (sequences
-  // differ in length, so equal shares cannot be dealt from here).
-  long long n = std::max<long long>(1, slots / units);
-  n = std::min(n, (span + 127) / 128);
-  if (units > slots / 2) n = std::max(n, (span + 1023) / 1024);
-  long long chunk = ((span + n - 1) / n + 63) / 64 * 64;
-  p.chunk = (int)chunk;
-  p.n_splits = (int)((span + chunk - 1) / chunk);
-  p.ws_bytes = p.n_splits > 1 ? (size_t)p.n_splits * a.B * a.Sq * a.H * (a.D + 1) * sizeof(float) : 0;
-  if (p.n_splits > 1 && ws_available < p.ws_bytes) {
-    p.n_splits = 1;
-    p.chunk = (int)((span + 63) / 64 * 64);
-  }
+  if (a.window >= 0) span = std::min<long long>(span, (long long)a.window + a.Sq + 15);
+  const long long steps = (span + 15 + 16 * p.tiles - 1) / (16 * p.tiles);
+  const long long per_seq = (long long)a.Hkv * ((p.rows + p.R - 1) / p.R);
+  // (check() has seen to it that one sequence's steps stay below 2^31.)
+  p.nb = (int)std::min<long long>(std::min(a.B, kMaxSlice), std::max<long long>(1, 0x7fffffffLL / (per_seq * steps)));
+  const long long units = p.nb * per_seq, most = units * steps;
+  const int resident = a.num_sms * (a.D <= 128 ? 4 : 3);
+  p.coop = units <= resident;
+  p.shared = p.coop ? steps > 4 * kWarps && units < resident : steps > 1;
+  p.ctas = (int)std::min<long long>(resident, p.shared || !p.coop ? (most + kWarps - 1) / kWarps : units);
+  const long long workers = (long long)p.ctas * (p.coop ? 1 : kWarps);
+  p.per_unit = (int)std::min<long long>(workers, (workers + units - 1) / units);
+  p.ws_bytes = p.shared ? (size_t)workers * 2 * p.R * (a.D + 1) * sizeof(float) : 0;
   return p;
 }
 
-template <typename T, int D, int NT>
-cudaError_t launch_nt(const AttnArgs &a, const Kv4Args &c, const SplitPlan &p, void *ws, cudaStream_t s) {
-  constexpr size_t smem = Shape<D, NT>::kSmem;
+template <typename T, int D, int NQ, int SLOTS, bool COOP>
+cudaError_t launch_variant(const AttnArgs &a, const Kv4Args &c, const Plan &p, bool split, void *ws, cudaStream_t s) {
+  using Sh = Shape<D, NQ, SLOTS, COOP>;
+  const int smem = Sh::kSmem + p.nb * 12 + 4;
   if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kv4_attn_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<T, D, NQ, SLOTS, COOP>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  float *part_o = nullptr, *part_lse = nullptr;
-  const long long n_rows = (long long)a.B * a.Sq * a.H;
-  if (p.n_splits > 1) {
-    part_o = static_cast<float *>(ws);
-    part_lse = part_o + (size_t)p.n_splits * n_rows * D;
+  const size_t workers = (size_t)p.ctas * (COOP ? 1 : kWarps);
+  float *part_o = static_cast<float *>(ws);
+  float *part_lse = split ? part_o + workers * 2 * p.R * D : nullptr;
+  for (int b0 = 0; b0 < a.B; b0 += p.nb) {
+    Work wk;
+    wk.b0 = b0;
+    wk.nb = std::min(p.nb, a.B - b0);
+    wk.R = p.R;
+    wk.workers = (int)workers;
+    wk.min_steps = COOP ? kWarps : 1;
+    wk.split = split ? 1 : 0;
+    kv4_attn_kernel<T, D, NQ, SLOTS, COOP><<<p.ctas, kThreads, smem, s>>>(a, c, wk, part_o, part_lse);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    if (!split) continue;
+    // The merge's launch overlaps the shares; it waits for them itself.
+    const bool wide = p.per_unit > 8;
+    const long long out_rows = (long long)wk.nb * a.Sq * a.H;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(wide ? out_rows : (out_rows + kWarps - 1) / kWarps));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, wide ? kv4_merge_kernel<T, D, Sh::W, true> : kv4_merge_kernel<T, D, Sh::W, false>, a, wk,
+                           (const float *)part_o, (const float *)part_lse);
+    if (e != cudaSuccess) return e;
   }
-  const dim3 grid(p.n_splits, a.Hkv * p.row_blocks, a.B);
-  kv4_attn_kernel<T, D, NT><<<grid, kThreads, smem, s>>>(a, c, p.chunk, p.n_splits, p.row_blocks, part_o, part_lse);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || p.n_splits == 1) return e;
-  // The combine's launch overlaps the splits; it waits for them itself.
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((n_rows + 3) / 4));
-  cfg.blockDim = dim3(128);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D>, a, p.chunk, p.n_splits, (const float *)part_o,
-                            (const float *)part_lse);
+  return cudaSuccess;
+}
+
+template <typename T, int D, bool COOP>
+cudaError_t launch_coop(const AttnArgs &a, const Kv4Args &c, const Plan &p, bool split, void *ws, cudaStream_t s) {
+  if constexpr (D < 256) {
+    if (p.variant == 0) return launch_variant<T, D, 1, 2, COOP>(a, c, p, split, ws, s);
+    if (p.variant == 1) return launch_variant<T, D, 2, 2, COOP>(a, c, p, split, ws, s);
+  }
+  return launch_variant<T, D, 2, 1, COOP>(a, c, p, split, ws, s);
 }
 
 template <typename T, int D>
-cudaError_t launch_d(const AttnArgs &a, const Kv4Args &c, const SplitPlan &p, void *ws, cudaStream_t s) {
-  if (p.nt == 1) return launch_nt<T, D, 1>(a, c, p, ws, s);
-  if constexpr (max_nt<D>() >= 2) {
-    if (p.nt == 2) return launch_nt<T, D, 2>(a, c, p, ws, s);
-  }
-  if constexpr (max_nt<D>() >= 4) {
-    if (p.nt == 4) return launch_nt<T, D, 4>(a, c, p, ws, s);
-  }
-  return cudaErrorNotSupported;
+cudaError_t launch_d(const AttnArgs &a, const Kv4Args &c, const Plan &p, bool split, void *ws, cudaStream_t s) {
+  return p.coop ? launch_coop<T, D, true>(a, c, p, split, ws, s) : launch_coop<T, D, false>(a, c, p, split, ws, s);
 }
 
 template <typename T>
-cudaError_t launch_kv4_attn(const AttnArgs &a, const Kv4Args &c, const SplitPlan &p, void *ws, cudaStream_t s) {
+cudaError_t launch_kv4_attn(const AttnArgs &a, const Kv4Args &c, const Plan &p, bool split, void *ws, cudaStream_t s) {
   switch (a.D) {
-    case 64: return launch_d<T, 64>(a, c, p, ws, s);
-    case 128: return launch_d<T, 128>(a, c, p, ws, s);
-    case 256: return launch_d<T, 256>(a, c, p, ws, s);
+    case 64: return launch_d<T, 64>(a, c, p, split, ws, s);
+    case 128: return launch_d<T, 128>(a, c, p, split, ws, s);
+    case 256: return launch_d<T, 256>(a, c, p, split, ws, s);
   }
   return cudaErrorNotSupported;
 }
@@ -869,8 +1270,12 @@ llmx_status check(const llmx_attn_params *p, const llmx_kv4_cache *c, AttnArgs *
   if (p->algo == LLMX_ALGO_SIMT) return record_error(LLMX_ERR_UNSUPPORTED, "kv4: algo must be AUTO, DECODE or TCGEN05");
   if (((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->o)) & 1u) != 0)
     return bad("kv4: q and o must be aligned to their elements");
-  if ((long long)a->group * a->Sq > 0x3fffffffLL || (long long)a->Hkv * ((a->group * (long long)a->Sq + 7) / 8) > 65535)
+  if ((long long)a->group * a->Sq > 0x3fffffffLL || (long long)std::min(a->B, kMaxSlice) * a->Sq > 65535)
     return bad("kv4: too many query rows for one call");
+  if (((long long)a->Skv / 16 + 2) * a->Hkv * ((long long)a->group * a->Sq / 2 + 1) > 0x7fffffffLL)
+    return bad("kv4: too much work in one sequence (max_kv_len / 16 * n_heads * max_q_len / 2 must be below 2^31)");
+  k->vec = al16(p->q) && al16(p->o);
+  for (int i = 0; i < 3; ++i) k->vec = k->vec && p->q_stride[i] % 8 == 0 && p->o_stride[i] % 8 == 0;
   a->window = std::min(a->window, 1 << 30);  // past every length; keeps the ranges inside 32 bits
   return LLMX_OK;
 }
@@ -892,7 +1297,7 @@ extern "C" llmx_status llmx_kv4_attn_workspace_size(const llmx_attn_params *p, c
   llmx_status refused;
   const bool expand = use_expanded(a, p->algo, &refused);
   if (refused != LLMX_OK) return refused;
-  *bytes = expand ? 2 * expanded_rows_bytes(a) + kSm100WorkspaceBytes : plan_kv4(a, SIZE_MAX).ws_bytes;
+  *bytes = expand ? 2 * expanded_rows_bytes(a) + kSm100WorkspaceBytes : plan_kv4(a).ws_bytes;
   return LLMX_OK;
 }
 
@@ -934,9 +1339,10 @@ extern "C" llmx_status llmx_kv4_attn_fwd(const llmx_attn_params *p, const llmx_k
     return LLMX_OK;
   }
   if (refused != LLMX_OK) return refused;
-  const SplitPlan plan = plan_kv4(a, p->workspace != nullptr ? p->workspace_bytes : 0);
-  const cudaError_t e = a.dtype == LLMX_FP16 ? launch_kv4_attn<__half>(a, k, plan, p->workspace, st)
-                                             : launch_kv4_attn<__nv_bfloat16>(a, k, plan, p->workspace, st);
+  const Plan plan = plan_kv4(a);
+  const bool split = plan.shared && p->workspace != nullptr && p->workspace_bytes >= plan.ws_bytes;
+  const cudaError_t e = a.dtype == LLMX_FP16 ? launch_kv4_attn<__half>(a, k, plan, split, p->workspace, st)
+                                             : launch_kv4_attn<__nv_bfloat16>(a, k, plan, split, p->workspace, st);
   if (e != cudaSuccess) return record_error(LLMX_ERR_CUDA, (std::string("launch failed: ") + cudaGetErrorString(e)).c_str());
   return LLMX_OK;
 }

@@ -13,6 +13,7 @@ struct Kv4Args {
   const int *table;  // nullable
   long long page_stride, head_stride, table_stride;
   int n_pages, max_pages, page_size, Hkv, D;
+  int vec;  // attention: q and o rows can be read and written 16 bytes at a time
   unsigned int *err;
 };
 

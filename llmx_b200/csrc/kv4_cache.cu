@@ -1,8 +1,14 @@
 // Writing rows of K and V into the 4-bit cache and reading them back.
 //
-// One thread takes 8 consecutive channels of one (token, kv head) of K and of
-// V, which is one 32-bit code word of each; the 8 threads of a 64-channel
-// group reduce its minimum and maximum with shuffles.
+// A warp takes one tile of 16 tokens of one kv head, lane (g, t) the words that
+// the layout gives it: 16 channels of K of tokens g and g + 8 per group, 8
+// channels of V of tokens 2t, 2t + 1, 2t + 8, 2t + 9.  Dense rows are moved 16
+// bytes a lane in whole 32-byte sectors, a whole tile in 16-byte words; of a
+// tile that the rows cover in part only the words of their tokens are written.
+// Both are bound by HBM: 4 + 1.125 bytes per (K, V) pair of values.
+//
+// Few rows (a decode step's new token, a short tail) leave such warps idle or
+// alone on their SMs; there a thread takes 8 channels of one row of K and of V.
 #include <string>
 
 #include "kv4.cuh"
@@ -11,6 +17,8 @@ namespace llmx_b200 {
 namespace {
 
 constexpr int kRowThreads = 256;
+// From this many tiles on a warp takes a whole tile.
+constexpr int kManyTiles = 1024;
 
 struct RowArgs {
   const void *k, *v;
@@ -19,16 +27,19 @@ struct RowArgs {
   int B, S, pad;
 };
 
+// 8 consecutive channels.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_row8(const T *p, float (&f)[8]) {
+__device__ __forceinline__ uint4 load_row8(const T *p) {
   if constexpr (VEC) {
-    unpack8<T>(*reinterpret_cast<const uint4 *>(p), f);
+    return *reinterpret_cast<const uint4 *>(p);
   } else {
+    const unsigned short *e = reinterpret_cast<const unsigned short *>(p);
+    uint32_t u[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_f(p[i]);
+    for (int i = 0; i < 4; ++i) u[i] = (uint32_t)e[2 * i] | ((uint32_t)e[2 * i + 1] << 16);
+    return make_uint4(u[0], u[1], u[2], u[3]);
   }
 }
-
 template <typename T, bool VEC>
 __device__ __forceinline__ void store_row8(T *p, const float (&f)[8]) {
   if constexpr (VEC) {
@@ -39,16 +50,29 @@ __device__ __forceinline__ void store_row8(T *p, const float (&f)[8]) {
   }
 }
 
-// min / max that hand a NaN on.
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using type = __half2;
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+
+// Minimum and maximum of values two at a time, both halves apart; a NaN goes on.
+template <typename T>
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  using P = typename Pair<T>::type;
+  const P r = __hmin2_nan(*reinterpret_cast<const P *>(&a), *reinterpret_cast<const P *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&r);
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  using P = typename Pair<T>::type;
+  const P r = __hmax2_nan(*reinterpret_cast<const P *>(&a), *reinterpret_cast<const P *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&r);
 }
 
 template <typename T>
@@ -58,115 +82,379 @@ __device__ __forceinline__ __half round_up_to<__half>(float r) { return __float2
 template <>
 __device__ __forceinline__ __nv_bfloat16 round_up_to<__nv_bfloat16>(float r) { return __float2bfloat16_ru(r); }
 
-// The code word of this thread's 8 channels and the group's parameter word.
-// All 8 threads of the group call it.
-template <typename T>
-__device__ __forceinline__ void quantise8(const float (&f)[8], uint32_t &codes, uint32_t &param) {
-  float lo = f[0], hi = f[0];
+// (min, -max) of the channels of N 16-byte pieces, packed.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t low_high(const uint4 (&raw)[N]) {
+  uint32_t lo = raw[0].x, hi = raw[0].x;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, f[i]);
-    hi = max_nan(hi, f[i]);
-  }
+  for (int i = 0; i < N; ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-  for (int off = 1; off < 8; off <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-  }
-  const T st = round_up_to<T>(__fdiv_rn(hi - lo, 15.f));
-  const T mt = Elem<T>::from_f(lo);  // exact: lo is one of the inputs
-  const float s = Elem<T>::to_f(st);
-  codes = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // s > 0 fails for a NaN too; inf / inf converts to 0.  The group reads
-    // back as NaN then, through s or m.
-    const float q = s > 0.f ? __fdiv_rn(f[i] - lo, s) : 0.f;
-    codes |= (uint32_t)min(15, __float2int_rn(q)) << (4 * i);
-  }
-  const unsigned short sb = *reinterpret_cast<const unsigned short *>(&st);
-  const unsigned short mb = *reinterpret_cast<const unsigned short *>(&mt);
-  param = (uint32_t)sb | ((uint32_t)mb << 16);
-}
-
-template <typename T>
-__device__ __forceinline__ void dequantise8(uint32_t codes, uint32_t param, float (&f)[8]) {
-  const float2 p = kv4_unpack_param<T>(param);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = fmaf((float)((codes >> (4 * i)) & 15u), p.x, p.y);
-}
-
-// Where token `row` of sequence b lies (byte offset of the tile of kv head h)
-// and its place in the tile, or -1.
-__device__ __forceinline__ long long locate(const Kv4Args &a, int b, long long pos, int h, int &tok) {
-  if (pos < 0 || pos >= (long long)a.max_pages * a.page_size) {
-    raise_error(a.err, kDevErrBadPage);
-    return -1;
-  }
-  const int p = (int)(pos / a.page_size), in = (int)(pos - (long long)p * a.page_size);
-  const long long off = kv4_page_offset(a, b, p);
-  if (off < 0) return -1;
-  tok = in & 15;
-  return off + h * a.head_stride + (long long)(in >> 4) * kv4_tile_bytes(a.D);
-}
-
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kRowThreads) kv4_store_kernel(Kv4Args a, RowArgs r) {
-  const int C = a.D / 8, G = a.D / kKv4Group;
-  const int b = blockIdx.y;
-  const long long idx = (long long)blockIdx.x * kRowThreads + threadIdx.x;
-  const int c = (int)(idx % C);
-  const int h = (int)(idx / C % a.Hkv);
-  const long long row = idx / C / a.Hkv;
-  const bool live = row < clamp_len(r.lens, b, r.S);
-  float kf[8] = {}, vf[8] = {};
-  if (live) {
-    load_row8<T, VEC>(static_cast<const T *>(r.k) + b * r.ks[0] + row * r.ks[1] + h * r.ks[2] + c * 8, kf);
-    load_row8<T, VEC>(static_cast<const T *>(r.v) + b * r.vs[0] + row * r.vs[1] + h * r.vs[2] + c * 8, vf);
-  }
-  uint32_t kc, kp, vc, vp;
-  quantise8<T>(kf, kc, kp);
-  quantise8<T>(vf, vc, vp);
-  if (!live) return;
-  int tok = 0;
-  const long long off = locate(a, b, (r.start ? (long long)r.start[b] : 0) + row, h, tok);
-  if (off < 0) return;
-  unsigned char *tile = a.data + off;
-  *reinterpret_cast<uint32_t *>(tile + kv4_k_word(tok, c, G)) = kc;
-  *reinterpret_cast<uint32_t *>(tile + kv4_v_word(tok, c, G)) = vc;
-  if ((c & 7) == 0) {
-    *reinterpret_cast<uint32_t *>(tile + kv4_param(tok, 0, c >> 3, G)) = kp;
-    *reinterpret_cast<uint32_t *>(tile + kv4_param(tok, 1, c >> 3, G)) = vp;
-  }
-}
-
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kRowThreads) kv4_load_kernel(Kv4Args a, RowArgs r) {
-  const int C = a.D / 8, G = a.D / kKv4Group;
-  const int b = blockIdx.y;
-  const long long idx = (long long)blockIdx.x * kRowThreads + threadIdx.x;
-  const int c = (int)(idx % C);
-  const int h = (int)(idx / C % a.Hkv);
-  const long long row = idx / C / a.Hkv;
-  const int len = clamp_len(r.lens, b, r.S);
-  const int end = r.pad > 0 ? min(r.S, (len + r.pad - 1) / r.pad * r.pad) : r.S;
-  if (row >= end) return;
-  float kf[8] = {}, vf[8] = {};
-  if (row < len) {
-    int tok = 0;
-    const long long off = locate(a, b, (r.start ? (long long)r.start[b] : 0) + row, h, tok);
-    if (off >= 0) {
-      const unsigned char *tile = a.data + off;
-      const uint32_t kc = *reinterpret_cast<const uint32_t *>(tile + kv4_k_word(tok, c, G));
-      const uint32_t vc = *reinterpret_cast<const uint32_t *>(tile + kv4_v_word(tok, c, G));
-      const uint32_t kp = *reinterpret_cast<const uint32_t *>(tile + kv4_param(tok, 0, c >> 3, G));
-      const uint32_t vp = *reinterpret_cast<const uint32_t *>(tile + kv4_param(tok, 1, c >> 3, G));
-      dequantise8<T>(kc, kp, kf);
-      dequantise8<T>(vc, vp, vf);
+    for (int x = 0; x < 4; ++x) {
+      lo = min2<T>(lo, w[x]);
+      hi = max2<T>(hi, w[x]);
     }
   }
-  store_row8<T, VEC>(static_cast<T *>(const_cast<void *>(r.k)) + b * r.ks[0] + row * r.ks[1] + h * r.ks[2] + c * 8, kf);
-  store_row8<T, VEC>(static_cast<T *>(const_cast<void *>(r.v)) + b * r.vs[0] + row * r.vs[1] + h * r.vs[2] + c * 8, vf);
+  // The halves of lo and hi against each other: (lo, -hi) of one half with that of the other.
+  return min2<T>(__byte_perm(lo, hi, 0x5410) ^ 0x80000000u, __byte_perm(lo, hi, 0x7632) ^ 0x80000000u);
+}
+
+// A group's parameter word (s, m) from its packed (min, -max).
+template <typename T>
+__device__ __forceinline__ uint32_t param_of(uint32_t low_neg_high) {
+  const uint32_t hi_bits = (low_neg_high >> 16) ^ 0x8000u;
+  const unsigned short lo16 = (unsigned short)low_neg_high, hi16 = (unsigned short)hi_bits;
+  const float range = Elem<T>::to_f(*reinterpret_cast<const T *>(&hi16)) - Elem<T>::to_f(*reinterpret_cast<const T *>(&lo16));
+  const T st = round_up_to<T>(__fdiv_rn(range, 15.f));
+  return (uint32_t) * reinterpret_cast<const unsigned short *>(&st) | ((uint32_t)lo16 << 16);
+}
+// 1 / s, 0 for s = 0, or -1 where codes_any() has to divide: between these
+// bounds neither the reciprocal nor the products in codes()
+// leave fp32's normal range.
+__device__ __forceinline__ float inverse_of(float s) {
+  return s > 0x1p-100f && s < 0x1p100f ? __frcp_rn(s) : (s == 0.f ? 0.f : -1.f);
+}
+
+// Parameter words and reciprocal steps of N groups, of which the L lanes that
+// differ in the lane bits from FIRST on have a part each (packed (min, -max) in
+// v): the lanes reduce them so that each ends with its share of the groups,
+// computes those alone, and hands them round.  `own(j, param)` is called by one
+// lane for each group j.
+template <typename T, int N, int L, int FIRST, typename Own>
+__device__ __forceinline__ void finish_groups(uint32_t (&v)[N], uint32_t (&param)[N], float (&inv)[N], int lane, Own own) {
+  constexpr int kMine = N > L ? N / L : 1;
+  int cur = N;
+#pragma unroll
+  for (int off = L / 2 * FIRST; off >= FIRST; off /= 2) {
+    const bool upper = (lane & off) != 0;
+    if (cur > 1) {
+      cur /= 2;
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j)
+        if (j < cur) {
+          const uint32_t keep = upper ? v[j + cur] : v[j], send = upper ? v[j] : v[j + cur];
+          v[j] = min2<T>(keep, __shfl_xor_sync(0xffffffffu, send, off));
+        }
+    } else {
+      v[0] = min2<T>(v[0], __shfl_xor_sync(0xffffffffu, v[0], off));
+    }
+  }
+  const int li = lane / FIRST % L;
+  uint32_t p[kMine];
+  float iv[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    p[j] = param_of<T>(v[j]);
+    iv[j] = inverse_of(kv4_unpack_param<T>(p[j]).x);
+    if (N >= L || li % (L / N) == 0) own(N >= L ? li * kMine + j : li / (L / N), p[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int from = lane % FIRST + (N >= L ? j / kMine : j * (L / N)) * FIRST + lane / (FIRST * L) * (FIRST * L);
+    param[j] = __shfl_sync(0xffffffffu, p[j % kMine], from);
+    inv[j] = __shfl_sync(0xffffffffu, iv[j % kMine], from);
+  }
+}
+
+// The code word of 8 channels.  The quotient is the correctly rounded one
+// (Markstein: a product with the rounded reciprocal and one step with the
+// exact remainder), without the division; adding 1.5 * 2^23 rounds it to the
+// nearest even integer in the low bits, and sums of those times 16^i make the
+// word.
+template <typename T>
+__device__ __forceinline__ uint32_t codes(const uint4 &raw, uint32_t param, float inv) {
+  float f[8];
+  unpack8<T>(raw, f);
+  const float2 sm = kv4_unpack_param<T>(param);
+  uint32_t word = 0u - 0x4b400000u * 0x11111111u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float d = f[i] - sm.y;
+    const float q = d * inv;
+    const float r = fmaf(fmaf(-q, sm.x, d), inv, q);
+    word += __float_as_uint(r + 12582912.f) << (4 * i);
+  }
+  return word;
+}
+// The same for any step: outside the bounds above it divides, and a step that
+// is not finite gives 0 (the group reads back as NaN through s or m).
+template <typename T>
+__device__ __noinline__ uint32_t codes_any(uint4 raw, uint32_t param, float inv) {
+  if (inv >= 0.f) return codes<T>(raw, param, inv);
+  float f[8];
+  unpack8<T>(raw, f);
+  const float2 sm = kv4_unpack_param<T>(param);
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = sm.x > 0.f && sm.x < CUDART_INF_F ? __fdiv_rn(f[i] - sm.y, sm.x) : 0.f;
+    word |= (uint32_t)min(15, __float2int_rn(q)) << (4 * i);
+  }
+  return word;
+}
+
+template <typename T>
+__device__ __forceinline__ void dequantise8(uint32_t code, uint32_t param, float (&f)[8]) {
+  const float2 p = kv4_unpack_param<T>(param);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = fmaf((float)((code >> (4 * i)) & 15u), p.x, p.y);
+}
+
+// The tile that a warp takes: its place, and the row that its first token is.
+struct TileAt {
+  int b, h, len;
+  long long row0;          // row of token 0 (negative: the rows begin inside the tile)
+  unsigned char *tile;     // null where no page holds it
+};
+__device__ __forceinline__ TileAt tile_at(const Kv4Args &a, const RowArgs &r) {
+  TileAt t;
+  t.b = blockIdx.y;
+  const int warp = threadIdx.x / 32;
+  const uint32_t idx = blockIdx.x * (kRowThreads / 32) + warp;
+  t.h = (int)(idx % (uint32_t)a.Hkv);
+  t.len = clamp_len(r.lens, t.b, r.S);
+  const long long start = r.start ? (long long)r.start[t.b] : 0;
+  const long long tile = (start >> 4) + idx / (uint32_t)a.Hkv;
+  t.row0 = tile * 16 - start;
+  t.tile = nullptr;
+  if (t.row0 < t.len) {
+    const long long pos = tile * 16;
+    if (pos >= 0 && pos < (long long)a.max_pages * a.page_size) {
+      const int p = (int)pos / a.page_size, in = (int)pos - p * a.page_size;
+      const long long off = kv4_page_offset(a, t.b, p);
+      if (off >= 0) t.tile = a.data + off + t.h * a.head_stride + (long long)(in >> 4) * kv4_tile_bytes(a.D);
+    } else {
+      raise_error(a.err, kDevErrBadPage);
+    }
+  }
+  return t;
+}
+__device__ __forceinline__ bool row_here(const TileAt &t, int tok) {
+  return t.row0 + tok >= 0 && t.row0 + tok < t.len;
+}
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(kRowThreads, D == 256 ? 1 : 3) kv4_store_kernel(const __grid_constant__ Kv4Args a,
+                                                                const __grid_constant__ RowArgs r) {
+  constexpr int G = D / kKv4Group;
+  const int lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+  const TileAt at = tile_at(a, r);
+  if (at.tile == nullptr) return;
+  const bool whole = at.row0 >= 0 && at.row0 + 16 <= at.len;
+  const T *k = static_cast<const T *>(r.k) + at.b * r.ks[0] + at.h * r.ks[2];
+  const T *v = static_cast<const T *>(r.v) + at.b * r.vs[0] + at.h * r.vs[2];
+  uint4 kr[2][G][2], vr[4][G][1];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int tok = g + 8 * i;
+    const T *p = k + (at.row0 + tok) * r.ks[1] + 16 * t;
+    const bool here = whole || row_here(at, tok);
+#pragma unroll
+    for (int h = 0; h < G; ++h)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) kr[i][h][w] = here ? load_row8<T, VEC>(p + 64 * h + 8 * w) : make_uint4(0u, 0u, 0u, 0u);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
+    const T *p = v + (at.row0 + tok) * r.vs[1] + 8 * g;
+    const bool here = whole || row_here(at, tok);
+#pragma unroll
+    for (int h = 0; h < G; ++h) vr[i][h][0] = here ? load_row8<T, VEC>(p + 64 * h) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  // Groups: (i, h) of K over the lanes t, of V over the lanes g.
+  uint32_t kp[2 * G], vp[4 * G], x[2 * G], y[4 * G];
+  float ki[2 * G], vi[4 * G];
+  unsigned char *par = at.tile + 16 * D;
+#pragma unroll
+  for (int j = 0; j < 2 * G; ++j) x[j] = low_high<T, 2>(kr[j / G][j % G]);
+#pragma unroll
+  for (int j = 0; j < 4 * G; ++j) y[j] = low_high<T, 1>(vr[j / G][j % G]);
+  finish_groups<T, 2 * G, 4, 1>(x, kp, ki, lane, [&](int j, uint32_t param) {
+    const int tok = g + 8 * (j / G);
+    if (whole || row_here(at, tok)) *reinterpret_cast<uint32_t *>(par + (tok * 2 * G + j % G) * 4) = param;
+  });
+  finish_groups<T, 4 * G, 8, 4>(y, vp, vi, lane, [&](int j, uint32_t param) {
+    const int tok = 2 * t + (j / G & 1) + 8 * (j / G >> 1);
+    if (whole || row_here(at, tok)) *reinterpret_cast<uint32_t *>(par + (tok * 2 * G + G + j % G) * 4) = param;
+  });
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 4 * G; ++j) odd = odd || vi[j] < 0.f || ki[j / 2] < 0.f;
+  uint32_t kw[4 * G], vw[4 * G];
+  if (!__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+    for (int j = 0; j < 4 * G; ++j) {
+      kw[j] = codes<T>(kr[j / 2 / G][j / 2 % G][j % 2], kp[j / 2], ki[j / 2]);
+      vw[j] = codes<T>(vr[j / G][j % G][0], vp[j], vi[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4 * G; ++j) {
+      kw[j] = codes_any<T>(kr[j / 2 / G][j / 2 % G][j % 2], kp[j / 2], ki[j / 2]);
+      vw[j] = codes_any<T>(vr[j / G][j % G][0], vp[j], vi[j]);
+    }
+  }
+  unsigned char *kd = at.tile + lane * 16, *vd = kd + 8 * D;
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      *reinterpret_cast<uint4 *>(kd + 512 * i) = make_uint4(kw[4 * i], kw[4 * i + 1], kw[4 * i + 2], kw[4 * i + 3]);
+      *reinterpret_cast<uint4 *>(vd + 512 * i) = make_uint4(vw[4 * i], vw[4 * i + 1], vw[4 * i + 2], vw[4 * i + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < 4 * G; ++x) {
+      const int ki = x / (2 * G), vi = x / G;  // the token of word x
+      if (row_here(at, g + 8 * ki)) *reinterpret_cast<uint32_t *>(kd + x / 4 * 512 + x % 4 * 4) = kw[x];
+      if (row_here(at, 2 * t + (vi & 1) + 8 * (vi >> 1))) *reinterpret_cast<uint32_t *>(vd + x / 4 * 512 + x % 4 * 4) = vw[x];
+    }
+  }
+}
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) kv4_load_kernel(const __grid_constant__ Kv4Args a,
+                                                               const __grid_constant__ RowArgs r) {
+  constexpr int G = D / kKv4Group;
+  const int lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+  const TileAt at = tile_at(a, r);
+  const long long end = r.pad > 0 ? min((long long)r.S, ((long long)at.len + r.pad - 1) / r.pad * r.pad) : r.S;
+  if (at.row0 >= end) return;
+  T *k = static_cast<T *>(const_cast<void *>(r.k)) + at.b * r.ks[0] + at.h * r.ks[2];
+  T *v = static_cast<T *>(const_cast<void *>(r.v)) + at.b * r.vs[0] + at.h * r.vs[2];
+  uint32_t kw[4 * G], vw[4 * G];
+  const unsigned char *par = at.tile + 16 * D;
+  if (at.tile != nullptr) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const uint4 u = ld_stream16(at.tile + 512 * i + lane * 16), w = ld_stream16(at.tile + 8 * D + 512 * i + lane * 16);
+      kw[4 * i] = u.x;
+      kw[4 * i + 1] = u.y;
+      kw[4 * i + 2] = u.z;
+      kw[4 * i + 3] = u.w;
+      vw[4 * i] = w.x;
+      vw[4 * i + 1] = w.y;
+      vw[4 * i + 2] = w.z;
+      vw[4 * i + 3] = w.w;
+    }
+  }
+  // K: lanes t and t ^ 1 swap a word, so that each store of the two covers a
+  // whole 32-byte sector.
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int tok = g + 8 * i;
+    const bool held = at.tile != nullptr && row_here(at, tok);
+    const bool wanted = at.row0 + tok >= 0 && at.row0 + tok < end;
+    T *p = k + (at.row0 + tok) * r.ks[1] + 32 * (t >> 1) + 8 * (t & 1);
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      const uint32_t w0 = kw[(i * G + h) * 2], w1 = kw[(i * G + h) * 2 + 1];
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, t & 1 ? w0 : w1, 1);
+      const uint32_t word[2] = {t & 1 ? other : w0, t & 1 ? w1 : other};
+      const uint32_t param = held ? *reinterpret_cast<const uint32_t *>(par + (tok * 2 * G + h) * 4) : 0u;
+      if (wanted) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float f[8] = {};
+          if (held) dequantise8<T>(word[x], param, f);
+          store_row8<T, VEC>(p + 64 * h + 16 * x, f);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
+    const bool held = at.tile != nullptr && row_here(at, tok);
+    const bool wanted = at.row0 + tok >= 0 && at.row0 + tok < end;
+    T *p = v + (at.row0 + tok) * r.vs[1] + 8 * g;
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      const uint32_t param = held ? *reinterpret_cast<const uint32_t *>(par + (tok * 2 * G + G + h) * 4) : 0u;
+      if (wanted) {
+        float f[8] = {};
+        if (held) dequantise8<T>(vw[i * G + h], param, f);
+        store_row8<T, VEC>(p + 64 * h, f);
+      }
+    }
+  }
+}
+
+// ---- few rows: a thread takes channels [8c, 8c + 8) of one row and kv head
+
+struct RowAt {
+  int b, h, c, len, tok;
+  long long row;
+  unsigned char *tile;  // null where no page holds the row
+};
+template <int D>
+__device__ __forceinline__ RowAt row_at(const Kv4Args &a, const RowArgs &r) {
+  RowAt t;
+  t.b = blockIdx.y;
+  const uint32_t idx = blockIdx.x * kRowThreads + threadIdx.x;
+  t.c = (int)(idx % (D / 8));
+  t.h = (int)(idx / (D / 8) % (uint32_t)a.Hkv);
+  t.row = idx / (D / 8) / (uint32_t)a.Hkv;
+  t.len = clamp_len(r.lens, t.b, r.S);
+  t.tile = nullptr;
+  t.tok = 0;
+  if (t.row < t.len) {
+    const long long pos = (r.start ? (long long)r.start[t.b] : 0) + t.row;
+    if (pos >= 0 && pos < (long long)a.max_pages * a.page_size) {
+      const int p = (int)pos / a.page_size, in = (int)pos - p * a.page_size;
+      const long long off = kv4_page_offset(a, t.b, p);
+      t.tok = in & 15;
+      if (off >= 0) t.tile = a.data + off + t.h * a.head_stride + (long long)(in >> 4) * kv4_tile_bytes(D);
+    } else {
+      raise_error(a.err, kDevErrBadPage);
+    }
+  }
+  return t;
+}
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) kv4_store_few_kernel(const __grid_constant__ Kv4Args a,
+                                                                    const __grid_constant__ RowArgs r) {
+  constexpr int G = D / kKv4Group;
+  const RowAt at = row_at<D>(a, r);
+  uint4 kr[1] = {make_uint4(0u, 0u, 0u, 0u)}, vr[1] = {make_uint4(0u, 0u, 0u, 0u)};
+  if (at.row < at.len) {
+    kr[0] = load_row8<T, VEC>(static_cast<const T *>(r.k) + at.b * r.ks[0] + at.row * r.ks[1] + at.h * r.ks[2] + at.c * 8);
+    vr[0] = load_row8<T, VEC>(static_cast<const T *>(r.v) + at.b * r.vs[0] + at.row * r.vs[1] + at.h * r.vs[2] + at.c * 8);
+  }
+  // The 8 threads of a group are in one warp and all of them come here.
+  uint32_t kp[1], vp[1], x[1] = {low_high<T, 1>(kr)}, y[1] = {low_high<T, 1>(vr)};
+  float ki[1], vi[1];
+  const int lane = threadIdx.x % 32;
+  finish_groups<T, 1, 8, 1>(x, kp, ki, lane, [](int, uint32_t) {});
+  finish_groups<T, 1, 8, 1>(y, vp, vi, lane, [](int, uint32_t) {});
+  if (at.tile == nullptr) return;
+  *reinterpret_cast<uint32_t *>(at.tile + kv4_k_word(at.tok, at.c, G)) = codes_any<T>(kr[0], kp[0], ki[0]);
+  *reinterpret_cast<uint32_t *>(at.tile + kv4_v_word(at.tok, at.c, G)) = codes_any<T>(vr[0], vp[0], vi[0]);
+  if ((at.c & 7) == 0) {
+    *reinterpret_cast<uint32_t *>(at.tile + kv4_param(at.tok, 0, at.c >> 3, G)) = kp[0];
+    *reinterpret_cast<uint32_t *>(at.tile + kv4_param(at.tok, 1, at.c >> 3, G)) = vp[0];
+  }
+}
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) kv4_load_few_kernel(const __grid_constant__ Kv4Args a,
+                                                                   const __grid_constant__ RowArgs r) {
+  constexpr int G = D / kKv4Group;
+  const RowAt at = row_at<D>(a, r);
+  const long long end = r.pad > 0 ? min((long long)r.S, ((long long)at.len + r.pad - 1) / r.pad * r.pad) : r.S;
+  if (at.row >= end) return;
+  float kf[8] = {}, vf[8] = {};
+  if (at.tile != nullptr) {
+    const uint32_t kc = *reinterpret_cast<const uint32_t *>(at.tile + kv4_k_word(at.tok, at.c, G));
+    const uint32_t vc = *reinterpret_cast<const uint32_t *>(at.tile + kv4_v_word(at.tok, at.c, G));
+    const uint32_t kp = *reinterpret_cast<const uint32_t *>(at.tile + kv4_param(at.tok, 0, at.c >> 3, G));
+    const uint32_t vp = *reinterpret_cast<const uint32_t *>(at.tile + kv4_param(at.tok, 1, at.c >> 3, G));
+    dequantise8<T>(kc, kp, kf);
+    dequantise8<T>(vc, vp, vf);
+  }
+  store_row8<T, VEC>(static_cast<T *>(const_cast<void *>(r.k)) + at.b * r.ks[0] + at.row * r.ks[1] + at.h * r.ks[2] + at.c * 8, kf);
+  store_row8<T, VEC>(static_cast<T *>(const_cast<void *>(r.v)) + at.b * r.vs[0] + at.row * r.vs[1] + at.h * r.vs[2] + at.c * 8, vf);
 }
 
 bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -203,9 +491,43 @@ RowArgs row_args(const llmx_kv4_rows &r, int pad, bool *vec) {
   return a;
 }
 
-dim3 row_grid(const Kv4Args &k, const RowArgs &r) {
-  const long long n = (long long)r.S * k.Hkv * (k.D / 8);
-  return dim3((unsigned)((n + kRowThreads - 1) / kRowThreads), (unsigned)r.B);
+template <typename T, int D, bool VEC>
+cudaError_t launch_rows_v(bool store, const Kv4Args &k, const RowArgs &r, cudaStream_t s) {
+  // A warp for each tile that a sequence's rows can touch, heads fastest.
+  const long long tiles = ((long long)(r.S + 14) / 16 + 1) * k.Hkv;
+  if (r.S >= kKv4TileTokens && tiles * r.B >= kManyTiles) {
+    const dim3 grid((unsigned)((tiles + kRowThreads / 32 - 1) / (kRowThreads / 32)), (unsigned)r.B);
+    if (store) kv4_store_kernel<T, D, VEC><<<grid, kRowThreads, 0, s>>>(k, r);
+    else kv4_load_kernel<T, D, VEC><<<grid, kRowThreads, 0, s>>>(k, r);
+  } else {
+    const long long n = (long long)r.S * k.Hkv * (D / 8);
+    const dim3 grid((unsigned)((n + kRowThreads - 1) / kRowThreads), (unsigned)r.B);
+    if (store) kv4_store_few_kernel<T, D, VEC><<<grid, kRowThreads, 0, s>>>(k, r);
+    else kv4_load_few_kernel<T, D, VEC><<<grid, kRowThreads, 0, s>>>(k, r);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch_rows_d(bool store, const Kv4Args &k, const RowArgs &r, bool vec, cudaStream_t s) {
+  return vec ? launch_rows_v<T, D, true>(store, k, r, s) : launch_rows_v<T, D, false>(store, k, r, s);
+}
+
+template <typename T>
+cudaError_t launch_rows_t(bool store, const Kv4Args &k, const RowArgs &r, bool vec, cudaStream_t s) {
+  switch (k.D) {
+    case 64: return launch_rows_d<T, 64>(store, k, r, vec, s);
+    case 128: return launch_rows_d<T, 128>(store, k, r, vec, s);
+    case 256: return launch_rows_d<T, 256>(store, k, r, vec, s);
+  }
+  return cudaErrorNotSupported;
+}
+
+cudaError_t launch_rows(bool store, const Kv4Args &k, const llmx_kv4_rows &rows, int dtype, int pad, cudaStream_t s) {
+  bool vec = false;
+  const RowArgs r = row_args(rows, pad, &vec);
+  return dtype == LLMX_FP16 ? launch_rows_t<__half>(store, k, r, vec, s)
+                            : launch_rows_t<__nv_bfloat16>(store, k, r, vec, s);
 }
 
 }  // namespace
@@ -240,6 +562,7 @@ llmx_status validate_kv4(const llmx_kv4_cache *c, int batch, Kv4Args *k) {
   k->page_size = c->page_size;
   k->Hkv = c->n_kv_heads;
   k->D = c->head_dim;
+  k->vec = 0;
   k->err = nullptr;
   return LLMX_OK;
 }
@@ -252,17 +575,7 @@ llmx_status prepare_kv4(const llmx_kv4_cache *c, int batch, Kv4Args *k) {
 }
 
 cudaError_t launch_kv4_load(const Kv4Args &k, const llmx_kv4_rows &rows, int dtype, int pad, cudaStream_t s) {
-  bool vec = false;
-  const RowArgs r = row_args(rows, pad, &vec);
-  const dim3 grid = row_grid(k, r);
-  if (dtype == LLMX_FP16) {
-    if (vec) kv4_load_kernel<__half, true><<<grid, kRowThreads, 0, s>>>(k, r);
-    else kv4_load_kernel<__half, false><<<grid, kRowThreads, 0, s>>>(k, r);
-  } else {
-    if (vec) kv4_load_kernel<__nv_bfloat16, true><<<grid, kRowThreads, 0, s>>>(k, r);
-    else kv4_load_kernel<__nv_bfloat16, false><<<grid, kRowThreads, 0, s>>>(k, r);
-  }
-  return cudaGetLastError();
+  return launch_rows(false, k, rows, dtype, pad, s);
 }
 
 }  // namespace llmx_b200
@@ -284,18 +597,7 @@ extern "C" llmx_status llmx_kv4_store(const llmx_kv4_cache *c, const llmx_kv4_ro
   Kv4Args k;
   st = prepare_kv4(c, rows->batch, &k);
   if (st != LLMX_OK || rows->batch == 0 || rows->max_rows == 0) return st;
-  bool vec = false;
-  const RowArgs r = row_args(*rows, 0, &vec);
-  const dim3 grid = row_grid(k, r);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (c->dtype == LLMX_FP16) {
-    if (vec) kv4_store_kernel<__half, true><<<grid, kRowThreads, 0, s>>>(k, r);
-    else kv4_store_kernel<__half, false><<<grid, kRowThreads, 0, s>>>(k, r);
-  } else {
-    if (vec) kv4_store_kernel<__nv_bfloat16, true><<<grid, kRowThreads, 0, s>>>(k, r);
-    else kv4_store_kernel<__nv_bfloat16, false><<<grid, kRowThreads, 0, s>>>(k, r);
-  }
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_rows(true, k, *rows, c->dtype, 0, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? LLMX_OK : record_error(LLMX_ERR_CUDA, cudaGetErrorString(e));
 }
 

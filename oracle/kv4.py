@@ -115,6 +115,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_len: int, kv_
         # fp32 sums of at most 64 terms of size <= mag a group (2^-17 mag), and
         # a handful of fp32 roundings of the score itself.
         off = mag * 2.0 ** -17 + s.abs() * 2.0 ** -21
+        # q as an integer of at most 32512: half a step (and fp32's rounding of the product) a channel.
+        step = q[:q_len, h].double().abs().amax(-1, keepdim=True) / 32512
+        off = off + 0.51 * step * (kn[:, g].double() * spread(ks)[:, g]).sum(-1) * abs(sm_scale)
         if cap > 0:
             s = cap * torch.tanh(s / cap)
             off = off + cap * 2.0 ** -21  # tanhf: 2 ulp of at most 1

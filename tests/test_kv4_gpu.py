@@ -279,6 +279,34 @@ def test_long_sequences_split_and_unsplit(dtype, d, H, hkv, n, page):
     check(one, None, q, k, v, [1, 1], lens, dtype, sm_scale=d ** -0.5, what="one split")
 
 
+@pytest.mark.parametrize("d,H,hkv,sq", [(128, 8, 2, 5), (64, 4, 4, 2), (256, 4, 2, 3), (128, 8, 8, 1), (64, 32, 2, 3)])
+def test_rows_and_sequences_that_are_empty(d, H, hkv, sq):
+    """Query rows past their length next to long caches, sequences with no row, with no key, with neither."""
+    dtype = torch.bfloat16
+    gen = torch.Generator().manual_seed(sq)
+    lens, q_lens = [900, 0, 333, 2000, 70, 0, 1], [1, sq, 0, sq, max(sq - 1, 1), 0, sq]
+    cache, table, k, v = filled(gen, lens, hkv, d, dtype, 32)
+    q = torch.randn(len(lens), sq, H, d, generator=gen).to(dtype)
+    for causal in (True, False):
+        out, lse = torch.full_like(q, 7.0, device=DEV), torch.full((len(lens), H, sq), 7.0, device=DEV)
+        llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, kv_lens=torch.tensor(lens, device=DEV), block_table=table,
+                                q_lens=torch.tensor(q_lens, device=DEV), lse=lse, causal=causal)
+        check(out, lse, q, k, v, q_lens, lens, dtype, sm_scale=d ** -0.5, causal=causal, what=f"causal {causal}")
+
+
+def test_batch_of_many_sequences():
+    """More sequences than one launch takes, most of them short."""
+    dtype, d, H, hkv = torch.float16, 64, 2, 1
+    gen = torch.Generator().manual_seed(77)
+    lens = torch.randint(0, 40, (1201,), generator=gen).tolist()
+    lens[600], lens[1200] = 700, 300
+    cache, table, k, v = filled(gen, lens, hkv, d, dtype, 16)
+    q = torch.randn(len(lens), 1, H, d, generator=gen).to(dtype)
+    out, lse = torch.full_like(q, 7.0, device=DEV), torch.full((len(lens), H, 1), 7.0, device=DEV)
+    llmx_b200.kv4_attention(out, q.to(DEV), cache, 0.125, kv_lens=torch.tensor(lens, device=DEV), block_table=table, lse=lse)
+    check(out, lse, q, k, v, [1] * len(lens), lens, dtype, sm_scale=0.125)
+
+
 def test_scores_that_move_the_maximum():
     """Rising and falling scores, a weight that underflows everything before it, steps of very different sizes."""
     dtype, d, n = torch.bfloat16, 128, 700
