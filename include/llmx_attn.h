@@ -259,7 +259,7 @@ LLMX_API llmx_status llmx_convert(const void *src, int32_t src_dtype, void *dst,
  *   n = min(15, rint(fl32(fl32(x - m) / s)))  (0 where s = 0),
  *   value = n s + m.
  * A group with a NaN or an infinity in it (or, for bf16, a range max x - m
- * past fp32) reads back as NaN.  4.5 bits a value: 18 * head_dim bytes per
+ * past fp32) has s = NaN and reads back as NaN.  4.5 bits a value: 18 * head_dim bytes per
  * 16 tokens of K and V of one kv head.
  *
  * The cache is made of pages of page_size tokens (a multiple of 16).  Page p,
@@ -331,14 +331,17 @@ LLMX_API llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_rows 
  * and results (p->k, p->v and their strides are ignored; p->dtype, n_kv_heads
  * and head_dim must match the cache; p->max_kv_len <= max_pages * page_size
  * bounds kv_lens; kv_offset / kv_total must be 0).  p->algo:
- *   DECODE  reads the 4-bit tiles directly, in one pass per 8 to 32 (head,
- *           query row) pairs of a kv head; any max_q_len, any q / o alignment.
- *           The values n s + m are used unrounded.
+ *   DECODE  reads the 4-bit tiles directly, in one pass per 8 (head, query
+ *           row) pairs of a kv head; any max_q_len, any q / o alignment.  The
+ *           values n s + m are used unrounded; q is used in 16 bits of its
+ *           row's largest element (steps of 1/32512), p s in fp16.
  *   TCGEN05 expands the sequences into the workspace (values rounded to T)
  *           and runs the tensor-core prefill on them; needs its workspace.
- *   AUTO    DECODE, or for long query blocks TCGEN05 where it can run.
+ *   AUTO    DECODE, or for long query blocks TCGEN05 where it can run, is
+ *           expected to be faster and takes at most 4 GiB.
  * A call on the DECODE path given too little workspace runs without
- * splitting the keys. */
+ * splitting a sequence's keys.  Calls that share a workspace must not overlap
+ * on the GPU.  An infinity or NaN in q makes its row NaN. */
 LLMX_API llmx_status llmx_kv4_attn_workspace_size(const llmx_attn_params *p, const llmx_kv4_cache *c, size_t *bytes);
 LLMX_API llmx_status llmx_kv4_attn_fwd(const llmx_attn_params *p, const llmx_kv4_cache *c, void *stream);
 

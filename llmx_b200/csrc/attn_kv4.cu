@@ -10,7 +10,9 @@
 //   * K: the nibbles of a word are 4 + 4 bytes after two ANDs and a shift, and
 //     go as they are into the integer tensor product (m16n8k32, u8 x s8, exact
 //     in 32 bits).  q is a 16-bit integer of its row's largest value (steps of
-//     1/32512), its high and low byte two products.
+//     1/32512), its high and low byte two products.  What its rounding leaves of
+//     a group's sum, times 8, is where the product starts: the rounding then
+//     meets n - 8 and not n.
 //   * V: a nibble OR-ed into 1024 (0x6400) and 1032 (or 1152 = 1024 + 128 for
 //     bits 4-7) subtracted is n - 8 (16 (n - 8)), two operations per two
 //     values.  Centred, because the tensor core's fp32 accumulation would
@@ -33,13 +35,25 @@
 //
 // Work.  A unit is one (sequence, kv head, block of pairs); its tokens are cut
 // into steps of one or two tiles, and the steps of all units, end to end, are
-// dealt to the resident warps in equal shares.  A warp works alone: it copies
-// its tiles into its own ring in shared memory (one bulk copy a tile, issued
-// ahead across unit boundaries), and writes the result of a unit that it has
-// whole.  Of a unit that several warps share each writes a partial result (at
-// most two a warp, so the workspace does not grow with the sequences), and a
-// second kernel merges them as in attn_decode.cu.
+// dealt to the resident workers in equal shares: sequences of any lengths
+// finish together.  With more units than resident CTAs a worker is a warp,
+// which copies its tiles into its own ring in shared memory (one bulk copy a
+// tile, issued ahead across unit boundaries); with fewer it is a CTA, whose
+// warps take every fourth step and are merged in shared memory (COOP).  A
+// worker writes the result of a unit that it has whole.  Of a unit that several
+// share each writes a partial result (at most two a worker, so the workspace
+// does not grow with the sequences), and a second kernel merges them.
+//
+// Measured on one B200 (bytes of the visible cache, q and o): 64 sequences of
+// 256-4096 tokens, 32 heads of 128, ALiBi: 124-130 us, 5.1 TB/s (0.77 of the
+// copy rate); 32 sequences of 1001-8191 tokens, 32 heads on 8: 47 us, 3.6 TB/s;
+// 131071 tokens, 32 heads on 8: 43 us, 3.5 TB/s.  What bounds it is not HBM yet:
+// at 16 warps an SM (128 registers) the issue slots are 0.6 filled, the unpacking
+// keeps the integer pipe 0.6 busy, and more warps with fewer registers (20 of
+// 96) ran 15-25% slower, fewer with more (12 of 168) 4-8%.
 #include <algorithm>
+#include <atomic>
+#include <cmath>
 #include <string>
 
 #include "kv4.cuh"
@@ -55,11 +69,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum of a row moves only when a score passes it by this
 // much (log2): p reaches 2^6 at most, and p s at most 2^14 in fp16.
 constexpr float kLazyMax = 6.f;
+constexpr float kQTop = 32512.f;  // 127 * 256: q's largest value as an integer
 // The largest weight times the largest step stays in [2^7, 2^8) (times 2^6
 // under a lazy maximum): fp16 then keeps 11 bits of weights down to 2^-21 of
 // the largest.  Steps count from 2^-40 on (smaller ones lose bits from 2^-61
 // on), which keeps the sums of scaled weights inside fp32.
-constexpr float kQTop = 32512.f;  // 127 * 256: q's largest value as an integer
 constexpr int kStepExp = 7;
 constexpr int kMinStepExp = -40;
 constexpr int kMaxStepExp = 125;
@@ -81,12 +95,13 @@ __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1,
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same from the columns' starting values x (even) and y (odd).
 __device__ __forceinline__ void imma16832_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                uint32_t b0, uint32_t b1) {
+                                                uint32_t b0, uint32_t b1, int x, int y) {
   asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
       : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(x), "r"(y));
 }
 
 // 8x8 transpose of 16-bit elements across the warp: lane (g, t) gives row g,
@@ -166,7 +181,8 @@ struct Work {
   int b0, nb;      // sequences
   int R;           // pairs of a block
   int workers;     // warps (CTAs, where a CTA's warps work together) that take a share, at most
-  int min_steps;   // a share is at least this long
+  int min_steps;   // a share is at least this long, unless units are shorter
+  int units;       // at most
   int split;       // 0: shares end where units end
 };
 constexpr int kMaxSlice = 512;
@@ -180,8 +196,8 @@ __device__ __forceinline__ int share_of(uint32_t total, uint32_t step, int n) {
   return (int)((((unsigned long long)step + 1) * n - 1) / total);
 }
 __device__ __forceinline__ int share_count(const Work &wk, uint32_t total) {
-  const uint32_t n = total / wk.min_steps;
-  return n < 1 ? 1 : (n < (uint32_t)wk.workers ? (int)n : wk.workers);
+  const uint32_t n = max(total / wk.min_steps, min(total, (uint32_t)wk.units));
+  return (int)min(max(n, 1u), (uint32_t)wk.workers);
 }
 
 // Steps of all units before each sequence of the slice, prefix[nb] their sum,
@@ -329,7 +345,7 @@ struct Shape {
   static constexpr int kMinCtas = G <= 2 ? 4 : 3;
   static constexpr int kRing = kStages * W * kTile;
   static constexpr int kQFrag = G * 2 * 32 * 16;
-  static constexpr int kRows = kCols * (4 + G) * 4;  // factor, slope, lo, hi and group sums of each column
+  static constexpr int kRows = kCols * (4 + 2 * G) * 4;  // factor, slope, lo, hi, sums and starts of the groups
   // Each warp's ring; q and its columns, of each warp or of all; as many
   // zeros as q for the other tiles' columns; lengths and prefix sums.
   static constexpr int kZeros = SLOTS > 1 ? kQFrag : 0;
@@ -345,6 +361,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
                     float *part_o, float *part_lse) {
   using Sh = Shape<D, NQ, SLOTS, COOP>;
   constexpr int G = Sh::G, R = Sh::R, kStages = Sh::kStages, W = Sh::W, kCols = Sh::kCols;
+  // The other column of a lone pair takes what fp16 leaves of its weights: free,
+  // and of use where the output has fp16's own 11 bits.
+  constexpr bool kLow = NQ == 1 && std::is_same<T, __half>::value;
   constexpr int kTileCols = Sh::kTileCols, kColStep = NQ == 1 ? 2 : 1;  // pair r of a tile has column r * kColStep
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t sm_full[kWarps][kStages];
@@ -356,11 +375,13 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
   unsigned char *q_at0 = smem + kWarps * Sh::kRing + (COOP ? 0 : warp) * (Sh::kQFrag + Sh::kRows);
   uint4 *q_own = reinterpret_cast<uint4 *>(q_at0);
   float *row_f = reinterpret_cast<float *>(q_at0 + Sh::kQFrag);
-  float *row_slope = row_f + kCols, *row_qs = row_f + 2 * kCols;  // row_qs [G][kCols]
-  int *row_lo = reinterpret_cast<int *>(row_qs + G * kCols), *row_hi = row_lo + kCols;
+  float *row_slope = row_f + kCols;
+  int *row_lo = reinterpret_cast<int *>(row_f + 2 * kCols), *row_hi = row_lo + kCols;
+  float *row_qs = row_f + 4 * kCols;                           // [G][kCols]
+  int *row_begin = reinterpret_cast<int *>(row_qs + G * kCols);  // [G][kCols]
   unsigned char *zeros = smem + Sh::kSmem - Sh::kZeros;
   int2 *lens = reinterpret_cast<int2 *>(smem + Sh::kSmem);               // [nb]
-  uint32_t *prefix = reinterpret_cast<uint32_t *>(lens + wk.nb);  // [nb + 1]
+  uint32_t *prefix = reinterpret_cast<uint32_t *>(lens + wk.nb);         // [nb + 1]
 
   // The merge kernel may be set up while this one runs.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -502,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
     // q as 16-bit integers of its row's largest value, high and low byte, in
     // the order of the operand fragments; with the factor that undoes the
     // scale and the sums of the groups.  A lane takes 16 channels of a pair.
-    // An infinity makes the factor one, and so the scores NaN (0 inf).
+    // An infinity makes the factor NaN, a NaN the sums.
     __syncwarp();
     constexpr int kLanes = D / 16, kPass = 32 / kLanes;  // lanes of a pair, pairs side by side
 #pragma unroll
@@ -542,6 +563,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
       const float up = top > 0.f ? fminf(kQTop / top, 0x1p126f) : 0.f;
       const float scale = a.softcap > 0.f ? a.sm_scale / a.softcap : a.sm_scale * kLog2e;
       const int h = sub >> 2, tt = sub & 3;
+      float left = 0.f;  // of the group's sum, in steps
       if (here) {
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
@@ -551,6 +573,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
             // A word's even channels are the low nibbles of its bytes (the
             // first half of the 32 the product sums over), the odd ones the high.
             const int v = __float2int_rn(f[w][x] * up);
+            left += fmaf(f[w][x], up, -(float)v);
             hi8[x & 1] |= (uint32_t)((v + 128) >> 8 & 255) << (8 * (x >> 1));
             lo8[x & 1] |= (uint32_t)(v & 255) << (8 * (x >> 1));
           }
@@ -562,14 +585,23 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
             if constexpr (NQ == 1) dst[4] = make_uint4(lo8[0], lo8[1], 0u, 0u);
           }
         }
+      }
+      left += __shfl_xor_sync(0xffffffffu, left, 1);
+      left += __shfl_xor_sync(0xffffffffu, left, 2);
+      if (here) {
 #pragma unroll
         for (int sl = 0; sl < SLOTS; ++sl) {
           const int col = sl * kTileCols + pr * kColStep;
-          if (tt == 0) row_qs[h * kCols + col] = sum * scale;
+          if (tt == 0) {
+            row_qs[h * kCols + col] = sum * scale;
+            // The low byte's columns start with it; with NQ = 1 those are the odd ones.
+            row_begin[h * kCols + col + kColStep - 1] = __float2int_rn(8.f * left);
+            if constexpr (NQ == 1) row_begin[h * kCols + col] = 0;
+          }
           if (sub == 0) {
             int lo, hi;
             row_range(a, live ? i : ql - 1, ql, kl, lo, hi);  // a column without a row goes with the last one
-            row_f[col] = up > 0.f ? scale / up : 0.f;
+            row_f[col] = up > 0.f ? scale / up : (top > 0.f ? CUDART_NAN_F : 0.f);
             row_slope[col] = live && a.alibi != nullptr ? a.alibi[h0] * kLog2e : 0.f;
             row_lo[col] = lo;
             row_hi[col] = hi;
@@ -591,20 +623,18 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
     int step_exp = kMinStepExp;
     bool fresh = true;                   // some row has no reference yet (the same in all lanes)
     float limit = 0.f, next_step = 0.f;  // a score above `limit` or a step from `next_step` on moves the references
-    {
 #pragma unroll
-      for (int h = 0; h < G; ++h)
+    for (int h = 0; h < G; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[h][i][x] = 0.f;
+        for (int x = 0; x < 4; ++x) o[h][i][x] = 0.f;
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        l[q] = start[q] = after[q] = 0.f;
-        ref[q] = -CUDART_INF_F;
+    for (int q = 0; q < NQ; ++q) {
+      l[q] = start[q] = after[q] = 0.f;
+      ref[q] = -CUDART_INF_F;
 #pragma unroll
-        for (int h = 0; h < G; ++h) aff[q][h] = 0.f;
-      }
+      for (int h = 0; h < G; ++h) aff[q][h] = 0.f;
     }
 
     // SLOTS tiles at shared address `at`, tokens tok0 ..  PART: some row does
@@ -629,15 +659,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
             for (int w = 0; w < 2; ++w) {
               const uint32_t a0 = kw[0][w] & 0x0f0f0f0fu, a2 = (kw[0][w] >> 4) & 0x0f0f0f0fu;
               const uint32_t a1 = kw[1][w] & 0x0f0f0f0fu, a3 = (kw[1][w] >> 4) & 0x0f0f0f0fu;
-              {
-                const uint4 qw = lds16(q_at[sl] + (h * 2 + w) * 512);
-                if (w == 0 && sl == 0) {
-                  imma16832_first(acc[h][0], a0, a1, a2, a3, qw.x, qw.y);
-                  if constexpr (B == 2) imma16832_first(acc[h][B - 1], a0, a1, a2, a3, qw.z, qw.w);
-                } else {
-                  imma16832(acc[h][0], a0, a1, a2, a3, qw.x, qw.y);
-                  if constexpr (B == 2) imma16832(acc[h][B - 1], a0, a1, a2, a3, qw.z, qw.w);
-                }
+              const uint4 qw = lds16(q_at[sl] + (h * 2 + w) * 512);
+              if (w == 0 && sl == 0) {
+                const int2 begin = *reinterpret_cast<const int2 *>(&row_begin[h * kCols + 2 * t]);
+                if constexpr (B == 2) imma16832_first(acc[h][0], a0, a1, a2, a3, qw.x, qw.y, 0, 0);
+                imma16832_first(acc[h][B - 1], a0, a1, a2, a3, B == 2 ? qw.z : qw.x, B == 2 ? qw.w : qw.y, begin.x, begin.y);
+              } else {
+                imma16832(acc[h][0], a0, a1, a2, a3, qw.x, qw.y);
+                if constexpr (B == 2) imma16832(acc[h][B - 1], a0, a1, a2, a3, qw.z, qw.w);
               }
             }
           }
@@ -650,52 +679,52 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
           for (int h = 0; h < G; ++h) kp[r][h] = kv4_unpack_param<T>(par[h]);
         }
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            const float fac = row_f[2 * t + q];
-            float qs[G];
+        for (int q = 0; q < NQ; ++q) {
+          const float fac = row_f[2 * t + q];
+          float qs[G];
 #pragma unroll
-            for (int h = 0; h < G; ++h) qs[h] = row_qs[h * kCols + 2 * t + q];
+          for (int h = 0; h < G; ++h) qs[h] = row_qs[h * kCols + 2 * t + q];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              float dot = 0.f, off = start[q];
+          for (int r = 0; r < 2; ++r) {
+            float dot = 0.f, off = start[q];
 #pragma unroll
-              for (int h = 0; h < G; ++h) {
-                const int sum = NQ == 1 ? acc[h][0][2 * r] * 256 + acc[h][0][2 * r + 1]
-                                        : acc[h][0][2 * r + q] * 256 + acc[h][B - 1][2 * r + q];
-                dot = h == 0 ? kp[r][h].x * (float)sum : fmaf(kp[r][h].x, (float)sum, dot);
-                off = fmaf(kp[r][h].y, qs[h], off);
-              }
-              s[r][q] = fmaf(dot, fac, off);
+            for (int h = 0; h < G; ++h) {
+              const int sum = NQ == 1 ? acc[h][0][2 * r] * 256 + acc[h][0][2 * r + 1]
+                                      : acc[h][0][2 * r + q] * 256 + acc[h][B - 1][2 * r + q];
+              dot = h == 0 ? kp[r][h].x * (float)sum : fmaf(kp[r][h].x, (float)sum, dot);
+              off = fmaf(kp[r][h].y, qs[h], off);
             }
+            s[r][q] = fmaf(dot, fac, off);
           }
+        }
       }
       if (a.softcap > 0.f) {
         const float cap2 = a.softcap * kLog2e;
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) s[r][q] = fmaf(tanhf(s[r][q]), cap2, after[q]);
+          for (int q = 0; q < NQ; ++q) s[r][q] = fmaf(tanhf(s[r][q]), cap2, after[q]);
       }
       if (a.alibi != nullptr) {
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            const float slope = row_slope[2 * t + q];
+        for (int q = 0; q < NQ; ++q) {
+          const float slope = row_slope[2 * t + q];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) s[r][q] = fmaf(slope, (float)(tok + 8 * r), s[r][q]);
-          }
+          for (int r = 0; r < 2; ++r) s[r][q] = fmaf(slope, (float)(tok + 8 * r), s[r][q]);
+        }
       }
       uint32_t vis = 0;  // bit r NQ + q; only with PART
       if constexpr (PART) {
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            const int lo = row_lo[2 * t + q], hi = row_hi[2 * t + q];
+        for (int q = 0; q < NQ; ++q) {
+          const int lo = row_lo[2 * t + q], hi = row_hi[2 * t + q];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int j = tok + 8 * r;
-              if (j >= lo && j < hi && !(lost >> my_slot & 1u)) vis |= 1u << r * NQ + q;
-              else s[r][q] = -CUDART_INF_F;
-            }
+          for (int r = 0; r < 2; ++r) {
+            const int j = tok + 8 * r;
+            if (j >= lo && j < hi && !(lost >> my_slot & 1u)) vis |= 1u << r * NQ + q;
+            else s[r][q] = -CUDART_INF_F;
           }
+        }
       }
       // ---- V's steps and centres; a token that no row sees may hold anything
       float sv[2][G], cv[2][G];
@@ -707,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
         if constexpr (PART) {
           dead = true;
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) dead = dead && !(vis >> r * NQ + q & 1u);
+          for (int q = 0; q < NQ; ++q) dead = dead && !(vis >> r * NQ + q & 1u);
         }
 #pragma unroll
         for (int h = 0; h < G; ++h) {
@@ -721,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
       // passes its row's maximum by kLazyMax or a larger step turns up
       float most = -CUDART_INF_F, smax = 0.f;
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) most = max3(most, s[0][q], s[1][q]);
+      for (int q = 0; q < NQ; ++q) most = max3(most, s[0][q], s[1][q]);
 #pragma unroll
       for (int h = 0; h < G; ++h) smax = max3(smax, sv[0][h], sv[1][h]);
       if (__any_sync(0xffffffffu, fresh || most > limit || smax >= next_step)) {
@@ -740,34 +769,38 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
         next_step = pow2i(new_exp + 1);
         bool missing = false;
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            const bool none = ref[q] == -CUDART_INF_F;
-            const float shift = none ? 0.f : ref[q];
-            float v = fmaxf(s[0][q], s[1][q]) + shift;
+        for (int q = 0; q < NQ; ++q) {
+          const bool none = ref[q] == -CUDART_INF_F;
+          const float shift = none ? 0.f : ref[q];
+          float v = fmaxf(s[0][q], s[1][q]) + shift;
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-            const float m = none ? v : fmaxf(ref[q] + old_room, v);
-            const float now = m == -CUDART_INF_F ? m : m - new_room;
-            const float al = none ? 1.f : exp2_fast(ref[q] - now);
-            const float back = now == -CUDART_INF_F ? 0.f : shift - now;
-            ref[q] = now;
-            missing |= now == -CUDART_INF_F;
-            const float minus = now == -CUDART_INF_F ? 0.f : -now;
-            start[q] = a.softcap > 0.f ? 0.f : minus;
-            after[q] = minus;
-            s[0][q] += back;
-            s[1][q] += back;
-            l[q] *= al;
+          for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+          const float m = none ? v : fmaxf(ref[q] + old_room, v);
+          const float now = m == -CUDART_INF_F ? m : m - new_room;
+          const float al = none ? 1.f : exp2_fast(ref[q] - now);
+          const float back = now == -CUDART_INF_F ? 0.f : shift - now;
+          ref[q] = now;
+          missing |= now == -CUDART_INF_F;
+          const float minus = now == -CUDART_INF_F ? 0.f : -now;
+          start[q] = a.softcap > 0.f ? 0.f : minus;
+          after[q] = minus;
+          s[0][q] += back;
+          s[1][q] += back;
+          l[q] *= al;
 #pragma unroll
-            for (int h = 0; h < G; ++h) {
-              aff[q][h] *= al;
+          for (int h = 0; h < G; ++h) {
+            aff[q][h] *= al;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                o[h][i][q] *= al;
-                o[h][i][2 + q] *= al;
+            for (int i = 0; i < 4; ++i) {
+              o[h][i][q] *= al;
+              o[h][i][2 + q] *= al;
+              if constexpr (kLow) {
+                o[h][i][1] *= al;
+                o[h][i][3] *= al;
               }
             }
           }
+        }
         fresh = __any_sync(0xffffffffu, missing);
       }
       // ---- weights
@@ -797,6 +830,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
                 aff[q][h] = fmaf(p[r][q], cv[r][h], aff[q][h]);
               }
             }
+            if constexpr (kLow) w[1] = w[0] - __half2float(__float2half_rn(w[0]));
             pf[h][r] = transpose8x8(pack_half2(w[0], w[1]));
           }
       }
@@ -813,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[k] = word_of(vw[(k * G + h) / 4], (k * G + h) % 4);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) pb[r] = SLOTS == 1 || g / kTileCols == sl ? pf[h][r] : 0u;
+          for (int r = 0; r < 2; ++r) pb[r] = SLOTS == 1 || g / kTileCols == sl ? pf[h][r] : 0u;
 #pragma unroll
           for (int part16 = 0; part16 < 2; ++part16) {
             uint32_t z0 = __byte_perm(w[0], w[1], part16 ? 0x7632 : 0x5410);
@@ -868,87 +902,92 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
     // ---- the unit's result: sums over the tokens (lanes with the same t hold
     // the same rows), then over the tiles' columns
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
+    for (int q = 0; q < NQ; ++q) {
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          l[q] += __shfl_xor_sync(0xffffffffu, l[q], off);
+      for (int off = 4; off < 32; off <<= 1) {
+        l[q] += __shfl_xor_sync(0xffffffffu, l[q], off);
 #pragma unroll
-          for (int h = 0; h < G; ++h) aff[q][h] += __shfl_xor_sync(0xffffffffu, aff[q][h], off);
+        for (int h = 0; h < G; ++h) aff[q][h] += __shfl_xor_sync(0xffffffffu, aff[q][h], off);
+      }
+      float out[G][8];
+#pragma unroll
+      for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float even = o[h][i][q], odd = o[h][i][2 + q];
+          if constexpr (kLow) {
+            even += o[h][i][1];
+            odd += o[h][i][3];
+          }
+          out[h][2 * i] = even + aff[q][h];
+          out[h][2 * i + 1] = fmaf(odd, 0.0625f, aff[q][h]);
         }
-        float out[G][8];
+      float m = ref[q], sum = l[q];
+      if constexpr (SLOTS == 2) {
+        const float other = __shfl_xor_sync(0xffffffffu, m, 2);
+        const float both = fmaxf(m, other);
+        // Columns that saw no finite score add nothing, unless their sum is a NaN.
+        const float wt = m == -CUDART_INF_F ? (sum == sum ? 0.f : 1.f) : exp2_fast(m - both);
+        m = both;
+        sum *= wt;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
         for (int h = 0; h < G; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            out[h][2 * i] = o[h][i][q] + aff[q][h];
-            out[h][2 * i + 1] = fmaf(o[h][i][2 + q], 0.0625f, aff[q][h]);
+          for (int x = 0; x < 8; ++x) {
+            out[h][x] = wt == 0.f ? 0.f : out[h][x] * wt;
+            out[h][x] += __shfl_xor_sync(0xffffffffu, out[h][x], 2);
           }
-        float m = ref[q], sum = l[q];
-        if constexpr (SLOTS == 2) {
-          const float other = __shfl_xor_sync(0xffffffffu, m, 2);
-          const float both = fmaxf(m, other);
-          // Columns that saw no finite score add nothing, unless their sum is a NaN.
-          const float wt = m == -CUDART_INF_F ? (sum == sum ? 0.f : 1.f) : exp2_fast(m - both);
-          m = both;
-          sum *= wt;
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      }
+      const int pr = (2 * t + q) % kTileCols / kColStep, r = r0 + pr;
+      if constexpr (COOP) {
+        if (my_slot == 0 && r < rows) {
+          float *dst = reinterpret_cast<float *>(own) + pr * Sh::kMergeRow + 8 * g;
 #pragma unroll
-          for (int h = 0; h < G; ++h)
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              out[h][x] = wt == 0.f ? 0.f : out[h][x] * wt;
-              out[h][x] += __shfl_xor_sync(0xffffffffu, out[h][x], 2);
-            }
+          for (int h = 0; h < G; ++h) {
+            *reinterpret_cast<float4 *>(dst + 64 * h) = make_float4(out[h][0], out[h][1], out[h][2], out[h][3]);
+            *reinterpret_cast<float4 *>(dst + 64 * h + 4) = make_float4(out[h][4], out[h][5], out[h][6], out[h][7]);
+          }
+          if (g == 0) {
+            sm_m[warp][pr] = m;
+            sm_l[warp][pr] = sum;
+          }
         }
-        const int pr = (2 * t + q) % kTileCols / kColStep, r = r0 + pr;
-        if constexpr (COOP) {
-          if (my_slot == 0 && r < rows) {
-            float *dst = reinterpret_cast<float *>(own) + pr * Sh::kMergeRow + 8 * g;
+      } else if (my_slot == 0 && r < rows) {
+        const bool none = sum == 0.f;
+        const float inv = 1.f / sum;
+        const float lse = none ? -CUDART_INF_F : (m == -CUDART_INF_F ? sum : (m + log2f(sum)) * kLn2);
 #pragma unroll
-            for (int h = 0; h < G; ++h) {
-              *reinterpret_cast<float4 *>(dst + 64 * h) = make_float4(out[h][0], out[h][1], out[h][2], out[h][3]);
-              *reinterpret_cast<float4 *>(dst + 64 * h + 4) = make_float4(out[h][4], out[h][5], out[h][6], out[h][7]);
-            }
-            if (g == 0) {
-              sm_m[warp][pr] = m;
-              sm_l[warp][pr] = sum;
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) out[h][x] = none ? 0.f : out[h][x] * inv;
+        const int i = r / a.group, h0 = kvh * a.group + r % a.group;
+        if (n_steps == pl.steps) {
+          T *op = static_cast<T *>(a.o) + b * a.os[0] + i * a.os[1] + h0 * a.os[2] + 8 * g;
+#pragma unroll
+          for (int h = 0; h < G; ++h) {
+            if (c.vec) {
+              *reinterpret_cast<uint4 *>(op + 64 * h) = pack8<T>(out[h]);
+            } else {
+#pragma unroll
+              for (int x = 0; x < 8; ++x) op[64 * h + x] = Elem<T>::from_f(out[h][x]);
             }
           }
-        } else if (my_slot == 0 && r < rows) {
-          const bool none = sum == 0.f;
-          const float inv = 1.f / sum;
-          const float lse = none ? -CUDART_INF_F : (m == -CUDART_INF_F ? sum : (m + log2f(sum)) * kLn2);
+          if (a.lse != nullptr && g == 0) a.lse[((long long)b * a.H + h0) * a.Sq + i] = lse;
+        } else {
+          // Slot 1 for the unit that begins in this share, slot 0 for the
+          // one that began before it.
+          const long long row = ((long long)worker * 2 + (pl.at == 0 ? 1 : 0)) * R + pr;
+          float *dst = part_o + row * D + 8 * g;
 #pragma unroll
-          for (int h = 0; h < G; ++h)
-#pragma unroll
-            for (int x = 0; x < 8; ++x) out[h][x] = none ? 0.f : out[h][x] * inv;
-          const int i = r / a.group, h0 = kvh * a.group + r % a.group;
-          if (n_steps == pl.steps) {
-            T *op = static_cast<T *>(a.o) + b * a.os[0] + i * a.os[1] + h0 * a.os[2] + 8 * g;
-#pragma unroll
-            for (int h = 0; h < G; ++h) {
-              if (c.vec) {
-                *reinterpret_cast<uint4 *>(op + 64 * h) = pack8<T>(out[h]);
-              } else {
-#pragma unroll
-                for (int x = 0; x < 8; ++x) op[64 * h + x] = Elem<T>::from_f(out[h][x]);
-              }
-            }
-            if (a.lse != nullptr && g == 0) a.lse[((long long)b * a.H + h0) * a.Sq + i] = lse;
-          } else {
-            // Slot 1 for the unit that begins in this share, slot 0 for the
-            // one that began before it.
-            const long long row = ((long long)worker * 2 + (pl.at == 0 ? 1 : 0)) * R + pr;
-            float *dst = part_o + row * D + 8 * g;
-#pragma unroll
-            for (int h = 0; h < G; ++h) {
-              *reinterpret_cast<float4 *>(dst + 64 * h) = make_float4(out[h][0], out[h][1], out[h][2], out[h][3]);
-              *reinterpret_cast<float4 *>(dst + 64 * h + 4) = make_float4(out[h][4], out[h][5], out[h][6], out[h][7]);
-            }
-            if (g == 0) part_lse[row] = lse;
+          for (int h = 0; h < G; ++h) {
+            *reinterpret_cast<float4 *>(dst + 64 * h) = make_float4(out[h][0], out[h][1], out[h][2], out[h][3]);
+            *reinterpret_cast<float4 *>(dst + 64 * h + 4) = make_float4(out[h][4], out[h][5], out[h][6], out[h][7]);
           }
+          if (g == 0) part_lse[row] = lse;
         }
       }
+    }
     if constexpr (COOP) {
       // The warps' sums, four channels a thread.
       __syncthreads();
@@ -1024,30 +1063,33 @@ __global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const __grid_consta
   __shared__ float sm_m[kWarps], sm_l[kWarps], sm_o[WIDE ? kWarps : 1][WIDE ? D : 1];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const long long out_row = WIDE ? blockIdx.x : (long long)blockIdx.x * kWarps + warp;
-  if (out_row >= (long long)wk.nb * a.Sq * a.H) return;
   const int h = (int)(out_row % a.H), i = (int)(out_row / a.H % a.Sq), n = (int)(out_row / a.H / a.Sq), b = wk.b0 + n;
-  const int ql = clamp_len(a.q_lens, b, a.Sq);
-  if (i >= ql) return;  // 0 already
-  // Steps before this sequence, and of all.
-  uint32_t before = 0, all = 0;
-  for (int x = lane; x < wk.nb; x += 32) {
-    const Span sp = span_of<W>(a, wk.R, clamp_len(a.q_lens, wk.b0 + x, a.Sq), clamp_len(a.kv_lens, wk.b0 + x, a.Skv));
-    const uint32_t s = (uint32_t)sp.steps * sp.blocks * a.Hkv;
-    all += s;
-    if (x < n) before += s;
+  int w0 = 0, used = 0, R = wk.R, r = 0;
+  if (n < wk.nb) {
+    // Steps before this sequence, and of all.
+    uint32_t before = 0, all = 0;
+    for (int x = lane; x < wk.nb; x += 32) {
+      const Span sp = span_of<W>(a, R, clamp_len(a.q_lens, wk.b0 + x, a.Sq), clamp_len(a.kv_lens, wk.b0 + x, a.Skv));
+      const uint32_t s = (uint32_t)sp.steps * sp.blocks * a.Hkv;
+      all += s;
+      if (x < n) before += s;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    all = __reduce_add_sync(0xffffffffu, all);
+    const int ql = clamp_len(a.q_lens, b, a.Sq);
+    const Span sp = span_of<W>(a, R, ql, clamp_len(a.kv_lens, b, a.Skv));
+    if (i < ql && sp.steps > 0) {  // the others are 0 already
+      const int shares = share_count(wk, all);
+      r = i * a.group + h % a.group;
+      const uint32_t first = before + (uint32_t)(h / a.group * sp.blocks + r / R) * sp.steps;
+      w0 = share_of(all, first, shares);
+      used = share_of(all, first + sp.steps - 1, shares) - w0 + 1;
+    }
   }
-  before = __reduce_add_sync(0xffffffffu, before);
-  all = __reduce_add_sync(0xffffffffu, all);
-  const Span sp = span_of<W>(a, wk.R, ql, clamp_len(a.kv_lens, b, a.Skv));
-  if (sp.steps == 0) return;
-  const int shares = share_count(wk, all), R = wk.R;
-  const int r = i * a.group + h % a.group;
-  const uint32_t first = before + (uint32_t)(h / a.group * sp.blocks + r / R) * sp.steps;
-  const int w0 = share_of(all, first, shares), w1 = share_of(all, first + sp.steps - 1, shares);
-  if (w0 == w1) return;  // one worker had the unit whole
-  const int used = w1 - w0 + 1;
-
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the shares are written
+  // Every thread waits for the shares to be written, also where there is
+  // nothing to do, so that this kernel ends after them.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (used <= 1) return;  // one worker had the unit whole
   constexpr int kStride = WIDE ? kWarps : 1;
   float m = -CUDART_INF_F, sum = 0.f, o[E];
 #pragma unroll
@@ -1138,7 +1180,7 @@ Plan plan_kv4(const AttnArgs &a) {
   if (a.window >= 0) span = std::min<long long>(span, (long long)a.window + a.Sq + 15);
   const long long steps = (span + 15 + 16 * p.tiles - 1) / (16 * p.tiles);
   const long long per_seq = (long long)a.Hkv * ((p.rows + p.R - 1) / p.R);
-  // (check() has seen to it that one sequence's steps stay below 2^31.)
+  // (direct_fits() keeps one sequence's steps below 2^31.)
   p.nb = (int)std::min<long long>(std::min(a.B, kMaxSlice), std::max<long long>(1, 0x7fffffffLL / (per_seq * steps)));
   const long long units = p.nb * per_seq, most = units * steps;
   const int resident = a.num_sms * (a.D <= 128 ? 4 : 3);
@@ -1155,10 +1197,14 @@ template <typename T, int D, int NQ, int SLOTS, bool COOP>
 cudaError_t launch_variant(const AttnArgs &a, const Kv4Args &c, const Plan &p, bool split, void *ws, cudaStream_t s) {
   using Sh = Shape<D, NQ, SLOTS, COOP>;
   const int smem = Sh::kSmem + p.nb * 12 + 4;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<T, D, NQ, SLOTS, COOP>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<int> allowed[64];  // of each device: setting it costs a microsecond a launch
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (smem > 48 * 1024 && (dev < 0 || dev >= 64 || allowed[dev].load() < smem)) {
+    e = cudaFuncSetAttribute(kv4_attn_kernel<T, D, NQ, SLOTS, COOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) allowed[dev].store(smem);
   }
   const size_t workers = (size_t)p.ctas * (COOP ? 1 : kWarps);
   float *part_o = static_cast<float *>(ws);
@@ -1169,10 +1215,11 @@ cudaError_t launch_variant(const AttnArgs &a, const Kv4Args &c, const Plan &p, b
     wk.nb = std::min(p.nb, a.B - b0);
     wk.R = p.R;
     wk.workers = (int)workers;
-    wk.min_steps = COOP ? kWarps : 1;
+    wk.min_steps = COOP ? 2 * kWarps : 1;
+    wk.units = (int)std::min<long long>(0x7fffffff, (long long)wk.nb * a.Hkv * ((p.rows + p.R - 1) / p.R));
     wk.split = split ? 1 : 0;
     kv4_attn_kernel<T, D, NQ, SLOTS, COOP><<<p.ctas, kThreads, smem, s>>>(a, c, wk, part_o, part_lse);
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     if (!split) continue;
     // The merge's launch overlaps the shares; it waits for them itself.
@@ -1237,8 +1284,36 @@ bool expanded_request(const AttnArgs &a, unsigned char *ws, AttnArgs *e) {
   return a.Sq > 1 && sm100_supports(*e);
 }
 
-// From this many (head, query row) pairs of a kv head on AUTO expands.
-constexpr int kExpandRows = 256;
+// Which form AUTO takes, by what both were measured to cost on B200 (us):
+//   direct    8 + 0.0005 a 16-token tile, kv head and block of 8 pairs (twice
+//             that at head_dim 256): the unpacking is done again for each block
+//   expanded  10 + the expansion's bytes at 5.5 TB/s + 1.95 a block of 128 keys
+//             and wave of work items (256 query rows of a head; 128 at head_dim
+//             256): the prefill's items do not share their keys' axis
+// e.g. 2 sequences of 8192 tokens, 32 heads of 128 on 8 kv heads: 64 query rows
+// 129 against 142 us, 128 rows 242 against 142; one of 65536 tokens: 64 rows
+// 456 against 989, 512 rows 3517 against 992.  The expanded rows may take
+// kExpandedBytes at most: max_kv_len may be far above the lengths in use.
+constexpr double kExpandedBytes = 4294967296.0;
+bool expanded_is_faster(const AttnArgs &a) {
+  const double wide = a.D == 256 ? 2.0 : 1.0;
+  double span = a.Skv;
+  if (a.window >= 0) span = std::min<double>(span, (double)a.window + a.Sq + 15);
+  const double blocks = ((double)a.group * a.Sq + 7) / 8;
+  const double direct = 8 + 0.0005 * wide * a.B * a.Hkv * std::floor(blocks) * (span / 16);
+  const double rows = (double)a.B * a.Skv * a.Hkv * a.D;
+  const double item_rows = a.D == 256 ? 128 : 256;
+  const double waves = std::ceil((double)a.B * a.H * std::ceil(a.Sq / item_rows) / a.num_sms);
+  const double expanded = 10 + rows * 5.125 / 5.5e6 + 1.95 * waves * (span / 128);
+  return 4 * rows <= kExpandedBytes && expanded < direct;
+}
+
+// The direct form counts steps and output rows in 31 bits.
+bool direct_fits(const AttnArgs &a) {
+  const double pairs = (double)a.group * a.Sq;
+  return ((double)a.Skv / 16 + 2) * a.Hkv * (pairs / 2 + 1) < 2147483647.0 &&
+         (double)std::min(a.B, kMaxSlice) * a.Sq * a.H < 2147483647.0;
+}
 
 // Whether the request runs expanded; `s` gets the refusal of a forced form.
 bool use_expanded(const AttnArgs &a, int algo, llmx_status *s) {
@@ -1249,7 +1324,12 @@ bool use_expanded(const AttnArgs &a, int algo, llmx_status *s) {
   if (algo == LLMX_ALGO_TCGEN05 && !can)
     *s = record_error(LLMX_ERR_UNSUPPORTED,
                       "kv4: TCGEN05 needs max_q_len > 1, sm_scale > 0 and 16-byte aligned rows of q and o");
-  return can && (algo == LLMX_ALGO_TCGEN05 || (algo == LLMX_ALGO_AUTO && (long long)a.group * a.Sq >= kExpandRows));
+  const bool direct = direct_fits(a);
+  const bool expand = can && (algo == LLMX_ALGO_TCGEN05 || (algo == LLMX_ALGO_AUTO && (!direct || expanded_is_faster(a))));
+  if (*s == LLMX_OK && !expand && !direct)
+    *s = record_error(LLMX_ERR_UNSUPPORTED,
+                      "kv4: too many query rows for the direct form (max_kv_len / 16 * n_heads * max_q_len / 2 must stay below 2^31)");
+  return expand;
 }
 
 bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -1270,10 +1350,6 @@ llmx_status check(const llmx_attn_params *p, const llmx_kv4_cache *c, AttnArgs *
   if (p->algo == LLMX_ALGO_SIMT) return record_error(LLMX_ERR_UNSUPPORTED, "kv4: algo must be AUTO, DECODE or TCGEN05");
   if (((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->o)) & 1u) != 0)
     return bad("kv4: q and o must be aligned to their elements");
-  if ((long long)a->group * a->Sq > 0x3fffffffLL || (long long)std::min(a->B, kMaxSlice) * a->Sq > 65535)
-    return bad("kv4: too many query rows for one call");
-  if (((long long)a->Skv / 16 + 2) * a->Hkv * ((long long)a->group * a->Sq / 2 + 1) > 0x7fffffffLL)
-    return bad("kv4: too much work in one sequence (max_kv_len / 16 * n_heads * max_q_len / 2 must be below 2^31)");
   k->vec = al16(p->q) && al16(p->o);
   for (int i = 0; i < 3; ++i) k->vec = k->vec && p->q_stride[i] % 8 == 0 && p->o_stride[i] % 8 == 0;
   a->window = std::min(a->window, 1 << 30);  // past every length; keeps the ranges inside 32 bits

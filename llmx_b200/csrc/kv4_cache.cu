@@ -16,7 +16,7 @@
 namespace llmx_b200 {
 namespace {
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 // From this many tiles on a warp takes a whole tile.
 constexpr int kManyTiles = 1024;
 
@@ -105,7 +105,8 @@ __device__ __forceinline__ uint32_t param_of(uint32_t low_neg_high) {
   const uint32_t hi_bits = (low_neg_high >> 16) ^ 0x8000u;
   const unsigned short lo16 = (unsigned short)low_neg_high, hi16 = (unsigned short)hi_bits;
   const float range = Elem<T>::to_f(*reinterpret_cast<const T *>(&hi16)) - Elem<T>::to_f(*reinterpret_cast<const T *>(&lo16));
-  const T st = round_up_to<T>(__fdiv_rn(range, 15.f));
+  // A range that is not finite gives a step that is a NaN.
+  const T st = round_up_to<T>(range < CUDART_INF_F ? __fdiv_rn(range, 15.f) : CUDART_NAN_F);
   return (uint32_t) * reinterpret_cast<const unsigned short *>(&st) | ((uint32_t)lo16 << 16);
 }
 // 1 / s, 0 for s = 0, or -1 where codes_any() has to divide: between these
@@ -177,7 +178,7 @@ __device__ __forceinline__ uint32_t codes(const uint4 &raw, uint32_t param, floa
   return word;
 }
 // The same for any step: outside the bounds above it divides, and a step that
-// is not finite gives 0 (the group reads back as NaN through s or m).
+// is a NaN gives 0 (the group reads back as NaN).
 template <typename T>
 __device__ __noinline__ uint32_t codes_any(uint4 raw, uint32_t param, float inv) {
   if (inv >= 0.f) return codes<T>(raw, param, inv);
@@ -187,7 +188,7 @@ __device__ __noinline__ uint32_t codes_any(uint4 raw, uint32_t param, float inv)
   uint32_t word = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float q = sm.x > 0.f && sm.x < CUDART_INF_F ? __fdiv_rn(f[i] - sm.y, sm.x) : 0.f;
+    const float q = sm.x > 0.f ? __fdiv_rn(f[i] - sm.y, sm.x) : 0.f;
     word |= (uint32_t)min(15, __float2int_rn(q)) << (4 * i);
   }
   return word;
@@ -234,7 +235,7 @@ __device__ __forceinline__ bool row_here(const TileAt &t, int tok) {
 }
 
 template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(kRowThreads, D == 256 ? 1 : 3) kv4_store_kernel(const __grid_constant__ Kv4Args a,
+__global__ void __launch_bounds__(kRowThreads, D == 256 ? 2 : 4) kv4_store_kernel(const __grid_constant__ Kv4Args a,
                                                                 const __grid_constant__ RowArgs r) {
   constexpr int G = D / kKv4Group;
   const int lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;

@@ -23,6 +23,7 @@ def quantise(x: torch.Tensor):
     s = r.to(x.dtype)
     bumped = (s.view(torch.int16) + 1).view(x.dtype)
     s = torch.where(s.float() < r, bumped, s)
+    s = torch.where(r.isfinite(), s, torch.full_like(s, float("nan")))
     diff = (y.double() - m.double()[..., None]).float().double()
     q = (diff / s.double()[..., None]).float()
     n = torch.where(s.float()[..., None] > 0, q, torch.zeros_like(q)).nan_to_num(0.0).round().clamp(0, 15)
@@ -83,16 +84,18 @@ def write_token(tile: torch.Tensor, tok: int, k: torch.Tensor, v: torch.Tensor) 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_len: int, kv_len: int, *, sm_scale: float,
               causal: bool = True, window: int = -1, cap: float = 0.0, slopes: Optional[torch.Tensor] = None):
     """One sequence in fp64: q [S, H, D] and the cached x = raw keys / values
-    [N, Hkv, D] (quantised here).  Returns (o, lse, bound): the output, the
-    log-sum-exp and how far a kernel that keeps its sums in fp32 and rounds
-    p s to fp16 may be from it, before its output's own rounding."""
+    [N, Hkv, D] (quantised here).  Returns (o, lse, bound, lse_bound): the output, the
+    log-sum-exp, how far a kernel that keeps its sums in fp32 and rounds q to 16
+    bits of its row's maximum and p s to fp16 may be from the output, before the
+    output's own rounding, and how far from the log-sum-exp."""
     S, H, D = q.shape
     Hkv = k.shape[1]
     o = torch.zeros(S, H, D, dtype=torch.float64)
     lse = torch.full((H, S), -math.inf, dtype=torch.float64)
     bound = torch.zeros_like(o)
+    lse_bound = torch.zeros_like(lse)
     if kv_len == 0 or q_len == 0:
-        return o, lse, bound
+        return o, lse, bound, lse_bound
     k, v = k[:kv_len], v[:kv_len]
     kn, ks, km = quantise(k)
     kd = kn.double() * spread(ks) + spread(km)
@@ -115,9 +118,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_len: int, kv_
         # fp32 sums of at most 64 terms of size <= mag a group (2^-17 mag), and
         # a handful of fp32 roundings of the score itself.
         off = mag * 2.0 ** -17 + s.abs() * 2.0 ** -21
-        # q as an integer of at most 32512: half a step (and fp32's rounding of the product) a channel.
+        # q as an integer of at most 32512: half a step (and fp32's rounding of the product) a channel, which
+        # meets n - 8, and half a step a group from the rounding of what corrects for the 8.
         step = q[:q_len, h].double().abs().amax(-1, keepdim=True) / 32512
-        off = off + 0.51 * step * (kn[:, g].double() * spread(ks)[:, g]).sum(-1) * abs(sm_scale)
+        off = off + step * (0.51 * ((kn[:, g].double() - 8).abs() * spread(ks)[:, g]).sum(-1)
+                            + 0.51 * ks[:, g].double().sum(-1)) * abs(sm_scale)
         if cap > 0:
             s = cap * torch.tanh(s / cap)
             off = off + cap * 2.0 ** -21  # tanhf: 2 ulp of at most 1
@@ -133,6 +138,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_len: int, kv_
         p = p / l.masked_fill(none, 1.0)
         lse[h, :q_len] = (top + torch.log(l))[:, 0]
         o[:q_len, h] = p @ (vc[:, g] + va[:, g])
+        # A log-sum-exp moves by no more than the largest of its scores does; 2^-20 for the sum's terms
+        # (N 2^-23 more) and the logarithm, 2^-20 of its size for the roundings of a biased one.
+        worst = off.masked_fill(~seen, 0.0).amax(-1)
+        lse_bound[h, :q_len] = worst + 2.0 ** -20 + kv_len * 2.0 ** -23 + lse[h, :q_len].abs().nan_to_num(0, 0, 0) * 2.0 ** -20
         # Relative error of p: the score's, the exponential's, the sums' (N terms).
         rho = torch.expm1(2 * off.masked_fill(~seen, 0.0).amax(-1, keepdim=True)) + 2.0 ** -20 + kv_len * 2.0 ** -23
         size = p @ (vc[:, g].abs() + va[:, g].abs())
@@ -140,4 +149,4 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_len: int, kv_
         # of a scale that puts the largest s at 2^7 at least.
         tiny = kv_len * 8 * 2.0 ** -32 * float(spread(vs).nan_to_num(0.0, 0.0, 0.0).max())
         bound[:q_len, h] = p @ vc[:, g].abs() * 2.0 ** -11 + 2 * rho * size + tiny
-    return o, lse, bound
+    return o, lse, bound, lse_bound

@@ -177,6 +177,33 @@ def test_workspace_sizes():
     assert lib.llmx_kv4_attn_workspace_size(ctypes.byref(p), ctypes.byref(c), None) == 1
 
 
+def test_auto_form_follows_work_and_room():
+    """AUTO expands long query blocks, never into more than 4 GiB; DECODE and short blocks do not."""
+    lib = _lib.load()
+    ws = ctypes.c_size_t(0)
+
+    def size(algo, q_len, pages):
+        p = _params(max_q_len=q_len, algo=_lib.ALGO[algo], n_heads=32, n_kv_heads=8, max_kv_len=pages * 64)
+        lib.llmx_attn_set_contiguous_strides(ctypes.byref(p))
+        c = _cache(n_kv_heads=8, max_pages=pages, n_pages=2 * pages, page_stride=8 * 4 * 18 * 128)
+        assert lib.llmx_kv4_attn_workspace_size(ctypes.byref(p), ctypes.byref(c), ctypes.byref(ws)) == 0
+        return ws.value
+
+    expanded = 2 * 2 * 8192 * 8 * 128 * 2 + 256
+    assert size("tcgen05", 512, 128) == expanded and size("auto", 512, 128) == expanded
+    assert size("auto", 8, 128) == size("decode", 8, 128) < expanded
+    assert size("decode", 512, 128) < expanded
+    assert size("tcgen05", 512, 16384) > 4 << 30 > size("auto", 512, 16384)
+    # More query rows than the direct form counts: AUTO expands whatever it takes, DECODE refuses.
+    p = _params(max_q_len=1 << 16, algo=_lib.ALGO["decode"], n_heads=32, n_kv_heads=8, max_kv_len=16384 * 64)
+    lib.llmx_attn_set_contiguous_strides(ctypes.byref(p))
+    c = _cache(n_kv_heads=8, max_pages=16384, n_pages=32768, page_stride=8 * 4 * 18 * 128)
+    assert lib.llmx_kv4_attn_workspace_size(ctypes.byref(p), ctypes.byref(c), ctypes.byref(ws)) == 2
+    assert b"too many query rows" in lib.llmx_attn_last_error()
+    p.algo = _lib.ALGO["auto"]
+    assert lib.llmx_kv4_attn_workspace_size(ctypes.byref(p), ctypes.byref(c), ctypes.byref(ws)) == 0 and ws.value > 4 << 30
+
+
 def test_python_checks():
     with pytest.raises(RuntimeError, match="head_dim"):
         llmx_b200.kv4_empty(4, 2, 96, device="cpu")
