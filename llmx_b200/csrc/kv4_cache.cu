@@ -157,6 +157,20 @@ __device__ __forceinline__ void finish_groups(uint32_t (&v)[N], uint32_t (&param
   }
 }
 
+// x - m of the two halves of a register, straight from 16 bits.
+template <typename T>
+__device__ __forceinline__ void minus2(uint32_t x, float m, float &lo, float &hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %3;}"
+        : "=f"(lo), "=f"(hi)
+        : "r"(x), "f"(m));
+  } else {
+    asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.bf16 %0, l, %3;\n\tsub.rn.f32.bf16 %1, h, %3;}"
+        : "=f"(lo), "=f"(hi)
+        : "r"(x), "f"(m));
+  }
+}
+
 // The code word of 8 channels.  The quotient is the correctly rounded one
 // (Markstein: a product with the rounded reciprocal and one step with the
 // exact remainder), without the division; adding 1.5 * 2^23 rounds it to the
@@ -164,15 +178,17 @@ __device__ __forceinline__ void finish_groups(uint32_t (&v)[N], uint32_t (&param
 // word.
 template <typename T>
 __device__ __forceinline__ uint32_t codes(const uint4 &raw, uint32_t param, float inv) {
-  float f[8];
-  unpack8<T>(raw, f);
   const float2 sm = kv4_unpack_param<T>(param);
+  float d[8];
+  minus2<T>(raw.x, sm.y, d[0], d[1]);
+  minus2<T>(raw.y, sm.y, d[2], d[3]);
+  minus2<T>(raw.z, sm.y, d[4], d[5]);
+  minus2<T>(raw.w, sm.y, d[6], d[7]);
   uint32_t word = 0u - 0x4b400000u * 0x11111111u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float d = f[i] - sm.y;
-    const float q = d * inv;
-    const float r = fmaf(fmaf(-q, sm.x, d), inv, q);
+    const float q = d[i] * inv;
+    const float r = fmaf(fmaf(-q, sm.x, d[i]), inv, q);
     word += __float_as_uint(r + 12582912.f) << (4 * i);
   }
   return word;

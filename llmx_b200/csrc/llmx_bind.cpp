@@ -176,7 +176,8 @@ const int32_t *int_arg(const char *name, const std::optional<torch::Tensor> &t, 
                        torch::Tensor &keep) {
   if (!t.has_value()) return nullptr;
   TORCH_CHECK(t->is_cuda() && t->device() == dev, name, " must be on the cache's device");
-  keep = t->to(torch::kInt).contiguous();
+  // The usual tensor is taken as it is: each conversion call costs a microsecond even when it has nothing to do.
+  keep = t->scalar_type() == torch::kInt && t->is_contiguous() ? *t : t->to(torch::kInt).contiguous();
   TORCH_CHECK(keep.numel() == batch, name, " must have batch elements");
   return keep.data_ptr<int32_t>();
 }
