@@ -281,8 +281,8 @@ LLMX_API llmx_status llmx_convert(const void *src, int32_t src_dtype, void *dst,
  * no token of the sequence are not read.  An entry outside [0, n_pages), or a
  * position outside [0, max_pages * page_size), is skipped, never followed: a
  * store drops those rows, a load writes 0 for them, the attention does not
- * see them, and llmx_attn_device_status then returns
- * LLMX_ERR_INVALID_ARGUMENT.  Two rows stored to the same place by one call
+ * see them (its expanded form takes them as the load's zeros), and
+ * llmx_attn_device_status then returns LLMX_ERR_INVALID_ARGUMENT.  Two rows stored to the same place by one call
  * leave an undefined mix of both there. */
 #define LLMX_KV4_GROUP 64
 #define LLMX_KV4_TILE_TOKENS 16

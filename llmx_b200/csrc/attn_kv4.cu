@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
         const int page = tile / tpp;
         const long long off = kv4_page_offset(c, pl.b, page);
         bad = off < 0;
-        if (!bad) where = c.data + pl.kvh * c.head_stride + off + (tile - page * tpp) * Sh::kTile;
+        if (!bad) where = c.data + pl.kvh * c.head_stride + off + (long long)(tile - page * tpp) * Sh::kTile;
       }
     }
     bad_issue = __ballot_sync(0xffffffffu, bad);
@@ -1350,6 +1350,9 @@ llmx_status check(const llmx_attn_params *p, const llmx_kv4_cache *c, AttnArgs *
   if (p->algo == LLMX_ALGO_SIMT) return record_error(LLMX_ERR_UNSUPPORTED, "kv4: algo must be AUTO, DECODE or TCGEN05");
   if (((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->o)) & 1u) != 0)
     return bad("kv4: q and o must be aligned to their elements");
+  const int64_t extent[3] = {p->batch, p->max_q_len, p->n_heads};
+  for (int i = 0; i < 3; ++i)
+    if (p->o_stride[i] == 0 && extent[i] > 1) return bad("kv4: rows of o must not overlap (stride 0)");
   k->vec = al16(p->q) && al16(p->o);
   for (int i = 0; i < 3; ++i) k->vec = k->vec && p->q_stride[i] % 8 == 0 && p->o_stride[i] % 8 == 0;
   a->window = std::min(a->window, 1 << 30);  // past every length; keeps the ranges inside 32 bits

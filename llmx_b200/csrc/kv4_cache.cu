@@ -624,6 +624,10 @@ extern "C" llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_row
   Kv4Args k;
   st = prepare_kv4(c, rows->batch, &k);
   if (st != LLMX_OK || rows->batch == 0 || rows->max_rows == 0) return st;
+  const int64_t extent[3] = {rows->batch, rows->max_rows, c->n_kv_heads};
+  for (int i = 0; i < 3; ++i)
+    if (extent[i] > 1 && (rows->k_stride[i] == 0 || rows->v_stride[i] == 0))
+      return bad("kv4: rows that are written must not overlap (stride 0)");
   const cudaError_t e = launch_kv4_load(k, *rows, c->dtype, 0, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? LLMX_OK : record_error(LLMX_ERR_CUDA, cudaGetErrorString(e));
 }

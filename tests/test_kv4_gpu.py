@@ -646,3 +646,71 @@ def test_offsets_past_32_bits():
     out = torch.empty_like(q, device=DEV)
     llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, block_table=table, max_kv_len=200)
     check(out, None, q, k, v, [1], [200], dtype, sm_scale=d ** -0.5)
+
+
+def test_offsets_past_32_bits_inside_a_page():
+    """One page of 7.7 million tokens (2.2 GB): offsets of tiles in their page pass 2^31."""
+    dtype, d = torch.bfloat16, 256
+    tiles = 482000
+    cache = torch.empty(1, 1, tiles, 18 * d, dtype=torch.uint8, device=DEV)
+    n = 16 * tiles
+    gen = torch.Generator().manual_seed(52)
+    k, v = rows(gen, 150, 1, d, dtype)[None], rows(gen, 150, 1, d, dtype)[None]
+    start = torch.tensor([n - 150], device=DEV, dtype=torch.int32)
+    llmx_b200.kv4_store(cache, k.to(DEV), v.to(DEV), start=start)
+    ko, vo = torch.empty_like(k, device=DEV), torch.empty_like(v, device=DEV)
+    llmx_b200.kv4_load(cache, ko, vo, start=start)
+    assert torch.equal(ko.cpu(), okv4.values(k)[1]) and torch.equal(vo.cpu(), okv4.values(v)[1])
+    q = torch.randn(1, 1, 4, d, generator=gen).to(dtype)
+    out = torch.empty_like(q, device=DEV)
+    llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, 149)  # a window of the last 150 tokens
+    check(out, None, q, k, v, [1], [150], dtype, sm_scale=d ** -0.5)
+
+
+def test_expanded_form_with_empty_and_tiny_sequences():
+    dtype, d, H, hkv, sq = torch.float16, 128, 4, 2, 33
+    gen = torch.Generator().manual_seed(61)
+    lens = [0, 1, 200, 33]
+    cache, table, k, v = filled(gen, lens, hkv, d, dtype, 64)
+    q = torch.randn(len(lens), sq, H, d, generator=gen).to(dtype)
+    q_lens = [33, 1, 0, 20]
+    import oracle
+
+    ref = oracle.attention_ref_padded(q.float(), okv4.values(k)[1].float(), okv4.values(v)[1].float(), kv_lens=lens,
+                                      q_lens=q_lens, sm_scale=d ** -0.5)
+    for algo in ("tcgen05", "decode"):
+        poison = torch.full((1 << 20,), float("nan"), device=DEV)
+        del poison
+        out = torch.full_like(q, 3.0, device=DEV)
+        llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, kv_lens=torch.tensor(lens, device=DEV), block_table=table,
+                                q_lens=torch.tensor(q_lens, device=DEV), algo=algo)
+        assert (out.float().cpu() - ref).abs().max() <= HALF_MAX_ABS, algo
+
+
+def test_overlapping_outputs_are_refused():
+    cache = garbage(2, 2, 64, 16)
+    k = torch.zeros(1, 1, 1, 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(LlmxError, match="overlap"):
+        llmx_b200.kv4_load(cache, k.expand(2, 4, 2, 64), torch.empty(2, 4, 2, 64, dtype=torch.float16, device=DEV))
+    with pytest.raises(LlmxError, match="overlap"):
+        llmx_b200.kv4_attention(k.expand(2, 1, 4, 64), torch.zeros(2, 1, 4, 64, dtype=torch.float16, device=DEV), cache, 1.0)
+
+
+def test_pages_shared_by_sequences():
+    """Two sequences with a common prefix: their tables name the same pages."""
+    dtype, d, H, hkv, page = torch.bfloat16, 64, 4, 1, 16
+    gen = torch.Generator().manual_seed(71)
+    k, v = rows(gen, 60, hkv, d, dtype), rows(gen, 60, hkv, d, dtype)
+    cache = garbage(6, hkv, d, page)
+    # tokens 0 .. 31 in pages 4, 2; the tails 32 .. of the sequences in 0 and 5
+    llmx_b200.kv4_store(cache, k[None, :44].to(DEV), v[None, :44].to(DEV), block_table=torch.tensor([[4, 2, 0]], dtype=torch.int32, device=DEV))
+    tail = torch.tensor([32], device=DEV, dtype=torch.int32)
+    table = torch.tensor([[4, 2, 0], [4, 2, 5]], dtype=torch.int32, device=DEV)
+    llmx_b200.kv4_store(cache, k[None, 44:].to(DEV), v[None, 44:].to(DEV), start=tail, block_table=table[1:])
+    lens = [44, 48]
+    kk = torch.stack([torch.nn.functional.pad(k[:44], (0, 0, 0, 0, 0, 4)), torch.cat([k[:32], k[44:60]])])
+    vv = torch.stack([torch.nn.functional.pad(v[:44], (0, 0, 0, 0, 0, 4)), torch.cat([v[:32], v[44:60]])])
+    q = torch.randn(2, 2, H, d, generator=gen).to(dtype)
+    out = torch.empty_like(q, device=DEV)
+    llmx_b200.kv4_attention(out, q.to(DEV), cache, 0.125, kv_lens=torch.tensor(lens, device=DEV), block_table=table)
+    check(out, None, q, kk, vv, [2, 2], lens, dtype, sm_scale=0.125)
