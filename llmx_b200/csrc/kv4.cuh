@@ -17,8 +17,8 @@ struct Kv4Args {
   unsigned int *err;
 };
 
-// Checks *c for `batch` sequences and the current device; fills *k.
-llmx_status prepare_kv4(const llmx_kv4_cache *c, int batch, Kv4Args *k);
+// Checks *c for `rows` and the current device; fills *k.
+llmx_status prepare_kv4(const llmx_kv4_cache *c, const llmx_kv4_rows &rows, Kv4Args *k);
 // The checks alone, without a device.
 llmx_status validate_kv4(const llmx_kv4_cache *c, int batch, Kv4Args *k);
 // The rows' kernels without their checks, for the attention's expanded form:

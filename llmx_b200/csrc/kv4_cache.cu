@@ -478,6 +478,11 @@ bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 llmx_status bad(const char *msg) { return record_error(LLMX_ERR_INVALID_ARGUMENT, msg); }
 
+// What the kernels number in 32 bits: the tiles of a sequence's rows, all heads.
+bool rows_fit(const llmx_kv4_rows &r, int heads) {
+  return ((long long)r.max_rows / 16 + 2) * heads < (1LL << 31);
+}
+
 llmx_status validate_rows(const llmx_kv4_rows *r) {
   if (r == nullptr) return bad("kv4: rows is NULL");
   if (r->batch < 0 || r->batch > 65535 || r->max_rows < 0) return bad("kv4: batch must be in [0, 65535] and max_rows >= 0");
@@ -584,9 +589,10 @@ llmx_status validate_kv4(const llmx_kv4_cache *c, int batch, Kv4Args *k) {
   return LLMX_OK;
 }
 
-llmx_status prepare_kv4(const llmx_kv4_cache *c, int batch, Kv4Args *k) {
-  const llmx_status s = validate_kv4(c, batch, k);
+llmx_status prepare_kv4(const llmx_kv4_cache *c, const llmx_kv4_rows &rows, Kv4Args *k) {
+  const llmx_status s = validate_kv4(c, rows.batch, k);
   if (s != LLMX_OK) return s;
+  if (!rows_fit(rows, c->n_kv_heads)) return bad("kv4: max_rows / 16 * n_kv_heads must stay below 2^31");
   int sms = 0;
   return current_device_info(&k->err, &sms);
 }
@@ -612,7 +618,7 @@ extern "C" llmx_status llmx_kv4_store(const llmx_kv4_cache *c, const llmx_kv4_ro
   llmx_status st = validate_rows(rows);
   if (st != LLMX_OK) return st;
   Kv4Args k;
-  st = prepare_kv4(c, rows->batch, &k);
+  st = prepare_kv4(c, *rows, &k);
   if (st != LLMX_OK || rows->batch == 0 || rows->max_rows == 0) return st;
   const cudaError_t e = launch_rows(true, k, *rows, c->dtype, 0, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? LLMX_OK : record_error(LLMX_ERR_CUDA, cudaGetErrorString(e));
@@ -622,7 +628,7 @@ extern "C" llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_row
   llmx_status st = validate_rows(rows);
   if (st != LLMX_OK) return st;
   Kv4Args k;
-  st = prepare_kv4(c, rows->batch, &k);
+  st = prepare_kv4(c, *rows, &k);
   if (st != LLMX_OK || rows->batch == 0 || rows->max_rows == 0) return st;
   const int64_t extent[3] = {rows->batch, rows->max_rows, c->n_kv_heads};
   for (int i = 0; i < 3; ++i)

@@ -225,3 +225,13 @@ def test_python_checks():
         kv4.kv4_attention_ctypes(k, k, cache, 1.0)
     with pytest.raises(RuntimeError, match="CUDA"):
         kv4._rows_call("llmx_kv4_store", cache, k, k, None, None, None)
+
+
+def test_sizes_that_the_launches_cannot_number():
+    """Tiles of one sequence's rows past 31 bits are refused."""
+    lib = _lib.load()
+    c = _cache(n_kv_heads=60000, page_stride=60000 * 4 * 18 * 128)
+    r = _rows(max_rows=(1 << 31) - 1)
+    for fn in (lib.llmx_kv4_store, lib.llmx_kv4_load):
+        assert fn(ctypes.byref(c), ctypes.byref(r), None) == 1
+        assert b"max_rows" in lib.llmx_attn_last_error()
