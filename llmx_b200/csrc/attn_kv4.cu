@@ -70,11 +70,14 @@ constexpr float kLn2 = 0.6931471805599453f;
 // much (log2): p reaches 2^6 at most, and p s at most 2^14 in fp16.
 constexpr float kLazyMax = 6.f;
 constexpr float kQTop = 32512.f;  // 127 * 256: q's largest value as an integer
-// The largest weight times the largest step stays in [2^7, 2^8) (times 2^6
-// under a lazy maximum): fp16 then keeps 11 bits of weights down to 2^-21 of
-// the largest.  Steps count from 2^-40 on (smaller ones lose bits from 2^-61
-// on), which keeps the sums of scaled weights inside fp32.
+// The largest weight times the largest step that its row sees stays in
+// [2^7, 2^8) (times 2^6 under a lazy maximum): fp16 then keeps 11 bits of
+// weights down to 2^-21 of the largest.  Steps count from 2^-40 on (smaller
+// ones lose bits from 2^-61 on), and a centre m + 8 s counts as a step of 2^-20
+// of it: this keeps the sums of scaled weights, and of these times the centres,
+// inside fp32.
 constexpr int kStepExp = 7;
+constexpr float kCentreStep = 0x1p-20f;
 constexpr int kMinStepExp = -40;
 constexpr int kMaxStepExp = 125;
 constexpr uint64_t kWaitNs = 1000000000ull;
@@ -620,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
     // What a score starts from: minus its row's reference, which with a
     // soft-cap comes off behind the tanh.  0 while there is none.
     float start[NQ], after[NQ];
-    int step_exp = kMinStepExp;
+    int step_exp[NQ];                    // of the steps that the row has seen
     bool fresh = true;                   // some row has no reference yet (the same in all lanes)
     float limit = 0.f, next_step = 0.f;  // a score above `limit` or a step from `next_step` on moves the references
 #pragma unroll
@@ -633,6 +636,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
     for (int q = 0; q < NQ; ++q) {
       l[q] = start[q] = after[q] = 0.f;
       ref[q] = -CUDART_INF_F;
+      step_exp[q] = kMinStepExp;
 #pragma unroll
       for (int h = 0; h < G; ++h) aff[q][h] = 0.f;
     }
@@ -748,28 +752,37 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
       }
       // ---- the references move, with everything accumulated, when a score
       // passes its row's maximum by kLazyMax or a larger step turns up
-      float most = -CUDART_INF_F, smax = 0.f;
+      float most = -CUDART_INF_F, smax = 0.f, cmax = 0.f;
 #pragma unroll
       for (int q = 0; q < NQ; ++q) most = max3(most, s[0][q], s[1][q]);
 #pragma unroll
-      for (int h = 0; h < G; ++h) smax = max3(smax, sv[0][h], sv[1][h]);
-      if (__any_sync(0xffffffffu, fresh || most > limit || smax >= next_step)) {
-        uint32_t bits = 0;
+      for (int h = 0; h < G; ++h) {
+        smax = max3(smax, sv[0][h], sv[1][h]);
+        cmax = max3(cmax, fabsf(cv[0][h]), fabsf(cv[1][h]));
+      }
+      if (__any_sync(0xffffffffu, fresh || most > limit || smax >= next_step || cmax * kCentreStep >= next_step)) {
+        uint32_t bits[2] = {0u, 0u};  // the largest finite step of each token
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
           for (int h = 0; h < G; ++h) {
-            const uint32_t x = __float_as_uint(sv[r][h]);
-            bits = max(bits, x < 0x7f800000u ? x : 0u);
+            const uint32_t x = __float_as_uint(fmaxf(sv[r][h], fabsf(cv[r][h]) * kCentreStep));
+            bits[r] = max(bits[r], x < 0x7f800000u ? x : 0u);
           }
-        const int new_exp = max(step_exp, min(kMaxStepExp, (int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 127));
-        const float old_room = (float)(kStepExp - step_exp), new_room = (float)(kStepExp - new_exp);
-        step_exp = new_exp;
-        limit = kLazyMax + new_room;
-        next_step = pow2i(new_exp + 1);
         bool missing = false;
+        int least = kMaxStepExp, largest = kMinStepExp;  // exponents of this thread's rows
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
+          // Of the tokens that the row sees: a large step that it does not
+          // see must not push its weights out of fp16.
+          uint32_t top = max(!PART || (vis >> q & 1u) ? bits[0] : 0u, !PART || (vis >> NQ + q & 1u) ? bits[1] : 0u);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const int new_exp = max(step_exp[q], min(kMaxStepExp, (int)(top >> 23) - 127));
+          const float old_room = (float)(kStepExp - step_exp[q]), new_room = (float)(kStepExp - new_exp);
+          step_exp[q] = new_exp;
+          least = min(least, new_exp);
+          largest = max(largest, new_exp);
           const bool none = ref[q] == -CUDART_INF_F;
           const float shift = none ? 0.f : ref[q];
           float v = fmaxf(s[0][q], s[1][q]) + shift;
@@ -777,7 +790,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
           for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
           const float m = none ? v : fmaxf(ref[q] + old_room, v);
           const float now = m == -CUDART_INF_F ? m : m - new_room;
-          const float al = none ? 1.f : exp2_fast(ref[q] - now);
+          // In two halves: steps 2^126 apart still add up in the sum of weights.
+          const float root = none ? 1.f : exp2_fast(0.5f * (ref[q] - now)), al = root * root;
           const float back = now == -CUDART_INF_F ? 0.f : shift - now;
           ref[q] = now;
           missing |= now == -CUDART_INF_F;
@@ -786,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
           after[q] = minus;
           s[0][q] += back;
           s[1][q] += back;
-          l[q] *= al;
+          l[q] = l[q] * root * root;
 #pragma unroll
           for (int h = 0; h < G; ++h) {
             aff[q][h] *= al;
@@ -801,6 +815,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
             }
           }
         }
+        // The lower of two rows' thresholds: at worst the references are looked at more often.
+        limit = kLazyMax + (float)(kStepExp - largest);
+        next_step = pow2i(least + 1);
         fresh = __any_sync(0xffffffffu, missing);
       }
       // ---- weights
@@ -927,9 +944,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
         const float other = __shfl_xor_sync(0xffffffffu, m, 2);
         const float both = fmaxf(m, other);
         // Columns that saw no finite score add nothing, unless their sum is a NaN.
-        const float wt = m == -CUDART_INF_F ? (sum == sum ? 0.f : 1.f) : exp2_fast(m - both);
+        const float root = m == -CUDART_INF_F ? (sum == sum ? 0.f : 1.f) : exp2_fast(0.5f * (m - both)), wt = root * root;
         m = both;
-        sum *= wt;
+        sum = sum * root * root;
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
         for (int h = 0; h < G; ++h)
@@ -1007,9 +1024,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
           const float lw = sm_l[w][pr];
           // A warp that saw no finite score adds nothing, unless its sum is a NaN.
           if (mw[w] == -CUDART_INF_F && lw == lw) continue;
-          const float wt = mw[w] == -CUDART_INF_F ? 1.f : exp2_fast(mw[w] - top);
+          const float root = mw[w] == -CUDART_INF_F ? 1.f : exp2_fast(0.5f * (mw[w] - top)), wt = root * root;
           const float4 x = *reinterpret_cast<const float4 *>(smem + w * Sh::kRing + (pr * Sh::kMergeRow + d) * 4);
-          sum = fmaf(lw, wt, sum);
+          sum = fmaf(lw * root, root, sum);
           ov.x = fmaf(x.x, wt, ov.x);
           ov.y = fmaf(x.y, wt, ov.y);
           ov.z = fmaf(x.z, wt, ov.z);

@@ -146,7 +146,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_len: int, kv_
         rho = torch.expm1(2 * off.masked_fill(~seen, 0.0).amax(-1, keepdim=True)) + 2.0 ** -20 + kv_len * 2.0 ** -23
         size = p @ (vc[:, g].abs() + va[:, g].abs())
         # p s in fp16: half an ulp (2^-11), or below fp16's normal range 2^-25
-        # of a scale that puts the largest s at 2^7 at least.
-        tiny = kv_len * 8 * 2.0 ** -32 * float(spread(vs).nan_to_num(0.0, 0.0, 0.0).max())
+        # of a scale that puts the largest s (or 2^-20 of a centre) that the row sees at 2^7 at least.
+        widest = torch.maximum(spread(vs)[:, g], (spread(vm) + 8 * spread(vs))[:, g].abs() * 2.0 ** -20)
+        widest = widest.double().nan_to_num(0.0, 0.0, 0.0).amax(-1)  # [N]: of the token's groups
+        tiny = kv_len * 8 * 2.0 ** -32 * torch.where(seen, widest, 0.0).amax(-1, keepdim=True)
         bound[:q_len, h] = p @ vc[:, g].abs() * 2.0 ** -11 + 2 * rho * size + tiny
     return o, lse, bound, lse_bound

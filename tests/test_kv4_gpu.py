@@ -714,3 +714,48 @@ def test_pages_shared_by_sequences():
     out = torch.empty_like(q, device=DEV)
     llmx_b200.kv4_attention(out, q.to(DEV), cache, 0.125, kv_lens=torch.tensor(lens, device=DEV), block_table=table)
     check(out, None, q, kk, vv, [2, 2], lens, dtype, sm_scale=0.125)
+
+
+@pytest.mark.parametrize("opts", ["causal", "alibi", "window"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,H,hkv,sq,n", [(128, 8, 2, 4, 40), (64, 4, 4, 2, 16), (256, 4, 2, 3, 700), (128, 8, 8, 4, 90), (128, 2, 2, 2, 1300)])
+def test_large_values_that_a_row_does_not_see(d, H, hkv, sq, n, dtype, opts):
+    """Values far above the others in the last tokens, which only the last row sees, and with a window in the first
+    one, which only the first row sees: the other rows' weights keep their bits."""
+    gen = torch.Generator().manual_seed(d + n)
+    k, v = rows(gen, n, hkv, d, dtype), rows(gen, n, hkv, d, dtype)
+    small, large = (1e-2, 3e4 / 8) if dtype == torch.float16 else (1.0, 1e25)
+    v = (v * small).to(dtype)
+    window = n - sq if opts == "window" else -1
+    far = 0 if opts == "window" else n - 1
+    v[far] = (rows(gen, 1, hkv, d, dtype)[0].float() * large).to(dtype)
+    slopes = torch.linspace(0.01, 0.2, H) if opts == "alibi" else None
+    cache = garbage(-(-n // 16), hkv, d, 16)
+    table = torch.arange(-(-n // 16), dtype=torch.int32, device=DEV)[None]
+    llmx_b200.kv4_store(cache, k[None].to(DEV), v[None].to(DEV), block_table=table)
+    q = torch.randn(1, sq, H, d, generator=gen).to(dtype)
+    out, lse = torch.empty_like(q, device=DEV), torch.empty(1, H, sq, device=DEV)
+    llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, window, max_kv_len=n, block_table=table, lse=lse, algo="decode",
+                            alibi_slopes=None if slopes is None else slopes.to(DEV))
+    check(out, lse, q, k[None], v[None], [sq], [n], dtype, sm_scale=d ** -0.5, window=window, slopes=slopes, what=opts)
+
+
+@pytest.mark.parametrize("d,H", [(64, 1), (128, 4), (128, 8), (256, 2)])
+@pytest.mark.parametrize("n", [30, 400])
+def test_values_far_apart(d, H, n):
+    """Constant groups of large values (steps of 0), and steps 2^150 apart whose tokens count alike in the sums."""
+    dtype = torch.bfloat16
+    gen = torch.Generator().manual_seed(n + d)
+    k, base = rows(gen, n, 1, d, dtype), rows(gen, n, 1, d, dtype)
+    first = (torch.arange(n) < n // 2)[:, None, None]
+    constant = torch.full_like(base, 1e30)
+    for v in (constant, -constant, torch.where(first, constant, base), torch.where(first, base, constant),
+              torch.where(first, base * 1e-10, base * 1e36), torch.where(first, base * 1e36, base * 1e-10)):
+        v = v.to(dtype)
+        cache = garbage(-(-n // 64), 1, d, 64)
+        table = torch.arange(-(-n // 64), dtype=torch.int32, device=DEV)[None]
+        llmx_b200.kv4_store(cache, k[None].to(DEV), v[None].to(DEV), block_table=table)
+        q = torch.randn(1, 1, H, d, generator=gen).to(dtype)
+        out, lse = torch.empty_like(q, device=DEV), torch.empty(1, H, 1, device=DEV)
+        llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, max_kv_len=n, block_table=table, lse=lse)
+        check(out, lse, q, k[None], v[None], [1], [n], dtype, sm_scale=d ** -0.5, what="far apart")
