@@ -1218,7 +1218,8 @@ cudaError_t launch_variant(const AttnArgs &a, const Kv4Args &c, const Plan &p, b
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (smem > 48 * 1024 && (dev < 0 || dev >= 64 || allowed[dev].load() < smem)) {
+  // (48 KB without the attribute, the kernel's static part, under 1 KB, among them.)
+  if (smem > 47 * 1024 && (dev < 0 || dev >= 64 || allowed[dev].load() < smem)) {
     e = cudaFuncSetAttribute(kv4_attn_kernel<T, D, NQ, SLOTS, COOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) allowed[dev].store(smem);

@@ -759,3 +759,30 @@ def test_values_far_apart(d, H, n):
         out, lse = torch.empty_like(q, device=DEV), torch.empty(1, H, 1, device=DEV)
         llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, max_kv_len=n, block_table=table, lse=lse)
         check(out, lse, q, k[None], v[None], [1], [n], dtype, sm_scale=d ** -0.5, what="far apart")
+
+
+@pytest.mark.parametrize("d,H,hkv,sq,B,top", [
+    (128, 8, 2, 1, 120, 1200),  # a CTA for a unit, long ones too
+    (128, 8, 2, 2, 120, 2600),  # units shared by warps, fewer units than CTAs
+    (64, 8, 2, 1, 120, 2600),   # units shared by CTAs
+    (256, 4, 2, 1, 120, 1300),
+    (64, 4, 4, 1, 700, 90),     # a warp for a unit, in two launches
+    (128, 10, 5, 1, 520, 90),   # more units than warps
+    (128, 5, 5, 3, 520, 700),   # units shared by warps, in two launches
+])
+def test_each_way_of_dealing_units(d, H, hkv, sq, B, top):
+    dtype = torch.float16 if B == 120 else torch.bfloat16
+    gen = torch.Generator().manual_seed(B + top)
+    lens = torch.randint(0, 40, (B,), generator=gen).tolist()
+    lens[0], lens[B // 2], lens[B - 2] = top, 0, top // 2
+    cache, table, k, v = filled(gen, lens, hkv, d, dtype, 16)
+    q = torch.randn(B, sq, H, d, generator=gen).to(dtype)
+    q_lens = [sq] * B
+    q_lens[1] = 0
+    for slopes in (None, torch.linspace(0.01, 0.3, H)):
+        out, lse = torch.full_like(q, 7.0, device=DEV), torch.full((B, H, sq), 7.0, device=DEV)
+        llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, kv_lens=torch.tensor(lens, device=DEV), block_table=table, lse=lse,
+                                q_lens=torch.tensor(q_lens, device=DEV), algo="decode",
+                                alibi_slopes=None if slopes is None else slopes.to(DEV))
+        check(out, lse, q, k, v, q_lens, lens, dtype, sm_scale=d ** -0.5, slopes=slopes)
+    llmx_b200.device_status(0)
