@@ -422,6 +422,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
     if (worker >= n) return;
     begin = share_begin(total, worker, n);
     end = share_begin(total, worker + 1, n);
+  } else if (wk.units <= wk.workers) {
+    // Whole units, one for each worker.
+    const int per_seq = wk.units / wk.nb, i = worker / per_seq, unit = worker - i * per_seq;
+    if (i >= wk.nb) return;
+    const Span sp = span_of<W>(a, wk.R, lens[i].x, lens[i].y);
+    if (unit >= sp.blocks * a.Hkv) return;
+    begin = prefix[i] + (uint32_t)unit * sp.steps;
+    end = begin + sp.steps;
   } else {
     // Whole units: a share ends with the unit that holds its last step.
     auto snap = [&](uint32_t step) {
@@ -1201,8 +1209,22 @@ Plan plan_kv4(const AttnArgs &a) {
   p.nb = (int)std::min<long long>(std::min(a.B, kMaxSlice), std::max<long long>(1, 0x7fffffffLL / (per_seq * steps)));
   const long long units = p.nb * per_seq, most = units * steps;
   const int resident = a.num_sms * (a.D <= 128 ? 4 : 3);
-  p.coop = units <= resident;
-  p.shared = p.coop ? steps > 4 * kWarps && units < resident : steps > 1;
+  // Short sequences: a unit has one worker, which saves the merge's launch and
+  // the second part of a share.  Longer ones are shared out; with many units by
+  // warps, with few by CTAs (equal at about a third of the resident CTAs at
+  // head_dim 128, half of them at 64, all at 256).  Measured, us, 4 heads on each
+  // kv head, head_dim 128, half to all of the given tokens a sequence, whole /
+  // shared by CTAs / shared by warps:
+  //   256 units  600: 13.3 / 17.9 / 18.7   2000: 23 / 27.9 / 27.6    4000: 41 / 36.1 / 35.9
+  //   512 units  600: 18.1 / 26.1 / 25.8   2000: 37.5 / 40.1 / 38.0  4000: 59.9 / 59.9 / 56.2
+  // and whole by warps / shared by warps:
+  //   1024 units  300: 17.4 / 25.6   600: 27.9 / 32.1   1200: 47.8 / 43.4
+  // The rule shares earlier than these would, since one long sequence among short
+  // ones has to wait for a single worker.
+  const bool few = units <= resident;
+  const bool whole = steps <= (few ? 32 + units / 10 : 20);
+  p.coop = few && (whole || units * (a.D == 256 ? 1 : (a.D == 128 ? 3 : 2)) <= resident);
+  p.shared = !whole;
   p.ctas = (int)std::min<long long>(resident, p.shared || !p.coop ? (most + kWarps - 1) / kWarps : units);
   const long long workers = (long long)p.ctas * (p.coop ? 1 : kWarps);
   p.per_unit = (int)std::min<long long>(workers, (workers + units - 1) / units);
