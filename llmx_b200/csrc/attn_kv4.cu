@@ -1078,16 +1078,18 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
 }
 
 // O = sum_s exp(lse_s - lse) O_s over the shares of a unit that several workers
-// have.  A warp per output row, or with many shares (WIDE) a CTA, whose warps
-// take every fourth one.  A lane has D / 32 channels; four shares are read at
-// a time, before their weights are known.
-template <typename T, int D, int W, bool WIDE>
-__global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Work wk,
+// have.  A warp per output row, or with many shares a CTA of PARTS warps, which
+// take every PARTS-th one.  A lane has D / 32 channels; eight shares are read at
+// a time, before their weights are known: what this kernel takes is the latency
+// of a few loads in a row.
+constexpr int kAtOnce = 8;
+template <typename T, int D, int W, int PARTS>
+__global__ void __launch_bounds__(PARTS > 1 ? PARTS * 32 : kThreads) kv4_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Work wk,
                                                              const float *part_o, const float *part_lse) {
   constexpr int E = D / 32;
-  __shared__ float sm_m[kWarps], sm_l[kWarps], sm_o[WIDE ? kWarps : 1][WIDE ? D : 1];
+  __shared__ float sm_m[PARTS], sm_l[PARTS], sm_o[PARTS][PARTS > 1 ? D : 1];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const long long out_row = WIDE ? blockIdx.x : (long long)blockIdx.x * kWarps + warp;
+  const long long out_row = PARTS > 1 ? blockIdx.x : (long long)blockIdx.x * kWarps + warp;
   const int h = (int)(out_row % a.H), i = (int)(out_row / a.H % a.Sq), n = (int)(out_row / a.H / a.Sq), b = wk.b0 + n;
   int w0 = 0, used = 0, R = wk.R, r = 0;
   if (n < wk.nb) {
@@ -1115,15 +1117,14 @@ __global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const __grid_consta
   // nothing to do, so that this kernel ends after them.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (used <= 1) return;  // one worker had the unit whole
-  constexpr int kStride = WIDE ? kWarps : 1;
   float m = -CUDART_INF_F, sum = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s0 = WIDE ? warp : 0; s0 < used; s0 += 4 * kStride) {
-    float l[4], x[4][E];
+  for (int s0 = PARTS > 1 ? warp : 0; s0 < used; s0 += kAtOnce * PARTS) {
+    float l[kAtOnce], x[kAtOnce][E];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int s = s0 + u * kStride;
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int s = s0 + u * PARTS;
       l[u] = -CUDART_INF_F;
 #pragma unroll
       for (int e = 0; e < E; ++e) x[u][e] = 0.f;
@@ -1138,21 +1139,23 @@ __global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const __grid_consta
         }
       }
     }
-    const float top = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), m);
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) top = fmaxf(top, l[u]);
     const float al = m == -CUDART_INF_F ? 0.f : expf(m - top);
     m = top;
     sum *= al;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] *= al;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kAtOnce; ++u) {
       const float w = l[u] == -CUDART_INF_F ? 0.f : expf(l[u] - top);  // a NaN goes on into the sum
       sum += w;
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = fmaf(w, x[u][e], o[e]);
     }
   }
-  if constexpr (WIDE) {
+  if constexpr (PARTS > 1) {
     if (lane == 0) {
       sm_m[warp] = m;
       sm_l[warp] = sum;
@@ -1161,12 +1164,14 @@ __global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const __grid_consta
     for (int e = 0; e < E; ++e) sm_o[warp][lane * E + e] = o[e];
     __syncthreads();
     if (warp != 0) return;
-    m = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+    m = sm_m[0];
+#pragma unroll
+    for (int w = 1; w < PARTS; ++w) m = fmaxf(m, sm_m[w]);
     sum = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < PARTS; ++w) {
       const float wt = sm_m[w] == -CUDART_INF_F ? (sm_l[w] == sm_l[w] ? 0.f : 1.f) : expf(sm_m[w] - m);
       sum = fmaf(sm_l[w], wt, sum);
 #pragma unroll
@@ -1263,19 +1268,23 @@ cudaError_t launch_variant(const AttnArgs &a, const Kv4Args &c, const Plan &p, b
     if (e != cudaSuccess) return e;
     if (!split) continue;
     // The merge's launch overlaps the shares; it waits for them itself.
-    const bool wide = p.per_unit > 8;
+    // Warps of a row by its shares: 8 of them against 4 take 1.8 us less with 74
+    // shares and 1.9 us more with 9 (us of the whole call: 41.0 and 42.7 for one
+    // sequence of 131071 tokens, 49.1 and 47.2 for 32 of up to 8191).
+    const int parts = p.per_unit > 32 ? 8 : (p.per_unit > 8 ? 4 : 1);
     const long long out_rows = (long long)wk.nb * a.Sq * a.H;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(wide ? out_rows : (out_rows + kWarps - 1) / kWarps));
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3((unsigned)(parts > 1 ? out_rows : (out_rows + kWarps - 1) / kWarps));
+    cfg.blockDim = dim3(parts > 1 ? parts * 32 : kThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, wide ? kv4_merge_kernel<T, D, Sh::W, true> : kv4_merge_kernel<T, D, Sh::W, false>, a, wk,
-                           (const float *)part_o, (const float *)part_lse);
+    const auto merge = parts == 8 ? kv4_merge_kernel<T, D, Sh::W, 8>
+                                  : (parts == 4 ? kv4_merge_kernel<T, D, Sh::W, 4> : kv4_merge_kernel<T, D, Sh::W, 1>);
+    e = cudaLaunchKernelEx(&cfg, merge, a, wk, (const float *)part_o, (const float *)part_lse);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
