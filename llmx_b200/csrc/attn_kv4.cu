@@ -161,7 +161,7 @@ __device__ __forceinline__ void row_range(const AttnArgs &a, int i, int ql, int 
 // begin to the last row's end).
 struct Span {
   int first, steps;
-  int blocks;  // of R pairs
+  int blocks;  // of R pairs (a power of two)
 };
 template <int W>
 __device__ __forceinline__ Span span_of(const AttnArgs &a, int R, int ql, int kl) {
@@ -173,7 +173,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int R, int ql, int kl
     s.first = lo & ~15;
     if (hi > lo) {
       s.steps = (hi - s.first + 16 * W - 1) / (16 * W);
-      s.blocks = (ql * a.group + R - 1) / R;
+      s.blocks = (ql * a.group + R - 1) >> (31 - __clz(R));
     }
   }
   return s;
@@ -190,13 +190,19 @@ struct Work {
 };
 constexpr int kMaxSlice = 512;
 
-// Shares: worker w of `n` has the steps [begin(w), begin(w + 1)) of `total`
-// (below 2^31, which the host sees to).
+// Shares: worker w of `n` (below 2^16) has the steps [begin(w), begin(w + 1)) of
+// `total` (below 2^31, which the host sees to), begin(w) = floor(total w / n)
+// without a 64-bit division.
 __device__ __forceinline__ uint32_t share_begin(uint32_t total, int w, int n) {
-  return (uint32_t)((unsigned long long)total * w / n);
+  const uint32_t each = total / n, rest = total - each * n;
+  return each * w + rest * w / n;
 }
+// The share of a step: an estimate (within one of it, n being small), put right.
 __device__ __forceinline__ int share_of(uint32_t total, uint32_t step, int n) {
-  return (int)((((unsigned long long)step + 1) * n - 1) / total);
+  int w = min(n - 1, (int)__fdividef((float)step * (float)n, (float)total));
+  while (w > 0 && share_begin(total, w, n) > step) --w;
+  while (w < n - 1 && share_begin(total, w + 1, n) <= step) ++w;
+  return w;
 }
 __device__ __forceinline__ int share_count(const Work &wk, uint32_t total) {
   const uint32_t n = max(total / wk.min_steps, min(total, (uint32_t)wk.units));
@@ -1089,8 +1095,9 @@ __global__ void __launch_bounds__(PARTS > 1 ? PARTS * 32 : kThreads) kv4_merge_k
   constexpr int E = D / 32;
   __shared__ float sm_m[PARTS], sm_l[PARTS], sm_o[PARTS][PARTS > 1 ? D : 1];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const long long out_row = PARTS > 1 ? blockIdx.x : (long long)blockIdx.x * kWarps + warp;
-  const int h = (int)(out_row % a.H), i = (int)(out_row / a.H % a.Sq), n = (int)(out_row / a.H / a.Sq), b = wk.b0 + n;
+  const uint32_t out_row = PARTS > 1 ? blockIdx.x : blockIdx.x * kWarps + warp;  // (below 2^31: direct_fits())
+  const uint32_t query = out_row / a.H;
+  const int h = (int)(out_row - query * a.H), n = (int)(query / a.Sq), i = (int)(query - n * a.Sq), b = wk.b0 + n;
   int w0 = 0, used = 0, R = wk.R, r = 0;
   if (n < wk.nb) {
     // Steps before this sequence, and of all.
