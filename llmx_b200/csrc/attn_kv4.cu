@@ -34,20 +34,21 @@
 // the cache's bytes, not the products.
 //
 // Work.  A unit is one (sequence, kv head, block of pairs); its tokens are cut
-// into steps of one or two tiles, and the steps of all units, end to end, are
-// dealt to the resident workers in equal shares: sequences of any lengths
-// finish together.  With more units than resident CTAs a worker is a warp,
-// which copies its tiles into its own ring in shared memory (one bulk copy a
-// tile, issued ahead across unit boundaries); with fewer it is a CTA, whose
-// warps take every fourth step and are merged in shared memory (COOP).  A
-// worker writes the result of a unit that it has whole.  Of a unit that several
-// share each writes a partial result (at most two a worker, so the workspace
-// does not grow with the sequences), and a second kernel merges them.
+// into steps of one or two tiles.  Short units have a worker each.  Of longer
+// ones the steps of all, end to end, are dealt to the resident workers in equal
+// shares: sequences of any lengths finish together.  With many units a worker
+// is a warp, which copies its tiles into its own ring in shared memory (one
+// bulk copy a tile, issued ahead across unit boundaries); with few it is a CTA,
+// whose warps take every fourth step and are merged in shared memory (COOP;
+// plan_kv4() chooses).  A worker writes the result of a unit that it has whole.
+// Of a unit that several share each writes a partial result (at most two a
+// worker, so the workspace does not grow with the sequences), and a second
+// kernel merges them.
 //
 // Measured on one B200 (bytes of the visible cache, q and o): 64 sequences of
-// 256-4096 tokens, 32 heads of 128, ALiBi: 124-130 us, 5.1 TB/s (0.77 of the
+// 256-4096 tokens, 32 heads of 128, ALiBi: 124-134 us, 5.1 TB/s (0.77 of the
 // copy rate); 32 sequences of 1001-8191 tokens, 32 heads on 8: 47 us, 3.6 TB/s;
-// 131071 tokens, 32 heads on 8: 43 us, 3.5 TB/s.  What bounds it is not HBM yet:
+// 131071 tokens, 32 heads on 8: 41 us, 3.7 TB/s.  What bounds it is not HBM yet:
 // at 16 warps an SM (128 registers) the issue slots are 0.6 filled, the unpacking
 // keeps the integer pipe 0.6 busy, and more warps with fewer registers (20 of
 // 96) ran 15-25% slower, fewer with more (12 of 168) 4-8%.
