@@ -1249,15 +1249,20 @@ template <typename T, int D, int NQ, int SLOTS, bool COOP>
 cudaError_t launch_variant(const AttnArgs &a, const Kv4Args &c, const Plan &p, bool split, void *ws, cudaStream_t s) {
   using Sh = Shape<D, NQ, SLOTS, COOP>;
   const int smem = Sh::kSmem + p.nb * 12 + 4;
-  static std::atomic<int> allowed[64];  // of each device: setting it costs a microsecond a launch
+  // The limit on dynamic shared memory is the most that any slice takes, the same
+  // value from every call: host threads that launch at the same time cannot
+  // lower it for one another, in whatever order they come.  Once for each
+  // device, since setting it costs a microsecond a launch.
+  constexpr int most = Sh::kSmem + kMaxSlice * 12 + 4;
+  static std::atomic<bool> allowed[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   // (48 KB without the attribute, the kernel's static part, under 1 KB, among them.)
-  if (smem > 47 * 1024 && (dev < 0 || dev >= 64 || allowed[dev].load() < smem)) {
-    e = cudaFuncSetAttribute(kv4_attn_kernel<T, D, NQ, SLOTS, COOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (most > 47 * 1024 && (dev < 0 || dev >= 64 || !allowed[dev].load())) {
+    e = cudaFuncSetAttribute(kv4_attn_kernel<T, D, NQ, SLOTS, COOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) allowed[dev].store(smem);
+    if (dev >= 0 && dev < 64) allowed[dev].store(true);
   }
   const size_t workers = (size_t)p.ctas * (COOP ? 1 : kWarps);
   float *part_o = static_cast<float *>(ws);

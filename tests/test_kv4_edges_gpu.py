@@ -1,0 +1,135 @@
+"""The 4-bit key/value cache on the GPU at its edges: host threads at once,
+empty sequences, numbers at the ends of their types, tokens that a row must not
+see, sizes near 31 bits, workspaces that are missing."""
+import ctypes
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+import llmx_b200
+from gpu_helpers import needs_cuda
+from llmx_b200 import _lib, kv4
+from oracle import kv4 as okv4
+
+pytestmark = [pytest.mark.gpu, needs_cuda]
+
+DEV = "cuda"
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+# Host threads that call the C entry at the same moment, step by step; each has
+# its own requests (of growing batches), stream and results.
+GATE_C = r"""
+#include <pthread.h>
+#include <stdatomic.h>
+#include <stddef.h>
+#include "llmx_attn.h"
+struct job { const llmx_attn_params *p; const llmx_kv4_cache *c; void *stream; int n, threads; int *status; atomic_int *gate; };
+static void *work(void *arg) {
+  struct job *j = arg;
+  for (int i = 0; i < j->n; ++i) {
+    atomic_fetch_add(j->gate, 1);
+    while (atomic_load(j->gate) < j->threads * (i + 1)) {}
+    j->status[i] = llmx_kv4_attn_fwd(j->p + i, j->c + i, j->stream);
+  }
+  return NULL;
+}
+int run(int threads, int n, const llmx_attn_params **p, const llmx_kv4_cache **c, void **streams, int *status) {
+  pthread_t t[16];
+  struct job j[16];
+  atomic_int gate = 0;
+  for (int i = 0; i < threads; ++i) {
+    j[i] = (struct job){p[i], c[i], streams[i], n, threads, status + i * n, &gate};
+    if (pthread_create(&t[i], NULL, work, &j[i]) != 0) return 1;
+  }
+  for (int i = 0; i < threads; ++i) pthread_join(t[i], NULL);
+  return 0;
+}
+"""
+THREADS = r"""
+import ctypes, sys
+import torch
+from llmx_b200 import _lib, kv4
+
+lib, gate = _lib.load(), ctypes.CDLL(sys.argv[1])
+THREADS, failed = 4, []
+for dtype in (torch.bfloat16, torch.float16):
+    for d, heads, most in ((256, 1, 440), (256, 9, 440), (128, 1, 440), (128, 4, 440), (128, 8, 512), (64, 2, 512)):
+        cache = torch.zeros(most, 1, 1, 18 * d, dtype=torch.uint8, device="cuda")
+        n, keep, streams = most // THREADS, [], [torch.cuda.Stream() for _ in range(THREADS)]
+        ps, cs = [(_lib.AttnParams * n)() for _ in range(THREADS)], [(_lib.Kv4Cache * n)() for _ in range(THREADS)]
+        for t in range(THREADS):
+            q = torch.zeros(most, 1, heads, d, dtype=dtype, device="cuda")
+            out = torch.empty_like(q)
+            keep += [q, out]
+            for i in range(n):
+                b, p, c = THREADS * i + t + 1, ps[t][i], kv4._cache_arg(cache, THREADS * i + t + 1, dtype, d, None, keep)
+                c.max_pages = 1
+                cs[t][i] = c
+                lib.llmx_attn_params_init(ctypes.byref(p))
+                p.dtype, p.batch, p.n_heads, p.n_kv_heads, p.head_dim, p.max_q_len, p.max_kv_len = c.dtype, b, heads, 1, d, 1, 16
+                p.q, p.o, p.sm_scale = q.data_ptr(), out.data_ptr(), 1.0
+                lib.llmx_attn_set_contiguous_strides(ctypes.byref(p))
+        torch.cuda.synchronize()
+        status = (ctypes.c_int * (n * THREADS))()
+        ptrs = lambda xs: (ctypes.c_void_p * THREADS)(*xs)
+        assert gate.run(THREADS, n, ptrs(map(ctypes.addressof, ps)), ptrs(map(ctypes.addressof, cs)),
+                        ptrs(s.cuda_stream for s in streams), status) == 0
+        torch.cuda.synchronize()
+        failed += [(str(dtype), d, heads, i) for i, s in enumerate(status) if s != 0]
+print("failed", len(failed), failed[:5], lib.llmx_attn_last_error())
+sys.exit(1 if failed else 0)
+"""
+
+
+def test_host_threads_with_different_batches(tmp_path):
+    """A fresh process: each kernel's shared-memory limit is set by its first calls."""
+    src, so = tmp_path / "gate.c", tmp_path / "gate.so"
+    src.write_text(GATE_C)
+    lib = os.path.join(ROOT, "llmx_b200")
+    subprocess.run(["gcc", "-O2", "-shared", "-fPIC", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(so), "-L", lib,
+                    "-lllmx_attn", "-Wl,-rpath," + lib, "-lpthread"], check=True)
+    r = subprocess.run([sys.executable, "-c", THREADS, str(so)], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr[-2000:]
+
+
+def request(cache, table, q, out, lens, *, scale, algo="auto", lse=None, slopes=None, max_kv_len=0):
+    """(params, cache, what they point to) of a call of the C entry; the caller sets the workspace."""
+    lib, keep = _lib.load(), [q, out, lens, table, lse, slopes]
+    B, sq, H, d = q.shape
+    c = kv4._cache_arg(cache, B, q.dtype, d, table, keep)
+    p = _lib.AttnParams()
+    lib.llmx_attn_params_init(ctypes.byref(p))
+    p.dtype, p.batch, p.n_heads, p.n_kv_heads, p.head_dim, p.max_q_len = c.dtype, B, H, c.n_kv_heads, d, sq
+    p.max_kv_len = max_kv_len or c.max_pages * c.page_size
+    p.q, p.o, p.kv_lens, p.sm_scale, p.algo = q.data_ptr(), out.data_ptr(), lens.data_ptr(), scale, _lib.ALGO[algo]
+    p.lse = None if lse is None else lse.data_ptr()
+    p.alibi_slopes = None if slopes is None else slopes.data_ptr()
+    lib.llmx_attn_set_contiguous_strides(ctypes.byref(p))
+    return p, c, keep
+
+
+def stored(k, v, page=64):
+    """A cache without a table that holds k, v [B, S, Hkv, D]."""
+    B, S, hkv, d = k.shape
+    cache = llmx_b200.kv4_empty(B * -(-S // page), hkv, d, page, device=DEV)
+    cache.fill_(255)
+    llmx_b200.kv4_store(cache, k.to(DEV), v.to(DEV))
+    return cache
+
+
+def check(out, lse, q, k, v, kv_len, dtype, *, sm_scale, slopes=None, causal=True, window=-1, what=""):
+    """One sequence, element by element, to the oracle's bound and half a step of the output's type."""
+    o, le, bound, le_bound = okv4.attention(q, k, v, q.shape[0], kv_len, sm_scale=sm_scale, slopes=slopes, causal=causal,
+                                            window=window)
+    half = torch.finfo(dtype).eps / 2
+    room = bound * (1 + 2 ** -10) + (o.abs() + bound) * half + torch.finfo(dtype).smallest_normal * half
+    off = (out.double().cpu() - o).abs()
+    assert (off <= room).all(), f"{what}: worst {float((off / room).nan_to_num(1e9).max()):.3g} of the bound"
+    if lse is not None:
+        off = (lse.double().cpu() - le).abs()
+        seen = le != -math.inf
+        assert (off <= le_bound)[seen].all(), f"{what}: lse, worst {float((off / le_bound)[seen].nan_to_num(1e9).max()):.3g} of the bound"
