@@ -234,7 +234,9 @@ __device__ __forceinline__ TileAt tile_at(const Kv4Args &a, const RowArgs &r) {
   const long long tile = (start >> 4) + idx / (uint32_t)a.Hkv;
   t.row0 = tile * 16 - start;
   t.tile = nullptr;
-  if (t.row0 < t.len) {
+  // A row of the call lies in the tile.  (Without one, which a first tile that
+  // begins before row 0 can be, the table holds nothing for it.)
+  if (t.len > 0 && t.row0 < t.len) {
     const long long pos = tile * 16;
     if (pos >= 0 && pos < (long long)a.max_pages * a.page_size) {
       const int p = (int)pos / a.page_size, in = (int)pos - p * a.page_size;

@@ -133,3 +133,22 @@ def check(out, lse, q, k, v, kv_len, dtype, *, sm_scale, slopes=None, causal=Tru
         off = (lse.double().cpu() - le).abs()
         seen = le != -math.inf
         assert (off <= le_bound)[seen].all(), f"{what}: lse, worst {float((off / le_bound)[seen].nan_to_num(1e9).max()):.3g} of the bound"
+
+
+@pytest.mark.parametrize("start", [5, 63, 10 ** 6 + 3])
+def test_an_empty_sequence_reads_no_page(start):
+    """Rows enough for a tile a warp; the first sequence has none of them, and nothing valid in its table."""
+    dtype, d, hkv, S = torch.bfloat16, 128, 16, 600
+    gen = torch.Generator().manual_seed(start)
+    k, v = (torch.randn(2, S, hkv, d, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    table = torch.tensor([[-1] * 10, list(range(10))], dtype=torch.int32, device=DEV)
+    cache = llmx_b200.kv4_empty(10, hkv, d, 64, device=DEV)
+    kw = dict(start=torch.tensor([start, 0], device=DEV), lens=torch.tensor([0, S], device=DEV), block_table=table)
+    llmx_b200.device_status(0)
+    llmx_b200.kv4_store(cache, k, v, **kw)
+    llmx_b200.device_status(0)
+    ko, vo = torch.full_like(k, 9.0), torch.full_like(v, 9.0)
+    llmx_b200.kv4_load(cache, ko, vo, **kw)
+    llmx_b200.device_status(0)
+    assert (ko[0] == 0).all() and (vo[0] == 0).all()
+    assert torch.equal(ko[1].cpu(), okv4.values(k[1].cpu())[1]) and torch.equal(vo[1].cpu(), okv4.values(v[1].cpu())[1])
