@@ -518,7 +518,7 @@ RowArgs row_args(const llmx_kv4_rows &r, int pad, bool *vec) {
 template <typename T, int D, bool VEC>
 cudaError_t launch_rows_v(bool store, const Kv4Args &k, const RowArgs &r, cudaStream_t s) {
   // A warp for each tile that a sequence's rows can touch, heads fastest.
-  const long long tiles = ((long long)(r.S + 14) / 16 + 1) * k.Hkv;
+  const long long tiles = (((long long)r.S + 14) / 16 + 1) * k.Hkv;
   if (r.S >= kKv4TileTokens && tiles * r.B >= kManyTiles) {
     const dim3 grid((unsigned)((tiles + kRowThreads / 32 - 1) / (kRowThreads / 32)), (unsigned)r.B);
     if (store) kv4_store_kernel<T, D, VEC><<<grid, kRowThreads, 0, s>>>(k, r);

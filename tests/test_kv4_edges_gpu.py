@@ -152,3 +152,20 @@ def test_an_empty_sequence_reads_no_page(start):
     llmx_b200.device_status(0)
     assert (ko[0] == 0).all() and (vo[0] == 0).all()
     assert torch.equal(ko[1].cpu(), okv4.values(k[1].cpu())[1]) and torch.equal(vo[1].cpu(), okv4.values(v[1].cpu())[1])
+
+
+def test_a_row_count_near_31_bits():
+    """max_rows as the largest integer, over rows of stride 0, with a length of a few."""
+    dtype, d, hkv = torch.float16, 256, 15
+    gen = torch.Generator().manual_seed(7)
+    x = torch.randn(1, 1, hkv, d, generator=gen).to(dtype)
+    cache = llmx_b200.kv4_empty(1, hkv, d, 16, device=DEV)
+    cache.fill_(255)
+    wide = x.to(DEV).expand(1, 2 ** 31 - 1, hkv, d)
+    llmx_b200.kv4_store(cache, wide, wide, lens=torch.tensor([3], device=DEV, dtype=torch.int32))
+    want = torch.full((hkv, 18 * d), 255, dtype=torch.uint8)
+    for h in range(hkv):
+        for tok in range(3):
+            okv4.write_token(want[h], tok, x[0, 0, h], x[0, 0, h])
+    assert torch.equal(cache[0, :, 0].cpu(), want)
+    llmx_b200.device_status(0)
