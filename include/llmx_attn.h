@@ -255,9 +255,10 @@ LLMX_API llmx_status llmx_convert(const void *src, int32_t src_dtype, void *dst,
  * no cache).  K and V (fp16 / bf16, head_dim 64, 128 or 256) are quantised
  * in groups of LLMX_KV4_GROUP channels of one (token, kv head), each with a
  * step s and a minimum m held in the type T of K and V:
- *   m = min x,  r = fl32(fl32(max x - m) / 15),  s = the smallest T >= r,
+ *   m = min x,  r = fl32(fl32(max x - m) / 15),  s = the smallest T >= r
+ *   (the next one below where 15 s + m would round to infinity in T),
  *   n = min(15, rint(fl32(fl32(x - m) / s)))  (0 where s = 0),
- *   value = n s + m.
+ *   value = n s + m, within s / 2 of x; finite x read back finite.
  * A group with a NaN or an infinity in it (or, for bf16, a range max x - m
  * past fp32) has s = NaN and reads back as NaN.  4.5 bits a value: 18 * head_dim bytes per
  * 16 tokens of K and V of one kv head.

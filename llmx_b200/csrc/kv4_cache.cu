@@ -104,10 +104,19 @@ template <typename T>
 __device__ __forceinline__ uint32_t param_of(uint32_t low_neg_high) {
   const uint32_t hi_bits = (low_neg_high >> 16) ^ 0x8000u;
   const unsigned short lo16 = (unsigned short)low_neg_high, hi16 = (unsigned short)hi_bits;
-  const float range = Elem<T>::to_f(*reinterpret_cast<const T *>(&hi16)) - Elem<T>::to_f(*reinterpret_cast<const T *>(&lo16));
+  const float lo = Elem<T>::to_f(*reinterpret_cast<const T *>(&lo16));
+  const float range = Elem<T>::to_f(*reinterpret_cast<const T *>(&hi16)) - lo;
   // A range that is not finite gives a step that is a NaN.
   const T st = round_up_to<T>(range < CUDART_INF_F ? __fdiv_rn(range, 15.f) : CUDART_NAN_F);
-  return (uint32_t) * reinterpret_cast<const unsigned short *>(&st) | ((uint32_t)lo16 << 16);
+  unsigned short s16 = *reinterpret_cast<const unsigned short *>(&st);
+  // At the end of the type 15 s + m, which passes the maximum by up to 15 of s's
+  // last bits, would round to infinity (from the largest number and half its last
+  // bit on).  The next s below is under range / 15, so 15 s + m then is not past
+  // the maximum, which stays within half a step: 15 last bits of s are at most
+  // 15 2^-7 s, and the quotients below 15.5.
+  constexpr float kInfinite = std::is_same<T, __half>::value ? 65520.f : 0x1.ffp127f;
+  if (fmaf(15.f, Elem<T>::to_f(st), lo) >= kInfinite) --s16;
+  return (uint32_t)s16 | ((uint32_t)lo16 << 16);
 }
 // 1 / s, 0 for s = 0, or -1 where codes_any() has to divide: between these
 // bounds neither the reciprocal nor the products in codes()

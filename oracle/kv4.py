@@ -23,6 +23,9 @@ def quantise(x: torch.Tensor):
     s = r.to(x.dtype)
     bumped = (s.view(torch.int16) + 1).view(x.dtype)
     s = torch.where(s.float() < r, bumped, s)
+    # At the end of the type: the next s below where 15 s + m would round to infinity.
+    past = (15.0 * s.double() + m.double()).float().to(x.dtype).isinf() & r.isfinite()
+    s = torch.where(past, (s.view(torch.int16) - 1).view(x.dtype), s)
     s = torch.where(r.isfinite(), s, torch.full_like(s, float("nan")))
     diff = (y.double() - m.double()[..., None]).float().double()
     q = (diff / s.double()[..., None]).float()

@@ -154,6 +154,36 @@ def test_an_empty_sequence_reads_no_page(start):
     assert torch.equal(ko[1].cpu(), okv4.values(k[1].cpu())[1]) and torch.equal(vo[1].cpu(), okv4.values(v[1].cpu())[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,hkv,S", [(64, 1, 5), (128, 24, 700), (256, 2, 40)])
+def test_finite_values_at_the_ends_of_the_type(dtype, d, hkv, S):
+    """Groups that reach the type's largest numbers read back finite, each value within half a step."""
+    top = torch.finfo(dtype).max
+    gen = torch.Generator().manual_seed(d)
+    x = (torch.rand(1, S, hkv, d, generator=gen, dtype=torch.float64) * top).to(dtype)
+    x[..., 0], x[..., 1] = 0.0, top
+    x[:, 1::4] = -x[:, 1::4]
+    if dtype == torch.float16:  # (for bf16 this range passes fp32)
+        x[:, 2::4, :, 0] = -top
+    x[:, 3::4, :, 0] = 0.01 * top
+    cache = stored(x, x)
+    n, s, m = okv4.quantise(x)
+    ko, vo = torch.empty_like(x, device=DEV), torch.empty_like(x, device=DEV)
+    llmx_b200.kv4_load(cache, ko, vo)
+    want = okv4.values(x)[1]
+    assert want.isfinite().all() and torch.equal(ko.cpu(), want) and torch.equal(vo.cpu(), want)
+    # Half a step, fp32's rounding of the difference, and the read-back's own rounding.
+    room = okv4.spread(s) * 0.5 * (1 + 2.0 ** -20) + want.double().abs() * torch.finfo(dtype).eps
+    assert ((ko.double().cpu() - x.double()).abs() <= room).all()
+    # A row that sees one token gets its values.
+    for b in range(4):
+        q = torch.zeros(1, 1, hkv, d, dtype=dtype, device=DEV)
+        out = torch.empty_like(q)
+        one = torch.zeros(1, 1, hkv, d, dtype=dtype)
+        llmx_b200.kv4_attention(out, q, stored(one, x[:, b:b + 1]), 1.0, max_kv_len=1)
+        check(out[0], None, q[0].cpu(), one[0], x[0, b:b + 1], 1, dtype, sm_scale=1.0, what=f"token {b}")
+
+
 def test_a_row_count_near_31_bits():
     """max_rows as the largest integer, over rows of stride 0, with a length of a few."""
     dtype, d, hkv = torch.float16, 256, 15
