@@ -149,6 +149,7 @@ llmx_status validate(const llmx_attn_params *p, AttnArgs *a) {
   a->err = nullptr;
   a->num_sms = 148;
   a->xs_n = a->xs_slice = a->xs_row_base = 0;
+  a->expanded = 0;
   for (int i = 0; i < LLMX_SCATTER_MAX_DST; ++i) {
     a->xs_o[i] = nullptr;
     a->xs_lse[i] = nullptr;

@@ -40,6 +40,9 @@ struct AttnArgs {
   int xs_n, xs_slice, xs_row_base;
   void *xs_o[LLMX_SCATTER_MAX_DST];
   float *xs_lse[LLMX_SCATTER_MAX_DST];
+  // The prefill of a 4-bit cache's expanded form: rows that a NaN or an infinity
+  // reaches are NaN, not 0.
+  int expanded;
 };
 
 // Split-KV decode plan: how many splits of how many keys.

@@ -1474,6 +1474,7 @@ extern "C" llmx_status llmx_kv4_attn_fwd(const llmx_attn_params *p, const llmx_k
     // The prefill reads whole blocks of 128 keys: what a block holds behind a
     // sequence is multiplied by 0 and so has to be finite.
     cudaError_t err = launch_kv4_load(k, r, a.dtype, 128, st);
+    e.expanded = 1;
     if (err == cudaSuccess) err = launch_sm100(e, ws + 2 * rows, kSm100WorkspaceBytes, st);
     if (err != cudaSuccess)
       return record_error(LLMX_ERR_CUDA, (std::string("launch failed: ") + cudaGetErrorString(err)).c_str());

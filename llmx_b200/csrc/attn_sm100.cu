@@ -720,6 +720,14 @@ __device__ __forceinline__ void transpose_units4(uint4 (&u)[4]) {
   }
 }
 
+// Whether a row's output is O / l, not 0.  In the expanded form every row that
+// sees a key (of an item that has blocks: one not above the keys' begin) is one:
+// its l is 0 or a NaN where an infinity or NaN made its scores so, and O / l
+// then is a NaN.
+__device__ __forceinline__ bool row_valid(const AttnArgs &a, bool have, int qi, int ql, int kl, float l) {
+  return qi < ql && (l > 0.f || (a.expanded != 0 && have && (!a.causal || qi + diag_shift(a, ql, kl) >= 0)));
+}
+
 // ------------------------------------------------------------ softmax role
 // One work item.  Thread r of warpgroup t owns query row r of tile t (TMEM
 // lane r).  blk_base: key blocks of earlier items (barrier phases).  Returns
@@ -817,7 +825,7 @@ __device__ bool softmax_tile(const AttnArgs &a, Bars *bars, uint32_t tmem, int w
     }
   }
   const bool have = !aborted && br.nb > 0;
-  const bool valid = qi < ql && l > 0.f;  // padded rows and rows with no visible key -> 0
+  const bool valid = row_valid(a, have, qi, ql, kl, l);  // padded rows and rows with no visible key -> 0
   const float inv = valid ? 1.f / l : 0.f;
   // Each group of four lanes (four consecutive rows) swaps 16-byte pieces so
   // that every store instruction writes 64 contiguous bytes of 8 rows.
@@ -876,7 +884,7 @@ __device__ bool softmax_tile(const AttnArgs &a, Bars *bars, uint32_t tmem, int w
       if (a.lse != nullptr) a.lse[((long long)b * a.H + h) * a.Sq + row] = kNegInf;
     }
   }
-  const float lse_v = valid ? (m_used + log2f(l)) * kLn2 : kNegInf;
+  const float lse_v = valid ? (l > 0.f ? (m_used + log2f(l)) * kLn2 : CUDART_NAN_F) : kNegInf;
   if (a.xs_n > 0) {
     if (qi < a.Sq) {
       const int rr = a.xs_row_base + qi;
@@ -1307,7 +1315,7 @@ __device__ bool softmax_256(const AttnArgs &a, Bars256 *bars, uint32_t tmem, int
     }
   }
   const bool have = !aborted && br.nb > 0;
-  const bool valid = qi < ql && l > 0.f;
+  const bool valid = row_valid(a, have, qi, ql, kl, l);
   const float inv = valid ? 1.f / l : 0.f;
   const int gi = threadIdx.x & 3;
   const int qi_group = qi - gi;
@@ -1347,7 +1355,7 @@ __device__ bool softmax_256(const AttnArgs &a, Bars256 *bars, uint32_t tmem, int
     }
   }
   if (a.lse != nullptr && qi < a.Sq)
-    a.lse[((long long)b * a.H + h) * a.Sq + qi] = valid ? (m_used + log2f(l)) * kLn2 : kNegInf;
+    a.lse[((long long)b * a.H + h) * a.Sq + qi] = valid ? (l > 0.f ? (m_used + log2f(l)) * kLn2 : CUDART_NAN_F) : kNegInf;
   return !aborted;
 }
 

@@ -184,6 +184,33 @@ def test_finite_values_at_the_ends_of_the_type(dtype, d, hkv, S):
         check(out[0], None, q[0].cpu(), one[0], x[0, b:b + 1], 1, dtype, sm_scale=1.0, what=f"token {b}")
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,H,hkv,sq,n", [(128, 8, 2, 160, 400), (64, 4, 4, 200, 200), (256, 3, 1, 140, 130)])
+def test_infinities_and_nan_in_q_make_their_rows_nan(dtype, d, H, hkv, sq, n):
+    """Both forms; rows above the keys' begin stay 0, also with such a q.  (The first rows see few keys: all scores -inf is one outcome.)"""
+    gen = torch.Generator().manual_seed(n)
+    k, v = (torch.randn(1, n, hkv, d, generator=gen).to(dtype) for _ in range(2))
+    q = torch.randn(1, sq, H, d, generator=gen).to(dtype)
+    bad = torch.zeros(sq, H, dtype=torch.bool)
+    bad[torch.randperm(sq, generator=gen)[:40], torch.randint(0, H, (40,), generator=gen)] = True
+    bad[max(0, sq - n):max(0, sq - n) + 4] = True
+    for i, h in bad.nonzero().tolist():
+        q[0, i, h, (7 * i + h) % d] = [math.inf, -math.inf, math.nan][(i + h) % 3]
+    cache = stored(k, v)
+    only_nan = torch.where(q.isinf(), torch.full_like(q, math.nan), q)  # (a soft-cap makes finite scores of infinite ones)
+    for opts in (dict(), dict(sliding_window=20), dict(causal=False), dict(logits_soft_cap=4.0), dict(alibi_slopes=torch.rand(H, device=DEV))):
+        qd = (only_nan if "logits_soft_cap" in opts else q).to(DEV)
+        seen = (torch.arange(sq) + n - sq >= 0) | (not opts.get("causal", True))
+        for algo in ("decode", "tcgen05"):
+            out, lse = torch.full_like(q, 7.0, device=DEV), torch.zeros(1, H, sq, device=DEV)
+            llmx_b200.kv4_attention(out, qd, cache, d ** -0.5, max_kv_len=n, lse=lse, algo=algo, **opts)
+            o, nan, what = out[0].cpu(), bad & seen[:, None], f"{algo} {opts}"
+            assert torch.equal(o.isnan(), nan[..., None].expand_as(o)), what
+            assert torch.equal(lse[0].cpu().isnan(), nan.T), what
+            assert (o[~seen] == 0).all() and (lse[0].cpu()[:, ~seen] == -math.inf).all(), what
+    llmx_b200.device_status(0)
+
+
 def test_a_row_count_near_31_bits():
     """max_rows as the largest integer, over rows of stride 0, with a length of a few."""
     dtype, d, hkv = torch.float16, 256, 15
