@@ -342,9 +342,10 @@ LLMX_API llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_rows 
  *           expected to be faster and takes at most 4 GiB.
  * A call on the DECODE path given too little workspace runs without
  * splitting a sequence's keys.  Calls that share a workspace must not overlap
- * on the GPU.  An infinity or NaN in q or in a K that a row sees makes
- * the row NaN (TCGEN05 with a soft-cap takes the infinite scores of q as +- the
- * cap). A row's p s keeps
+ * on the GPU.  A NaN reaches the rows that see it and no others: one in K makes
+ * the row NaN, one in V the channels of its group (TCGEN05: the row and its lse
+ * as well), and an infinity or NaN in q its row (TCGEN05 with a soft-cap takes
+ * the infinite scores as +- the cap).  A row's p s keeps
  * 11 bits down to 2^-21 of its largest, by the largest p and the largest V step
  * that the row sees; a bf16 K is taken up to 2^96 in size. */
 LLMX_API llmx_status llmx_kv4_attn_workspace_size(const llmx_attn_params *p, const llmx_kv4_cache *c, size_t *bytes);

@@ -21,9 +21,13 @@ struct Kv4Args {
 llmx_status prepare_kv4(const llmx_kv4_cache *c, const llmx_kv4_rows &rows, Kv4Args *k);
 // The checks alone, without a device.
 llmx_status validate_kv4(const llmx_kv4_cache *c, int batch, Kv4Args *k);
-// The rows' kernels without their checks, for the attention's expanded form:
-// rows [lens[b], lens[b] rounded up to `pad`) are written as 0 and the ones
-// behind them are left alone (pad 0: all of them are written as 0).
+// The load without its checks, for the attention's expanded form: rows
+// [lens[b], lens[b] rounded up to `pad`) are written as 0 and the ones behind
+// them are left alone (pad 0: all of them are written as 0).  With a pad a V
+// group that holds a NaN is written as 0, and K's group of its token as NaN: the
+// prefill multiplies V by weights that are 0 for the rows that do not see the
+// token, and 0 times NaN would reach them; a score is of one token alone, and
+// masked ones are replaced.
 cudaError_t launch_kv4_load(const Kv4Args &k, const llmx_kv4_rows &r, int dtype, int pad, cudaStream_t s);
 
 constexpr int kKv4Group = LLMX_KV4_GROUP;
@@ -68,6 +72,12 @@ __device__ __forceinline__ float2 kv4_unpack_param(uint32_t w) {
   } else {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
+}
+
+// Whether the group of a parameter word reads back as NaN.
+template <typename T>
+__device__ __forceinline__ bool kv4_nan_step(uint32_t w) {
+  return (w & 0x7fffu) > (std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);
 }
 
 }  // namespace llmx_b200

@@ -379,7 +379,11 @@ __global__ void __launch_bounds__(kRowThreads) kv4_load_kernel(const __grid_cons
       const uint32_t w0 = kw[(i * G + h) * 2], w1 = kw[(i * G + h) * 2 + 1];
       const uint32_t other = __shfl_xor_sync(0xffffffffu, t & 1 ? w0 : w1, 1);
       const uint32_t word[2] = {t & 1 ? other : w0, t & 1 ? w1 : other};
-      const uint32_t param = held ? *reinterpret_cast<const uint32_t *>(par + (tok * 2 * G + h) * 4) : 0u;
+      uint32_t param = held ? *reinterpret_cast<const uint32_t *>(par + (tok * 2 * G + h) * 4) : 0u;
+      if (r.pad > 0 && held) {
+        const uint32_t of_v = *reinterpret_cast<const uint32_t *>(par + (tok * 2 * G + G + h) * 4);
+        if (kv4_nan_step<T>(of_v)) param = of_v;
+      }
       if (wanted) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -398,7 +402,8 @@ __global__ void __launch_bounds__(kRowThreads) kv4_load_kernel(const __grid_cons
     T *p = v + (at.row0 + tok) * r.vs[1] + 8 * g;
 #pragma unroll
     for (int h = 0; h < G; ++h) {
-      const uint32_t param = held ? *reinterpret_cast<const uint32_t *>(par + (tok * 2 * G + G + h) * 4) : 0u;
+      uint32_t param = held ? *reinterpret_cast<const uint32_t *>(par + (tok * 2 * G + G + h) * 4) : 0u;
+      if (r.pad > 0 && kv4_nan_step<T>(param)) param = 0u;
       if (wanted) {
         float f[8] = {};
         if (held) dequantise8<T>(vw[i * G + h], param, f);
@@ -476,8 +481,12 @@ __global__ void __launch_bounds__(kRowThreads) kv4_load_few_kernel(const __grid_
   if (at.tile != nullptr) {
     const uint32_t kc = *reinterpret_cast<const uint32_t *>(at.tile + kv4_k_word(at.tok, at.c, G));
     const uint32_t vc = *reinterpret_cast<const uint32_t *>(at.tile + kv4_v_word(at.tok, at.c, G));
-    const uint32_t kp = *reinterpret_cast<const uint32_t *>(at.tile + kv4_param(at.tok, 0, at.c >> 3, G));
-    const uint32_t vp = *reinterpret_cast<const uint32_t *>(at.tile + kv4_param(at.tok, 1, at.c >> 3, G));
+    uint32_t kp = *reinterpret_cast<const uint32_t *>(at.tile + kv4_param(at.tok, 0, at.c >> 3, G));
+    uint32_t vp = *reinterpret_cast<const uint32_t *>(at.tile + kv4_param(at.tok, 1, at.c >> 3, G));
+    if (r.pad > 0 && kv4_nan_step<T>(vp)) {
+      kp = vp;
+      vp = 0u;
+    }
     dequantise8<T>(kc, kp, kf);
     dequantise8<T>(vc, vp, vf);
   }

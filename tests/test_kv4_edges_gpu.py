@@ -185,6 +185,63 @@ def test_finite_values_at_the_ends_of_the_type(dtype, d, hkv, S):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,H,hkv,sq,lens", [(128, 8, 2, 160, [900, 400]), (64, 4, 4, 200, [513, 200]), (256, 3, 1, 140, [700, 140])])
+def test_nan_tokens_reach_only_the_rows_that_see_them(dtype, d, H, hkv, sq, lens):
+    """A NaN in K makes the rows that see the token NaN, one in V their channels of its group (expanded: the whole rows)."""
+    import oracle
+
+    gen = torch.Generator().manual_seed(sq)
+    B, S, page = len(lens), max(lens), 64
+    k, v = (torch.randn(B, S, hkv, d, generator=gen).to(dtype) for _ in range(2))
+    q = torch.randn(B, sq, H, d, generator=gen).to(dtype)
+    bad_v = [(0, lens[0] - 3, 0, d - 1), (0, lens[0] - sq // 2, hkv - 1, 5), (0, 11, hkv - 1, 3), (1, lens[1] - 40, 0, 7),
+             (1, lens[1] - 41, hkv - 1, d - 2), (1, lens[1] - 1, 0, 0)]
+    bad_k = [(0, lens[0] - 20, 0), (1, lens[1] - 30, hkv - 1)]
+    kx, vx = k.clone(), v.clone()
+    for b, j, h, c in bad_v:
+        vx[b, j, h, c] = math.nan
+        v[b, j, h, c // 64 * 64:c // 64 * 64 + 64] = 0.0  # what the others of the reference see
+    for b, j, h in bad_k:
+        kx[b, j, h, 1] = math.inf
+        k[b, j, h] = 0.0
+    cache = stored(kx, vx, page)
+    slopes = torch.pow(2.0, -8.0 * torch.arange(1, H + 1) / H).float()
+    kv = torch.tensor(lens, device=DEV, dtype=torch.int32)
+    kd, vd = okv4.values(k)[1].float(), okv4.values(v)[1].float()
+    for opts in (dict(), dict(window=25), dict(causal=False, window=30), dict(alibi=slopes), dict(cap=5.0)):
+        causal, window = opts.get("causal", True), opts.get("window", -1)
+        ref = oracle.attention_ref_padded(q.float(), kd, vd, kv_lens=lens, sm_scale=d ** -0.5, causal=causal,
+                                          **({"sliding_window": window} if window >= 0 else {}),
+                                          **({"alibi": slopes} if "alibi" in opts else {}),
+                                          **({"logits_soft_cap": 5.0} if "cap" in opts else {}))
+        nan, nan_lse = torch.zeros(B, sq, H, d, dtype=torch.bool), torch.zeros(B, H, sq, dtype=torch.bool)
+        group = H // hkv
+
+        def rows_that_see(b, j):
+            diag = torch.arange(sq) + lens[b] - sq
+            return ((j <= diag) | (not causal)) & ((diag - j <= window) | (window < 0))
+
+        for b, j, h, c in bad_v:
+            nan[b, rows_that_see(b, j), h * group:(h + 1) * group, c // 64 * 64:c // 64 * 64 + 64] = True
+        for b, j, h in bad_k:
+            nan[b, rows_that_see(b, j), h * group:(h + 1) * group] = True
+            nan_lse[b, h * group:(h + 1) * group, rows_that_see(b, j)] = True
+        for algo in ("decode", "tcgen05"):
+            out, lse = torch.full_like(q, 7.0, device=DEV), torch.zeros(B, H, sq, device=DEV)
+            llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, window, opts.get("cap", 0.0), kv_lens=kv, causal=causal,
+                                    alibi_slopes=slopes.to(DEV) if "alibi" in opts else None, lse=lse, algo=algo)
+            what, want = f"{algo} {opts}", nan
+            if algo == "tcgen05":
+                want = nan.any(-1, keepdim=True).expand_as(nan)
+                nan_lse = want[..., 0].transpose(1, 2)
+            assert torch.equal(lse.cpu().isnan(), nan_lse), what
+            assert torch.equal(out.cpu().isnan(), want), f"{what}: {int((out.cpu().isnan() != want).sum())} differ"
+            err = (out.float().cpu() - ref).abs()[~want]
+            assert err.numel() == 0 or err.max() <= 2e-2, f"{what}: {float(err.max())}"
+    llmx_b200.device_status(0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("d,H,hkv,sq,n", [(128, 8, 2, 160, 400), (64, 4, 4, 200, 200), (256, 3, 1, 140, 130)])
 def test_infinities_and_nan_in_q_make_their_rows_nan(dtype, d, H, hkv, sq, n):
     """Both forms; rows above the keys' begin stay 0, also with such a q.  (The first rows see few keys: all scores -inf is one outcome.)"""
@@ -209,6 +266,21 @@ def test_infinities_and_nan_in_q_make_their_rows_nan(dtype, d, H, hkv, sq, n):
             assert torch.equal(lse[0].cpu().isnan(), nan.T), what
             assert (o[~seen] == 0).all() and (lse[0].cpu()[:, ~seen] == -math.inf).all(), what
     llmx_b200.device_status(0)
+
+
+def test_a_cache_full_of_nan():
+    """Every V group NaN: all rows that see a key are NaN, rows without one are 0."""
+    dtype, d, H, hkv, sq = torch.bfloat16, 128, 4, 2, 300
+    cache = llmx_b200.kv4_empty(2 * 8, hkv, d, 64, device=DEV)
+    x = torch.full((2, 512, hkv, d), math.nan, dtype=dtype, device=DEV)
+    llmx_b200.kv4_store(cache, torch.zeros_like(x), x)
+    q = torch.randn(2, sq, H, d, device=DEV, dtype=dtype)
+    for algo in ("decode", "tcgen05"):
+        out = torch.full_like(q, 7.0)
+        llmx_b200.kv4_attention(out, q, cache, 0.1, kv_lens=torch.tensor([500, 100], device=DEV), algo=algo)
+        seen = torch.ones(2, sq, dtype=torch.bool)
+        seen[1, :200] = False
+        assert torch.equal(out.isnan().all(-1).all(-1).cpu(), seen) and (out[~seen.to(DEV)] == 0).all(), algo
 
 
 def test_a_row_count_near_31_bits():
