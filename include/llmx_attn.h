@@ -339,7 +339,8 @@ LLMX_API llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_rows 
  *   TCGEN05 expands the sequences into the workspace (values rounded to T)
  *           and runs the tensor-core prefill on them; needs its workspace.
  *   AUTO    DECODE, or for long query blocks TCGEN05 where it can run, is
- *           expected to be faster and takes at most 4 GiB.
+ *           expected to be faster, takes at most 4 GiB and has its workspace
+ *           (without it, TCGEN05 where DECODE cannot count the rows: an error).
  * A call on the DECODE path given too little workspace runs without
  * splitting a sequence's keys.  Calls that share a workspace must not overlap
  * on the GPU.  A NaN reaches the rows that see it and no others: one in K makes

@@ -1453,12 +1453,17 @@ extern "C" llmx_status llmx_kv4_attn_fwd(const llmx_attn_params *p, const llmx_k
   if (p->workspace != nullptr && !al16(p->workspace)) return bad("workspace must be 16-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   llmx_status refused;
-  if (use_expanded(a, p->algo, &refused)) {
-    const size_t rows = expanded_rows_bytes(a);
-    unsigned char *ws = static_cast<unsigned char *>(p->workspace);
-    if (ws == nullptr || p->workspace_bytes < 2 * rows + kSm100WorkspaceBytes)
+  bool expand = use_expanded(a, p->algo, &refused);
+  const size_t rows = expanded_rows_bytes(a);
+  if (expand && (p->workspace == nullptr || p->workspace_bytes < 2 * rows + kSm100WorkspaceBytes)) {
+    // AUTO then takes the direct form, which needs no workspace, where that can run.
+    if (p->algo != LLMX_ALGO_AUTO || !direct_fits(a))
       return record_error(LLMX_ERR_WORKSPACE_TOO_SMALL,
                           "kv4: the expanded form needs the workspace that llmx_kv4_attn_workspace_size gives");
+    expand = false;
+  }
+  if (expand) {
+    unsigned char *ws = static_cast<unsigned char *>(p->workspace);
     AttnArgs e;
     expanded_request(a, ws, &e);
     llmx_kv4_rows r{};

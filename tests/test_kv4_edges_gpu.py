@@ -283,6 +283,34 @@ def test_a_cache_full_of_nan():
         assert torch.equal(out.isnan().all(-1).all(-1).cpu(), seen) and (out[~seen.to(DEV)] == 0).all(), algo
 
 
+@pytest.mark.parametrize("H,hkv,sq", [(8, 2, 256), (4, 4, 400)])
+def test_auto_without_its_workspace_runs_the_direct_form(H, hkv, sq):
+    dtype, d, n = torch.bfloat16, 128, 1500
+    gen = torch.Generator().manual_seed(sq)
+    k, v = (torch.randn(1, n, hkv, d, generator=gen).to(dtype) for _ in range(2))
+    cache, q = stored(k, v), torch.randn(1, sq, H, d, generator=gen).to(dtype)
+    qd, lens = q.to(DEV), torch.tensor([n], device=DEV, dtype=torch.int32)
+    out, lib = torch.empty_like(qd), _lib.load()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    ws = ctypes.c_size_t(0)
+    need = {}
+    for algo in ("auto", "tcgen05", "decode"):
+        p, c, keep = request(cache, None, qd, out, lens, scale=d ** -0.5, algo=algo)
+        _lib.check(lib.llmx_kv4_attn_workspace_size(ctypes.byref(p), ctypes.byref(c), ctypes.byref(ws)))
+        need[algo] = ws.value
+    assert need["auto"] == need["tcgen05"]  # a request that AUTO expands
+    p, c, keep = request(cache, None, qd, out, lens, scale=d ** -0.5, algo="tcgen05")
+    assert lib.llmx_kv4_attn_fwd(ctypes.byref(p), ctypes.byref(c), stream) == 3, lib.llmx_attn_last_error()
+    small = torch.empty(need["decode"] + 16, dtype=torch.uint8, device=DEV)
+    for ptr, size in ((None, 0), (small.data_ptr(), small.numel())):
+        p, c, keep = request(cache, None, qd, out, lens, scale=d ** -0.5)
+        p.workspace, p.workspace_bytes = ptr, size
+        out.fill_(7.0)
+        _lib.check(lib.llmx_kv4_attn_fwd(ctypes.byref(p), ctypes.byref(c), stream))
+        torch.cuda.synchronize()
+        check(out[0], None, q[0], k[0], v[0], n, dtype, sm_scale=d ** -0.5)
+
+
 def test_a_row_count_near_31_bits():
     """max_rows as the largest integer, over rows of stride 0, with a length of a few."""
     dtype, d, hkv = torch.float16, 256, 15
