@@ -283,7 +283,7 @@ def test_a_cache_full_of_nan():
         assert torch.equal(out.isnan().all(-1).all(-1).cpu(), seen) and (out[~seen.to(DEV)] == 0).all(), algo
 
 
-@pytest.mark.parametrize("H,hkv,sq", [(8, 2, 256), (4, 4, 400)])
+@pytest.mark.parametrize("H,hkv,sq", [(8, 2, 1024), (16, 4, 700)])
 def test_auto_without_its_workspace_runs_the_direct_form(H, hkv, sq):
     dtype, d, n = torch.bfloat16, 128, 1500
     gen = torch.Generator().manual_seed(sq)
