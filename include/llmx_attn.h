@@ -348,7 +348,8 @@ LLMX_API llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_rows 
  * as well), and an infinity or NaN in q its row (TCGEN05 with a soft-cap takes
  * the infinite scores as +- the cap).  A row's p s keeps
  * 11 bits down to 2^-21 of its largest, by the largest p and the largest V step
- * that the row sees; a bf16 K is taken up to 2^96 in size. */
+ * that the row sees, and p itself in sums and lse down to 2^-48; a bf16 K is
+ * taken up to 2^96 in size. */
 LLMX_API llmx_status llmx_kv4_attn_workspace_size(const llmx_attn_params *p, const llmx_kv4_cache *c, size_t *bytes);
 LLMX_API llmx_status llmx_kv4_attn_fwd(const llmx_attn_params *p, const llmx_kv4_cache *c, void *stream);
 

@@ -81,6 +81,11 @@ constexpr int kStepExp = 7;
 constexpr float kCentreStep = 0x1p-20f;
 constexpr int kMinStepExp = -40;
 constexpr int kMaxStepExp = 125;
+// A weight below 2^-126 is 0 and missing from its row's sum as well.  bf16 has
+// steps up to 2^125, which would leave the weights 8 binades; their products
+// with the steps take a factor of 2^-kFarShift there, so that the weights keep
+// 48 (and reach 2^93 beside the smallest steps).
+constexpr int kFarShift = 40;
 constexpr uint64_t kWaitNs = 1000000000ull;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -374,6 +379,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
   // The other column of a lone pair takes what fp16 leaves of its weights: free,
   // and of use where the output has fp16's own 11 bits.
   constexpr bool kLow = NQ == 1 && std::is_same<T, __half>::value;
+  constexpr int kFar = std::is_same<T, __nv_bfloat16>::value ? kFarShift : 0;  // fp16 steps stay below 2^16
   constexpr int kTileCols = Sh::kTileCols, kColStep = NQ == 1 ? 2 : 1;  // pair r of a tile has column r * kColStep
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t sm_full[kWarps][kStages];
@@ -794,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
           const int new_exp = max(step_exp[q], min(kMaxStepExp, (int)(top >> 23) - 127));
-          const float old_room = (float)(kStepExp - step_exp[q]), new_room = (float)(kStepExp - new_exp);
+          const float old_room = (float)(kStepExp + kFar - step_exp[q]), new_room = (float)(kStepExp + kFar - new_exp);
           step_exp[q] = new_exp;
           least = min(least, new_exp);
           largest = max(largest, new_exp);
@@ -831,7 +837,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
           }
         }
         // The lower of two rows' thresholds: at worst the references are looked at more often.
-        limit = kLazyMax + (float)(kStepExp - largest);
+        limit = kLazyMax + (float)(kStepExp + kFar - largest);
         next_step = pow2i(least + 1);
         fresh = __any_sync(0xffffffffu, missing);
       }
@@ -853,7 +859,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
             float w[2] = {0.f, 0.f};
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
-              w[q] = p[r][q] * sv[r][h];
+              w[q] = (kFar > 0 ? p[r][q] * pow2i(-kFar) : p[r][q]) * sv[r][h];
               if constexpr (PART) {
                 const bool ok = vis >> r * NQ + q & 1u;
                 if (!ok) w[q] = 0.f;
@@ -951,8 +957,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
             even += o[h][i][1];
             odd += o[h][i][3];
           }
-          out[h][2 * i] = even + aff[q][h];
-          out[h][2 * i + 1] = fmaf(odd, 0.0625f, aff[q][h]);
+          out[h][2 * i] = fmaf(even, pow2i(kFar), aff[q][h]);
+          out[h][2 * i + 1] = fmaf(odd, 0.0625f * pow2i(kFar), aff[q][h]);
         }
       float m = ref[q], sum = l[q];
       if constexpr (SLOTS == 2) {

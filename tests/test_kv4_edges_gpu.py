@@ -311,6 +311,39 @@ def test_auto_without_its_workspace_runs_the_direct_form(H, hkv, sq):
         check(out[0], None, q[0], k[0], v[0], n, dtype, sm_scale=d ** -0.5)
 
 
+@pytest.mark.parametrize("H,hkv,d", [(1, 1, 64), (4, 1, 128), (8, 1, 128), (8, 8, 128), (2, 1, 256), (6, 2, 64)])
+@pytest.mark.parametrize("batch", [1, 40])
+def test_many_small_weights_beside_large_steps(H, hkv, d, batch):
+    """One token at the maximum and 8192 that weigh 2^-12 of it each, V near bf16's end: the small ones are two thirds of the sum."""
+    dtype, n = torch.bfloat16, 8193
+    gen = torch.Generator().manual_seed(d + H)
+    v = ((torch.rand(1, n, hkv, d, generator=gen) * 2 - 1) * 1e38).to(dtype)
+    k = torch.zeros(1, n, hkv, d, dtype=dtype)
+    k[:, 100] = 1.0  # a score of 12 ln 2 over the rest
+    q = torch.full((1, 1, H, d), 12 * math.log(2.0) / d, dtype=torch.float32).to(dtype)
+    cache = stored(k.expand(batch, -1, -1, -1), v.expand(batch, -1, -1, -1))
+    out, lse = torch.empty(batch, 1, H, d, dtype=dtype, device=DEV), torch.empty(batch, H, 1, device=DEV)
+    llmx_b200.kv4_attention(out, q.to(DEV).expand(batch, -1, -1, -1), cache, 1.0, max_kv_len=n, lse=lse, algo="decode")
+    for b in {0, batch // 2, batch - 1}:
+        check(out[b], lse[b], q[0], k[0], v[0], n, dtype, sm_scale=1.0, what=f"sequence {b}")
+
+
+def test_the_log_sum_exp_of_scores_that_move_the_maximum():
+    """Rising and falling scores, steps of very different sizes: the log-sum-exp beside the output."""
+    dtype, d, n = torch.bfloat16, 128, 700
+    gen = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(n, 1, d, generator=gen).to(dtype) for _ in range(2))
+    ramp = torch.linspace(0.0, 8.0, n)[:, None, None]
+    size = torch.pow(10.0, torch.linspace(-6, 6, n))[torch.randperm(n, generator=gen)][:, None, None]
+    for kk, vv in (((k * ramp).to(dtype), v), ((k * ramp.flip(0)).to(dtype), v), (k, (v * size).to(dtype)),
+                   ((k * ramp).to(dtype), (v * ramp * 1e-3).to(dtype)), (k, (v * size * 1e30).to(dtype))):
+        cache = stored(kk[None], vv[None])
+        q = (torch.randn(1, 1, 8, d, generator=gen) * torch.tensor([1e-20, 1e-3, 1, 1, 2, 4, 8, 30])[None, None, :, None]).to(dtype)
+        out, lse = torch.empty_like(q, device=DEV), torch.empty(1, 8, 1, device=DEV)
+        llmx_b200.kv4_attention(out, q.to(DEV), cache, d ** -0.5, max_kv_len=n, lse=lse)
+        check(out[0], lse[0], q[0], kk, vv, n, dtype, sm_scale=d ** -0.5)
+
+
 def test_a_row_count_near_31_bits():
     """max_rows as the largest integer, over rows of stride 0, with a length of a few."""
     dtype, d, hkv = torch.float16, 256, 15
