@@ -162,6 +162,12 @@ __device__ __forceinline__ void row_range(const AttnArgs &a, int i, int ql, int 
   lo = a.window >= 0 ? max(0, diag - a.window) : 0;
 }
 
+// ALiBi counts from the token of the row's largest bias, which changes no weight:
+// slope j itself would take the scores' last bits with it far into a sequence
+// (2^-7 of 158,000 at a slope of 0.84 and 131,072 tokens).  The log-sum-exp gets
+// slope times this token back.
+__device__ __forceinline__ int bias_origin(float slope, int lo, int hi) { return slope > 0.f ? hi - 1 : lo; }
+
 // The tokens of sequence b that its rows see between them, as steps of W
 // tiles from a 16-token boundary (rows' ranges move one way: the first row's
 // begin to the last row's end).
@@ -360,7 +366,7 @@ struct Shape {
   static constexpr int kMinCtas = G <= 2 ? 4 : 3;
   static constexpr int kRing = kStages * W * kTile;
   static constexpr int kQFrag = G * 2 * 32 * 16;
-  static constexpr int kRows = kCols * (4 + 2 * G) * 4;  // factor, slope, lo, hi, sums and starts of the groups
+  static constexpr int kRows = kCols * (5 + 2 * G) * 4;  // factor, slope, lo, hi, origin, sums and starts of the groups
   // Each warp's ring; q and its columns, of each warp or of all; as many
   // zeros as q for the other tiles' columns; lengths and prefix sums.
   static constexpr int kZeros = SLOTS > 1 ? kQFrag : 0;
@@ -393,7 +399,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
   float *row_f = reinterpret_cast<float *>(q_at0 + Sh::kQFrag);
   float *row_slope = row_f + kCols;
   int *row_lo = reinterpret_cast<int *>(row_f + 2 * kCols), *row_hi = row_lo + kCols;
-  float *row_qs = row_f + 4 * kCols;                           // [G][kCols]
+  int *row_origin = row_lo + 2 * kCols;
+  float *row_qs = row_f + 5 * kCols;                           // [G][kCols]
   int *row_begin = reinterpret_cast<int *>(row_qs + G * kCols);  // [G][kCols]
   unsigned char *zeros = smem + Sh::kSmem - Sh::kZeros;
   int2 *lens = reinterpret_cast<int2 *>(smem + Sh::kSmem);               // [nb]
@@ -626,7 +633,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
             int lo, hi;
             row_range(a, live ? i : ql - 1, ql, kl, lo, hi);  // a column without a row goes with the last one
             row_f[col] = up > 0.f ? scale / up : (top > 0.f ? CUDART_NAN_F : 0.f);
-            row_slope[col] = live && a.alibi != nullptr ? a.alibi[h0] * kLog2e : 0.f;
+            const float slope = live && a.alibi != nullptr ? a.alibi[h0] * kLog2e : 0.f;
+            row_slope[col] = slope;
+            row_origin[col] = bias_origin(slope, lo, hi);
             row_lo[col] = lo;
             row_hi[col] = hi;
           }
@@ -733,9 +742,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
       if (a.alibi != nullptr) {
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-          const float slope = row_slope[2 * t + q];
+          const float slope = row_slope[2 * t + q], dist = (float)(tok - row_origin[2 * t + q]);
 #pragma unroll
-          for (int r = 0; r < 2; ++r) s[r][q] = fmaf(slope, (float)(tok + 8 * r), s[r][q]);
+          for (int r = 0; r < 2; ++r) s[r][q] = fmaf(slope, dist + 8.f * r, s[r][q]);
         }
       }
       uint32_t vis = 0;  // bit r NQ + q; only with PART
@@ -937,6 +946,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
       }
     }
 
+    // What the log-sum-exp of pair `pr` gets back.
+    auto origin_bias = [&](int h0, int pr) {
+      return a.alibi != nullptr ? a.alibi[h0] * (float)row_origin[pr * kColStep] : 0.f;
+    };
+
     // ---- the unit's result: sums over the tokens (lanes with the same t hold
     // the same rows), then over the tiles' columns
 #pragma unroll
@@ -1011,7 +1025,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
               for (int x = 0; x < 8; ++x) op[64 * h + x] = Elem<T>::from_f(out[h][x]);
             }
           }
-          if (a.lse != nullptr && g == 0) a.lse[((long long)b * a.H + h0) * a.Sq + i] = lse;
+          if (a.lse != nullptr && g == 0) a.lse[((long long)b * a.H + h0) * a.Sq + i] = lse + origin_bias(h0, pr);
         } else {
           // Slot 1 for the unit that begins in this share, slot 0 for the
           // one that began before it.
@@ -1069,7 +1083,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NQ, SLOTS, COOP>::kMinCtas)
             op[2] = Elem<T>::from_f(ov.z);
             op[3] = Elem<T>::from_f(ov.w);
           }
-          if (a.lse != nullptr && d == 0) a.lse[((long long)b * a.H + h0) * a.Sq + i] = lse;
+          if (a.lse != nullptr && d == 0) a.lse[((long long)b * a.H + h0) * a.Sq + i] = lse + origin_bias(h0, pr);
         } else {
           const long long row = ((long long)worker * 2 + (pl.at == 0 ? 1 : 0)) * R + pr;
           *reinterpret_cast<float4 *>(part_o + row * D + d) = ov;
@@ -1197,8 +1211,15 @@ __global__ void __launch_bounds__(PARTS > 1 ? PARTS * 32 : kThreads) kv4_merge_k
   T *op = static_cast<T *>(a.o) + b * a.os[0] + i * a.os[1] + h * a.os[2] + lane * E;
 #pragma unroll
   for (int e = 0; e < E; ++e) op[e] = Elem<T>::from_f(o[e] * inv);
-  if (a.lse != nullptr && lane == 0)
-    a.lse[((long long)b * a.H + h) * a.Sq + i] = none ? -CUDART_INF_F : m + logf(sum);
+  if (a.lse != nullptr && lane == 0) {
+    float bias = 0.f;
+    if (a.alibi != nullptr) {
+      int lo, hi;
+      row_range(a, i, clamp_len(a.q_lens, b, a.Sq), clamp_len(a.kv_lens, b, a.Skv), lo, hi);
+      bias = a.alibi[h] * (float)bias_origin(a.alibi[h], lo, hi);
+    }
+    a.lse[((long long)b * a.H + h) * a.Sq + i] = none ? -CUDART_INF_F : m + logf(sum) + bias;
+  }
 }
 
 struct Plan {

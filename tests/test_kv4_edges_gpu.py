@@ -344,6 +344,43 @@ def test_the_log_sum_exp_of_scores_that_move_the_maximum():
         check(out[0], lse[0], q[0], kk, vv, n, dtype, sm_scale=d ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,H,hkv,sq", [(64, 8, 2, 1), (128, 4, 4, 1), (64, 8, 1, 3), (256, 4, 2, 1), (128, 8, 1, 2)])
+@pytest.mark.parametrize("batch", [1, 150])
+def test_alibi_goes_by_distance_however_far(dtype, d, H, hkv, sq, batch):
+    """The same tokens behind windows that end early and late in a sequence: the biases differ by a constant, which a softmax does
+    not see.  Steep and flat slopes of both signs; the pages before the window are one page, never read."""
+    gen = torch.Generator().manual_seed(d + H + sq)
+    page, n, window = 2 ** 14, 1000, 800
+    k, v = (torch.randn(1, n, hkv, d, generator=gen).to(dtype) for _ in range(2))
+    q = torch.randn(1, sq, H, d, generator=gen).to(dtype)
+    slopes = torch.tensor([0.84, -0.5, 0.25, 0.003, -0.01, 0.0, 0.71, 1.0])[:H]
+    cache = llmx_b200.kv4_empty(2, hkv, d, page, device=DEV)
+    cache.fill_(255)
+    got = []
+    for far in (0, 2 ** 17, 2 ** 20, 2 ** 25):
+        table = torch.ones(batch, far // page + 1, dtype=torch.int32, device=DEV)
+        table[:, -1] = 0
+        at = torch.full((batch,), far, dtype=torch.int32, device=DEV)
+        llmx_b200.kv4_store(cache, k.to(DEV), v.to(DEV), start=at[:1], block_table=table[:1])
+        out, lse = torch.empty(batch, sq, H, d, dtype=dtype, device=DEV), torch.empty(batch, H, sq, device=DEV)
+        llmx_b200.kv4_attention(out, q.to(DEV).expand(batch, -1, -1, -1), cache, d ** -0.5, window, kv_lens=at + n, block_table=table,
+                                alibi_slopes=slopes.to(DEV), lse=lse, algo="decode")
+        got.append((far, out.double().cpu(), lse.double().cpu()))
+    o, le, _, _ = okv4.attention(q[0], k[0], v[0], sq, n, sm_scale=d ** -0.5, slopes=slopes, window=window)
+    half = torch.finfo(dtype).eps / 2
+    # What differs from call to call: each p s is rounded to fp16 (2^-11) from another reference, at most 8 steps (half the range) of V
+    # each; sums in fp32 (1000 terms of at most 2^-24, over outputs of at most 8 steps) and the output's own rounding.
+    steps = okv4.quantise(v)[1].double().max()
+    for far, out, lse in got[1:]:
+        room = 2 * (8 * steps * (2 ** -11 + 2 ** -14) + half * o.abs() + half * 8 * steps * 2 ** -8)
+        off = (out - got[0][1]).abs()
+        assert (off <= room).all(), f"{far}: worst {float((off / room).max()):.3g} of the room"
+        # fp32 numbers of the size of the log-sum-exp: three roundings each, and the sum's.
+        want = got[0][2] + (slopes.double() * far)[None, :, None]
+        assert ((lse - want).abs() <= (lse.abs() + le.abs()) * 2 ** -22 + 2 ** -12).all(), f"{far}: lse"
+
+
 def test_a_row_count_near_31_bits():
     """max_rows as the largest integer, over rows of stride 0, with a length of a few."""
     dtype, d, hkv = torch.float16, 256, 15
