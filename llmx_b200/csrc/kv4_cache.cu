@@ -132,7 +132,7 @@ __device__ __forceinline__ float inverse_of(float s) {
 // lane for each group j.
 template <typename T, int N, int L, int FIRST, typename Own>
 __device__ __forceinline__ void finish_groups(uint32_t (&v)[N], uint32_t (&param)[N], float (&inv)[N], int lane, Own own) {
-  constexpr int kMine = N > L ? N / L : 1;
+  constexpr int kMine = N > L ? N / L : 1, kSame = N < L ? L / N : 1;  // groups of a lane, lanes of a group
   int cur = N;
 #pragma unroll
   for (int off = L / 2 * FIRST; off >= FIRST; off /= 2) {
@@ -156,11 +156,11 @@ __device__ __forceinline__ void finish_groups(uint32_t (&v)[N], uint32_t (&param
   for (int j = 0; j < kMine; ++j) {
     p[j] = param_of<T>(v[j]);
     iv[j] = inverse_of(kv4_unpack_param<T>(p[j]).x);
-    if (N >= L || li % (L / N) == 0) own(N >= L ? li * kMine + j : li / (L / N), p[j]);
+    if (li % kSame == 0) own(li * kMine / kSame + j, p[j]);
   }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int from = lane % FIRST + (N >= L ? j / kMine : j * (L / N)) * FIRST + lane / (FIRST * L) * (FIRST * L);
+    const int from = lane % FIRST + j * kSame / kMine * FIRST + lane / (FIRST * L) * (FIRST * L);
     param[j] = __shfl_sync(0xffffffffu, p[j % kMine], from);
     inv[j] = __shfl_sync(0xffffffffu, iv[j % kMine], from);
   }
