@@ -177,7 +177,10 @@ const int32_t *int_arg(const char *name, const std::optional<torch::Tensor> &t, 
   if (!t.has_value()) return nullptr;
   TORCH_CHECK(t->is_cuda() && t->device() == dev, name, " must be on the cache's device");
   // The usual tensor is taken as it is: each conversion call costs a microsecond even when it has nothing to do.
-  keep = t->scalar_type() == torch::kInt && t->is_contiguous() ? *t : t->to(torch::kInt).contiguous();
+  // Of 64 bits, what 32 do not hold becomes the nearest number that they do, not its low half.
+  if (t->scalar_type() == torch::kInt) keep = t->is_contiguous() ? *t : t->contiguous();
+  else if (t->scalar_type() == torch::kLong) keep = t->clamp((int64_t)INT32_MIN, (int64_t)INT32_MAX).to(torch::kInt).contiguous();
+  else keep = t->to(torch::kInt).contiguous();
   TORCH_CHECK(keep.numel() == batch, name, " must have batch elements");
   return keep.data_ptr<int32_t>();
 }

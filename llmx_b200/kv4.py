@@ -46,6 +46,8 @@ def _int_arg(name: str, t: Optional[torch.Tensor], batch: int, device, keep):
     if t is None:
         return None
     _req(t.is_cuda and t.device == device, f"{name} must be on the cache's device")
+    if t.dtype == torch.int64:  # what 32 bits do not hold becomes the nearest number that they do, not its low half
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
     t = t.to(torch.int32).contiguous()
     _req(t.numel() == batch, f"{name} must have batch elements")
     keep.append(t)

@@ -396,3 +396,36 @@ def test_a_row_count_near_31_bits():
             okv4.write_token(want[h], tok, x[0, 0, h], x[0, 0, h])
     assert torch.equal(cache[0, :, 0].cpu(), want)
     llmx_b200.device_status(0)
+
+
+@pytest.mark.parametrize("binding", [True, False])
+@pytest.mark.parametrize("start", [2 ** 32 + 3, -2 ** 32 + 3, 2 ** 40])
+def test_positions_past_32_bits_are_reported(binding, start):
+    """int64 positions whose low halves are inside the cache: dropped and reported, like any other outside it."""
+    dtype, d, hkv = torch.bfloat16, 64, 2
+    cache = llmx_b200.kv4_empty(1, hkv, d, 16, device=DEV)
+    cache.fill_(255)
+    k = torch.randn(1, 2, hkv, d, device=DEV).to(dtype)
+    at = torch.tensor([start], device=DEV, dtype=torch.int64)
+    llmx_b200.device_status(0)
+    if binding:
+        llmx_b200.kv4_store(cache, k, k, start=at)
+    else:
+        kv4._rows_call("llmx_kv4_store", cache, k, k, at, None, None)
+    with pytest.raises(_lib.LlmxError, match="position"):
+        llmx_b200.device_status(0)
+    assert (cache == 255).all()
+    # Lengths too: past the cache means all of it.
+    q = torch.randn(1, 1, hkv, d, device=DEV).to(dtype)
+    x = torch.randn(1, 16, hkv, d, device=DEV).to(dtype)
+    llmx_b200.kv4_store(cache, x, x)
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    call = llmx_b200.kv4_attention if binding else kv4.kv4_attention_ctypes
+    call(a, q, cache, 0.1, kv_lens=torch.tensor([2 ** 32 + 3], device=DEV))
+    call(b, q, cache, 0.1)
+    assert torch.equal(a, b)
+    # Narrow types have nothing to lose.
+    for t in (torch.int16, torch.uint8):
+        call(a, q, cache, 0.1, kv_lens=torch.tensor([7], device=DEV, dtype=t))
+        call(b, q, cache, 0.1, kv_lens=torch.tensor([7], device=DEV, dtype=torch.int32))
+        assert torch.equal(a, b)
