@@ -260,8 +260,8 @@ LLMX_API llmx_status llmx_convert(const void *src, int32_t src_dtype, void *dst,
  *   n = min(15, rint(fl32(fl32(x - m) / s)))  (0 where s = 0),
  *   value = n s + m, within s / 2 of x; finite x read back finite.
  * A group with a NaN or an infinity in it (or, for bf16, a range max x - m
- * past fp32) has s = NaN and reads back as NaN.  4.5 bits a value: 18 * head_dim bytes per
- * 16 tokens of K and V of one kv head.
+ * past fp32) has s = NaN and reads back as NaN.  4.5 bits a value:
+ * 18 * head_dim bytes per 16 tokens of K and V of one kv head.
  *
  * The cache is made of pages of page_size tokens (a multiple of 16).  Page p,
  * kv head h starts at data + p * page_stride + h * head_stride and holds
@@ -339,8 +339,9 @@ LLMX_API llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_rows 
  *   TCGEN05 expands the sequences into the workspace (values rounded to T)
  *           and runs the tensor-core prefill on them; needs its workspace.
  *   AUTO    DECODE, or for long query blocks TCGEN05 where it can run, is
- *           expected to be faster, takes at most 4 GiB and has its workspace
- *           (without it, TCGEN05 where DECODE cannot count the rows: an error).
+ *           expected to be faster, takes at most 4 GiB and has its workspace.
+ *           (Query blocks that DECODE cannot count take TCGEN05 in any case,
+ *           and fail without its workspace.)
  * A call on the DECODE path given too little workspace runs without
  * splitting a sequence's keys.  Calls that share a workspace must not overlap
  * on the GPU.  A NaN reaches the rows that see it and no others: one in K makes

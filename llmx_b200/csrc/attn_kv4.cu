@@ -28,10 +28,8 @@
 // linear copies in shared memory to registers to the tensor core; P^T changes
 // from the accumulator's layout to the operand's with one 8x8 transpose
 // (movmatrix) per 8 tokens and group.  mma.sync and not tcgen05: the operands
-// are made in registers, 8 columns are all there are in a decode, and what
-// bounds the pass is the integer unit that unpacks the nibbles (two cycles an
-// operation and warp, 88 operations a 16-token tile of 128 channels) next to
-// the cache's bytes, not the products.
+// are made in registers, 8 columns are all there are in a decode, and the
+// products are not what bounds the pass (the tensor pipe is a quarter filled).
 //
 // Work.  A unit is one (sequence, kv head, block of pairs); its tokens are cut
 // into steps of one or two tiles.  Short units have a worker each.  Of longer
@@ -46,12 +44,16 @@
 // kernel merges them.
 //
 // Measured on one B200 (bytes of the visible cache, q and o): 64 sequences of
-// 256-4096 tokens, 32 heads of 128, ALiBi: 124-134 us, 5.1 TB/s (0.77 of the
-// copy rate); 32 sequences of 1001-8191 tokens, 32 heads on 8: 47 us, 3.6 TB/s;
-// 131071 tokens, 32 heads on 8: 41 us, 3.7 TB/s.  What bounds it is not HBM yet:
-// at 16 warps an SM (128 registers) the issue slots are 0.6 filled, the unpacking
-// keeps the integer pipe 0.6 busy, and more warps with fewer registers (20 of
-// 96) ran 15-25% slower, fewer with more (12 of 168) 4-8%.
+// 256-4096 tokens, 32 heads of 128, ALiBi: 126-135 us from box to box, 4.8-5.1
+// TB/s (0.73-0.78 of the copy rate); 32 sequences of 1001-8191 tokens, 32 heads
+// on 8: 47 us, 3.6 TB/s; 131071 tokens, 32 heads on 8: 41 us, 3.7 TB/s.  Nothing
+// is full: DRAM 0.48-0.65 of its peak, issue slots 0.54-0.60, the integer pipe
+// that unpacks the nibbles 0.41-0.59.  A tile's scores, softmax and output
+// product are one chain of results, and at 16 warps an SM (128 registers) a warp
+// mostly waits for its own last one.  More warps with fewer registers (20 of 96)
+// ran 15-25% slower, fewer with more (12 of 168) 4-8%.  With 8 pairs a warp at
+// head_dim 128 the registers do not hold all: 28 bytes are spilled and 100 read
+// back by warps, 60 and 92 by CTAs.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -1248,6 +1250,11 @@ Plan plan_kv4(const AttnArgs &a) {
   // (direct_fits() keeps one sequence's steps below 2^31.)
   p.nb = (int)std::min<long long>(std::min(a.B, kMaxSlice), std::max<long long>(1, 0x7fffffffLL / (per_seq * steps)));
   const long long units = p.nb * per_seq, most = units * steps;
+  // (At head_dim 256 only two fit beside the lengths of more than 256 sequences,
+  // and a third of the shares then comes after the others.  Launches of 256
+  // sequences instead cost another start and merge: 512 sequences of 1024-2048
+  // tokens, 8 heads on 2, 141 us against 167, but 300 of 512-1024 88 against 78,
+  // so it is left.)
   const int resident = a.num_sms * (a.D <= 128 ? 4 : 3);
   // Short sequences: a unit has one worker, which saves the merge's launch and
   // the second part of a share.  Longer ones are shared out; with many units by
@@ -1300,6 +1307,11 @@ cudaError_t launch_variant(const AttnArgs &a, const Kv4Args &c, const Plan &p, b
     wk.nb = std::min(p.nb, a.B - b0);
     wk.R = p.R;
     wk.workers = (int)workers;
+    // A share of CTAs has at least two steps a warp.  Measured, us with 4 / 8 /
+    // 16 / 32 steps, 32 heads on 8 of 128: 1 sequence of 2048 tokens 8.9 / 9.4 /
+    // 10.8 / 13.8, of 8192 12.0 / 11.4 / 12.5 / 14.4, 4 of 8192 19.3 / 19.4 /
+    // 16.7 / 19.6, 16 of 2048 20.2 / 20.2 / 16.6 / 19.5; 1 of 16384, 16 heads on 4
+    // of 64: 12.0 / 10.6 / 10.9 / 12.2.
     wk.min_steps = COOP ? 2 * kWarps : 1;
     wk.units = (int)std::min<long long>(0x7fffffff, (long long)wk.nb * a.Hkv * ((p.rows + p.R - 1) / p.R));
     wk.split = split ? 1 : 0;
@@ -1308,9 +1320,10 @@ cudaError_t launch_variant(const AttnArgs &a, const Kv4Args &c, const Plan &p, b
     if (e != cudaSuccess) return e;
     if (!split) continue;
     // The merge's launch overlaps the shares; it waits for them itself.
-    // Warps of a row by its shares: 8 of them against 4 take 1.8 us less with 74
-    // shares and 1.9 us more with 9 (us of the whole call: 41.0 and 42.7 for one
-    // sequence of 131071 tokens, 49.1 and 47.2 for 32 of up to 8191).
+    // Warps of a row by its shares.  Measured, us of the whole call with 1 / 4 / 8
+    // warps, 32 heads on 8 of 128: 5 shares 20.1 / 20.1 / 23.7 (16 sequences of
+    // 2048 tokens), 10 41.3 / 40.9 / 47.2 (32 of 4096), 19 21.9 / 19.4 / 19.4 (4 of
+    // 8192), 64 16.2 / 11.7 / 11.4 (1 of 8192), 74 29.8 / 19.4 / 17.7 (1 of 32768).
     const int parts = p.per_unit > 32 ? 8 : (p.per_unit > 8 ? 4 : 1);
     const long long out_rows = (long long)wk.nb * a.Sq * a.H;
     cudaLaunchConfig_t cfg{};
