@@ -338,6 +338,8 @@ LLMX_API llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_rows 
  *           row's largest element (steps of 1/32512), p s in fp16.
  *   TCGEN05 expands the sequences into the workspace (values rounded to T)
  *           and runs the tensor-core prefill on them; needs its workspace.
+ *           ALiBi adds slope * position in fp32, as llmx_attn_fwd does (DECODE:
+ *           the distance from the row's largest bias).
  *   AUTO    DECODE, or for long query blocks TCGEN05 where it can run, is
  *           expected to be faster, takes at most 4 GiB and has its workspace.
  *           (Query blocks that DECODE cannot count take TCGEN05 in any case,
