@@ -356,13 +356,110 @@ LLMX_API llmx_status llmx_kv4_load(const llmx_kv4_cache *c, const llmx_kv4_rows 
 LLMX_API llmx_status llmx_kv4_attn_workspace_size(const llmx_attn_params *p, const llmx_kv4_cache *c, size_t *bytes);
 LLMX_API llmx_status llmx_kv4_attn_fwd(const llmx_attn_params *p, const llmx_kv4_cache *c, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Paged key/value cache in 16 bits.  No counterpart in the reference (it has
+ * no cache).  K and V (fp16 / bf16, head_dim 64, 128 or 256) lie in pages of
+ * page_size tokens (a multiple of 16), each with its own element strides
+ * {page, kv head, token} and unit stride on head_dim; strides are multiples
+ * of 8 and pointers 16-byte aligned, and no two elements may share a place.
+ * Token j of sequence b lies in page block_table[b * table_stride + j /
+ * page_size] (NULL: page b * max_pages + j / page_size).  Entries that hold
+ * no token of a sequence are not read, and neither is what a page holds
+ * behind a sequence's length.  An entry outside [0, n_pages), or a position
+ * outside [0, max_pages * page_size), is never followed: rows there are not
+ * written and read as zeros, and llmx_attn_device_status then returns
+ * LLMX_ERR_INVALID_ARGUMENT.
+ *   key_weights (NULL or device fp32, element strides {page, kv head}, unit
+ * stride on the token; 16-byte aligned, strides multiples of 4) has a weight
+ * for every cached (token, kv head), in the same pages. */
+typedef struct llmx_paged_cache {
+  int32_t dtype;      /* llmx_dtype of K and V: fp16 or bf16              */
+  int32_t n_kv_heads; /* >= 1                                             */
+  int32_t head_dim;   /* 64, 128 or 256                                   */
+  int32_t page_size;  /* tokens, a multiple of 16                         */
+  int32_t n_pages;    /* >= 1                                             */
+  int32_t max_pages;  /* pages of one sequence (columns of block_table);
+                         max_pages * page_size <= 2^30                    */
+  void *k;
+  void *v;
+  int64_t k_stride[3]; /* elements: page, kv head, token                  */
+  int64_t v_stride[3];
+  const int32_t *block_table; /* device [batch, max_pages] or NULL        */
+  int64_t table_stride;       /* elements between its rows                */
+  float *key_weights;
+  int64_t w_stride[2]; /* elements: page, kv head                         */
+} llmx_paged_cache;
+
+/* Copies the rows of K and V (the same description of rows as the 4-bit
+ * cache's) into the cache: row i < lens[b] becomes token start[b] + i of
+ * sequence b.  Nothing else of the cache changes.  Two rows stored to the
+ * same place by one call leave an undefined mix of both there. */
+LLMX_API llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv4_rows *rows, void *stream);
+
+/* llmx_attn_fwd over the cache instead of dense K / V: same request, masks
+ * and results (p->k, p->v and their strides are ignored; p->dtype, n_kv_heads
+ * and head_dim must match the cache; p->max_kv_len <= max_pages * page_size
+ * bounds kv_lens; kv_offset / kv_total must be 0; q and o rows 16-byte
+ * aligned).  Any max_q_len: one new token a sequence, a few, or a chunk of a
+ * prompt; a sequence's query rows are its last q_len tokens under the causal
+ * mask.  p->algo:
+ *   DECODE  streams K and V once for every 16, 32 or 64 (query row, head)
+ *           pairs of a kv head, split over the machine.
+ *   TCGEN05 tensor-core tiles of 128 such pairs; sm_scale > 0.
+ *   AUTO    DECODE up to 64 pairs, TCGEN05 above where it can run.
+ * ALiBi's biases count from each row's largest one, so that they keep their
+ * bits far into a sequence; lse is that of slope * position.  A NaN or an
+ * infinity in a cached token reaches the rows that see the token and no
+ * others; one in V may make such a row (and its lse) NaN as a whole.
+ *   With c->key_weights, the weight of every token j < kv_lens[b] of every kv
+ * head becomes
+ *   decay * (what was there) + sum of softmax(row)[j] over the query rows and
+ *                              the query heads of the kv head,
+ * where what was there counts as 0 for the call's own tokens (causal: the
+ * last q_lens[b] ones), and for all where decay is 0 (it is not read then).
+ * decay must be finite and >= 0.
+ *   A call given too little workspace for its partial results runs without
+ * splitting sequences; with key_weights it is refused
+ * (LLMX_ERR_WORKSPACE_TOO_SMALL).  Calls that share a workspace must not
+ * overlap on the GPU. */
+LLMX_API llmx_status llmx_paged_attn_workspace_size(const llmx_attn_params *p, const llmx_paged_cache *c,
+                                                    size_t *bytes);
+LLMX_API llmx_status llmx_paged_attn_fwd(const llmx_attn_params *p, const llmx_paged_cache *c, float decay,
+                                         void *stream);
+
+/* Eviction by weight.  Of each sequence b and kv head the n = min(kv_lens[b],
+ * budget) tokens are kept that are
+ *   the first `sinks`, the last `recent`, and of the others those of the
+ *   largest key_weights (of equal ones the earliest; a NaN counts as -inf),
+ * in their order.  Their rows of K, V and key_weights become tokens 0 .. n - 1
+ * of the pages of out_table[b] (NULL: of the sequence's own pages, in place;
+ * sequences must then share no page).  With an out_table its pages must hold
+ * no token that the call reads, and share none with one another.  kept [batch, n_kv_heads,
+ * budget] gets their former positions (-1 behind n), new_lens[b] = n; it may
+ * be kv_lens itself.  Nothing else of the cache changes.  No workspace. */
+typedef struct llmx_paged_evict_params {
+  int32_t batch;
+  int32_t budget;            /* >= 1, >= sinks + recent                   */
+  int32_t recent;            /* >= 0                                      */
+  int32_t sinks;             /* >= 0                                      */
+  int32_t max_kv_len;        /* bounds kv_lens; <= max_pages * page_size  */
+  int32_t out_pages;         /* columns of out_table                      */
+  const int32_t *kv_lens;    /* device [batch]                            */
+  const int32_t *out_table;  /* device [batch, out_pages] or NULL         */
+  int64_t out_table_stride;  /* elements between its rows                 */
+  int32_t *kept;             /* device [batch, n_kv_heads, budget]        */
+  int32_t *new_lens;         /* device [batch]                            */
+} llmx_paged_evict_params;
+
+LLMX_API llmx_status llmx_paged_evict(const llmx_paged_cache *c, const llmx_paged_evict_params *e, void *stream);
+
 /* Which kernel family llmx_attn_fwd would run for *p (an llmx_attn_algo). */
 LLMX_API llmx_status llmx_attn_select_algo(const llmx_attn_params *p, int32_t *algo);
 
 /* Synchronises `device` and reads (and optionally clears) its device-side
  * error word: LLMX_ERR_TIMEOUT if any kernel gave up on a bounded wait,
- * LLMX_ERR_INVALID_ARGUMENT if a 4-bit cache was given a page or position
- * outside it. */
+ * LLMX_ERR_INVALID_ARGUMENT if a cache was given a page or position outside
+ * it. */
 LLMX_API llmx_status llmx_attn_device_status(int32_t device, int32_t clear);
 
 LLMX_API const char *llmx_status_string(llmx_status s);

@@ -124,6 +124,45 @@ class Kv4Rows(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """Mirror of ``llmx_paged_cache``."""
+
+    _fields_ = [
+        ("dtype", _i32),
+        ("n_kv_heads", _i32),
+        ("head_dim", _i32),
+        ("page_size", _i32),
+        ("n_pages", _i32),
+        ("max_pages", _i32),
+        ("k", _vp),
+        ("v", _vp),
+        ("k_stride", _i64x3),
+        ("v_stride", _i64x3),
+        ("block_table", _vp),
+        ("table_stride", ctypes.c_int64),
+        ("key_weights", _vp),
+        ("w_stride", ctypes.c_int64 * 2),
+    ]
+
+
+class PagedEvictParams(ctypes.Structure):
+    """Mirror of ``llmx_paged_evict_params``."""
+
+    _fields_ = [
+        ("batch", _i32),
+        ("budget", _i32),
+        ("recent", _i32),
+        ("sinks", _i32),
+        ("max_kv_len", _i32),
+        ("out_pages", _i32),
+        ("kv_lens", _vp),
+        ("out_table", _vp),
+        ("out_table_stride", ctypes.c_int64),
+        ("kept", _vp),
+        ("new_lens", _vp),
+    ]
+
+
 IPC_HANDLE_BYTES = 64
 
 # Every function include/llmx_attn.h declares: name -> (restype, argtypes).
@@ -156,6 +195,13 @@ SIGNATURES = {
         [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache), ctypes.POINTER(ctypes.c_size_t)],
     ),
     "llmx_kv4_attn_fwd": (_i32, [ctypes.POINTER(AttnParams), ctypes.POINTER(Kv4Cache), _vp]),
+    "llmx_paged_store": (_i32, [ctypes.POINTER(PagedCache), ctypes.POINTER(Kv4Rows), _vp]),
+    "llmx_paged_attn_workspace_size": (
+        _i32,
+        [ctypes.POINTER(AttnParams), ctypes.POINTER(PagedCache), ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "llmx_paged_attn_fwd": (_i32, [ctypes.POINTER(AttnParams), ctypes.POINTER(PagedCache), ctypes.c_float, _vp]),
+    "llmx_paged_evict": (_i32, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedEvictParams), _vp]),
     "llmx_convert": (_i32, [_vp, _i32, _vp, _i32, ctypes.c_size_t, _vp]),
     "llmx_attn_device_status": (_i32, [_i32, _i32]),
     "llmx_status_string": (ctypes.c_char_p, [_i32]),

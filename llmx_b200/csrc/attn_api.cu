@@ -441,7 +441,7 @@ llmx_status llmx_attn_device_status(int32_t device, int32_t clear) {
   if (word & kDevErrTimeout) return fail(LLMX_ERR_TIMEOUT, "a device-side bounded wait expired");
   if (word & kDevErrTmemAlloc) return fail(LLMX_ERR_TIMEOUT, "tensor-memory allocation timed out");
   if (word & kDevErrBadPage)
-    return fail(LLMX_ERR_INVALID_ARGUMENT, "a 4-bit cache was given a page or position outside it");
+    return fail(LLMX_ERR_INVALID_ARGUMENT, "a cache was given a page or position outside it");
   return LLMX_OK;
 }
 

@@ -15,7 +15,7 @@ namespace llmx_b200 {
 enum DeviceError : unsigned int {
   kDevErrTimeout = 1u,   // a bounded mbarrier / flag wait gave up
   kDevErrTmemAlloc = 2u, // tensor-memory allocation did not return in time
-  kDevErrBadPage = 4u    // a 4-bit cache page or position outside the cache
+  kDevErrBadPage = 4u    // a page or position outside a paged cache
 };
 
 // A validated, normalised request (all shapes positive, strides in elements).
@@ -60,7 +60,7 @@ DecodePlan plan_decode(const AttnArgs &a, size_t ws_available, bool have_ws);
 // (error word and SM count included).  Records the message on failure.
 llmx_status prepare_decode_request(const llmx_attn_params *p, AttnArgs *a);
 llmx_status record_error(llmx_status s, const char *msg);
-// The checks of a request that reads a 4-bit cache: *p without k, v and their
+// The checks of a request that reads a paged cache: *p without k, v and their
 // strides, and no kernel family; fills *a (with the default SM count).
 llmx_status validate_without_kv(const llmx_attn_params *p, AttnArgs *a);
 // The current device's error word and SM count.

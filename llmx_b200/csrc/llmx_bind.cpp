@@ -329,6 +329,200 @@ void kv4_attention(torch::Tensor output, torch::Tensor q, torch::Tensor cache, d
   check_status(llmx_kv4_attn_fwd(&p, &c, at::cuda::getCurrentCUDAStream(q.device().index()).stream()));
 }
 
+// ---- paged 16-bit key/value cache (llmx_b200/paged.py documents the arguments) -----
+
+namespace {
+
+const int32_t *paged_table(const char *name, const torch::Tensor &t, int64_t batch, torch::Device dev, torch::Tensor &keep) {
+  TORCH_CHECK(t.is_cuda() && t.device() == dev, "paged: ", name, " must be on the cache's device");
+  TORCH_CHECK(t.scalar_type() == torch::kInt && t.dim() == 2 && t.size(0) == batch && t.size(1) >= 1 && t.size(1) <= INT32_MAX,
+              "paged: ", name, " must be int32 [batch, max_pages]");
+  keep = t.stride(1) == 1 ? t : t.contiguous();
+  return keep.data_ptr<int32_t>();
+}
+
+llmx_paged_cache paged_cache(const torch::Tensor &k, const torch::Tensor &v, int64_t batch,
+                             const std::optional<torch::Tensor> &block_table,
+                             const std::optional<torch::Tensor> &key_weights, torch::Tensor &keep) {
+  TORCH_CHECK(k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes(),
+              "paged: the cache must be two tensors [n_pages, n_kv_heads, page_size, head_dim]");
+  TORCH_CHECK(k.is_cuda() && k.device() == v.device(), "paged: the cache must be on one CUDA device");
+  TORCH_CHECK(k.scalar_type() == v.scalar_type() && (k.scalar_type() == torch::kHalf || k.scalar_type() == torch::kBFloat16),
+              "paged: only float16 and bfloat16 are supported");
+  TORCH_CHECK(k.stride(3) == 1 && v.stride(3) == 1, "paged: the cache must have a unit stride on head_dim");
+  TORCH_CHECK(batch <= INT32_MAX, "paged: batch must fit 31 bits");
+  for (int i = 0; i < 4; ++i) TORCH_CHECK(k.size(i) <= INT32_MAX, "paged: cache dimensions must fit 31 bits");
+  llmx_paged_cache c{};
+  c.dtype = llmx_dtype_of(k);
+  c.n_pages = (int32_t)k.size(0);
+  c.n_kv_heads = (int32_t)k.size(1);
+  c.page_size = (int32_t)k.size(2);
+  c.head_dim = (int32_t)k.size(3);
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  set_strides(c.k_stride, k, true);
+  set_strides(c.v_stride, v, true);
+  if (block_table.has_value()) {
+    c.block_table = paged_table("block_table", *block_table, batch, k.device(), keep);
+    c.max_pages = (int32_t)keep.size(1);
+    c.table_stride = keep.stride(0);
+  } else {
+    TORCH_CHECK(batch == 0 || k.size(0) >= batch, "paged: without a block_table the cache needs a page per sequence");
+    c.max_pages = (int32_t)(k.size(0) / std::max<int64_t>(batch, 1));
+  }
+  if (key_weights.has_value()) {
+    const torch::Tensor &w = *key_weights;
+    TORCH_CHECK(w.scalar_type() == torch::kFloat && w.dim() == 3 && w.size(0) == k.size(0) && w.size(1) == k.size(1) &&
+                    w.size(2) == k.size(2) && w.device() == k.device() && w.stride(2) == 1,
+                "paged: key_weights must be fp32 [n_pages, n_kv_heads, page_size] on the cache's device, unit stride on tokens");
+    c.key_weights = w.data_ptr<float>();
+    c.w_stride[0] = w.stride(0);
+    c.w_stride[1] = w.stride(1);
+  }
+  return c;
+}
+
+}  // namespace
+
+void paged_store(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k, torch::Tensor v,
+                 std::optional<torch::Tensor> start, std::optional<torch::Tensor> lens,
+                 std::optional<torch::Tensor> block_table) {
+  TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(), "paged: k and v must be [batch, rows, n_kv_heads, head_dim]");
+  TORCH_CHECK(k.scalar_type() == v.scalar_type() && k.scalar_type() == k_cache.scalar_type(),
+              "paged: k and v must have the cache's dtype");
+  TORCH_CHECK(k.device() == v.device() && k.device() == k_cache.device(), "paged: k, v and the cache must be on one CUDA device");
+  TORCH_CHECK(k_cache.dim() == 4 && k.size(2) == k_cache.size(1) && k.size(3) == k_cache.size(3),
+              "paged: k and v must have the cache's n_kv_heads and head_dim");
+  TORCH_CHECK(k.size(1) <= INT32_MAX, "paged: rows must fit 31 bits");
+  if (k.stride(-1) != 1) k = k.contiguous();
+  if (v.stride(-1) != 1) v = v.contiguous();
+  torch::Tensor keep_table, keep_start, keep_lens;
+  const llmx_paged_cache c = paged_cache(k_cache, v_cache, k.size(0), block_table, std::nullopt, keep_table);
+  const c10::cuda::CUDAGuard guard(k.device());
+  llmx_kv4_rows r{};
+  r.batch = (int32_t)k.size(0);
+  r.max_rows = (int32_t)k.size(1);
+  r.k = k.data_ptr();
+  r.v = v.data_ptr();
+  set_strides(r.k_stride, k, true);
+  set_strides(r.v_stride, v, true);
+  r.start = int_arg("start", start, k.size(0), k.device(), keep_start);
+  r.lens = int_arg("lens", lens, k.size(0), k.device(), keep_lens);
+  check_status(llmx_paged_store(&c, &r, at::cuda::getCurrentCUDAStream(k.device().index()).stream()));
+}
+
+void paged_attention(torch::Tensor output, torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, double sm_scale,
+                     int64_t sliding_window, double logits_soft_cap, std::optional<torch::Tensor> kv_lens,
+                     std::optional<torch::Tensor> block_table, std::optional<torch::Tensor> q_lens,
+                     std::optional<torch::Tensor> alibi_slopes, bool causal, std::optional<torch::Tensor> lse,
+                     std::optional<torch::Tensor> key_weights, double decay, const std::string &algo, int64_t max_kv_len) {
+  TORCH_CHECK(q.dim() == 4 && output.dim() == 4, "paged: q must be [batch, q_len, n_heads, head_dim]");
+  TORCH_CHECK(output.scalar_type() == q.scalar_type() && output.sizes() == q.sizes(),
+              "output must have the shape and dtype of q");
+  TORCH_CHECK(q.is_cuda() && output.is_cuda() && q.device() == output.device() && q.device() == k_cache.device(),
+              "q, output and the cache must be on one CUDA device");
+  TORCH_CHECK(output.stride(-1) == 1, "output must have a unit stride on head_dim");
+  TORCH_CHECK(k_cache.dim() == 4 && q.scalar_type() == k_cache.scalar_type() && q.size(3) == k_cache.size(3),
+              "paged: q must have the cache's dtype and head_dim");
+  if (q.stride(-1) != 1) q = q.contiguous();
+  const int64_t B = q.size(0), Sq = q.size(1), H = q.size(2), D = q.size(3);
+  if (q.numel() == 0) {
+    TORCH_CHECK(!key_weights.has_value(), "paged: key_weights need query rows");
+    return;
+  }
+  TORCH_CHECK(B <= INT32_MAX && Sq <= INT32_MAX && H <= INT32_MAX, "paged: the sizes of q must fit 31 bits");
+  const c10::cuda::CUDAGuard guard(q.device());
+  torch::Tensor keep_table, ql, kl, slopes;
+  const llmx_paged_cache c = paged_cache(k_cache, v_cache, B, block_table, key_weights, keep_table);
+  llmx_attn_params p;
+  check_status(llmx_attn_params_init(&p));
+  p.dtype = c.dtype;
+  p.batch = (int32_t)B;
+  p.n_heads = (int32_t)H;
+  p.n_kv_heads = c.n_kv_heads;
+  p.head_dim = (int32_t)D;
+  p.max_q_len = (int32_t)Sq;
+  const int64_t room = (int64_t)c.max_pages * c.page_size;
+  TORCH_CHECK(max_kv_len <= room, "max_kv_len must be at most max_pages * page_size");
+  p.max_kv_len = (int32_t)std::min<int64_t>(max_kv_len > 0 ? max_kv_len : room, INT32_MAX);
+  p.q = q.data_ptr();
+  p.o = output.data_ptr();
+  set_strides(p.q_stride, q, true);
+  set_strides(p.o_stride, output, true);
+  p.q_lens = int_arg("q_lens", q_lens, B, q.device(), ql);
+  p.kv_lens = int_arg("kv_lens", kv_lens, B, q.device(), kl);
+  if (alibi_slopes.has_value()) {
+    TORCH_CHECK(alibi_slopes->is_cuda() && alibi_slopes->device() == q.device(), "alibi_slopes must be on q's device");
+    slopes = alibi_slopes->to(torch::kFloat).contiguous();
+    TORCH_CHECK(slopes.numel() == H, "alibi_slopes must have n_heads elements");
+    p.alibi_slopes = slopes.data_ptr<float>();
+  }
+  if (lse.has_value()) {
+    TORCH_CHECK(lse->scalar_type() == torch::kFloat && lse->is_contiguous() && lse->device() == q.device() &&
+                    lse->dim() == 3 && lse->size(0) == B && lse->size(1) == H && lse->size(2) == Sq,
+                "lse must be contiguous fp32 [batch, n_heads, max_q_len] on q's device");
+    p.lse = lse->data_ptr<float>();
+  }
+  p.sm_scale = (float)sm_scale;
+  p.causal = causal ? 1 : 0;
+  p.sliding_window = (int32_t)std::min<int64_t>(std::max<int64_t>(sliding_window, -1), 1 << 30);
+  p.logits_soft_cap = (float)logits_soft_cap;
+  TORCH_CHECK(algo == "auto" || algo == "decode" || algo == "tcgen05", "paged: algo must be one of auto, decode, tcgen05");
+  p.algo = algo_code(algo);
+  size_t ws_bytes = 0;
+  check_status(llmx_paged_attn_workspace_size(&p, &c, &ws_bytes));
+  torch::Tensor ws;
+  if (ws_bytes > 0) {
+    ws = torch::empty({(int64_t)ws_bytes}, q.options().dtype(torch::kByte));
+    p.workspace = ws.data_ptr();
+    p.workspace_bytes = ws_bytes;
+  }
+  check_status(llmx_paged_attn_fwd(&p, &c, (float)decay, at::cuda::getCurrentCUDAStream(q.device().index()).stream()));
+}
+
+std::tuple<torch::Tensor, torch::Tensor> paged_evict(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor key_weights,
+                                                     int64_t budget, torch::Tensor kv_lens,
+                                                     std::optional<torch::Tensor> block_table, int64_t recent, int64_t sinks,
+                                                     std::optional<torch::Tensor> out_table, std::optional<torch::Tensor> kept,
+                                                     std::optional<torch::Tensor> new_lens, int64_t max_kv_len) {
+  TORCH_CHECK(budget >= 1 && budget <= INT32_MAX && recent >= 0 && recent <= INT32_MAX && sinks >= 0 && sinks <= INT32_MAX,
+              "paged: budget must be >= 1, recent and sinks >= 0");
+  TORCH_CHECK(kv_lens.dim() == 1, "kv_lens must be [batch]");
+  const int64_t B = kv_lens.size(0);
+  torch::Tensor keep_table, keep_out, keep_lens;
+  const llmx_paged_cache c = paged_cache(k_cache, v_cache, B, block_table, key_weights, keep_table);
+  const torch::Device dev = k_cache.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto ints = torch::TensorOptions().dtype(torch::kInt).device(dev);
+  const torch::Tensor out_kept = kept.has_value() ? *kept : torch::empty({B, k_cache.size(1), budget}, ints);
+  const torch::Tensor out_lens = new_lens.has_value() ? *new_lens : torch::empty({B}, ints);
+  TORCH_CHECK(out_kept.scalar_type() == torch::kInt && out_kept.dim() == 3 && out_kept.size(0) == B &&
+                  out_kept.size(1) == k_cache.size(1) && out_kept.size(2) == budget && out_kept.is_contiguous() &&
+                  out_kept.device() == dev,
+              "paged: kept must be contiguous int32 [batch, n_kv_heads, budget] on the cache's device");
+  TORCH_CHECK(out_lens.scalar_type() == torch::kInt && out_lens.dim() == 1 && out_lens.size(0) == B && out_lens.is_contiguous() &&
+                  out_lens.device() == dev,
+              "paged: new_lens must be contiguous int32 [batch] on the cache's device");
+  llmx_paged_evict_params e{};
+  const int64_t room = (int64_t)c.max_pages * c.page_size;
+  TORCH_CHECK(max_kv_len <= room, "max_kv_len must be at most max_pages * page_size");
+  e.batch = (int32_t)B;
+  e.budget = (int32_t)budget;
+  e.recent = (int32_t)recent;
+  e.sinks = (int32_t)sinks;
+  e.max_kv_len = (int32_t)std::min<int64_t>(max_kv_len > 0 ? max_kv_len : room, INT32_MAX);
+  e.kv_lens = int_arg("kv_lens", kv_lens, B, dev, keep_lens);
+  if (out_table.has_value()) {
+    e.out_table = paged_table("out_table", *out_table, B, dev, keep_out);
+    e.out_table_stride = keep_out.stride(0);
+    e.out_pages = (int32_t)keep_out.size(1);
+  }
+  e.kept = out_kept.data_ptr<int32_t>();
+  e.new_lens = out_lens.data_ptr<int32_t>();
+  check_status(llmx_paged_evict(&c, &e, at::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return {out_kept, out_lens};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "llmx attention op on B200 (sm_100a): torch binding over libllmx_attn.so";
   static py::object error_cls = py::module_::import("llmx_b200._lib").attr("LlmxError");
@@ -354,5 +548,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("kv_lens") = py::none(), py::arg("block_table") = py::none(), py::arg("q_lens") = py::none(),
         py::arg("alibi_slopes") = py::none(), py::arg("causal") = true, py::arg("lse") = py::none(),
         py::arg("algo") = "auto", py::arg("max_kv_len") = 0);
+  m.def("paged_store", &paged_store, py::arg("k_cache"), py::arg("v_cache"), py::arg("k"), py::arg("v"), py::kw_only(),
+        py::arg("start") = py::none(), py::arg("lens") = py::none(), py::arg("block_table") = py::none());
+  m.def("paged_attention", &paged_attention, py::arg("output"), py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("sm_scale"), py::arg("sliding_window") = -1, py::arg("logits_soft_cap") = 0.0, py::kw_only(),
+        py::arg("kv_lens") = py::none(), py::arg("block_table") = py::none(), py::arg("q_lens") = py::none(),
+        py::arg("alibi_slopes") = py::none(), py::arg("causal") = true, py::arg("lse") = py::none(),
+        py::arg("key_weights") = py::none(), py::arg("decay") = 1.0, py::arg("algo") = "auto", py::arg("max_kv_len") = 0);
+  m.def("paged_evict", &paged_evict, py::arg("k_cache"), py::arg("v_cache"), py::arg("key_weights"), py::arg("budget"),
+        py::kw_only(), py::arg("kv_lens"), py::arg("block_table") = py::none(), py::arg("recent") = 0, py::arg("sinks") = 0,
+        py::arg("out_table") = py::none(), py::arg("kept") = py::none(), py::arg("new_lens") = py::none(),
+        py::arg("max_kv_len") = 0);
   m.def("abi_version", [] { return llmx_attn_abi_version(); });
 }

@@ -1,0 +1,547 @@
+// Paged 16-bit key/value cache: storing rows, and eviction of the tokens with
+// the least weight.  No counterpart in the reference (it has no cache); the
+// layout and the rules are in include/llmx_attn.h.
+//
+// Store: a copy, bound by HBM on prompts and by its launch on single tokens.
+//
+// Eviction, two launches:
+//   select   a cluster of CTAs per (sequence, kv head) finds the k-th largest
+//            weight by radix (four rounds of 8 bits over the order-preserving
+//            image of the fp32 weights, held in shared memory after one read)
+//            and writes the kept positions in ascending order;
+//   compact  moves the kept rows of K, V and the weights to the front.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "paged.cuh"
+
+namespace llmx_b200 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+llmx_status bad(const char *msg) { return record_error(LLMX_ERR_INVALID_ARGUMENT, msg); }
+bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Whether elements at i * s[0] + j * s[1] + k * s[2] + l (l < inner) are all
+// different, for strides that nest (each one spans what lies inside it).
+bool nested(const long long *s, const long long *n, int dims, long long inner) {
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + dims, [&](int x, int y) { return s[x] < s[y]; });
+  long long span = inner;
+  for (int i = 0; i < dims; ++i) {
+    const int d = order[i];
+    if (n[d] <= 1) continue;
+    if (s[d] < span) return false;
+    span = s[d] * (n[d] - 1) + span;
+  }
+  return true;
+}
+
+// ------------------------------------------------------------------- store
+struct StoreArgs {
+  const void *k, *v;
+  long long ks[3], vs[3];  // batch, row, head
+  const int *start, *lens;
+  int B, rows;
+};
+
+constexpr int kStoreThreads = 256;
+
+// A CTA copies `tokens` rows of one sequence, K and V: a thread moves 16-byte
+// pieces (VEC; single elements where rows are not 16-byte aligned) of the
+// rows' [head][channel] order, so that dense rows are read and pages written in
+// whole lines.  kUnroll pieces of each are in flight a thread.
+template <bool VEC>
+__global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const PagedArgs a, const StoreArgs r, int tokens) {
+  constexpr int kUnroll = 4;
+  using Piece = typename std::conditional<VEC, uint4, uint16_t>::type;
+  constexpr int kPer = sizeof(Piece) / 2;
+  const int per_head = a.D / kPer;
+  const int log_per_head = 31 - __clz(per_head);  // D is a power of two
+  const int pieces = a.Hkv * per_head;
+  for (int b = blockIdx.y; b < r.B; b += gridDim.y) {
+    const int n = clamp_len(r.lens, b, r.rows);
+    const long long first = r.start != nullptr ? r.start[b] : 0;
+    const int lo = blockIdx.x * tokens, hi = min(n, lo + tokens);
+    if (lo >= hi) continue;
+    // Pieces of the CTA's tokens in the order token, head, chunk.
+    const int total = (hi - lo) * pieces;  // tokens * pieces is at most 2^31 - 1 (launch_store)
+    for (int base = threadIdx.x; base < total; base += kStoreThreads * kUnroll) {
+      Piece x[kUnroll], y[kUnroll];
+      long long kd[kUnroll], vd[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int i = base + u * kStoreThreads;
+        kd[u] = -1;
+        if (i < total) {
+          const int t = i / pieces, p = i - t * pieces;
+          const int h = p >> log_per_head, c = (p & (per_head - 1)) * kPer;
+          const long long j = first + lo + t;
+          const int page = j < 0 ? -1 : paged_page(a, b, j / a.page_size);
+          if (j < 0) raise_error(a.err, kDevErrBadPage);
+          if (page >= 0) {
+            const long long off = j % a.page_size;
+            kd[u] = page * a.ks[0] + h * a.ks[1] + off * a.ks[2] + c;
+            vd[u] = page * a.vs[0] + h * a.vs[1] + off * a.vs[2] + c;
+            const long long row = lo + t;
+            x[u] = *reinterpret_cast<const Piece *>(static_cast<const uint16_t *>(r.k) + b * r.ks[0] + row * r.ks[1] +
+                                                    h * r.ks[2] + c);
+            y[u] = *reinterpret_cast<const Piece *>(static_cast<const uint16_t *>(r.v) + b * r.vs[0] + row * r.vs[1] +
+                                                    h * r.vs[2] + c);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (kd[u] >= 0) {
+          *reinterpret_cast<Piece *>(static_cast<uint16_t *>(a.k) + kd[u]) = x[u];
+          *reinterpret_cast<Piece *>(static_cast<uint16_t *>(a.v) + vd[u]) = y[u];
+        }
+    }
+  }
+}
+
+cudaError_t launch_store(const PagedArgs &a, const StoreArgs &r, bool vec, int num_sms, cudaStream_t s) {
+  const long long pieces = (long long)a.Hkv * a.D / (vec ? 8 : 1);
+  // One round of kUnroll pieces a thread, and at least one token.
+  const int tokens = (int)std::max<long long>(1, std::min<long long>(r.rows, kStoreThreads * 4 / pieces));
+  const dim3 grid((r.rows + tokens - 1) / tokens, std::min(r.B, 65535));
+  if (vec)
+    paged_store_kernel<true><<<grid, kStoreThreads, 0, s>>>(a, r, tokens);
+  else
+    paged_store_kernel<false><<<grid, kStoreThreads, 0, s>>>(a, r, tokens);
+  return cudaGetLastError();
+}
+
+// ---------------------------------------------------------------- eviction
+struct EvictArgs {
+  int B, budget, recent, sinks, max_kv;
+  const int *kv_lens;
+  const int *out_table;  // nullable: in place
+  long long out_stride;
+  int out_pages;
+  int *kept, *new_lens;
+};
+
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelHeld = 16384;  // weights of a CTA held in shared memory; more are read again in each round
+
+// The image of a weight under which unsigned order is the order of the
+// weights: the sign bit flipped, or all bits of negative ones.  -0 counts as 0
+// and a NaN as -inf.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) w = -CUDART_INF_F;
+  const uint32_t u = __float_as_uint(w + 0.f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+struct SelShared {
+  uint32_t hist[2][256];
+  uint32_t warp_gt[kSelWarps], warp_eq[kSelWarps];
+  uint32_t gt, eq;              // this CTA's counts, read by the others
+  uint32_t digit, need, taken;  // a round's result
+};
+
+// Cluster `g` of CTAs handles (sequence, kv head) g; CTA `rank` of it the
+// candidates [rank * per, (rank + 1) * per) of positions sinks .. L - recent - 1.
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedArgs a, const EvictArgs e) {
+  extern __shared__ uint32_t held[];
+  __shared__ SelShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+  const int unit = blockIdx.x / ranks;
+  const int b = unit / a.Hkv, h = unit % a.Hkv;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int L = clamp_len(e.kv_lens, b, e.max_kv);
+  const int n = min(L, e.budget);
+  int *kept = e.kept + ((long long)b * a.Hkv + h) * e.budget;
+  const int at = rank * kSelThreads + tid, all = ranks * kSelThreads;
+  for (int i = n + at; i < e.budget; i += all) kept[i] = -1;
+  if (L <= e.budget) {  // the same in all CTAs of the cluster
+    for (int i = at; i < n; i += all) kept[i] = i;
+    return;
+  }
+  for (int i = at; i < e.sinks; i += all) kept[i] = i;
+  for (int i = at; i < e.recent; i += all) kept[n - e.recent + i] = L - e.recent + i;
+  const uint32_t want = n - e.sinks - e.recent;  // of the candidates; fewer than there are
+  if (want == 0) return;
+
+  const int candidates = L - e.sinks - e.recent;
+  const int per = (candidates + ranks - 1) / ranks;
+  const int c0 = min(candidates, rank * per), mine = min(candidates, c0 + per) - c0;
+  auto read = [&](int i) {  // the key of candidate c0 + i
+    const int j = e.sinks + c0 + i;
+    const int page = paged_page(a, b, j / a.page_size);
+    return weight_key(page < 0 ? CUDART_NAN_F : a.w[page * a.ws[0] + h * a.ws[1] + j % a.page_size]);
+  };
+  for (int i = tid; i < min(mine, kSelHeld); i += kSelThreads) held[i] = read(i);
+  auto key = [&](int i) { return i < kSelHeld ? held[i] : read(i); };
+
+  // After round r the top 8 (r + 1) bits of the threshold are `prefix`; `need`
+  // of the candidates with exactly these bits are still to be taken, all with
+  // more are.  Once all with these bits are needed the rest decides nothing.
+  uint32_t prefix = 0, need = want;
+  int shift = 32;
+  bool whole = false;  // all candidates with the prefix are taken
+  for (int round = 0; round < 4 && !whole; ++round) {
+    uint32_t *hist = sh.hist[round & 1];
+    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    const int below = shift - 8;
+    for (int i = tid; i < mine; i += kSelThreads) {
+      const uint32_t k = key(i);
+      if (shift == 32 || (k >> shift) == prefix) atomicAdd(&hist[(k >> below) & 255u], 1u);
+    }
+    cluster.sync();
+    if (warp == 0) {
+      // Lane l has digits 255 - 8 l down to 248 - 8 l, so that a prefix sum over the
+      // lanes counts from the largest digit.
+      uint32_t c[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        c[i] = 0;
+        for (int r = 0; r < ranks; ++r) c[i] += cluster.map_shared_rank(hist, r)[255 - 8 * lane - i];
+        sum += c[i];
+      }
+      uint32_t before = sum;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t o = __shfl_up_sync(0xffffffffu, before, off);
+        if (lane >= off) before += o;
+      }
+      before -= sum;
+      if (before < need && need <= before + sum) {  // one lane
+        int i = 0;
+#pragma unroll
+        for (int d = 0; d < 7; ++d)
+          if (i == d && before + c[d] < need) {
+            before += c[d];
+            ++i;
+          }
+        uint32_t ci = c[0];
+#pragma unroll
+        for (int d = 1; d < 8; ++d) ci = i == d ? c[d] : ci;
+        sh.digit = 255 - 8 * lane - i;
+        sh.need = need - before;
+        sh.taken = ci == need - before;
+      }
+    }
+    __syncthreads();
+    prefix = (prefix << 8) | sh.digit;
+    need = sh.need;
+    whole = sh.taken != 0;
+    shift = below;
+    // The other histogram is cleared next; this one only after every CTA has
+    // passed the next round's cluster barrier, and so has read it.
+  }
+
+  // Positions: a candidate above the threshold is taken, and of those with the
+  // threshold's bits the first `need` ones.  Warp w has a contiguous part of the
+  // CTA's candidates, so one pass counts and a second one writes.
+  const int part = ((mine + kSelThreads - 1) / kSelThreads) * 32;
+  const int w0 = min(mine, warp * part), w1 = min(mine, w0 + part);
+  auto classify = [&](int i, bool &gt, bool &eq) {
+    gt = eq = false;
+    if (i < w1) {
+      const uint32_t top = shift == 0 ? key(i) : key(i) >> shift;
+      gt = top > prefix;
+      eq = top == prefix;
+    }
+  };
+  uint32_t gt_n = 0, eq_n = 0;
+  for (int i = w0; i < w1; i += 32) {
+    bool gt, eq;
+    classify(i + lane, gt, eq);
+    gt_n += __popc(__ballot_sync(0xffffffffu, gt));
+    eq_n += __popc(__ballot_sync(0xffffffffu, eq));
+  }
+  if (lane == 0) {
+    sh.warp_gt[warp] = gt_n;
+    sh.warp_eq[warp] = eq_n;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t g = 0, q = 0;
+    for (int w = 0; w < kSelWarps; ++w) {
+      const uint32_t gw = sh.warp_gt[w], qw = sh.warp_eq[w];
+      sh.warp_gt[w] = g;
+      sh.warp_eq[w] = q;
+      g += gw;
+      q += qw;
+    }
+    sh.gt = g;
+    sh.eq = q;
+  }
+  cluster.sync();
+  uint32_t g0 = sh.warp_gt[warp], q0 = sh.warp_eq[warp];
+  for (int r = 0; r < rank; ++r) {
+    const SelShared *o = cluster.map_shared_rank(&sh, r);
+    g0 += o->gt;
+    q0 += o->eq;
+  }
+  const uint32_t lt = (1u << lane) - 1u;
+  for (int i = w0; i < w1; i += 32) {
+    bool gt, eq;
+    classify(i + lane, gt, eq);
+    const uint32_t gm = __ballot_sync(0xffffffffu, gt), qm = __ballot_sync(0xffffffffu, eq);
+    const uint32_t g = g0 + __popc(gm & lt), q = q0 + __popc(qm & lt);
+    if (gt || (eq && q < need)) kept[e.sinks + g + min(q, need)] = e.sinks + c0 + i + lane;
+    g0 += __popc(gm);
+    q0 += __popc(qm);
+  }
+  cluster.sync();  // no CTA leaves while another reads its counts
+}
+
+constexpr int kMoveThreads = 256;
+
+// Moves columns [first, first + width) of the kept rows of one of K, V and the
+// weights of a (sequence, kv head).  In place row r's source kept[r] >= r, so a
+// CTA that handles all rows of its columns in ascending order may write a
+// batch once it has read that batch: what later batches read lies behind it.
+// Different columns never meet, which is what spreads a unit over CTAs.  To
+// other pages there is no order to keep and the rows are spread as well.
+struct MoveArgs {
+  int pieces;      // 16-byte pieces of a K or V row that one CTA moves
+  int chunk_rows;  // rows of one CTA
+  int chunks;      // CTAs along the rows
+  int col_ctas;    // CTAs along the columns of K (and of V); the weights have one
+};
+
+template <typename Piece>
+__device__ __forceinline__ void move_rows(const PagedArgs &a, const EvictArgs &e, Piece *base, const long long *st, int b,
+                                          int h, const int *kept, int lo, int hi, int pieces, int col) {
+  constexpr int kUnroll = 8;
+  const bool in_place = e.out_table == nullptr;
+  const int per_pass = kMoveThreads / pieces;  // rows
+  const int row = threadIdx.x / pieces, c = col + threadIdx.x % pieces;
+  const bool idle = row >= per_pass;
+  Piece *const head = base + h * st[1] + c;
+  for (int r0 = lo; r0 < hi; r0 += per_pass * kUnroll) {
+    Piece x[kUnroll];
+    long long to[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int r = r0 + u * per_pass + row;
+      to[u] = -1;
+      if (idle || r >= hi) continue;
+      const int j = kept[r];
+      if (j < 0 || (in_place && j == r)) continue;
+      const int from = paged_page(a, b, j / a.page_size);
+      const int dest = in_place ? paged_page(a, b, r / a.page_size)
+                                : paged_page(a, e.out_table, e.out_stride, e.out_pages, b, r / a.page_size);
+      if (from < 0 || dest < 0) continue;
+      x[u] = head[from * st[0] + (j % a.page_size) * st[2]];
+      to[u] = dest * st[0] + (r % a.page_size) * st[2];
+    }
+    if (in_place) __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (to[u] >= 0) head[to[u]] = x[u];
+  }
+}
+
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const PagedArgs a, const EvictArgs e, const MoveArgs m) {
+  const int cols = 2 * m.col_ctas + 1;
+  const int col = blockIdx.x % cols, rest = blockIdx.x / cols;
+  const int chunk = rest % m.chunks, unit = rest / m.chunks;
+  const int b = unit / a.Hkv, h = unit % a.Hkv;
+  // new_lens may be kv_lens: the minimum is the same before and after its write.
+  const int n = min(clamp_len(e.kv_lens, b, e.max_kv), e.budget);
+  if (col == 2 * m.col_ctas && chunk == 0 && h == 0 && threadIdx.x == 0) e.new_lens[b] = n;
+  const int lo = chunk * m.chunk_rows, hi = min(n, lo + m.chunk_rows);
+  if (lo >= hi) return;
+  const int *kept = e.kept + ((long long)b * a.Hkv + h) * e.budget;
+  if (col == 2 * m.col_ctas) {
+    const long long st[3] = {a.ws[0], a.ws[1], 1};
+    move_rows<float>(a, e, a.w, st, b, h, kept, lo, hi, 1, 0);
+  } else {
+    const bool is_v = col >= m.col_ctas;
+    const long long *s = is_v ? a.vs : a.ks;
+    const long long st[3] = {s[0] / 8, s[1] / 8, s[2] / 8};
+    move_rows<uint4>(a, e, static_cast<uint4 *>(is_v ? a.v : a.k), st, b, h, kept, lo, hi, m.pieces,
+                     (is_v ? col - m.col_ctas : col) * m.pieces);
+  }
+}
+
+cudaError_t launch_evict(const PagedArgs &a, const EvictArgs &e, int num_sms, cudaStream_t s) {
+  const long long units = (long long)e.B * a.Hkv;
+  const int candidates = std::max(0, e.max_kv - e.sinks - e.recent);
+  // CTAs of a cluster: enough that the weights stay in shared memory, and as
+  // many as keep the machine busy when there are few units.
+  int ranks = 1;
+  while (ranks < 8 && (candidates > ranks * kSelHeld || (units * ranks * 2 <= num_sms && candidates > ranks * 1024)))
+    ranks *= 2;
+  const int per = (candidates + ranks - 1) / ranks;
+  const size_t smem = (size_t)std::min(per, kSelHeld) * 4;
+  if (units * ranks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  static std::once_flag once;
+  static cudaError_t attr = cudaSuccess;
+  std::call_once(once, [] {
+    attr = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelHeld * 4);
+  });
+  if (attr != cudaSuccess) return attr;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * ranks));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ranks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t err = cudaLaunchKernelEx(&cfg, evict_select_kernel, a, e);
+  if (err != cudaSuccess) return err;
+
+  MoveArgs m;
+  const int row_pieces = a.D / 8;
+  const int most = std::min(e.budget, e.max_kv);
+  if (e.out_table != nullptr) {
+    m.pieces = row_pieces;
+    m.chunk_rows = kMoveThreads / row_pieces * 8;
+  } else {
+    m.pieces = units * (2 * row_pieces / 4) >= 2LL * num_sms ? 4 : 2;  // 64 bytes; 32 with few units
+    m.chunk_rows = std::max(1, most);
+  }
+  m.col_ctas = row_pieces / m.pieces;
+  m.chunks = std::max(1, (most + m.chunk_rows - 1) / m.chunk_rows);
+  const long long grid = units * m.chunks * (2 * m.col_ctas + 1);
+  if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+  evict_move_kernel<<<(unsigned)grid, kMoveThreads, 0, s>>>(a, e, m);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+llmx_status validate_paged(const llmx_paged_cache *c, int batch, PagedArgs *k) {
+  if (c == nullptr) return bad("paged: cache is NULL");
+  if (c->dtype != LLMX_FP16 && c->dtype != LLMX_BF16)
+    return record_error(LLMX_ERR_UNSUPPORTED, "paged: dtype must be fp16 or bf16");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return record_error(LLMX_ERR_UNSUPPORTED, "paged: head_dim must be 64, 128 or 256");
+  if (c->n_kv_heads < 1 || c->n_kv_heads > 65535) return bad("paged: n_kv_heads must be in [1, 65535]");
+  if (c->page_size < 16 || c->page_size % 16) return bad("paged: page_size must be a multiple of 16");
+  if (c->n_pages < 1 || c->max_pages < 1) return bad("paged: n_pages and max_pages must be >= 1");
+  if ((long long)c->max_pages * c->page_size > (1LL << 30))
+    return bad("paged: max_pages * page_size must be at most 2^30");
+  if (c->k == nullptr || c->v == nullptr || !al16(c->k) || !al16(c->v))
+    return bad("paged: k and v must be non-NULL and 16-byte aligned");
+  const long long extent[3] = {c->n_pages, c->n_kv_heads, c->page_size};
+  long long ks[3], vs[3];
+  for (int i = 0; i < 3; ++i) {
+    ks[i] = c->k_stride[i];
+    vs[i] = c->v_stride[i];
+    // Every offset stays below 2^60 elements.
+    const long long most = (1LL << 58) / extent[i];
+    if (ks[i] < 0 || ks[i] % 8 || ks[i] > most || vs[i] < 0 || vs[i] % 8 || vs[i] > most)
+      return bad("paged: strides of k and v must be >= 0 and multiples of 8");
+  }
+  if (!nested(ks, extent, 3, c->head_dim) || !nested(vs, extent, 3, c->head_dim))
+    return bad("paged: pages, heads and tokens of k and v must not overlap");
+  if (c->block_table != nullptr && c->table_stride < 0) return bad("paged: table_stride must be >= 0");
+  if (c->block_table == nullptr && (long long)batch * c->max_pages > c->n_pages)
+    return bad("paged: without a block table the cache must hold batch * max_pages pages");
+  if (c->key_weights != nullptr) {
+    const long long ws[2] = {c->w_stride[0], c->w_stride[1]};
+    if (!al16(c->key_weights)) return bad("paged: key_weights must be 16-byte aligned");
+    for (int i = 0; i < 2; ++i)
+      if (ws[i] < 0 || ws[i] % 4 || ws[i] > (1LL << 58) / extent[i])
+        return bad("paged: strides of key_weights must be >= 0 and multiples of 4");
+    if (!nested(ws, extent, 2, c->page_size)) return bad("paged: pages and heads of key_weights must not overlap");
+  }
+  k->k = c->k;
+  k->v = c->v;
+  for (int i = 0; i < 3; ++i) {
+    k->ks[i] = ks[i];
+    k->vs[i] = vs[i];
+  }
+  k->table = c->block_table;
+  k->table_stride = c->table_stride;
+  k->w = c->key_weights;
+  k->ws[0] = c->w_stride[0];
+  k->ws[1] = c->w_stride[1];
+  k->n_pages = c->n_pages;
+  k->max_pages = c->max_pages;
+  k->page_size = c->page_size;
+  k->Hkv = c->n_kv_heads;
+  k->D = c->head_dim;
+  k->err = nullptr;
+  return LLMX_OK;
+}
+
+}  // namespace llmx_b200
+
+using namespace llmx_b200;
+
+extern "C" llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv4_rows *rows, void *stream) {
+  if (rows == nullptr) return bad("paged: rows is NULL");
+  if (rows->batch < 0 || rows->max_rows < 0) return bad("paged: batch and max_rows must be >= 0");
+  PagedArgs k;
+  llmx_status st = validate_paged(c, rows->batch, &k);
+  if (st != LLMX_OK) return st;
+  if (rows->batch == 0 || rows->max_rows == 0) return LLMX_OK;
+  if (rows->k == nullptr || rows->v == nullptr) return bad("paged: the rows' k and v must be non-NULL");
+  StoreArgs r;
+  bool vec = al16(rows->k) && al16(rows->v);
+  for (int i = 0; i < 3; ++i) {
+    r.ks[i] = rows->k_stride[i];
+    r.vs[i] = rows->v_stride[i];
+    if (r.ks[i] < 0 || r.vs[i] < 0) return bad("paged: strides must be >= 0");
+    vec = vec && r.ks[i] % 8 == 0 && r.vs[i] % 8 == 0;
+  }
+  r.k = rows->k;
+  r.v = rows->v;
+  r.start = rows->start;
+  r.lens = rows->lens;
+  r.B = rows->batch;
+  r.rows = rows->max_rows;
+  int sms = 0;
+  st = current_device_info(&k.err, &sms);
+  if (st != LLMX_OK) return st;
+  const cudaError_t e = launch_store(k, r, vec, sms, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? LLMX_OK : record_error(LLMX_ERR_CUDA, cudaGetErrorString(e));
+}
+
+extern "C" llmx_status llmx_paged_evict(const llmx_paged_cache *c, const llmx_paged_evict_params *e, void *stream) {
+  if (e == nullptr) return bad("paged evict: params is NULL");
+  if (e->batch < 0) return bad("paged evict: batch must be >= 0");
+  PagedArgs k;
+  llmx_status st = validate_paged(c, e->batch, &k);
+  if (st != LLMX_OK) return st;
+  if (k.w == nullptr) return bad("paged evict: the cache has no key_weights");
+  if (e->budget < 1 || e->recent < 0 || e->sinks < 0 || (long long)e->recent + e->sinks > e->budget)
+    return bad("paged evict: budget must be >= 1 and hold sinks + recent, both >= 0");
+  const long long room = (long long)k.max_pages * k.page_size;
+  if (e->max_kv_len < 1 || e->max_kv_len > room)
+    return bad("paged evict: max_kv_len must be in [1, max_pages * page_size]");
+  if (e->batch == 0) return LLMX_OK;
+  if (e->kv_lens == nullptr || e->kept == nullptr || e->new_lens == nullptr)
+    return bad("paged evict: kv_lens, kept and new_lens must be non-NULL");
+  EvictArgs a;
+  a.B = e->batch;
+  a.budget = e->budget;
+  a.recent = e->recent;
+  a.sinks = e->sinks;
+  a.max_kv = e->max_kv_len;
+  a.kv_lens = e->kv_lens;
+  a.out_table = e->out_table;
+  a.out_stride = e->out_table_stride;
+  a.out_pages = e->out_pages;
+  a.kept = e->kept;
+  a.new_lens = e->new_lens;
+  if (a.out_table != nullptr) {
+    if (a.out_pages < 1 || a.out_stride < 0) return bad("paged evict: out_pages must be >= 1 and its stride >= 0");
+    if ((long long)a.out_pages * k.page_size < std::min(a.budget, a.max_kv))
+      return bad("paged evict: out_table must hold min(budget, max_kv_len) tokens a sequence");
+  }
+  int sms = 0;
+  st = current_device_info(&k.err, &sms);
+  if (st != LLMX_OK) return st;
+  const cudaError_t err = launch_evict(k, a, sms, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? LLMX_OK : record_error(LLMX_ERR_CUDA, cudaGetErrorString(err));
+}
