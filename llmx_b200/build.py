@@ -31,7 +31,8 @@ NVCC_FLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
 # the C++ Tensor / attention API units export their whole public surface.
 HIDDEN = ["-Xcompiler", "-fvisibility=hidden"]
 SOURCES = ["attn_api.cu", "attn_simt.cu", "attn_decode.cu", "attn_sm100.cu", "attn_merge.cu", "attn_kv4.cu",
-           "kv4_cache.cu", "attn_paged.cu", "paged_cache.cu", "llmx_convert.cu",
+           "kv4_cache.cu", "attn_paged.cu", "attn_paged_tc.cu",
+           "paged_cache.cu", "llmx_convert.cu",
            "llmx_tensor.cu", "attention_api.cu", "llmx_ops.cu"]
 # The C++ Tensor / attention / registry units; every other unit is compiled hidden.
 CXX_API_UNITS = ("llmx_tensor.cu", "attention_api.cu", "llmx_ops.cu")

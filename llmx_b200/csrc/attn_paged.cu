@@ -42,6 +42,8 @@ using sm100::smem_u32;
 constexpr int kThreads = 128;
 constexpr int kWarps = 4;
 constexpr int kStep = 64;  // tokens of a step
+constexpr int kStepRows = 64;  // AUTO: packed rows of a kv head up to which this form is taken
+constexpr size_t kCounterBytes = 256;
 
 // fp16 weights are taken 2^10 times as large: a weight 2^-24 of the largest
 // still has 10 bits then; bf16 has the exponents of fp32.
@@ -60,7 +62,7 @@ struct StepWork {
   int split;      // 0: CTA i has unit i whole
   float *part_o;  // [2 workers][rows of a block][D]
   float *part_ml;  // [2 workers][rows of a block][2]
-  float *stat;     // nullable [units][rows of a block]: log2 of the sum of 2^score
+  float *stat;     // nullable [B * Hkv][R]: log2 of the sum of 2^score
   float *score;    // nullable [B * Hkv][R][pitch], log2 units
   long long pitch;
   float decay;
@@ -540,7 +542,6 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D>::kCtas)
     }
     if (kg == 0) {
       const bool whole = part0 == 0 && part1 == sp.steps();
-      const long long unit = ((long long)cur.b * a.Hkv + cur.kvh) * wk.nrb + cur.rb;
       const long long slot = 2LL * worker + (part0 == 0 ? 1 : 0);
 #pragma unroll
       for (int rr = 0; rr < 2; ++rr) {
@@ -559,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D>::kCtas)
             if (a.lse != nullptr)
               a.lse[((long long)cur.b * a.H + h) * a.Sq + i] =
                   sees ? lse2 * kPagedLn2 + (a.alibi != nullptr ? a.alibi[h] * (float)ref[rr] : 0.f) : -CUDART_INF_F;
-            if (wk.stat != nullptr) wk.stat[unit * kRows + in_block] = lse2;
+            if (wk.stat != nullptr) wk.stat[((long long)cur.b * a.Hkv + cur.kvh) * wk.R + r] = lse2;
           }
         } else {
           float *po = wk.part_o + (slot * kRows + in_block) * D + 2 * t;
@@ -654,7 +655,7 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
         a.lse[((long long)b * a.H + h) * a.Sq + i] =
             sees ? lse2 * kPagedLn2 + (a.alibi != nullptr ? slope * (float)alibi_ref(v, slope) : 0.f) : -CUDART_INF_F;
       }
-      if (wk.stat != nullptr) wk.stat[(long long)unit * rows + in_block] = lse2;
+      if (wk.stat != nullptr) wk.stat[((long long)b * a.Hkv + kvh) * wk.R + r] = lse2;
     }
   }
 }
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
 // sum over rows of 2^(score - lse2).  A thread has four tokens.
 constexpr int kWeightRows = 64;  // rows whose sums lie in shared memory at a time
 __global__ void __launch_bounds__(kThreads) paged_weights_kernel(const __grid_constant__ AttnArgs a,
-                                                                  const __grid_constant__ StepWork wk, int rows) {
+                                                                  const __grid_constant__ StepWork wk) {
   __shared__ float lse2[kWeightRows];
   __shared__ Visible vis[kWeightRows];
   const int unit = blockIdx.y;
@@ -679,7 +680,7 @@ __global__ void __launch_bounds__(kThreads) paged_weights_kernel(const __grid_co
     const int n = min(kWeightRows, R - r0);
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const int r = r0 + i;
-      lse2[i] = wk.stat[((long long)unit * wk.nrb + r / rows) * rows + r % rows];
+      lse2[i] = wk.stat[(long long)unit * wk.R + r];
       vis[i] = row_visible(a, r / a.group, ql, kl);
     }
     __syncthreads();
@@ -719,36 +720,21 @@ struct StepPlan {
 
 int ctas_of(int D) { return D == 64 ? StepCfg<64>::kCtas : (D == 128 ? StepCfg<128>::kCtas : StepCfg<256>::kCtas); }
 
-size_t up16(size_t n) { return (n + 255) / 256 * 256; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 StepPlan plan_step(const AttnArgs &a, bool weights) {
   StepPlan p{};
   const long long R = (long long)a.Sq * a.group;
   p.rt = R <= 16 ? 1 : (R <= 32 ? 2 : 4);
   const int rows = 16 * p.rt;
-  const long long units = (long long)a.B * a.Hkv * ((R + rows - 1) / rows);
   p.workers = a.num_sms * ctas_of(a.D);
   // Up to four steps a unit there is too little to share.
   p.split = a.Skv > 4 * kStep;
-  p.part_bytes = p.split ? up16((size_t)2 * p.workers * rows * (a.D + 2) * sizeof(float)) : 0;
-  p.stat_bytes = weights ? up16((size_t)units * rows * sizeof(float)) : 0;
+  p.part_bytes = p.split ? up256((size_t)2 * p.workers * rows * (a.D + 2) * sizeof(float)) : 0;
+  p.stat_bytes = weights ? up256((size_t)a.B * a.Hkv * R * sizeof(float)) : 0;
   p.pitch = ((long long)a.Skv + 15) / 16 * 16;
-  p.score_bytes = weights ? up16((size_t)a.B * a.Hkv * R * p.pitch * sizeof(float)) : 0;
+  p.score_bytes = weights ? up256((size_t)a.B * a.Hkv * R * p.pitch * sizeof(float)) : 0;
   return p;
-}
-
-template <typename K, typename... Args>
-cudaError_t launch_after(K kernel, dim3 grid, cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <typename T, int D, int RT>
@@ -764,10 +750,10 @@ cudaError_t launch_step_t(const AttnArgs &a, const StepWork &wk, long long units
   kern<<<grid, kThreads, StepCfg<D>::kSmem, s>>>(a, wk);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (wk.split) e = launch_after(paged_merge_kernel<T, D>, dim3((unsigned)units), s, a, wk, 16 * RT);
+  if (wk.split) e = launch_paged_after(paged_merge_kernel<T, D>, dim3((unsigned)units), s, a, wk, 16 * RT);
   if (e != cudaSuccess || wk.score == nullptr) return e;
   const dim3 grid_w((unsigned)((a.Skv + kThreads * 4 - 1) / (kThreads * 4)), (unsigned)(a.B * a.Hkv));
-  return launch_after(paged_weights_kernel, grid_w, s, a, wk, 16 * RT);
+  return launch_paged_after(paged_weights_kernel, grid_w, s, a, wk);
 }
 
 template <typename T, int D>
@@ -828,8 +814,6 @@ llmx_status prepare(const llmx_attn_params *p, const llmx_paged_cache *c, AttnAr
     return bad("paged attention: max_kv_len must be at most max_pages * page_size");
   if ((long long)a->Sq * a->group > (1LL << 30)) return bad("paged attention: max_q_len * group must be at most 2^30");
   if (p->algo == LLMX_ALGO_SIMT) return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: algo must be AUTO, DECODE or TCGEN05");
-  if (p->algo == LLMX_ALGO_TCGEN05)
-    return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: TCGEN05 needs sm_scale > 0");
   if ((reinterpret_cast<uintptr_t>(a->q) & 15u) || (reinterpret_cast<uintptr_t>(a->o) & 15u))
     return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: q and o must be 16-byte aligned");
   const int extent[3] = {a->B, a->Sq, a->H};
@@ -842,6 +826,31 @@ llmx_status prepare(const llmx_attn_params *p, const llmx_paged_cache *c, AttnAr
   if (blocks > INT_MAX / 2 || (k->w != nullptr && (long long)a->B * a->Hkv > 65535))
     return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: too many sequences, heads and rows for one call");
   a->window = std::min(a->window, 1 << 30);
+  return LLMX_OK;
+}
+
+// A request's form and its workspace: [work counter][partial results][the
+// rows' sums][scores].
+struct Plan {
+  bool tc;
+  StepPlan step;
+  PagedTcPlan tcp;
+  size_t bytes;
+};
+
+llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs &k, Plan *plan) {
+  const bool can = paged_tc_supports(a, k) && k.w == nullptr;
+  if (p->algo == LLMX_ALGO_TCGEN05 && !can)
+    return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: TCGEN05 needs head_dim 64 or 128, sm_scale > 0 and at most 128 "
+                                              "query heads a kv head");
+  plan->tc = can && (p->algo == LLMX_ALGO_TCGEN05 || (p->algo == LLMX_ALGO_AUTO && (long long)a.Sq * a.group > kStepRows));
+  if (plan->tc) {
+    plan->tcp = plan_paged_tc(a, true);
+    plan->bytes = kCounterBytes + plan->tcp.part_bytes;
+  } else {
+    plan->step = plan_step(a, k.w != nullptr);
+    plan->bytes = plan->step.part_bytes + plan->step.stat_bytes + plan->step.score_bytes;
+  }
   return LLMX_OK;
 }
 
@@ -859,9 +868,10 @@ extern "C" llmx_status llmx_paged_attn_workspace_size(const llmx_attn_params *p,
   unsigned int *err = nullptr;
   int sms = 0;
   if (current_device_info(&err, &sms) == LLMX_OK) a.num_sms = sms;
-  const StepPlan plan = plan_step(a, k.w != nullptr);
-  *bytes = plan.part_bytes + plan.stat_bytes + plan.score_bytes;
-  return LLMX_OK;
+  Plan plan;
+  const llmx_status st = choose(p, a, k, &plan);
+  if (st == LLMX_OK) *bytes = plan.bytes;
+  return st;
 }
 
 extern "C" llmx_status llmx_paged_attn_fwd(const llmx_attn_params *p, const llmx_paged_cache *c, float decay, void *stream) {
@@ -871,17 +881,31 @@ extern "C" llmx_status llmx_paged_attn_fwd(const llmx_attn_params *p, const llmx
   if (s != LLMX_OK) return s;
   if (k.w != nullptr && !(decay >= 0.f && decay <= 3.4e38f)) return bad("paged attention: decay must be finite and >= 0");
   if (reinterpret_cast<uintptr_t>(p->workspace) & 15u) return bad("paged attention: workspace must be 16-byte aligned");
+  Plan plan;
+  s = choose(p, a, k, &plan);
+  if (s != LLMX_OK) return s;
   s = current_device_info(&a.err, &a.num_sms);
   if (s != LLMX_OK) return s;
   k.err = a.err;
-  StepPlan plan = plan_step(a, k.w != nullptr);
+  s = choose(p, a, k, &plan);  // with the device's SM count
+  if (s != LLMX_OK) return s;
   const size_t have = p->workspace != nullptr ? p->workspace_bytes : 0;
-  if (have < plan.part_bytes + plan.stat_bytes + plan.score_bytes) {
+  if (have < plan.bytes) {
     if (k.w != nullptr)
       return record_error(LLMX_ERR_WORKSPACE_TOO_SMALL, "paged attention: key_weights need the workspace");
-    plan.split = false;
-    plan.part_bytes = 0;
+    plan.step.split = false;
+    plan.step.part_bytes = 0;
+    if (plan.tc) plan.tcp = plan_paged_tc(a, false);
   }
-  const cudaError_t e = launch_step(a, k, plan, decay, p->workspace, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (plan.tc) {
+    unsigned char *ws = static_cast<unsigned char *>(p->workspace);
+    int *const ctr = have >= kCounterBytes ? reinterpret_cast<int *>(ws) : nullptr;
+    float *const part = plan.tcp.part_bytes > 0 ? reinterpret_cast<float *>(ws + kCounterBytes) : nullptr;
+    e = launch_paged_tc(a, k, plan.tcp, ctr, part, nullptr, st);
+  } else {
+    e = launch_step(a, k, plan.step, decay, p->workspace, st);
+  }
   return e == cudaSuccess ? LLMX_OK : record_error(LLMX_ERR_CUDA, cudaGetErrorString(e));
 }

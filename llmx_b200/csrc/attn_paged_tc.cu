@@ -1,0 +1,893 @@
+// Attention over a paged 16-bit key/value cache on the tensor cores: chunks of
+// query rows (more than 64 rows of a kv head), head_dim 64 and 128.
+//
+// The scheme is the dense prefill's (attn_sm100.cu): a CTA has two tiles of up
+// to 128 rows, S = Q K^T and O += P V on tcgen05.mma with both accumulators in
+// tensor memory, a softmax warpgroup for each tile, lazy rescaling.  What is
+// different:
+//
+//  * Rows are packed: a tile has M = (128 / group) * group rows, all query heads
+//    of a kv head for 128 / group query rows (one TMA box over [head][row]), so
+//    that K and V go through shared memory once for the whole group.
+//  * K and V come by pages: a 128-key block is made of boxes of
+//    gcd(page_size, 128) rows, one lane of the TMA warp each, whose pages are
+//    looked up a block ahead.  Boxes behind the sequence (and pages outside the
+//    cache) are loaded from a page index outside the tensor map, which fills
+//    zeros: nothing there is read, and the byte count stays the same.
+//  * One warp passes V blocks on to the MMA thread.  In blocks that not every
+//    row sees whole it first writes zeros over the rows behind the sequence's
+//    length and over infinities and NaN (0 * NaN would reach the rows that do
+//    not see the token); a bit for each token that lost a value goes to the
+//    softmax threads, and rows that see such a token become NaN.
+//  * ALiBi: the folded slope (x_offset) is a row's own, and biases count from
+//    the row's largest one (alibi_ref).
+//  * Work: items (a unit's pair of tiles) longest first over one CTA an SM; the
+//    items of the last, part-filled wave are cut along the keys into `parts`
+//    pieces, whose partial results a second launch merges.
+#include <algorithm>
+#include <climits>
+#include <numeric>
+
+#include "paged_attn.cuh"
+#include "sm100_fmha.cuh"
+
+namespace llmx_b200 {
+namespace {
+
+constexpr int kVWarp = 10;     // passes V blocks on
+constexpr int kSlopeWarp = 11; // writes A' (ALiBi)
+constexpr int kConsumers = 1 + 8 + 2;
+constexpr int kItemRows = kTiles * kBM;
+
+template <typename T>
+constexpr int tc_shift() {
+  return std::is_same<T, __half>::value ? 10 : 0;
+}
+
+// A launch's items.
+struct TcWork {
+  PagedArgs c;
+  int R;            // packed rows of a kv head
+  int M;            // rows of a tile
+  int n_mblocks;    // items of a unit
+  int group_units;  // units whose K / V fit in L2 together
+  int n_whole;      // items [0, n_whole) are whole, the others in `parts` pieces
+  int parts;
+  int n_work;
+  int box;         // tokens of a TMA box
+  float *part_o;   // [pieces][256][D]
+  float *part_ml;  // [pieces][256][2]
+  float *stat;     // nullable [units][R]: log2 of the sum of 2^score
+};
+
+struct Item {
+  int b, kvh, ql, kl, m0;
+  BlockRange br;
+  int nb0;   // blocks that tile 0 takes part in, >= 1
+  int slot;  // of its partial result, or -1: whole
+};
+
+struct PBars {
+  uint64_t q_full[2], q_empty[2];
+  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
+  uint64_t s_full[2], p_full[2], o_done[2];
+  uint64_t v_landed[3];  // V's copy has arrived; v_full: the V warp has passed it on
+  uint64_t drain;
+  uint64_t sched_full[kSchedSlots], sched_empty[kSchedSlots];
+  int sched_w[kSchedSlots];
+  Item sched_item[kSchedSlots];
+  uint32_t lost[3][4];  // tokens of the stage's V block that lost a value
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+static_assert(sizeof(PBars) <= 1024, "barriers");
+
+// The tokens that rows [m0, m0 + n) of a sequence see: some row [lo, hi), every
+// row [all_lo, all_hi).
+struct RowsSee {
+  int lo, hi, all_lo, all_hi;
+};
+__device__ __forceinline__ RowsSee rows_see(const AttnArgs &a, int m0, int n, int ql, int kl) {
+  RowsSee s{0, 0, 0, 0};
+  const int i0 = m0 / a.group;
+  if (i0 >= ql) return s;
+  const int i1 = min(ql - 1, (m0 + n - 1) / a.group);
+  const Visible f = row_visible(a, i0, ql, kl), l = row_visible(a, i1, ql, kl);
+  s.lo = f.lo;
+  s.hi = max(0, l.hi);
+  s.all_lo = l.lo;
+  s.all_hi = f.hi;
+  return s;
+}
+// Whether some row of them does not see the whole block.
+__device__ __forceinline__ bool partly(const RowsSee &s, int n0) { return n0 < s.all_lo || n0 + kBN > s.all_hi; }
+
+// Work item w: units in groups whose K / V fit in L2 together, inside a group the
+// last rows (which see the most keys) first, as in the dense prefill.
+__device__ __forceinline__ Item decode_item(const AttnArgs &a, const TcWork &wk, int w) {
+  Item t;
+  int idx = w, part = 0, parts = 1;
+  t.slot = -1;
+  if (w >= wk.n_whole && wk.parts > 1) {
+    t.slot = w - wk.n_whole;
+    idx = wk.n_whole + t.slot / wk.parts;
+    part = t.slot % wk.parts;
+    parts = wk.parts;
+  }
+  const int units = a.B * a.Hkv;
+  const int per_group = wk.group_units * wk.n_mblocks;
+  const int g = idx / per_group, within = idx - g * per_group;
+  const int gu = min(wk.group_units, units - g * wk.group_units);
+  const int rank = within / gu, unit = g * wk.group_units + within % gu;
+  const int mblk = a.causal ? wk.n_mblocks - 1 - rank : rank;
+  t.kvh = unit % a.Hkv;
+  t.b = unit / a.Hkv;
+  t.ql = clamp_len(a.q_lens, t.b, a.Sq);
+  t.kl = clamp_len(a.kv_lens, t.b, a.Skv);
+  t.m0 = mblk * 2 * wk.M;
+  const RowsSee s = rows_see(a, t.m0, 2 * wk.M, t.ql, t.kl);
+  const int lo = s.lo / kBN * kBN;
+  int nb = s.hi > s.lo ? (s.hi - lo + kBN - 1) / kBN : 0;
+  int nb0 = nb;
+  if (nb > 0) {
+    const RowsSee s0 = rows_see(a, t.m0, wk.M, t.ql, t.kl);
+    nb0 = (max(s0.hi, lo) - lo + kBN - 1) / kBN;
+  }
+  const int p0 = (int)((long long)nb * part / parts), p1 = (int)((long long)nb * (part + 1) / parts);
+  t.br.n_start = lo + p0 * kBN;
+  t.br.nb = p1 - p0;
+  t.nb0 = min(t.br.nb, max(min(1, t.br.nb), nb0 - p0));
+  return t;
+}
+
+__device__ __forceinline__ bool publish(PBars *bars, int n, int w, const Item &t) {
+  const int slot = n % kSchedSlots;
+  if (n >= kSchedSlots &&
+      !mbar_wait_or_abort(&bars->sched_empty[slot], ((n / kSchedSlots) - 1) & 1, kTimeoutNs, &bars->abort_flag))
+    return false;
+  bars->sched_w[slot] = w;
+  bars->sched_item[slot] = t;
+  mbar_arrive(&bars->sched_full[slot]);  // release: orders the stores above
+  return true;
+}
+
+// The n-th item for a consumer role (w >= n_work: the end), or -1 on abort.
+__device__ __forceinline__ int take(PBars *bars, int n, bool warp_wide, Item &t) {
+  const int slot = n % kSchedSlots;
+  bool ok = mbar_wait_or_abort(&bars->sched_full[slot], (n / kSchedSlots) & 1, kTimeoutNs, &bars->abort_flag);
+  if (warp_wide) ok = __all_sync(0xffffffffu, ok);
+  if (!ok) return -1;
+  const int w = *reinterpret_cast<volatile int *>(&bars->sched_w[slot]);
+  t = bars->sched_item[slot];
+  if (warp_wide) __syncwarp();
+  if (!warp_wide || (threadIdx.x % 32) == 0) mbar_arrive(&bars->sched_empty[slot]);
+  return w;
+}
+
+// ---------------------------------------------------------------- TMA warp
+// Loads of one item: Q tile 0, then per key block K (and after the first K, Q
+// tile 1) and V.  Lane i < 128 / box has box i of a block.
+struct Loads {
+  int k = 0, v = 0, q[2] = {0, 0};
+};
+
+template <int D, bool kReverse>
+__device__ bool load_item(const CUtensorMap *tm_q, const CUtensorMap *tm_k, const CUtensorMap *tm_v, uint8_t *smem, PBars *bars,
+                          const AttnArgs &a, const TcWork &wk, const Item &t, int tile_it, int kv_base, Loads &n) {
+  using C = Cfg<D>;
+  const int lane = threadIdx.x % 32;
+  const int boxes = kBN / wk.box;
+  auto wait = [&](uint64_t *bar, uint32_t par) {
+    const bool ok = mbar_wait_or_abort(bar, par, kTimeoutNs, &bars->abort_flag);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
+  auto load_q = [&](int q) {
+    if (tile_it > 0 && !wait(&bars->q_empty[q], (tile_it - 1) & 1)) return false;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&bars->q_full[q], C::kChunks * wk.M * 128);
+      for (int c = 0; c < C::kChunks; ++c)
+        tma_load_4d(smem + C::kQOff + q * C::kTileBytes + c * C::kChunkBytes, tm_q, &bars->q_full[q], c * 64, t.kvh * a.group,
+                    (t.m0 + q * wk.M) / a.group, t.b);
+    }
+    n.q[q] = tile_it + 1;
+    return true;
+  };
+  // Where this lane's box of the block at n0 lies; a page index of n_pages reads as zeros.
+  struct Place {
+    int page, row;
+  };
+  auto place = [&](int n0) {
+    Place p{wk.c.n_pages, 0};
+    const int j = n0 + lane * wk.box;
+    if (lane < boxes && j < t.kl) {
+      const int slot = j / wk.c.page_size;
+      const int id = paged_page(wk.c, t.b, slot);
+      if (id >= 0) {
+        p.page = id;
+        p.row = j - slot * wk.c.page_size;
+      }
+    }
+    return p;
+  };
+  auto load_block = [&](uint8_t *dst, const CUtensorMap *tm, uint64_t *bar, const Place &p) {
+    if (lane == 0) mbar_arrive_expect_tx(bar, C::kTileBytes);
+    __syncwarp();
+    if (lane < boxes)
+      for (int c = 0; c < C::kChunks; ++c)
+        tma_load_4d(dst + c * C::kChunkBytes + lane * wk.box * 128, tm, bar, c * 64, p.row, t.kvh, p.page);
+  };
+  Place next = place(block_n0<kReverse>(t.br, 0));
+  if (!load_q(0)) return false;
+  for (int j = 0; j < t.br.nb; ++j) {
+    const int g = kv_base + j;
+    const int s = g % C::kStages;
+    const uint32_t par = ((g / C::kStages) & 1) ^ 1;
+    const Place p = next;
+    if (j + 1 < t.br.nb) next = place(block_n0<kReverse>(t.br, j + 1));
+    if (!wait(&bars->k_empty[s], par)) return false;
+    load_block(smem + C::kKOff + s * C::kTileBytes, tm_k, &bars->k_full[s], p);
+    n.k = g + 1;
+    if (j == 0 && !load_q(1)) return false;
+    if (!wait(&bars->v_empty[s], par)) return false;
+    load_block(smem + C::kVOff + s * C::kTileBytes, tm_v, &bars->v_landed[s], p);
+    n.v = g + 1;
+  }
+  return true;
+}
+
+// Every load issued must have landed before the CTA may exit.
+template <int D>
+__device__ void drain_loads(PBars *bars, const Loads &n) {
+  using C = Cfg<D>;
+  for (int q = 0; q < 2; ++q)
+    if (n.q[q] > 0) mbar_wait(&bars->q_full[q], (n.q[q] - 1) & 1, kTimeoutNs);
+  for (int g = max(0, n.k - C::kStages); g < n.k; ++g)
+    mbar_wait(&bars->k_full[g % C::kStages], (g / C::kStages) & 1, kTimeoutNs);
+  for (int g = max(0, n.v - C::kStages); g < n.v; ++g)
+    mbar_wait(&bars->v_landed[g % C::kStages], (g / C::kStages) & 1, kTimeoutNs);
+}
+
+// ------------------------------------------------------------------ V warp
+// Lane l has rows l, l + 32, .. of the block.  16-byte chunk c of row r lies at
+// chunk c ^ (r % 8) of its 128 bytes, so lanes that take the same c do not meet
+// in a bank.
+template <typename T, int D>
+__device__ void clean_block(uint8_t *v, uint32_t (&lost)[4], int rows) {
+  using C = Cfg<D>;
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  const int lane = threadIdx.x % 32;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 32 + lane;
+    bool bad = false;
+    uint8_t *row = v + r * 128;
+    if (r >= rows) {
+      for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<uint4 *>(row + c * C::kChunkBytes + ((k ^ (r & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          uint4 *at = reinterpret_cast<uint4 *>(row + c * C::kChunkBytes + ((k ^ (r & 7)) << 4));
+          const uint4 x = *at;
+          uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          bool any = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t m = (w[e] & kExp) ^ kExp;  // a half that is 0: all exponent bits set
+            if ((m & 0xffffu) == 0u) {
+              w[e] &= 0xffff0000u;
+              any = true;
+            }
+            if ((m >> 16) == 0u) {
+              w[e] &= 0x0000ffffu;
+              any = true;
+            }
+          }
+          if (any) {
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
+            bad = true;
+          }
+        }
+    }
+    const uint32_t bits = __ballot_sync(0xffffffffu, bad);
+    if (lane == 0) lost[i] = bits;
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// ------------------------------------------------------------ softmax role
+// As softmax_tile of the dense prefill; thread r of warpgroup t has packed row
+// m0 + t M + r.  blk_base: blocks of this tile in earlier items, kv_base: blocks
+// of earlier items.
+template <typename T, int D, bool kAlibi, bool kSoftcap>
+__device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, uint32_t tmem, int warp, const Item &w, int blk_base,
+                             int kv_base) {
+  using C = Cfg<D>;
+  constexpr int kShift = tc_shift<T>();
+  const float kNegInf = -CUDART_INF_F;
+  const int t = warp / 4;
+  BlockRange br = w.br;
+  if (t == 0) br.nb = w.nb0;
+  const int r = threadIdx.x % kBM;
+  const int row0 = w.m0 + t * wk.M;
+  const int pr = row0 + r;
+  const bool real = r < wk.M && pr < wk.R;
+  const int qi = real ? pr / a.group : 0;
+  const int h = w.kvh * a.group + (real ? pr - qi * a.group : 0);
+  const Visible vis = real ? row_visible(a, qi, w.ql, w.kl) : Visible{0, 0};
+  const RowsSee tile = rows_see(a, row0, wk.M, w.ql, w.kl);
+  const RowsSee both = rows_see(a, w.m0, 2 * wk.M, w.ql, w.kl);
+  const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
+  const uint32_t tS = tmem + lane_off + (t ? C::kTmemS1 : C::kTmemS0);
+  const uint32_t tO = tmem + lane_off + (t ? C::kTmemO1 : C::kTmemO0);
+  const float scale2 = a.sm_scale * kLog2e;
+  const float slope = kAlibi ? a.alibi[h] : 0.f;
+  const float slope2 = slope * kLog2e;
+  const int ref = kAlibi ? alibi_ref(vis, slope) : 0;
+  const float cap_in = kSoftcap ? a.sm_scale / a.softcap : 0.f;
+  const float cap_out = kSoftcap ? a.softcap * kLog2e : 0.f;
+  float m_used = kNegInf, l = 0.f;
+  bool aborted = false;
+
+  for (int j = 0; j < br.nb; ++j) {
+    const int n0 = block_n0<kAlibi>(br, j);
+    bool ok = mbar_wait_or_abort(&bars->s_full[t], (blk_base + j) & 1, kTimeoutNs, &bars->abort_flag);
+    if (!__all_sync(0xffffffffu, ok)) {
+      set_abort(bars, a.err);
+      aborted = true;
+      break;
+    }
+    tc_fence_after();
+    const int lo = max(0, vis.lo - n0), hi = min(kBN, vis.hi - n0);
+    const bool need_mask = partly(tile, n0);
+    float alpha = 1.f;
+    bool rescale = false;
+    if (need_mask && __all_sync(0xffffffffu, hi <= lo)) {
+      uint32_t z[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) z[c] = 0u;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tmem_st16(tS + q * 16, z);
+    } else if (need_mask) {
+      softmax_block<T, kAlibi, kSoftcap, true, kShift>(tS, n0 - ref, 0, lo, hi, scale2, slope2, cap_in, cap_out, m_used, l, alpha,
+                                                       rescale);
+    } else {
+      softmax_block<T, kAlibi, kSoftcap, false, kShift>(tS, n0 - ref, 0, lo, hi, scale2, slope2, cap_in, cap_out, m_used, l, alpha,
+                                                        rescale);
+    }
+    if (partly(both, n0)) {
+      // The V warp has looked at this block: a row that sees a token whose
+      // infinity or NaN was taken as 0 is NaN.  (Block index in the item: tile
+      // 0's blocks are the last ones in reverse order.)
+      const int g = kv_base + (kAlibi && t == 0 ? w.br.nb - w.nb0 : 0) + j;
+      const int s = g % C::kStages;
+      ok = mbar_wait_or_abort(&bars->v_full[s], (g / C::kStages) & 1, kTimeoutNs, &bars->abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        set_abort(bars, a.err);
+        aborted = true;
+        break;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t bits = *reinterpret_cast<volatile uint32_t *>(&bars->lost[s][i]);
+        if (bits != 0u) {
+          const int b0 = min(max(lo - i * 32, 0), 32), b1 = min(max(hi - i * 32, 0), 32);
+          const uint32_t below1 = b1 >= 32 ? 0xffffffffu : ((1u << b1) - 1u);
+          const uint32_t below0 = b0 >= 32 ? 0xffffffffu : ((1u << b0) - 1u);
+          if (bits & below1 & ~below0) l = CUDART_NAN_F;
+        }
+      }
+    }
+    if (__any_sync(0xffffffffu, rescale)) {
+      ok = mbar_wait_or_abort(&bars->o_done[t], (blk_base + j - 1) & 1, kTimeoutNs, &bars->abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        set_abort(bars, a.err);
+        aborted = true;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll 1
+      for (int ch = 0; ch < D / 32; ++ch) {
+        uint32_t o[32];
+        tmem_ld32(tO + ch * 32, o);
+        tmem_wait_ld();
+        reg_fence32(o);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+        tmem_st32(tO + ch * 32, o);
+      }
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(&bars->p_full[t]);
+  }
+
+  if (!aborted && br.nb > 0) {
+    bool ok = mbar_wait_or_abort(&bars->o_done[t], (blk_base + br.nb - 1) & 1, kTimeoutNs, &bars->abort_flag);
+    if (!__all_sync(0xffffffffu, ok)) {
+      set_abort(bars, a.err);
+      aborted = true;
+    } else {
+      tc_fence_after();
+    }
+  }
+  const bool have = !aborted && br.nb > 0;
+  if (w.slot >= 0) {
+    // A piece: O and l as they are (P of the row's maximum is 2^kShift).
+    const long long prow = (long long)w.slot * kItemRows + t * kBM + r;
+    float *po = wk.part_o + prow * D;
+#pragma unroll 1
+    for (int ch = 0; ch < D / 32; ++ch) {
+      uint32_t o[32];
+      if (have) {
+        tmem_ld32(tO + ch * 32, o);
+        tmem_wait_ld();
+        reg_fence32(o);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] = 0u;
+      }
+      if (real) {
+#pragma unroll
+        for (int c = 0; c < 32; c += 4)
+          *reinterpret_cast<uint4 *>(po + ch * 32 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+      }
+    }
+    if (real) *reinterpret_cast<float2 *>(wk.part_ml + prow * 2) = make_float2(m_used, l);
+    return !aborted;
+  }
+  const bool sees = vis.hi > vis.lo && have;
+  const float inv = sees ? 1.f / l : 0.f;
+  // As in the dense prefill, groups of four lanes swap pieces so that a store
+  // writes 64 contiguous bytes of 8 rows.
+  const int gi = threadIdx.x & 3;
+  T *to[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int rk = r - gi + k, pk = row0 + rk;
+    to[k] = nullptr;
+    if (rk < wk.M && pk < wk.R) {
+      const int i = pk / a.group;
+      to[k] = static_cast<T *>(a.o) + w.b * a.os[0] + i * a.os[1] + (w.kvh * a.group + pk - i * a.group) * a.os[2] + gi * 8;
+    }
+  }
+#pragma unroll 1
+  for (int ch = 0; ch < D / 32; ++ch) {
+    uint32_t o[32];
+    if (have) {
+      tmem_ld32(tO + ch * 32, o);
+      tmem_wait_ld();
+      reg_fence32(o);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) o[c] = 0u;
+    }
+    uint32_t x[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      x[c] = sees ? pack2<T>(__uint_as_float(o[2 * c]) * inv, __uint_as_float(o[2 * c + 1]) * inv) : 0u;
+    uint4 u[4];
+#pragma unroll
+    for (int v4 = 0; v4 < 4; ++v4) u[v4] = make_uint4(x[4 * v4], x[4 * v4 + 1], x[4 * v4 + 2], x[4 * v4 + 3]);
+    transpose_units4(u);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (to[k] != nullptr) *reinterpret_cast<uint4 *>(to[k] + ch * 32) = u[k];
+  }
+  if (real) {
+    const float lse2 = m_used - (float)kShift + log2f(l);
+    if (a.lse != nullptr)
+      a.lse[((long long)w.b * a.H + h) * a.Sq + qi] = sees ? lse2 * kLn2 + (kAlibi ? slope * (float)ref : 0.f) : kNegInf;
+    if (wk.stat != nullptr) wk.stat[((long long)w.b * a.Hkv + w.kvh) * wk.R + pr] = lse2;
+  }
+  return !aborted;
+}
+
+// ------------------------------------------------------------------ kernel
+template <typename T, int D, bool kAlibi, bool kSoftcap>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnArgs a,
+                    const __grid_constant__ TcWork wk, int *work_ctr) {
+  using C = Cfg<D>;
+  constexpr bool kFold = kAlibi && !kSoftcap;
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  PBars *bars = reinterpret_cast<PBars *>(smem + C::kBarOff);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (threadIdx.x == 0) {
+    for (int q = 0; q < kTiles; ++q) {
+      mbar_init(&bars->q_full[q], kFold ? 2 : 1);
+      mbar_init(&bars->q_empty[q], 1);
+      mbar_init(&bars->s_full[q], 1);
+      mbar_init(&bars->p_full[q], kBM);
+      mbar_init(&bars->o_done[q], 1);
+    }
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->k_empty[s], 1);
+      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->v_landed[s], 1);
+      mbar_init(&bars->v_empty[s], 1);
+    }
+    for (int i = 0; i < kSchedSlots; ++i) {
+      mbar_init(&bars->sched_full[i], 1);
+      mbar_init(&bars->sched_empty[i], kConsumers);
+    }
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if constexpr (kFold) {
+    // B' row c = [c, c, c, 0, ...]; A' zero (its columns 0-2 are written per item).
+    for (int u = threadIdx.x; u < 3 * 256; u += kThreads) {
+      const int op = u >> 8, e = u & 255;
+      const int r = (e >> 4) * 8 + (e & 7), khalf = (e >> 3) & 1;
+      const float c = (op == 2 && khalf == 0) ? (float)r : 0.f;
+      const float f[8] = {c, c, c, 0.f, 0.f, 0.f, 0.f, 0.f};
+      *reinterpret_cast<uint4 *>(smem + C::kXOff + op * C::kXBytes + x_offset(r, khalf * 8)) = pack8<T>(f);
+    }
+    fence_proxy_async_smem();
+  }
+  if (warp == kTmaWarp && lane == 0) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&bars->tmem_base, C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+
+  if (warp >= 8) {
+    regs_decrease<kRegsControl>();
+    if (warp == kTmaWarp) {
+      Loads n;
+      int kv = 0, it = 0;
+      int w = (int)blockIdx.x;
+      for (int seq = 0;; ++seq) {
+        Item t{};
+        if (w < wk.n_work) t = decode_item(a, wk, w);
+        bool ok = true;
+        if (lane == 0) ok = publish(bars, seq, w, t);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          set_abort(bars, a.err);
+          break;
+        }
+        if (w >= wk.n_work) break;
+        if (t.br.nb > 0) {
+          ok = load_item<D, kAlibi>(&tm_q, &tm_k, &tm_v, smem, bars, a, wk, t, it, kv, n);
+          kv += t.br.nb;
+          ++it;
+          if (!ok) {
+            set_abort(bars, a.err);
+            break;
+          }
+        }
+        int next = wk.n_work;
+        if (work_ctr != nullptr) {
+          if (lane == 0) next = (int)gridDim.x + atomicAdd(work_ctr, 1);
+          next = __shfl_sync(0xffffffffu, next, 0);
+        }
+        w = next;
+      }
+      drain_loads<D>(bars, n);
+    } else if (warp == kMmaWarp && lane == 0) {
+      int kv = 0, it = 0, blk0 = 0;
+      for (int seq = 0;; ++seq) {
+        Item t;
+        const int w = take(bars, seq, false, t);
+        if (w < 0) {
+          set_abort(bars, a.err);
+          break;
+        }
+        if (w >= wk.n_work) break;
+        if (t.br.nb == 0) continue;
+        const bool ok = mma_tile<D, kBF16, kFold, kAlibi>(smem, bars, tmem, t.br.nb, t.nb0, it, kv, blk0, kv);
+        kv += t.br.nb;
+        blk0 += t.nb0;
+        ++it;
+        if (!ok) {
+          set_abort(bars, a.err);
+          break;
+        }
+      }
+      tc_commit(&bars->drain);
+      mbar_wait(&bars->drain, 0, kTimeoutNs);
+    } else if (warp == kVWarp) {
+      int kv = 0;
+      for (int seq = 0;; ++seq) {
+        Item t;
+        const int w = take(bars, seq, true, t);
+        if (w < 0) {
+          set_abort(bars, a.err);
+          break;
+        }
+        if (w >= wk.n_work) break;
+        const RowsSee both = rows_see(a, t.m0, 2 * wk.M, t.ql, t.kl);
+        bool ok = true;
+        for (int j = 0; j < t.br.nb && ok; ++j) {
+          const int g = kv + j, s = g % C::kStages;
+          ok = mbar_wait_or_abort(&bars->v_landed[s], (g / C::kStages) & 1, kTimeoutNs, &bars->abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int n0 = block_n0<kAlibi>(t.br, j);
+          if (partly(both, n0)) clean_block<T, D>(smem + C::kVOff + s * C::kTileBytes, bars->lost[s], t.kl - n0);
+          if (lane == 0) mbar_arrive(&bars->v_full[s]);
+        }
+        kv += t.br.nb;
+        if (!ok) {
+          set_abort(bars, a.err);
+          break;
+        }
+      }
+    } else if (warp == kSlopeWarp) {
+      int it = 0;
+      for (int seq = 0;; ++seq) {
+        Item t;
+        const int w = take(bars, seq, true, t);
+        if (w < 0) {
+          set_abort(bars, a.err);
+          break;
+        }
+        if (w >= wk.n_work) break;
+        if constexpr (kFold) {
+          if (t.br.nb == 0) continue;
+          bool ok = true;
+          for (int q = 0; q < kTiles && ok; ++q) {
+            if (it > 0) ok = mbar_wait_or_abort(&bars->q_empty[q], (it - 1) & 1, kTimeoutNs, &bars->abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+#pragma unroll 1
+            for (int r = lane; r < kBM; r += 32) {
+              // beta = slope / sm_scale as three 16-bit parts (each the rounding of
+              // what the ones before it leave), in columns 0-2.
+              const float b = a.alibi[t.kvh * a.group + (t.m0 + q * wk.M + r) % a.group] / a.sm_scale;
+              const float r1 = b - Elem<T>::to_f(Elem<T>::from_f(b));
+              const float r2 = r1 - Elem<T>::to_f(Elem<T>::from_f(r1));
+              const float f[8] = {b, r1, r2, 0.f, 0.f, 0.f, 0.f, 0.f};
+              *reinterpret_cast<uint4 *>(smem + C::kXOff + q * C::kXBytes + x_offset(r, 0)) = pack8<T>(f);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->q_full[q]);
+          }
+          ++it;
+          if (!ok) {
+            set_abort(bars, a.err);
+            break;
+          }
+        }
+      }
+    }
+  } else {
+    regs_increase<kRegsSoftmax>();
+    int blk = 0, kv = 0;
+    for (int seq = 0;; ++seq) {
+      Item t;
+      const int w = take(bars, seq, true, t);
+      if (w < 0) {
+        set_abort(bars, a.err);
+        break;
+      }
+      if (w >= wk.n_work) break;
+      if (!softmax_rows<T, D, kAlibi, kSoftcap>(a, wk, bars, tmem, warp, t, blk, kv)) break;
+      blk += warp < 4 ? t.nb0 : t.br.nb;
+      kv += t.br.nb;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// Merges the pieces of the items that were cut: a warp a row, 32 rows a CTA.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) paged_tc_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ TcWork wk) {
+  constexpr int E = D / 32;
+  constexpr float kShift = (float)tc_shift<T>();
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int cut = blockIdx.x / (kItemRows / 32), first = blockIdx.x % (kItemRows / 32) * 32;
+  const Item t = decode_item(a, wk, wk.n_whole + cut * wk.parts);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int in_item = first + warp; in_item < first + 32; in_item += 4) {
+    const int tile = in_item / kBM, r = in_item % kBM;
+    const int pr = t.m0 + tile * wk.M + r;
+    if (r >= wk.M || pr >= wk.R) continue;
+    auto at = [&](int s) { return ((long long)cut * wk.parts + s) * kItemRows + in_item; };
+    float m = -CUDART_INF_F;
+    for (int s = lane; s < wk.parts; s += 32) m = fmaxf(m, wk.part_ml[at(s) * 2]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float base = m == -CUDART_INF_F ? 0.f : m;
+    float l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < wk.parts; ++s) {
+      const float2 ml = *reinterpret_cast<const float2 *>(wk.part_ml + at(s) * 2);
+      const float w = ex2_approx(ml.x - base);
+      const float *po = wk.part_o + at(s) * D + lane * E;
+      l = fmaf(w, ml.y, l);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 v = *reinterpret_cast<const float2 *>(po + e);
+        o[e] = fmaf(w, v.x, o[e]);
+        o[e + 1] = fmaf(w, v.y, o[e + 1]);
+      }
+    }
+    const int i = pr / a.group, h = t.kvh * a.group + pr % a.group;
+    const Visible v = row_visible(a, i, t.ql, t.kl);
+    const bool sees = v.hi > v.lo;
+    const float inv = sees ? 1.f / l : 0.f;
+    T *op = static_cast<T *>(a.o) + t.b * a.os[0] + i * a.os[1] + h * a.os[2] + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(op + e) = sees ? pack2<T>(o[e] * inv, o[e + 1] * inv) : 0u;
+    if (lane == 0) {
+      const float lse2 = m - kShift + log2f(l);
+      if (a.lse != nullptr) {
+        const float slope = a.alibi != nullptr ? a.alibi[h] : 0.f;
+        a.lse[((long long)t.b * a.H + h) * a.Sq + i] =
+            sees ? lse2 * kLn2 + (a.alibi != nullptr ? slope * (float)alibi_ref(v, slope) : 0.f) : -CUDART_INF_F;
+      }
+      if (wk.stat != nullptr) wk.stat[((long long)t.b * a.Hkv + t.kvh) * wk.R + pr] = lse2;
+    }
+  }
+}
+
+// -------------------------------------------------------------------- host
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == LLMX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+bool make_map(CUtensorMap *m, const void *base, int dtype, const cuuint64_t (&dims)[4], const long long (&st)[3],
+              const cuuint32_t (&box)[4]) {
+  EncodeTiledFn enc = encode_tiled();
+  if (enc == nullptr) return false;
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    strides[i] = (cuuint64_t)st[i] * 2u;
+    // A dimension of extent 1 is never stepped along; give it any legal stride.
+    if (dims[i + 1] <= 1 && (strides[i] == 0 || strides[i] >= (1ULL << 40))) strides[i] = 16;
+  }
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return enc(m, map_type(dtype), 4, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// [.., 64 channels] x heads x rows of q: one box is a tile's packed rows.
+bool make_q_map(CUtensorMap *m, const AttnArgs &a, int M) {
+  const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.H, (cuuint64_t)a.Sq, (cuuint64_t)a.B};
+  const long long st[3] = {a.qs[2], a.qs[1], a.qs[0]};
+  const cuuint32_t box[4] = {64, (cuuint32_t)a.group, (cuuint32_t)(M / a.group), 1};
+  return make_map(m, a.q, a.dtype, dims, st, box);
+}
+// Tokens x kv heads x pages of K or V.
+bool make_page_map(CUtensorMap *m, const PagedArgs &c, const void *base, const long long *s, int dtype, int box_rows) {
+  const cuuint64_t dims[4] = {(cuuint64_t)c.D, (cuuint64_t)c.page_size, (cuuint64_t)c.Hkv, (cuuint64_t)c.n_pages};
+  const long long st[3] = {s[2], s[1], s[0]};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  return make_map(m, base, dtype, dims, st, box);
+}
+
+template <typename T, int D, bool kAlibi, bool kSoftcap>
+cudaError_t launch_tc_t(const AttnArgs &a, const TcWork &wk, int grid, int *ctr, cudaStream_t s) {
+  using C = Cfg<D>;
+  CUtensorMap tq, tk, tv;
+  if (!make_q_map(&tq, a, wk.M) || !make_page_map(&tk, wk.c, wk.c.k, wk.c.ks, a.dtype, wk.box) ||
+      !make_page_map(&tv, wk.c, wk.c.v, wk.c.vs, a.dtype, wk.box))
+    return cudaErrorInvalidValue;
+  auto kern = paged_tc_kernel<T, D, kAlibi, kSoftcap>;
+  static std::once_flag once;
+  static cudaError_t attr = cudaSuccess;
+  std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes); });
+  if (attr != cudaSuccess) return attr;
+  kern<<<grid, kThreads, C::kSmemBytes, s>>>(tq, tk, tv, a, wk, ctr);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || wk.parts == 1) return e;
+  const int cut = (wk.n_work - wk.n_whole) / wk.parts;
+  return launch_paged_after(paged_tc_merge_kernel<T, D>, dim3(cut * (kItemRows / 32)), s, a, wk);
+}
+
+template <typename T, int D>
+cudaError_t launch_tc_d(const AttnArgs &a, const TcWork &wk, int grid, int *ctr, cudaStream_t s) {
+  const bool alibi = a.alibi != nullptr, cap = a.softcap > 0.f;
+  if (alibi) return cap ? launch_tc_t<T, D, true, true>(a, wk, grid, ctr, s) : launch_tc_t<T, D, true, false>(a, wk, grid, ctr, s);
+  return cap ? launch_tc_t<T, D, false, true>(a, wk, grid, ctr, s) : launch_tc_t<T, D, false, false>(a, wk, grid, ctr, s);
+}
+
+}  // namespace
+
+bool paged_tc_supports(const AttnArgs &a, const PagedArgs &c) {
+  // The softmax takes the row max on raw scores (sm_scale > 0).  A tile holds
+  // whole groups.  Bytes of a stride of a tensor map stay below 2^40.
+  if ((a.D != 64 && a.D != 128) || !(a.sm_scale > 0.f) || a.group > kBM) return false;
+  const long long units = (long long)a.B * a.Hkv;
+  const long long M = kBM / a.group * a.group;
+  if (units * (((long long)a.Sq * a.group + 2 * M - 1) / (2 * M)) > INT_MAX / 128) return false;
+  const int extent[3] = {a.B, a.Sq, a.H}, kv_extent[3] = {c.n_pages, c.Hkv, c.page_size};
+  for (int i = 0; i < 3; ++i) {
+    if (extent[i] > 1 && (a.qs[i] == 0 || a.qs[i] >= (1LL << 39))) return false;
+    if (kv_extent[i] > 1 && (c.ks[i] >= (1LL << 39) || c.vs[i] >= (1LL << 39))) return false;
+  }
+  return true;
+}
+
+PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws) {
+  PagedTcPlan p{};
+  p.M = kBM / a.group * a.group;
+  p.n_mblocks = (int)(((long long)a.Sq * a.group + 2 * p.M - 1) / (2 * p.M));
+  const int items = a.B * a.Hkv * p.n_mblocks;
+  const int sms = std::max(1, a.num_sms);
+  p.parts = 1;
+  p.n_whole = items;
+  if (have_ws) {
+    // The items of the last, part-filled wave, in pieces: waves * (blocks of a
+    // piece + about 3 for its start and end), and for each piece of an item 0.15
+    // for the merge, which reads 128 KB of it.
+    const int cut = items % sms;
+    const int nb = (a.Skv + kBN - 1) / kBN;
+    double best = 1e30;
+    for (int s = 1; cut > 0 && s <= std::min(64, std::max(1, nb / 4)); ++s) {
+      const int waves = (int)(((long long)cut * s + sms - 1) / sms);
+      const double cost = waves * ((double)nb / s + 3.0) + (s > 1 ? 3.0 + 0.15 * s * cut / sms : 0.0);
+      if (cost < best) {
+        best = cost;
+        p.parts = s;
+      }
+    }
+    if (p.parts > 1) p.n_whole = items - cut;
+    p.part_bytes = p.parts > 1 ? (size_t)cut * p.parts * kItemRows * (a.D + 2) * sizeof(float) : 0;
+  }
+  p.n_work = p.n_whole + (items - p.n_whole) * p.parts;
+  return p;
+}
+
+cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTcPlan &p, int *ctr, float *part, float *stat,
+                            cudaStream_t s) {
+  TcWork wk{};
+  wk.c = c;
+  wk.R = a.Sq * a.group;
+  wk.M = p.M;
+  wk.n_mblocks = p.n_mblocks;
+  const long long kv_unit = std::max<long long>(1, (long long)a.Skv * a.D * 4);
+  wk.group_units = (int)std::max<long long>(1, std::min<long long>((long long)a.B * a.Hkv, (64ll << 20) / kv_unit));
+  wk.n_whole = p.n_whole;
+  wk.parts = p.parts;
+  wk.n_work = p.n_work;
+  wk.box = std::gcd(c.page_size, kBN);
+  wk.part_o = part;
+  wk.part_ml = p.parts > 1 ? part + (size_t)(p.n_work - p.n_whole) * kItemRows * a.D : nullptr;
+  wk.stat = stat;
+  int grid = p.n_work;
+  if (ctr != nullptr && p.n_work > a.num_sms) {
+    const cudaError_t e = cudaMemsetAsync(ctr, 0, sizeof(int), s);
+    if (e != cudaSuccess) return e;
+    grid = a.num_sms;
+  } else {
+    ctr = nullptr;
+  }
+  if (a.dtype == LLMX_FP16)
+    return a.D == 64 ? launch_tc_d<__half, 64>(a, wk, grid, ctr, s) : launch_tc_d<__half, 128>(a, wk, grid, ctr, s);
+  return a.D == 64 ? launch_tc_d<__nv_bfloat16, 64>(a, wk, grid, ctr, s) : launch_tc_d<__nv_bfloat16, 128>(a, wk, grid, ctr, s);
+}
+
+}  // namespace llmx_b200

@@ -31,4 +31,33 @@ __device__ __forceinline__ Visible row_visible(const AttnArgs &a, int i, int ql,
 // far into a sequence; the log-sum-exp gets slope * ref back.
 __device__ __forceinline__ int alibi_ref(const Visible &v, float slope) { return slope >= 0.f ? v.hi - 1 : v.lo; }
 
+// The tensor-core form (attn_paged_tc.cu): which requests it takes, how a
+// request is cut (part_bytes of partial results with a workspace), and the
+// launch.  ctr: an int for the work counter, or NULL; stat: nullable
+// [B * Hkv][R], log2 of each packed row's sum of 2^score.
+struct PagedTcPlan {
+  int M, n_mblocks, n_whole, parts, n_work;
+  size_t part_bytes;
+};
+bool paged_tc_supports(const AttnArgs &a, const PagedArgs &c);
+PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws);
+cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTcPlan &p, int *ctr, float *part, float *stat,
+                            cudaStream_t s);
+
+// A launch of 128 threads a CTA that may be set up while the kernel before it
+// still runs (it waits for that kernel itself).
+template <typename K, typename... Args>
+cudaError_t launch_paged_after(K kernel, dim3 grid, cudaStream_t s, const Args &...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace llmx_b200

@@ -109,6 +109,34 @@ def test_attention(dtype, shape, algo):
         c.check(algo=algo, what=str(mask) + " weights", weights=True, **kw)
 
 
+TC_SHAPES = [
+    # d, heads, hkv, page, q_len, lens, q_lens
+    (64, 8, 2, 16, 1, [77, 0, 300], None),
+    (128, 8, 2, 64, 5, [300, 3, 5, 0, 640], [5, 5, 4, 2, 0]),
+    (64, 2, 2, 16, 150, [150, 400], [150, 31]),
+    (128, 6, 2, 112, 100, [100, 613, 90], [100, 77, 90]),
+    (128, 1, 1, 128, 300, [300], None),
+    (128, 7, 1, 32, 40, [1000, 40, 41], None),
+    (64, 128, 1, 256, 3, [513, 2], None),
+    (128, 4, 4, 48, 257, [700, 257, 128, 0], [257, 200, 1, 0]),
+    (64, 16, 8, 64, 33, [5000, 33], None),
+    (128, 32, 8, 64, 130, [900] * 5, None),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", TC_SHAPES, ids=lambda s: "d%d_h%d_%d_p%d_q%d" % s[:5])
+def test_attention_in_tiles(dtype, shape):
+    d, heads, hkv, page, q_len, lens, q_lens = shape
+    c = Case(dtype, d, heads, hkv, page, q_len, lens, q_lens=q_lens, seed=d + heads + q_len)
+    for mask in MASKS:
+        kw = dict(mask)
+        if kw.pop("alibi", False):
+            kw["slopes"] = slopes_of(heads)
+        c.check(algo="tcgen05", what=str(mask), **kw)
+    llmx_b200.device_status(0)
+
+
 @pytest.mark.parametrize("algo", ["auto", "decode"])
 @pytest.mark.parametrize("q_len", [1, 3, 40])
 def test_other_layouts_and_scales(q_len, algo):
@@ -146,7 +174,7 @@ def test_without_a_table():
     assert torch.equal(out, c.run()[0])
 
 
-@pytest.mark.parametrize("algo", ["auto", "decode"])
+@pytest.mark.parametrize("algo", ["auto", "decode", "tcgen05"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("q_len", [1, 4, 90])
 def test_non_finite_tokens_reach_the_rows_that_see_them_only(dtype, q_len, algo):
@@ -279,7 +307,7 @@ def test_same_bits_again_on_other_streams_and_in_graphs(q_len, lens):
     graph.replay()
     c.lens = kl.tolist()
     c.k, c.v = [k[:n] for k, n in zip(c.k, c.lens)], [v[:n] for v, n in zip(c.v, c.lens)]
-    assert torch.equal(c.run(max_kv_len=table.shape[1] * 64)[0], o2)
+    assert torch.equal(c.run(weights=w, decay=0.0, max_kv_len=table.shape[1] * 64)[0], o2)
 
 
 def test_without_workspace_runs_unsplit_and_weights_are_refused():
