@@ -32,7 +32,7 @@ NVCC_FLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
 HIDDEN = ["-Xcompiler", "-fvisibility=hidden"]
 SOURCES = ["attn_api.cu", "attn_simt.cu", "attn_decode.cu", "attn_sm100.cu", "attn_merge.cu", "attn_kv4.cu",
            "kv4_cache.cu", "attn_paged.cu", "attn_paged_tc.cu",
-           "paged_cache.cu", "llmx_convert.cu",
+           "paged_weights.cu", "paged_cache.cu", "llmx_convert.cu",
            "llmx_tensor.cu", "attention_api.cu", "llmx_ops.cu"]
 # The C++ Tensor / attention / registry units; every other unit is compiled hidden.
 CXX_API_UNITS = ("llmx_tensor.cu", "attention_api.cu", "llmx_ops.cu")

@@ -722,7 +722,8 @@ int ctas_of(int D) { return D == 64 ? StepCfg<64>::kCtas : (D == 128 ? StepCfg<1
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-StepPlan plan_step(const AttnArgs &a, bool weights) {
+// `weights`: the rows' sums are wanted; `scores`: and their scores kept.
+StepPlan plan_step(const AttnArgs &a, bool weights, bool scores) {
   StepPlan p{};
   const long long R = (long long)a.Sq * a.group;
   p.rt = R <= 16 ? 1 : (R <= 32 ? 2 : 4);
@@ -733,7 +734,7 @@ StepPlan plan_step(const AttnArgs &a, bool weights) {
   p.part_bytes = p.split ? up256((size_t)2 * p.workers * rows * (a.D + 2) * sizeof(float)) : 0;
   p.stat_bytes = weights ? up256((size_t)a.B * a.Hkv * R * sizeof(float)) : 0;
   p.pitch = ((long long)a.Skv + 15) / 16 * 16;
-  p.score_bytes = weights ? up256((size_t)a.B * a.Hkv * R * p.pitch * sizeof(float)) : 0;
+  p.score_bytes = scores ? up256((size_t)a.B * a.Hkv * R * p.pitch * sizeof(float)) : 0;
   return p;
 }
 
@@ -750,10 +751,10 @@ cudaError_t launch_step_t(const AttnArgs &a, const StepWork &wk, long long units
   kern<<<grid, kThreads, StepCfg<D>::kSmem, s>>>(a, wk);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (wk.split) e = launch_paged_after(paged_merge_kernel<T, D>, dim3((unsigned)units), s, a, wk, 16 * RT);
+  if (wk.split) e = launch_paged_after(paged_merge_kernel<T, D>, dim3((unsigned)units), kThreads, 0, s, a, wk, 16 * RT);
   if (e != cudaSuccess || wk.score == nullptr) return e;
   const dim3 grid_w((unsigned)((a.Skv + kThreads * 4 - 1) / (kThreads * 4)), (unsigned)(a.B * a.Hkv));
-  return launch_paged_after(paged_weights_kernel, grid_w, s, a, wk);
+  return launch_paged_after(paged_weights_kernel, grid_w, kThreads, 0, s, a, wk);
 }
 
 template <typename T, int D>
@@ -789,10 +790,8 @@ cudaError_t launch_step(const AttnArgs &a, const PagedArgs &c, const StepPlan &p
     wk.part_ml = wk.part_o + (size_t)2 * p.workers * 16 * p.rt * a.D;
     at += p.part_bytes;
   }
-  if (p.score_bytes != 0) {
-    wk.stat = reinterpret_cast<float *>(at);
-    wk.score = reinterpret_cast<float *>(at + p.stat_bytes);
-  }
+  if (p.stat_bytes != 0) wk.stat = reinterpret_cast<float *>(at);
+  if (p.score_bytes != 0) wk.score = reinterpret_cast<float *>(at + p.stat_bytes);
   wk.pitch = p.pitch;
   wk.decay = decay;
   const long long units = (long long)a.B * a.Hkv * wk.nrb;
@@ -833,22 +832,36 @@ llmx_status prepare(const llmx_attn_params *p, const llmx_paged_cache *c, AttnAr
 // rows' sums][scores].
 struct Plan {
   bool tc;
+  bool again;  // key weights by computing the scores again
   StepPlan step;
   PagedTcPlan tcp;
-  size_t bytes;
+  size_t stat_at, bytes;
 };
 
+// Key weights: the scores of a few rows are kept, 8 bytes written and read a row
+// and token (at 32 rows as much as K itself at head_dim 128), if that takes at
+// most 1 GiB; otherwise they are computed again.
+constexpr int kScoreRows = 32;
+constexpr size_t kScoreBytes = size_t(1) << 30;
+
 llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs &k, Plan *plan) {
-  const bool can = paged_tc_supports(a, k) && k.w == nullptr;
+  const bool can = paged_tc_supports(a, k);
   if (p->algo == LLMX_ALGO_TCGEN05 && !can)
     return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: TCGEN05 needs head_dim 64 or 128, sm_scale > 0 and at most 128 "
                                               "query heads a kv head");
   plan->tc = can && (p->algo == LLMX_ALGO_TCGEN05 || (p->algo == LLMX_ALGO_AUTO && (long long)a.Sq * a.group > kStepRows));
+  const bool weights = k.w != nullptr;
+  const long long R = (long long)a.Sq * a.group;
   if (plan->tc) {
+    plan->again = weights;
     plan->tcp = plan_paged_tc(a, true);
-    plan->bytes = kCounterBytes + plan->tcp.part_bytes;
+    plan->stat_at = kCounterBytes + plan->tcp.part_bytes;
+    plan->bytes = plan->stat_at + (weights ? (size_t)a.B * a.Hkv * R * sizeof(float) : 0);
   } else {
-    plan->step = plan_step(a, k.w != nullptr);
+    plan->step = plan_step(a, weights, weights);
+    plan->again = weights && (R > kScoreRows || plan->step.score_bytes > kScoreBytes) && a.sm_scale > 0.f && paged_weights_supports(a, k);
+    if (plan->again) plan->step.score_bytes = 0;
+    plan->stat_at = plan->step.part_bytes;
     plan->bytes = plan->step.part_bytes + plan->step.stat_bytes + plan->step.score_bytes;
   }
   return LLMX_OK;
@@ -899,13 +912,15 @@ extern "C" llmx_status llmx_paged_attn_fwd(const llmx_attn_params *p, const llmx
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
+  unsigned char *ws = static_cast<unsigned char *>(p->workspace);
+  float *const stat = k.w != nullptr ? reinterpret_cast<float *>(ws + plan.stat_at) : nullptr;
   if (plan.tc) {
-    unsigned char *ws = static_cast<unsigned char *>(p->workspace);
     int *const ctr = have >= kCounterBytes ? reinterpret_cast<int *>(ws) : nullptr;
     float *const part = plan.tcp.part_bytes > 0 ? reinterpret_cast<float *>(ws + kCounterBytes) : nullptr;
-    e = launch_paged_tc(a, k, plan.tcp, ctr, part, nullptr, st);
+    e = launch_paged_tc(a, k, plan.tcp, ctr, part, stat, st);
   } else {
-    e = launch_step(a, k, plan.step, decay, p->workspace, st);
+    e = launch_step(a, k, plan.step, decay, ws, st);
   }
+  if (e == cudaSuccess && plan.again) e = launch_paged_weights(a, k, stat, decay, st);
   return e == cudaSuccess ? LLMX_OK : record_error(LLMX_ERR_CUDA, cudaGetErrorString(e));
 }

@@ -28,8 +28,7 @@
 #include <climits>
 #include <numeric>
 
-#include "paged_attn.cuh"
-#include "sm100_fmha.cuh"
+#include "paged_tc.cuh"
 
 namespace llmx_b200 {
 namespace {
@@ -81,26 +80,6 @@ struct PBars {
   volatile int abort_flag;
 };
 static_assert(sizeof(PBars) <= 1024, "barriers");
-
-// The tokens that rows [m0, m0 + n) of a sequence see: some row [lo, hi), every
-// row [all_lo, all_hi).
-struct RowsSee {
-  int lo, hi, all_lo, all_hi;
-};
-__device__ __forceinline__ RowsSee rows_see(const AttnArgs &a, int m0, int n, int ql, int kl) {
-  RowsSee s{0, 0, 0, 0};
-  const int i0 = m0 / a.group;
-  if (i0 >= ql) return s;
-  const int i1 = min(ql - 1, (m0 + n - 1) / a.group);
-  const Visible f = row_visible(a, i0, ql, kl), l = row_visible(a, i1, ql, kl);
-  s.lo = f.lo;
-  s.hi = max(0, l.hi);
-  s.all_lo = l.lo;
-  s.all_hi = f.hi;
-  return s;
-}
-// Whether some row of them does not see the whole block.
-__device__ __forceinline__ bool partly(const RowsSee &s, int n0) { return n0 < s.all_lo || n0 + kBN > s.all_hi; }
 
 // Work item w: units in groups whose K / V fit in L2 together, inside a group the
 // last rows (which see the most keys) first, as in the dense prefill.
@@ -176,7 +155,6 @@ __device__ bool load_item(const CUtensorMap *tm_q, const CUtensorMap *tm_k, cons
                           const AttnArgs &a, const TcWork &wk, const Item &t, int tile_it, int kv_base, Loads &n) {
   using C = Cfg<D>;
   const int lane = threadIdx.x % 32;
-  const int boxes = kBN / wk.box;
   auto wait = [&](uint64_t *bar, uint32_t par) {
     const bool ok = mbar_wait_or_abort(bar, par, kTimeoutNs, &bars->abort_flag);
     return __all_sync(0xffffffffu, ok) != 0;
@@ -192,44 +170,20 @@ __device__ bool load_item(const CUtensorMap *tm_q, const CUtensorMap *tm_k, cons
     n.q[q] = tile_it + 1;
     return true;
   };
-  // Where this lane's box of the block at n0 lies; a page index of n_pages reads as zeros.
-  struct Place {
-    int page, row;
-  };
-  auto place = [&](int n0) {
-    Place p{wk.c.n_pages, 0};
-    const int j = n0 + lane * wk.box;
-    if (lane < boxes && j < t.kl) {
-      const int slot = j / wk.c.page_size;
-      const int id = paged_page(wk.c, t.b, slot);
-      if (id >= 0) {
-        p.page = id;
-        p.row = j - slot * wk.c.page_size;
-      }
-    }
-    return p;
-  };
-  auto load_block = [&](uint8_t *dst, const CUtensorMap *tm, uint64_t *bar, const Place &p) {
-    if (lane == 0) mbar_arrive_expect_tx(bar, C::kTileBytes);
-    __syncwarp();
-    if (lane < boxes)
-      for (int c = 0; c < C::kChunks; ++c)
-        tma_load_4d(dst + c * C::kChunkBytes + lane * wk.box * 128, tm, bar, c * 64, p.row, t.kvh, p.page);
-  };
-  Place next = place(block_n0<kReverse>(t.br, 0));
+  BoxPlace next = box_place(wk.c, wk.box, t.b, t.kl, block_n0<kReverse>(t.br, 0));
   if (!load_q(0)) return false;
   for (int j = 0; j < t.br.nb; ++j) {
     const int g = kv_base + j;
     const int s = g % C::kStages;
     const uint32_t par = ((g / C::kStages) & 1) ^ 1;
-    const Place p = next;
-    if (j + 1 < t.br.nb) next = place(block_n0<kReverse>(t.br, j + 1));
+    const BoxPlace p = next;
+    if (j + 1 < t.br.nb) next = box_place(wk.c, wk.box, t.b, t.kl, block_n0<kReverse>(t.br, j + 1));
     if (!wait(&bars->k_empty[s], par)) return false;
-    load_block(smem + C::kKOff + s * C::kTileBytes, tm_k, &bars->k_full[s], p);
+    load_boxes<D>(smem + C::kKOff + s * C::kTileBytes, tm_k, &bars->k_full[s], wk.box, t.kvh, p);
     n.k = g + 1;
     if (j == 0 && !load_q(1)) return false;
     if (!wait(&bars->v_empty[s], par)) return false;
-    load_block(smem + C::kVOff + s * C::kTileBytes, tm_v, &bars->v_landed[s], p);
+    load_boxes<D>(smem + C::kVOff + s * C::kTileBytes, tm_v, &bars->v_landed[s], wk.box, t.kvh, p);
     n.v = g + 1;
   }
   return true;
@@ -754,40 +708,6 @@ __global__ void __launch_bounds__(128) paged_tc_merge_kernel(const __grid_consta
 }
 
 // -------------------------------------------------------------------- host
-CUtensorMapDataType map_type(int dtype) {
-  return dtype == LLMX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-}
-
-bool make_map(CUtensorMap *m, const void *base, int dtype, const cuuint64_t (&dims)[4], const long long (&st)[3],
-              const cuuint32_t (&box)[4]) {
-  EncodeTiledFn enc = encode_tiled();
-  if (enc == nullptr) return false;
-  cuuint64_t strides[3];
-  for (int i = 0; i < 3; ++i) {
-    strides[i] = (cuuint64_t)st[i] * 2u;
-    // A dimension of extent 1 is never stepped along; give it any legal stride.
-    if (dims[i + 1] <= 1 && (strides[i] == 0 || strides[i] >= (1ULL << 40))) strides[i] = 16;
-  }
-  const cuuint32_t one[4] = {1, 1, 1, 1};
-  return enc(m, map_type(dtype), 4, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// [.., 64 channels] x heads x rows of q: one box is a tile's packed rows.
-bool make_q_map(CUtensorMap *m, const AttnArgs &a, int M) {
-  const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.H, (cuuint64_t)a.Sq, (cuuint64_t)a.B};
-  const long long st[3] = {a.qs[2], a.qs[1], a.qs[0]};
-  const cuuint32_t box[4] = {64, (cuuint32_t)a.group, (cuuint32_t)(M / a.group), 1};
-  return make_map(m, a.q, a.dtype, dims, st, box);
-}
-// Tokens x kv heads x pages of K or V.
-bool make_page_map(CUtensorMap *m, const PagedArgs &c, const void *base, const long long *s, int dtype, int box_rows) {
-  const cuuint64_t dims[4] = {(cuuint64_t)c.D, (cuuint64_t)c.page_size, (cuuint64_t)c.Hkv, (cuuint64_t)c.n_pages};
-  const long long st[3] = {s[2], s[1], s[0]};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-  return make_map(m, base, dtype, dims, st, box);
-}
-
 template <typename T, int D, bool kAlibi, bool kSoftcap>
 cudaError_t launch_tc_t(const AttnArgs &a, const TcWork &wk, int grid, int *ctr, cudaStream_t s) {
   using C = Cfg<D>;
@@ -804,7 +724,7 @@ cudaError_t launch_tc_t(const AttnArgs &a, const TcWork &wk, int grid, int *ctr,
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || wk.parts == 1) return e;
   const int cut = (wk.n_work - wk.n_whole) / wk.parts;
-  return launch_paged_after(paged_tc_merge_kernel<T, D>, dim3(cut * (kItemRows / 32)), s, a, wk);
+  return launch_paged_after(paged_tc_merge_kernel<T, D>, dim3(cut * (kItemRows / 32)), 128, 0, s, a, wk);
 }
 
 template <typename T, int D>
@@ -817,18 +737,12 @@ cudaError_t launch_tc_d(const AttnArgs &a, const TcWork &wk, int grid, int *ctr,
 }  // namespace
 
 bool paged_tc_supports(const AttnArgs &a, const PagedArgs &c) {
-  // The softmax takes the row max on raw scores (sm_scale > 0).  A tile holds
-  // whole groups.  Bytes of a stride of a tensor map stay below 2^40.
+  // The softmax takes the row max on raw scores (sm_scale > 0).
   if ((a.D != 64 && a.D != 128) || !(a.sm_scale > 0.f) || a.group > kBM) return false;
   const long long units = (long long)a.B * a.Hkv;
   const long long M = kBM / a.group * a.group;
   if (units * (((long long)a.Sq * a.group + 2 * M - 1) / (2 * M)) > INT_MAX / 128) return false;
-  const int extent[3] = {a.B, a.Sq, a.H}, kv_extent[3] = {c.n_pages, c.Hkv, c.page_size};
-  for (int i = 0; i < 3; ++i) {
-    if (extent[i] > 1 && (a.qs[i] == 0 || a.qs[i] >= (1LL << 39))) return false;
-    if (kv_extent[i] > 1 && (c.ks[i] >= (1LL << 39) || c.vs[i] >= (1LL << 39))) return false;
-  }
-  return true;
+  return paged_weights_supports(a, c);
 }
 
 PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws) {

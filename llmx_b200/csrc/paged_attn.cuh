@@ -44,13 +44,19 @@ PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws);
 cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTcPlan &p, int *ctr, float *part, float *stat,
                             cudaStream_t s);
 
-// A launch of 128 threads a CTA that may be set up while the kernel before it
-// still runs (it waits for that kernel itself).
+// Key weights of a chunk from the rows' sums (paged_weights.cu), after the
+// attention that wrote them.
+bool paged_weights_supports(const AttnArgs &a, const PagedArgs &c);
+cudaError_t launch_paged_weights(const AttnArgs &a, const PagedArgs &c, const float *stat, float decay, cudaStream_t s);
+
+// A launch that may be set up while the kernel before it still runs (it waits
+// for that kernel itself).
 template <typename K, typename... Args>
-cudaError_t launch_paged_after(K kernel, dim3 grid, cudaStream_t s, const Args &...args) {
+cudaError_t launch_paged_after(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const Args &...args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

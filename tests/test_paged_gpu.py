@@ -90,6 +90,7 @@ SHAPES = [
     (64, 2, 1, 16, 150, [150, 400], [150, 31]),
     (128, 6, 2, 112, 100, [100, 613, 90], [100, 77, 90]),
     (256, 4, 1, 32, 80, [81, 260], None),
+    (256, 3, 3, 16, 300, [300, 700, 512], [300, 299, 1]),
 ]
 MASKS = [dict(), dict(causal=False), dict(window=20), dict(window=0), dict(cap=5.0), dict(alibi=True),
          dict(causal=False, window=33, cap=3.0), dict(window=100, alibi=True)]
@@ -134,6 +135,7 @@ def test_attention_in_tiles(dtype, shape):
         if kw.pop("alibi", False):
             kw["slopes"] = slopes_of(heads)
         c.check(algo="tcgen05", what=str(mask), **kw)
+        c.check(algo="tcgen05", what=str(mask) + " weights", weights=True, **kw)
     llmx_b200.device_status(0)
 
 
@@ -307,7 +309,7 @@ def test_same_bits_again_on_other_streams_and_in_graphs(q_len, lens):
     graph.replay()
     c.lens = kl.tolist()
     c.k, c.v = [k[:n] for k, n in zip(c.k, c.lens)], [v[:n] for v, n in zip(c.v, c.lens)]
-    assert torch.equal(c.run(weights=w, decay=0.0, max_kv_len=table.shape[1] * 64)[0], o2)
+    assert torch.equal(c.run(max_kv_len=table.shape[1] * 64)[0], o2)
 
 
 def test_without_workspace_runs_unsplit_and_weights_are_refused():
