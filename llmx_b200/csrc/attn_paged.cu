@@ -2,55 +2,49 @@
 // request's checks and the choice between its two forms, and the form for few
 // query rows, which streams K and V once past all rows of a kv head.
 //
-// Work.  A unit is one (sequence, kv head) and a block of up to 16 * RT packed
-// rows.  Its visible tokens are taken in steps of 64, 16 of which belong to one
-// page, whatever the page size.  The steps of all units, end to end, are dealt
-// to the resident CTAs in equal shares, so that sequences of any lengths finish
+// Products.  A unit is one (sequence, kv head) and a block of up to N packed rows
+// (16 or 32; 64 at head_dim 256).  Both products are transposed, so that the 128 rows of the
+// tensor core's tile are tokens or channels, which there are enough of, and the
+// few query rows are its columns:
+//   S^T [128 tokens x N] = K Q^T,   O^T [channels x N] += V^T P^T
+// on tcgen05.mma with both accumulators in tensor memory.  A softmax thread has
+// one token and N scores: no work is done for rows that are not there, and the
+// sum over tokens stays in its registers until the unit's end.  A row's
+// reference for the exponentials is common to all threads and moves (and O^T is
+// rescaled) only when some score passes it by more than a limit, which one
+// barrier with a vote finds out; the first block sets it.
+//
+// Work.  The blocks of 128 tokens of all units, end to end, are dealt to the
+// resident CTAs in equal shares, so that sequences of any lengths finish
 // together; a CTA writes the result of a unit that it has whole and a partial
-// result (unnormalised O, maximum and sum; at most two a CTA) of one that it
+// result (unnormalised O, reference and sum; at most two a CTA) of one that it
 // shares, which a second, overlapped launch merges.
 //
-// A CTA's four warps hold RT row tiles of 16 rows, and 4 / RT warps of a row
-// tile take different 16 tokens of a step and are merged in shared memory at
-// the unit's end.  K and V go through a ring of steps in shared memory by
-// 16-byte asynchronous copies, which write zeros for tokens that no row sees
-// (nothing behind a sequence's length is read), swizzled so that the matrix
-// loads of the fragments are free of conflicts; the next step's page is looked
-// up one step ahead.  Products are m16n8k16 with fp32 sums.  At 16 rows a step
-// of head_dim 128 costs a warp about 700 cycles against 2800 that its 32 KB
-// cost an SM at the HBM rate, which is why the legacy matrix instruction is
-// enough here and tiles of 128 rows (attn_paged_tc.cu) start above 64 rows.
+// A CTA: warps 0-3 softmax, warp 4 issues the products, warp 5 the copies: K and
+// V by TMA boxes from the pages into one ring of slots, in the order in which
+// they are used (K of a block comes before V of the block before it).
 //
 // Masked tokens.  A NaN or an infinity in K only reaches scores that are
-// replaced.  One in V would reach every row of the tile through 0 * V, so in
-// steps that some rows see and others do not such values are taken as 0 and
-// the rows that see their token become NaN.
+// replaced.  One in V would reach every row through 0 * V, so in blocks that not
+// every row sees whole, the thread of a token first writes zeros over such
+// values (and over all of a token that no row sees: nothing behind a sequence's
+// length counts), and its weight becomes NaN for the rows that see it.
 #include <algorithm>
 #include <climits>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <numeric>
 
-#include "paged_attn.cuh"
-#include "sm100_ptx.cuh"
+#include "paged_tc.cuh"
 
 namespace llmx_b200 {
 namespace {
 
-using sm100::smem_u32;
-
-constexpr int kThreads = 128;
-constexpr int kWarps = 4;
-constexpr int kStep = 64;  // tokens of a step
-constexpr int kStepRows = 64;  // AUTO: packed rows of a kv head up to which this form is taken
+constexpr int kStepThreads = 192;
+constexpr int kStepMma = 4, kStepTma = 5;  // warps
+constexpr int kStepRows = 32;  // AUTO: packed rows of a kv head up to which this form is taken
 constexpr size_t kCounterBytes = 256;
-
-// fp16 weights are taken 2^10 times as large: a weight 2^-24 of the largest
-// still has 10 bits then; bf16 has the exponents of fp32.
-template <typename T>
-constexpr float weight_shift() {
-  return std::is_same<T, __half>::value ? 10.f : 0.f;
-}
 
 // A launch's units and shares.
 struct StepWork {
@@ -60,34 +54,36 @@ struct StepWork {
   int workers;    // CTAs that take a share, at most
   int min_steps;  // a share is at least this long
   int split;      // 0: CTA i has unit i whole
-  float *part_o;  // [2 workers][rows of a block][D]
-  float *part_ml;  // [2 workers][rows of a block][2]
+  int reverse;    // a unit's blocks go last to first (ALiBi: the largest biases come first)
+  int box;        // tokens of a TMA box
+  float *part_o;   // [2 workers][N][D]
+  float *part_ml;  // [2 workers][N][2]
   float *stat;     // nullable [B * Hkv][R]: log2 of the sum of 2^score
   float *score;    // nullable [B * Hkv][R][pitch], log2 units
   long long pitch;
   float decay;
 };
 
-// Steps of row block rb of sequence b: tokens lo16 + 64 i .., those in [lo, hi)
-// are visible to some row.  At least one step, which may have no token.
+// Row block rb of sequence b: blocks of 128 tokens lo128 + 128 i .., tokens in
+// [lo, hi) are visible to some row.  At least one step, which may have no token.
 struct Span {
-  int ql, kl, lo, hi, q0, q1;  // q0 .. q1: query rows of the block
-  __device__ __forceinline__ int lo16() const { return lo & ~15; }
-  __device__ __forceinline__ int steps() const { return max(1, (hi - lo16() + kStep - 1) / kStep); }
+  int ql, kl, lo, hi, all_lo, all_hi;
+  __device__ __forceinline__ int lo128() const { return lo & ~(kBN - 1); }
+  __device__ __forceinline__ int blocks() const { return hi > lo ? (hi - lo128() + kBN - 1) / kBN : 0; }
+  __device__ __forceinline__ int steps() const { return max(1, blocks()); }
+  // First token of the unit's block in step `at`.
+  __device__ __forceinline__ int token(int at, int reverse) const { return lo128() + (reverse ? blocks() - 1 - at : at) * kBN; }
 };
 __device__ __forceinline__ Span span_of(const AttnArgs &a, int R, int rows, int b, int rb) {
   Span s;
   s.ql = clamp_len(a.q_lens, b, a.Sq);
   s.kl = clamp_len(a.kv_lens, b, a.Skv);
-  s.q0 = rb * rows / a.group;
-  s.q1 = min(s.ql, (min(R, (rb + 1) * rows) - 1) / a.group + 1);
-  s.lo = s.hi = 0;
-  if (s.q0 < s.q1) {
-    const Visible first = row_visible(a, s.q0, s.ql, s.kl), last = row_visible(a, s.q1 - 1, s.ql, s.kl);
-    s.lo = first.lo;
-    s.hi = last.hi;
-    if (s.hi <= s.lo) s.lo = s.hi = 0;
-  }
+  const RowsSee v = rows_see(a, rb * rows, min(rows, R - rb * rows), s.ql, s.kl);
+  s.lo = v.lo;
+  s.hi = v.hi;
+  s.all_lo = v.all_lo;
+  s.all_hi = v.all_hi;
+  if (s.hi <= s.lo) s.lo = s.hi = 0;
   return s;
 }
 
@@ -102,173 +98,325 @@ __device__ __forceinline__ long long steps_of(const AttnArgs &a, const StepWork 
 __device__ __forceinline__ int share_count(const StepWork &wk, long long total) {
   return (int)max(1LL, min((long long)wk.workers, total / wk.min_steps));
 }
-__device__ __forceinline__ long long share_begin(long long total, int w, int n) { return total * w / n; }
+__device__ __forceinline__ long long share_begin(long long total, int w, int n) {
+  const unsigned long long x = (unsigned long long)total * w;  // a division of 32 bits where that is enough
+  return x >> 32 ? x / n : (uint32_t)x / (uint32_t)n;
+}
 __device__ __forceinline__ int share_of(long long total, long long step, int n) {
-  int w = (int)(step * n / total);
+  const unsigned long long x = (unsigned long long)step * n;
+  int w = (int)(x >> 32 ? x / total : (uint32_t)x / (uint32_t)total);
   while (w > 0 && share_begin(total, w, n) > step) --w;
   while (w < n - 1 && share_begin(total, w + 1, n) <= step) ++w;
   return w;
 }
 
-// A scan over the sequences by the whole CTA: the steps before sequence b, of
-// sequence b, and of all.  pick(b, before, steps) says which b is meant.
+// A scan over the sequences by the whole CTA: the steps of all, then of the
+// sequence b that pick(b, before, steps, total) names, and the steps before it.
 struct ScanShared {
-  long long warp_sum[kWarps];
-  long long before, total;
+  long long warp_sum[8];
+  long long before, steps, total;
   int b;
 };
 template <typename F>
 __device__ void scan_steps(const AttnArgs &a, const StepWork &wk, int rows, ScanShared &sh, F pick) {
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  long long base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    const int b = b0 + tid;
-    const long long mine = b < a.B ? steps_of(a, wk, rows, b) : 0;
-    long long x = mine;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, threads = blockDim.x;
+  const int rounds = (a.B + threads - 1) / threads;
+  long long total = 0;
+  // With one round of threads the second pass has its numbers already.
+  for (int pass = 0; pass < 2; ++pass) {
+    long long base = 0;
+    for (int round = 0; round < rounds; ++round) {
+      const int b = round * threads + tid;
+      const long long mine = b < a.B ? steps_of(a, wk, rows, b) : 0;
+      long long x = mine;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, x, off);
-      if (lane >= off) x += o;
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += o;
+      }
+      if (lane == 31) sh.warp_sum[warp] = x;
+      __syncthreads();
+      long long before = base + x - mine;
+      for (int w = 0; w < threads / 32; ++w) {
+        if (w < warp) before += sh.warp_sum[w];
+        base += sh.warp_sum[w];
+      }
+      if (pass == 0) total = base;
+      if ((pass == 1 || rounds == 1) && b < a.B && pick(b, before, mine, total)) {
+        sh.b = b;
+        sh.before = before;
+        sh.steps = mine;
+      }
+      __syncthreads();
     }
-    if (lane == 31) sh.warp_sum[warp] = x;
-    __syncthreads();
-    long long before = base;
-    for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
-    before += x - mine;
-    if (b < a.B && pick(b, before, mine)) {
-      sh.b = b;
-      sh.before = before;
-    }
-    for (int w = 0; w < kWarps; ++w) base += sh.warp_sum[w];
-    __syncthreads();
+    if (rounds == 1) break;
   }
-  if (tid == 0) sh.total = base;
+  if (tid == 0) sh.total = total;
   __syncthreads();
 }
 
-// ------------------------------------------------------------- instructions
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
+// A share's position: `left` steps from step `at` of unit (b, kvh, rb) on.
+struct Cursor {
+  int b, kvh, rb, at;
+  long long left;
+  Span sp;
+  __device__ __forceinline__ int end() const { return (int)min((long long)sp.steps(), at + left); }
+  // Past this unit's part, to the next unit.  False at the share's end.
+  __device__ __forceinline__ bool next(const AttnArgs &a, const StepWork &wk, int rows) {
+    left -= end() - at;
+    if (left <= 0) return false;
+    at = 0;
+    if (++rb == wk.nrb) {
+      rb = 0;
+      if (++kvh == a.Hkv) {
+        kvh = 0;
+        ++b;
+      }
+    }
+    sp = span_of(a, wk.R, rows, b, rb);
+    return true;
   }
-}
-// The halves of w that are infinite or NaN become 0; bits says which.
-template <typename T>
-__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w, int &bits) {
-  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  bits = 0;
-  if ((w & kExp) == kExp) {
-    bits |= 1;
-    w &= 0xffff0000u;
-  }
-  if ((w & (kExp << 16)) == (kExp << 16)) {
-    bits |= 2;
-    w &= 0x0000ffffu;
-  }
-  return w;
-}
-
-// ------------------------------------------------------------------ kernel
-// Steps in the ring and CTAs an SM: 64 KB and more of copies in flight an SM.
-template <int D>
-struct StepCfg {
-  static constexpr int kStepBytes = 2 * kStep * D * 2;  // K and V
-  static constexpr int kStages = D == 64 ? 4 : 3;
-  static constexpr int kCtas = D == 64 ? 3 : (D == 128 ? 2 : 1);
-  // A row tile's O in fragments (and m, l) for the merge of a row tile's warps:
-  // at most two are handed over at a time.
-  static constexpr int kTileFloats = 16 * D + 8 * 4;
-  static constexpr int kSmem = kStages * kStepBytes + 2 * kTileFloats * 4;
-  static_assert(kCtas * (kSmem + 1024 + 256) <= 228 * 1024, "shared memory of an SM");
 };
 
-// The result of a part of a unit, or of the whole: rows of one warp.
-template <typename T, int D, int RT>
-__global__ void __launch_bounds__(kThreads, StepCfg<D>::kCtas)
-    paged_step_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ StepWork wk) {
-  using C = StepCfg<D>;
-  constexpr int kRows = 16 * RT;
-  constexpr int kKG = kWarps / RT;  // warps of a row tile
-  constexpr int kKS = D / 16;       // products of a score
-  constexpr int kNT = D / 8;        // column tiles of O
-  constexpr int kChunks = D / 8;    // 16-byte chunks of a token
-  constexpr int kRowBytes = D * 2;
-  extern __shared__ __align__(128) unsigned char smem[];
+// ------------------------------------------------------------------ kernel
+// A slot of the ring holds 128 tokens x up to 128 channels of K or V.  Two CTAs
+// an SM where their rings are deep enough (a CTA's start and end are then
+// covered by the other), else one; about 200 KB of copies an SM either way.
+template <int D, int N>
+struct StepCfg {
+  static constexpr int kDH = D < 128 ? D : 128;  // channels of a slot
+  static constexpr int kHalves = D / kDH;        // slots of a block of K or V
+  static constexpr int kSlot = kBN * kDH * 2;
+  static constexpr int kCtas = D == 256 || N == 64 || (D == 128 && N == 32) ? 1 : 2;
+  static constexpr int kQ = N * D * 2, kP = N * kBN * 2;
+  static constexpr int kInfo = N == 16 ? 1280 : (N == 32 ? 2048 : 4096);  // RowInfo, barriers
+  static constexpr int kBudget = (kCtas == 2 ? 113 : 227) * 1024 - 1024 - 256;  // less alignment and static arrays
+  static constexpr int kFit = (kBudget - kQ - 2 * kP - kInfo) / kSlot;
+  static constexpr int kSlots = kFit < 12 ? kFit : 12;
+  static_assert(kSlots >= 3 * kHalves || (kHalves == 2 && kSlots >= 4), "ring");
+  static constexpr int kQOff = kSlots * kSlot, kPOff = kQOff + kQ, kInfoOff = kPOff + 2 * kP;
+  static constexpr int kSmem = kInfoOff + kInfo + 1024;
+  // Tensor memory: two score accumulators, then O^T (one for each 128 channels).
+  static constexpr uint32_t kO = 2 * N;
+  static constexpr uint32_t kCols = N == 16 ? 64 : (N == 32 ? 128 : 256);
+  static_assert(2 * N + kHalves * N <= (int)kCols, "tensor memory");
+};
+
+template <int N>
+struct RowInfo {
+  float base[N];   // what is subtracted from a score: the reference less the weights' shift
+  float limit[N];  // scores above it move the reference; -inf before the first
+  float ref[N];    // the reference
+  float alpha[N];
+  float slope2[N];
+  int bias0[N];  // the token whose ALiBi bias counts as 0
+  int lo[N], hi[N];
+  float wmax[4][N];  // by warp: maxima, then sums
+  float inv[N];
+};
+struct SBars {
+  uint64_t full[12], empty[12];
+  uint64_t q_full, s_full[2], p_full[2], o_done[2], drain;  // [2]: by the block's parity
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+// fp16 weights are taken 2^10 times as large, so that small ones keep their
+// bits, and pass the reference by 2^5 at most; bf16 has the exponents of fp32.
+template <typename T>
+constexpr float weight_shift() {
+  return std::is_same<T, __half>::value ? 10.f : 0.f;
+}
+template <typename T>
+constexpr float weight_room() {
+  return std::is_same<T, __half>::value ? 5.f : 64.f;
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ld_n(uint32_t at, float (&x)[N]) {
+  if constexpr (N == 16) {
+    uint32_t v[16];
+    tmem_ld16(at, v);
+    tmem_wait_ld();
+    reg_fence16(v);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(v[i]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; c += 32) {
+      uint32_t v[32];
+      tmem_ld32(at + c, v);
+      tmem_wait_ld();
+      reg_fence32(v);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[c + i] = __uint_as_float(v[i]);
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void tmem_st_n(uint32_t at, const float (&x)[N]) {
+  if constexpr (N == 16) {
+    uint32_t v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(x[i]);
+    tmem_st16(at, v);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; c += 32) {
+      uint32_t v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(x[c + i]);
+      tmem_st32(at + c, v);
+    }
+  }
+}
+
+// The four softmax warps: a barrier, and one with a vote.  These are not
+// bounded: every warp runs through all blocks of the share, also after an abort.
+__device__ __forceinline__ void wg_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool wg_any(bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)p)
+      : "memory");
+  return r != 0;
+}
+
+// Reduces v[0 .. N) over a warp's lanes, each exchange handing over half of what
+// is left: N - 1 to N + 1 shuffles instead of 5 N.  Lane l gets row l (N = 32),
+// rows l and l + 32 in v[0], v[32] (64), or row l / 2 (16).
+template <int N, typename Op>
+__device__ __forceinline__ void reduce_rows(float (&v)[N], Op op) {
+  const int lane = threadIdx.x % 32;
+  constexpr int M = N < 32 ? N : 32;
+#pragma unroll
+  for (int base = 0; base < N; base += M) {
+#pragma unroll
+    for (int h = M / 2, bit = 16; h >= 1; h /= 2, bit /= 2) {
+      const bool up = lane & bit;
+#pragma unroll
+      for (int i = 0; i < h; ++i) {
+        const float lo = v[base + i], hi = v[base + i + h];
+        v[base + i] = op(up ? hi : lo, __shfl_xor_sync(0xffffffffu, up ? lo : hi, bit));
+      }
+    }
+    if constexpr (M == 16) v[base] = op(v[base], __shfl_xor_sync(0xffffffffu, v[base], 1));
+  }
+}
+template <int N>
+__device__ __forceinline__ void put_rows(float *to, const float (&v)[N]) {
+  const int lane = threadIdx.x % 32;
+  if constexpr (N == 16) {
+    if (!(lane & 1)) to[lane / 2] = v[0];
+  } else {
+#pragma unroll
+    for (int base = 0; base < N; base += 32) to[base + lane] = v[base];
+  }
+}
+
+// A token's channels of V in a slot (its row `r`): infinities and NaN become 0
+// (true if there was one), or everything does.  16-byte chunk c lies at chunk
+// c ^ (r % 8) of the row's 128 bytes.
+template <typename T, int DH>
+__device__ __forceinline__ bool clean_row(uint8_t *slot, int r, bool all) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  bool lost = false;
+#pragma unroll 1
+  for (int c = 0; c < DH / 64; ++c)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint4 *const at = reinterpret_cast<uint4 *>(slot + c * 128 * 128 + r * 128 + ((k ^ (r & 7)) << 4));
+      if (all) {
+        *at = make_uint4(0u, 0u, 0u, 0u);
+        continue;
+      }
+      const uint4 x = *at;
+      uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t m = (w[e] & kExp) ^ kExp;  // a half that is 0: all exponent bits set
+        if ((m & 0xffffu) == 0u) {
+          w[e] &= 0xffff0000u;
+          any = true;
+        }
+        if ((m >> 16) == 0u) {
+          w[e] &= 0x0000ffffu;
+          any = true;
+        }
+      }
+      if (any) {
+        *at = make_uint4(w[0], w[1], w[2], w[3]);
+        lost = true;
+      }
+    }
+  return lost;
+}
+
+// kMode: 1 ALiBi, 2 a soft-cap (with ALiBi or without), 0 neither.
+template <typename T, int D, int N, int kMode>
+__global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
+    paged_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                      const __grid_constant__ AttnArgs a, const __grid_constant__ StepWork wk) {
+  using C = StepCfg<D, N>;
+  constexpr int H = C::kHalves;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  RowInfo<N> *const info = reinterpret_cast<RowInfo<N> *>(smem + C::kInfoOff);
+  SBars *const bars = reinterpret_cast<SBars *>(smem + C::kInfoOff + sizeof(RowInfo<N>));
+  static_assert(sizeof(RowInfo<N>) % 16 == 0 && sizeof(RowInfo<N>) + sizeof(SBars) <= C::kInfo, "row info");
   __shared__ ScanShared sh;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int g = lane / 4, t = lane % 4;
-  const int rt = warp % RT, kg = warp / RT;
-  const uint32_t ring = smem_u32(smem);
-  float *const hand = reinterpret_cast<float *>(smem + C::kStages * C::kStepBytes);
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    mbar_init(&bars->q_full, 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], 128);
+      mbar_init(&bars->o_done[i], 1);
+    }
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kStepTma && lane == 0) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
 
-  // ---- this CTA's share: `left` steps from step `at` of unit (b, kvh, rb) on
-  struct Cursor {
-    int b, kvh, rb, at;
-    Span sp;
-  };
+  // ---- this CTA's share
   Cursor cur;
-  long long left;
   const int worker = blockIdx.x;
   if (wk.split) {
-    scan_steps(a, wk, kRows, sh, [](int, long long, long long) { return false; });
+    scan_steps(a, wk, N, sh, [&](int, long long before, long long steps, long long total) {
+      const int n = share_count(wk, total);
+      if (worker >= n) return false;
+      const long long begin = share_begin(total, worker, n);
+      return before <= begin && begin < before + steps;
+    });
     const long long total = sh.total;
     const int n = share_count(wk, total);
     if (worker >= n) return;
     const long long begin = share_begin(total, worker, n);
-    left = share_begin(total, worker + 1, n) - begin;
-    if (left <= 0) return;
-    __syncthreads();
-    scan_steps(a, wk, kRows, sh, [begin](int, long long before, long long steps) { return before <= begin && begin < before + steps; });
+    cur.left = share_begin(total, worker + 1, n) - begin;
+    if (cur.left <= 0) return;
     cur.b = sh.b;
     long long within = begin - sh.before;
-    const long long per_head = steps_of(a, wk, kRows, cur.b) / a.Hkv;
+    const long long per_head = sh.steps / a.Hkv;
     cur.kvh = (int)(within / per_head);
     within -= cur.kvh * per_head;
     for (cur.rb = 0;; ++cur.rb) {
-      cur.sp = span_of(a, wk.R, kRows, cur.b, cur.rb);
+      cur.sp = span_of(a, wk.R, N, cur.b, cur.rb);
       if (within < cur.sp.steps()) break;
       within -= cur.sp.steps();
     }
@@ -278,318 +426,370 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D>::kCtas)
     const int u = worker / wk.nrb;
     cur.kvh = u % a.Hkv;
     cur.b = u / a.Hkv;
-    cur.sp = span_of(a, wk.R, kRows, cur.b, cur.rb);
+    cur.sp = span_of(a, wk.R, N, cur.b, cur.rb);
     cur.at = 0;
-    left = cur.sp.steps();
+    cur.left = cur.sp.steps();
   }
-  auto next_unit = [&](Cursor &c) {
-    c.at = 0;
-    if (++c.rb == wk.nrb) {
-      c.rb = 0;
-      if (++c.kvh == a.Hkv) {
-        c.kvh = 0;
-        ++c.b;
+  if (warp == kStepMma) {
+    tmem_alloc(&bars->tmem_base, C::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  auto wait = [&](uint64_t *bar, uint32_t par) { return mbar_wait_or_abort(bar, par, kTimeoutNs, &bars->abort_flag); };
+
+  if (warp == kStepTma) {
+    // ---- copies, in the order K 0, K 1, V 0, K 2, V 1, ..
+    int g = 0;  // slots filled
+    bool ok = true;
+    auto copy = [&](const CUtensorMap *tm, const BoxPlace &p) {
+      for (int half = 0; half < H && ok; ++half, ++g) {
+        const int s = g % C::kSlots;
+        ok = __all_sync(0xffffffffu, wait(&bars->empty[s], ((g / C::kSlots) & 1) ^ 1)) != 0;
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&bars->full[s], C::kSlot);
+        __syncwarp();
+        if (lane < kBN / wk.box)
+          for (int c = 0; c < C::kDH / 64; ++c)
+            tma_load_4d(smem + s * C::kSlot + c * 128 * 128 + lane * wk.box * 128, tm, &bars->full[s], half * 128 + c * 64, p.row,
+                        cur.kvh, p.page);
       }
+    };
+    do {
+      const int b1 = cur.sp.hi > cur.sp.lo ? cur.end() : cur.at;
+      BoxPlace kp, vp;
+      if (cur.at < b1) {
+        kp = box_place(wk.c, wk.box, cur.b, cur.sp.kl, cur.sp.token(cur.at, wk.reverse));
+        vp = kp;
+        copy(&tm_k, kp);
+      }
+      for (int j = cur.at; j < b1 && ok; ++j) {
+        if (j + 1 < b1) {
+          kp = box_place(wk.c, wk.box, cur.b, cur.sp.kl, cur.sp.token(j + 1, wk.reverse));
+          copy(&tm_k, kp);
+        }
+        if (ok) copy(&tm_v, vp);
+        vp = kp;
+      }
+    } while (ok && cur.next(a, wk, N));
+    if (!ok) set_abort(bars, a.err);
+    // Every copy issued lands before the CTA may exit.
+    for (int i = max(0, g - C::kSlots); i < g; ++i) mbar_wait(&bars->full[i % C::kSlots], (i / C::kSlots) & 1, kTimeoutNs);
+  } else if (warp == kStepMma) {
+    if (lane == 0) {
+      // ---- products: S^T(j + 1) is issued before O^T += .. (j)
+      constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+      constexpr uint32_t idesc_s = idesc_f16(128, N, kBF16, false);
+      constexpr uint32_t idesc_o = idesc_f16(128, N, kBF16, true) | (1u << 15);  // V^T: M-major
+      int g = 0, blk = 0, parts = 0;  // slots used, blocks, parts with blocks
+      bool ok = true;
+      const uint32_t q_base = smem_u32(smem + C::kQOff), p_base = smem_u32(smem + C::kPOff), ring = smem_u32(smem);
+      auto scores = [&](int at) {
+        for (int half = 0; half < H && ok; ++half, ++g) {
+          const int s = g % C::kSlots;
+          ok = wait(&bars->full[s], (g / C::kSlots) & 1);
+          if (!ok) return;
+          tc_fence_after();
+          uint64_t da = smem_desc_sw128(ring + s * C::kSlot, 16, 1024);
+          uint64_t db = smem_desc_sw128(q_base + half * 2 * N * 128, 16, 1024);
+          asm volatile("" : "+l"(da), "+l"(db));
+#pragma unroll
+          for (int kk = 0; kk < C::kDH / 16; ++kk)
+            mma_ss(tmem + (at & 1) * N, da + (uint64_t)(((kk / 4) * 128 * 128 + (kk % 4) * 32) >> 4),
+                   db + (uint64_t)(((kk / 4) * N * 128 + (kk % 4) * 32) >> 4), idesc_s, (half > 0 || kk > 0) ? 1u : 0u);
+          tc_commit(&bars->empty[s]);
+        }
+        if (ok) tc_commit(&bars->s_full[at & 1]);
+      };
+      do {
+        const int b1 = cur.sp.hi > cur.sp.lo ? cur.end() : cur.at;
+        if (cur.at >= b1) continue;
+        ok = wait(&bars->q_full, parts & 1);
+        ++parts;
+        if (!ok) break;
+        scores(blk);
+        for (int j = cur.at; j < b1 && ok; ++j, ++blk) {
+          if (j + 1 < b1) scores(blk + 1);
+          if (!ok) break;
+          ok = wait(&bars->p_full[blk & 1], (blk >> 1) & 1);
+          for (int half = 0; half < H && ok; ++half, ++g) {
+            const int s = g % C::kSlots;
+            ok = wait(&bars->full[s], (g / C::kSlots) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            // V^T by 64-channel chunks; at head_dim 64 the second 64 rows of the
+            // tile repeat the first and are not used.
+            uint64_t da = smem_desc_sw128(ring + s * C::kSlot, D == 64 ? 0 : 128 * 128, 1024);
+            // P^T: 8 tokens x 8 rows of 128 bytes, 128 bytes apart along the
+            // tokens and 2048 along the rows.
+            uint64_t db = smem_desc_noswz(p_base + (blk & 1) * C::kP, 128, 2048);
+            asm volatile("" : "+l"(da), "+l"(db));
+#pragma unroll
+            for (int kk = 0; kk < kBN / 16; ++kk)
+              mma_ss(tmem + C::kO + half * N, da + (uint64_t)((kk * 16 * 128) >> 4), db + (uint64_t)((kk * 256) >> 4), idesc_o,
+                     (j > cur.at || kk > 0) ? 1u : 0u);
+            tc_commit(&bars->empty[s]);
+          }
+          if (ok) tc_commit(&bars->o_done[blk & 1]);
+        }
+      } while (ok && cur.next(a, wk, N));
+      if (!ok) set_abort(bars, a.err);
+      tc_commit(&bars->drain);
+      mbar_wait(&bars->drain, 0, kTimeoutNs);
     }
-    c.sp = span_of(a, wk.R, kRows, c.b, c.rb);
-  };
-
-  // ---- copies.  Warp w copies tokens 16 w .. of each step.
-  Cursor pre = cur;  // the next step to be copied
-  long long pre_left = left;
-  auto first_token = [&](const Cursor &c) { return c.sp.lo16() + c.at * kStep + warp * 16; };
-  // The page of the warp's tokens of the step, or -1 where there is nothing to read.
-  auto look_up = [&](const Cursor &c) {
-    const int j = first_token(c);
-    return j < c.sp.hi ? paged_page(wk.c, c.b, j / wk.c.page_size) : -1;
-  };
-  int page = look_up(pre);
-  auto copy_step = [&](int stage) {
-    if (pre_left > 0) {
-      const int j = first_token(pre);
-      const int in_page = j % wk.c.page_size;
-      constexpr int kPerPass = 32 / kChunks;  // tokens of one instruction
-      const int row0 = lane / kChunks, chunk = lane % kChunks;
-      const long long pg = max(page, 0);
-      const T *const kp = static_cast<const T *>(wk.c.k) + pg * wk.c.ks[0] + pre.kvh * wk.c.ks[1] + chunk * 8;
-      const T *const vp = static_cast<const T *>(wk.c.v) + pg * wk.c.vs[0] + pre.kvh * wk.c.vs[1] + chunk * 8;
-      const uint32_t dst = ring + stage * C::kStepBytes;
-#pragma unroll
-      for (int i = 0; i < 16 / kPerPass; ++i) {
-        const int row = i * kPerPass + row0;
-        const bool valid = page >= 0 && j + row >= pre.sp.lo && j + row < pre.sp.hi;
-        const long long tok = valid ? in_page + row : 0;
-        const uint32_t at = (warp * 16 + row) * kRowBytes + ((chunk ^ (row & 7)) << 4);
-        cp_async16(dst + at, kp + tok * wk.c.ks[2], valid);
-        cp_async16(dst + kStep * kRowBytes + at, vp + tok * wk.c.vs[2], valid);
+  } else {
+    // ---- softmax: thread tid has token tid of each block, and channel tid (and
+    // tid + 128) of O^T
+    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    const float scale2 = a.sm_scale * kLog2e;
+    const float cap_in = kMode == 2 ? a.sm_scale / a.softcap : 0.f, cap_out = a.softcap * kLog2e;
+    constexpr float kShift = weight_shift<T>();
+    int g = 0, blk = 0;
+    bool ok = true;
+    auto wait_all = [&](uint64_t *bar, uint32_t par) {
+      const bool w = __all_sync(0xffffffffu, wait(bar, par)) != 0;
+      if (!w && ok) set_abort(bars, a.err);
+      ok = ok && w;
+    };
+    do {
+      const Span sp = cur.sp;
+      const int b0 = cur.at, e0 = cur.end(), b1 = sp.hi > sp.lo ? e0 : b0;
+      const int row0 = cur.rb * N, rows = min(N, wk.R - row0);
+      // Everything of the last part has been read (the barriers at its end).
+      if (tid < N) {
+        const int r = row0 + tid, i = r / a.group;
+        const bool real = tid < rows && i < sp.ql;
+        const Visible v = real ? row_visible(a, i, sp.ql, sp.kl) : Visible{0, 0};
+        const float slope = kMode != 0 && a.alibi != nullptr && real ? a.alibi[cur.kvh * a.group + r % a.group] : 0.f;
+        info->lo[tid] = v.lo;
+        info->hi[tid] = v.hi;
+        info->slope2[tid] = slope * kLog2e;
+        info->bias0[tid] = alibi_ref(v, slope);
+        info->ref[tid] = info->limit[tid] = -CUDART_INF_F;
+        info->base[tid] = -kShift;
       }
-      if (--pre_left > 0) {
-        if (++pre.at == pre.sp.steps()) next_unit(pre);
-        page = look_up(pre);
+      if (b0 < b1) {
+        // Q [row][64 channels] in 128 bytes a row, chunk c at c ^ (row % 8).
+        for (int u = tid; u < N * D / 8; u += 128) {
+          const int r = u / (D / 8), c = u % (D / 8);
+          const int pr = row0 + r, i = pr / a.group;
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (r < rows && i < sp.ql)
+            x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + cur.b * a.qs[0] + i * a.qs[1] +
+                                                 (cur.kvh * a.group + pr - i * a.group) * a.qs[2] + c * 8);
+          *reinterpret_cast<uint4 *>(smem + C::kQOff + (c / 8) * N * 128 + r * 128 + (((c % 8) ^ (r & 7)) << 4)) = x;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&bars->q_full);
       }
-    }
-    cp_async_commit();
-  };
+      wg_sync();  // the rows' values
+      float l[N];
 #pragma unroll
-  for (int i = 0; i < C::kStages - 1; ++i) copy_step(i);
+      for (int r = 0; r < N; ++r) l[r] = 0.f;
 
-  const float scale2 = a.sm_scale * kPagedLog2e;
-  const float cap_in = a.softcap > 0.f ? a.sm_scale / a.softcap : 0.f, cap_out = a.softcap * kPagedLog2e;
-  constexpr float kShift = weight_shift<T>();
-  int stage = 0;
-
-  while (left > 0) {
-    // ---- a unit, or the share's part of it
-    const Span sp = cur.sp;
-    const int part0 = cur.at, part1 = (int)min((long long)sp.steps(), part0 + left);
-    uint32_t qf[kKS][4];
-    float slope2[2];
-    Visible vis[2];
-    int ref[2];
+      for (int at = b0; at < b1; ++at, ++blk) {
+        const int buf = blk & 1;
+        wait_all(&bars->s_full[buf], (blk >> 1) & 1);
+        tc_fence_after();
+        float x[N];
+        tmem_ld_n<N>(tmem + lane_off + buf * N, x);
+        const int n0 = sp.token(at, wk.reverse), j = n0 + tid;
+        const bool part = n0 < sp.all_lo || n0 + kBN > sp.all_hi;
 #pragma unroll
-    for (int rr = 0; rr < 2; ++rr) {
-      const int r = cur.rb * kRows + rt * 16 + g + 8 * rr;
-      const int i = r / a.group, h = cur.kvh * a.group + r % a.group;
-      const bool real = r < wk.R && i < sp.ql;
-      vis[rr] = real ? row_visible(a, i, sp.ql, sp.kl) : Visible{0, 0};
-      const float slope = a.alibi != nullptr && real ? a.alibi[h] : 0.f;
-      slope2[rr] = slope * kPagedLog2e;
-      ref[rr] = alibi_ref(vis[rr], slope);
-      const T *qp = static_cast<const T *>(a.q) + (real ? cur.b * a.qs[0] + i * a.qs[1] + h * a.qs[2] : 0) + 2 * t;
+        for (int r = 0; r < N; r += 4) {
+          if constexpr (kMode != 0) {
+            const float4 sl = *reinterpret_cast<const float4 *>(&info->slope2[r]);
+            const int4 b = *reinterpret_cast<const int4 *>(&info->bias0[r]);
+            const float s4[4] = {sl.x, sl.y, sl.z, sl.w};
+            const int b4[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int ks = 0; ks < kKS; ++ks) {
-        qf[ks][rr] = real ? *reinterpret_cast<const uint32_t *>(qp + ks * 16) : 0u;
-        qf[ks][2 + rr] = real ? *reinterpret_cast<const uint32_t *>(qp + ks * 16 + 8) : 0u;
-      }
-    }
-    // Every row of the block sees the tokens [all_lo, all_hi).
-    const int all_lo = sp.q0 < sp.q1 ? row_visible(a, sp.q1 - 1, sp.ql, sp.kl).lo : 0;
-    const int all_hi = sp.q0 < sp.q1 ? row_visible(a, sp.q0, sp.ql, sp.kl).hi : 0;
-    const bool mixed = sp.q1 - sp.q0 > 1;  // rows that see different tokens
-    float o[kNT][4], m[2], l[2];
-#pragma unroll
-    for (int n = 0; n < kNT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
-    m[0] = m[1] = -CUDART_INF_F;
-    l[0] = l[1] = 0.f;
-
-    for (int at = part0; at < part1; ++at) {
-      cp_async_wait<C::kStages - 2>();
-      __syncthreads();
-      copy_step(stage == 0 ? C::kStages - 1 : stage - 1);
-      const uint32_t kbase = ring + stage * C::kStepBytes, vbase = kbase + kStep * kRowBytes;
-      stage = stage == C::kStages - 1 ? 0 : stage + 1;
-#pragma unroll 1
-      for (int sub = kg; sub < 4; sub += kKG) {
-        const int j0 = sp.lo16() + at * kStep + sub * 16;
-        if (j0 >= sp.hi) break;
-        // ---- scores of 16 rows and 16 tokens
-        float s[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
-        {
-          const int key = ((lane >> 4) << 3) + (lane & 7);
-          const uint32_t row = kbase + (sub * 16 + key) * kRowBytes;
-          const int half = (lane >> 3) & 1;
-#pragma unroll
-          for (int ks = 0; ks < kKS; ++ks) {
-            uint32_t kf[4];
-            ldmatrix4(row + (((2 * ks + half) ^ (key & 7)) << 4), kf);
-            mma16816<T>(s[0], qf[ks], kf[0], kf[1]);
-            mma16816<T>(s[1], qf[ks], kf[2], kf[3]);
-          }
-        }
-        const bool need_mask = j0 < all_lo || j0 + 16 > all_hi;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rr = i >> 1, j = j0 + n * 8 + 2 * t + (i & 1);
-            float x = a.softcap > 0.f ? tanhf(s[n][i] * cap_in) * cap_out : s[n][i] * scale2;
-            if (a.alibi != nullptr) x = fmaf(slope2[rr], (float)(j - ref[rr]), x);
-            if (need_mask && (j < vis[rr].lo || j >= vis[rr].hi)) x = -CUDART_INF_F;
-            s[n][i] = x;
-          }
-        if (wk.score != nullptr) {
-#pragma unroll
-          for (int rr = 0; rr < 2; ++rr) {
-            const int r = cur.rb * kRows + rt * 16 + g + 8 * rr;
-            if (r < wk.R) {
-              float *sc = wk.score + (((long long)cur.b * a.Hkv + cur.kvh) * wk.R + r) * wk.pitch + j0 + 2 * t;
-              *reinterpret_cast<float2 *>(sc) = make_float2(s[0][2 * rr], s[0][2 * rr + 1]);
-              *reinterpret_cast<float2 *>(sc + 8) = make_float2(s[1][2 * rr], s[1][2 * rr + 1]);
-            }
-          }
-        }
-        // ---- running maximum and sum
-        float alpha[2];
-        bool moved = false;
-#pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-          float mx = fmaxf(fmaxf(s[0][2 * rr], s[0][2 * rr + 1]), fmaxf(s[1][2 * rr], s[1][2 * rr + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          alpha[rr] = 1.f;
-          if (mx > m[rr]) {
-            alpha[rr] = ex2(m[rr] - mx);
-            m[rr] = mx;
-            moved = true;
-          }
-        }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int rr = 0; rr < 2; ++rr) l[rr] *= alpha[rr];
-#pragma unroll
-          for (int n = 0; n < kNT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[n][i] *= alpha[i >> 1];
-        }
-        uint32_t pf[4];
-#pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-          const float base = (m[rr] == -CUDART_INF_F ? 0.f : m[rr]) - kShift;
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const float p0 = ex2(s[n][2 * rr] - base), p1 = ex2(s[n][2 * rr + 1] - base);
-            l[rr] += p0 + p1;
-            pf[2 * n + rr] = pack2<T>(p0, p1);
-          }
-        }
-        // ---- O += P V
-        {
-          const int key = (((lane >> 3) & 1) << 3) + (lane & 7);
-          const uint32_t row = vbase + (sub * 16 + key) * kRowBytes;
-          const int half = lane >> 4;
-          if (!(need_mask && mixed)) {
-#pragma unroll
-            for (int n = 0; n < kNT; n += 2) {
-              uint32_t vf[4];
-              ldmatrix4_trans(row + (((n + half) ^ (key & 7)) << 4), vf);
-              mma16816<T>(o[n], pf, vf[0], vf[1]);
-              mma16816<T>(o[n + 1], pf, vf[2], vf[3]);
+            for (int e = 0; e < 4; ++e) {
+              x[r + e] = kMode == 2 ? tanhf(x[r + e] * cap_in) * cap_out : x[r + e] * scale2;
+              x[r + e] = fmaf(s4[e], (float)(j - b4[e]), x[r + e]);
             }
           } else {
-            uint32_t lost = 0;  // tokens of the 16 with an infinity or NaN in V
 #pragma unroll
-            for (int n = 0; n < kNT; n += 2) {
-              uint32_t vf[4];
-              ldmatrix4_trans(row + (((n + half) ^ (key & 7)) << 4), vf);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                int bits;
-                vf[i] = finite_or_zero<T>(vf[i], bits);
-                lost |= (uint32_t)bits << (2 * t + 8 * (i & 1));
-              }
-              mma16816<T>(o[n], pf, vf[0], vf[1]);
-              mma16816<T>(o[n + 1], pf, vf[2], vf[3]);
-            }
-            lost = __reduce_or_sync(0xffffffffu, lost);
-            if (lost != 0) {
-#pragma unroll
-              for (int rr = 0; rr < 2; ++rr) {
-                const int lo = min(max(vis[rr].lo - j0, 0), 16), hi = min(max(vis[rr].hi - j0, 0), 16);
-                if (hi > lo && (lost & ((1u << hi) - (1u << lo))) != 0) l[rr] = CUDART_NAN_F;
-              }
-            }
+            for (int e = 0; e < 4; ++e) x[r + e] *= scale2;
           }
         }
+        if (part) {
+          bool lost = false;
+          const int v0 = g + H * (min(at - b0 + 2, b1 - b0) + at - b0);  // V's first slot of the block
+#pragma unroll
+          for (int half = 0; half < H; ++half) {
+            const int s = (v0 + half) % C::kSlots;
+            wait_all(&bars->full[s], ((v0 + half) / C::kSlots) & 1);
+            if (ok) lost |= clean_row<T, C::kDH>(smem + s * C::kSlot, tid, j < sp.lo || j >= sp.hi);
+          }
+#pragma unroll
+          for (int r = 0; r < N; ++r) {
+            const bool vis = j >= info->lo[r] && j < info->hi[r];
+            x[r] = vis ? (lost ? CUDART_NAN_F : x[r]) : -CUDART_INF_F;
+          }
+        }
+        if (wk.score != nullptr && j < wk.pitch) {
+          float *sc = wk.score + (((long long)cur.b * a.Hkv + cur.kvh) * wk.R + row0) * wk.pitch + j;
+#pragma unroll
+          for (int r = 0; r < N; ++r)
+            if (r < rows) sc[r * wk.pitch] = x[r];
+        }
+        bool over = false;
+#pragma unroll
+        for (int r = 0; r < N; r += 4) {
+          const float4 lim = *reinterpret_cast<const float4 *>(&info->limit[r]);
+          over |= x[r] > lim.x || x[r + 1] > lim.y || x[r + 2] > lim.z || x[r + 3] > lim.w;
+        }
+        if (wg_any(over)) {
+          // Some score passes its row's limit: new references.
+          {
+            float mx[N];
+#pragma unroll
+            for (int r = 0; r < N; ++r) mx[r] = x[r];
+            reduce_rows<N>(mx, [](float p, float q) { return fmaxf(p, q); });
+            put_rows<N>(info->wmax[warp], mx);
+          }
+          wg_sync();
+          if (tid < N) {
+            const float mx = fmaxf(fmaxf(info->wmax[0][tid], info->wmax[1][tid]), fmaxf(info->wmax[2][tid], info->wmax[3][tid]));
+            const float old = info->ref[tid];
+            float alpha = 1.f;
+            if (mx > info->limit[tid]) {
+              alpha = old == -CUDART_INF_F ? 1.f : ex2_approx(old - mx);
+              info->ref[tid] = mx;
+              info->base[tid] = mx - kShift;
+              info->limit[tid] = mx + weight_room<T>();
+            }
+            info->alpha[tid] = alpha;
+          }
+          wg_sync();
+#pragma unroll
+          for (int r = 0; r < N; ++r) l[r] *= info->alpha[r];
+          if (at > b0) {
+            // O^T holds the blocks before once their products are done.
+            wait_all(&bars->o_done[(blk - 1) & 1], ((blk - 1) >> 1) & 1);
+            tc_fence_after();
+#pragma unroll 1
+            for (int half = 0; half < H; ++half) {
+              float o[N];
+              tmem_ld_n<N>(tmem + lane_off + C::kO + half * N, o);
+#pragma unroll
+              for (int r = 0; r < N; ++r) o[r] *= info->alpha[r];
+              tmem_st_n<N>(tmem + lane_off + C::kO + half * N, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        uint8_t *const pt = smem + C::kPOff + buf * C::kP + tid * 16;
+#pragma unroll
+        for (int r = 0; r < N; r += 8) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const float4 bs = *reinterpret_cast<const float4 *>(&info->base[r + e]);
+            const float p0 = ex2_approx(x[r + e] - bs.x), p1 = ex2_approx(x[r + e + 1] - bs.y);
+            const float p2 = ex2_approx(x[r + e + 2] - bs.z), p3 = ex2_approx(x[r + e + 3] - bs.w);
+            l[r + e] += p0;
+            l[r + e + 1] += p1;
+            l[r + e + 2] += p2;
+            l[r + e + 3] += p3;
+            w[e / 2] = pack2<T>(p0, p1);
+            w[e / 2 + 1] = pack2<T>(p2, p3);
+          }
+          *reinterpret_cast<uint4 *>(pt + (r / 8) * 2048) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(&bars->p_full[buf]);
       }
-    }
+      g += 2 * H * (b1 - b0);
 
-    // ---- the unit's end: the sums of a row's four lanes, then its warps
-#pragma unroll
-    for (int rr = 0; rr < 2; ++rr) {
-      l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 1);
-      l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 2);
-    }
-#pragma unroll
-    for (int half = kKG / 2; half >= 1; half /= 2) {
-      if (kg >= half && kg < 2 * half) {
-        float *const buf = hand + ((kg - half) * RT + rt) * C::kTileFloats;
-#pragma unroll
-        for (int n = 0; n < kNT; ++n)
-          *reinterpret_cast<float4 *>(buf + (n * 32 + lane) * 4) = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
-        if (t == 0) *reinterpret_cast<float4 *>(buf + 16 * D + g * 4) = make_float4(m[0], m[1], l[0], l[1]);
+      // ---- the part's end
+      reduce_rows<N>(l, [](float p, float q) { return p + q; });
+      put_rows<N>(info->wmax[warp], l);
+      if (b0 < b1) {
+        // (The products complete in order, and those two blocks back are done, since
+        // the last block's scores were issued after them: no phase is passed over.)
+        wait_all(&bars->o_done[(blk - 1) & 1], ((blk - 1) >> 1) & 1);
+        tc_fence_after();
       }
-      __syncthreads();
-      if (kg < half) {
-        const float *const buf = hand + (kg * RT + rt) * C::kTileFloats;
-        const float4 ml = *reinterpret_cast<const float4 *>(buf + 16 * D + g * 4);
-        const float om[2] = {ml.x, ml.y}, ol[2] = {ml.z, ml.w};
-        float w0[2], w1[2];
-#pragma unroll
-        for (int rr = 0; rr < 2; ++rr) {
-          const float mn = fmaxf(m[rr], om[rr]);
-          const float base = mn == -CUDART_INF_F ? 0.f : mn;
-          w0[rr] = ex2(m[rr] - base);
-          w1[rr] = ex2(om[rr] - base);
-          m[rr] = mn;
-          l[rr] = l[rr] * w0[rr] + ol[rr] * w1[rr];
-        }
-#pragma unroll
-        for (int n = 0; n < kNT; ++n) {
-          const float4 x = *reinterpret_cast<const float4 *>(buf + (n * 32 + lane) * 4);
-          o[n][0] = o[n][0] * w0[0] + x.x * w1[0];
-          o[n][1] = o[n][1] * w0[0] + x.y * w1[0];
-          o[n][2] = o[n][2] * w0[1] + x.z * w1[1];
-          o[n][3] = o[n][3] * w0[1] + x.w * w1[1];
-        }
-      }
-      __syncthreads();
-    }
-    if (kg == 0) {
-      const bool whole = part0 == 0 && part1 == sp.steps();
-      const long long slot = 2LL * worker + (part0 == 0 ? 1 : 0);
-#pragma unroll
-      for (int rr = 0; rr < 2; ++rr) {
-        const int in_block = rt * 16 + g + 8 * rr, r = cur.rb * kRows + in_block;
-        if (r >= wk.R) continue;
+      wg_sync();
+      const bool whole = b0 == 0 && e0 == sp.steps();
+      const long long slot = 2LL * worker + (b0 == 0 ? 1 : 0);
+      if (tid < rows) {
+        const float sum = (info->wmax[0][tid] + info->wmax[1][tid]) + (info->wmax[2][tid] + info->wmax[3][tid]);
+        const int r = row0 + tid;
         if (whole) {
           const int i = r / a.group, h = cur.kvh * a.group + r % a.group;
-          const bool sees = vis[rr].hi > vis[rr].lo;
-          const float inv = sees ? 1.f / l[rr] : 0.f;
-          const float lse2 = m[rr] - kShift + log2f(l[rr]);
-          T *op = static_cast<T *>(a.o) + cur.b * a.os[0] + i * a.os[1] + h * a.os[2] + 2 * t;
-#pragma unroll
-          for (int n = 0; n < kNT; ++n)
-            *reinterpret_cast<uint32_t *>(op + n * 8) = sees ? pack2<T>(o[n][2 * rr] * inv, o[n][2 * rr + 1] * inv) : 0u;
-          if (t == 0) {
-            if (a.lse != nullptr)
-              a.lse[((long long)cur.b * a.H + h) * a.Sq + i] =
-                  sees ? lse2 * kPagedLn2 + (a.alibi != nullptr ? a.alibi[h] * (float)ref[rr] : 0.f) : -CUDART_INF_F;
-            if (wk.stat != nullptr) wk.stat[((long long)cur.b * a.Hkv + cur.kvh) * wk.R + r] = lse2;
-          }
+          const bool sees = info->hi[tid] > info->lo[tid];
+          const float lse2 = info->ref[tid] - kShift + log2f(sum);
+          info->inv[tid] = sees ? 1.f / sum : 0.f;
+          if (a.lse != nullptr)
+            a.lse[((long long)cur.b * a.H + h) * a.Sq + i] =
+                sees ? lse2 * kLn2 + (kMode != 0 && a.alibi != nullptr ? a.alibi[h] * (float)info->bias0[tid] : 0.f) : -CUDART_INF_F;
+          if (wk.stat != nullptr) wk.stat[((long long)cur.b * a.Hkv + cur.kvh) * wk.R + r] = lse2;
         } else {
-          float *po = wk.part_o + (slot * kRows + in_block) * D + 2 * t;
-#pragma unroll
-          for (int n = 0; n < kNT; ++n) *reinterpret_cast<float2 *>(po + n * 8) = make_float2(o[n][2 * rr], o[n][2 * rr + 1]);
-          if (t == 0) *reinterpret_cast<float2 *>(wk.part_ml + (slot * kRows + in_block) * 2) = make_float2(m[rr], l[rr]);
+          *reinterpret_cast<float2 *>(wk.part_ml + (slot * N + tid) * 2) = make_float2(info->ref[tid], sum);
         }
       }
-    }
-    left -= part1 - part0;
-    if (left > 0) next_unit(cur);
+      wg_sync();
+#pragma unroll 1
+      for (int half = 0; half < H; ++half) {
+        float o[N];
+        if (b0 < b1) {
+          tmem_ld_n<N>(tmem + lane_off + C::kO + half * N, o);
+        } else {
+#pragma unroll
+          for (int r = 0; r < N; ++r) o[r] = 0.f;
+        }
+        if (tid >= C::kDH) continue;
+        const int ch = half * 128 + tid;
+        if (whole) {
+#pragma unroll
+          for (int r = 0; r < N; ++r)
+            if (r < rows) {
+              const int i = (row0 + r) / a.group, h = cur.kvh * a.group + (row0 + r) % a.group;
+              const bool sees = info->hi[r] > info->lo[r];
+              static_cast<T *>(a.o)[cur.b * a.os[0] + i * a.os[1] + h * a.os[2] + ch] = Elem<T>::from_f(sees ? o[r] * info->inv[r] : 0.f);
+            }
+        } else {
+          float *po = wk.part_o + slot * N * D + ch;
+#pragma unroll
+          for (int r = 0; r < N; ++r)
+            if (r < rows) po[r * D] = o[r];
+        }
+      }
+      tc_fence_before();  // O^T is read before the next part's products write it
+      wg_sync();          // and the rows' values before they are set anew
+    } while (cur.next(a, wk, N));
   }
-  cp_async_wait<0>();
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kStepMma) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
 }
 
 // O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the shares of a unit
-// that several CTAs have: a CTA a unit, a warp a row, a lane D / 32 channels.
+// that several CTAs have: a warp a row, a lane D / 32 channels, four rows a CTA.
+constexpr int kMergeThreads = 128;
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_constant__ AttnArgs a,
-                                                                const __grid_constant__ StepWork wk, int rows) {
+__global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid_constant__ AttnArgs a,
+                                                                     const __grid_constant__ StepWork wk, int rows) {
   constexpr int E = D / 32;
   __shared__ ScanShared sh;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int unit = blockIdx.x;
   const int rb = unit % wk.nrb, kvh = unit / wk.nrb % a.Hkv, b = unit / wk.nrb / a.Hkv;
-  scan_steps(a, wk, rows, sh, [b](int x, long long, long long) { return x == b; });
+  const int in_block = blockIdx.y * (kMergeThreads / 32) + warp;
+  scan_steps(a, wk, rows, sh, [b](int x, long long, long long, long long) { return x == b; });
   const long long total = sh.total;
-  long long first = sh.before + steps_of(a, wk, rows, b) / a.Hkv * kvh;
+  long long first = sh.before + sh.steps / a.Hkv * kvh;
   for (int i = 0; i < rb; ++i) first += span_of(a, wk.R, rows, b, i).steps();
   const Span sp = span_of(a, wk.R, rows, b, rb);
   const int n = share_count(wk, total);
@@ -599,9 +799,9 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (used <= 1) return;
   constexpr float kShift = weight_shift<T>();
-  for (int in_block = warp; in_block < rows; in_block += kWarps) {
+  {
     const int r = rb * rows + in_block;
-    if (r >= wk.R) break;
+    if (in_block >= rows || r >= wk.R) return;
     auto slot = [&](int s) { return (2LL * (w0 + s) + (s == 0 ? 1 : 0)) * rows + in_block; };
     // The maximum first (a lane a share), then the weighted sums.
     float m = -CUDART_INF_F;
@@ -635,7 +835,7 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
       }
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
-        const float w = ex2(ml[u].x - base);
+        const float w = ex2_approx(ml[u].x - base);
         l = fmaf(w, ml[u].y, l);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = fmaf(w, x[u][e], o[e]);
@@ -653,7 +853,7 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
       if (a.lse != nullptr) {
         const float slope = a.alibi != nullptr ? a.alibi[h] : 0.f;
         a.lse[((long long)b * a.H + h) * a.Sq + i] =
-            sees ? lse2 * kPagedLn2 + (a.alibi != nullptr ? slope * (float)alibi_ref(v, slope) : 0.f) : -CUDART_INF_F;
+            sees ? lse2 * kLn2 + (a.alibi != nullptr ? slope * (float)alibi_ref(v, slope) : 0.f) : -CUDART_INF_F;
       }
       if (wk.stat != nullptr) wk.stat[((long long)b * a.Hkv + kvh) * wk.R + r] = lse2;
     }
@@ -663,22 +863,23 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const __grid_cons
 // The weight of each cached token from the scores that the attention left:
 // sum over rows of 2^(score - lse2).  A thread has four tokens.
 constexpr int kWeightRows = 64;  // rows whose sums lie in shared memory at a time
-__global__ void __launch_bounds__(kThreads) paged_weights_kernel(const __grid_constant__ AttnArgs a,
+constexpr int kWeightThreads = 128;
+__global__ void __launch_bounds__(kWeightThreads) paged_weights_kernel(const __grid_constant__ AttnArgs a,
                                                                   const __grid_constant__ StepWork wk) {
   __shared__ float lse2[kWeightRows];
   __shared__ Visible vis[kWeightRows];
   const int unit = blockIdx.y;
   const int b = unit / a.Hkv, kvh = unit % a.Hkv;
   const int ql = clamp_len(a.q_lens, b, a.Sq), kl = clamp_len(a.kv_lens, b, a.Skv);
-  const int j0 = (blockIdx.x * kThreads + threadIdx.x) * 4;
+  const int j0 = (blockIdx.x * kWeightThreads + threadIdx.x) * 4;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if ((int)blockIdx.x * kThreads * 4 >= kl) return;
+  if ((int)blockIdx.x * kWeightThreads * 4 >= kl) return;
   float w[4] = {0.f, 0.f, 0.f, 0.f};
   const int R = min(wk.R, ql * a.group);
   for (int r0 = 0; r0 < R; r0 += kWeightRows) {
     __syncthreads();
     const int n = min(kWeightRows, R - r0);
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += kWeightThreads) {
       const int r = r0 + i;
       lse2[i] = wk.stat[(long long)unit * wk.R + r];
       vis[i] = row_visible(a, r / a.group, ql, kl);
@@ -694,7 +895,7 @@ __global__ void __launch_bounds__(kThreads) paged_weights_kernel(const __grid_co
       const float xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (j0 + e >= v.lo && j0 + e < v.hi) w[e] += ex2(xs[e] - lse2[i]);
+        if (j0 + e >= v.lo && j0 + e < v.hi) w[e] += ex2_approx(xs[e] - lse2[i]);
     }
   }
   if (j0 >= kl) return;
@@ -711,14 +912,17 @@ __global__ void __launch_bounds__(kThreads) paged_weights_kernel(const __grid_co
 
 // -------------------------------------------------------------------- host
 struct StepPlan {
-  int rt;  // row tiles: 1, 2 or 4
+  int rows;  // of a block: 16, 32 or 64
   int workers;
   bool split;
   size_t part_bytes, stat_bytes, score_bytes;
   long long pitch;
 };
 
-int ctas_of(int D) { return D == 64 ? StepCfg<64>::kCtas : (D == 128 ? StepCfg<128>::kCtas : StepCfg<256>::kCtas); }
+template <int N>
+constexpr int ctas_of(int D) {
+  return D == 64 ? StepCfg<64, N>::kCtas : (D == 128 ? StepCfg<128, N>::kCtas : StepCfg<256, N>::kCtas);
+}
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -726,52 +930,60 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 StepPlan plan_step(const AttnArgs &a, bool weights, bool scores) {
   StepPlan p{};
   const long long R = (long long)a.Sq * a.group;
-  p.rt = R <= 16 ? 1 : (R <= 32 ? 2 : 4);
-  const int rows = 16 * p.rt;
-  p.workers = a.num_sms * ctas_of(a.D);
-  // Up to four steps a unit there is too little to share.
-  p.split = a.Skv > 4 * kStep;
-  p.part_bytes = p.split ? up256((size_t)2 * p.workers * rows * (a.D + 2) * sizeof(float)) : 0;
+  p.rows = R <= 16 ? 16 : (R <= 32 || a.D != 256 ? 32 : 64);
+  p.workers = a.num_sms * (p.rows == 16 ? ctas_of<16>(a.D) : (p.rows == 32 ? ctas_of<32>(a.D) : StepCfg<256, 64>::kCtas));
+  // Up to two blocks a unit there is too little to share.
+  p.split = a.Skv > 2 * kBN;
+  p.part_bytes = p.split ? up256((size_t)2 * p.workers * p.rows * (a.D + 2) * sizeof(float)) : 0;
   p.stat_bytes = weights ? up256((size_t)a.B * a.Hkv * R * sizeof(float)) : 0;
   p.pitch = ((long long)a.Skv + 15) / 16 * 16;
   p.score_bytes = scores ? up256((size_t)a.B * a.Hkv * R * p.pitch * sizeof(float)) : 0;
   return p;
 }
 
-template <typename T, int D, int RT>
+template <typename T, int D, int N, int kMode>
 cudaError_t launch_step_t(const AttnArgs &a, const StepWork &wk, long long units, cudaStream_t s) {
-  auto kern = paged_step_kernel<T, D, RT>;
+  using C = StepCfg<D, N>;
+  CUtensorMap tk, tv;
+  if (!make_page_map(&tk, wk.c, wk.c.k, wk.c.ks, a.dtype, wk.box) || !make_page_map(&tv, wk.c, wk.c.v, wk.c.vs, a.dtype, wk.box))
+    return cudaErrorInvalidValue;
+  auto kern = paged_step_kernel<T, D, N, kMode>;
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [&] {
-    attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, StepCfg<D>::kSmem);
-  });
+  std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem); });
   if (attr != cudaSuccess) return attr;
   const unsigned grid = (unsigned)(wk.split ? wk.workers : units);
-  kern<<<grid, kThreads, StepCfg<D>::kSmem, s>>>(a, wk);
+  kern<<<grid, kStepThreads, C::kSmem, s>>>(tk, tv, a, wk);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (wk.split) e = launch_paged_after(paged_merge_kernel<T, D>, dim3((unsigned)units), kThreads, 0, s, a, wk, 16 * RT);
+  if (wk.split) {
+    const dim3 grid_m((unsigned)units, (unsigned)((std::min(wk.R, N) + 3) / 4));
+    e = launch_paged_after(paged_merge_kernel<T, D>, grid_m, kMergeThreads, 0, s, a, wk, N);
+  }
   if (e != cudaSuccess || wk.score == nullptr) return e;
-  const dim3 grid_w((unsigned)((a.Skv + kThreads * 4 - 1) / (kThreads * 4)), (unsigned)(a.B * a.Hkv));
-  return launch_paged_after(paged_weights_kernel, grid_w, kThreads, 0, s, a, wk);
+  const dim3 grid_w((unsigned)((a.Skv + kWeightThreads * 4 - 1) / (kWeightThreads * 4)), (unsigned)(a.B * a.Hkv));
+  return launch_paged_after(paged_weights_kernel, grid_w, kWeightThreads, 0, s, a, wk);
 }
 
+template <typename T, int D, int N>
+cudaError_t launch_step_m(const AttnArgs &a, const StepWork &wk, long long units, cudaStream_t s) {
+  if (a.softcap > 0.f) return launch_step_t<T, D, N, 2>(a, wk, units, s);
+  return a.alibi != nullptr ? launch_step_t<T, D, N, 1>(a, wk, units, s) : launch_step_t<T, D, N, 0>(a, wk, units, s);
+}
 template <typename T, int D>
-cudaError_t launch_step_r(const AttnArgs &a, const StepWork &wk, int rt, long long units, cudaStream_t s) {
-  switch (rt) {
-    case 1: return launch_step_t<T, D, 1>(a, wk, units, s);
-    case 2: return launch_step_t<T, D, 2>(a, wk, units, s);
-    default: return launch_step_t<T, D, 4>(a, wk, units, s);
-  }
+cudaError_t launch_step_r(const AttnArgs &a, const StepWork &wk, int rows, long long units, cudaStream_t s) {
+  if (rows == 16) return launch_step_m<T, D, 16>(a, wk, units, s);
+  if constexpr (D == 256)
+    if (rows == 64) return launch_step_m<T, D, 64>(a, wk, units, s);
+  return launch_step_m<T, D, 32>(a, wk, units, s);
 }
 
 template <typename T>
-cudaError_t launch_step_d(const AttnArgs &a, const StepWork &wk, int rt, long long units, cudaStream_t s) {
+cudaError_t launch_step_d(const AttnArgs &a, const StepWork &wk, int rows, long long units, cudaStream_t s) {
   switch (a.D) {
-    case 64: return launch_step_r<T, 64>(a, wk, rt, units, s);
-    case 128: return launch_step_r<T, 128>(a, wk, rt, units, s);
-    case 256: return launch_step_r<T, 256>(a, wk, rt, units, s);
+    case 64: return launch_step_r<T, 64>(a, wk, rows, units, s);
+    case 128: return launch_step_r<T, 128>(a, wk, rows, units, s);
+    case 256: return launch_step_r<T, 256>(a, wk, rows, units, s);
   }
   return cudaErrorNotSupported;
 }
@@ -780,14 +992,16 @@ cudaError_t launch_step(const AttnArgs &a, const PagedArgs &c, const StepPlan &p
   StepWork wk{};
   wk.c = c;
   wk.R = a.Sq * a.group;
-  wk.nrb = (wk.R + 16 * p.rt - 1) / (16 * p.rt);
+  wk.nrb = (wk.R + p.rows - 1) / p.rows;
   wk.workers = p.workers;
-  wk.min_steps = 4;
+  wk.min_steps = 2;
   wk.split = p.split;
+  wk.reverse = a.alibi != nullptr;
+  wk.box = std::gcd(c.page_size, kBN);
   unsigned char *at = static_cast<unsigned char *>(ws);
   if (p.split) {
     wk.part_o = reinterpret_cast<float *>(at);
-    wk.part_ml = wk.part_o + (size_t)2 * p.workers * 16 * p.rt * a.D;
+    wk.part_ml = wk.part_o + (size_t)2 * p.workers * p.rows * a.D;
     at += p.part_bytes;
   }
   if (p.stat_bytes != 0) wk.stat = reinterpret_cast<float *>(at);
@@ -795,8 +1009,8 @@ cudaError_t launch_step(const AttnArgs &a, const PagedArgs &c, const StepPlan &p
   wk.pitch = p.pitch;
   wk.decay = decay;
   const long long units = (long long)a.B * a.Hkv * wk.nrb;
-  return a.dtype == LLMX_FP16 ? launch_step_d<__half>(a, wk, p.rt, units, s)
-                              : launch_step_d<__nv_bfloat16>(a, wk, p.rt, units, s);
+  return a.dtype == LLMX_FP16 ? launch_step_d<__half>(a, wk, p.rows, units, s)
+                              : launch_step_d<__nv_bfloat16>(a, wk, p.rows, units, s);
 }
 
 llmx_status bad(const char *msg) { return record_error(LLMX_ERR_INVALID_ARGUMENT, msg); }
@@ -821,6 +1035,11 @@ llmx_status prepare(const llmx_attn_params *p, const llmx_paged_cache *c, AttnAr
       return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: strides of q and o must be multiples of 8");
     if (extent[i] > 1 && a->os[i] == 0) return bad("paged attention: rows of o must not overlap (stride 0)");
   }
+  // Bytes of a stride of a tensor map stay below 2^40.
+  const int kv_extent[3] = {k->n_pages, k->Hkv, k->page_size};
+  for (int i = 0; i < 3; ++i)
+    if (kv_extent[i] > 1 && (k->ks[i] >= (1LL << 39) || k->vs[i] >= (1LL << 39)))
+      return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: strides of the cache must stay below 2^39 elements");
   const long long blocks = (long long)a->B * a->Hkv * (((long long)a->Sq * a->group + 15) / 16);
   if (blocks > INT_MAX / 2 || (k->w != nullptr && (long long)a->B * a->Hkv > 65535))
     return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: too many sequences, heads and rows for one call");
@@ -845,7 +1064,7 @@ constexpr int kScoreRows = 32;
 constexpr size_t kScoreBytes = size_t(1) << 30;
 
 llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs &k, Plan *plan) {
-  const bool can = paged_tc_supports(a, k);
+  const bool can = paged_tc_supports(a);
   if (p->algo == LLMX_ALGO_TCGEN05 && !can)
     return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: TCGEN05 needs head_dim 64 or 128, sm_scale > 0 and at most 128 "
                                               "query heads a kv head");
@@ -859,7 +1078,7 @@ llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs
     plan->bytes = plan->stat_at + (weights ? (size_t)a.B * a.Hkv * R * sizeof(float) : 0);
   } else {
     plan->step = plan_step(a, weights, weights);
-    plan->again = weights && (R > kScoreRows || plan->step.score_bytes > kScoreBytes) && a.sm_scale > 0.f && paged_weights_supports(a, k);
+    plan->again = weights && (R > kScoreRows || plan->step.score_bytes > kScoreBytes) && a.sm_scale > 0.f && paged_weights_supports(a);
     if (plan->again) plan->step.score_bytes = 0;
     plan->stat_at = plan->step.part_bytes;
     plan->bytes = plan->step.part_bytes + plan->step.stat_bytes + plan->step.score_bytes;

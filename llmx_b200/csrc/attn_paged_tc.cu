@@ -736,13 +736,13 @@ cudaError_t launch_tc_d(const AttnArgs &a, const TcWork &wk, int grid, int *ctr,
 
 }  // namespace
 
-bool paged_tc_supports(const AttnArgs &a, const PagedArgs &c) {
+bool paged_tc_supports(const AttnArgs &a) {
   // The softmax takes the row max on raw scores (sm_scale > 0).
   if ((a.D != 64 && a.D != 128) || !(a.sm_scale > 0.f) || a.group > kBM) return false;
   const long long units = (long long)a.B * a.Hkv;
   const long long M = kBM / a.group * a.group;
   if (units * (((long long)a.Sq * a.group + 2 * M - 1) / (2 * M)) > INT_MAX / 128) return false;
-  return paged_weights_supports(a, c);
+  return paged_weights_supports(a);
 }
 
 PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws) {

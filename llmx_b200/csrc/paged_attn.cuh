@@ -10,8 +10,8 @@
 
 namespace llmx_b200 {
 
-constexpr float kPagedLog2e = 1.4426950408889634f;
-constexpr float kPagedLn2 = 0.6931471805599453f;
+
+
 
 // The tokens [lo, hi) that query row i of a sequence sees (empty: lo >= hi).
 struct Visible {
@@ -39,14 +39,14 @@ struct PagedTcPlan {
   int M, n_mblocks, n_whole, parts, n_work;
   size_t part_bytes;
 };
-bool paged_tc_supports(const AttnArgs &a, const PagedArgs &c);
+bool paged_tc_supports(const AttnArgs &a);
 PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws);
 cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTcPlan &p, int *ctr, float *part, float *stat,
                             cudaStream_t s);
 
 // Key weights of a chunk from the rows' sums (paged_weights.cu), after the
 // attention that wrote them.
-bool paged_weights_supports(const AttnArgs &a, const PagedArgs &c);
+bool paged_weights_supports(const AttnArgs &a);
 cudaError_t launch_paged_weights(const AttnArgs &a, const PagedArgs &c, const float *stat, float decay, cudaStream_t s);
 
 // A launch that may be set up while the kernel before it still runs (it waits

@@ -394,15 +394,13 @@ cudaError_t launch_weight(const AttnArgs &a, const WeightWork &wk, cudaStream_t 
 
 }  // namespace
 
-bool paged_weights_supports(const AttnArgs &a, const PagedArgs &c) {
-  // A block holds whole groups.  Bytes of a stride of a tensor map stay below 2^40.
+bool paged_weights_supports(const AttnArgs &a) {
+  // A block holds whole groups.  Bytes of a stride of q's tensor map stay below 2^40.
   if (a.group > kBM) return false;
   if ((long long)a.B * a.Hkv * ((a.Skv + kBN - 1) / kBN) > INT_MAX / 2) return false;
-  const int extent[3] = {a.B, a.Sq, a.H}, kv_extent[3] = {c.n_pages, c.Hkv, c.page_size};
-  for (int i = 0; i < 3; ++i) {
+  const int extent[3] = {a.B, a.Sq, a.H};
+  for (int i = 0; i < 3; ++i)
     if (extent[i] > 1 && (a.qs[i] == 0 || a.qs[i] >= (1LL << 39))) return false;
-    if (kv_extent[i] > 1 && (c.ks[i] >= (1LL << 39) || c.vs[i] >= (1LL << 39))) return false;
-  }
   return true;
 }
 
