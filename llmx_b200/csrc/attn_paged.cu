@@ -65,14 +65,16 @@ struct StepWork {
 };
 
 // Row block rb of sequence b: blocks of 128 tokens lo128 + 128 i .., tokens in
-// [lo, hi) are visible to some row.  At least one step, which may have no token.
+// [lo, hi) are visible to some row.  A unit's steps are its blocks and, before
+// them, kUnitSteps that stand for what starting and ending a unit costs.
+constexpr int kUnitSteps = 2;
 struct Span {
   int ql, kl, lo, hi, all_lo, all_hi;
   __device__ __forceinline__ int lo128() const { return lo & ~(kBN - 1); }
   __device__ __forceinline__ int blocks() const { return hi > lo ? (hi - lo128() + kBN - 1) / kBN : 0; }
-  __device__ __forceinline__ int steps() const { return max(1, blocks()); }
-  // First token of the unit's block in step `at`.
-  __device__ __forceinline__ int token(int at, int reverse) const { return lo128() + (reverse ? blocks() - 1 - at : at) * kBN; }
+  __device__ __forceinline__ int steps() const { return kUnitSteps + blocks(); }
+  // First token of the unit's i-th block.
+  __device__ __forceinline__ int token(int i, int reverse) const { return lo128() + (reverse ? blocks() - 1 - i : i) * kBN; }
 };
 __device__ __forceinline__ Span span_of(const AttnArgs &a, int R, int rows, int b, int rb) {
   Span s;
@@ -87,24 +89,22 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int R, int rows, int 
   return s;
 }
 
-// Steps of all units of sequence b.
-__device__ __forceinline__ long long steps_of(const AttnArgs &a, const StepWork &wk, int rows, int b) {
-  long long n = 0;
+// Steps of all units of sequence b.  (All steps of a launch stay below 2^31:
+// plan_step.)
+__device__ __forceinline__ int steps_of(const AttnArgs &a, const StepWork &wk, int rows, int b) {
+  int n = 0;
   for (int rb = 0; rb < wk.nrb; ++rb) n += span_of(a, wk.R, rows, b, rb).steps();
   return n * a.Hkv;
 }
 
 // Shares: worker w of n has the steps [total * w / n, total * (w + 1) / n).
-__device__ __forceinline__ int share_count(const StepWork &wk, long long total) {
-  return (int)max(1LL, min((long long)wk.workers, total / wk.min_steps));
+__device__ __forceinline__ int share_count(const StepWork &wk, int total) { return max(1, min(wk.workers, total / wk.min_steps)); }
+__device__ __forceinline__ int share_begin(int total, int w, int n) {
+  const int q = total / n, r = total - q * n;  // r, w <= n, a few per SM
+  return q * w + r * w / n;
 }
-__device__ __forceinline__ long long share_begin(long long total, int w, int n) {
-  const unsigned long long x = (unsigned long long)total * w;  // a division of 32 bits where that is enough
-  return x >> 32 ? x / n : (uint32_t)x / (uint32_t)n;
-}
-__device__ __forceinline__ int share_of(long long total, long long step, int n) {
-  const unsigned long long x = (unsigned long long)step * n;
-  int w = (int)(x >> 32 ? x / total : (uint32_t)x / (uint32_t)total);
+__device__ __forceinline__ int share_of(int total, int step, int n) {
+  int w = min(n - 1, (int)((float)step * (float)n / (float)total));  // within a few of it, put right
   while (w > 0 && share_begin(total, w, n) > step) --w;
   while (w < n - 1 && share_begin(total, w + 1, n) <= step) ++w;
   return w;
@@ -113,30 +113,30 @@ __device__ __forceinline__ int share_of(long long total, long long step, int n) 
 // A scan over the sequences by the whole CTA: the steps of all, then of the
 // sequence b that pick(b, before, steps, total) names, and the steps before it.
 struct ScanShared {
-  long long warp_sum[8];
-  long long before, steps, total;
+  int warp_sum[8];
+  int before, steps, total;
   int b;
 };
 template <typename F>
 __device__ void scan_steps(const AttnArgs &a, const StepWork &wk, int rows, ScanShared &sh, F pick) {
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, threads = blockDim.x;
   const int rounds = (a.B + threads - 1) / threads;
-  long long total = 0;
+  int total = 0;
   // With one round of threads the second pass has its numbers already.
   for (int pass = 0; pass < 2; ++pass) {
-    long long base = 0;
+    int base = 0;
     for (int round = 0; round < rounds; ++round) {
       const int b = round * threads + tid;
-      const long long mine = b < a.B ? steps_of(a, wk, rows, b) : 0;
-      long long x = mine;
+      const int mine = b < a.B ? steps_of(a, wk, rows, b) : 0;
+      int x = mine;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, x, off);
+        const int o = __shfl_up_sync(0xffffffffu, x, off);
         if (lane >= off) x += o;
       }
       if (lane == 31) sh.warp_sum[warp] = x;
       __syncthreads();
-      long long before = base + x - mine;
+      int before = base + x - mine;
       for (int w = 0; w < threads / 32; ++w) {
         if (w < warp) before += sh.warp_sum[w];
         base += sh.warp_sum[w];
@@ -157,10 +157,14 @@ __device__ void scan_steps(const AttnArgs &a, const StepWork &wk, int rows, Scan
 
 // A share's position: `left` steps from step `at` of unit (b, kvh, rb) on.
 struct Cursor {
-  int b, kvh, rb, at;
-  long long left;
+  int b, kvh, rb, at, left;
   Span sp;
-  __device__ __forceinline__ int end() const { return (int)min((long long)sp.steps(), at + left); }
+  __device__ __forceinline__ int end() const { return min(sp.steps(), at + left); }
+  // The part's blocks [first(), last()).  A part without any is not the unit's,
+  // but of a unit that has none the one with its first step is.
+  __device__ __forceinline__ int first() const { return max(0, at - kUnitSteps); }
+  __device__ __forceinline__ int last() const { return max(0, end() - kUnitSteps); }
+  __device__ __forceinline__ bool none() const { return sp.hi > sp.lo ? first() == last() : at > 0; }
   // Past this unit's part, to the next unit.  False at the share's end.
   __device__ __forceinline__ bool next(const AttnArgs &a, const StepWork &wk, int rows) {
     left -= end() - at;
@@ -189,7 +193,7 @@ struct StepCfg {
   static constexpr int kSlot = kBN * kDH * 2;
   static constexpr int kCtas = D == 256 || N == 64 || (D == 128 && N == 32) ? 1 : 2;
   static constexpr int kQ = N * D * 2, kP = N * kBN * 2;
-  static constexpr int kInfo = N == 16 ? 1280 : (N == 32 ? 2048 : 4096);  // RowInfo, barriers
+  static constexpr int kInfo = N == 16 ? 1280 : (N == 32 ? 2304 : 4352);  // RowInfo, barriers
   static constexpr int kBudget = (kCtas == 2 ? 113 : 227) * 1024 - 1024 - 256;  // less alignment and static arrays
   static constexpr int kFit = (kBudget - kQ - 2 * kP - kInfo) / kSlot;
   static constexpr int kSlots = kFit < 12 ? kFit : 12;
@@ -204,6 +208,7 @@ struct StepCfg {
 
 template <int N>
 struct RowInfo {
+  long long out[N];  // where the row's output begins
   float base[N];   // what is subtracted from a score: the reference less the weights' shift
   float limit[N];  // scores above it move the reference; -inf before the first
   float ref[N];    // the reference
@@ -398,21 +403,21 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
   Cursor cur;
   const int worker = blockIdx.x;
   if (wk.split) {
-    scan_steps(a, wk, N, sh, [&](int, long long before, long long steps, long long total) {
+    scan_steps(a, wk, N, sh, [&](int, int before, int steps, int total) {
       const int n = share_count(wk, total);
       if (worker >= n) return false;
-      const long long begin = share_begin(total, worker, n);
+      const int begin = share_begin(total, worker, n);
       return before <= begin && begin < before + steps;
     });
-    const long long total = sh.total;
+    const int total = sh.total;
     const int n = share_count(wk, total);
     if (worker >= n) return;
-    const long long begin = share_begin(total, worker, n);
+    const int begin = share_begin(total, worker, n);
     cur.left = share_begin(total, worker + 1, n) - begin;
     if (cur.left <= 0) return;
     cur.b = sh.b;
-    long long within = begin - sh.before;
-    const long long per_head = sh.steps / a.Hkv;
+    int within = begin - sh.before;
+    const int per_head = sh.steps / a.Hkv;
     cur.kvh = (int)(within / per_head);
     within -= cur.kvh * per_head;
     for (cur.rb = 0;; ++cur.rb) {
@@ -458,14 +463,14 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
       }
     };
     do {
-      const int b1 = cur.sp.hi > cur.sp.lo ? cur.end() : cur.at;
+      const int b0 = cur.first(), b1 = cur.last();
       BoxPlace kp, vp;
-      if (cur.at < b1) {
-        kp = box_place(wk.c, wk.box, cur.b, cur.sp.kl, cur.sp.token(cur.at, wk.reverse));
+      if (b0 < b1) {
+        kp = box_place(wk.c, wk.box, cur.b, cur.sp.kl, cur.sp.token(b0, wk.reverse));
         vp = kp;
         copy(&tm_k, kp);
       }
-      for (int j = cur.at; j < b1 && ok; ++j) {
+      for (int j = b0; j < b1 && ok; ++j) {
         if (j + 1 < b1) {
           kp = box_place(wk.c, wk.box, cur.b, cur.sp.kl, cur.sp.token(j + 1, wk.reverse));
           copy(&tm_k, kp);
@@ -504,13 +509,13 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
         if (ok) tc_commit(&bars->s_full[at & 1]);
       };
       do {
-        const int b1 = cur.sp.hi > cur.sp.lo ? cur.end() : cur.at;
-        if (cur.at >= b1) continue;
+        const int b0 = cur.first(), b1 = cur.last();
+        if (b0 == b1) continue;
         ok = wait(&bars->q_full, parts & 1);
         ++parts;
         if (!ok) break;
         scores(blk);
-        for (int j = cur.at; j < b1 && ok; ++j, ++blk) {
+        for (int j = b0; j < b1 && ok; ++j, ++blk) {
           if (j + 1 < b1) scores(blk + 1);
           if (!ok) break;
           ok = wait(&bars->p_full[blk & 1], (blk >> 1) & 1);
@@ -529,7 +534,7 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
 #pragma unroll
             for (int kk = 0; kk < kBN / 16; ++kk)
               mma_ss(tmem + C::kO + half * N, da + (uint64_t)((kk * 16 * 128) >> 4), db + (uint64_t)((kk * 256) >> 4), idesc_o,
-                     (j > cur.at || kk > 0) ? 1u : 0u);
+                     (j > b0 || kk > 0) ? 1u : 0u);
             tc_commit(&bars->empty[s]);
           }
           if (ok) tc_commit(&bars->o_done[blk & 1]);
@@ -553,37 +558,60 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
       if (!w && ok) set_abort(bars, a.err);
       ok = ok && w;
     };
-    do {
+    // Q [row][64 channels] in 128 bytes a row, chunk c at c ^ (row % 8).  The next
+    // part's rows are read while this one's blocks pass (at 64 rows: with it).
+    constexpr int kPieces = N * D / 8 / 128;  // of a thread
+    constexpr bool kAhead = kPieces <= 8;
+    uint4 qx[kPieces];
+    auto read_q = [&](const Cursor &c) {
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        const int r = (u * 128 + tid) / (D / 8), ch = (u * 128 + tid) % (D / 8);
+        const int pr = c.rb * N + r, i = pr / a.group;
+        qx[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (pr < wk.R && i < c.sp.ql && c.first() < c.last())
+          qx[u] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + c.b * a.qs[0] + i * a.qs[1] +
+                                                   (c.kvh * a.group + pr - i * a.group) * a.qs[2] + ch * 8);
+      }
+    };
+    if (kAhead) read_q(cur);
+    for (bool more = true; more;) {
+      Cursor nx = cur;
+      const bool none = cur.none();
+      more = nx.next(a, wk, N);
+      if (none) {
+        cur = nx;
+        if (kAhead && more) read_q(cur);
+        continue;
+      }
       const Span sp = cur.sp;
-      const int b0 = cur.at, e0 = cur.end(), b1 = sp.hi > sp.lo ? e0 : b0;
+      const int b0 = cur.first(), b1 = cur.last();
       const int row0 = cur.rb * N, rows = min(N, wk.R - row0);
-      // Everything of the last part has been read (the barriers at its end).
+      if (!kAhead) read_q(cur);
+      // Everything of the last part has been read (the barrier at its end).
       if (tid < N) {
-        const int r = row0 + tid, i = r / a.group;
+        const int r = row0 + tid, i = r / a.group, h = cur.kvh * a.group + r - i * a.group;
         const bool real = tid < rows && i < sp.ql;
         const Visible v = real ? row_visible(a, i, sp.ql, sp.kl) : Visible{0, 0};
-        const float slope = kMode != 0 && a.alibi != nullptr && real ? a.alibi[cur.kvh * a.group + r % a.group] : 0.f;
+        const float slope = kMode != 0 && a.alibi != nullptr && real ? a.alibi[h] : 0.f;
         info->lo[tid] = v.lo;
         info->hi[tid] = v.hi;
         info->slope2[tid] = slope * kLog2e;
         info->bias0[tid] = alibi_ref(v, slope);
         info->ref[tid] = info->limit[tid] = -CUDART_INF_F;
         info->base[tid] = -kShift;
+        info->out[tid] = cur.b * a.os[0] + i * a.os[1] + h * a.os[2];
       }
       if (b0 < b1) {
-        // Q [row][64 channels] in 128 bytes a row, chunk c at c ^ (row % 8).
-        for (int u = tid; u < N * D / 8; u += 128) {
-          const int r = u / (D / 8), c = u % (D / 8);
-          const int pr = row0 + r, i = pr / a.group;
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (r < rows && i < sp.ql)
-            x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + cur.b * a.qs[0] + i * a.qs[1] +
-                                                 (cur.kvh * a.group + pr - i * a.group) * a.qs[2] + c * 8);
-          *reinterpret_cast<uint4 *>(smem + C::kQOff + (c / 8) * N * 128 + r * 128 + (((c % 8) ^ (r & 7)) << 4)) = x;
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+          const int r = (u * 128 + tid) / (D / 8), c = (u * 128 + tid) % (D / 8);
+          *reinterpret_cast<uint4 *>(smem + C::kQOff + (c / 8) * N * 128 + r * 128 + (((c % 8) ^ (r & 7)) << 4)) = qx[u];
         }
         fence_proxy_async_smem();
         mbar_arrive(&bars->q_full);
       }
+      if (kAhead && more) read_q(nx);
       wg_sync();  // the rows' values
       float l[N];
 #pragma unroll
@@ -615,18 +643,24 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
           }
         }
         if (part) {
+          // Tokens that no row sees are zeros in V; ones that only some rows see must
+          // not hand an infinity or NaN to the others.
+          const bool none = j < sp.lo || j >= sp.hi, some = j < sp.all_lo || j >= sp.all_hi;
           bool lost = false;
           const int v0 = g + H * (min(at - b0 + 2, b1 - b0) + at - b0);  // V's first slot of the block
-#pragma unroll
+#pragma unroll 1
           for (int half = 0; half < H; ++half) {
             const int s = (v0 + half) % C::kSlots;
             wait_all(&bars->full[s], ((v0 + half) / C::kSlots) & 1);
-            if (ok) lost |= clean_row<T, C::kDH>(smem + s * C::kSlot, tid, j < sp.lo || j >= sp.hi);
+            if (some && ok) lost |= clean_row<T, C::kDH>(smem + s * C::kSlot, tid, none);
           }
 #pragma unroll
-          for (int r = 0; r < N; ++r) {
-            const bool vis = j >= info->lo[r] && j < info->hi[r];
-            x[r] = vis ? (lost ? CUDART_NAN_F : x[r]) : -CUDART_INF_F;
+          for (int r = 0; r < N; r += 4) {
+            const int4 lo = *reinterpret_cast<const int4 *>(&info->lo[r]), hi = *reinterpret_cast<const int4 *>(&info->hi[r]);
+            const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[r + e] = j >= l4[e] && j < h4[e] ? (lost ? CUDART_NAN_F : x[r + e]) : -CUDART_INF_F;
           }
         }
         if (wk.score != nullptr && j < wk.pitch) {
@@ -665,7 +699,13 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
           }
           wg_sync();
 #pragma unroll
-          for (int r = 0; r < N; ++r) l[r] *= info->alpha[r];
+          for (int r = 0; r < N; r += 4) {
+            const float4 al = *reinterpret_cast<const float4 *>(&info->alpha[r]);
+            l[r] *= al.x;
+            l[r + 1] *= al.y;
+            l[r + 2] *= al.z;
+            l[r + 3] *= al.w;
+          }
           if (at > b0) {
             // O^T holds the blocks before once their products are done.
             wait_all(&bars->o_done[(blk - 1) & 1], ((blk - 1) >> 1) & 1);
@@ -675,7 +715,13 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
               float o[N];
               tmem_ld_n<N>(tmem + lane_off + C::kO + half * N, o);
 #pragma unroll
-              for (int r = 0; r < N; ++r) o[r] *= info->alpha[r];
+              for (int r = 0; r < N; r += 4) {
+                const float4 al = *reinterpret_cast<const float4 *>(&info->alpha[r]);
+                o[r] *= al.x;
+                o[r + 1] *= al.y;
+                o[r + 2] *= al.z;
+                o[r + 3] *= al.w;
+              }
               tmem_st_n<N>(tmem + lane_off + C::kO + half * N, o);
             }
             tmem_wait_st();
@@ -715,8 +761,8 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
         tc_fence_after();
       }
       wg_sync();
-      const bool whole = b0 == 0 && e0 == sp.steps();
-      const long long slot = 2LL * worker + (b0 == 0 ? 1 : 0);
+      const bool whole = b0 == 0 && b1 == sp.blocks();
+      const long long slot = 2LL * worker + (cur.at == 0 ? 1 : 0);
       if (tid < rows) {
         const float sum = (info->wmax[0][tid] + info->wmax[1][tid]) + (info->wmax[2][tid] + info->wmax[3][tid]);
         const int r = row0 + tid;
@@ -748,11 +794,8 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
         if (whole) {
 #pragma unroll
           for (int r = 0; r < N; ++r)
-            if (r < rows) {
-              const int i = (row0 + r) / a.group, h = cur.kvh * a.group + (row0 + r) % a.group;
-              const bool sees = info->hi[r] > info->lo[r];
-              static_cast<T *>(a.o)[cur.b * a.os[0] + i * a.os[1] + h * a.os[2] + ch] = Elem<T>::from_f(sees ? o[r] * info->inv[r] : 0.f);
-            }
+            if (r < rows)
+              static_cast<T *>(a.o)[info->out[r] + ch] = Elem<T>::from_f(o[r] * info->inv[r]);  // 0 for a row that sees nothing
         } else {
           float *po = wk.part_o + slot * N * D + ch;
 #pragma unroll
@@ -762,7 +805,8 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
       }
       tc_fence_before();  // O^T is read before the next part's products write it
       wg_sync();          // and the rows' values before they are set anew
-    } while (cur.next(a, wk, N));
+      cur = nx;
+    }
   }
 
   tc_fence_before();
@@ -787,13 +831,16 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
   const int unit = blockIdx.x;
   const int rb = unit % wk.nrb, kvh = unit / wk.nrb % a.Hkv, b = unit / wk.nrb / a.Hkv;
   const int in_block = blockIdx.y * (kMergeThreads / 32) + warp;
-  scan_steps(a, wk, rows, sh, [b](int x, long long, long long, long long) { return x == b; });
-  const long long total = sh.total;
-  long long first = sh.before + sh.steps / a.Hkv * kvh;
+  scan_steps(a, wk, rows, sh, [b](int x, int, int, int) { return x == b; });
+  const int total = sh.total;
+  int first = sh.before + sh.steps / a.Hkv * kvh;
   for (int i = 0; i < rb; ++i) first += span_of(a, wk.R, rows, b, i).steps();
   const Span sp = span_of(a, wk.R, rows, b, rb);
   const int n = share_count(wk, total);
-  const int w0 = share_of(total, first, n), used = share_of(total, first + sp.steps() - 1, n) - w0 + 1;
+  // The shares from the one that has the unit's first block on.
+  const int w0 = share_of(total, first + min(kUnitSteps, sp.steps() - 1), n);
+  const int used = share_of(total, first + sp.steps() - 1, n) - w0 + 1;
+  const int slot0 = share_begin(total, w0, n) <= first ? 1 : 0;
   // Every thread waits for the shares, also where there is nothing to do, so
   // that this kernel ends after them.
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -802,7 +849,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_merge_kernel(const __grid
   {
     const int r = rb * rows + in_block;
     if (in_block >= rows || r >= wk.R) return;
-    auto slot = [&](int s) { return (2LL * (w0 + s) + (s == 0 ? 1 : 0)) * rows + in_block; };
+    auto slot = [&](int s) { return (2LL * (w0 + s) + (s == 0 ? slot0 : 0)) * rows + in_block; };
     // The maximum first (a lane a share), then the weighted sums.
     float m = -CUDART_INF_F;
     for (int s = lane; s < used; s += 32) m = fmaxf(m, wk.part_ml[slot(s) * 2]);
@@ -932,8 +979,9 @@ StepPlan plan_step(const AttnArgs &a, bool weights, bool scores) {
   const long long R = (long long)a.Sq * a.group;
   p.rows = R <= 16 ? 16 : (R <= 32 || a.D != 256 ? 32 : 64);
   p.workers = a.num_sms * (p.rows == 16 ? ctas_of<16>(a.D) : (p.rows == 32 ? ctas_of<32>(a.D) : StepCfg<256, 64>::kCtas));
-  // Up to two blocks a unit there is too little to share.
-  p.split = a.Skv > 2 * kBN;
+  // Up to two blocks a unit there is too little to share.  Steps are counted in 32 bits.
+  const double steps = (double)a.B * a.Hkv * ((R + p.rows - 1) / p.rows) * (a.Skv / kBN + 2 + kUnitSteps);
+  p.split = a.Skv > 2 * kBN && steps < 2147483647.0;
   p.part_bytes = p.split ? up256((size_t)2 * p.workers * p.rows * (a.D + 2) * sizeof(float)) : 0;
   p.stat_bytes = weights ? up256((size_t)a.B * a.Hkv * R * sizeof(float)) : 0;
   p.pitch = ((long long)a.Skv + 15) / 16 * 16;
@@ -994,7 +1042,7 @@ cudaError_t launch_step(const AttnArgs &a, const PagedArgs &c, const StepPlan &p
   wk.R = a.Sq * a.group;
   wk.nrb = (wk.R + p.rows - 1) / p.rows;
   wk.workers = p.workers;
-  wk.min_steps = 2;
+  wk.min_steps = 2 + kUnitSteps;
   wk.split = p.split;
   wk.reverse = a.alibi != nullptr;
   wk.box = std::gcd(c.page_size, kBN);
