@@ -20,9 +20,11 @@
 // result (unnormalised O, reference and sum; at most two a CTA) of one that it
 // shares, which a second, overlapped launch merges.
 //
-// A CTA: warps 0-3 softmax, warp 4 issues the products, warp 5 the copies: K and
-// V by TMA boxes from the pages into one ring of slots, in the order in which
-// they are used (K of a block comes before V of the block before it).
+// A CTA: one warpgroup for the softmax (two, each with half of the rows, from 32
+// rows on: the code that a cold instruction cache has to fetch stays small), a
+// warp that issues the products, and one for the copies: K and V by TMA boxes
+// from the pages into one ring of slots, in the order in which they are used (K
+// of a block comes before V of the block before it).
 //
 // Masked tokens.  A NaN or an infinity in K only reaches scores that are
 // replaced.  One in V would reach every row through 0 * V, so in blocks that not
@@ -41,8 +43,6 @@
 namespace llmx_b200 {
 namespace {
 
-constexpr int kStepThreads = 192;
-constexpr int kStepMma = 4, kStepTma = 5;  // warps
 constexpr int kStepRows = 32;  // AUTO: packed rows of a kv head up to which this form is taken
 constexpr size_t kCounterBytes = 256;
 
@@ -113,7 +113,7 @@ __device__ __forceinline__ int share_of(int total, int step, int n) {
 // A scan over the sequences by the whole CTA: the steps of all, then of the
 // sequence b that pick(b, before, steps, total) names, and the steps before it.
 struct ScanShared {
-  int warp_sum[8];
+  int warp_sum[12];
   int before, steps, total;
   int b;
 };
@@ -188,12 +188,16 @@ struct Cursor {
 // covered by the other), else one; about 200 KB of copies an SM either way.
 template <int D, int N>
 struct StepCfg {
+  static constexpr int kGroups = N == 16 ? 1 : 2;  // softmax warpgroups
+  static constexpr int kCols = N / kGroups;        // rows of one of them
+  static constexpr int kSoftmax = 128 * kGroups, kThreads = kSoftmax + 64;
+  static constexpr int kMmaWarp = 4 * kGroups, kTmaWarp = kMmaWarp + 1;
   static constexpr int kDH = D < 128 ? D : 128;  // channels of a slot
   static constexpr int kHalves = D / kDH;        // slots of a block of K or V
   static constexpr int kSlot = kBN * kDH * 2;
-  static constexpr int kCtas = D == 256 || N == 64 || (D == 128 && N == 32) ? 1 : 2;
+  static constexpr int kCtas = D == 256 || N > 16 ? 1 : 2;
   static constexpr int kQ = N * D * 2, kP = N * kBN * 2;
-  static constexpr int kInfo = N == 16 ? 1280 : (N == 32 ? 2304 : 4352);  // RowInfo, barriers
+  static constexpr int kInfo = N == 16 ? 1792 : (N == 32 ? 2816 : 4864);  // RowInfo, barriers
   static constexpr int kBudget = (kCtas == 2 ? 113 : 227) * 1024 - 1024 - 256;  // less alignment and static arrays
   static constexpr int kFit = (kBudget - kQ - 2 * kP - kInfo) / kSlot;
   static constexpr int kSlots = kFit < 12 ? kFit : 12;
@@ -202,8 +206,8 @@ struct StepCfg {
   static constexpr int kSmem = kInfoOff + kInfo + 1024;
   // Tensor memory: two score accumulators, then O^T (one for each 128 channels).
   static constexpr uint32_t kO = 2 * N;
-  static constexpr uint32_t kCols = N == 16 ? 64 : (N == 32 ? 128 : 256);
-  static_assert(2 * N + kHalves * N <= (int)kCols, "tensor memory");
+  static constexpr uint32_t kTmem = N == 16 ? 64 : (N == 32 ? 128 : 256);
+  static_assert(2 * N + kHalves * N <= (int)kTmem, "tensor memory");
 };
 
 template <int N>
@@ -222,6 +226,7 @@ struct RowInfo {
 struct SBars {
   uint64_t full[12], empty[12];
   uint64_t q_full, s_full[2], p_full[2], o_done[2], drain;  // [2]: by the block's parity
+  uint8_t lost[2][2][128];  // by the block's parity and the warpgroup: the token lost a value of V
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -276,18 +281,19 @@ __device__ __forceinline__ void tmem_st_n(uint32_t at, const float (&x)[N]) {
   }
 }
 
-// The four softmax warps: a barrier, and one with a vote.  These are not
-// bounded: every warp runs through all blocks of the share, also after an abort.
-__device__ __forceinline__ void wg_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool wg_any(bool p) {
+// The four warps of softmax warpgroup g: a barrier, and one with a vote.  These
+// are not bounded: every warp runs through all blocks of the share, also after
+// an abort.
+__device__ __forceinline__ void wg_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
+__device__ __forceinline__ bool wg_any(int g, bool p) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "bar.red.or.pred q, %2, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)p)
+      : "r"((uint32_t)p), "r"(1 + g)
       : "memory");
   return r != 0;
 }
@@ -324,48 +330,46 @@ __device__ __forceinline__ void put_rows(float *to, const float (&v)[N]) {
   }
 }
 
-// A token's channels of V in a slot (its row `r`): infinities and NaN become 0
-// (true if there was one), or everything does.  16-byte chunk c lies at chunk
-// c ^ (r % 8) of the row's 128 bytes.
-template <typename T, int DH>
-__device__ __forceinline__ bool clean_row(uint8_t *slot, int r, bool all) {
+// A token's channels of V in a slot (its row `r`), `n` 16-byte pieces from piece
+// `first` on: infinities and NaN become 0 (true if there was one), or everything
+// does.  Piece p lies in 64-channel chunk p / 8 at (p % 8) ^ (r % 8).
+template <typename T>
+__device__ __forceinline__ bool clean_row(uint8_t *slot, int r, int first, int n, bool all) {
   constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
   bool lost = false;
-#pragma unroll 1
-  for (int c = 0; c < DH / 64; ++c)
+#pragma unroll 2
+  for (int p = first; p < first + n; ++p) {
+    uint4 *const at = reinterpret_cast<uint4 *>(slot + (p / 8) * 128 * 128 + r * 128 + (((p % 8) ^ (r & 7)) << 4));
+    if (all) {
+      *at = make_uint4(0u, 0u, 0u, 0u);
+      continue;
+    }
+    const uint4 x = *at;
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    bool any = false;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint4 *const at = reinterpret_cast<uint4 *>(slot + c * 128 * 128 + r * 128 + ((k ^ (r & 7)) << 4));
-      if (all) {
-        *at = make_uint4(0u, 0u, 0u, 0u);
-        continue;
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t m = (w[e] & kExp) ^ kExp;  // a half that is 0: all exponent bits set
+      if ((m & 0xffffu) == 0u) {
+        w[e] &= 0xffff0000u;
+        any = true;
       }
-      const uint4 x = *at;
-      uint32_t w[4] = {x.x, x.y, x.z, x.w};
-      bool any = false;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t m = (w[e] & kExp) ^ kExp;  // a half that is 0: all exponent bits set
-        if ((m & 0xffffu) == 0u) {
-          w[e] &= 0xffff0000u;
-          any = true;
-        }
-        if ((m >> 16) == 0u) {
-          w[e] &= 0x0000ffffu;
-          any = true;
-        }
-      }
-      if (any) {
-        *at = make_uint4(w[0], w[1], w[2], w[3]);
-        lost = true;
+      if ((m >> 16) == 0u) {
+        w[e] &= 0x0000ffffu;
+        any = true;
       }
     }
+    if (any) {
+      *at = make_uint4(w[0], w[1], w[2], w[3]);
+      lost = true;
+    }
+  }
   return lost;
 }
 
 // kMode: 1 ALiBi, 2 a soft-cap (with ALiBi or without), 0 neither.
 template <typename T, int D, int N, int kMode>
-__global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
+__global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
     paged_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ AttnArgs a, const __grid_constant__ StepWork wk) {
   using C = StepCfg<D, N>;
@@ -384,17 +388,17 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
       mbar_init(&bars->full[i], 1);
       mbar_init(&bars->empty[i], 1);
     }
-    mbar_init(&bars->q_full, 128);
+    mbar_init(&bars->q_full, C::kSoftmax);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
-      mbar_init(&bars->p_full[i], 128);
+      mbar_init(&bars->p_full[i], C::kSoftmax);
       mbar_init(&bars->o_done[i], 1);
     }
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == kStepTma && lane == 0) {
+  if (warp == C::kTmaWarp && lane == 0) {
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
   }
@@ -435,8 +439,8 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
     cur.at = 0;
     cur.left = cur.sp.steps();
   }
-  if (warp == kStepMma) {
-    tmem_alloc(&bars->tmem_base, C::kCols);
+  if (warp == C::kMmaWarp) {
+    tmem_alloc(&bars->tmem_base, C::kTmem);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -445,7 +449,7 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
   const uint32_t tmem = bars->tmem_base;
   auto wait = [&](uint64_t *bar, uint32_t par) { return mbar_wait_or_abort(bar, par, kTimeoutNs, &bars->abort_flag); };
 
-  if (warp == kStepTma) {
+  if (warp == C::kTmaWarp) {
     // ---- copies, in the order K 0, K 1, V 0, K 2, V 1, ..
     int g = 0;  // slots filled
     bool ok = true;
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
     if (!ok) set_abort(bars, a.err);
     // Every copy issued lands before the CTA may exit.
     for (int i = max(0, g - C::kSlots); i < g; ++i) mbar_wait(&bars->full[i % C::kSlots], (i / C::kSlots) & 1, kTimeoutNs);
-  } else if (warp == kStepMma) {
+  } else if (warp == C::kMmaWarp) {
     if (lane == 0) {
       // ---- products: S^T(j + 1) is issued before O^T += .. (j)
       constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -545,9 +549,11 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
       mbar_wait(&bars->drain, 0, kTimeoutNs);
     }
   } else {
-    // ---- softmax: thread tid has token tid of each block, and channel tid (and
-    // tid + 128) of O^T
-    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+    // ---- softmax: a thread has a token of each block and a channel (or two) of
+    // O^T, and its warpgroup's rows c0 .. of them
+    constexpr int W = C::kCols;
+    const int wg = warp / 4, tok = tid % 128, c0 = wg * W;
+    const uint32_t lane_off = (uint32_t)(warp % 4 * 32) << 16;
     const float scale2 = a.sm_scale * kLog2e;
     const float cap_in = kMode == 2 ? a.sm_scale / a.softcap : 0.f, cap_out = a.softcap * kLog2e;
     constexpr float kShift = weight_shift<T>();
@@ -559,14 +565,14 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
       ok = ok && w;
     };
     // Q [row][64 channels] in 128 bytes a row, chunk c at c ^ (row % 8).  The next
-    // part's rows are read while this one's blocks pass (at 64 rows: with it).
-    constexpr int kPieces = N * D / 8 / 128;  // of a thread
-    constexpr bool kAhead = kPieces <= 8;
+    // part's rows are read while this one's blocks pass (where they are few).
+    constexpr int kPieces = N * D / 8 / C::kSoftmax;  // of a thread
+    constexpr bool kAhead = kPieces <= 4;
     uint4 qx[kPieces];
     auto read_q = [&](const Cursor &c) {
 #pragma unroll
       for (int u = 0; u < kPieces; ++u) {
-        const int r = (u * 128 + tid) / (D / 8), ch = (u * 128 + tid) % (D / 8);
+        const int r = (u * C::kSoftmax + tid) / (D / 8), ch = (u * C::kSoftmax + tid) % (D / 8);
         const int pr = c.rb * N + r, i = pr / a.group;
         qx[u] = make_uint4(0u, 0u, 0u, 0u);
         if (pr < wk.R && i < c.sp.ql && c.first() < c.last())
@@ -589,47 +595,47 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
       const int row0 = cur.rb * N, rows = min(N, wk.R - row0);
       if (!kAhead) read_q(cur);
       // Everything of the last part has been read (the barrier at its end).
-      if (tid < N) {
-        const int r = row0 + tid, i = r / a.group, h = cur.kvh * a.group + r - i * a.group;
-        const bool real = tid < rows && i < sp.ql;
+      if (tok < W) {
+        const int row = c0 + tok, r = row0 + row, i = r / a.group, h = cur.kvh * a.group + r - i * a.group;
+        const bool real = row < rows && i < sp.ql;
         const Visible v = real ? row_visible(a, i, sp.ql, sp.kl) : Visible{0, 0};
         const float slope = kMode != 0 && a.alibi != nullptr && real ? a.alibi[h] : 0.f;
-        info->lo[tid] = v.lo;
-        info->hi[tid] = v.hi;
-        info->slope2[tid] = slope * kLog2e;
-        info->bias0[tid] = alibi_ref(v, slope);
-        info->ref[tid] = info->limit[tid] = -CUDART_INF_F;
-        info->base[tid] = -kShift;
-        info->out[tid] = cur.b * a.os[0] + i * a.os[1] + h * a.os[2];
+        info->lo[row] = v.lo;
+        info->hi[row] = v.hi;
+        info->slope2[row] = slope * kLog2e;
+        info->bias0[row] = alibi_ref(v, slope);
+        info->ref[row] = info->limit[row] = -CUDART_INF_F;
+        info->base[row] = -kShift;
+        info->out[row] = cur.b * a.os[0] + i * a.os[1] + h * a.os[2];
       }
       if (b0 < b1) {
 #pragma unroll
         for (int u = 0; u < kPieces; ++u) {
-          const int r = (u * 128 + tid) / (D / 8), c = (u * 128 + tid) % (D / 8);
+          const int r = (u * C::kSoftmax + tid) / (D / 8), c = (u * C::kSoftmax + tid) % (D / 8);
           *reinterpret_cast<uint4 *>(smem + C::kQOff + (c / 8) * N * 128 + r * 128 + (((c % 8) ^ (r & 7)) << 4)) = qx[u];
         }
         fence_proxy_async_smem();
         mbar_arrive(&bars->q_full);
       }
       if (kAhead && more) read_q(nx);
-      wg_sync();  // the rows' values
-      float l[N];
+      wg_sync(wg);  // the rows' values
+      float l[W];
 #pragma unroll
-      for (int r = 0; r < N; ++r) l[r] = 0.f;
+      for (int r = 0; r < W; ++r) l[r] = 0.f;
 
       for (int at = b0; at < b1; ++at, ++blk) {
         const int buf = blk & 1;
         wait_all(&bars->s_full[buf], (blk >> 1) & 1);
         tc_fence_after();
-        float x[N];
-        tmem_ld_n<N>(tmem + lane_off + buf * N, x);
-        const int n0 = sp.token(at, wk.reverse), j = n0 + tid;
+        float x[W];
+        tmem_ld_n<W>(tmem + lane_off + buf * N + c0, x);
+        const int n0 = sp.token(at, wk.reverse), j = n0 + tok;
         const bool part = n0 < sp.all_lo || n0 + kBN > sp.all_hi;
 #pragma unroll
-        for (int r = 0; r < N; r += 4) {
+        for (int r = 0; r < W; r += 4) {
           if constexpr (kMode != 0) {
-            const float4 sl = *reinterpret_cast<const float4 *>(&info->slope2[r]);
-            const int4 b = *reinterpret_cast<const int4 *>(&info->bias0[r]);
+            const float4 sl = *reinterpret_cast<const float4 *>(&info->slope2[c0 + r]);
+            const int4 b = *reinterpret_cast<const int4 *>(&info->bias0[c0 + r]);
             const float s4[4] = {sl.x, sl.y, sl.z, sl.w};
             const int b4[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -644,7 +650,8 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
         }
         if (part) {
           // Tokens that no row sees are zeros in V; ones that only some rows see must
-          // not hand an infinity or NaN to the others.
+          // not hand an infinity or NaN to the others.  Each warpgroup does its share
+          // of the channels.
           const bool none = j < sp.lo || j >= sp.hi, some = j < sp.all_lo || j >= sp.all_hi;
           bool lost = false;
           const int v0 = g + H * (min(at - b0 + 2, b1 - b0) + at - b0);  // V's first slot of the block
@@ -652,11 +659,20 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
           for (int half = 0; half < H; ++half) {
             const int s = (v0 + half) % C::kSlots;
             wait_all(&bars->full[s], ((v0 + half) / C::kSlots) & 1);
-            if (some && ok) lost |= clean_row<T, C::kDH>(smem + s * C::kSlot, tid, none);
+            constexpr int kShare = C::kDH / 8 / C::kGroups;
+            if (some && ok) lost |= clean_row<T>(smem + s * C::kSlot, tok, wg * kShare, kShare, none);
+          }
+          if constexpr (C::kGroups > 1) {
+            // Where some rows see a token that others do not, the shares' findings meet.
+            if (max(n0, sp.lo) < sp.all_lo || min(n0 + kBN, sp.hi) > sp.all_hi) {
+              bars->lost[buf][wg][tok] = lost;
+              asm volatile("bar.sync 3, 256;" ::: "memory");
+              lost = bars->lost[buf][0][tok] | bars->lost[buf][1][tok];
+            }
           }
 #pragma unroll
-          for (int r = 0; r < N; r += 4) {
-            const int4 lo = *reinterpret_cast<const int4 *>(&info->lo[r]), hi = *reinterpret_cast<const int4 *>(&info->hi[r]);
+          for (int r = 0; r < W; r += 4) {
+            const int4 lo = *reinterpret_cast<const int4 *>(&info->lo[c0 + r]), hi = *reinterpret_cast<const int4 *>(&info->hi[c0 + r]);
             const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -664,43 +680,44 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
           }
         }
         if (wk.score != nullptr && j < wk.pitch) {
-          float *sc = wk.score + (((long long)cur.b * a.Hkv + cur.kvh) * wk.R + row0) * wk.pitch + j;
+          float *sc = wk.score + (((long long)cur.b * a.Hkv + cur.kvh) * wk.R + row0 + c0) * wk.pitch + j;
 #pragma unroll
-          for (int r = 0; r < N; ++r)
-            if (r < rows) sc[r * wk.pitch] = x[r];
+          for (int r = 0; r < W; ++r)
+            if (c0 + r < rows) sc[r * wk.pitch] = x[r];
         }
         bool over = false;
 #pragma unroll
-        for (int r = 0; r < N; r += 4) {
-          const float4 lim = *reinterpret_cast<const float4 *>(&info->limit[r]);
+        for (int r = 0; r < W; r += 4) {
+          const float4 lim = *reinterpret_cast<const float4 *>(&info->limit[c0 + r]);
           over |= x[r] > lim.x || x[r + 1] > lim.y || x[r + 2] > lim.z || x[r + 3] > lim.w;
         }
-        if (wg_any(over)) {
+        if (wg_any(wg, over)) {
           // Some score passes its row's limit: new references.
           {
-            float mx[N];
+            float mx[W];
 #pragma unroll
-            for (int r = 0; r < N; ++r) mx[r] = x[r];
-            reduce_rows<N>(mx, [](float p, float q) { return fmaxf(p, q); });
-            put_rows<N>(info->wmax[warp], mx);
+            for (int r = 0; r < W; ++r) mx[r] = x[r];
+            reduce_rows<W>(mx, [](float p, float q) { return fmaxf(p, q); });
+            put_rows<W>(info->wmax[warp % 4] + c0, mx);
           }
-          wg_sync();
-          if (tid < N) {
-            const float mx = fmaxf(fmaxf(info->wmax[0][tid], info->wmax[1][tid]), fmaxf(info->wmax[2][tid], info->wmax[3][tid]));
-            const float old = info->ref[tid];
+          wg_sync(wg);
+          if (tok < W) {
+            const int row = c0 + tok;
+            const float mx = fmaxf(fmaxf(info->wmax[0][row], info->wmax[1][row]), fmaxf(info->wmax[2][row], info->wmax[3][row]));
+            const float old = info->ref[row];
             float alpha = 1.f;
-            if (mx > info->limit[tid]) {
+            if (mx > info->limit[row]) {
               alpha = old == -CUDART_INF_F ? 1.f : ex2_approx(old - mx);
-              info->ref[tid] = mx;
-              info->base[tid] = mx - kShift;
-              info->limit[tid] = mx + weight_room<T>();
+              info->ref[row] = mx;
+              info->base[row] = mx - kShift;
+              info->limit[row] = mx + weight_room<T>();
             }
-            info->alpha[tid] = alpha;
+            info->alpha[row] = alpha;
           }
-          wg_sync();
+          wg_sync(wg);
 #pragma unroll
-          for (int r = 0; r < N; r += 4) {
-            const float4 al = *reinterpret_cast<const float4 *>(&info->alpha[r]);
+          for (int r = 0; r < W; r += 4) {
+            const float4 al = *reinterpret_cast<const float4 *>(&info->alpha[c0 + r]);
             l[r] *= al.x;
             l[r + 1] *= al.y;
             l[r + 2] *= al.z;
@@ -712,28 +729,28 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
             tc_fence_after();
 #pragma unroll 1
             for (int half = 0; half < H; ++half) {
-              float o[N];
-              tmem_ld_n<N>(tmem + lane_off + C::kO + half * N, o);
+              float o[W];
+              tmem_ld_n<W>(tmem + lane_off + C::kO + half * N + c0, o);
 #pragma unroll
-              for (int r = 0; r < N; r += 4) {
-                const float4 al = *reinterpret_cast<const float4 *>(&info->alpha[r]);
+              for (int r = 0; r < W; r += 4) {
+                const float4 al = *reinterpret_cast<const float4 *>(&info->alpha[c0 + r]);
                 o[r] *= al.x;
                 o[r + 1] *= al.y;
                 o[r + 2] *= al.z;
                 o[r + 3] *= al.w;
               }
-              tmem_st_n<N>(tmem + lane_off + C::kO + half * N, o);
+              tmem_st_n<W>(tmem + lane_off + C::kO + half * N + c0, o);
             }
             tmem_wait_st();
           }
         }
-        uint8_t *const pt = smem + C::kPOff + buf * C::kP + tid * 16;
+        uint8_t *const pt = smem + C::kPOff + buf * C::kP + c0 / 8 * 2048 + tok * 16;
 #pragma unroll
-        for (int r = 0; r < N; r += 8) {
+        for (int r = 0; r < W; r += 8) {
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 8; e += 4) {
-            const float4 bs = *reinterpret_cast<const float4 *>(&info->base[r + e]);
+            const float4 bs = *reinterpret_cast<const float4 *>(&info->base[c0 + r + e]);
             const float p0 = ex2_approx(x[r + e] - bs.x), p1 = ex2_approx(x[r + e + 1] - bs.y);
             const float p2 = ex2_approx(x[r + e + 2] - bs.z), p3 = ex2_approx(x[r + e + 3] - bs.w);
             l[r + e] += p0;
@@ -752,69 +769,70 @@ __global__ void __launch_bounds__(kStepThreads, StepCfg<D, N>::kCtas)
       g += 2 * H * (b1 - b0);
 
       // ---- the part's end
-      reduce_rows<N>(l, [](float p, float q) { return p + q; });
-      put_rows<N>(info->wmax[warp], l);
+      reduce_rows<W>(l, [](float p, float q) { return p + q; });
+      put_rows<W>(info->wmax[warp % 4] + c0, l);
       if (b0 < b1) {
         // (The products complete in order, and those two blocks back are done, since
         // the last block's scores were issued after them: no phase is passed over.)
         wait_all(&bars->o_done[(blk - 1) & 1], ((blk - 1) >> 1) & 1);
         tc_fence_after();
       }
-      wg_sync();
+      wg_sync(wg);
       const bool whole = b0 == 0 && b1 == sp.blocks();
       const long long slot = 2LL * worker + (cur.at == 0 ? 1 : 0);
-      if (tid < rows) {
-        const float sum = (info->wmax[0][tid] + info->wmax[1][tid]) + (info->wmax[2][tid] + info->wmax[3][tid]);
-        const int r = row0 + tid;
+      if (tok < W && c0 + tok < rows) {
+        const int row = c0 + tok;
+        const float sum = (info->wmax[0][row] + info->wmax[1][row]) + (info->wmax[2][row] + info->wmax[3][row]);
+        const int r = row0 + row;
         if (whole) {
           const int i = r / a.group, h = cur.kvh * a.group + r % a.group;
-          const bool sees = info->hi[tid] > info->lo[tid];
-          const float lse2 = info->ref[tid] - kShift + log2f(sum);
-          info->inv[tid] = sees ? 1.f / sum : 0.f;
+          const bool sees = info->hi[row] > info->lo[row];
+          const float lse2 = info->ref[row] - kShift + log2f(sum);
+          info->inv[row] = sees ? 1.f / sum : 0.f;
           if (a.lse != nullptr)
             a.lse[((long long)cur.b * a.H + h) * a.Sq + i] =
-                sees ? lse2 * kLn2 + (kMode != 0 && a.alibi != nullptr ? a.alibi[h] * (float)info->bias0[tid] : 0.f) : -CUDART_INF_F;
+                sees ? lse2 * kLn2 + (kMode != 0 && a.alibi != nullptr ? a.alibi[h] * (float)info->bias0[row] : 0.f) : -CUDART_INF_F;
           if (wk.stat != nullptr) wk.stat[((long long)cur.b * a.Hkv + cur.kvh) * wk.R + r] = lse2;
         } else {
-          *reinterpret_cast<float2 *>(wk.part_ml + (slot * N + tid) * 2) = make_float2(info->ref[tid], sum);
+          *reinterpret_cast<float2 *>(wk.part_ml + (slot * N + row) * 2) = make_float2(info->ref[row], sum);
         }
       }
-      wg_sync();
+      wg_sync(wg);
 #pragma unroll 1
       for (int half = 0; half < H; ++half) {
-        float o[N];
+        float o[W];
         if (b0 < b1) {
-          tmem_ld_n<N>(tmem + lane_off + C::kO + half * N, o);
+          tmem_ld_n<W>(tmem + lane_off + C::kO + half * N + c0, o);
         } else {
 #pragma unroll
-          for (int r = 0; r < N; ++r) o[r] = 0.f;
+          for (int r = 0; r < W; ++r) o[r] = 0.f;
         }
-        if (tid >= C::kDH) continue;
-        const int ch = half * 128 + tid;
+        if (tok >= C::kDH) continue;
+        const int ch = half * 128 + tok;
         if (whole) {
 #pragma unroll
-          for (int r = 0; r < N; ++r)
-            if (r < rows)
-              static_cast<T *>(a.o)[info->out[r] + ch] = Elem<T>::from_f(o[r] * info->inv[r]);  // 0 for a row that sees nothing
+          for (int r = 0; r < W; ++r)
+            if (c0 + r < rows)
+              static_cast<T *>(a.o)[info->out[c0 + r] + ch] = Elem<T>::from_f(o[r] * info->inv[c0 + r]);  // 0 for a row that sees nothing
         } else {
-          float *po = wk.part_o + slot * N * D + ch;
+          float *po = wk.part_o + (slot * N + c0) * D + ch;
 #pragma unroll
-          for (int r = 0; r < N; ++r)
-            if (r < rows) po[r * D] = o[r];
+          for (int r = 0; r < W; ++r)
+            if (c0 + r < rows) po[r * D] = o[r];
         }
       }
       tc_fence_before();  // O^T is read before the next part's products write it
-      wg_sync();          // and the rows' values before they are set anew
+      wg_sync(wg);          // and the rows' values before they are set anew
       cur = nx;
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kStepMma) {
+  if (warp == C::kMmaWarp) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, C::kCols);
+    tmem_dealloc(tmem, C::kTmem);
   }
 }
 
@@ -1001,7 +1019,7 @@ cudaError_t launch_step_t(const AttnArgs &a, const StepWork &wk, long long units
   std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem); });
   if (attr != cudaSuccess) return attr;
   const unsigned grid = (unsigned)(wk.split ? wk.workers : units);
-  kern<<<grid, kStepThreads, C::kSmem, s>>>(tk, tv, a, wk);
+  kern<<<grid, C::kThreads, C::kSmem, s>>>(tk, tv, a, wk);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   if (wk.split) {
