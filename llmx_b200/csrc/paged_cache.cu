@@ -13,6 +13,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <climits>
 #include <mutex>
 
 #include "paged.cuh"
@@ -50,48 +51,65 @@ struct StoreArgs {
 
 constexpr int kStoreThreads = 256;
 
-// A CTA copies `tokens` rows of one sequence, K and V: a thread moves 16-byte
-// pieces (VEC; single elements where rows are not 16-byte aligned) of the
-// rows' [head][channel] order, so that dense rows are read and pages written in
-// whole lines.  kUnroll pieces of each are in flight a thread.
+// A CTA copies `tokens` rows of one sequence, K and V: their places are looked up
+// once, then a thread moves 16-byte pieces (VEC; single elements where rows are
+// not 16-byte aligned) of the rows' [head][channel] order, so that dense rows are
+// read and pages written in whole lines; kUnroll of K and of V in flight a thread.
+constexpr int kStoreTokens = 64;  // of a CTA, at most
 template <bool VEC>
 __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const PagedArgs a, const StoreArgs r, int tokens) {
   constexpr int kUnroll = 4;
   using Piece = typename std::conditional<VEC, uint4, uint16_t>::type;
   constexpr int kPer = sizeof(Piece) / 2;
+  __shared__ int2 place[kStoreTokens];  // page (-1: none) and row
   const int per_head = a.D / kPer;
   const int log_per_head = 31 - __clz(per_head);  // D is a power of two
   const int pieces = a.Hkv * per_head;
   for (int b = blockIdx.y; b < r.B; b += gridDim.y) {
     const int n = clamp_len(r.lens, b, r.rows);
-    const long long first = r.start != nullptr ? r.start[b] : 0;
     const int lo = blockIdx.x * tokens, hi = min(n, lo + tokens);
     if (lo >= hi) continue;
-    // Pieces of the CTA's tokens in the order token, head, chunk.
-    const int total = (hi - lo) * pieces;  // tokens * pieces is at most 2^31 - 1 (launch_store)
+    const long long first = r.start != nullptr ? r.start[b] : 0;
+    __syncthreads();  // the places of the sequence before have been read
+    if (threadIdx.x < hi - lo) {
+      const long long j = first + lo + threadIdx.x;
+      int2 p = make_int2(-1, 0);
+      if (j >= 0 && j <= INT_MAX) {
+        const int slot = (int)j / a.page_size;
+        p = make_int2(paged_page(a, b, slot), (int)j - slot * a.page_size);
+      } else {
+        raise_error(a.err, kDevErrBadPage);
+      }
+      place[threadIdx.x] = p;
+    }
+    __syncthreads();
+    // Pieces of the CTA's tokens in the order token, head, chunk; tokens * pieces
+    // is at most 2^31 - 1 (launch_store).
+    const int total = (hi - lo) * pieces;
+    int t = threadIdx.x / pieces, p = threadIdx.x - t * pieces;  // of this thread's next piece
     for (int base = threadIdx.x; base < total; base += kStoreThreads * kUnroll) {
       Piece x[kUnroll], y[kUnroll];
       long long kd[kUnroll], vd[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        const int i = base + u * kStoreThreads;
         kd[u] = -1;
-        if (i < total) {
-          const int t = i / pieces, p = i - t * pieces;
+        if (base + u * kStoreThreads < total) {
           const int h = p >> log_per_head, c = (p & (per_head - 1)) * kPer;
-          const long long j = first + lo + t;
-          const int page = j < 0 ? -1 : paged_page(a, b, j / a.page_size);
-          if (j < 0) raise_error(a.err, kDevErrBadPage);
-          if (page >= 0) {
-            const long long off = j % a.page_size;
-            kd[u] = page * a.ks[0] + h * a.ks[1] + off * a.ks[2] + c;
-            vd[u] = page * a.vs[0] + h * a.vs[1] + off * a.vs[2] + c;
+          const int2 at = place[t];
+          if (at.x >= 0) {
+            kd[u] = at.x * a.ks[0] + h * a.ks[1] + at.y * a.ks[2] + c;
+            vd[u] = at.x * a.vs[0] + h * a.vs[1] + at.y * a.vs[2] + c;
             const long long row = lo + t;
             x[u] = *reinterpret_cast<const Piece *>(static_cast<const uint16_t *>(r.k) + b * r.ks[0] + row * r.ks[1] +
                                                     h * r.ks[2] + c);
             y[u] = *reinterpret_cast<const Piece *>(static_cast<const uint16_t *>(r.v) + b * r.vs[0] + row * r.vs[1] +
                                                     h * r.vs[2] + c);
           }
+        }
+        p += kStoreThreads;
+        while (p >= pieces) {
+          p -= pieces;
+          ++t;
         }
       }
 #pragma unroll
@@ -107,7 +125,7 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const PagedA
 cudaError_t launch_store(const PagedArgs &a, const StoreArgs &r, bool vec, int num_sms, cudaStream_t s) {
   const long long pieces = (long long)a.Hkv * a.D / (vec ? 8 : 1);
   // One round of kUnroll pieces a thread, and at least one token.
-  const int tokens = (int)std::max<long long>(1, std::min<long long>(r.rows, kStoreThreads * 4 / pieces));
+  const int tokens = (int)std::max<long long>(1, std::min<long long>(std::min(r.rows, kStoreTokens), kStoreThreads * 4 / pieces));
   const dim3 grid((r.rows + tokens - 1) / tokens, std::min(r.B, 65535));
   if (vec)
     paged_store_kernel<true><<<grid, kStoreThreads, 0, s>>>(a, r, tokens);
@@ -146,11 +164,12 @@ struct SelShared {
   uint32_t digit, need, taken;  // a round's result
 };
 
-// Cluster `g` of CTAs handles (sequence, kv head) g; CTA `rank` of it the
-// candidates [rank * per, (rank + 1) * per) of positions sinks .. L - recent - 1.
+// Cluster `g` of CTAs handles (sequence, kv head) g; CTA `rank` of it an equal
+// part of the positions, of which sinks .. L - recent - 1 are candidates.
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedArgs a, const EvictArgs e) {
   extern __shared__ uint32_t held[];
   __shared__ SelShared sh;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
   const int unit = blockIdx.x / ranks;
@@ -170,16 +189,53 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
   const uint32_t want = n - e.sinks - e.recent;  // of the candidates; fewer than there are
   if (want == 0) return;
 
-  const int candidates = L - e.sinks - e.recent;
-  const int per = (candidates + ranks - 1) / ranks;
-  const int c0 = min(candidates, rank * per), mine = min(candidates, c0 + per) - c0;
-  auto read = [&](int i) {  // the key of candidate c0 + i
-    const int j = e.sinks + c0 + i;
+  // This CTA's positions [j0, j0 + mine); what is no candidate has the image 0,
+  // below that of every weight, and is never needed.
+  const int per = ((L + ranks - 1) / ranks + 3) & ~3;
+  const int j0 = min(L, rank * per), mine = min(L, j0 + per) - j0;
+  const int first = e.sinks - j0, last = L - e.recent - j0;  // candidates, from j0
+  auto read = [&](int i) {
+    if (i < first || i >= last) return 0u;
+    const int j = j0 + i;
     const int page = paged_page(a, b, j / a.page_size);
     return weight_key(page < 0 ? CUDART_NAN_F : a.w[page * a.ws[0] + h * a.ws[1] + j % a.page_size]);
   };
-  for (int i = tid; i < min(mine, kSelHeld); i += kSelThreads) held[i] = read(i);
+  {
+    // Four weights a load (pages hold a multiple of 16), four loads in flight.
+    const int n_held = min(mine, kSelHeld);
+    for (int base = tid * 4; base < n_held; base += kSelThreads * 16) {
+      float4 w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + base + u * kSelThreads * 4;
+        w[u] = make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F);
+        if (j - j0 < n_held) {
+          const int slot = j / a.page_size;
+          const int page = paged_page(a, b, slot);
+          if (page >= 0)
+            w[u] = *reinterpret_cast<const float4 *>(a.w + page * a.ws[0] + h * a.ws[1] + (j - slot * a.page_size));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int at = base + u * kSelThreads * 4;
+        if (at < n_held) {
+          const float x[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+          uint32_t k[4];
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4) k[e4] = at + e4 >= first && at + e4 < last ? weight_key(x[e4]) : 0u;
+          *reinterpret_cast<uint4 *>(held + at) = make_uint4(k[0], k[1], k[2], k[3]);
+        }
+      }
+    }
+  }
   auto key = [&](int i) { return i < kSelHeld ? held[i] : read(i); };
+  auto sync_all = [&] {
+    if (ranks > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
 
   // After round r the top 8 (r + 1) bits of the threshold are `prefix`; `need`
   // of the candidates with exactly these bits are still to be taken, all with
@@ -196,7 +252,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
       const uint32_t k = key(i);
       if (shift == 32 || (k >> shift) == prefix) atomicAdd(&hist[(k >> below) & 255u], 1u);
     }
-    cluster.sync();
+    sync_all();
     if (warp == 0) {
       // Lane l has digits 255 - 8 l down to 248 - 8 l, so that a prefix sum over the
       // lanes counts from the largest digit.
@@ -276,7 +332,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
     sh.gt = g;
     sh.eq = q;
   }
-  cluster.sync();
+  sync_all();
   uint32_t g0 = sh.warp_gt[warp], q0 = sh.warp_eq[warp];
   for (int r = 0; r < rank; ++r) {
     const SelShared *o = cluster.map_shared_rank(&sh, r);
@@ -289,93 +345,127 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
     classify(i + lane, gt, eq);
     const uint32_t gm = __ballot_sync(0xffffffffu, gt), qm = __ballot_sync(0xffffffffu, eq);
     const uint32_t g = g0 + __popc(gm & lt), q = q0 + __popc(qm & lt);
-    if (gt || (eq && q < need)) kept[e.sinks + g + min(q, need)] = e.sinks + c0 + i + lane;
+    if (gt || (eq && q < need)) kept[e.sinks + g + min(q, need)] = j0 + i + lane;
     g0 += __popc(gm);
     q0 += __popc(qm);
   }
-  cluster.sync();  // no CTA leaves while another reads its counts
+  if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its counts
 }
 
 constexpr int kMoveThreads = 256;
 
-// Moves columns [first, first + width) of the kept rows of one of K, V and the
-// weights of a (sequence, kv head).  In place row r's source kept[r] >= r, so a
-// CTA that handles all rows of its columns in ascending order may write a
-// batch once it has read that batch: what later batches read lies behind it.
-// Different columns never meet, which is what spreads a unit over CTAs.  To
-// other pages there is no order to keep and the rows are spread as well.
+// Moves the kept rows of K, V and the weights of a (sequence, kv head).  In
+// place row r's source kept[r] >= r, so a CTA that handles all rows of its
+// columns in ascending order may write a batch once it has read that batch: what
+// later batches read lies behind it.  Different columns never meet, which is
+// what spreads a unit over CTAs.  To other pages there is no order to keep, and
+// the rows are spread over CTAs instead.  Bound by HBM: 16-byte pieces, eight in
+// flight a thread, whose places are looked up once a row, a batch ahead.
 struct MoveArgs {
-  int pieces;      // 16-byte pieces of a K or V row that one CTA moves
-  int chunk_rows;  // rows of one CTA
-  int chunks;      // CTAs along the rows
-  int col_ctas;    // CTAs along the columns of K (and of V); the weights have one
+  int pieces;    // 16-byte pieces of a K and of a V row that one CTA moves
+  int batch;     // rows at a time, at most kMoveThreads
+  int rows;      // of one CTA: a multiple of batch
+  int chunks;    // CTAs along the rows
+  int col_ctas;  // CTAs along the columns of K and V; one more has the weights
 };
 
-template <typename Piece>
-__device__ __forceinline__ void move_rows(const PagedArgs &a, const EvictArgs &e, Piece *base, const long long *st, int b,
-                                          int h, const int *kept, int lo, int hi, int pieces, int col) {
-  constexpr int kUnroll = 8;
-  const bool in_place = e.out_table == nullptr;
-  const int per_pass = kMoveThreads / pieces;  // rows
-  const int row = threadIdx.x / pieces, c = col + threadIdx.x % pieces;
-  const bool idle = row >= per_pass;
-  Piece *const head = base + h * st[1] + c;
-  for (int r0 = lo; r0 < hi; r0 += per_pass * kUnroll) {
-    Piece x[kUnroll];
-    long long to[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int r = r0 + u * per_pass + row;
-      to[u] = -1;
-      if (idle || r >= hi) continue;
-      const int j = kept[r];
-      if (j < 0 || (in_place && j == r)) continue;
-      const int from = paged_page(a, b, j / a.page_size);
-      const int dest = in_place ? paged_page(a, b, r / a.page_size)
-                                : paged_page(a, e.out_table, e.out_stride, e.out_pages, b, r / a.page_size);
-      if (from < 0 || dest < 0) continue;
-      x[u] = head[from * st[0] + (j % a.page_size) * st[2]];
-      to[u] = dest * st[0] + (r % a.page_size) * st[2];
-    }
-    if (in_place) __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (to[u] >= 0) head[to[u]] = x[u];
-  }
+// Where a row comes from and goes to (pages; -1 for neither: it stays).
+struct MovePlace {
+  int from, from_row, to, to_row;
+};
+__device__ __forceinline__ MovePlace move_place(const PagedArgs &a, const EvictArgs &e, int b, const int *kept, int r, int hi) {
+  MovePlace p{-1, 0, -1, 0};
+  if (r >= hi) return p;
+  const int j = kept[r];
+  if (j < 0 || (e.out_table == nullptr && j == r)) return p;
+  const int from_slot = j / a.page_size, to_slot = r / a.page_size;
+  p.from = paged_page(a, b, from_slot);
+  p.from_row = j - from_slot * a.page_size;
+  p.to = e.out_table == nullptr ? paged_page(a, b, to_slot)
+                                : paged_page(a, e.out_table, e.out_stride, e.out_pages, b, to_slot);
+  p.to_row = r - to_slot * a.page_size;
+  if (p.to < 0) p.from = -1;
+  return p;
 }
 
+template <bool kInPlace>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const PagedArgs a, const EvictArgs e, const MoveArgs m) {
-  const int cols = 2 * m.col_ctas + 1;
+  __shared__ MovePlace places[2][kMoveThreads];
+  const int tid = threadIdx.x;
+  const int cols = m.col_ctas + 1;
   const int col = blockIdx.x % cols, rest = blockIdx.x / cols;
   const int chunk = rest % m.chunks, unit = rest / m.chunks;
   const int b = unit / a.Hkv, h = unit % a.Hkv;
   // new_lens may be kv_lens: the minimum is the same before and after its write.
   const int n = min(clamp_len(e.kv_lens, b, e.max_kv), e.budget);
-  if (col == 2 * m.col_ctas && chunk == 0 && h == 0 && threadIdx.x == 0) e.new_lens[b] = n;
-  const int lo = chunk * m.chunk_rows, hi = min(n, lo + m.chunk_rows);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // kept is there
+  if (col == m.col_ctas && chunk == 0 && h == 0 && tid == 0) e.new_lens[b] = n;
+  const int lo = chunk * m.rows, hi = min(n, lo + m.rows);
   if (lo >= hi) return;
   const int *kept = e.kept + ((long long)b * a.Hkv + h) * e.budget;
-  if (col == 2 * m.col_ctas) {
-    const long long st[3] = {a.ws[0], a.ws[1], 1};
-    move_rows<float>(a, e, a.w, st, b, h, kept, lo, hi, 1, 0);
-  } else {
-    const bool is_v = col >= m.col_ctas;
-    const long long *s = is_v ? a.vs : a.ks;
-    const long long st[3] = {s[0] / 8, s[1] / 8, s[2] / 8};
-    move_rows<uint4>(a, e, static_cast<uint4 *>(is_v ? a.v : a.k), st, b, h, kept, lo, hi, m.pieces,
-                     (is_v ? col - m.col_ctas : col) * m.pieces);
+  auto look_up = [&](int r0, int buf) {
+    if (tid < m.batch) places[buf][tid] = move_place(a, e, b, kept, r0 + tid, hi);
+  };
+  if (col == m.col_ctas) {
+    // The weights: a thread a row.
+    float *const w = a.w + h * a.ws[1];
+    for (int r0 = lo; r0 < hi; r0 += kMoveThreads) {
+      const MovePlace p = move_place(a, e, b, kept, r0 + tid, hi);
+      float x = 0.f;
+      if (p.from >= 0) x = w[p.from * a.ws[0] + p.from_row];
+      if (kInPlace) __syncthreads();
+      if (p.from >= 0) w[p.to * a.ws[0] + p.to_row] = x;
+    }
+    return;
+  }
+  constexpr int kUnroll = 8;
+  const int log_p = 31 - __clz(m.pieces);  // a power of two
+  const int c0 = col * m.pieces;
+  const int items = m.batch * m.pieces * 2;  // of a batch; in place at most kUnroll a thread
+  look_up(lo, 0);
+  __syncthreads();
+  int buf = 0;
+  for (int r0 = lo; r0 < hi; r0 += m.batch, buf ^= 1) {
+    for (int i0 = tid; i0 < items; i0 += kMoveThreads * kUnroll) {
+      uint4 x[kUnroll];
+      uint4 *to[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int i = i0 + u * kMoveThreads;
+        to[u] = nullptr;
+        if (i >= items) continue;
+        const int c = c0 + (i & (m.pieces - 1)), row = i >> (log_p + 1);
+        const bool is_v = (i >> log_p) & 1;
+        const MovePlace p = places[buf][row];
+        if (p.from < 0) continue;
+        const long long *st = is_v ? a.vs : a.ks;
+        uint4 *const head = static_cast<uint4 *>(is_v ? a.v : a.k) + h * (st[1] / 8) + c;
+        x[u] = head[p.from * (st[0] / 8) + p.from_row * (st[2] / 8)];
+        to[u] = head + p.to * (st[0] / 8) + p.to_row * (st[2] / 8);
+      }
+      if (kInPlace) {
+        look_up(r0 + m.batch, buf ^ 1);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (to[u] != nullptr) *to[u] = x[u];
+    }
+    if (!kInPlace && r0 + m.batch < hi) {
+      look_up(r0 + m.batch, buf ^ 1);
+      __syncthreads();
+    }
   }
 }
 
 cudaError_t launch_evict(const PagedArgs &a, const EvictArgs &e, int num_sms, cudaStream_t s) {
   const long long units = (long long)e.B * a.Hkv;
-  const int candidates = std::max(0, e.max_kv - e.sinks - e.recent);
   // CTAs of a cluster: enough that the weights stay in shared memory, and as
   // many as keep the machine busy when there are few units.
   int ranks = 1;
-  while (ranks < 8 && (candidates > ranks * kSelHeld || (units * ranks * 2 <= num_sms && candidates > ranks * 1024)))
+  while (ranks < 8 && (e.max_kv > ranks * kSelHeld || (units * ranks * 2 <= num_sms && e.max_kv > ranks * 1024)))
     ranks *= 2;
-  const int per = (candidates + ranks - 1) / ranks;
+  const int per = ((e.max_kv + ranks - 1) / ranks + 3) & ~3;
   const size_t smem = (size_t)std::min(per, kSelHeld) * 4;
   if (units * ranks > 0x7fffffffLL) return cudaErrorInvalidValue;
   static std::once_flag once;
@@ -403,17 +493,28 @@ cudaError_t launch_evict(const PagedArgs &a, const EvictArgs &e, int num_sms, cu
   const int most = std::min(e.budget, e.max_kv);
   if (e.out_table != nullptr) {
     m.pieces = row_pieces;
-    m.chunk_rows = kMoveThreads / row_pieces * 8;
+    m.batch = 128;
+    m.rows = m.batch;
   } else {
-    m.pieces = units * (2 * row_pieces / 4) >= 2LL * num_sms ? 4 : 2;  // 64 bytes; 32 with few units
-    m.chunk_rows = std::max(1, most);
+    m.pieces = units * (row_pieces / 4) >= 2LL * num_sms ? 4 : 2;  // 64 bytes; 32 with few units
+    m.batch = kMoveThreads;
+    m.rows = (most + m.batch - 1) / m.batch * m.batch;
   }
   m.col_ctas = row_pieces / m.pieces;
-  m.chunks = std::max(1, (most + m.chunk_rows - 1) / m.chunk_rows);
-  const long long grid = units * m.chunks * (2 * m.col_ctas + 1);
+  m.chunks = (most + m.rows - 1) / m.rows;
+  const long long grid = units * m.chunks * (m.col_ctas + 1);
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  evict_move_kernel<<<(unsigned)grid, kMoveThreads, 0, s>>>(a, e, m);
-  return cudaGetLastError();
+  cudaLaunchConfig_t mc = {};
+  mc.gridDim = dim3((unsigned)grid);
+  mc.blockDim = dim3(kMoveThreads);
+  mc.stream = s;
+  cudaLaunchAttribute ma[1];
+  ma[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  ma[0].val.programmaticStreamSerializationAllowed = 1;
+  mc.attrs = ma;
+  mc.numAttrs = 1;
+  return e.out_table != nullptr ? cudaLaunchKernelEx(&mc, evict_move_kernel<false>, a, e, m)
+                                : cudaLaunchKernelEx(&mc, evict_move_kernel<true>, a, e, m);
 }
 
 }  // namespace
