@@ -157,8 +157,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-struct SelShared {
+struct alignas(16) SelShared {
   uint32_t hist[2][256];
+  uint32_t sum[256];  // of the cluster's histograms
   uint32_t warp_gt[kSelWarps], warp_eq[kSelWarps];
   uint32_t gt, eq;              // this CTA's counts, read by the others
   uint32_t digit, need, taken;  // a round's result
@@ -229,7 +230,10 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
       }
     }
   }
-  auto key = [&](int i) { return i < kSelHeld ? held[i] : read(i); };
+  // The images of positions i .. i + 3 (i a multiple of 4; 0 behind the last).
+  auto keys = [&](int i) {
+    return i < kSelHeld ? *reinterpret_cast<const uint4 *>(held + i) : make_uint4(read(i), read(i + 1), read(i + 2), read(i + 3));
+  };
   auto sync_all = [&] {
     if (ranks > 1)
       cluster.sync();
@@ -248,19 +252,37 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
     for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
     __syncthreads();
     const int below = shift - 8;
-    for (int i = tid; i < mine; i += kSelThreads) {
-      const uint32_t k = key(i);
-      if (shift == 32 || (k >> shift) == prefix) atomicAdd(&hist[(k >> below) & 255u], 1u);
+    for (int i = tid * 4; i < mine; i += kSelThreads * 4) {
+      const uint4 k4 = keys(i);
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+      if (round == 0) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) atomicAdd(&hist[k[u] >> 24], 1u);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if ((k[u] >> shift) == prefix) atomicAdd(&hist[(k[u] >> below) & 255u], 1u);
+      }
     }
     sync_all();
+    if (ranks > 1) {
+      if (tid < 256) {
+        uint32_t v[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = r < ranks ? cluster.map_shared_rank(hist, r)[tid] : 0u;
+        sh.sum[tid] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+      }
+      __syncthreads();
+    }
     if (warp == 0) {
       // Lane l has digits 255 - 8 l down to 248 - 8 l, so that a prefix sum over the
       // lanes counts from the largest digit.
-      uint32_t c[8], sum = 0;
+      const uint32_t *const count = ranks > 1 ? sh.sum : hist;
+      const uint4 hi4 = *reinterpret_cast<const uint4 *>(count + 252 - 8 * lane), lo4 = *reinterpret_cast<const uint4 *>(count + 248 - 8 * lane);
+      const uint32_t c[8] = {hi4.w, hi4.z, hi4.y, hi4.x, lo4.w, lo4.z, lo4.y, lo4.x};
+      uint32_t sum = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        c[i] = 0;
-        for (int r = 0; r < ranks; ++r) c[i] += cluster.map_shared_rank(hist, r)[255 - 8 * lane - i];
         sum += c[i];
       }
       uint32_t before = sum;
@@ -297,24 +319,29 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
 
   // Positions: a candidate above the threshold is taken, and of those with the
   // threshold's bits the first `need` ones.  Warp w has a contiguous part of the
-  // CTA's candidates, so one pass counts and a second one writes.
-  const int part = ((mine + kSelThreads - 1) / kSelThreads) * 32;
+  // CTA's positions, four a lane, so one pass counts and a second one writes.
+  const int part = ((mine + kSelThreads * 4 - 1) / (kSelThreads * 4)) * 128;
   const int w0 = min(mine, warp * part), w1 = min(mine, w0 + part);
-  auto classify = [&](int i, bool &gt, bool &eq) {
-    gt = eq = false;
-    if (i < w1) {
-      const uint32_t top = shift == 0 ? key(i) : key(i) >> shift;
-      gt = top > prefix;
-      eq = top == prefix;
+  // How many of the four are above, and (times 2^16) have the threshold's bits.
+  auto classify = [&](int i, uint32_t (&c)[4]) {
+    const uint4 k4 = i < w1 ? keys(i) : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t top = k[u] >> shift;  // shift is 24 at most
+      c[u] = (top > prefix ? 1u : 0u) + (k[u] != 0u && top == prefix ? 65536u : 0u);
     }
+    return (c[0] + c[1]) + (c[2] + c[3]);
   };
   uint32_t gt_n = 0, eq_n = 0;
-  for (int i = w0; i < w1; i += 32) {
-    bool gt, eq;
-    classify(i + lane, gt, eq);
-    gt_n += __popc(__ballot_sync(0xffffffffu, gt));
-    eq_n += __popc(__ballot_sync(0xffffffffu, eq));
+  for (int i = w0 + lane * 4; i < w1; i += 128) {
+    uint32_t c[4];
+    const uint32_t n4 = classify(i, c);
+    gt_n += n4 & 65535u;
+    eq_n += n4 >> 16;
   }
+  gt_n = __reduce_add_sync(0xffffffffu, gt_n);
+  eq_n = __reduce_add_sync(0xffffffffu, eq_n);
   if (lane == 0) {
     sh.warp_gt[warp] = gt_n;
     sh.warp_eq[warp] = eq_n;
@@ -339,15 +366,25 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
     g0 += o->gt;
     q0 += o->eq;
   }
-  const uint32_t lt = (1u << lane) - 1u;
-  for (int i = w0; i < w1; i += 32) {
-    bool gt, eq;
-    classify(i + lane, gt, eq);
-    const uint32_t gm = __ballot_sync(0xffffffffu, gt), qm = __ballot_sync(0xffffffffu, eq);
-    const uint32_t g = g0 + __popc(gm & lt), q = q0 + __popc(qm & lt);
-    if (gt || (eq && q < need)) kept[e.sinks + g + min(q, need)] = j0 + i + lane;
-    g0 += __popc(gm);
-    q0 += __popc(qm);
+  for (int i = w0; i < w1; i += 128) {
+    uint32_t c[4];
+    const uint32_t n4 = classify(i + lane * 4, c);
+    uint32_t upto = n4;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += o;
+    }
+    uint32_t g = g0 + ((upto - n4) & 65535u), q = q0 + ((upto - n4) >> 16);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if ((c[u] & 1u) || (c[u] != 0u && q < need)) kept[e.sinks + g + min(q, need)] = j0 + i + lane * 4 + u;
+      g += c[u] & 65535u;
+      q += c[u] >> 16;
+    }
+    const uint32_t all4 = __shfl_sync(0xffffffffu, upto, 31);
+    g0 += all4 & 65535u;
+    q0 += all4 >> 16;
   }
   if (ranks > 1) cluster.sync();  // no CTA leaves while another reads its counts
 }
