@@ -144,8 +144,6 @@ struct EvictArgs {
   int *kept, *new_lens;
 };
 
-constexpr int kSelThreads = 512;
-constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelHeld = 16384;  // weights of a CTA held in shared memory; more are read again in each round
 
 // The image of a weight under which unsigned order is the order of the
@@ -158,17 +156,20 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 struct alignas(16) SelShared {
-  uint32_t hist[2][256];
-  uint32_t sum[256];  // of the cluster's histograms
-  uint32_t warp_gt[kSelWarps], warp_eq[kSelWarps];
+  uint4 hist[2][256];  // four copies, a lane's is lane % 4: few digits are hot
+  uint32_t sum[2][256];  // of the copies, read by the cluster's other CTAs
+  uint32_t warp_gt[32], warp_eq[32];
   uint32_t gt, eq;              // this CTA's counts, read by the others
   uint32_t digit, need, taken;  // a round's result
 };
 
 // Cluster `g` of CTAs handles (sequence, kv head) g; CTA `rank` of it an equal
 // part of the positions, of which sinks .. L - recent - 1 are candidates.
+// 1024 threads where a unit has several CTAs (few units), else 512.
+template <int kSelThreads>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedArgs a, const EvictArgs e) {
-  extern __shared__ uint32_t held[];
+  constexpr int kSelWarps = kSelThreads / 32;
+  extern __shared__ __align__(16) uint32_t held[];
   __shared__ SelShared sh;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   cg::cluster_group cluster = cg::this_cluster();
@@ -248,8 +249,9 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
   int shift = 32;
   bool whole = false;  // all candidates with the prefix are taken
   for (int round = 0; round < 4 && !whole; ++round) {
-    uint32_t *hist = sh.hist[round & 1];
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
+    uint4 *const hist = sh.hist[round & 1];
+    uint32_t *const mine_hist = reinterpret_cast<uint32_t *>(hist) + lane % 4;
+    if (tid < 256) hist[tid] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     const int below = shift - 8;
     for (int i = tid * 4; i < mine; i += kSelThreads * 4) {
@@ -257,55 +259,44 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
       const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
       if (round == 0) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) atomicAdd(&hist[k[u] >> 24], 1u);
+        for (int u = 0; u < 4; ++u) atomicAdd(&mine_hist[(k[u] >> 24) * 4], 1u);
       } else {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if ((k[u] >> shift) == prefix) atomicAdd(&hist[(k[u] >> below) & 255u], 1u);
+          if ((k[u] >> shift) == prefix) atomicAdd(&mine_hist[((k[u] >> below) & 255u) * 4], 1u);
       }
     }
-    sync_all();
+    __syncthreads();
+    uint32_t *const local = sh.sum[round & 1];
+    uint32_t count = 0;  // thread t has digit 255 - t
+    if (tid < 256) {
+      const uint4 v = hist[255 - tid];
+      count = (v.x + v.y) + (v.z + v.w);
+      if (ranks > 1) local[tid] = count;
+    }
     if (ranks > 1) {
+      cluster.sync();
       if (tid < 256) {
         uint32_t v[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] = r < ranks ? cluster.map_shared_rank(hist, r)[tid] : 0u;
-        sh.sum[tid] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        for (int r = 0; r < 8; ++r) v[r] = r < ranks ? cluster.map_shared_rank(local, r)[tid] : 0u;
+        count = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
       }
-      __syncthreads();
     }
-    if (warp == 0) {
-      // Lane l has digits 255 - 8 l down to 248 - 8 l, so that a prefix sum over the
-      // lanes counts from the largest digit.
-      const uint32_t *const count = ranks > 1 ? sh.sum : hist;
-      const uint4 hi4 = *reinterpret_cast<const uint4 *>(count + 252 - 8 * lane), lo4 = *reinterpret_cast<const uint4 *>(count + 248 - 8 * lane);
-      const uint32_t c[8] = {hi4.w, hi4.z, hi4.y, hi4.x, lo4.w, lo4.z, lo4.y, lo4.x};
-      uint32_t sum = 0;
+    uint32_t upto = count;  // with the digits above, within the warp
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum += c[i];
-      }
-      uint32_t before = sum;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const uint32_t o = __shfl_up_sync(0xffffffffu, before, off);
-        if (lane >= off) before += o;
-      }
-      before -= sum;
-      if (before < need && need <= before + sum) {  // one lane
-        int i = 0;
-#pragma unroll
-        for (int d = 0; d < 7; ++d)
-          if (i == d && before + c[d] < need) {
-            before += c[d];
-            ++i;
-          }
-        uint32_t ci = c[0];
-#pragma unroll
-        for (int d = 1; d < 8; ++d) ci = i == d ? c[d] : ci;
-        sh.digit = 255 - 8 * lane - i;
-        sh.need = need - before;
-        sh.taken = ci == need - before;
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += o;
+    }
+    if (tid < 256 && lane == 31) sh.warp_gt[warp] = upto;
+    __syncthreads();
+    if (tid < 256) {
+      for (int w = 0; w < warp; ++w) upto += sh.warp_gt[w];
+      if (upto - count < need && need <= upto) {  // one thread
+        sh.digit = 255 - tid;
+        sh.need = need - (upto - count);
+        sh.taken = count == need - (upto - count);
       }
     }
     __syncthreads();
@@ -400,10 +391,9 @@ constexpr int kMoveThreads = 256;
 // flight a thread, whose places are looked up once a row, a batch ahead.
 struct MoveArgs {
   int pieces;    // 16-byte pieces of a K and of a V row that one CTA moves
-  int batch;     // rows at a time, at most kMoveThreads
-  int rows;      // of one CTA: a multiple of batch
+  int batch;     // rows at a time
   int chunks;    // CTAs along the rows
-  int col_ctas;  // CTAs along the columns of K and V; one more has the weights
+  int col_ctas;  // CTAs along the columns of K and V; the first has the weights too
 };
 
 // Where a row comes from and goes to (pages; -1 for neither: it stays).
@@ -425,73 +415,103 @@ __device__ __forceinline__ MovePlace move_place(const PagedArgs &a, const EvictA
   return p;
 }
 
-template <bool kInPlace>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const PagedArgs a, const EvictArgs e, const MoveArgs m) {
-  __shared__ MovePlace places[2][kMoveThreads];
+// One batch of a thread: its pieces of K and V and a weight, and where they go.
+template <int kThreads, int kItems>
+struct MoveBatch {
+  uint4 x[kItems];
+  uint4 *to[kItems];
+  float wx;
+  float *w_to;
+  __device__ __forceinline__ void load(const PagedArgs &a, const MoveArgs &m, const MovePlace *places, int h, int col, int i0) {
+    const int tid = threadIdx.x, log_p = 31 - __clz(m.pieces);  // a power of two
+    const int items = m.batch * m.pieces * 2;
+    w_to = nullptr;
+    if (col == 0 && i0 == 0 && tid < m.batch) {
+      const MovePlace p = places[tid];
+      if (p.from >= 0) {
+        float *const w = a.w + h * a.ws[1];
+        wx = w[p.from * a.ws[0] + p.from_row];
+        w_to = w + p.to * a.ws[0] + p.to_row;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      const int i = i0 + u * kThreads + tid;
+      to[u] = nullptr;
+      if (i >= items) continue;
+      const int c = col * m.pieces + (i & (m.pieces - 1));
+      const bool is_v = (i >> log_p) & 1;
+      const MovePlace p = places[i >> (log_p + 1)];
+      if (p.from < 0) continue;
+      const long long *st = is_v ? a.vs : a.ks;
+      uint4 *const head = static_cast<uint4 *>(is_v ? a.v : a.k) + h * (st[1] / 8) + c;
+      x[u] = head[p.from * (st[0] / 8) + p.from_row * (st[2] / 8)];
+      to[u] = head + p.to * (st[0] / 8) + p.to_row * (st[2] / 8);
+    }
+  }
+  __device__ __forceinline__ void store() {
+#pragma unroll
+    for (int u = 0; u < kItems; ++u)
+      if (to[u] != nullptr) *to[u] = x[u];
+    if (w_to != nullptr) *w_to = wx;
+  }
+};
+
+constexpr int kInPlaceItems = 4;
+
+// In place: two pieces of K and of V of 512 rows at a time, or with many units
+// four of 128 (64 bytes, which HBM likes better, and two CTAs an SM).
+template <int kInPlaceThreads>
+__global__ void __launch_bounds__(kInPlaceThreads) evict_in_place_kernel(const PagedArgs a, const EvictArgs e, const MoveArgs m) {
+  __shared__ MovePlace places[3][kInPlaceThreads];
   const int tid = threadIdx.x;
-  const int cols = m.col_ctas + 1;
-  const int col = blockIdx.x % cols, rest = blockIdx.x / cols;
-  const int chunk = rest % m.chunks, unit = rest / m.chunks;
+  const int col = blockIdx.x % m.col_ctas, unit = blockIdx.x / m.col_ctas;
   const int b = unit / a.Hkv, h = unit % a.Hkv;
   // new_lens may be kv_lens: the minimum is the same before and after its write.
   const int n = min(clamp_len(e.kv_lens, b, e.max_kv), e.budget);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // kept is there
-  if (col == m.col_ctas && chunk == 0 && h == 0 && tid == 0) e.new_lens[b] = n;
-  const int lo = chunk * m.rows, hi = min(n, lo + m.rows);
-  if (lo >= hi) return;
+  if (col == 0 && h == 0 && tid == 0) e.new_lens[b] = n;
   const int *kept = e.kept + ((long long)b * a.Hkv + h) * e.budget;
-  auto look_up = [&](int r0, int buf) {
-    if (tid < m.batch) places[buf][tid] = move_place(a, e, b, kept, r0 + tid, hi);
+  auto look_up = [&](int batch) {
+    if (tid < m.batch) places[batch % 3][tid] = move_place(a, e, b, kept, batch * m.batch + tid, n);
   };
-  if (col == m.col_ctas) {
-    // The weights: a thread a row.
-    float *const w = a.w + h * a.ws[1];
-    for (int r0 = lo; r0 < hi; r0 += kMoveThreads) {
-      const MovePlace p = move_place(a, e, b, kept, r0 + tid, hi);
-      float x = 0.f;
-      if (p.from >= 0) x = w[p.from * a.ws[0] + p.from_row];
-      if (kInPlace) __syncthreads();
-      if (p.from >= 0) w[p.to * a.ws[0] + p.to_row] = x;
-    }
-    return;
-  }
-  constexpr int kUnroll = 8;
-  const int log_p = 31 - __clz(m.pieces);  // a power of two
-  const int c0 = col * m.pieces;
-  const int items = m.batch * m.pieces * 2;  // of a batch; in place at most kUnroll a thread
-  look_up(lo, 0);
+  // A batch is read before the one before it is written; its places are looked up
+  // a batch earlier still.
+  const int batches = (n + m.batch - 1) / m.batch;
+  MoveBatch<kInPlaceThreads, kInPlaceItems> cur, next;
+  if (batches == 0) return;
+  look_up(0);
+  look_up(1);
   __syncthreads();
-  int buf = 0;
-  for (int r0 = lo; r0 < hi; r0 += m.batch, buf ^= 1) {
-    for (int i0 = tid; i0 < items; i0 += kMoveThreads * kUnroll) {
-      uint4 x[kUnroll];
-      uint4 *to[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int i = i0 + u * kMoveThreads;
-        to[u] = nullptr;
-        if (i >= items) continue;
-        const int c = c0 + (i & (m.pieces - 1)), row = i >> (log_p + 1);
-        const bool is_v = (i >> log_p) & 1;
-        const MovePlace p = places[buf][row];
-        if (p.from < 0) continue;
-        const long long *st = is_v ? a.vs : a.ks;
-        uint4 *const head = static_cast<uint4 *>(is_v ? a.v : a.k) + h * (st[1] / 8) + c;
-        x[u] = head[p.from * (st[0] / 8) + p.from_row * (st[2] / 8)];
-        to[u] = head + p.to * (st[0] / 8) + p.to_row * (st[2] / 8);
-      }
-      if (kInPlace) {
-        look_up(r0 + m.batch, buf ^ 1);
-        __syncthreads();
-      }
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (to[u] != nullptr) *to[u] = x[u];
-    }
-    if (!kInPlace && r0 + m.batch < hi) {
-      look_up(r0 + m.batch, buf ^ 1);
-      __syncthreads();
-    }
+  cur.load(a, m, places[0], h, col, 0);
+  for (int i = 0; i < batches; ++i) {
+    if (i + 1 < batches) next.load(a, m, places[(i + 1) % 3], h, col, 0);
+    look_up(i + 2);
+    __syncthreads();  // all have read batch i (and what it overwrites lies in batches up to i)
+    cur.store();
+    cur = next;
+  }
+}
+
+// To other pages: a batch of 128 rows a CTA, whole rows.
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const PagedArgs a, const EvictArgs e, const MoveArgs m) {
+  __shared__ MovePlace places[kMoveThreads];
+  const int tid = threadIdx.x;
+  const int chunk = blockIdx.x % m.chunks, unit = blockIdx.x / m.chunks;
+  const int b = unit / a.Hkv, h = unit % a.Hkv;
+  const int n = min(clamp_len(e.kv_lens, b, e.max_kv), e.budget);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (chunk == 0 && h == 0 && tid == 0) e.new_lens[b] = n;
+  const int lo = chunk * m.batch;
+  if (lo >= n) return;
+  const int *kept = e.kept + ((long long)b * a.Hkv + h) * e.budget;
+  if (tid < m.batch) places[tid] = move_place(a, e, b, kept, lo + tid, n);
+  __syncthreads();
+  constexpr int kItems = 8;
+  for (int i0 = 0; i0 < m.batch * m.pieces * 2; i0 += kMoveThreads * kItems) {
+    MoveBatch<kMoveThreads, kItems> x;
+    x.load(a, m, places, h, 0, i0);
+    x.store();
   }
 }
 
@@ -508,12 +528,13 @@ cudaError_t launch_evict(const PagedArgs &a, const EvictArgs &e, int num_sms, cu
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
   std::call_once(once, [] {
-    attr = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelHeld * 4);
+    for (auto kern : {evict_select_kernel<512>, evict_select_kernel<1024>})
+      if (attr == cudaSuccess) attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelHeld * 4);
   });
   if (attr != cudaSuccess) return attr;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * ranks));
-  cfg.blockDim = dim3(kSelThreads);
+  cfg.blockDim = dim3(ranks > 1 ? 1024 : 512);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -522,7 +543,7 @@ cudaError_t launch_evict(const PagedArgs &a, const EvictArgs &e, int num_sms, cu
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  cudaError_t err = cudaLaunchKernelEx(&cfg, evict_select_kernel, a, e);
+  cudaError_t err = cudaLaunchKernelEx(&cfg, ranks > 1 ? evict_select_kernel<1024> : evict_select_kernel<512>, a, e);
   if (err != cudaSuccess) return err;
 
   MoveArgs m;
@@ -531,27 +552,30 @@ cudaError_t launch_evict(const PagedArgs &a, const EvictArgs &e, int num_sms, cu
   if (e.out_table != nullptr) {
     m.pieces = row_pieces;
     m.batch = 128;
-    m.rows = m.batch;
+    m.col_ctas = 1;
+    m.chunks = (most + m.batch - 1) / m.batch;
   } else {
-    m.pieces = units * (row_pieces / 4) >= 2LL * num_sms ? 4 : 2;  // 64 bytes; 32 with few units
-    m.batch = kMoveThreads;
-    m.rows = (most + m.batch - 1) / m.batch * m.batch;
+    // Both ways measured, us: 256 units of 1024 rows of head_dim 128 in 32 bytes 123,
+    // in 64 bytes 109; 8 units of 16384 rows 123 and 177.
+    m.pieces = units * (row_pieces / 4) >= 2LL * num_sms ? 4 : 2;
+    m.batch = (m.pieces == 4 ? 256 : 512) * kInPlaceItems / (2 * m.pieces);
+    m.col_ctas = row_pieces / m.pieces;
+    m.chunks = 1;
   }
-  m.col_ctas = row_pieces / m.pieces;
-  m.chunks = (most + m.rows - 1) / m.rows;
-  const long long grid = units * m.chunks * (m.col_ctas + 1);
+  const long long grid = units * m.chunks * m.col_ctas;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
   cudaLaunchConfig_t mc = {};
   mc.gridDim = dim3((unsigned)grid);
-  mc.blockDim = dim3(kMoveThreads);
+  mc.blockDim = dim3(e.out_table != nullptr ? kMoveThreads : (m.pieces == 4 ? 256 : 512));
   mc.stream = s;
   cudaLaunchAttribute ma[1];
   ma[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   ma[0].val.programmaticStreamSerializationAllowed = 1;
   mc.attrs = ma;
   mc.numAttrs = 1;
-  return e.out_table != nullptr ? cudaLaunchKernelEx(&mc, evict_move_kernel<false>, a, e, m)
-                                : cudaLaunchKernelEx(&mc, evict_move_kernel<true>, a, e, m);
+  if (e.out_table != nullptr) return cudaLaunchKernelEx(&mc, evict_move_kernel, a, e, m);
+  return m.pieces == 4 ? cudaLaunchKernelEx(&mc, evict_in_place_kernel<256>, a, e, m)
+                       : cudaLaunchKernelEx(&mc, evict_in_place_kernel<512>, a, e, m);
 }
 
 }  // namespace
