@@ -636,7 +636,7 @@ constexpr int kSchedConsumers256 = 1 + 1 + 4;  // MMA thread, V thread, one lane
 
 struct Bars256 {
   uint64_t q_full, q_empty, k_full, k_empty, v_full, v_empty;
-  uint64_t s_full[2], p_full[2], o_done;
+  uint64_t s_full[2], p_full[2], o_done[2];  // by the block's parity
   uint64_t drain;
   uint64_t sched_full[kSchedSlots], sched_empty[kSchedSlots];
   int sched_w[kSchedSlots];
@@ -697,7 +697,9 @@ __device__ bool tma_v256(const CUtensorMap *tm_v, uint8_t *smem, Bars256 *bars, 
 
 // MMAs of one item: QK(g0), QK(g0 + 1), then per block PV(g), QK(g + 2).
 // Block g's scores live in S_(g & 1); s_full / p_full of a buffer complete
-// once per block that uses it (phase g >> 1); o_done once per block.
+// once per block that uses it (phase g >> 1), and o_done alike: with one
+// barrier for both, the last wait of an item could find two phases completed,
+// and a wait for the parity of the older one then never returns.
 template <bool kBF16, bool kFold>
 __device__ bool mma_256(uint8_t *smem, Bars256 *bars, uint32_t tmem, int nb, int tile_it, int g0) {
   using C = Cfg256;
@@ -755,7 +757,7 @@ __device__ bool mma_256(uint8_t *smem, Bars256 *bars, uint32_t tmem, int nb, int
     if (!wait(&bars->v_full, g & 1) || !wait(&bars->p_full[g & 1], (g >> 1) & 1)) return false;
     tc_fence_after();
     issue_pv(g & 1, j > 0);
-    tc_commit(&bars->o_done);
+    tc_commit(&bars->o_done[g & 1]);
     tc_commit(&bars->v_empty);
     if (j + 2 < nb && !qk_block(g + 2, j + 3 == nb)) return false;
     if (bars->abort_flag) return false;
@@ -821,9 +823,7 @@ __device__ bool softmax_256(const AttnArgs &a, Bars256 *bars, uint32_t tmem, int
     }
     if (__any_sync(0xffffffffu, rescale)) {
       // O holds blocks 0..j-1 once PV(g - 1) is done; rescale it in place.
-      // (S(g) arriving means PV(g - 2) completed, so o_done is at most one
-      // phase behind the one waited for.)
-      ok = mbar_wait_or_abort(&bars->o_done, (g - 1) & 1, kTimeoutNs, &bars->abort_flag);
+      ok = mbar_wait_or_abort(&bars->o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, kTimeoutNs, &bars->abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         set_abort(bars, a.err);
         aborted = true;
@@ -847,14 +847,8 @@ __device__ bool softmax_256(const AttnArgs &a, Bars256 *bars, uint32_t tmem, int
   }
 
   if (!aborted && br.nb > 0) {
-    // QK(g) is issued before PV(g - 1), so when the last block's scores
-    // arrived only PV(last - 2) was known complete: wait for o_done's phase
-    // last - 1 and then last (a parity wait must never be two phases ahead
-    // of the barrier, or it would match the older phase of equal parity).
     const int gl = g0 + br.nb - 1;
-    bool ok = true;
-    if (br.nb >= 2) ok = mbar_wait_or_abort(&bars->o_done, (gl - 1) & 1, kTimeoutNs, &bars->abort_flag);
-    ok = ok && mbar_wait_or_abort(&bars->o_done, gl & 1, kTimeoutNs, &bars->abort_flag);
+    bool ok = mbar_wait_or_abort(&bars->o_done[gl & 1], (gl >> 1) & 1, kTimeoutNs, &bars->abort_flag);
     if (!__all_sync(0xffffffffu, ok)) {
       set_abort(bars, a.err);
       aborted = true;
@@ -930,8 +924,8 @@ __global__ void __launch_bounds__(kThreads256, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_full[i], kBM);
+      mbar_init(&bars->o_done[i], 1);
     }
-    mbar_init(&bars->o_done, 1);
     for (int i = 0; i < kSchedSlots; ++i) {
       mbar_init(&bars->sched_full[i], 1);
       mbar_init(&bars->sched_empty[i], kSchedConsumers256);
