@@ -1132,8 +1132,7 @@ constexpr size_t kScoreBytes = size_t(1) << 30;
 llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs &k, Plan *plan) {
   const bool can = paged_tc_supports(a);
   if (p->algo == LLMX_ALGO_TCGEN05 && !can)
-    return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: TCGEN05 needs head_dim 64 or 128, sm_scale > 0 and at most 128 "
-                                              "query heads a kv head");
+    return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: TCGEN05 needs sm_scale > 0 and at most 128 query heads a kv head");
   plan->tc = can && (p->algo == LLMX_ALGO_TCGEN05 || (p->algo == LLMX_ALGO_AUTO && (long long)a.Sq * a.group > kStepRows));
   const bool weights = k.w != nullptr;
   const long long R = (long long)a.Sq * a.group;

@@ -1,10 +1,10 @@
 // Attention over a paged 16-bit key/value cache on the tensor cores: chunks of
-// query rows (more than 64 rows of a kv head), head_dim 64 and 128.
+// query rows (more than 32 rows of a kv head).
 //
 // The scheme is the dense prefill's (attn_sm100.cu): a CTA has two tiles of up
 // to 128 rows, S = Q K^T and O += P V on tcgen05.mma with both accumulators in
-// tensor memory, a softmax warpgroup for each tile, lazy rescaling.  What is
-// different:
+// tensor memory, a softmax warpgroup for each tile, lazy rescaling; at head_dim
+// 256 one tile with two score accumulators.  What is different:
 //
 //  * Rows are packed: a tile has M = (128 / group) * group rows, all query heads
 //    of a kv head for 128 / group query rows (one TMA box over [head][row]), so
@@ -33,10 +33,28 @@
 namespace llmx_b200 {
 namespace {
 
-constexpr int kVWarp = 10;     // passes V blocks on
-constexpr int kSlopeWarp = 11; // writes A' (ALiBi)
-constexpr int kConsumers = 1 + 8 + 2;
-constexpr int kItemRows = kTiles * kBM;
+// What differs between head_dim 64, 128 (two tiles; warps 0-7 softmax) and 256 (one
+// tile; warps 0-3).
+template <int D>
+struct PCfg : Cfg<D> {
+  static constexpr bool kOne = false;
+  static constexpr int kItemRows = kTiles * kBM;
+  static constexpr int kThreads = llmx_b200::kThreads;
+  static constexpr int kMma = kMmaWarp, kLoad = kTmaWarp;
+  static constexpr int kV = 10;  // passes V blocks on; the last warp writes A' (ALiBi)
+  static constexpr int kConsumers = 1 + 8 + 2;
+};
+template <>
+struct PCfg<256> : Cfg256 {
+  static constexpr bool kOne = true;
+  static constexpr int kItemRows = kBM;
+  static constexpr int kStages = 1;
+  static constexpr uint32_t kTmemO0 = kTmemO, kTmemO1 = kTmemO;
+  static constexpr int kThreads = 256;
+  static constexpr int kMma = 4, kLoad = 5, kLoadV = 6;
+  static constexpr int kV = 7;  // writes A', then passes V blocks on
+  static constexpr int kConsumers = 1 + 4 + 2;
+};
 
 template <typename T>
 constexpr int tc_shift() {
@@ -48,14 +66,15 @@ struct TcWork {
   PagedArgs c;
   int R;            // packed rows of a kv head
   int M;            // rows of a tile
+  int tiles;        // of an item
   int n_mblocks;    // items of a unit
   int group_units;  // units whose K / V fit in L2 together
   int n_whole;      // items [0, n_whole) are whole, the others in `parts` pieces
   int parts;
   int n_work;
   int box;         // tokens of a TMA box
-  float *part_o;   // [pieces][256][D]
-  float *part_ml;  // [pieces][256][2]
+  float *part_o;   // [pieces][128 tiles][D]
+  float *part_ml;  // [pieces][128 tiles][2]
   float *stat;     // nullable [units][R]: log2 of the sum of 2^score
 };
 
@@ -103,12 +122,12 @@ __device__ __forceinline__ Item decode_item(const AttnArgs &a, const TcWork &wk,
   t.b = unit / a.Hkv;
   t.ql = clamp_len(a.q_lens, t.b, a.Sq);
   t.kl = clamp_len(a.kv_lens, t.b, a.Skv);
-  t.m0 = mblk * 2 * wk.M;
-  const RowsSee s = rows_see(a, t.m0, 2 * wk.M, t.ql, t.kl);
+  t.m0 = mblk * wk.tiles * wk.M;
+  const RowsSee s = rows_see(a, t.m0, wk.tiles * wk.M, t.ql, t.kl);
   const int lo = s.lo / kBN * kBN;
   int nb = s.hi > s.lo ? (s.hi - lo + kBN - 1) / kBN : 0;
   int nb0 = nb;
-  if (nb > 0) {
+  if (nb > 0 && wk.tiles == 2) {
     const RowsSee s0 = rows_see(a, t.m0, wk.M, t.ql, t.kl);
     nb0 = (max(s0.hi, lo) - lo + kBN - 1) / kBN;
   }
@@ -150,10 +169,11 @@ struct Loads {
   int k = 0, v = 0, q[2] = {0, 0};
 };
 
-template <int D, bool kReverse>
+// kWhat: 3 all, 1 Q and K, 2 V.
+template <int D, bool kReverse, int kWhat>
 __device__ bool load_item(const CUtensorMap *tm_q, const CUtensorMap *tm_k, const CUtensorMap *tm_v, uint8_t *smem, PBars *bars,
                           const AttnArgs &a, const TcWork &wk, const Item &t, int tile_it, int kv_base, Loads &n) {
-  using C = Cfg<D>;
+  using C = PCfg<D>;
   const int lane = threadIdx.x % 32;
   auto wait = [&](uint64_t *bar, uint32_t par) {
     const bool ok = mbar_wait_or_abort(bar, par, kTimeoutNs, &bars->abort_flag);
@@ -171,20 +191,24 @@ __device__ bool load_item(const CUtensorMap *tm_q, const CUtensorMap *tm_k, cons
     return true;
   };
   BoxPlace next = box_place(wk.c, wk.box, t.b, t.kl, block_n0<kReverse>(t.br, 0));
-  if (!load_q(0)) return false;
+  if ((kWhat & 1) && !load_q(0)) return false;
   for (int j = 0; j < t.br.nb; ++j) {
     const int g = kv_base + j;
     const int s = g % C::kStages;
     const uint32_t par = ((g / C::kStages) & 1) ^ 1;
     const BoxPlace p = next;
     if (j + 1 < t.br.nb) next = box_place(wk.c, wk.box, t.b, t.kl, block_n0<kReverse>(t.br, j + 1));
-    if (!wait(&bars->k_empty[s], par)) return false;
-    load_boxes<D>(smem + C::kKOff + s * C::kTileBytes, tm_k, &bars->k_full[s], wk.box, t.kvh, p);
-    n.k = g + 1;
-    if (j == 0 && !load_q(1)) return false;
-    if (!wait(&bars->v_empty[s], par)) return false;
-    load_boxes<D>(smem + C::kVOff + s * C::kTileBytes, tm_v, &bars->v_landed[s], wk.box, t.kvh, p);
-    n.v = g + 1;
+    if (kWhat & 1) {
+      if (!wait(&bars->k_empty[s], par)) return false;
+      load_boxes<D>(smem + C::kKOff + s * C::kTileBytes, tm_k, &bars->k_full[s], wk.box, t.kvh, p);
+      n.k = g + 1;
+      if (!C::kOne && j == 0 && !load_q(1)) return false;
+    }
+    if (kWhat & 2) {
+      if (!wait(&bars->v_empty[s], par)) return false;
+      load_boxes<D>(smem + C::kVOff + s * C::kTileBytes, tm_v, &bars->v_landed[s], wk.box, t.kvh, p);
+      n.v = g + 1;
+    }
   }
   return true;
 }
@@ -192,7 +216,7 @@ __device__ bool load_item(const CUtensorMap *tm_q, const CUtensorMap *tm_k, cons
 // Every load issued must have landed before the CTA may exit.
 template <int D>
 __device__ void drain_loads(PBars *bars, const Loads &n) {
-  using C = Cfg<D>;
+  using C = PCfg<D>;
   for (int q = 0; q < 2; ++q)
     if (n.q[q] > 0) mbar_wait(&bars->q_full[q], (n.q[q] - 1) & 1, kTimeoutNs);
   for (int g = max(0, n.k - C::kStages); g < n.k; ++g)
@@ -207,7 +231,7 @@ __device__ void drain_loads(PBars *bars, const Loads &n) {
 // in a bank.
 template <typename T, int D>
 __device__ void clean_block(uint8_t *v, uint32_t (&lost)[4], int rows) {
-  using C = Cfg<D>;
+  using C = PCfg<D>;
   constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
   const int lane = threadIdx.x % 32;
 #pragma unroll 1
@@ -260,12 +284,12 @@ __device__ void clean_block(uint8_t *v, uint32_t (&lost)[4], int rows) {
 template <typename T, int D, bool kAlibi, bool kSoftcap>
 __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, uint32_t tmem, int warp, const Item &w, int blk_base,
                              int kv_base) {
-  using C = Cfg<D>;
+  using C = PCfg<D>;
   constexpr int kShift = tc_shift<T>();
   const float kNegInf = -CUDART_INF_F;
-  const int t = warp / 4;
+  const int t = C::kOne ? 0 : warp / 4;
   BlockRange br = w.br;
-  if (t == 0) br.nb = w.nb0;
+  if (!C::kOne && t == 0) br.nb = w.nb0;
   const int r = threadIdx.x % kBM;
   const int row0 = w.m0 + t * wk.M;
   const int pr = row0 + r;
@@ -274,9 +298,8 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
   const int h = w.kvh * a.group + (real ? pr - qi * a.group : 0);
   const Visible vis = real ? row_visible(a, qi, w.ql, w.kl) : Visible{0, 0};
   const RowsSee tile = rows_see(a, row0, wk.M, w.ql, w.kl);
-  const RowsSee both = rows_see(a, w.m0, 2 * wk.M, w.ql, w.kl);
+  const RowsSee both = rows_see(a, w.m0, wk.tiles * wk.M, w.ql, w.kl);
   const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
-  const uint32_t tS = tmem + lane_off + (t ? C::kTmemS1 : C::kTmemS0);
   const uint32_t tO = tmem + lane_off + (t ? C::kTmemO1 : C::kTmemO0);
   const float scale2 = a.sm_scale * kLog2e;
   const float slope = kAlibi ? a.alibi[h] : 0.f;
@@ -286,10 +309,15 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
   const float cap_out = kSoftcap ? a.softcap * kLog2e : 0.f;
   float m_used = kNegInf, l = 0.f;
   bool aborted = false;
+  // The barrier of block i of the launch and its phase: a tile's own, or with one
+  // tile by the block's parity, as the score accumulators.
+  auto which = [&](int i) { return C::kOne ? i & 1 : t; };
+  auto phase = [&](int i) { return (uint32_t)(C::kOne ? (i >> 1) & 1 : i & 1); };
 
   for (int j = 0; j < br.nb; ++j) {
-    const int n0 = block_n0<kAlibi>(br, j);
-    bool ok = mbar_wait_or_abort(&bars->s_full[t], (blk_base + j) & 1, kTimeoutNs, &bars->abort_flag);
+    const int n0 = block_n0<kAlibi>(br, j), i = blk_base + j;
+    const uint32_t tS = tmem + lane_off + (which(i) ? C::kTmemS1 : C::kTmemS0);
+    bool ok = mbar_wait_or_abort(&bars->s_full[which(i)], phase(i), kTimeoutNs, &bars->abort_flag);
     if (!__all_sync(0xffffffffu, ok)) {
       set_abort(bars, a.err);
       aborted = true;
@@ -326,10 +354,10 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
         break;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t bits = *reinterpret_cast<volatile uint32_t *>(&bars->lost[s][i]);
+      for (int word = 0; word < 4; ++word) {
+        const uint32_t bits = *reinterpret_cast<volatile uint32_t *>(&bars->lost[s][word]);
         if (bits != 0u) {
-          const int b0 = min(max(lo - i * 32, 0), 32), b1 = min(max(hi - i * 32, 0), 32);
+          const int b0 = min(max(lo - word * 32, 0), 32), b1 = min(max(hi - word * 32, 0), 32);
           const uint32_t below1 = b1 >= 32 ? 0xffffffffu : ((1u << b1) - 1u);
           const uint32_t below0 = b0 >= 32 ? 0xffffffffu : ((1u << b0) - 1u);
           if (bits & below1 & ~below0) l = CUDART_NAN_F;
@@ -337,7 +365,7 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
       }
     }
     if (__any_sync(0xffffffffu, rescale)) {
-      ok = mbar_wait_or_abort(&bars->o_done[t], (blk_base + j - 1) & 1, kTimeoutNs, &bars->abort_flag);
+      ok = mbar_wait_or_abort(&bars->o_done[which(i - 1)], phase(i - 1), kTimeoutNs, &bars->abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         set_abort(bars, a.err);
         aborted = true;
@@ -357,11 +385,12 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
     }
     tmem_wait_st();
     tc_fence_before();
-    mbar_arrive(&bars->p_full[t]);
+    mbar_arrive(&bars->p_full[which(i)]);
   }
 
   if (!aborted && br.nb > 0) {
-    bool ok = mbar_wait_or_abort(&bars->o_done[t], (blk_base + br.nb - 1) & 1, kTimeoutNs, &bars->abort_flag);
+    const int i = blk_base + br.nb - 1;
+    bool ok = mbar_wait_or_abort(&bars->o_done[which(i)], phase(i), kTimeoutNs, &bars->abort_flag);
     if (!__all_sync(0xffffffffu, ok)) {
       set_abort(bars, a.err);
       aborted = true;
@@ -372,7 +401,7 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
   const bool have = !aborted && br.nb > 0;
   if (w.slot >= 0) {
     // A piece: O and l as they are (P of the row's maximum is 2^kShift).
-    const long long prow = (long long)w.slot * kItemRows + t * kBM + r;
+    const long long prow = (long long)w.slot * C::kItemRows + t * kBM + r;
     float *po = wk.part_o + prow * D;
 #pragma unroll 1
     for (int ch = 0; ch < D / 32; ++ch) {
@@ -443,11 +472,11 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
 
 // ------------------------------------------------------------------ kernel
 template <typename T, int D, bool kAlibi, bool kSoftcap>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnArgs a,
                     const __grid_constant__ TcWork wk, int *work_ctr) {
-  using C = Cfg<D>;
+  using C = PCfg<D>;
   constexpr bool kFold = kAlibi && !kSoftcap;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
@@ -473,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kSchedSlots; ++i) {
       mbar_init(&bars->sched_full[i], 1);
-      mbar_init(&bars->sched_empty[i], kConsumers);
+      mbar_init(&bars->sched_empty[i], C::kConsumers);
     }
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
@@ -481,21 +510,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if constexpr (kFold) {
     // B' row c = [c, c, c, 0, ...]; A' zero (its columns 0-2 are written per item).
-    for (int u = threadIdx.x; u < 3 * 256; u += kThreads) {
+    constexpr int kA = C::kOne ? 1 : 2;  // of A'
+    for (int u = threadIdx.x; u < (kA + 1) * 256; u += C::kThreads) {
       const int op = u >> 8, e = u & 255;
       const int r = (e >> 4) * 8 + (e & 7), khalf = (e >> 3) & 1;
-      const float c = (op == 2 && khalf == 0) ? (float)r : 0.f;
+      const float c = (op == kA && khalf == 0) ? (float)r : 0.f;
       const float f[8] = {c, c, c, 0.f, 0.f, 0.f, 0.f, 0.f};
       *reinterpret_cast<uint4 *>(smem + C::kXOff + op * C::kXBytes + x_offset(r, khalf * 8)) = pack8<T>(f);
     }
     fence_proxy_async_smem();
   }
-  if (warp == kTmaWarp && lane == 0) {
+  if (warp == C::kLoad && lane == 0) {
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
   }
-  if (warp == kMmaWarp) {
+  if (warp == C::kMma) {
     tmem_alloc(&bars->tmem_base, C::kTmemCols);
     tmem_relinquish();
   }
@@ -504,9 +534,56 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
 
-  if (warp >= 8) {
-    regs_decrease<kRegsControl>();
-    if (warp == kTmaWarp) {
+  // Each role runs through the items; what it does with one returns false when the
+  // kernel is aborting.
+  auto each_item = [&](bool warp_wide, auto role) {
+    for (int seq = 0;; ++seq) {
+      Item t;
+      const int w = take(bars, seq, warp_wide, t);
+      if (w >= wk.n_work) break;
+      if (w < 0 || !role(t)) {
+        set_abort(bars, a.err);
+        break;
+      }
+    }
+  };
+  // A' of an item (ALiBi): beta = slope / sm_scale as three 16-bit parts (each the
+  // rounding of what the ones before it leave), in columns 0-2 of the rows.
+  auto write_slopes = [&](const Item &t, int it) {
+    for (int q = 0; q < wk.tiles; ++q) {
+      bool ok = true;
+      if (it > 0) ok = mbar_wait_or_abort(&bars->q_empty[q], (it - 1) & 1, kTimeoutNs, &bars->abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+#pragma unroll 1
+      for (int r = lane; r < kBM; r += 32) {
+        const float b = a.alibi[t.kvh * a.group + (t.m0 + q * wk.M + r) % a.group] / a.sm_scale;
+        const float r1 = b - Elem<T>::to_f(Elem<T>::from_f(b));
+        const float r2 = r1 - Elem<T>::to_f(Elem<T>::from_f(r1));
+        const float f[8] = {b, r1, r2, 0.f, 0.f, 0.f, 0.f, 0.f};
+        *reinterpret_cast<uint4 *>(smem + C::kXOff + q * C::kXBytes + x_offset(r, 0)) = pack8<T>(f);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_full[q]);
+    }
+    return true;
+  };
+  auto pass_v = [&](const Item &t, int kv) {
+    const RowsSee both = rows_see(a, t.m0, wk.tiles * wk.M, t.ql, t.kl);
+    for (int j = 0; j < t.br.nb; ++j) {
+      const int g = kv + j, s = g % C::kStages;
+      const bool ok = mbar_wait_or_abort(&bars->v_landed[s], (g / C::kStages) & 1, kTimeoutNs, &bars->abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      const int n0 = block_n0<kAlibi>(t.br, j);
+      if (partly(both, n0)) clean_block<T, D>(smem + C::kVOff + s * C::kTileBytes, bars->lost[s], t.kl - n0);
+      if (lane == 0) mbar_arrive(&bars->v_full[s]);
+    }
+    return true;
+  };
+  constexpr int kSoftmaxWarps = C::kOne ? 4 : 8;
+  if (warp >= kSoftmaxWarps) {
+    if constexpr (!C::kOne) regs_decrease<kRegsControl>();
+    if (warp == C::kLoad) {
       Loads n;
       int kv = 0, it = 0;
       int w = (int)blockIdx.x;
@@ -522,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (w >= wk.n_work) break;
         if (t.br.nb > 0) {
-          ok = load_item<D, kAlibi>(&tm_q, &tm_k, &tm_v, smem, bars, a, wk, t, it, kv, n);
+          ok = load_item<D, kAlibi, C::kOne ? 1 : 3>(&tm_q, &tm_k, &tm_v, smem, bars, a, wk, t, it, kv, n);
           kv += t.br.nb;
           ++it;
           if (!ok) {
@@ -538,114 +615,72 @@ __global__ void __launch_bounds__(kThreads, 1)
         w = next;
       }
       drain_loads<D>(bars, n);
-    } else if (warp == kMmaWarp && lane == 0) {
-      int kv = 0, it = 0, blk0 = 0;
-      for (int seq = 0;; ++seq) {
-        Item t;
-        const int w = take(bars, seq, false, t);
-        if (w < 0) {
-          set_abort(bars, a.err);
-          break;
-        }
-        if (w >= wk.n_work) break;
-        if (t.br.nb == 0) continue;
-        const bool ok = mma_tile<D, kBF16, kFold, kAlibi>(smem, bars, tmem, t.br.nb, t.nb0, it, kv, blk0, kv);
-        kv += t.br.nb;
-        blk0 += t.nb0;
-        ++it;
-        if (!ok) {
-          set_abort(bars, a.err);
-          break;
-        }
-      }
-      tc_commit(&bars->drain);
-      mbar_wait(&bars->drain, 0, kTimeoutNs);
-    } else if (warp == kVWarp) {
-      int kv = 0;
-      for (int seq = 0;; ++seq) {
-        Item t;
-        const int w = take(bars, seq, true, t);
-        if (w < 0) {
-          set_abort(bars, a.err);
-          break;
-        }
-        if (w >= wk.n_work) break;
-        const RowsSee both = rows_see(a, t.m0, 2 * wk.M, t.ql, t.kl);
-        bool ok = true;
-        for (int j = 0; j < t.br.nb && ok; ++j) {
-          const int g = kv + j, s = g % C::kStages;
-          ok = mbar_wait_or_abort(&bars->v_landed[s], (g / C::kStages) & 1, kTimeoutNs, &bars->abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int n0 = block_n0<kAlibi>(t.br, j);
-          if (partly(both, n0)) clean_block<T, D>(smem + C::kVOff + s * C::kTileBytes, bars->lost[s], t.kl - n0);
-          if (lane == 0) mbar_arrive(&bars->v_full[s]);
-        }
-        kv += t.br.nb;
-        if (!ok) {
-          set_abort(bars, a.err);
-          break;
-        }
-      }
-    } else if (warp == kSlopeWarp) {
-      int it = 0;
-      for (int seq = 0;; ++seq) {
-        Item t;
-        const int w = take(bars, seq, true, t);
-        if (w < 0) {
-          set_abort(bars, a.err);
-          break;
-        }
-        if (w >= wk.n_work) break;
-        if constexpr (kFold) {
-          if (t.br.nb == 0) continue;
-          bool ok = true;
-          for (int q = 0; q < kTiles && ok; ++q) {
-            if (it > 0) ok = mbar_wait_or_abort(&bars->q_empty[q], (it - 1) & 1, kTimeoutNs, &bars->abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-#pragma unroll 1
-            for (int r = lane; r < kBM; r += 32) {
-              // beta = slope / sm_scale as three 16-bit parts (each the rounding of
-              // what the ones before it leave), in columns 0-2.
-              const float b = a.alibi[t.kvh * a.group + (t.m0 + q * wk.M + r) % a.group] / a.sm_scale;
-              const float r1 = b - Elem<T>::to_f(Elem<T>::from_f(b));
-              const float r2 = r1 - Elem<T>::to_f(Elem<T>::from_f(r1));
-              const float f[8] = {b, r1, r2, 0.f, 0.f, 0.f, 0.f, 0.f};
-              *reinterpret_cast<uint4 *>(smem + C::kXOff + q * C::kXBytes + x_offset(r, 0)) = pack8<T>(f);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->q_full[q]);
+    } else if (warp == C::kMma) {
+      if (lane == 0) {
+        int kv = 0, it = 0, blk0 = 0;
+        each_item(false, [&](const Item &t) {
+          if (t.br.nb == 0) return true;
+          bool ok;
+          if constexpr (C::kOne) {
+            const Mma256Bars mb = {bars->q_full, bars->q_empty, bars->k_full, bars->k_empty, bars->v_full, bars->v_empty,
+                                   bars->s_full, bars->p_full,  bars->o_done, &bars->abort_flag};
+            ok = mma_256<kBF16, kFold>(smem, mb, tmem, t.br.nb, it, kv);
+          } else {
+            ok = mma_tile<D, kBF16, kFold, kAlibi>(smem, bars, tmem, t.br.nb, t.nb0, it, kv, blk0, kv);
           }
+          kv += t.br.nb;
+          blk0 += t.nb0;
           ++it;
-          if (!ok) {
-            set_abort(bars, a.err);
-            break;
-          }
-        }
+          return ok;
+        });
+        tc_commit(&bars->drain);
+        mbar_wait(&bars->drain, 0, kTimeoutNs);
+      }
+    } else if (warp == C::kV) {
+      int kv = 0, it = 0;
+      each_item(true, [&](const Item &t) {
+        if (t.br.nb == 0) return true;
+        if constexpr (C::kOne && kFold)
+          if (!write_slopes(t, it)) return false;
+        const bool ok = pass_v(t, kv);
+        kv += t.br.nb;
+        ++it;
+        return ok;
+      });
+    } else {
+      if constexpr (C::kOne) {
+        // V's loads.
+        Loads n;
+        int kv = 0;
+        each_item(true, [&](const Item &t) {
+          if (t.br.nb == 0) return true;
+          const bool ok = load_item<D, kAlibi, 2>(&tm_q, &tm_k, &tm_v, smem, bars, a, wk, t, 0, kv, n);
+          kv += t.br.nb;
+          return ok;
+        });
+        drain_loads<D>(bars, n);
+      } else {
+        int it = 0;
+        each_item(true, [&](const Item &t) {
+          if (!kFold || t.br.nb == 0) return true;
+          return write_slopes(t, it++);
+        });
       }
     }
   } else {
-    regs_increase<kRegsSoftmax>();
+    if constexpr (!C::kOne) regs_increase<kRegsSoftmax>();
     int blk = 0, kv = 0;
-    for (int seq = 0;; ++seq) {
-      Item t;
-      const int w = take(bars, seq, true, t);
-      if (w < 0) {
-        set_abort(bars, a.err);
-        break;
-      }
-      if (w >= wk.n_work) break;
-      if (!softmax_rows<T, D, kAlibi, kSoftcap>(a, wk, bars, tmem, warp, t, blk, kv)) break;
-      blk += warp < 4 ? t.nb0 : t.br.nb;
+    each_item(true, [&](const Item &t) {
+      const bool ok = softmax_rows<T, D, kAlibi, kSoftcap>(a, wk, bars, tmem, warp, t, blk, kv);
+      blk += !C::kOne && warp < 4 ? t.nb0 : t.br.nb;
       kv += t.br.nb;
-    }
+      return ok;
+    });
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == C::kMma) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmemCols);
@@ -655,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Merges the pieces of the items that were cut: a warp a row, 32 rows a CTA.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) paged_tc_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ TcWork wk) {
-  constexpr int E = D / 32;
+  constexpr int E = D / 32, kItemRows = PCfg<D>::kItemRows;
   constexpr float kShift = (float)tc_shift<T>();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int cut = blockIdx.x / (kItemRows / 32), first = blockIdx.x % (kItemRows / 32) * 32;
@@ -710,7 +745,7 @@ __global__ void __launch_bounds__(128) paged_tc_merge_kernel(const __grid_consta
 // -------------------------------------------------------------------- host
 template <typename T, int D, bool kAlibi, bool kSoftcap>
 cudaError_t launch_tc_t(const AttnArgs &a, const TcWork &wk, int grid, int *ctr, cudaStream_t s) {
-  using C = Cfg<D>;
+  using C = PCfg<D>;
   CUtensorMap tq, tk, tv;
   if (!make_q_map(&tq, a, wk.M) || !make_page_map(&tk, wk.c, wk.c.k, wk.c.ks, a.dtype, wk.box) ||
       !make_page_map(&tv, wk.c, wk.c.v, wk.c.vs, a.dtype, wk.box))
@@ -720,11 +755,11 @@ cudaError_t launch_tc_t(const AttnArgs &a, const TcWork &wk, int grid, int *ctr,
   static cudaError_t attr = cudaSuccess;
   std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes); });
   if (attr != cudaSuccess) return attr;
-  kern<<<grid, kThreads, C::kSmemBytes, s>>>(tq, tk, tv, a, wk, ctr);
+  kern<<<grid, C::kThreads, C::kSmemBytes, s>>>(tq, tk, tv, a, wk, ctr);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || wk.parts == 1) return e;
   const int cut = (wk.n_work - wk.n_whole) / wk.parts;
-  return launch_paged_after(paged_tc_merge_kernel<T, D>, dim3(cut * (kItemRows / 32)), 128, 0, s, a, wk);
+  return launch_paged_after(paged_tc_merge_kernel<T, D>, dim3(cut * (C::kItemRows / 32)), 128, 0, s, a, wk);
 }
 
 template <typename T, int D>
@@ -734,21 +769,31 @@ cudaError_t launch_tc_d(const AttnArgs &a, const TcWork &wk, int grid, int *ctr,
   return cap ? launch_tc_t<T, D, false, true>(a, wk, grid, ctr, s) : launch_tc_t<T, D, false, false>(a, wk, grid, ctr, s);
 }
 
+template <typename T>
+cudaError_t launch_tc(const AttnArgs &a, const TcWork &wk, int grid, int *ctr, cudaStream_t s) {
+  switch (a.D) {
+    case 64: return launch_tc_d<T, 64>(a, wk, grid, ctr, s);
+    case 128: return launch_tc_d<T, 128>(a, wk, grid, ctr, s);
+    default: return launch_tc_d<T, 256>(a, wk, grid, ctr, s);
+  }
+}
+
 }  // namespace
 
 bool paged_tc_supports(const AttnArgs &a) {
   // The softmax takes the row max on raw scores (sm_scale > 0).
-  if ((a.D != 64 && a.D != 128) || !(a.sm_scale > 0.f) || a.group > kBM) return false;
+  if (!(a.sm_scale > 0.f) || a.group > kBM) return false;
   const long long units = (long long)a.B * a.Hkv;
   const long long M = kBM / a.group * a.group;
-  if (units * (((long long)a.Sq * a.group + 2 * M - 1) / (2 * M)) > INT_MAX / 128) return false;
+  if (units * (((long long)a.Sq * a.group + M - 1) / M) > INT_MAX / 128) return false;
   return paged_weights_supports(a);
 }
 
 PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws) {
   PagedTcPlan p{};
   p.M = kBM / a.group * a.group;
-  p.n_mblocks = (int)(((long long)a.Sq * a.group + 2 * p.M - 1) / (2 * p.M));
+  const int tiles = a.D == 256 ? 1 : kTiles;
+  p.n_mblocks = (int)(((long long)a.Sq * a.group + tiles * p.M - 1) / (tiles * p.M));
   const int items = a.B * a.Hkv * p.n_mblocks;
   const int sms = std::max(1, a.num_sms);
   p.parts = 1;
@@ -769,7 +814,7 @@ PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws) {
       }
     }
     if (p.parts > 1) p.n_whole = items - cut;
-    p.part_bytes = p.parts > 1 ? (size_t)cut * p.parts * kItemRows * (a.D + 2) * sizeof(float) : 0;
+    p.part_bytes = p.parts > 1 ? (size_t)cut * p.parts * tiles * kBM * (a.D + 2) * sizeof(float) : 0;
   }
   p.n_work = p.n_whole + (items - p.n_whole) * p.parts;
   return p;
@@ -781,6 +826,7 @@ cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTc
   wk.c = c;
   wk.R = a.Sq * a.group;
   wk.M = p.M;
+  wk.tiles = a.D == 256 ? 1 : kTiles;
   wk.n_mblocks = p.n_mblocks;
   const long long kv_unit = std::max<long long>(1, (long long)a.Skv * a.D * 4);
   wk.group_units = (int)std::max<long long>(1, std::min<long long>((long long)a.B * a.Hkv, (64ll << 20) / kv_unit));
@@ -789,7 +835,7 @@ cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTc
   wk.n_work = p.n_work;
   wk.box = std::gcd(c.page_size, kBN);
   wk.part_o = part;
-  wk.part_ml = p.parts > 1 ? part + (size_t)(p.n_work - p.n_whole) * kItemRows * a.D : nullptr;
+  wk.part_ml = p.parts > 1 ? part + (size_t)(p.n_work - p.n_whole) * wk.tiles * kBM * a.D : nullptr;
   wk.stat = stat;
   int grid = p.n_work;
   if (ctr != nullptr && p.n_work > a.num_sms) {
@@ -799,9 +845,7 @@ cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTc
   } else {
     ctr = nullptr;
   }
-  if (a.dtype == LLMX_FP16)
-    return a.D == 64 ? launch_tc_d<__half, 64>(a, wk, grid, ctr, s) : launch_tc_d<__half, 128>(a, wk, grid, ctr, s);
-  return a.D == 64 ? launch_tc_d<__nv_bfloat16, 64>(a, wk, grid, ctr, s) : launch_tc_d<__nv_bfloat16, 128>(a, wk, grid, ctr, s);
+  return a.dtype == LLMX_FP16 ? launch_tc<__half>(a, wk, grid, ctr, s) : launch_tc<__nv_bfloat16>(a, wk, grid, ctr, s);
 }
 
 }  // namespace llmx_b200

@@ -615,21 +615,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Shared memory holds Q and one 64 KB slot each for K and V (plus the ALiBi
 // operands); K and V have their own TMA threads, so a K load never queues
 // behind a V load.
-struct Cfg256 {
-  static constexpr int D = 256;
-  static constexpr int kChunks = D / 64;
-  static constexpr int kChunkBytes = 128 * 128;
-  static constexpr int kTileBytes = 128 * D * 2;
-  static constexpr int kQOff = 0;
-  static constexpr int kKOff = kTileBytes;
-  static constexpr int kVOff = 2 * kTileBytes;
-  static constexpr int kXOff = 3 * kTileBytes;  // A' (8 KB) then B' (8 KB)
-  static constexpr int kXBytes = 8192;
-  static constexpr int kBarOff = kXOff + 2 * kXBytes;
-  static constexpr int kSmemBytes = kBarOff + 1024 + 1024;
-  static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
-  static constexpr uint32_t kTmemS0 = 0, kTmemS1 = 128, kTmemO = 256, kTmemCols = 512;
-};
 constexpr int kThreads256 = 256;  // warps 0-3 softmax, 4 MMA, 5 K + Q loads, 6 V loads, 7 idle
 constexpr int kMmaWarp256 = 4, kKWarp256 = 5, kVWarp256 = 6;
 constexpr int kSchedConsumers256 = 1 + 1 + 4;  // MMA thread, V thread, one lane per softmax warp
@@ -690,76 +675,6 @@ __device__ bool tma_v256(const CUtensorMap *tm_v, uint8_t *smem, Bars256 *bars, 
       tma_load_4d(smem + C::kVOff + c * C::kChunkBytes, tm_v, &bars->v_full, c * 64, t.kvh,
                   block_n0<kReverse>(t.br, j), t.b);
     v_issued = g + 1;
-    if (bars->abort_flag) return false;
-  }
-  return true;
-}
-
-// MMAs of one item: QK(g0), QK(g0 + 1), then per block PV(g), QK(g + 2).
-// Block g's scores live in S_(g & 1); s_full / p_full of a buffer complete
-// once per block that uses it (phase g >> 1), and o_done alike: with one
-// barrier for both, the last wait of an item could find two phases completed,
-// and a wait for the parity of the older one then never returns.
-template <bool kBF16, bool kFold>
-__device__ bool mma_256(uint8_t *smem, Bars256 *bars, uint32_t tmem, int nb, int tile_it, int g0) {
-  using C = Cfg256;
-  constexpr int D = C::D;
-  constexpr uint32_t idesc_qk = idesc_f16(128, kBN, kBF16, false);
-  constexpr uint32_t idesc_pv = idesc_f16(128, D, kBF16, true);
-  const uint32_t q_base = smem_u32(smem + C::kQOff);
-  const uint32_t k_base = smem_u32(smem + C::kKOff);
-  const uint32_t v_base = smem_u32(smem + C::kVOff);
-  const uint32_t x_base = smem_u32(smem + C::kXOff);
-  auto wait = [&](uint64_t *bar, uint32_t par) {
-    return mbar_wait_or_abort(bar, par, kTimeoutNs, &bars->abort_flag);
-  };
-  auto issue_qk = [&](int buf) {
-    const uint32_t d_tmem = tmem + (buf ? C::kTmemS1 : C::kTmemS0);
-    uint64_t da = smem_desc_sw128(q_base, 16, 1024);
-    uint64_t db = smem_desc_sw128(k_base, 16, 1024);
-    asm volatile("" : "+l"(da), "+l"(db));
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      const uint64_t off = (uint64_t)(((kk / 4) * C::kChunkBytes + (kk % 4) * 32) >> 4);
-      mma_ss(d_tmem, da + off, db + off, idesc_qk, kk > 0 ? 1u : 0u);
-    }
-    if constexpr (kFold) {
-      uint64_t dx = smem_desc_noswz(x_base, 128, 256);
-      uint64_t dk = smem_desc_noswz(x_base + C::kXBytes, 128, 256);
-      asm volatile("" : "+l"(dx), "+l"(dk));
-      mma_ss(d_tmem, dx, dk, idesc_qk, 1u);
-    }
-  };
-  auto issue_pv = [&](int buf, bool acc) {
-    const uint32_t d_tmem = tmem + C::kTmemO;
-    const uint32_t p_tmem = tmem + (buf ? C::kTmemS1 : C::kTmemS0);
-    uint64_t db = smem_desc_sw128(v_base, C::kChunkBytes, 1024);
-    asm volatile("" : "+l"(db));
-#pragma unroll
-    for (int kk = 0; kk < kBN / 16; ++kk)
-      mma_ts(d_tmem, p_tmem + kk * 8, db + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv, (acc || kk > 0) ? 1u : 0u);
-  };
-  // QK^T of block g (its K is in the single K slot).
-  auto qk_block = [&](int g, bool last) {
-    if (!wait(&bars->k_full, g & 1)) return false;
-    tc_fence_after();
-    issue_qk(g & 1);
-    tc_commit(&bars->s_full[g & 1]);
-    tc_commit(&bars->k_empty);
-    if (last) tc_commit(&bars->q_empty);
-    return true;
-  };
-  if (!wait(&bars->q_full, tile_it & 1)) return false;
-  if (!qk_block(g0, nb == 1)) return false;
-  if (nb > 1 && !qk_block(g0 + 1, nb == 2)) return false;
-  for (int j = 0; j < nb; ++j) {
-    const int g = g0 + j;
-    if (!wait(&bars->v_full, g & 1) || !wait(&bars->p_full[g & 1], (g >> 1) & 1)) return false;
-    tc_fence_after();
-    issue_pv(g & 1, j > 0);
-    tc_commit(&bars->o_done[g & 1]);
-    tc_commit(&bars->v_empty);
-    if (j + 2 < nb && !qk_block(g + 2, j + 3 == nb)) return false;
     if (bars->abort_flag) return false;
   }
   return true;
@@ -1011,6 +926,8 @@ __global__ void __launch_bounds__(kThreads256, 1)
     }
     if (v_issued > 0) mbar_wait(&bars->v_full, (v_issued - 1) & 1, kTimeoutNs);
   } else if (warp == kMmaWarp256 && lane == 0) {
+    const Mma256Bars mma_bars = {&bars->q_full, &bars->q_empty, &bars->k_full, &bars->k_empty, &bars->v_full, &bars->v_empty,
+                                 bars->s_full,  bars->p_full,   bars->o_done,  &bars->abort_flag};
     int g = 0, it = 0;
     for (int seq = 0;; ++seq) {
       const int w = sched_take(bars, seq, false);
@@ -1021,7 +938,7 @@ __global__ void __launch_bounds__(kThreads256, 1)
       if (w >= n_work) break;
       const Work t = decode_work(a, w, n_mblocks, group_units, kBM);
       if (t.br.nb == 0) continue;
-      const bool ok = mma_256<kBF16, kFold>(smem, bars, tmem, t.br.nb, it, g);
+      const bool ok = mma_256<kBF16, kFold>(smem, mma_bars, tmem, t.br.nb, it, g);
       g += t.br.nb;
       ++it;
       if (!ok) {

@@ -223,6 +223,98 @@ __device__ bool mma_tile(uint8_t *smem, B *bars, uint32_t tmem, int nb, int nb0,
   return true;
 }
 
+// head_dim 256: one tile (attn_sm100.cu describes the scheme).
+struct Cfg256 {
+  static constexpr int D = 256;
+  static constexpr int kChunks = D / 64;
+  static constexpr int kChunkBytes = 128 * 128;
+  static constexpr int kTileBytes = 128 * D * 2;
+  static constexpr int kQOff = 0;
+  static constexpr int kKOff = kTileBytes;
+  static constexpr int kVOff = 2 * kTileBytes;
+  static constexpr int kXOff = 3 * kTileBytes;  // A' (8 KB) then B' (8 KB)
+  static constexpr int kXBytes = 8192;
+  static constexpr int kBarOff = kXOff + 2 * kXBytes;
+  static constexpr int kSmemBytes = kBarOff + 1024 + 1024;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
+  static constexpr uint32_t kTmemS0 = 0, kTmemS1 = 128, kTmemO = 256, kTmemCols = 512;
+};
+
+// MMAs of one item: QK(g0), QK(g0 + 1), then per block PV(g), QK(g + 2).
+// Block g's scores live in S_(g & 1); s_full / p_full of a buffer complete
+// once per block that uses it (phase g >> 1), and o_done alike: with one
+// barrier for both, the last wait of an item could find two phases completed,
+// and a wait for the parity of the older one then never returns.
+struct Mma256Bars {
+  uint64_t *q_full, *q_empty, *k_full, *k_empty, *v_full, *v_empty;
+  uint64_t *s_full, *p_full, *o_done;  // [2] each
+  volatile int *abort_flag;
+};
+template <bool kBF16, bool kFold>
+__device__ bool mma_256(uint8_t *smem, const Mma256Bars &bars, uint32_t tmem, int nb, int tile_it, int g0) {
+  using C = Cfg256;
+  constexpr int D = C::D;
+  constexpr uint32_t idesc_qk = idesc_f16(128, kBN, kBF16, false);
+  constexpr uint32_t idesc_pv = idesc_f16(128, D, kBF16, true);
+  const uint32_t q_base = smem_u32(smem + C::kQOff);
+  const uint32_t k_base = smem_u32(smem + C::kKOff);
+  const uint32_t v_base = smem_u32(smem + C::kVOff);
+  const uint32_t x_base = smem_u32(smem + C::kXOff);
+  auto wait = [&](uint64_t *bar, uint32_t par) {
+    return mbar_wait_or_abort(bar, par, kTimeoutNs, bars.abort_flag);
+  };
+  auto issue_qk = [&](int buf) {
+    const uint32_t d_tmem = tmem + (buf ? C::kTmemS1 : C::kTmemS0);
+    uint64_t da = smem_desc_sw128(q_base, 16, 1024);
+    uint64_t db = smem_desc_sw128(k_base, 16, 1024);
+    asm volatile("" : "+l"(da), "+l"(db));
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint64_t off = (uint64_t)(((kk / 4) * C::kChunkBytes + (kk % 4) * 32) >> 4);
+      mma_ss(d_tmem, da + off, db + off, idesc_qk, kk > 0 ? 1u : 0u);
+    }
+    if constexpr (kFold) {
+      uint64_t dx = smem_desc_noswz(x_base, 128, 256);
+      uint64_t dk = smem_desc_noswz(x_base + C::kXBytes, 128, 256);
+      asm volatile("" : "+l"(dx), "+l"(dk));
+      mma_ss(d_tmem, dx, dk, idesc_qk, 1u);
+    }
+  };
+  auto issue_pv = [&](int buf, bool acc) {
+    const uint32_t d_tmem = tmem + C::kTmemO;
+    const uint32_t p_tmem = tmem + (buf ? C::kTmemS1 : C::kTmemS0);
+    uint64_t db = smem_desc_sw128(v_base, C::kChunkBytes, 1024);
+    asm volatile("" : "+l"(db));
+#pragma unroll
+    for (int kk = 0; kk < kBN / 16; ++kk)
+      mma_ts(d_tmem, p_tmem + kk * 8, db + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv, (acc || kk > 0) ? 1u : 0u);
+  };
+  // QK^T of block g (its K is in the single K slot).
+  auto qk_block = [&](int g, bool last) {
+    if (!wait(bars.k_full, g & 1)) return false;
+    tc_fence_after();
+    issue_qk(g & 1);
+    tc_commit(&bars.s_full[g & 1]);
+    tc_commit(bars.k_empty);
+    if (last) tc_commit(bars.q_empty);
+    return true;
+  };
+  if (!wait(bars.q_full, tile_it & 1)) return false;
+  if (!qk_block(g0, nb == 1)) return false;
+  if (nb > 1 && !qk_block(g0 + 1, nb == 2)) return false;
+  for (int j = 0; j < nb; ++j) {
+    const int g = g0 + j;
+    if (!wait(bars.v_full, g & 1) || !wait(&bars.p_full[g & 1], (g >> 1) & 1)) return false;
+    tc_fence_after();
+    issue_pv(g & 1, j > 0);
+    tc_commit(&bars.o_done[g & 1]);
+    tc_commit(bars.v_empty);
+    if (j + 2 < nb && !qk_block(g + 2, j + 3 == nb)) return false;
+    if (*bars.abort_flag) return false;
+  }
+  return true;
+}
+
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

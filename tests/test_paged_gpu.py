@@ -122,6 +122,9 @@ TC_SHAPES = [
     (128, 4, 4, 48, 257, [700, 257, 128, 0], [257, 200, 1, 0]),
     (64, 16, 8, 64, 33, [5000, 33], None),
     (128, 32, 8, 64, 130, [900] * 5, None),
+    (256, 4, 2, 32, 70, [600, 0, 71, 128], [70, 3, 69, 1]),
+    (256, 5, 1, 16, 60, [300], None),
+    (256, 2, 2, 128, 290, [1000, 290], None),
 ]
 
 
