@@ -43,7 +43,8 @@
 namespace llmx_b200 {
 namespace {
 
-constexpr int kStepRows = 32;  // AUTO: packed rows of a kv head up to which this form is taken
+// AUTO: packed rows of a kv head up to which this form is taken.
+constexpr int step_rows(int D) { return D == 256 ? 128 : 32; }
 constexpr size_t kCounterBytes = 256;
 
 // A launch's units and shares.
@@ -640,7 +641,7 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
             const int b4[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              x[r + e] = kMode == 2 ? tanhf(x[r + e] * cap_in) * cap_out : x[r + e] * scale2;
+              x[r + e] = kMode == 2 ? cap_tanh(x[r + e] * cap_in) * cap_out : x[r + e] * scale2;
               x[r + e] = fmaf(s4[e], (float)(j - b4[e]), x[r + e]);
             }
           } else {
@@ -1133,7 +1134,7 @@ llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs
   const bool can = paged_tc_supports(a);
   if (p->algo == LLMX_ALGO_TCGEN05 && !can)
     return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: TCGEN05 needs sm_scale > 0 and at most 128 query heads a kv head");
-  plan->tc = can && (p->algo == LLMX_ALGO_TCGEN05 || (p->algo == LLMX_ALGO_AUTO && (long long)a.Sq * a.group > kStepRows));
+  plan->tc = can && (p->algo == LLMX_ALGO_TCGEN05 || (p->algo == LLMX_ALGO_AUTO && (long long)a.Sq * a.group > step_rows(a.D)));
   const bool weights = k.w != nullptr;
   const long long R = (long long)a.Sq * a.group;
   if (plan->tc) {

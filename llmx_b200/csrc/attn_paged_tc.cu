@@ -22,8 +22,9 @@
 //  * ALiBi: the folded slope (x_offset) is a row's own, and biases count from
 //    the row's largest one (alibi_ref).
 //  * Work: items (a unit's pair of tiles) longest first over one CTA an SM; the
-//    items of the last, part-filled wave are cut along the keys into `parts`
-//    pieces, whose partial results a second launch merges.
+//    items of the last, part-filled wave (of sequences of different lengths: all
+//    items) are cut along the keys into pieces, whose partial results a second
+//    launch merges.
 #include <algorithm>
 #include <climits>
 #include <numeric>
@@ -51,7 +52,7 @@ struct PCfg<256> : Cfg256 {
   static constexpr int kStages = 1;
   static constexpr uint32_t kTmemO0 = kTmemO, kTmemO1 = kTmemO;
   static constexpr int kThreads = 256;
-  static constexpr int kMma = 4, kLoad = 5, kLoadV = 6;
+  static constexpr int kMma = 4, kLoad = 5;  // 6: V
   static constexpr int kV = 7;  // writes A', then passes V blocks on
   static constexpr int kConsumers = 1 + 4 + 2;
 };
@@ -69,8 +70,9 @@ struct TcWork {
   int tiles;        // of an item
   int n_mblocks;    // items of a unit
   int group_units;  // units whose K / V fit in L2 together
-  int n_whole;      // items [0, n_whole) are whole, the others in `parts` pieces
-  int parts;
+  int n_whole;      // items [0, n_whole) are whole,
+  int piece;        // the others in pieces of so many blocks,
+  int parts;        // at most so many
   int n_work;
   int box;         // tokens of a TMA box
   float *part_o;   // [pieces][128 tiles][D]
@@ -83,6 +85,8 @@ struct Item {
   BlockRange br;
   int nb0;   // blocks that tile 0 takes part in, >= 1
   int slot;  // of its partial result, or -1: whole
+  int pieces;  // of the item
+  bool none;
 };
 
 struct PBars {
@@ -104,13 +108,12 @@ static_assert(sizeof(PBars) <= 1024, "barriers");
 // last rows (which see the most keys) first, as in the dense prefill.
 __device__ __forceinline__ Item decode_item(const AttnArgs &a, const TcWork &wk, int w) {
   Item t;
-  int idx = w, part = 0, parts = 1;
+  int idx = w, part = 0;
   t.slot = -1;
-  if (w >= wk.n_whole && wk.parts > 1) {
-    t.slot = w - wk.n_whole;
-    idx = wk.n_whole + t.slot / wk.parts;
-    part = t.slot % wk.parts;
-    parts = wk.parts;
+  const bool cut = w >= wk.n_whole && wk.parts > 1;
+  if (cut) {
+    idx = wk.n_whole + (w - wk.n_whole) / wk.parts;
+    part = (w - wk.n_whole) % wk.parts;
   }
   const int units = a.B * a.Hkv;
   const int per_group = wk.group_units * wk.n_mblocks;
@@ -131,7 +134,16 @@ __device__ __forceinline__ Item decode_item(const AttnArgs &a, const TcWork &wk,
     const RowsSee s0 = rows_see(a, t.m0, wk.M, t.ql, t.kl);
     nb0 = (max(s0.hi, lo) - lo + kBN - 1) / kBN;
   }
-  const int p0 = (int)((long long)nb * part / parts), p1 = (int)((long long)nb * (part + 1) / parts);
+  int p0 = 0, p1 = nb;
+  if (cut) {
+    t.pieces = (nb + wk.piece - 1) / wk.piece;
+    p0 = min(nb, part * wk.piece);
+    p1 = min(nb, p0 + wk.piece);
+    if (t.pieces > 1) t.slot = w - wk.n_whole;
+  } else {
+    t.pieces = 1;
+  }
+  t.none = part > 0 && p0 == p1;  // the item has fewer pieces
   t.br.n_start = lo + p0 * kBN;
   t.br.nb = p1 - p0;
   t.nb0 = min(t.br.nb, max(min(1, t.br.nb), nb0 - p0));
@@ -335,10 +347,10 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
 #pragma unroll
       for (int q = 0; q < 4; ++q) tmem_st16(tS + q * 16, z);
     } else if (need_mask) {
-      softmax_block<T, kAlibi, kSoftcap, true, kShift>(tS, n0 - ref, 0, lo, hi, scale2, slope2, cap_in, cap_out, m_used, l, alpha,
+      softmax_block<T, kAlibi, kSoftcap, true, kShift, true>(tS, n0 - ref, 0, lo, hi, scale2, slope2, cap_in, cap_out, m_used, l, alpha,
                                                        rescale);
     } else {
-      softmax_block<T, kAlibi, kSoftcap, false, kShift>(tS, n0 - ref, 0, lo, hi, scale2, slope2, cap_in, cap_out, m_used, l, alpha,
+      softmax_block<T, kAlibi, kSoftcap, false, kShift, true>(tS, n0 - ref, 0, lo, hi, scale2, slope2, cap_in, cap_out, m_used, l, alpha,
                                                         rescale);
     }
     if (partly(both, n0)) {
@@ -589,7 +601,18 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
       int w = (int)blockIdx.x;
       for (int seq = 0;; ++seq) {
         Item t{};
-        if (w < wk.n_work) t = decode_item(a, wk, w);
+        auto next = [&] {
+          int n = wk.n_work;
+          if (work_ctr != nullptr) {
+            if (lane == 0) n = (int)gridDim.x + atomicAdd(work_ctr, 1);
+            n = __shfl_sync(0xffffffffu, n, 0);
+          }
+          return n;
+        };
+        for (; w < wk.n_work; w = next()) {
+          t = decode_item(a, wk, w);
+          if (!t.none) break;
+        }
         bool ok = true;
         if (lane == 0) ok = publish(bars, seq, w, t);
         ok = __all_sync(0xffffffffu, ok);
@@ -607,12 +630,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             break;
           }
         }
-        int next = wk.n_work;
-        if (work_ctr != nullptr) {
-          if (lane == 0) next = (int)gridDim.x + atomicAdd(work_ctr, 1);
-          next = __shfl_sync(0xffffffffu, next, 0);
-        }
-        w = next;
+        w = next();
       }
       drain_loads<D>(bars, n);
     } else if (warp == C::kMma) {
@@ -687,23 +705,24 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
   }
 }
 
-// Merges the pieces of the items that were cut: a warp a row, 32 rows a CTA.
+// Merges the pieces of the items that were cut: a warp a row, four rows a CTA.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) paged_tc_merge_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ TcWork wk) {
   constexpr int E = D / 32, kItemRows = PCfg<D>::kItemRows;
   constexpr float kShift = (float)tc_shift<T>();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int cut = blockIdx.x / (kItemRows / 32), first = blockIdx.x % (kItemRows / 32) * 32;
-  const Item t = decode_item(a, wk, wk.n_whole + cut * wk.parts);
+  const int cut = blockIdx.x / (kItemRows / 4), in_item = blockIdx.x % (kItemRows / 4) * 4 + warp;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Item t = decode_item(a, wk, wk.n_whole + cut * wk.parts);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int in_item = first + warp; in_item < first + 32; in_item += 4) {
+  if (t.slot < 0) return;
+  {
     const int tile = in_item / kBM, r = in_item % kBM;
     const int pr = t.m0 + tile * wk.M + r;
-    if (r >= wk.M || pr >= wk.R) continue;
+    if (r >= wk.M || pr >= wk.R) return;
     auto at = [&](int s) { return ((long long)cut * wk.parts + s) * kItemRows + in_item; };
     float m = -CUDART_INF_F;
-    for (int s = lane; s < wk.parts; s += 32) m = fmaxf(m, wk.part_ml[at(s) * 2]);
+    for (int s = lane; s < t.pieces; s += 32) m = fmaxf(m, wk.part_ml[at(s) * 2]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
     const float base = m == -CUDART_INF_F ? 0.f : m;
@@ -711,7 +730,7 @@ __global__ void __launch_bounds__(128) paged_tc_merge_kernel(const __grid_consta
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < wk.parts; ++s) {
+    for (int s = 0; s < t.pieces; ++s) {
       const float2 ml = *reinterpret_cast<const float2 *>(wk.part_ml + at(s) * 2);
       const float w = ex2_approx(ml.x - base);
       const float *po = wk.part_o + at(s) * D + lane * E;
@@ -759,7 +778,7 @@ cudaError_t launch_tc_t(const AttnArgs &a, const TcWork &wk, int grid, int *ctr,
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || wk.parts == 1) return e;
   const int cut = (wk.n_work - wk.n_whole) / wk.parts;
-  return launch_paged_after(paged_tc_merge_kernel<T, D>, dim3(cut * (C::kItemRows / 32)), 128, 0, s, a, wk);
+  return launch_paged_after(paged_tc_merge_kernel<T, D>, dim3(cut * (C::kItemRows / 4)), 128, 0, s, a, wk);
 }
 
 template <typename T, int D>
@@ -798,21 +817,32 @@ PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws) {
   const int sms = std::max(1, a.num_sms);
   p.parts = 1;
   p.n_whole = items;
+  // Blocks of the longest item.
+  long long keys = a.Skv;
+  if (a.window >= 0 && a.causal) keys = std::min<long long>(keys, (long long)a.window + tiles * p.M / a.group + kBN);
+  const int nb = (int)((keys + kBN - 1) / kBN);
+  p.piece = nb;
   if (have_ws) {
-    // The items of the last, part-filled wave, in pieces: waves * (blocks of a
-    // piece + about 3 for its start and end), and for each piece of an item 0.15
-    // for the merge, which reads 128 KB of it.
-    const int cut = items % sms;
-    const int nb = (a.Skv + kBN - 1) / kBN;
+    // In blocks of 128 keys: a piece costs its blocks and about 3 for its start and
+    // end, and 0.15 of an SM's for the merge, which reads 128 KB of it.  Lengths that
+    // only the device knows are taken to be 0.6 of the longest, and the launch to
+    // end half a piece after its mean; of equal ones only the items of the last,
+    // part-filled wave are cut, by the number of waves.
+    const bool ragged = a.B > 1 && a.kv_lens != nullptr;
+    const int cut = ragged ? (items < 4 * sms ? items : 0) : items % sms;
     double best = 1e30;
     for (int s = 1; cut > 0 && s <= std::min(64, std::max(1, nb / 4)); ++s) {
-      const int waves = (int)(((long long)cut * s + sms - 1) / sms);
-      const double cost = waves * ((double)nb / s + 3.0) + (s > 1 ? 3.0 + 0.15 * s * cut / sms : 0.0);
+      const double piece = (double)nb / s + 3.0;
+      const double merge = s > 1 ? 3.0 + 0.15 * s * cut / sms : 0.0;
+      const double mean = (double)cut * (0.6 * nb + 3.0 * (0.4 + 0.6 * s)) / sms;
+      const double cost = merge + (ragged ? std::max(piece, mean + 0.5 * piece)
+                                          : (double)(((long long)cut * s + sms - 1) / sms) * piece);
       if (cost < best) {
         best = cost;
-        p.parts = s;
+        p.piece = (nb + s - 1) / s;
       }
     }
+    p.parts = (nb + p.piece - 1) / p.piece;
     if (p.parts > 1) p.n_whole = items - cut;
     p.part_bytes = p.parts > 1 ? (size_t)cut * p.parts * tiles * kBM * (a.D + 2) * sizeof(float) : 0;
   }
@@ -831,6 +861,7 @@ cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTc
   const long long kv_unit = std::max<long long>(1, (long long)a.Skv * a.D * 4);
   wk.group_units = (int)std::max<long long>(1, std::min<long long>((long long)a.B * a.Hkv, (64ll << 20) / kv_unit));
   wk.n_whole = p.n_whole;
+  wk.piece = p.piece;
   wk.parts = p.parts;
   wk.n_work = p.n_work;
   wk.box = std::gcd(c.page_size, kBN);

@@ -36,7 +36,7 @@ __device__ __forceinline__ int alibi_ref(const Visible &v, float slope) { return
 // launch.  ctr: an int for the work counter, or NULL; stat: nullable
 // [B * Hkv][R], log2 of each packed row's sum of 2^score.
 struct PagedTcPlan {
-  int M, n_mblocks, n_whole, parts, n_work;
+  int M, n_mblocks, n_whole, piece, parts, n_work;
   size_t part_bytes;
 };
 bool paged_tc_supports(const AttnArgs &a);

@@ -27,9 +27,10 @@ template <int D>
 struct WCfg {
   static constexpr int kNT = D == 256 ? 1 : 2;                     // token tiles
   static constexpr int kTile = 128 * D * 2;                        // bytes of a tile
-  static constexpr int kStages = D == 64 ? 4 : (D == 128 ? 3 : 2);  // blocks of rows in the ring
+  static constexpr int kKBufs = D == 256 ? 1 : 2;  // an item's tokens are loaded while the one before is worked on
+  static constexpr int kStages = D == 64 ? 4 : 2;  // blocks of rows in the ring
   static constexpr int kKOff = 0;
-  static constexpr int kQOff = kNT * kTile;
+  static constexpr int kQOff = kKBufs * kNT * kTile;
   static constexpr int kConstOff = kQOff + kStages * kTile;  // [warpgroup][2][128] offsets, then slopes
   static constexpr int kOtherOff = kConstOff + 2 * 2 * 2 * 128 * 4;  // the first warpgroup's sums, at NT = 1
   static constexpr int kBarOff = kOtherOff + 128 * 4;
@@ -38,7 +39,7 @@ struct WCfg {
 };
 
 struct WBars {
-  uint64_t k_full, k_empty;
+  uint64_t k_full[2], k_empty[2];
   uint64_t q_full[4], q_empty[4];
   uint64_t s_full[2][2], s_empty[2][2];  // [warpgroup][accumulator]
   uint64_t c_full[2][2];                 // offsets of a block's columns are written
@@ -99,8 +100,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   WBars *bars = reinterpret_cast<WBars *>(smem + C::kBarOff);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    mbar_init(&bars->k_full, NT);
-    mbar_init(&bars->k_empty, 1);
+    for (int i = 0; i < C::kKBufs; ++i) {
+      mbar_init(&bars->k_full[i], NT);
+      mbar_init(&bars->k_empty[i], 1);
+    }
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&bars->q_full[s], 1);
       mbar_init(&bars->q_empty[s], 1);
@@ -145,10 +148,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         BoxPlace p[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) p[i] = box_place(wk.c, wk.box, t.b, t.kl, t.n0 + i * kBN);
-        if (item > 0) ok = wait_all(&bars->k_empty, (item - 1) & 1);
+        const int kb = item % C::kKBufs;
+        ok = wait_all(&bars->k_empty[kb], ((item / C::kKBufs) & 1) ^ 1);
         if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) load_boxes<D>(smem + C::kKOff + i * C::kTile, &tm_k, &bars->k_full, wk.box, t.kvh, p[i]);
+        for (int i = 0; i < NT; ++i)
+          load_boxes<D>(smem + C::kKOff + (kb * NT + i) * C::kTile, &tm_k, &bars->k_full[kb], wk.box, t.kvh, p[i]);
         ++item;
         for (int q = t.q0; q < t.q1 && ok; ++q, ++block) {
           const int s = block % C::kStages;
@@ -165,7 +170,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) set_abort(bars, a.err);
       // Every load issued lands before the CTA may exit.
-      if (item > 0) mbar_wait(&bars->k_full, (item - 1) & 1, kTimeoutNs);
+      for (int i = max(0, item - C::kKBufs); i < item; ++i)
+        mbar_wait(&bars->k_full[i % C::kKBufs], (i / C::kKBufs) & 1, kTimeoutNs);
       for (int g = max(0, block - C::kStages); g < block; ++g)
         mbar_wait(&bars->q_full[g % C::kStages], (g / C::kStages) & 1, kTimeoutNs);
     } else if (warp == kMmaWarp && lane == 0) {
@@ -175,7 +181,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int w = blockIdx.x; w < wk.n_work && ok; w += gridDim.x) {
         const WItem t = weight_item<NT>(a, wk, w);
         if (t.q1 <= t.q0) continue;
-        ok = wait1(&bars->k_full, item & 1);
+        const int kb = item % C::kKBufs;
+        ok = wait1(&bars->k_full[kb], (item / C::kKBufs) & 1);
         for (int q = t.q0; q < t.q1 && ok; ++q, ++block) {
           const int s = block % C::kStages;
           ok = wait1(&bars->q_full[s], (block / C::kStages) & 1);
@@ -185,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (n[g] >= 2) ok = wait1(&bars->s_empty[g][buf], ((n[g] >> 1) - 1) & 1);
             if (!ok) break;
             tc_fence_after();
-            uint64_t da = smem_desc_sw128(smem_u32(smem + C::kKOff + i * C::kTile), 16, 1024);
+            uint64_t da = smem_desc_sw128(smem_u32(smem + C::kKOff + (kb * NT + i) * C::kTile), 16, 1024);
             uint64_t db = smem_desc_sw128(smem_u32(smem + C::kQOff + s * C::kTile), 16, 1024);
             asm volatile("" : "+l"(da), "+l"(db));
 #pragma unroll
@@ -198,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (ok) tc_commit(&bars->q_empty[s]);
         }
-        if (ok) tc_commit(&bars->k_empty);
+        if (ok) tc_commit(&bars->k_empty[kb]);
         ++item;
       }
       if (!ok) set_abort(bars, a.err);
@@ -213,8 +220,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float cap_in = kSoftcap ? a.sm_scale / a.softcap : 0.f, cap_out = kSoftcap ? a.softcap * kLog2e : 0.f;
     int block = 0, n = 0, handed = 0;
     bool ok = true;
+    // What is added to column tid's score in row block q of item t: -stat, and with
+    // ALiBi slope * (n0 - ref).
+    auto column = [&](const WItem &t, int q, float &add, float &slope2) {
+      const int pr = q * wk.M + tid;
+      add = -CUDART_INF_F;
+      slope2 = 0.f;
+      if (tid < wk.M && pr < t.ql * a.group) {
+        add = -wk.stat[((long long)t.b * a.Hkv + t.kvh) * wk.R + pr];
+        if constexpr (kAlibi) {
+          const int i = pr / a.group;
+          const Visible v = row_visible(a, i, t.ql, t.kl);
+          const float slope = a.alibi[t.kvh * a.group + pr - i * a.group];
+          slope2 = slope * kLog2e;
+          add = fmaf(slope2, (float)(t.n0 + (NT == 2 ? g * kBN : 0) - alibi_ref(v, slope)), add);
+        }
+      }
+    };
+    // This warpgroup's first block of an item that begins with the launch's block
+    // number `at`: all are, or every second one.
+    auto first_of = [&](int at) { return NT == 2 || (at & 1) == g ? 0 : 1; };
+    constexpr int kEvery = NT == 2 ? 1 : 2;
+    WItem next_t = weight_item<NT>(a, wk, min((int)blockIdx.x, wk.n_work - 1));
+    float next_add = 0.f, next_slope = 0.f;
+    if (next_t.q0 + first_of(0) < next_t.q1) column(next_t, next_t.q0 + first_of(0), next_add, next_slope);
     for (int w = blockIdx.x; w < wk.n_work && ok; w += gridDim.x) {
-      const WItem t = weight_item<NT>(a, wk, w);
+      const WItem t = next_t;
+      float add = next_add, slope2 = next_slope;
+      const int blocks = t.q1 - t.q0, first = first_of(block);
+      if (w + (int)gridDim.x < wk.n_work) {  // the next item's first column is read while this one is worked on
+        next_t = weight_item<NT>(a, wk, w + gridDim.x);
+        const int q = next_t.q0 + first_of(block + blocks);
+        if (q < next_t.q1) column(next_t, q, next_add, next_slope);
+      }
       if (t.n0 >= t.kl) continue;
       const int n0 = t.n0 + (NT == 2 ? g * kBN : 0);
       const int j = n0 + tid;
@@ -230,36 +268,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       sees(n0 + kBN - 1, last0, last1);
       const int row_lo = see0 * a.group, row_hi = max(see0, see1) * a.group;  // as packed rows
       const int all_lo = last0 * a.group, all_hi = first1 * a.group;
-      const long long unit = (long long)t.b * a.Hkv + t.kvh;
-      // What is added to column c's score: -stat, and with ALiBi slope * (n0 - ref).
-      auto column = [&](int q, float &add, float &slope2) {
-        const int pr = q * wk.M + tid;
-        add = -CUDART_INF_F;
-        slope2 = 0.f;
-        if (tid < wk.M && pr < t.ql * a.group) {
-          add = -wk.stat[unit * wk.R + pr];
-          if constexpr (kAlibi) {
-            const int i = pr / a.group;
-            const Visible v = row_visible(a, i, t.ql, t.kl);
-            const float slope = a.alibi[t.kvh * a.group + pr - i * a.group];
-            slope2 = slope * kLog2e;
-            add = fmaf(slope2, (float)(n0 - alibi_ref(v, slope)), add);
-          }
-        }
-      };
       uint64_t acc0 = f2(0.f, 0.f), acc1 = f2(0.f, 0.f);
-      float add = 0.f, slope2 = 0.f;
-      // This warpgroup's blocks: all, or every second one of the launch's count.
-      const int blocks = t.q1 - t.q0;
-      const int first = NT == 2 ? 0 : ((block & 1) == g ? 0 : 1);
-      constexpr int kEvery = NT == 2 ? 1 : 2;
-      if (first < blocks) column(t.q0 + first, add, slope2);
       for (int i = first; i < blocks; i += kEvery, ++n) {
         const int q = t.q0 + i;
         const int buf = n & 1;
         cst[buf * 256 + tid] = add;
         if constexpr (kAlibi) cst[buf * 256 + 128 + tid] = slope2;
-        if (i + kEvery < blocks) column(q + kEvery, add, slope2);
+        if (i + kEvery < blocks) column(t, q + kEvery, add, slope2);
         mbar_arrive(&bars->c_full[g][buf]);
         ok = wait_all(&bars->c_full[g][buf], (n >> 1) & 1) && wait_all(&bars->s_full[g][buf], (n >> 1) & 1);
         if (!ok) break;
@@ -299,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               if constexpr (kSoftcap) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = fmaf(tanhf(__uint_as_float(v[ch][c + e]) * cap_in), cap_out, x[e]);
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(cap_tanh(__uint_as_float(v[ch][c + e]) * cap_in), cap_out, x[e]);
               } else {
                 const uint64_t sc = f2(scale2, scale2);
                 f2_split(fma2(f2(__uint_as_float(v[ch][c]), __uint_as_float(v[ch][c + 1])), sc, f2(x[0], x[1])), x[0], x[1]);

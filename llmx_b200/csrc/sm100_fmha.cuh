@@ -321,12 +321,21 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
+// tanh by two special-function instructions: 1 - 2 / (1 + e^2|z|), within 2^-21 of
+// it.  A soft-cap needs absolute accuracy: cap * 2^-21 on a score.
+__device__ __forceinline__ float cap_tanh(float z) {
+  float u;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(u) : "f"(ex2_approx(fabsf(z) * (2.f * kLog2e)) + 1.f));
+  return copysignf(fmaf(-2.f, u, 1.f), z);
+}
+
 // Score of column c (0..127 inside the block) in log2 units, before masking.
-template <bool kAlibi, bool kSoftcap>
+// kFast (the paged cache's kernels): cap_tanh instead of tanhf.
+template <bool kAlibi, bool kSoftcap, bool kFast = false>
 __device__ __forceinline__ float score2(uint32_t raw, int c, float scale2, float slope2, float jf, float cap_in,
                                         float cap_out) {
   const float v = __uint_as_float(raw);
-  float y = kSoftcap ? tanhf(v * cap_in) * cap_out : v * scale2;
+  float y = kSoftcap ? (kFast ? cap_tanh(v * cap_in) : tanhf(v * cap_in)) * cap_out : v * scale2;
   if (kAlibi) y = fmaf(slope2, (float)c, fmaf(slope2, jf, y));
   return y;
 }
@@ -352,7 +361,7 @@ __device__ __forceinline__ void mask_chunk(uint32_t (&v)[32], int c0, int lo, in
 }
 
 // Max of 32 scores (columns c0..c0+31), four independent chains.
-template <bool kAlibi, bool kSoftcap, bool kMask>
+template <bool kAlibi, bool kSoftcap, bool kMask, bool kFast = false>
 __device__ __forceinline__ float chunk_max(const uint32_t (&v)[32], int c0, int lo, int hi, float scale2,
                                            float slope2, float jf, float cap_in, float cap_out) {
   float m[4];
@@ -371,12 +380,12 @@ __device__ __forceinline__ float chunk_max(const uint32_t (&v)[32], int c0, int 
       m[(c >> 1) & 3] = fmax3(m[(c >> 1) & 3], y0, y1);
     }
     const float raw = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-    return raw == -CUDART_INF_F ? raw : score2<false, kSoftcap>(__float_as_uint(raw), 0, scale2, 0.f, 0.f, cap_in, cap_out);
+    return raw == -CUDART_INF_F ? raw : score2<false, kSoftcap, kFast>(__float_as_uint(raw), 0, scale2, 0.f, 0.f, cap_in, cap_out);
   } else {
 #pragma unroll
     for (int c = 0; c < 32; c += 2) {
-      float y0 = score2<kAlibi, kSoftcap>(v[c], c0 + c, scale2, slope2, jf, cap_in, cap_out);
-      float y1 = score2<kAlibi, kSoftcap>(v[c + 1], c0 + c + 1, scale2, slope2, jf, cap_in, cap_out);
+      float y0 = score2<kAlibi, kSoftcap, kFast>(v[c], c0 + c, scale2, slope2, jf, cap_in, cap_out);
+      float y1 = score2<kAlibi, kSoftcap, kFast>(v[c + 1], c0 + c + 1, scale2, slope2, jf, cap_in, cap_out);
       if (kMask) {
         y0 = (c0 + c >= lo && c0 + c < hi) ? y0 : -CUDART_INF_F;
         y1 = (c0 + c + 1 >= lo && c0 + c + 1 < hi) ? y1 : -CUDART_INF_F;
@@ -389,15 +398,15 @@ __device__ __forceinline__ float chunk_max(const uint32_t (&v)[32], int c0, int 
 
 // p = 2^(score - m) for 32 columns, packed in pairs into pk[0..15];
 // returns the sum of the unrounded p (four independent chains).
-template <typename T, bool kAlibi, bool kSoftcap, bool kMask>
+template <typename T, bool kAlibi, bool kSoftcap, bool kMask, bool kFast = false>
 __device__ __forceinline__ float chunk_exp(const uint32_t (&v)[32], uint32_t (&pk)[16], int c0, int lo, int hi,
                                            float scale2, float slope2, float jf, float cap_in, float cap_out,
                                            float m) {
   float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < 32; c += 2) {
-    float y0 = score2<kAlibi, kSoftcap>(v[c], c0 + c, scale2, slope2, jf, cap_in, cap_out);
-    float y1 = score2<kAlibi, kSoftcap>(v[c + 1], c0 + c + 1, scale2, slope2, jf, cap_in, cap_out);
+    float y0 = score2<kAlibi, kSoftcap, kFast>(v[c], c0 + c, scale2, slope2, jf, cap_in, cap_out);
+    float y1 = score2<kAlibi, kSoftcap, kFast>(v[c + 1], c0 + c + 1, scale2, slope2, jf, cap_in, cap_out);
     if (kMask) {
       y0 = (c0 + c >= lo && c0 + c < hi) ? y0 : -CUDART_INF_F;
       y1 = (c0 + c + 1 >= lo && c0 + c + 1 < hi) ? y1 : -CUDART_INF_F;
@@ -458,7 +467,7 @@ __device__ __forceinline__ float chunk_exp_plain2(const uint32_t (&v)[32], uint3
 // pairs, and the running sum.  kMask selects the per-column interval test;
 // the two variants are separate code paths.  kShift: P is taken 2^kShift times
 // as large (and l with it), so that small weights keep fp16's bits.
-template <typename T, bool kAlibi, bool kSoftcap, bool kMask, int kShift = 0>
+template <typename T, bool kAlibi, bool kSoftcap, bool kMask, int kShift = 0, bool kFast = false>
 __device__ __forceinline__ void softmax_block(uint32_t tS, int n0, int kv_offset, int lo, int hi, float scale2,
                                               float slope2,
                                               float cap_in, float cap_out, float &m_used, float &l, float &alpha,
@@ -492,7 +501,7 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, int n0, int kv_offset
   float mx = kNegInf;
 #pragma unroll
   for (int q = 0; q < 4; ++q)
-    mx = fmaxf(mx, chunk_max<kCol, kSoftcap, kMaskPass>(sr[q], q * 32, lo, hi, scale2, sl, jf, cap_in, cap_out));
+    mx = fmaxf(mx, chunk_max<kCol, kSoftcap, kMaskPass, kFast>(sr[q], q * 32, lo, hi, scale2, sl, jf, cap_in, cap_out));
   if constexpr (kFold) mx += off;  // -inf stays -inf
   // Fresh names for the raw scores: pass 2 recomputes each transformed
   // score instead of keeping pass 1's values alive next to the raw row.
@@ -514,7 +523,7 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, int n0, int kv_offset
     if constexpr (!kCol && !kSoftcap)
       psum += chunk_exp_plain2<T>(sr[q], pk, scale2, m_eff - off);
     else
-      psum += chunk_exp<T, kCol, kSoftcap, kMaskPass>(sr[q], pk, q * 32, lo, hi, scale2, sl, jf, cap_in, cap_out,
+      psum += chunk_exp<T, kCol, kSoftcap, kMaskPass, kFast>(sr[q], pk, q * 32, lo, hi, scale2, sl, jf, cap_in, cap_out,
                                                     m_eff - off);
     tmem_st16(tS + q * 16, pk);
   }
