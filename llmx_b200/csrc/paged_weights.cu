@@ -7,13 +7,14 @@
 // accumulator) and sums along its row in registers, so there is no exchange
 // between threads and the sum's order is fixed.  A CTA keeps NT tiles of 128
 // tokens in shared memory and streams the query rows that see them past in
-// blocks of up to 128 packed rows; two warpgroups, each with two accumulators in
-// tensor memory, so that products and exponentials overlap.  At head_dim 64 and
-// 128 each warpgroup has a token tile; at 256, where two tiles and the ring do
-// not fit, both have the same and take blocks of rows in turn.
+// blocks of up to 128 packed rows.  Four warpgroups, each with an accumulator in
+// tensor memory, share a tile's row blocks by turns (two for each of two tiles;
+// at head_dim 256, where two tiles and the ring do not fit, four for one), so
+// that products and exponentials overlap and the special-function units have
+// four warps each to draw on (two left them idle half of the time).
 //
-// Bound by the exponentials: 128 x 128 of them take an SM 1024 cycles on the
-// MUFU (16 a cycle) beside 512 cycles of products at head_dim 128.
+// Bound by the exponentials: 128 x 128 of them take an SM 1024 cycles (16 a
+// cycle) beside 512 cycles of products at head_dim 128.
 #include <algorithm>
 #include <climits>
 #include <numeric>
@@ -23,17 +24,22 @@
 namespace llmx_b200 {
 namespace {
 
+constexpr int kGroups = 4;  // softmax warpgroups
+constexpr int kWThreads = 128 * kGroups + 64;
+constexpr int kWMmaWarp = 4 * kGroups, kWTmaWarp = kWMmaWarp + 1;
+
 template <int D>
 struct WCfg {
-  static constexpr int kNT = D == 256 ? 1 : 2;                     // token tiles
+  static constexpr int kNT = D == 256 ? 1 : 2;      // token tiles
+  static constexpr int kEvery = kGroups / kNT;      // warpgroups of a tile
   static constexpr int kTile = 128 * D * 2;                        // bytes of a tile
   static constexpr int kKBufs = D == 256 ? 1 : 2;  // an item's tokens are loaded while the one before is worked on
   static constexpr int kStages = D == 64 ? 4 : 2;  // blocks of rows in the ring
   static constexpr int kKOff = 0;
   static constexpr int kQOff = kKBufs * kNT * kTile;
   static constexpr int kConstOff = kQOff + kStages * kTile;  // [warpgroup][2][128] offsets, then slopes
-  static constexpr int kOtherOff = kConstOff + 2 * 2 * 2 * 128 * 4;  // the first warpgroup's sums, at NT = 1
-  static constexpr int kBarOff = kOtherOff + 128 * 4;
+  static constexpr int kOtherOff = kConstOff + kGroups * 2 * 2 * 128 * 4;  // [warpgroup][128] sums handed over
+  static constexpr int kBarOff = kOtherOff + kGroups * 128 * 4;
   static constexpr int kSmem = kBarOff + 1024 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
 };
@@ -41,9 +47,9 @@ struct WCfg {
 struct WBars {
   uint64_t k_full[2], k_empty[2];
   uint64_t q_full[4], q_empty[4];
-  uint64_t s_full[2][2], s_empty[2][2];  // [warpgroup][accumulator]
-  uint64_t c_full[2][2];                 // offsets of a block's columns are written
-  uint64_t other_full, other_empty;      // NT = 1: the sums handed over
+  uint64_t s_full[kGroups], s_empty[kGroups];
+  uint64_t c_full[kGroups][2];                       // offsets of a block's columns are written
+  uint64_t other_full[kGroups], other_empty[kGroups];  // sums handed over to a tile's first warpgroup
   uint64_t drain;
   uint32_t tmem_base;
   volatile int abort_flag;
@@ -52,7 +58,7 @@ struct WBars {
 struct WeightWork {
   PagedArgs c;
   int R, M;
-  int tiles;   // items of a unit: ceil(max_kv_len / (128 NT))
+  int units;
   int n_work;
   int box;
   const float *stat;  // [units][R]
@@ -67,12 +73,13 @@ struct WItem {
 template <int NT>
 __device__ __forceinline__ WItem weight_item(const AttnArgs &a, const WeightWork &wk, int w) {
   WItem t;
-  const int unit = w / wk.tiles;
+  // Tiles outside, units inside: CTAs that take every grid-th item get some of each length.
+  const int tile = w / wk.units, unit = w - tile * wk.units;
   t.kvh = unit % a.Hkv;
   t.b = unit / a.Hkv;
   t.ql = clamp_len(a.q_lens, t.b, a.Sq);
   t.kl = clamp_len(a.kv_lens, t.b, a.Skv);
-  t.n0 = (w - unit * wk.tiles) * kBN * NT;
+  t.n0 = tile * kBN * NT;
   t.q0 = t.q1 = 0;
   if (t.n0 < t.kl && t.ql > 0) {
     // Row i sees token j where j <= i + off (causal) and i + off - j <= window.
@@ -89,7 +96,7 @@ __device__ __forceinline__ WItem weight_item(const AttnArgs &a, const WeightWork
 }
 
 template <typename T, int D, bool kAlibi, bool kSoftcap>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kWThreads, 1)
     paged_weight_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ AttnArgs a, const __grid_constant__ WeightWork wk) {
   using C = WCfg<D>;
@@ -108,23 +115,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->q_full[s], 1);
       mbar_init(&bars->q_empty[s], 1);
     }
-    for (int g = 0; g < 2; ++g)
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&bars->s_full[g][i], 1);
-        mbar_init(&bars->s_empty[g][i], 128);
-        mbar_init(&bars->c_full[g][i], 128);
-      }
-    mbar_init(&bars->other_full, 128);
-    mbar_init(&bars->other_empty, 128);
+    for (int g = 0; g < kGroups; ++g) {
+      mbar_init(&bars->s_full[g], 1);
+      mbar_init(&bars->s_empty[g], 128);
+      mbar_init(&bars->c_full[g][0], 128);
+      mbar_init(&bars->c_full[g][1], 128);
+      mbar_init(&bars->other_full[g], 128);
+      mbar_init(&bars->other_empty[g], 128);
+    }
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == kTmaWarp && lane == 0) {
+  if (warp == kWTmaWarp && lane == 0) {
     prefetch_tmap(&tm_q);
     prefetch_tmap(&tm_k);
   }
-  if (warp == kMmaWarp) {
+  if (warp == kWMmaWarp) {
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
@@ -138,8 +145,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait1 = [&](uint64_t *bar, uint32_t par) { return mbar_wait_or_abort(bar, par, kTimeoutNs, &bars->abort_flag); };
   auto wait_all = [&](uint64_t *bar, uint32_t par) { return __all_sync(0xffffffffu, wait1(bar, par)) != 0; };
   // `block` counts the row blocks of all items, `item` the items that have any.
-  if (warp >= 8) {
-    if (warp == kTmaWarp) {
+  if (warp >= 4 * kGroups) {
+    if (warp == kWTmaWarp) {
       int block = 0, item = 0;
       bool ok = true;
       for (int w = blockIdx.x; w < wk.n_work && ok; w += gridDim.x) {
@@ -174,9 +181,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(&bars->k_full[i % C::kKBufs], (i / C::kKBufs) & 1, kTimeoutNs);
       for (int g = max(0, block - C::kStages); g < block; ++g)
         mbar_wait(&bars->q_full[g % C::kStages], (g / C::kStages) & 1, kTimeoutNs);
-    } else if (warp == kMmaWarp && lane == 0) {
+    } else if (warp == kWMmaWarp && lane == 0) {
       constexpr uint32_t idesc = idesc_f16(128, 128, kBF16, false);
-      int block = 0, item = 0, n[2] = {0, 0};  // n: accumulators handed to each warpgroup
+      int block = 0, item = 0;
       bool ok = true;
       for (int w = blockIdx.x; w < wk.n_work && ok; w += gridDim.x) {
         const WItem t = weight_item<NT>(a, wk, w);
@@ -187,9 +194,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int s = block % C::kStages;
           ok = wait1(&bars->q_full[s], (block / C::kStages) & 1);
           for (int i = 0; i < NT && ok; ++i) {
-            const int g = NT == 2 ? i : (block & 1);
-            const int buf = n[g] & 1;
-            if (n[g] >= 2) ok = wait1(&bars->s_empty[g][buf], ((n[g] >> 1) - 1) & 1);
+            const int g = i * C::kEvery + block % C::kEvery, use = block / C::kEvery;
+            ok = wait1(&bars->s_empty[g], (use & 1) ^ 1);
             if (!ok) break;
             tc_fence_after();
             uint64_t da = smem_desc_sw128(smem_u32(smem + C::kKOff + (kb * NT + i) * C::kTile), 16, 1024);
@@ -198,10 +204,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint64_t o = (uint64_t)(((kk / 4) * 128 * 128 + (kk % 4) * 32) >> 4);
-              mma_ss(tmem + (g * 2 + buf) * 128, da + o, db + o, idesc, kk > 0 ? 1u : 0u);
+              mma_ss(tmem + g * 128, da + o, db + o, idesc, kk > 0 ? 1u : 0u);
             }
-            tc_commit(&bars->s_full[g][buf]);
-            ++n[g];
+            tc_commit(&bars->s_full[g]);
           }
           if (ok) tc_commit(&bars->q_empty[s]);
         }
@@ -214,11 +219,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     const int g = warp / 4, tid = threadIdx.x % 128;
+    constexpr int kEvery = C::kEvery;
+    const int tile = g / kEvery, turn = g % kEvery;
     float *const cst = reinterpret_cast<float *>(smem + C::kConstOff) + g * 2 * 256;  // [2][offsets 128, slopes 128]
     const uint32_t lane_off = (uint32_t)((warp % 4) * 32) << 16;
     const float scale2 = a.sm_scale * kLog2e;
     const float cap_in = kSoftcap ? a.sm_scale / a.softcap : 0.f, cap_out = kSoftcap ? a.softcap * kLog2e : 0.f;
-    int block = 0, n = 0, handed = 0;
+    int block = 0, handed = 0;
     bool ok = true;
     // What is added to column tid's score in row block q of item t: -stat, and with
     // ALiBi slope * (n0 - ref).
@@ -233,28 +240,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           const Visible v = row_visible(a, i, t.ql, t.kl);
           const float slope = a.alibi[t.kvh * a.group + pr - i * a.group];
           slope2 = slope * kLog2e;
-          add = fmaf(slope2, (float)(t.n0 + (NT == 2 ? g * kBN : 0) - alibi_ref(v, slope)), add);
+          add = fmaf(slope2, (float)(t.n0 + tile * kBN - alibi_ref(v, slope)), add);
         }
       }
     };
     // This warpgroup's first block of an item that begins with the launch's block
-    // number `at`: all are, or every second one.
-    auto first_of = [&](int at) { return NT == 2 || (at & 1) == g ? 0 : 1; };
-    constexpr int kEvery = NT == 2 ? 1 : 2;
-    WItem next_t = weight_item<NT>(a, wk, min((int)blockIdx.x, wk.n_work - 1));
+    // number `at`: every kEvery-th is its.
+    auto first_of = [&](int at) { return (turn + kEvery - at % kEvery) % kEvery; };
+    // The first column of an item is read while the item before it is worked on.
     float next_add = 0.f, next_slope = 0.f;
-    if (next_t.q0 + first_of(0) < next_t.q1) column(next_t, next_t.q0 + first_of(0), next_add, next_slope);
+    auto first_column = [&](int w, int at) {
+      if (w >= wk.n_work) return;
+      const WItem t = weight_item<NT>(a, wk, w);
+      const int q = t.q0 + first_of(at);
+      if (q < t.q1) column(t, q, next_add, next_slope);
+    };
+    first_column(blockIdx.x, 0);
     for (int w = blockIdx.x; w < wk.n_work && ok; w += gridDim.x) {
-      const WItem t = next_t;
+      const WItem t = weight_item<NT>(a, wk, w);
       float add = next_add, slope2 = next_slope;
       const int blocks = t.q1 - t.q0, first = first_of(block);
-      if (w + (int)gridDim.x < wk.n_work) {  // the next item's first column is read while this one is worked on
-        next_t = weight_item<NT>(a, wk, w + gridDim.x);
-        const int q = next_t.q0 + first_of(block + blocks);
-        if (q < next_t.q1) column(next_t, q, next_add, next_slope);
-      }
+      first_column(w + gridDim.x, block + blocks);
       if (t.n0 >= t.kl) continue;
-      const int n0 = t.n0 + (NT == 2 ? g * kBN : 0);
+      const int n0 = t.n0 + tile * kBN;
       const int j = n0 + tid;
       const int off = t.kl - t.ql;
       // The query rows [see0, see1) that see token j, and those that see every token of the tile.
@@ -269,64 +277,62 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row_lo = see0 * a.group, row_hi = max(see0, see1) * a.group;  // as packed rows
       const int all_lo = last0 * a.group, all_hi = first1 * a.group;
       uint64_t acc0 = f2(0.f, 0.f), acc1 = f2(0.f, 0.f);
-      for (int i = first; i < blocks; i += kEvery, ++n) {
-        const int q = t.q0 + i;
-        const int buf = n & 1;
+      for (int i = first; i < blocks; i += kEvery) {
+        const int q = t.q0 + i, use = (block + i) / kEvery, buf = use & 1;
         cst[buf * 256 + tid] = add;
         if constexpr (kAlibi) cst[buf * 256 + 128 + tid] = slope2;
         if (i + kEvery < blocks) column(t, q + kEvery, add, slope2);
         mbar_arrive(&bars->c_full[g][buf]);
-        ok = wait_all(&bars->c_full[g][buf], (n >> 1) & 1) && wait_all(&bars->s_full[g][buf], (n >> 1) & 1);
+        ok = wait_all(&bars->c_full[g][buf], (use >> 1) & 1) && wait_all(&bars->s_full[g], use & 1);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t tS = tmem + lane_off + (g * 2 + buf) * 128;
+        const uint32_t tS = tmem + lane_off + g * 128;
         const int base = q * wk.M;
         const int lo = min(max(row_lo - base, 0), 128), hi = min(max(row_hi - base, 0), wk.M);
         const bool need_mask = base < all_lo || base + 128 > all_hi || wk.M < 128;
         const float4 *const ca = reinterpret_cast<const float4 *>(cst + buf * 256);
         const float4 *const cs = ca + 32;
         const float kf = (float)tid;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t v[2][32];
-          tmem_ld32(tS + half * 64, v[0]);
-          tmem_ld32(tS + half * 64 + 32, v[1]);
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t vc[32];
+          tmem_ld32(tS + ch * 32, vc);
           tmem_wait_ld();
-          reg_fence32(v[0]);
-          reg_fence32(v[1]);
-          if (half == 1) {
+          reg_fence32(vc);
+          if (ch == 3) {
             tc_fence_before();
-            mbar_arrive(&bars->s_empty[g][buf]);
+            mbar_arrive(&bars->s_empty[g]);
+          }
+          uint32_t seen = 0xffffffffu;
+          if (need_mask) {
+            const int b0 = min(max(lo - ch * 32, 0), 32), b1 = min(max(hi - ch * 32, 0), 32);
+            seen = (b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u) & ~(b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u);
           }
 #pragma unroll
-          for (int ch = 0; ch < 2; ++ch) {
-#pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const int col = half * 64 + ch * 32 + c;
-              const float4 ad = ca[col / 4];
-              float x[4] = {ad.x, ad.y, ad.z, ad.w};
-              if constexpr (kAlibi) {
-                const float4 sl = cs[col / 4];
-                x[0] = fmaf(sl.x, kf, x[0]);
-                x[1] = fmaf(sl.y, kf, x[1]);
-                x[2] = fmaf(sl.z, kf, x[2]);
-                x[3] = fmaf(sl.w, kf, x[3]);
-              }
-              if constexpr (kSoftcap) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = fmaf(cap_tanh(__uint_as_float(v[ch][c + e]) * cap_in), cap_out, x[e]);
-              } else {
-                const uint64_t sc = f2(scale2, scale2);
-                f2_split(fma2(f2(__uint_as_float(v[ch][c]), __uint_as_float(v[ch][c + 1])), sc, f2(x[0], x[1])), x[0], x[1]);
-                f2_split(fma2(f2(__uint_as_float(v[ch][c + 2]), __uint_as_float(v[ch][c + 3])), sc, f2(x[2], x[3])), x[2], x[3]);
-              }
-              if (need_mask) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = (col + e >= lo && col + e < hi) ? x[e] : -CUDART_INF_F;
-              }
-              acc0 = add2(acc0, f2(ex2_approx(x[0]), ex2_approx(x[1])));
-              acc1 = add2(acc1, f2(ex2_approx(x[2]), ex2_approx(x[3])));
+          for (int c = 0; c < 32; c += 4) {
+            const float4 ad = ca[ch * 8 + c / 4];
+            float x[4] = {ad.x, ad.y, ad.z, ad.w};
+            if constexpr (kAlibi) {
+              const float4 sl = cs[ch * 8 + c / 4];
+              x[0] = fmaf(sl.x, kf, x[0]);
+              x[1] = fmaf(sl.y, kf, x[1]);
+              x[2] = fmaf(sl.z, kf, x[2]);
+              x[3] = fmaf(sl.w, kf, x[3]);
             }
+            if constexpr (kSoftcap) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = fmaf(cap_tanh(__uint_as_float(vc[c + e]) * cap_in), cap_out, x[e]);
+            } else {
+              const uint64_t sc = f2(scale2, scale2);
+              f2_split(fma2(f2(__uint_as_float(vc[c]), __uint_as_float(vc[c + 1])), sc, f2(x[0], x[1])), x[0], x[1]);
+              f2_split(fma2(f2(__uint_as_float(vc[c + 2]), __uint_as_float(vc[c + 3])), sc, f2(x[2], x[3])), x[2], x[3]);
+            }
+            if (need_mask) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = (seen & (1u << (c + e))) ? x[e] : -CUDART_INF_F;
+            }
+            acc0 = add2(acc0, f2(ex2_approx(x[0]), ex2_approx(x[1])));
+            acc1 = add2(acc1, f2(ex2_approx(x[2]), ex2_approx(x[3])));
           }
         }
       }
@@ -336,22 +342,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       f2_split(acc0, s0, s1);
       f2_split(acc1, s2, s3);
       float sum = (s0 + s1) + (s2 + s3);
-      if constexpr (NT == 1) {
-        // Both warpgroups have the same tokens: the first one's sums are handed to the second.
+      {
+        // The sums of a tile's other warpgroups are handed to its first one.
         float *const other = reinterpret_cast<float *>(smem + C::kOtherOff);
-        if (g == 0) {
-          if (handed > 0) ok = wait_all(&bars->other_empty, (handed - 1) & 1);
+        const int turn_no = handed++;
+        if (turn != 0) {
+          ok = wait_all(&bars->other_empty[g], (turn_no & 1) ^ 1);
           if (!ok) break;
-          other[tid] = sum;
-          mbar_arrive(&bars->other_full);
-          ++handed;
+          other[g * 128 + tid] = sum;
+          mbar_arrive(&bars->other_full[g]);
           continue;
         }
-        ok = wait_all(&bars->other_full, handed & 1);
+#pragma unroll
+        for (int o = 1; o < kEvery; ++o) {
+          ok = ok && wait_all(&bars->other_full[g + o], turn_no & 1);
+          if (!ok) break;
+          sum += other[(g + o) * 128 + tid];
+          mbar_arrive(&bars->other_empty[g + o]);
+        }
         if (!ok) break;
-        sum = other[tid] + sum;
-        mbar_arrive(&bars->other_empty);
-        ++handed;
       }
       if (j < t.kl) {
         const int page = paged_page(wk.c, t.b, j / wk.c.page_size);
@@ -367,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kWMmaWarp) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -380,8 +389,8 @@ cudaError_t launch_weight_t(const AttnArgs &a, WeightWork wk, cudaStream_t s) {
   using C = WCfg<D>;
   CUtensorMap tq, tk;
   if (!make_q_map(&tq, a, wk.M) || !make_page_map(&tk, wk.c, wk.c.k, wk.c.ks, a.dtype, wk.box)) return cudaErrorInvalidValue;
-  wk.tiles = (a.Skv + kBN * C::kNT - 1) / (kBN * C::kNT);
-  const long long work = (long long)a.B * a.Hkv * wk.tiles;
+  wk.units = a.B * a.Hkv;
+  const long long work = (long long)wk.units * ((a.Skv + kBN * C::kNT - 1) / (kBN * C::kNT));
   if (work > INT_MAX / 2) return cudaErrorInvalidValue;
   wk.n_work = (int)work;
   auto kern = paged_weight_kernel<T, D, kAlibi, kSoftcap>;
@@ -389,7 +398,7 @@ cudaError_t launch_weight_t(const AttnArgs &a, WeightWork wk, cudaStream_t s) {
   static cudaError_t attr = cudaSuccess;
   std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem); });
   if (attr != cudaSuccess) return attr;
-  return launch_paged_after(kern, dim3(std::min(wk.n_work, std::max(1, a.num_sms))), kThreads, C::kSmem, s, tq, tk, a, wk);
+  return launch_paged_after(kern, dim3(std::min(wk.n_work, std::max(1, a.num_sms))), kWThreads, C::kSmem, s, tq, tk, a, wk);
 }
 
 template <typename T, int D>
