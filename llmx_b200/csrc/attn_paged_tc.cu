@@ -182,9 +182,11 @@ struct Loads {
 };
 
 // kWhat: 3 all, 1 Q and K, 2 V.
-template <int D, bool kReverse, int kWhat>
+// `first` is where the lane's box of the first block lies; after() runs once that
+// block's loads are issued.
+template <int D, bool kReverse, int kWhat, typename F>
 __device__ bool load_item(const CUtensorMap *tm_q, const CUtensorMap *tm_k, const CUtensorMap *tm_v, uint8_t *smem, PBars *bars,
-                          const AttnArgs &a, const TcWork &wk, const Item &t, int tile_it, int kv_base, Loads &n) {
+                          const AttnArgs &a, const TcWork &wk, const Item &t, const BoxPlace &first, int tile_it, int kv_base, Loads &n, F after) {
   using C = PCfg<D>;
   const int lane = threadIdx.x % 32;
   auto wait = [&](uint64_t *bar, uint32_t par) {
@@ -202,7 +204,7 @@ __device__ bool load_item(const CUtensorMap *tm_q, const CUtensorMap *tm_k, cons
     n.q[q] = tile_it + 1;
     return true;
   };
-  BoxPlace next = box_place(wk.c, wk.box, t.b, t.kl, block_n0<kReverse>(t.br, 0));
+  BoxPlace next = first;
   if ((kWhat & 1) && !load_q(0)) return false;
   for (int j = 0; j < t.br.nb; ++j) {
     const int g = kv_base + j;
@@ -221,6 +223,7 @@ __device__ bool load_item(const CUtensorMap *tm_q, const CUtensorMap *tm_k, cons
       load_boxes<D>(smem + C::kVOff + s * C::kTileBytes, tm_v, &bars->v_landed[s], wk.box, t.kvh, p);
       n.v = g + 1;
     }
+    if (j == 0) after();
   }
   return true;
 }
@@ -238,49 +241,60 @@ __device__ void drain_loads(PBars *bars, const Loads &n) {
 }
 
 // ------------------------------------------------------------------ V warp
-// Lane l has rows l, l + 32, .. of the block.  16-byte chunk c of row r lies at
-// chunk c ^ (r % 8) of its 128 bytes, so lanes that take the same c do not meet
-// in a bank.
+// Lane l has rows l, l + 32, .. of the block at n0.  16-byte chunk c of row r
+// lies at chunk c ^ (r % 8) of its 128 bytes, so lanes that take the same c do
+// not meet in a bank.  Tokens that no row of the item sees become zeros; of
+// those that only some see, infinities and NaN do; the others stay.
+template <typename T>
+__device__ __forceinline__ uint32_t fma_zero(uint32_t x, uint32_t acc) {  // acc + 0 * x: NaN from an infinity or NaN on
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&x), __float2half2_rn(0.f), *reinterpret_cast<const __half2 *>(&acc));
+    return *reinterpret_cast<const uint32_t *>(&r);
+  } else {
+    const __nv_bfloat162 r =
+        __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&x), __float2bfloat162_rn(0.f), *reinterpret_cast<const __nv_bfloat162 *>(&acc));
+    return *reinterpret_cast<const uint32_t *>(&r);
+  }
+}
 template <typename T, int D>
-__device__ void clean_block(uint8_t *v, uint32_t (&lost)[4], int rows) {
+__device__ void clean_block(uint8_t *v, uint32_t (&lost)[4], const RowsSee &see, int n0) {
   using C = PCfg<D>;
-  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   const int lane = threadIdx.x % 32;
 #pragma unroll 1
   for (int i = 0; i < 4; ++i) {
-    const int r = i * 32 + lane;
+    const int r = i * 32 + lane, j = n0 + r;
     bool bad = false;
-    uint8_t *row = v + r * 128;
-    if (r >= rows) {
-      for (int c = 0; c < C::kChunks; ++c)
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          *reinterpret_cast<uint4 *>(row + c * C::kChunkBytes + ((k ^ (r & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
-    } else {
-      for (int c = 0; c < C::kChunks; ++c)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          uint4 *at = reinterpret_cast<uint4 *>(row + c * C::kChunkBytes + ((k ^ (r & 7)) << 4));
-          const uint4 x = *at;
+    uint8_t *const row = v + r * 128;
+    auto at = [&](int p) { return reinterpret_cast<uint4 *>(row + p / 8 * C::kChunkBytes + (((p % 8) ^ (r & 7)) << 4)); };
+    if (j < see.lo || j >= see.hi) {
+#pragma unroll 8
+      for (int p = 0; p < D / 8; ++p) *at(p) = make_uint4(0u, 0u, 0u, 0u);
+    } else if (j < see.all_lo || j >= see.all_hi) {
+      uint32_t acc[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 8
+      for (int p = 0; p < D / 8; ++p) {
+        const uint4 x = *at(p);
+        acc[0] = fma_zero<T>(x.x, acc[0]);
+        acc[1] = fma_zero<T>(x.y, acc[1]);
+        acc[2] = fma_zero<T>(x.z, acc[2]);
+        acc[3] = fma_zero<T>(x.w, acc[3]);
+      }
+      const uint32_t any = acc[0] | acc[1] | acc[2] | acc[3];  // NaN in one of them sets all exponent bits
+      bad = (any & kExp) == kExp || ((any >> 16) & kExp) == kExp;
+      if (bad) {
+#pragma unroll 1
+        for (int p = 0; p < D / 8; ++p) {
+          const uint4 x = *at(p);
           uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          bool any = false;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t m = (w[e] & kExp) ^ kExp;  // a half that is 0: all exponent bits set
-            if ((m & 0xffffu) == 0u) {
-              w[e] &= 0xffff0000u;
-              any = true;
-            }
-            if ((m >> 16) == 0u) {
-              w[e] &= 0x0000ffffu;
-              any = true;
-            }
+            if ((w[e] & kExp) == kExp) w[e] &= 0xffff0000u;
+            if (((w[e] >> 16) & kExp) == kExp) w[e] &= 0x0000ffffu;
           }
-          if (any) {
-            *at = make_uint4(w[0], w[1], w[2], w[3]);
-            bad = true;
-          }
+          *at(p) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+      }
     }
     const uint32_t bits = __ballot_sync(0xffffffffu, bad);
     if (lane == 0) lost[i] = bits;
@@ -587,7 +601,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
       const bool ok = mbar_wait_or_abort(&bars->v_landed[s], (g / C::kStages) & 1, kTimeoutNs, &bars->abort_flag);
       if (!__all_sync(0xffffffffu, ok)) return false;
       const int n0 = block_n0<kAlibi>(t.br, j);
-      if (partly(both, n0)) clean_block<T, D>(smem + C::kVOff + s * C::kTileBytes, bars->lost[s], t.kl - n0);
+      if (partly(both, n0)) clean_block<T, D>(smem + C::kVOff + s * C::kTileBytes, bars->lost[s], both, n0);
       if (lane == 0) mbar_arrive(&bars->v_full[s]);
     }
     return true;
@@ -596,42 +610,55 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
   if (warp >= kSoftmaxWarps) {
     if constexpr (!C::kOne) regs_decrease<kRegsControl>();
     if (warp == C::kLoad) {
+      // The item after the one that is loaded is fetched, published and its first
+      // pages looked up while that one's loads run.
       Loads n;
-      int kv = 0, it = 0;
-      int w = (int)blockIdx.x;
-      for (int seq = 0;; ++seq) {
-        Item t{};
-        auto next = [&] {
-          int n = wk.n_work;
-          if (work_ctr != nullptr) {
-            if (lane == 0) n = (int)gridDim.x + atomicAdd(work_ctr, 1);
-            n = __shfl_sync(0xffffffffu, n, 0);
-          }
-          return n;
-        };
-        for (; w < wk.n_work; w = next()) {
+      int kv = 0, it = 0, seq = 0, w = 0;
+      Item t{};
+      BoxPlace first{0, 0};
+      bool ok = true;
+      auto fetch = [&](int from) {  // the item of ticket `from`, or of the first one after it that has work
+        for (w = from; w < wk.n_work;) {
           t = decode_item(a, wk, w);
           if (!t.none) break;
-        }
-        bool ok = true;
-        if (lane == 0) ok = publish(bars, seq, w, t);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          set_abort(bars, a.err);
-          break;
-        }
-        if (w >= wk.n_work) break;
-        if (t.br.nb > 0) {
-          ok = load_item<D, kAlibi, C::kOne ? 1 : 3>(&tm_q, &tm_k, &tm_v, smem, bars, a, wk, t, it, kv, n);
-          kv += t.br.nb;
-          ++it;
-          if (!ok) {
-            set_abort(bars, a.err);
-            break;
+          w = wk.n_work;
+          if (work_ctr != nullptr) {
+            if (lane == 0) w = (int)gridDim.x + atomicAdd(work_ctr, 1);
+            w = __shfl_sync(0xffffffffu, w, 0);
           }
         }
-        w = next();
+        bool done = true;
+        if (lane == 0) done = publish(bars, seq, w, t);
+        ok = __all_sync(0xffffffffu, done) != 0;
+        ++seq;
+        if (w < wk.n_work && t.br.nb > 0) first = box_place(wk.c, wk.box, t.b, t.kl, block_n0<kAlibi>(t.br, 0));
+      };
+      auto ticket = [&] {
+        int x = wk.n_work;
+        if (work_ctr != nullptr) {
+          if (lane == 0) x = (int)gridDim.x + atomicAdd(work_ctr, 1);
+          x = __shfl_sync(0xffffffffu, x, 0);
+        }
+        return x;
+      };
+      fetch((int)blockIdx.x);
+      while (ok && w < wk.n_work) {
+        const Item now = t;
+        const BoxPlace now_first = first;
+        if (now.br.nb == 0) {
+          fetch(ticket());
+          continue;
+        }
+        bool fetched = true;
+        const bool done = load_item<D, kAlibi, C::kOne ? 1 : 3>(&tm_q, &tm_k, &tm_v, smem, bars, a, wk, now, now_first, it, kv, n, [&] {
+          fetch(ticket());
+          fetched = ok;
+        });
+        kv += now.br.nb;
+        ++it;
+        ok = done && fetched;
       }
+      if (!ok) set_abort(bars, a.err);
       drain_loads<D>(bars, n);
     } else if (warp == C::kMma) {
       if (lane == 0) {
@@ -672,7 +699,8 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         int kv = 0;
         each_item(true, [&](const Item &t) {
           if (t.br.nb == 0) return true;
-          const bool ok = load_item<D, kAlibi, 2>(&tm_q, &tm_k, &tm_v, smem, bars, a, wk, t, 0, kv, n);
+          const BoxPlace first = box_place(wk.c, wk.box, t.b, t.kl, block_n0<kAlibi>(t.br, 0));
+          const bool ok = load_item<D, kAlibi, 2>(&tm_q, &tm_k, &tm_v, smem, bars, a, wk, t, first, 0, kv, n, [] {});
           kv += t.br.nb;
           return ok;
         });
