@@ -403,10 +403,12 @@ LLMX_API llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv4_
  * aligned).  Any max_q_len: one new token a sequence, a few, or a chunk of a
  * prompt; a sequence's query rows are its last q_len tokens under the causal
  * mask.  p->algo:
- *   DECODE  streams K and V once for every 16, 32 or 64 (query row, head)
- *           pairs of a kv head, split over the machine.
- *   TCGEN05 tensor-core tiles of 128 such pairs; sm_scale > 0.
- *   AUTO    DECODE up to 64 pairs, TCGEN05 above where it can run.
+ *   DECODE  streams K and V once for every 16 or 32 (head_dim 256: or 64)
+ *           (query row, head) pairs of a kv head, split over the machine.
+ *   TCGEN05 tiles of 128 such pairs; sm_scale > 0, at most 128 query heads a
+ *           kv head.
+ *   AUTO    DECODE up to 32 pairs (head_dim 256: 128), TCGEN05 above where it
+ *           can run.
  * ALiBi's biases count from each row's largest one, so that they keep their
  * bits far into a sequence; lse is that of slope * position.  A NaN or an
  * infinity in a cached token reaches the rows that see the token and no
@@ -417,7 +419,8 @@ LLMX_API llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv4_
  *                              the query heads of the kv head,
  * where what was there counts as 0 for the call's own tokens (causal: the
  * last q_lens[b] ones), and for all where decay is 0 (it is not read then).
- * decay must be finite and >= 0.
+ * decay must be finite and >= 0.  o must then not overlap q, and sequences that
+ * share a page leave either's weights there.
  *   A call given too little workspace for its partial results runs without
  * splitting sequences; with key_weights it is refused
  * (LLMX_ERR_WORKSPACE_TOO_SMALL).  Calls that share a workspace must not

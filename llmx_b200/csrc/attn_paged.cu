@@ -35,7 +35,6 @@
 #include <climits>
 #include <cstdio>
 #include <cstring>
-#include <mutex>
 #include <numeric>
 
 #include "paged_tc.cuh"
@@ -384,7 +383,7 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (tid == 0) {
+  if (warp == C::kTmaWarp && lane == 0) {  // which then needs no one to start copying
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&bars->full[i], 1);
       mbar_init(&bars->empty[i], 1);
@@ -398,8 +397,6 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
     fence_mbar_init();
-  }
-  if (warp == C::kTmaWarp && lane == 0) {
     prefetch_tmap(&tm_k);
     prefetch_tmap(&tm_v);
   }
@@ -440,20 +437,21 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
     cur.at = 0;
     cur.left = cur.sp.steps();
   }
-  if (warp == C::kMmaWarp) {
-    tmem_alloc(&bars->tmem_base, C::kTmem);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  // Each role meets the others when it has its first loads under way.
+  uint32_t tmem = 0;
+  auto meet = [&] {
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    tmem = bars->tmem_base;
+  };
   auto wait = [&](uint64_t *bar, uint32_t par) { return mbar_wait_or_abort(bar, par, kTimeoutNs, &bars->abort_flag); };
 
   if (warp == C::kTmaWarp) {
     // ---- copies, in the order K 0, K 1, V 0, K 2, V 1, ..
     int g = 0;  // slots filled
     bool ok = true;
+    __syncwarp();  // the barriers are set up
     auto copy = [&](const CUtensorMap *tm, const BoxPlace &p) {
       for (int half = 0; half < H && ok; ++half, ++g) {
         const int s = g % C::kSlots;
@@ -467,6 +465,7 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
                         cur.kvh, p.page);
       }
     };
+    bool met = false;
     do {
       const int b0 = cur.first(), b1 = cur.last();
       BoxPlace kp, vp;
@@ -475,6 +474,8 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
         vp = kp;
         copy(&tm_k, kp);
       }
+      if (!met) meet();
+      met = true;
       for (int j = b0; j < b1 && ok; ++j) {
         if (j + 1 < b1) {
           kp = box_place(wk.c, wk.box, cur.b, cur.sp.kl, cur.sp.token(j + 1, wk.reverse));
@@ -488,6 +489,9 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
     // Every copy issued lands before the CTA may exit.
     for (int i = max(0, g - C::kSlots); i < g; ++i) mbar_wait(&bars->full[i % C::kSlots], (i / C::kSlots) & 1, kTimeoutNs);
   } else if (warp == C::kMmaWarp) {
+    tmem_alloc(&bars->tmem_base, C::kTmem);
+    tmem_relinquish();
+    meet();
     if (lane == 0) {
       // ---- products: S^T(j + 1) is issued before O^T += .. (j)
       constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -582,6 +586,7 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
       }
     };
     if (kAhead) read_q(cur);
+    meet();
     for (bool more = true; more;) {
       Cursor nx = cur;
       const bool none = cur.none();
@@ -1014,10 +1019,8 @@ cudaError_t launch_step_t(const AttnArgs &a, const StepWork &wk, long long units
   CUtensorMap tk, tv;
   if (!make_page_map(&tk, wk.c, wk.c.k, wk.c.ks, a.dtype, wk.box) || !make_page_map(&tv, wk.c, wk.c.v, wk.c.vs, a.dtype, wk.box))
     return cudaErrorInvalidValue;
-  auto kern = paged_step_kernel<T, D, N, kMode>;
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem); });
+  constexpr auto kern = paged_step_kernel<T, D, N, kMode>;
+  const cudaError_t attr = allow_smem<kern>(C::kSmem);
   if (attr != cudaSuccess) return attr;
   const unsigned grid = (unsigned)(wk.split ? wk.workers : units);
   kern<<<grid, C::kThreads, C::kSmem, s>>>(tk, tv, a, wk);
@@ -1098,6 +1101,7 @@ llmx_status prepare(const llmx_attn_params *p, const llmx_paged_cache *c, AttnAr
     return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: q and o must be 16-byte aligned");
   const int extent[3] = {a->B, a->Sq, a->H};
   for (int i = 0; i < 3; ++i) {
+    if (extent[i] == 1) a->qs[i] = a->os[i] = 0;  // never stepped along
     if (a->qs[i] % 8 || a->os[i] % 8)
       return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: strides of q and o must be multiples of 8");
     if (extent[i] > 1 && a->os[i] == 0) return bad("paged attention: rows of o must not overlap (stride 0)");
@@ -1144,7 +1148,7 @@ llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs
     plan->bytes = plan->stat_at + (weights ? (size_t)a.B * a.Hkv * R * sizeof(float) : 0);
   } else {
     plan->step = plan_step(a, weights, weights);
-    plan->again = weights && (R > kScoreRows || plan->step.score_bytes > kScoreBytes) && a.sm_scale > 0.f && paged_weights_supports(a);
+    plan->again = weights && (R > kScoreRows || plan->step.score_bytes > kScoreBytes) && paged_weights_supports(a);
     if (plan->again) plan->step.score_bytes = 0;
     plan->stat_at = plan->step.part_bytes;
     plan->bytes = plan->step.part_bytes + plan->step.stat_bytes + plan->step.score_bytes;
@@ -1178,6 +1182,7 @@ extern "C" llmx_status llmx_paged_attn_fwd(const llmx_attn_params *p, const llmx
   llmx_status s = prepare(p, c, &a, &k);
   if (s != LLMX_OK) return s;
   if (k.w != nullptr && !(decay >= 0.f && decay <= 3.4e38f)) return bad("paged attention: decay must be finite and >= 0");
+  if (k.w != nullptr && p->q == p->o) return bad("paged attention: with key_weights o must not be q, which is read again");
   if (reinterpret_cast<uintptr_t>(p->workspace) & 15u) return bad("paged attention: workspace must be 16-byte aligned");
   Plan plan;
   s = choose(p, a, k, &plan);

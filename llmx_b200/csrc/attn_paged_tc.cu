@@ -797,10 +797,8 @@ cudaError_t launch_tc_t(const AttnArgs &a, const TcWork &wk, int grid, int *ctr,
   if (!make_q_map(&tq, a, wk.M) || !make_page_map(&tk, wk.c, wk.c.k, wk.c.ks, a.dtype, wk.box) ||
       !make_page_map(&tv, wk.c, wk.c.v, wk.c.vs, a.dtype, wk.box))
     return cudaErrorInvalidValue;
-  auto kern = paged_tc_kernel<T, D, kAlibi, kSoftcap>;
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes); });
+  constexpr auto kern = paged_tc_kernel<T, D, kAlibi, kSoftcap>;
+  const cudaError_t attr = allow_smem<kern>(C::kSmemBytes);
   if (attr != cudaSuccess) return attr;
   kern<<<grid, C::kThreads, C::kSmemBytes, s>>>(tq, tk, tv, a, wk, ctr);
   cudaError_t e = cudaGetLastError();

@@ -6,6 +6,8 @@
 // V are read once for all of them.
 #pragma once
 
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace llmx_b200 {
@@ -48,6 +50,20 @@ cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTc
 // attention that wrote them.
 bool paged_weights_supports(const AttnArgs &a);
 cudaError_t launch_paged_weights(const AttnArgs &a, const PagedArgs &c, const float *stat, float decay, cudaStream_t s);
+
+// Allows a kernel `bytes` of dynamic shared memory on the current device, once a
+// device (the attribute belongs to the device that is current).  The
+// flags are one for each kernel: the template's argument is the kernel itself.
+template <auto kKernel>
+cudaError_t allow_smem(size_t bytes) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev].load())) return e;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true);
+  return e;
+}
 
 // A launch that may be set up while the kernel before it still runs (it waits
 // for that kernel itself).

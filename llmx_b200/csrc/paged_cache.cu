@@ -14,9 +14,8 @@
 
 #include <algorithm>
 #include <climits>
-#include <mutex>
 
-#include "paged.cuh"
+#include "paged_attn.cuh"
 
 namespace llmx_b200 {
 namespace {
@@ -525,12 +524,7 @@ cudaError_t launch_evict(const PagedArgs &a, const EvictArgs &e, int num_sms, cu
   const int per = ((e.max_kv + ranks - 1) / ranks + 3) & ~3;
   const size_t smem = (size_t)std::min(per, kSelHeld) * 4;
   if (units * ranks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [] {
-    for (auto kern : {evict_select_kernel<512>, evict_select_kernel<1024>})
-      if (attr == cudaSuccess) attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelHeld * 4);
-  });
+  const cudaError_t attr = ranks > 1 ? allow_smem<evict_select_kernel<1024>>(kSelHeld * 4) : allow_smem<evict_select_kernel<512>>(kSelHeld * 4);
   if (attr != cudaSuccess) return attr;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * ranks));
@@ -596,8 +590,8 @@ llmx_status validate_paged(const llmx_paged_cache *c, int batch, PagedArgs *k) {
   const long long extent[3] = {c->n_pages, c->n_kv_heads, c->page_size};
   long long ks[3], vs[3];
   for (int i = 0; i < 3; ++i) {
-    ks[i] = c->k_stride[i];
-    vs[i] = c->v_stride[i];
+    ks[i] = extent[i] > 1 ? c->k_stride[i] : 0;  // an extent of 1 is never stepped along
+    vs[i] = extent[i] > 1 ? c->v_stride[i] : 0;
     // Every offset stays below 2^60 elements.
     const long long most = (1LL << 58) / extent[i];
     if (ks[i] < 0 || ks[i] % 8 || ks[i] > most || vs[i] < 0 || vs[i] % 8 || vs[i] > most)
@@ -609,7 +603,7 @@ llmx_status validate_paged(const llmx_paged_cache *c, int batch, PagedArgs *k) {
   if (c->block_table == nullptr && (long long)batch * c->max_pages > c->n_pages)
     return bad("paged: without a block table the cache must hold batch * max_pages pages");
   if (c->key_weights != nullptr) {
-    const long long ws[2] = {c->w_stride[0], c->w_stride[1]};
+    const long long ws[2] = {extent[0] > 1 ? c->w_stride[0] : 0, extent[1] > 1 ? c->w_stride[1] : 0};
     if (!al16(c->key_weights)) return bad("paged: key_weights must be 16-byte aligned");
     for (int i = 0; i < 2; ++i)
       if (ws[i] < 0 || ws[i] % 4 || ws[i] > (1LL << 58) / extent[i])
@@ -625,8 +619,8 @@ llmx_status validate_paged(const llmx_paged_cache *c, int batch, PagedArgs *k) {
   k->table = c->block_table;
   k->table_stride = c->table_stride;
   k->w = c->key_weights;
-  k->ws[0] = c->w_stride[0];
-  k->ws[1] = c->w_stride[1];
+  k->ws[0] = extent[0] > 1 ? c->w_stride[0] : 0;
+  k->ws[1] = extent[1] > 1 ? c->w_stride[1] : 0;
   k->n_pages = c->n_pages;
   k->max_pages = c->max_pages;
   k->page_size = c->page_size;
@@ -651,8 +645,9 @@ extern "C" llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv
   StoreArgs r;
   bool vec = al16(rows->k) && al16(rows->v);
   for (int i = 0; i < 3; ++i) {
-    r.ks[i] = rows->k_stride[i];
-    r.vs[i] = rows->v_stride[i];
+    const long long extent = i == 0 ? rows->batch : (i == 1 ? rows->max_rows : k.Hkv);
+    r.ks[i] = extent > 1 ? rows->k_stride[i] : 0;
+    r.vs[i] = extent > 1 ? rows->v_stride[i] : 0;
     if (r.ks[i] < 0 || r.vs[i] < 0) return bad("paged: strides must be >= 0");
     vec = vec && r.ks[i] % 8 == 0 && r.vs[i] % 8 == 0;
   }

@@ -393,10 +393,8 @@ cudaError_t launch_weight_t(const AttnArgs &a, WeightWork wk, cudaStream_t s) {
   const long long work = (long long)wk.units * ((a.Skv + kBN * C::kNT - 1) / (kBN * C::kNT));
   if (work > INT_MAX / 2) return cudaErrorInvalidValue;
   wk.n_work = (int)work;
-  auto kern = paged_weight_kernel<T, D, kAlibi, kSoftcap>;
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem); });
+  constexpr auto kern = paged_weight_kernel<T, D, kAlibi, kSoftcap>;
+  const cudaError_t attr = allow_smem<kern>(C::kSmem);
   if (attr != cudaSuccess) return attr;
   return launch_paged_after(kern, dim3(std::min(wk.n_work, std::max(1, a.num_sms))), kWThreads, C::kSmem, s, tq, tk, a, wk);
 }

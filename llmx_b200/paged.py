@@ -145,8 +145,9 @@ def paged_attention(output: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor
 
     ``max_kv_len`` (0: all the table can hold) bounds kv_lens where the caller
     knows a bound: the work is split by it.  ``algo``: "decode" streams the cache
-    once for up to 64 (row, head) pairs of a kv head, "tcgen05" takes tiles of
-    128 on the tensor cores, "auto" chooses by the pairs."""
+    once for every 16 to 64 (row, head) pairs of a kv head, "tcgen05" takes tiles
+    of 128, "auto" chooses by the pairs.  ``output`` must not overlap the cache,
+    and with ``key_weights`` not q."""
     ext = ops._extension()
     call = ext.paged_attention if ext is not None else paged_attention_ctypes
     call(output, q, k_cache, v_cache, float(sm_scale), int(sliding_window), float(logits_soft_cap), kv_lens=kv_lens,

@@ -98,7 +98,7 @@ def test_bad_caches_are_refused_by_every_entry_point(over, status, text):
     (dict(n_kv_heads=4), 1, "cache's"), (dict(dtype=1), 1, "cache's"), (dict(head_dim=64), 1, "cache's"),
     (dict(kv_offset=1), 1, "kv_offset"), (dict(kv_total=9), 1, "kv_offset"), (dict(max_kv_len=257), 1, "max_kv_len"),
     (dict(algo=1), 2, "algo"), (dict(algo=7), 1, "algo"), (dict(q=0x40008), 2, "aligned"), (dict(o=0x50002), 2, "aligned"),
-    (dict(q_stride=[1024, 1028, 128]), 2, "multiples of 8"), (dict(o_stride=[0, 1024, 128]), 1, "overlap"),
+    (dict(q_stride=[1024, 1024, 132]), 2, "multiples of 8"), (dict(o_stride=[0, 1024, 128]), 1, "overlap"),
     (dict(o_stride=[1024, 1024, 0]), 1, "overlap"), (dict(max_q_len=1 << 29), 1, "2^30"), (dict(q=0), 1, "NULL"),
     (dict(sm_scale=float("inf")), 1, "sm_scale"), (dict(workspace=0xc0008, workspace_bytes=16), 1, "workspace"),
     (dict(algo=3, sm_scale=-1.0), 2, "sm_scale"),
@@ -128,6 +128,12 @@ def test_bad_decay_is_refused(decay):
     p, c = request(), cache(key_weights=0xb0000, w_stride=[128, 64])
     assert _lib.load().llmx_paged_attn_fwd(ctypes.byref(p), ctypes.byref(c), decay, None) == 1
     assert "decay" in message()
+
+
+def test_output_over_q_is_refused_with_weights():
+    p, c = request(o=0x40000), cache(key_weights=0xb0000, w_stride=[128, 64])
+    assert _lib.load().llmx_paged_attn_fwd(ctypes.byref(p), ctypes.byref(c), 1.0, None) == 1
+    assert "read again" in message()
 
 
 @pytest.mark.parametrize("over", [dict(batch=-1), dict(max_rows=-1), dict(k=0), dict(v=0)])

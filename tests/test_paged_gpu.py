@@ -281,6 +281,87 @@ def test_pages_outside_the_cache_read_as_zeros():
     llmx_b200.device_status(0)
 
 
+@pytest.mark.parametrize("algo", ["decode", "tcgen05"])
+def test_pages_outside_the_cache_in_each_form(algo):
+    c = Case(torch.float16, 128, 4, 2, 32, 30, [200, 90])
+    c.table[0, 2], c.table[1, 0] = 2 ** 31 - 1, -5
+    c.k[0][64:96] = 0
+    c.v[0][64:96] = 0
+    c.k[1][:32] = 0
+    c.v[1][:32] = 0
+    w = torch.zeros(c.k_cache.shape[:3], device=DEV)
+    out, lse = c.run(algo=algo, weights=w)
+    with pytest.raises(LlmxError):
+        llmx_b200.device_status(0)
+    for b in range(2):
+        check_attention(out[b], lse[b], None, c.want(b), c.dtype)
+    llmx_b200.device_status(0)
+
+
+@pytest.mark.parametrize("algo", ["decode", "tcgen05"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_garbage_in_padded_rows_stays_there(d, algo):
+    """Rows at or past q_lens hold NaN: they are written as 0 and reach nothing."""
+    c = Case(torch.bfloat16, d, 6, 2, 32, 40, [300, 77, 40], q_lens=[33, 0, 7])
+    for b, n in enumerate(c.q_lens):
+        c.q[b, n:] = math.nan
+    for weights in (False, True):
+        out, _ = c.check(algo=algo, weights=weights)
+        for b, n in enumerate(c.q_lens):
+            assert not out[b, n:].any()
+
+
+def test_lengths_past_the_bounds_are_clamped():
+    c = Case(torch.float16, 64, 2, 1, 16, 4, [64, 10])
+    out, lse = c.run()
+    args = dict(kv_lens=torch.tensor([2 ** 40, 10], device=DEV), q_lens=torch.tensor([99, 2 ** 33], device=DEV))
+    o2 = torch.empty_like(out)
+    llmx_b200.paged_attention(o2, c.q.to(DEV), c.k_cache, c.v_cache, 64 ** -0.5, block_table=c.table.to(DEV), **args)
+    assert torch.equal(o2, out)  # the table holds 64 tokens a sequence
+    llmx_b200.paged_attention(o2, c.q.to(DEV), c.k_cache, c.v_cache, 64 ** -0.5, block_table=c.table.to(DEV),
+                              kv_lens=ints([-3, 0]))
+    assert not o2.any()
+
+
+def test_strides_of_extents_of_one_do_not_matter():
+    c = Case(torch.bfloat16, 64, 2, 1, 16, 1, [40], extra=0)
+    q = c.q.to(DEV).as_strided((1, 1, 2, 64), (3, 5, 64, 1))
+    kc, vc = (x.as_strided(x.shape, (x.stride(0), 7, 64, 1)) for x in (c.k_cache, c.v_cache))
+    out = torch.empty_like(c.q, device=DEV)
+    w = torch.zeros(c.k_cache.shape[:3], device=DEV)
+    llmx_b200.paged_attention(out, q, kc, vc, 64 ** -0.5, kv_lens=ints([40]), block_table=c.table.to(DEV),
+                              key_weights=w.as_strided(w.shape, (w.stride(0), 3, 1)))
+    check_attention(out[0], None, None, c.want(0), c.dtype)
+    assert abs(float(w.sum()) - 2) < 1e-4
+
+
+def test_output_over_q_is_refused_with_weights():
+    c = Case(torch.bfloat16, 64, 2, 1, 16, 3, [40])
+    want, _ = c.run()
+    q = c.q.to(DEV)
+    args = dict(kv_lens=ints([40]), block_table=c.table.to(DEV))
+    with pytest.raises(LlmxError):
+        llmx_b200.paged_attention(q, q, c.k_cache, c.v_cache, 64 ** -0.5, key_weights=torch.zeros(c.k_cache.shape[:3], device=DEV), **args)
+    llmx_b200.paged_attention(q, q, c.k_cache, c.v_cache, 64 ** -0.5, **args)
+    assert torch.equal(q, want)
+
+
+def test_calls_at_once_on_two_streams():
+    cases = [Case(torch.bfloat16, 128, 8, 2, 64, q, [900, 333], seed=q) for q in (1, 9, 64)]
+    want = [c.run()[0] for c in cases]
+    args = [(c.q.to(DEV), c.k_cache, c.v_cache, ints(c.lens), c.table.to(DEV)) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [torch.empty_like(w) for w in want]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, (q, k, v, lens, table), o in zip(streams, args, outs):
+            with torch.cuda.stream(s):
+                llmx_b200.paged_attention(o, q, k, v, 128 ** -0.5, kv_lens=lens, block_table=table)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+
+
 @pytest.mark.parametrize("q_len,lens", [(1, [3000, 100]), (33, [500, 90]), (200, [700, 300])])
 def test_same_bits_again_on_other_streams_and_in_graphs(q_len, lens):
     c = Case(torch.bfloat16, 128, 8, 2, 64, q_len, lens)
