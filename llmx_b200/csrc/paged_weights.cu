@@ -308,6 +308,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
             const int b0 = min(max(lo - ch * 32, 0), 32), b1 = min(max(hi - ch * 32, 0), 32);
             seen = (b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u) & ~(b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u);
           }
+          bool small = false;
+          if constexpr (kSoftcap) small = __all_sync(0xffffffffu, chunk_size(vc) * cap_in <= kCapSmall);
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const float4 ad = ca[ch * 8 + c / 4];
@@ -319,7 +321,11 @@ __global__ void __launch_bounds__(kWThreads, 1)
               x[2] = fmaf(sl.z, kf, x[2]);
               x[3] = fmaf(sl.w, kf, x[3]);
             }
-            if constexpr (kSoftcap) {
+            if (kSoftcap && small) {
+              const CapPoly cap(cap_in, cap_out);
+              f2_split(cap(f2(__uint_as_float(vc[c]), __uint_as_float(vc[c + 1])), f2(x[0], x[1])), x[0], x[1]);
+              f2_split(cap(f2(__uint_as_float(vc[c + 2]), __uint_as_float(vc[c + 3])), f2(x[2], x[3])), x[2], x[3]);
+            } else if constexpr (kSoftcap) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) x[e] = fmaf(cap_tanh(__uint_as_float(vc[c + e]) * cap_in), cap_out, x[e]);
             } else {
