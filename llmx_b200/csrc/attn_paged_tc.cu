@@ -71,9 +71,13 @@ struct TcWork {
   int n_mblocks;    // items of a unit
   int group_units;  // units whose K / V fit in L2 together
   int n_whole;      // items [0, n_whole) are whole,
-  int piece;        // the others in pieces of so many blocks,
-  int parts;        // at most so many
+  int piece;        // the others in pieces of so many blocks (the last: the rest),
+  int parts;        // at most so many (cut_items may take fewer)
   int n_work;
+  int cut;          // items that are cut
+  int *how;         // nullable: the device cuts; piece and parts that it took
+  float per_query, per_sm;  // for it: items of a query, 1 / SMs,
+  int most_keys;            // and what an item sees of a window at most
   int box;         // tokens of a TMA box
   float *part_o;   // [pieces][128 tiles][D]
   float *part_ml;  // [pieces][128 tiles][2]
@@ -104,16 +108,84 @@ struct PBars {
 };
 static_assert(sizeof(PBars) <= 1024, "barriers");
 
+// What a cut of the longest item, of nb blocks, into s pieces costs, in blocks of
+// 128 keys on an SM.  A piece costs its blocks and about 3 for its start and end, and
+// 1.5 for the merge, as it writes and reads 128 KB of it.  `share` is the items' mean
+// length over the longest's.  The launch ends with its last wave, or, as the pieces
+// are dealt as CTAs come free, a part of a piece after its mean.
+__host__ __device__ __forceinline__ float cut_cost(float nb, float s, float items, float share, float per_sm) {
+  const float n = items * (1.f - share + share * s) * per_sm;  // pieces of an SM
+  const float piece = ceilf(nb / s) + 3.f;
+  const float mean = items * share * nb * per_sm + 3.f * n;
+  return (s > 1.f ? 2.f + 1.5f * n : 0.f) +
+         fminf(ceilf(items * s * per_sm) * piece, fmaxf(piece, mean + (0.2f + 0.8f * share) * piece));
+}
+
+// The cut that suits the lengths that the device has, at most as many pieces as the
+// workspace was laid out for: 16 sequences of 4,096 tokens with 64 queries, 32 heads
+// over 8 of 128, took 115 us cut for ragged lengths, of 0.6 of the longest one's in
+// the mean, and take 82 us; of 8,192 tokens 184 and 144 us.
+struct Cut {
+  int piece, parts, n_work;
+};
+__device__ __forceinline__ int seen_blocks(const RowsSee &s) {
+  return s.hi > s.lo ? (s.hi - s.lo / kBN * kBN + kBN - 1) / kBN : 0;
+}
+__device__ __forceinline__ Cut cut_items(const AttnArgs &a, const TcWork &wk) {  // by the load warp
+  Cut c{wk.piece, wk.parts, wk.n_work};
+  if (wk.how == nullptr) return c;
+  // Few instructions: the first item waits for them, and they come from L2.  An
+  // item sees about as much as the middle row of its sequence.
+  const int lane = threadIdx.x % 32;
+  const bool windowed = a.causal && a.window >= 0;
+  float items = 0.f, total = 0.f, longest = 1.f;
+#pragma unroll 1
+  for (int b = lane; b < a.B; b += 32) {
+    const int ql = clamp_len(a.q_lens, b, a.Sq), kl = clamp_len(a.kv_lens, b, a.Skv);
+    const float n = kl > 0 ? ceilf((float)ql * wk.per_query) : 0.f;
+    const float most = (float)(windowed ? min(kl, wk.most_keys) : kl) * (1.f / kBN);
+    items += n;
+    total += n * (a.causal && !windowed ? fmaxf(most - (float)ql * (0.5f / kBN), 0.f) : most);
+    if (n > 0.f) longest = fmaxf(longest, ceilf(most));
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    items += __shfl_xor_sync(0xffffffffu, items, off);
+    total += __shfl_xor_sync(0xffffffffu, total, off);
+    longest = fmaxf(longest, __shfl_xor_sync(0xffffffffu, longest, off));
+  }
+  const float share = items > 0.f ? fminf(1.f, __fdividef(total, items * longest)) : 1.f;
+  items = fminf(items * (float)a.Hkv, (float)wk.cut);
+  float best = CUDART_INF_F;
+  int s = 1;
+#pragma unroll 1
+  for (int t = lane + 1; t <= min(wk.parts, (int)longest / 4); t += 32) {
+    const float cost = cut_cost(longest, (float)t, items, share, wk.per_sm);
+    if (cost < best) best = cost, s = t;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    const float cost = __shfl_xor_sync(0xffffffffu, best, off);
+    const int t = __shfl_xor_sync(0xffffffffu, s, off);
+    if (cost < best || (cost == best && t < s)) best = cost, s = t;
+  }
+  c.piece = (int)ceilf(__fdividef(longest, (float)s));
+  c.parts = s;
+  c.n_work = wk.n_whole + wk.cut * s;
+  if (blockIdx.x == 0 && lane == 0) wk.how[0] = c.piece, wk.how[1] = c.parts;  // for the merge
+  return c;
+}
+
 // Work item w: units in groups whose K / V fit in L2 together, inside a group the
 // last rows (which see the most keys) first, as in the dense prefill.
-__device__ __forceinline__ Item decode_item(const AttnArgs &a, const TcWork &wk, int w) {
+__device__ __forceinline__ Item decode_item(const AttnArgs &a, const TcWork &wk, const Cut &c, int w) {
   Item t;
   int idx = w, part = 0;
   t.slot = -1;
-  const bool cut = w >= wk.n_whole && wk.parts > 1;
+  const bool cut = w >= wk.n_whole && c.parts > 1;
   if (cut) {
-    idx = wk.n_whole + (w - wk.n_whole) / wk.parts;
-    part = (w - wk.n_whole) % wk.parts;
+    idx = wk.n_whole + (w - wk.n_whole) / c.parts;
+    part = (w - wk.n_whole) % c.parts;
   }
   const int units = a.B * a.Hkv;
   const int per_group = wk.group_units * wk.n_mblocks;
@@ -128,7 +200,7 @@ __device__ __forceinline__ Item decode_item(const AttnArgs &a, const TcWork &wk,
   t.m0 = mblk * wk.tiles * wk.M;
   const RowsSee s = rows_see(a, t.m0, wk.tiles * wk.M, t.ql, t.kl);
   const int lo = s.lo / kBN * kBN;
-  int nb = s.hi > s.lo ? (s.hi - lo + kBN - 1) / kBN : 0;
+  const int nb = seen_blocks(s);
   int nb0 = nb;
   if (nb > 0 && wk.tiles == 2) {
     const RowsSee s0 = rows_see(a, t.m0, wk.M, t.ql, t.kl);
@@ -136,9 +208,9 @@ __device__ __forceinline__ Item decode_item(const AttnArgs &a, const TcWork &wk,
   }
   int p0 = 0, p1 = nb;
   if (cut) {
-    t.pieces = (nb + wk.piece - 1) / wk.piece;
-    p0 = min(nb, part * wk.piece);
-    p1 = min(nb, p0 + wk.piece);
+    t.pieces = min(c.parts, (nb + c.piece - 1) / c.piece);
+    p0 = min(nb, part * c.piece);
+    p1 = part == c.parts - 1 ? nb : min(nb, p0 + c.piece);
     if (t.pieces > 1) t.slot = w - wk.n_whole;
   } else {
     t.pieces = 1;
@@ -617,9 +689,10 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
       Item t{};
       BoxPlace first{0, 0};
       bool ok = true;
+      const Cut cut = cut_items(a, wk);
       auto fetch = [&](int from) {  // the item of ticket `from`, or of the first one after it that has work
-        for (w = from; w < wk.n_work;) {
-          t = decode_item(a, wk, w);
+        for (w = from; w < cut.n_work;) {
+          t = decode_item(a, wk, cut, w);
           if (!t.none) break;
           w = wk.n_work;
           if (work_ctr != nullptr) {
@@ -627,6 +700,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             w = __shfl_sync(0xffffffffu, w, 0);
           }
         }
+        if (w >= cut.n_work) w = wk.n_work;
         bool done = true;
         if (lane == 0) done = publish(bars, seq, w, t);
         ok = __all_sync(0xffffffffu, done) != 0;
@@ -741,16 +815,24 @@ __global__ void __launch_bounds__(128) paged_tc_merge_kernel(const __grid_consta
   constexpr int E = D / 32, kItemRows = PCfg<D>::kItemRows;
   constexpr float kShift = (float)tc_shift<T>();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int cut = blockIdx.x / (kItemRows / 4), in_item = blockIdx.x % (kItemRows / 4) * 4 + warp;
+  constexpr int kPerItem = kItemRows / 4;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const Item t = decode_item(a, wk, wk.n_whole + cut * wk.parts);
+  Cut how{wk.piece, wk.parts, wk.n_work};
+  Item t;
+  if (wk.how == nullptr) t = decode_item(a, wk, how, wk.n_whole + blockIdx.x / kPerItem * how.parts);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (t.slot < 0) return;
-  {
+  if (wk.how != nullptr) {
+    how = {wk.how[0], wk.how[1], 0};
+    if (how.parts == 1) return;
+  }
+  for (int x = blockIdx.x; x < wk.cut * kPerItem; x += gridDim.x) {
+    const int cut = x / kPerItem, in_item = x % kPerItem * 4 + warp;
+    if (wk.how != nullptr) t = decode_item(a, wk, how, wk.n_whole + cut * how.parts);
+    if (t.slot < 0) continue;
     const int tile = in_item / kBM, r = in_item % kBM;
     const int pr = t.m0 + tile * wk.M + r;
-    if (r >= wk.M || pr >= wk.R) return;
-    auto at = [&](int s) { return ((long long)cut * wk.parts + s) * kItemRows + in_item; };
+    if (r >= wk.M || pr >= wk.R) continue;
+    auto at = [&](int s) { return ((long long)cut * how.parts + s) * kItemRows + in_item; };
     float m = -CUDART_INF_F;
     for (int s = lane; s < t.pieces; s += 32) m = fmaxf(m, wk.part_ml[at(s) * 2]);
 #pragma unroll
@@ -815,8 +897,9 @@ cudaError_t launch_tc_t(const AttnArgs &a, const TcWork &wk, int grid, int *ctr,
   kern<<<grid, C::kThreads, C::kSmemBytes, s>>>(tq, tk, tv, a, wk, ctr);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || wk.parts == 1) return e;
-  const int cut = (wk.n_work - wk.n_whole) / wk.parts;
-  return launch_paged_after(paged_tc_merge_kernel<T, D>, dim3(cut * (C::kItemRows / 4)), 128, 0, s, a, wk);
+  const int groups = wk.cut * (C::kItemRows / 4);
+  return launch_paged_after(paged_tc_merge_kernel<T, D>, dim3(wk.how != nullptr ? std::min(groups, 16 * a.num_sms) : groups),
+                            128, 0, s, a, wk);
 }
 
 template <typename T, int D>
@@ -861,24 +944,27 @@ PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws) {
   const int nb = (int)((keys + kBN - 1) / kBN);
   p.piece = nb;
   if (have_ws) {
-    // In blocks of 128 keys: a piece costs its blocks and about 3 for its start and
-    // end, and 0.15 of an SM's for the merge, which reads 128 KB of it.  Lengths that
-    // only the device knows are taken to be 0.6 of the longest, and the launch to
-    // end half a piece after its mean; of equal ones only the items of the last,
-    // part-filled wave are cut, by the number of waves.
-    const bool ragged = a.B > 1 && a.kv_lens != nullptr;
+    // Of equal lengths only the items of the last, part-filled wave are cut; with
+    // lengths that only the device knows all of them, where they are few.
+    const bool ragged = a.B > 1 && (a.kv_lens != nullptr || a.q_lens != nullptr);
     const int cut = ragged ? (items < 4 * sms ? items : 0) : items % sms;
-    double best = 1e30;
-    for (int s = 1; cut > 0 && s <= std::min(64, std::max(1, nb / 4)); ++s) {
-      const double piece = (double)nb / s + 3.0;
-      const double merge = s > 1 ? 3.0 + 0.15 * s * cut / sms : 0.0;
-      const double mean = (double)cut * (0.6 * nb + 3.0 * (0.4 + 0.6 * s)) / sms;
-      const double cost = merge + (ragged ? std::max(piece, mean + 0.5 * piece)
-                                          : (double)(((long long)cut * s + sms - 1) / sms) * piece);
-      if (cost < best) {
-        best = cost;
-        p.piece = (nb + s - 1) / s;
+    const int most = std::min(64, std::max(1, nb / 4));
+    auto best = [&](float share) {
+      int at = 1;
+      for (int s = 2; s <= most; ++s)
+        if (cut_cost((float)nb, (float)s, (float)cut, share, 1.f / sms) < cut_cost((float)nb, (float)at, (float)cut, share, 1.f / sms)) at = s;
+      return at;
+    };
+    if (cut > 0) {
+      int s = best(1.f);
+      if (ragged) {
+        // The device may cut a few long ones among short ones into more pieces.  Short
+        // ones are left whole: its choice and the merge's launch cost about 8 us.
+        s = std::max(s, best(0.6f));
+        if (nb >= 32) s = std::max(s, std::min(most, 2 * sms / cut));
+        p.on_device = s > 1;
       }
+      p.piece = (nb + s - 1) / s;
     }
     p.parts = (nb + p.piece - 1) / p.piece;
     if (p.parts > 1) p.n_whole = items - cut;
@@ -902,6 +988,11 @@ cudaError_t launch_paged_tc(const AttnArgs &a, const PagedArgs &c, const PagedTc
   wk.piece = p.piece;
   wk.parts = p.parts;
   wk.n_work = p.n_work;
+  wk.cut = (p.n_work - p.n_whole) / p.parts;
+  wk.how = p.on_device && p.parts > 1 ? ctr + 1 : nullptr;
+  wk.per_query = (float)a.group / (float)(wk.tiles * p.M);
+  wk.per_sm = 1.f / (float)std::max(1, a.num_sms);
+  wk.most_keys = std::min(std::max(0, a.window), 1 << 30) + wk.tiles * p.M / a.group + kBN;
   wk.box = std::gcd(c.page_size, kBN);
   wk.part_o = part;
   wk.part_ml = p.parts > 1 ? part + (size_t)(p.n_work - p.n_whole) * wk.tiles * kBM * a.D : nullptr;

@@ -39,6 +39,7 @@ __device__ __forceinline__ int alibi_ref(const Visible &v, float slope) { return
 // [B * Hkv][R], log2 of each packed row's sum of 2^score.
 struct PagedTcPlan {
   int M, n_mblocks, n_whole, piece, parts, n_work;
+  bool on_device;  // the device cuts, by the lengths that it has
   size_t part_bytes;
 };
 bool paged_tc_supports(const AttnArgs &a);
