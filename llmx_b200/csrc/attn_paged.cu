@@ -26,6 +26,10 @@
 // from the pages into one ring of slots, in the order in which they are used (K
 // of a block comes before V of the block before it).
 //
+// Bound by HBM: 32 sequences of 1001-8191 tokens, 32 heads on 8 of 128, take 102 us
+// (5.9 TB/s, 0.90 of the measured copy rate), one of 131071 tokens 94 us (5.7 TB/s);
+// what is missing is the start and the merge.  Short calls are their launch (8 us).
+//
 // Masked tokens.  A NaN or an infinity in K only reaches scores that are
 // replaced.  One in V would reach every row through 0 * V, so in blocks that not
 // every row sees whole, the thread of a token first writes zeros over such

