@@ -234,6 +234,16 @@ def test_long_sequence_among_short_ones():
     c.check(weights=True)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens,q_lens", [([4200, 4200, 4200], None), ([6000, 40, 0, 4100], [50, 40, 0, 7]), ([9, 1, 5000], [9, 1, 50])])
+def test_tiles_cut_by_the_lengths_on_the_device(d, lens, q_lens):
+    c = Case(torch.bfloat16, d, 8, 2, 64, 50, lens, q_lens=q_lens, seed=d + len(lens))
+    for kw in (dict(), dict(causal=False), dict(window=4500, cap=20.0), dict(slopes=slopes_of(8))):
+        c.check(algo="tcgen05", what=str(list(kw)), **kw)
+    c.check(algo="tcgen05", weights=True)
+    llmx_b200.device_status(0)
+
+
 def test_many_sequences():
     lens = [(37 * i) % 200 for i in range(300)]
     c = Case(torch.float16, 64, 2, 1, 16, 1, lens, seed=4)
