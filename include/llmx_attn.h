@@ -407,8 +407,7 @@ LLMX_API llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv4_
  *           (query row, head) pairs of a kv head, split over the machine.
  *   TCGEN05 tiles of 128 such pairs; sm_scale > 0, at most 128 query heads a
  *           kv head.
- *   AUTO    DECODE up to 32 pairs (head_dim 256: 128), TCGEN05 above where it
- *           can run.
+ *   AUTO    DECODE up to 32 pairs, TCGEN05 above where it can run.
  * ALiBi's biases count from each row's largest one, so that they keep their
  * bits far into a sequence; lse is that of slope * position.  A NaN or an
  * infinity in a cached token reaches the rows that see the token and no

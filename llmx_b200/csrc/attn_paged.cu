@@ -46,8 +46,12 @@
 namespace llmx_b200 {
 namespace {
 
-// AUTO: packed rows of a kv head up to which this form is taken.
-constexpr int step_rows(int D) { return D == 256 ? 128 : 32; }
+// AUTO: packed rows of a kv head up to which this form is taken.  Both forms, us, at
+// 16 / 32 / 48 / 64 / 128 rows (L2 flushed): 16 sequences of 4096 tokens, 8 kv heads of
+// 128: this 69 / 75 / 118 / 120 / 202, tiles 84 at all; one of 32768: 48 / 48 / 58 / 56 /
+// 93, 50 / 52 / 52 / 54 / 56; 4 of 4096 at head_dim 256: 50 / 50 / 54 / 54 / 75, 51 / 53 /
+// 55 / 55 / 59; 16 of 2048 at 256: 77 / 81 / 89 / 93 / 142, 69 at all.
+constexpr int kStepRows = 32;
 constexpr size_t kCounterBytes = 256;
 
 // A launch's units and shares.
@@ -1142,7 +1146,7 @@ llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs
   const bool can = paged_tc_supports(a);
   if (p->algo == LLMX_ALGO_TCGEN05 && !can)
     return record_error(LLMX_ERR_UNSUPPORTED, "paged attention: TCGEN05 needs sm_scale > 0 and at most 128 query heads a kv head");
-  plan->tc = can && (p->algo == LLMX_ALGO_TCGEN05 || (p->algo == LLMX_ALGO_AUTO && (long long)a.Sq * a.group > step_rows(a.D)));
+  plan->tc = can && (p->algo == LLMX_ALGO_TCGEN05 || (p->algo == LLMX_ALGO_AUTO && (long long)a.Sq * a.group > kStepRows));
   const bool weights = k.w != nullptr;
   const long long R = (long long)a.Sq * a.group;
   if (plan->tc) {
