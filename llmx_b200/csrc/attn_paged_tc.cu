@@ -449,7 +449,16 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
       // 0's blocks are the last ones in reverse order.)
       const int g = kv_base + (kAlibi && t == 0 ? w.br.nb - w.nb0 : 0) + j;
       const int s = g % C::kStages;
-      ok = mbar_wait_or_abort(&bars->v_full[s], (g / C::kStages) & 1, kTimeoutNs, &bars->abort_flag);
+      // A wait by parity needs the stage's block before this one to have been passed
+      // on, else it returns a phase early.  With two tiles the MMA thread has waited
+      // for that before it issued these scores.  With one stage it is block g - 1,
+      // which the products may still be waiting for when these scores are there: its
+      // product is waited for first (the next one on that barrier needs this thread's
+      // P of a later block, so this phase cannot be passed over; before an item's first
+      // block the epilogue has waited for it).
+      ok = true;
+      if (C::kOne && j > 0) ok = mbar_wait_or_abort(&bars->o_done[which(i - 1)], phase(i - 1), kTimeoutNs, &bars->abort_flag);
+      ok = ok && mbar_wait_or_abort(&bars->v_full[s], (g / C::kStages) & 1, kTimeoutNs, &bars->abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         set_abort(bars, a.err);
         aborted = true;

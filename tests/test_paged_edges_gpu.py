@@ -1,0 +1,72 @@
+"""The paged 16-bit cache on the GPU where a value, a length or a page is at the edge of
+what a call may hold: infinities and NaN beside masks, padded rows, pages outside the
+cache, sizes near 2^31, soft-caps of any size."""
+import math
+
+import pytest
+import torch
+
+import llmx_b200
+from gpu_helpers import needs_cuda
+from paged_helpers import DEV, Case
+
+pytestmark = [pytest.mark.gpu, needs_cuda]
+
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def rows_that_see(c, b, tokens, window=-1):
+    """Which query rows of sequence b see one of the tokens (causal)."""
+    ql = c.q_len if c.q_lens is None else c.q_lens[b]
+    i = torch.arange(c.q_len)
+    diag = i + c.lens[b] - ql
+    hit = torch.zeros(c.q_len, dtype=torch.bool)
+    for t in tokens:
+        hit |= (t <= diag) & (i < ql) & ((diag - t <= window) if window >= 0 else True)
+    return hit
+
+
+def check_spread(c, poison, value, where="v", **kw):
+    """`value` in channel 7 of kv head 1 of the tokens poison[b] of sequence b:
+    rows that do not see one of them, and the other heads, keep their bits; with a
+    NaN the rows that do become NaN."""
+    clean, _ = c.run(**kw)
+    assert clean.isfinite().all()
+    group = c.heads // c.hkv
+    for b, tokens in poison.items():
+        for t in tokens:
+            (c.k if where == "k" else c.v)[b][t, 1, 7] = value
+        c.put(b)
+    for _ in range(3):
+        out, _ = c.run(**kw)
+        for b in range(len(c.lens)):
+            hit = rows_that_see(c, b, poison.get(b, ()), kw.get("window", -1))
+            keep = torch.ones(c.q_len, c.heads, dtype=torch.bool)
+            keep[hit, group:2 * group] = False
+            assert torch.equal(out[b, keep], clean[b, keep]), f"sequence {b}"
+            if math.isnan(value):
+                assert out[b, hit.to(DEV), group:2 * group].isnan().flatten(2).any(-1).all(), f"sequence {b}"
+    llmx_b200.device_status(0)
+
+
+# Tiles: several items a CTA (160 of them and more), contexts of several blocks before
+# the diagonal, so that the products of a block may be behind the next one's scores.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_non_finite_v_in_tiles(dtype, d, value):
+    lens = [900 - 7 * i for i in range(40)]
+    for kw in (dict(), dict(window=200)):
+        c = Case(dtype, d, 4, 2, 32, 150, lens, seed=d)
+        poison = {b: (lens[b] - 1, lens[b] - 77, lens[b] - 140, 300) for b in range(0, 40, 3)}
+        check_spread(c, poison, value, algo="tcgen05", **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tiles_of_head_dim_256_without_anything_non_finite(dtype):
+    c = Case(dtype, 256, 4, 2, 64, 200, [1500 - 31 * i for i in range(30)], seed=1)
+    first, _ = c.check(algo="tcgen05", weights=True)
+    for _ in range(5):
+        out, lse = c.run(algo="tcgen05")
+        assert torch.equal(out, first) and lse.isfinite().all()
+    llmx_b200.device_status(0)
