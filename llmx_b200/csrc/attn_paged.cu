@@ -209,7 +209,9 @@ struct StepCfg {
   static constexpr int kBudget = (kCtas == 2 ? 113 : 227) * 1024 - 1024 - 256;  // less alignment and static arrays
   static constexpr int kFit = (kBudget - kQ - 2 * kP - kInfo) / kSlot;
   static constexpr int kSlots = kFit < 12 ? kFit : 12;
-  static_assert(kSlots >= 3 * kHalves || (kHalves == 2 && kSlots >= 4), "ring");
+  // What the products need, and what the softmax's wait for V does (where it looks at V).
+  static_assert(kSlots >= 3 || kHalves > 1, "ring");
+  static_assert(kSlots >= 2 * kHalves, "ring");
   static constexpr int kQOff = kSlots * kSlot, kPOff = kQOff + kQ, kInfoOff = kPOff + 2 * kP;
   static constexpr int kSmem = kInfoOff + kInfo + 1024;
   // Tensor memory: two score accumulators, then O^T (one for each 128 channels).
@@ -668,6 +670,14 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
           // of the channels.
           const bool none = j < sp.lo || j >= sp.hi, some = j < sp.all_lo || j >= sp.all_hi;
           bool lost = false;
+          // A wait by parity needs the slot's filling before V's to be over, else it
+          // returns a phase early.  The scores show that K of this block and V of two
+          // blocks back have come; in a ring of fewer than three blocks the filling
+          // before may be V of the last block, whose product is waited for (the next
+          // one on that barrier needs this thread's weights of the block after this
+          // one, so the phase cannot be passed over; another part's slots have all
+          // been used up).
+          if (C::kSlots < 3 * H && at > b0) wait_all(&bars->o_done[(blk - 1) & 1], ((blk - 1) >> 1) & 1);
           const int v0 = g + H * (min(at - b0 + 2, b1 - b0) + at - b0);  // V's first slot of the block
 #pragma unroll 1
           for (int half = 0; half < H; ++half) {

@@ -70,3 +70,17 @@ def test_tiles_of_head_dim_256_without_anything_non_finite(dtype):
         out, lse = c.run(algo="tcgen05")
         assert torch.equal(out, first) and lse.isfinite().all()
     llmx_b200.device_status(0)
+
+
+# Few rows at head_dim 256, whose ring holds fewer than three blocks: the new rows lie
+# across a border of 128 tokens, so that the last block but one is partly seen while V
+# of the block before it may still be on its way.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,q_len", [(16, 3), (16, 4), (16, 7), (6, 8), (6, 20)])
+@pytest.mark.parametrize("value", [math.nan, -math.inf])
+def test_non_finite_v_of_few_rows_across_a_block(dtype, heads, q_len, value):
+    for lens in ([1025, 898, 385, 257], [129 + 128 * (i % 9) for i in range(90)]):
+        c = Case(dtype, 256, heads, 2, 64, q_len, lens, seed=heads + q_len)
+        poison = {b: (n // 128 * 128 - 1, n - 1, n // 128 * 128 - 2) for b, n in enumerate(lens) if b % 3 != 1}
+        check_spread(c, poison, value, algo="decode")
+        check_spread(Case(dtype, 256, heads, 2, 64, q_len, lens, seed=3), poison, value, algo="decode", window=150)
