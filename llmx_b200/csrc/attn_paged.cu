@@ -836,8 +836,12 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
         if (whole) {
 #pragma unroll
           for (int r = 0; r < W; ++r)
-            if (c0 + r < rows)
-              static_cast<T *>(a.o)[info->out[c0 + r] + ch] = Elem<T>::from_f(o[r] * info->inv[c0 + r]);  // 0 for a row that sees nothing
+            if (c0 + r < rows) {
+              // 0 for a row that sees nothing, and chosen so: the sums of a padded row,
+              // which is not masked where all others see a block, may be anything.
+              const float inv = info->inv[c0 + r];
+              static_cast<T *>(a.o)[info->out[c0 + r] + ch] = Elem<T>::from_f(inv != 0.f ? o[r] * inv : 0.f);
+            }
         } else {
           float *po = wk.part_o + (slot * N + c0) * D + ch;
 #pragma unroll

@@ -84,3 +84,18 @@ def test_non_finite_v_of_few_rows_across_a_block(dtype, heads, q_len, value):
         poison = {b: (n // 128 * 128 - 1, n - 1, n // 128 * 128 - 2) for b, n in enumerate(lens) if b % 3 != 1}
         check_spread(c, poison, value, algo="decode")
         check_spread(Case(dtype, 256, heads, 2, 64, q_len, lens, seed=3), poison, value, algo="decode", window=150)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("algo", ["decode", "tcgen05"])
+def test_padded_rows_beside_non_finite_tokens_are_zero(dtype, d, algo):
+    """Rows at or past q_lens see no token: they are 0 (lse -inf) whatever the cache holds,
+    in short sequences, which one CTA has whole, and in long ones."""
+    for lens in ([200, 130, 256, 9], [2000, 130, 700, 9]):
+        for where, value in (("v", math.nan), ("v", math.inf), ("k", math.nan), ("k", -math.inf)):
+            c = Case(dtype, d, 4, 2, 32, 4, lens, q_lens=[1, 3, 0, 2], seed=d)
+            check_spread(c, {0: (5,), 1: (0, 40), 2: (100,)}, value, where=where, algo=algo)
+            out, lse = c.run(algo=algo)
+            for b, n in enumerate(c.q_lens):
+                assert not out[b, n:].any() and (lse[b, :, n:] == -math.inf).all(), (where, value, b)
