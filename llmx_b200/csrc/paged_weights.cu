@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
             seen = (b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u) & ~(b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u);
           }
           bool small = false;
-          if constexpr (kSoftcap) small = __all_sync(0xffffffffu, chunk_size(vc) * cap_in <= kCapSmall);
+          if constexpr (kSoftcap) small = __all_sync(0xffffffffu, chunk_size(vc) * fabsf(cap_in) <= kCapSmall);  // any scale
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const float4 ad = ca[ch * 8 + c / 4];

@@ -99,3 +99,13 @@ def test_padded_rows_beside_non_finite_tokens_are_zero(dtype, d, algo):
             out, lse = c.run(algo=algo)
             for b, n in enumerate(c.q_lens):
                 assert not out[b, n:].any() and (lse[b, :, n:] == -math.inf).all(), (where, value, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_weights_of_a_chunk_with_a_negative_scale_and_a_cap(dtype, d):
+    """Scores to well past the cap on both sides."""
+    c = Case(dtype, d, 4, 2, 32, 40, [333, 77], seed=d)
+    for cap in (3.0, 40.0):
+        c.check(algo="decode", sm_scale=-4.0 * d ** -0.5, cap=cap, weights=True, what=f"cap {cap}")
+        c.check(algo="decode", sm_scale=-4.0 * d ** -0.5, cap=cap, weights=True, slopes=torch.tensor([0.5, 0.1, 0.02, 0.004]))
