@@ -411,7 +411,8 @@ LLMX_API llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv4_
  * ALiBi's biases count from each row's largest one, so that they keep their
  * bits far into a sequence; lse is that of slope * position.  A NaN or an
  * infinity in a cached token reaches the rows that see the token and no
- * others; one in V may make such a row (and its lse) NaN as a whole.
+ * others; one in V may make such a row of o NaN as a whole, and shows in
+ * neither lse nor key weights.
  *   With c->key_weights, the weight of every token j < kv_lens[b] of every kv
  * head becomes
  *   decay * (what was there) + sum of softmax(row)[j] over the query rows and

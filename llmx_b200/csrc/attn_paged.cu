@@ -34,7 +34,8 @@
 // replaced.  One in V would reach every row through 0 * V, so in blocks that not
 // every row sees whole, the thread of a token first writes zeros over such
 // values (and over all of a token that no row sees: nothing behind a sequence's
-// length counts), and its weight becomes NaN for the rows that see it.
+// length counts), and the output of the rows that see it becomes NaN (their sums,
+// lse and key weights do not: V has no part in them).
 #include <algorithm>
 #include <climits>
 #include <cstdio>
@@ -231,7 +232,7 @@ struct RowInfo {
   int bias0[N];  // the token whose ALiBi bias counts as 0
   int lo[N], hi[N];
   float wmax[4][N];  // by warp: maxima, then sums
-  float inv[N];
+  float scale[N];    // 1, or NaN: the row sees a token that lost a value of V; of a whole unit then over the sum
 };
 struct SBars {
   uint64_t full[12], empty[12];
@@ -622,6 +623,7 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
         info->bias0[row] = alibi_ref(v, slope);
         info->ref[row] = info->limit[row] = -CUDART_INF_F;
         info->base[row] = -kShift;
+        info->scale[row] = 1.f;
         info->out[row] = cur.b * a.os[0] + i * a.os[1] + h * a.os[2];
       }
       if (b0 < b1) {
@@ -700,7 +702,12 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
             const int l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              x[r + e] = j >= l4[e] && j < h4[e] ? (lost ? CUDART_NAN_F : x[r + e]) : -CUDART_INF_F;
+              x[r + e] = j >= l4[e] && j < h4[e] ? x[r + e] : -CUDART_INF_F;
+          }
+          if (lost) {  // the rows that see the token; scores and sums have nothing to do with V
+#pragma unroll 1
+            for (int r = c0; r < c0 + W; ++r)
+              if (j >= info->lo[r] && j < info->hi[r]) info->scale[r] = CUDART_NAN_F;
           }
         }
         if (wk.score != nullptr && j < wk.pitch) {
@@ -812,7 +819,7 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
           const int i = r / a.group, h = cur.kvh * a.group + r % a.group;
           const bool sees = info->hi[row] > info->lo[row];
           const float lse2 = info->ref[row] - kShift + log2f(sum);
-          info->inv[row] = sees ? 1.f / sum : 0.f;
+          info->scale[row] = sees ? info->scale[row] / sum : 0.f;
           if (a.lse != nullptr)
             a.lse[((long long)cur.b * a.H + h) * a.Sq + i] =
                 sees ? lse2 * kLn2 + (kMode != 0 && a.alibi != nullptr ? a.alibi[h] * (float)info->bias0[row] : 0.f) : -CUDART_INF_F;
@@ -839,14 +846,14 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
             if (c0 + r < rows) {
               // 0 for a row that sees nothing, and chosen so: the sums of a padded row,
               // which is not masked where all others see a block, may be anything.
-              const float inv = info->inv[c0 + r];
-              static_cast<T *>(a.o)[info->out[c0 + r] + ch] = Elem<T>::from_f(inv != 0.f ? o[r] * inv : 0.f);
+              const float scale = info->scale[c0 + r];
+              static_cast<T *>(a.o)[info->out[c0 + r] + ch] = Elem<T>::from_f(scale != 0.f ? o[r] * scale : 0.f);
             }
         } else {
           float *po = wk.part_o + (slot * N + c0) * D + ch;
 #pragma unroll
           for (int r = 0; r < W; ++r)
-            if (c0 + r < rows) po[r * D] = o[r];
+            if (c0 + r < rows) po[r * D] = o[r] * info->scale[c0 + r];
         }
       }
       tc_fence_before();  // O^T is read before the next part's products write it

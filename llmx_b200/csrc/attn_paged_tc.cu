@@ -18,7 +18,7 @@
 //    row sees whole it first writes zeros over the rows behind the sequence's
 //    length and over infinities and NaN (0 * NaN would reach the rows that do
 //    not see the token); a bit for each token that lost a value goes to the
-//    softmax threads, and rows that see such a token become NaN.
+//    softmax threads, and the output of rows that see such a token becomes NaN.
 //  * ALiBi: the folded slope (x_offset) is a row's own, and biases count from
 //    the row's largest one (alibi_ref).
 //  * Work: items (a unit's pair of tiles) longest first over one CTA an SM; the
@@ -411,6 +411,7 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
   const float cap_out = kSoftcap ? a.softcap * kLog2e : 0.f;
   float m_used = kNegInf, l = 0.f;
   bool aborted = false;
+  bool lost = false;  // sees a token that lost a value of V: its output is NaN, not its sum
   // The barrier of block i of the launch and its phase: a tile's own, or with one
   // tile by the block's parity, as the score accumulators.
   auto which = [&](int i) { return C::kOne ? i & 1 : t; };
@@ -471,7 +472,7 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
           const int b0 = min(max(lo - word * 32, 0), 32), b1 = min(max(hi - word * 32, 0), 32);
           const uint32_t below1 = b1 >= 32 ? 0xffffffffu : ((1u << b1) - 1u);
           const uint32_t below0 = b0 >= 32 ? 0xffffffffu : ((1u << b0) - 1u);
-          if (bits & below1 & ~below0) l = CUDART_NAN_F;
+          if (bits & below1 & ~below0) lost = true;
         }
       }
     }
@@ -526,6 +527,10 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
         for (int c = 0; c < 32; ++c) o[c] = 0u;
       }
       if (real) {
+        if (lost) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(CUDART_NAN_F);
+        }
 #pragma unroll
         for (int c = 0; c < 32; c += 4)
           *reinterpret_cast<uint4 *>(po + ch * 32 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
@@ -535,7 +540,7 @@ __device__ bool softmax_rows(const AttnArgs &a, const TcWork &wk, PBars *bars, u
     return !aborted;
   }
   const bool sees = vis.hi > vis.lo && have;
-  const float inv = sees ? 1.f / l : 0.f;
+  const float inv = sees ? (lost ? CUDART_NAN_F : 1.f / l) : 0.f;
   // As in the dense prefill, groups of four lanes swap pieces so that a store
   // writes 64 contiguous bytes of 8 rows.
   const int gi = threadIdx.x & 3;

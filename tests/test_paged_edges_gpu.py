@@ -109,3 +109,22 @@ def test_weights_of_a_chunk_with_a_negative_scale_and_a_cap(dtype, d):
     for cap in (3.0, 40.0):
         c.check(algo="decode", sm_scale=-4.0 * d ** -0.5, cap=cap, weights=True, what=f"cap {cap}")
         c.check(algo="decode", sm_scale=-4.0 * d ** -0.5, cap=cap, weights=True, slopes=torch.tensor([0.5, 0.1, 0.02, 0.004]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("algo,q_len", [("decode", 1), ("decode", 5), ("decode", 40), ("tcgen05", 5), ("tcgen05", 150)])
+def test_weights_and_lse_do_not_depend_on_v(dtype, d, algo, q_len):
+    """Key weights and lse come from q and K: an infinity or NaN in V does not show in them,
+    in blocks that all rows see and in blocks that some do."""
+    for lens in ([250, 190], [1500, 600]):
+        for window in (-1, 100):
+            c = Case(dtype, d, 4, 2, 32, q_len, lens, seed=d)
+            w0, w1 = (torch.zeros(c.k_cache.shape[:3], device=DEV) for _ in range(2))
+            _, lse0 = c.run(algo=algo, weights=w0, decay=0.0, window=window)
+            c.v[0][[3, lens[0] - 1, lens[0] - 2, lens[0] - 80], 0, 9] = math.nan
+            c.v[1][[lens[1] - 1, lens[1] - 30], 1, 1] = math.inf
+            c.put(0), c.put(1)
+            out, lse1 = c.run(algo=algo, weights=w1, decay=0.0, window=window)
+            assert torch.equal(w0, w1) and torch.equal(lse0, lse1)
+            assert out[0, -1, :2].isnan().flatten(1).any(-1).all()
