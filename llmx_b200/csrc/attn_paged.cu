@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
     const int wg = warp / 4, tok = tid % 128, c0 = wg * W;
     const uint32_t lane_off = (uint32_t)(warp % 4 * 32) << 16;
     const float scale2 = a.sm_scale * kLog2e;
-    const float cap_in = kMode == 2 ? a.sm_scale / a.softcap : 0.f, cap_out = a.softcap * kLog2e;
+    const SoftCap cap(kMode == 2 ? a.sm_scale / a.softcap : 0.f, a.softcap * kLog2e);
     constexpr float kShift = weight_shift<T>();
     int g = 0, blk = 0;
     bool ok = true;
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(StepCfg<D, N>::kThreads, StepCfg<D, N>::kCtas)
             const int b4[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              x[r + e] = kMode == 2 ? cap_tanh(x[r + e] * cap_in) * cap_out : x[r + e] * scale2;
+              x[r + e] = kMode == 2 ? cap(x[r + e], 0.f) : x[r + e] * scale2;
               x[r + e] = fmaf(s4[e], (float)(j - b4[e]), x[r + e]);
             }
           } else {

@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
             seen = (b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u) & ~(b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u);
           }
           bool small = false;
+          const SoftCap cap(cap_in, cap_out);
           if constexpr (kSoftcap) small = __all_sync(0xffffffffu, chunk_size(vc) * fabsf(cap_in) <= kCapSmall);  // any scale
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
@@ -323,12 +324,11 @@ __global__ void __launch_bounds__(kWThreads, 1)
               x[3] = fmaf(sl.w, kf, x[3]);
             }
             if (kSoftcap && small) {
-              const CapPoly cap(cap_in, cap_out);
-              f2_split(cap(f2(__uint_as_float(vc[c]), __uint_as_float(vc[c + 1])), f2(x[0], x[1])), x[0], x[1]);
-              f2_split(cap(f2(__uint_as_float(vc[c + 2]), __uint_as_float(vc[c + 3])), f2(x[2], x[3])), x[2], x[3]);
+              f2_split(cap.small_pair(f2(__uint_as_float(vc[c]), __uint_as_float(vc[c + 1])), f2(x[0], x[1])), x[0], x[1]);
+              f2_split(cap.small_pair(f2(__uint_as_float(vc[c + 2]), __uint_as_float(vc[c + 3])), f2(x[2], x[3])), x[2], x[3]);
             } else if constexpr (kSoftcap) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = fmaf(cap_tanh(__uint_as_float(vc[c + e]) * cap_in), cap_out, x[e]);
+              for (int e = 0; e < 4; ++e) x[e] = cap(__uint_as_float(vc[c + e]), x[e]);
             } else {
               const uint64_t sc = f2(scale2, scale2);
               f2_split(fma2(f2(__uint_as_float(vc[c]), __uint_as_float(vc[c + 1])), sc, f2(x[0], x[1])), x[0], x[1]);

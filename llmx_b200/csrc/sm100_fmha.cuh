@@ -321,21 +321,43 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
-// tanh by two special-function instructions: 1 - 2 / (1 + e^2|z|), within 2^-21 of
-// it.  A soft-cap needs absolute accuracy: cap * 2^-21 on a score.
-__device__ __forceinline__ float cap_tanh(float z) {
-  float u;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(u) : "f"(ex2_approx(fabsf(z) * (2.f * kLog2e)) + 1.f));
-  return copysignf(fmaf(-2.f, u, 1.f), z);
-}
+// The soft-cap of the paged cache's kernels, tanh(v * in) * out + add, right to 2^-20
+// of itself.  For |z| <= 1/2, z = v * in, it is z P(z^2), P of degree 4, fitted to
+// tanh(z) / z by iteratively reweighted least squares on z times the error (2^-24);
+// above, tanh is 1 - 2 / (1 + e^2|z|) by two special-function instructions.  Taken for
+// a small z that form's error, 2^-22, does not shrink with z, and a large cap makes it
+// an error of the score: 0.09 at a cap of 1e6.
+constexpr float kCapSmall = 0.5f;
+struct SoftCap {
+  float in, out, k[5];  // the coefficients times out
+  __device__ __forceinline__ SoftCap(float cap_in, float cap_out) : in(cap_in), out(cap_out) {
+    constexpr float c[5] = {0.9999999403953552f, -0.3333277702331543f, 0.13320571184158325f, -0.05276213213801384f,
+                            0.016737567260861397f};
+#pragma unroll
+    for (int i = 0; i < 5; ++i) k[i] = c[i] * cap_out;
+  }
+  __device__ __forceinline__ float operator()(float v, float add) const {
+    const float z = __fmul_rn(v, in), w = __fmul_rn(z, z);
+    float p = fmaf(k[4], w, k[3]);
+    p = fmaf(p, w, k[2]);
+    p = fmaf(p, w, k[1]);
+    p = fmaf(p, w, k[0]);
+    float u;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(u) : "f"(ex2_approx(fabsf(z) * (2.f * kLog2e)) + 1.f));
+    const float large = fmaf(copysignf(fmaf(-2.f, u, 1.f), z), out, add);
+    return fabsf(z) <= kCapSmall ? fmaf(z, p, add) : large;
+  }
+  // The same bits for a pair of raw scores that are both small (|v * in| <= 1/2).
+  __device__ __forceinline__ uint64_t small_pair(uint64_t v, uint64_t add) const;
+};
 
 // Score of column c (0..127 inside the block) in log2 units, before masking.
-// kFast (the paged cache's kernels): cap_tanh instead of tanhf.
+// kFast (the paged cache's kernels): SoftCap instead of tanhf.
 template <bool kAlibi, bool kSoftcap, bool kFast = false>
 __device__ __forceinline__ float score2(uint32_t raw, int c, float scale2, float slope2, float jf, float cap_in,
                                         float cap_out) {
   const float v = __uint_as_float(raw);
-  float y = kSoftcap ? (kFast ? cap_tanh(v * cap_in) : tanhf(v * cap_in)) * cap_out : v * scale2;
+  float y = kSoftcap ? (kFast ? SoftCap(cap_in, cap_out)(v, 0.f) : tanhf(v * cap_in) * cap_out) : v * scale2;
   if (kAlibi) y = fmaf(slope2, (float)c, fmaf(slope2, jf, y));
   return y;
 }
@@ -467,33 +489,19 @@ __device__ __forceinline__ float chunk_exp_plain2(const uint32_t (&v)[32], uint3
   return (a + b) + (cc + d);
 }
 
-// tanh(z) = z P(z^2) for |z| <= 1/2, within 2^-24: P of degree 4, fitted to
-// tanh(z) / z by iteratively reweighted least squares on z times the error.  No
-// special function, so that a soft-cap whose scores stay below half of it (the
-// usual case) leaves those units to the softmax's own exponentials.  A warp takes
-// it for 32 columns at a time where all of them are small enough: one sequence of
-// 32,768 tokens, 4,096 queries, 32 heads over 8 of 128, in 2.86 ms against 4.45 ms
-// by cap_tanh (which a cap of 2 on unit scores still takes), 1.70 ms without a cap.
-constexpr float kCapSmall = 0.5f;
-struct CapPoly {
-  uint64_t in, k[5];  // z = v * in; the coefficients times cap_out, in pairs
-  __device__ __forceinline__ CapPoly(float cap_in, float cap_out) {
-    constexpr float c[5] = {0.9999999403953552f, -0.3333277702331543f, 0.13320571184158325f, -0.05276213213801384f,
-                            0.016737567260861397f};
-    in = f2(cap_in, cap_in);
-#pragma unroll
-    for (int i = 0; i < 5; ++i) k[i] = f2(c[i] * cap_out, c[i] * cap_out);
-  }
-  // tanh(v * cap_in) * cap_out + add for a pair of raw scores.
-  __device__ __forceinline__ uint64_t operator()(uint64_t v, uint64_t add) const {
-    const uint64_t z = mul2(v, in), w = mul2(z, z);
-    uint64_t p = fma2(k[4], w, k[3]);
-    p = fma2(p, w, k[2]);
-    p = fma2(p, w, k[1]);
-    p = fma2(p, w, k[0]);
-    return fma2(z, p, add);
-  }
-};
+// Small scores need no special function, so that a soft-cap whose scores stay below
+// half of it (the usual case) leaves those units to the softmax's own exponentials.  A
+// warp takes 32 columns this way at a time where all of them are small enough: one
+// sequence of 32,768 tokens, 4,096 queries, 32 heads over 8 of 128, 2.96 ms against
+// 5.57 ms both ways (which a cap of 2 on unit scores still takes), 1.70 ms without a cap.
+__device__ __forceinline__ uint64_t SoftCap::small_pair(uint64_t v, uint64_t add) const {
+  const uint64_t z = mul2(v, f2(in, in)), w = mul2(z, z);
+  uint64_t p = fma2(f2(k[4], k[4]), w, f2(k[3], k[3]));
+  p = fma2(p, w, f2(k[2], k[2]));
+  p = fma2(p, w, f2(k[1], k[1]));
+  p = fma2(p, w, f2(k[0], k[0]));
+  return fma2(z, p, add);
+}
 // The largest size of 32 raw scores (a NaN does not count: it stays one in P too).
 __device__ __forceinline__ float chunk_size(const uint32_t (&v)[32]) {
   float m[4] = {0.f, 0.f, 0.f, 0.f};
@@ -502,16 +510,16 @@ __device__ __forceinline__ float chunk_size(const uint32_t (&v)[32]) {
     m[(c >> 1) & 3] = fmax3(m[(c >> 1) & 3], fabsf(__uint_as_float(v[c])), fabsf(__uint_as_float(v[c + 1])));
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
-// chunk_exp with such a soft-cap (masked ones are replaced after it).
+// chunk_exp with a soft-cap of small scores (masked ones are replaced after it).
 template <typename T, bool kMask>
 __device__ __forceinline__ float chunk_exp_cap(const uint32_t (&v)[32], uint32_t (&pk)[16], int c0, int lo, int hi,
-                                               const CapPoly &cap, float m) {
+                                               const SoftCap &cap, float m) {
   uint64_t acc0 = f2(0.f, 0.f), acc1 = f2(0.f, 0.f);
   const uint64_t nm = f2(-m, -m);
 #pragma unroll
   for (int c = 0; c < 32; c += 2) {
     float y0, y1;
-    f2_split(cap(f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), nm), y0, y1);
+    f2_split(cap.small_pair(f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), nm), y0, y1);
     if (kMask) {
       y0 = (c0 + c >= lo && c0 + c < hi) ? y0 : -CUDART_INF_F;
       y1 = (c0 + c + 1 >= lo && c0 + c + 1 < hi) ? y1 : -CUDART_INF_F;
@@ -590,7 +598,7 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, int n0, int kv_offset
     if constexpr (!kCol && !kSoftcap)
       psum += chunk_exp_plain2<T>(sr[q], pk, scale2, m_eff - off);
     else if (kFast && !kAlibi && __all_sync(0xffffffffu, chunk_size(sr[q]) * cap_in <= kCapSmall))
-      psum += chunk_exp_cap<T, kMaskPass>(sr[q], pk, q * 32, lo, hi, CapPoly(cap_in, cap_out), m_eff);
+      psum += chunk_exp_cap<T, kMaskPass>(sr[q], pk, q * 32, lo, hi, SoftCap(cap_in, cap_out), m_eff);
     else
       psum += chunk_exp<T, kCol, kSoftcap, kMaskPass, kFast>(sr[q], pk, q * 32, lo, hi, scale2, sl, jf, cap_in, cap_out,
                                                     m_eff - off);

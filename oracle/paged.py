@@ -7,7 +7,7 @@ import math
 import torch
 
 
-def attention(q, k, v, q_len, kv_len, *, sm_scale, causal=True, window=-1, cap=0.0, slopes=None):
+def attention(q, k, v, q_len, kv_len, *, sm_scale, causal=True, window=-1, cap=0.0, slopes=None, cap_relative=False):
     """One sequence: q [S, H, D], k and v [N, H_kv, D] (rows behind the lengths
     are not looked at).  Returns out [S, H, D], lse [H, S], weights [H_kv, N]
     and a bound for each, `out` without the rounding to its own type.
@@ -17,7 +17,8 @@ def attention(q, k, v, q_len, kv_len, *, sm_scale, causal=True, window=-1, cap=0
     smallest number below the normal range), fp32 sums of the products (2^-24 for
     each of the D terms and 2^-22 for each 16 tokens, whose sums the tensor core
     may cut instead of rounding), 2^-22 for the exponential, and 2^-23 of the
-    numbers that the score is made of."""
+    numbers that the score is made of.  A soft-cap adds 2^-21 of the cap, or with
+    cap_relative 2^-20 of the capped score."""
     S, H, D = q.shape
     N, Hkv = k.shape[0], k.shape[1]
     G = H // Hkv
@@ -54,7 +55,7 @@ def attention(q, k, v, q_len, kv_len, *, sm_scale, causal=True, window=-1, cap=0
         # Relative error of a weight before its rounding.
         d = (D + 8) * 2.0 ** -24 * mag + 2.0 ** -21 + 2.0 ** -22 * (mag + bias.abs() + top.abs())
         if cap > 0:
-            d = d + 2.0 ** -21 * cap
+            d = d + (2.0 ** -20 * (torch.tanh(raw / cap) * cap).abs() if cap_relative else 2.0 ** -21 * cap)
         d = torch.where(p > 0, d, 0.0)
         sums = 2.0 ** -22 * (kv_len / 16 + 8)
         dsum = (p * d).sum(-1, keepdim=True) + sums

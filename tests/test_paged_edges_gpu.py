@@ -8,7 +8,7 @@ import torch
 
 import llmx_b200
 from gpu_helpers import needs_cuda
-from paged_helpers import DEV, Case
+from paged_helpers import DEV, Case, check_attention, read
 
 pytestmark = [pytest.mark.gpu, needs_cuda]
 
@@ -128,3 +128,20 @@ def test_weights_and_lse_do_not_depend_on_v(dtype, d, algo, q_len):
             out, lse1 = c.run(algo=algo, weights=w1, decay=0.0, window=window)
             assert torch.equal(w0, w1) and torch.equal(lse0, lse1)
             assert out[0, -1, :2].isnan().flatten(1).any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("algo,q_len", [("decode", 1), ("decode", 4), ("decode", 40), ("tcgen05", 70)])
+@pytest.mark.parametrize("cap", [0.5, 50.0, 1e3, 1e4, 1e6])
+def test_a_soft_cap_keeps_the_bits_of_the_scores(dtype, algo, q_len, cap):
+    """A capped score is right to 2^-20 of itself, whatever the cap: its argument, the product
+    with the cap and the fit or the special functions each cost a few 2^-24 of it."""
+    for d, scale in ((64, 0.25), (128, 3.0)):  # scores of spread 2, and of 34, past a cap of 50
+        c = Case(dtype, d, 4, 2, 32, q_len, [300, 90], seed=q_len)
+        kw = dict(cap=cap, sm_scale=scale)
+        for slopes in (None, torch.tensor([0.1, 0.03, 0.01, 0.002])):
+            w = torch.zeros(c.k_cache.shape[:3], device=DEV)
+            out, lse = c.run(algo=algo, weights=w, decay=0.0, alibi_slopes=None if slopes is None else slopes.to(DEV), **kw)
+            for b, n in enumerate(c.lens):
+                want = c.want(b, slopes=slopes, cap_relative=True, **kw)
+                check_attention(out[b], lse[b], read(w.unsqueeze(-1), c.table, b, n)[..., 0].T, want, dtype, f"{b} {scale}")
