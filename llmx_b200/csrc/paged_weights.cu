@@ -309,38 +309,43 @@ __global__ void __launch_bounds__(kWThreads, 1)
             const int b0 = min(max(lo - ch * 32, 0), 32), b1 = min(max(hi - ch * 32, 0), 32);
             seen = (b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u) & ~(b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u);
           }
-          bool small = false;
-          const SoftCap cap(cap_in, cap_out);
-          if constexpr (kSoftcap) small = __all_sync(0xffffffffu, chunk_size(vc) * fabsf(cap_in) <= kCapSmall);  // any scale
+          // Adds the 32 columns up; kSmall: all scores are small for the soft-cap.
+          auto add_up = [&](auto kSmall) {
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 ad = ca[ch * 8 + c / 4];
-            float x[4] = {ad.x, ad.y, ad.z, ad.w};
-            if constexpr (kAlibi) {
-              const float4 sl = cs[ch * 8 + c / 4];
-              x[0] = fmaf(sl.x, kf, x[0]);
-              x[1] = fmaf(sl.y, kf, x[1]);
-              x[2] = fmaf(sl.z, kf, x[2]);
-              x[3] = fmaf(sl.w, kf, x[3]);
-            }
-            if (kSoftcap && small) {
-              f2_split(cap.small_pair(f2(__uint_as_float(vc[c]), __uint_as_float(vc[c + 1])), f2(x[0], x[1])), x[0], x[1]);
-              f2_split(cap.small_pair(f2(__uint_as_float(vc[c + 2]), __uint_as_float(vc[c + 3])), f2(x[2], x[3])), x[2], x[3]);
-            } else if constexpr (kSoftcap) {
+            for (int c = 0; c < 32; c += 4) {
+              const float4 ad = ca[ch * 8 + c / 4];
+              float x[4] = {ad.x, ad.y, ad.z, ad.w};
+              if constexpr (kAlibi) {
+                const float4 sl = cs[ch * 8 + c / 4];
+                x[0] = fmaf(sl.x, kf, x[0]);
+                x[1] = fmaf(sl.y, kf, x[1]);
+                x[2] = fmaf(sl.z, kf, x[2]);
+                x[3] = fmaf(sl.w, kf, x[3]);
+              }
+              const uint64_t v0 = f2(__uint_as_float(vc[c]), __uint_as_float(vc[c + 1]));
+              const uint64_t v1 = f2(__uint_as_float(vc[c + 2]), __uint_as_float(vc[c + 3]));
+              if constexpr (kSoftcap) {
+                const SoftCap cap(cap_in, cap_out);
+                f2_split(cap.template pair<decltype(kSmall)::value>(v0, f2(x[0], x[1])), x[0], x[1]);
+                f2_split(cap.template pair<decltype(kSmall)::value>(v1, f2(x[2], x[3])), x[2], x[3]);
+              } else {
+                const uint64_t sc = f2(scale2, scale2);
+                f2_split(fma2(v0, sc, f2(x[0], x[1])), x[0], x[1]);
+                f2_split(fma2(v1, sc, f2(x[2], x[3])), x[2], x[3]);
+              }
+              if (need_mask) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = cap(__uint_as_float(vc[c + e]), x[e]);
-            } else {
-              const uint64_t sc = f2(scale2, scale2);
-              f2_split(fma2(f2(__uint_as_float(vc[c]), __uint_as_float(vc[c + 1])), sc, f2(x[0], x[1])), x[0], x[1]);
-              f2_split(fma2(f2(__uint_as_float(vc[c + 2]), __uint_as_float(vc[c + 3])), sc, f2(x[2], x[3])), x[2], x[3]);
+                for (int e = 0; e < 4; ++e) x[e] = (seen & (1u << (c + e))) ? x[e] : -CUDART_INF_F;
+              }
+              acc0 = add2(acc0, f2(ex2_approx(x[0]), ex2_approx(x[1])));
+              acc1 = add2(acc1, f2(ex2_approx(x[2]), ex2_approx(x[3])));
             }
-            if (need_mask) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = (seen & (1u << (c + e))) ? x[e] : -CUDART_INF_F;
-            }
-            acc0 = add2(acc0, f2(ex2_approx(x[0]), ex2_approx(x[1])));
-            acc1 = add2(acc1, f2(ex2_approx(x[2]), ex2_approx(x[3])));
-          }
+          };
+          // (By size: the scale may be negative.)
+          if (kSoftcap && !__all_sync(0xffffffffu, chunk_size(vc) * fabsf(cap_in) <= kCapSmall))
+            add_up(std::false_type{});
+          else
+            add_up(std::true_type{});
         }
       }
       block += blocks;

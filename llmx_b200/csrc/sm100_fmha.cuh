@@ -342,13 +342,16 @@ struct SoftCap {
     p = fmaf(p, w, k[2]);
     p = fmaf(p, w, k[1]);
     p = fmaf(p, w, k[0]);
+    return fabsf(z) <= kCapSmall ? fmaf(z, p, add) : large(z, add);
+  }
+  // The same bits for a pair of raw scores; kSmall: both are (|v * in| <= 1/2).
+  template <bool kSmall>
+  __device__ __forceinline__ uint64_t pair(uint64_t v, uint64_t add) const;
+  __device__ __forceinline__ float large(float z, float add) const {
     float u;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(u) : "f"(ex2_approx(fabsf(z) * (2.f * kLog2e)) + 1.f));
-    const float large = fmaf(copysignf(fmaf(-2.f, u, 1.f), z), out, add);
-    return fabsf(z) <= kCapSmall ? fmaf(z, p, add) : large;
+    return fmaf(copysignf(fmaf(-2.f, u, 1.f), z), out, add);
   }
-  // The same bits for a pair of raw scores that are both small (|v * in| <= 1/2).
-  __device__ __forceinline__ uint64_t small_pair(uint64_t v, uint64_t add) const;
 };
 
 // Score of column c (0..127 inside the block) in log2 units, before masking.
@@ -491,16 +494,24 @@ __device__ __forceinline__ float chunk_exp_plain2(const uint32_t (&v)[32], uint3
 
 // Small scores need no special function, so that a soft-cap whose scores stay below
 // half of it (the usual case) leaves those units to the softmax's own exponentials.  A
-// warp takes 32 columns this way at a time where all of them are small enough: one
-// sequence of 32,768 tokens, 4,096 queries, 32 heads over 8 of 128, 2.96 ms against
-// 5.57 ms both ways (which a cap of 2 on unit scores still takes), 1.70 ms without a cap.
-__device__ __forceinline__ uint64_t SoftCap::small_pair(uint64_t v, uint64_t add) const {
+// warp takes 32 columns this way at a time where all of them are small enough, which
+// decides the time only, no bit (the columns may be of rows or tokens that count for
+// nothing): one sequence of 32,768 tokens, 4,096 queries, 32 heads over 8 of 128, 2.85 ms
+// against 4.95 ms (which a cap of 2 on unit scores still takes), 1.73 ms without a cap.
+template <bool kSmall>
+__device__ __forceinline__ uint64_t SoftCap::pair(uint64_t v, uint64_t add) const {
   const uint64_t z = mul2(v, f2(in, in)), w = mul2(z, z);
   uint64_t p = fma2(f2(k[4], k[4]), w, f2(k[3], k[3]));
   p = fma2(p, w, f2(k[2], k[2]));
   p = fma2(p, w, f2(k[1], k[1]));
   p = fma2(p, w, f2(k[0], k[0]));
-  return fma2(z, p, add);
+  p = fma2(z, p, add);
+  if constexpr (kSmall) return p;
+  float z0, z1, p0, p1, a0, a1;
+  f2_split(z, z0, z1);
+  f2_split(p, p0, p1);
+  f2_split(add, a0, a1);
+  return f2(fabsf(z0) <= kCapSmall ? p0 : large(z0, a0), fabsf(z1) <= kCapSmall ? p1 : large(z1, a1));
 }
 // The largest size of 32 raw scores (a NaN does not count: it stays one in P too).
 __device__ __forceinline__ float chunk_size(const uint32_t (&v)[32]) {
@@ -510,8 +521,8 @@ __device__ __forceinline__ float chunk_size(const uint32_t (&v)[32]) {
     m[(c >> 1) & 3] = fmax3(m[(c >> 1) & 3], fabsf(__uint_as_float(v[c])), fabsf(__uint_as_float(v[c + 1])));
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
-// chunk_exp with a soft-cap of small scores (masked ones are replaced after it).
-template <typename T, bool kMask>
+// chunk_exp with a soft-cap (masked ones are replaced after it).
+template <typename T, bool kMask, bool kSmall>
 __device__ __forceinline__ float chunk_exp_cap(const uint32_t (&v)[32], uint32_t (&pk)[16], int c0, int lo, int hi,
                                                const SoftCap &cap, float m) {
   uint64_t acc0 = f2(0.f, 0.f), acc1 = f2(0.f, 0.f);
@@ -519,7 +530,7 @@ __device__ __forceinline__ float chunk_exp_cap(const uint32_t (&v)[32], uint32_t
 #pragma unroll
   for (int c = 0; c < 32; c += 2) {
     float y0, y1;
-    f2_split(cap.small_pair(f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), nm), y0, y1);
+    f2_split(cap.pair<kSmall>(f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), nm), y0, y1);
     if (kMask) {
       y0 = (c0 + c >= lo && c0 + c < hi) ? y0 : -CUDART_INF_F;
       y1 = (c0 + c + 1 >= lo && c0 + c + 1 < hi) ? y1 : -CUDART_INF_F;
@@ -597,9 +608,12 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, int n0, int kv_offset
     uint32_t pk[16];
     if constexpr (!kCol && !kSoftcap)
       psum += chunk_exp_plain2<T>(sr[q], pk, scale2, m_eff - off);
-    else if (kFast && !kAlibi && __all_sync(0xffffffffu, chunk_size(sr[q]) * cap_in <= kCapSmall))
-      psum += chunk_exp_cap<T, kMaskPass>(sr[q], pk, q * 32, lo, hi, SoftCap(cap_in, cap_out), m_eff);
-    else
+    else if constexpr (kFast && !kAlibi) {
+      const SoftCap cap(cap_in, cap_out);
+      psum += __all_sync(0xffffffffu, chunk_size(sr[q]) * cap_in <= kCapSmall)
+                  ? chunk_exp_cap<T, kMaskPass, true>(sr[q], pk, q * 32, lo, hi, cap, m_eff)
+                  : chunk_exp_cap<T, kMaskPass, false>(sr[q], pk, q * 32, lo, hi, cap, m_eff);
+    } else
       psum += chunk_exp<T, kCol, kSoftcap, kMaskPass, kFast>(sr[q], pk, q * 32, lo, hi, scale2, sl, jf, cap_in, cap_out,
                                                     m_eff - off);
     tmem_st16(tS + q * 16, pk);

@@ -145,3 +145,28 @@ def test_a_soft_cap_keeps_the_bits_of_the_scores(dtype, algo, q_len, cap):
             for b, n in enumerate(c.lens):
                 want = c.want(b, slopes=slopes, cap_relative=True, **kw)
                 check_attention(out[b], lse[b], read(w.unsqueeze(-1), c.table, b, n)[..., 0].T, want, dtype, f"{b} {scale}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,heads", [(64, 14), (128, 14), (256, 6), (128, 8)])
+@pytest.mark.parametrize("scale", [1.0, -1.0])
+def test_soft_capped_bits_do_not_depend_on_what_no_row_sees(dtype, d, heads, scale):
+    """Padded rows of q, the rest of a sequence's last page and whatever ran before:
+    groups that do not divide 128 leave rows of a tile unused."""
+    c = Case(dtype, d, heads, 2, 64, 50, [333, 70, 50], q_lens=[50, 33, 7], seed=heads)
+    algos = ("auto", "tcgen05") if scale > 0 else ("decode",)
+    for algo in algos:
+        for kw in (dict(cap=8.0), dict(cap=30.0, window=90), dict(cap=4.0, causal=False)):
+            first = None
+            for junk in (0.0, 3.0, -1000.0, math.nan, math.inf):
+                for b, n in enumerate(c.q_lens):
+                    c.q[b, n:] = junk
+                c.k_cache.fill_(junk), c.v_cache.fill_(junk)
+                for b in range(3):
+                    c.put(b)
+                w = torch.zeros(c.k_cache.shape[:3], device=DEV)
+                out, lse = c.run(algo=algo, weights=w, decay=0.0, sm_scale=scale * d ** -0.5, **kw)
+                if first is None:
+                    first = out, lse, w
+                for x, y in zip(first, (out, lse, w)):
+                    assert torch.equal(x, y), (algo, kw, junk)
