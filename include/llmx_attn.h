@@ -434,7 +434,8 @@ LLMX_API llmx_status llmx_paged_attn_fwd(const llmx_attn_params *p, const llmx_p
  * budget) tokens are kept that are
  *   the first `sinks`, the last `recent`, and of the others those of the
  *   largest key_weights (of equal ones the earliest; a NaN counts as -inf),
- * in their order.  Their rows of K, V and key_weights become tokens 0 .. n - 1
+ * in their order.  (A token whose page lies outside the cache ranks as -inf and, if
+ * kept, becomes zeros with weight 0.)  Their rows of K, V and key_weights become tokens 0 .. n - 1
  * of the pages of out_table[b] (NULL: of the sequence's own pages, in place;
  * sequences must then share no page).  With an out_table its pages must hold
  * no token that the call reads, and share none with one another.  kept [batch, n_kv_heads,

@@ -398,22 +398,25 @@ struct MoveArgs {
   int col_ctas;  // CTAs along the columns of K and V; the first has the weights too
 };
 
-// Where a row comes from and goes to (pages; -1 for neither: it stays).
+// Where a row comes from and goes to: pages; from kStays: nothing is written, from
+// kZeros: it lay outside the cache, where rows read as zeros.
+constexpr int kStays = -1, kZeros = -2;
 struct MovePlace {
   int from, from_row, to, to_row;
 };
 __device__ __forceinline__ MovePlace move_place(const PagedArgs &a, const EvictArgs &e, int b, const int *kept, int r, int hi) {
-  MovePlace p{-1, 0, -1, 0};
+  MovePlace p{kStays, 0, -1, 0};
   if (r >= hi) return p;
   const int j = kept[r];
   if (j < 0 || (e.out_table == nullptr && j == r)) return p;
   const int from_slot = j / a.page_size, to_slot = r / a.page_size;
   p.from = paged_page(a, b, from_slot);
+  if (p.from < 0) p.from = kZeros;
   p.from_row = j - from_slot * a.page_size;
   p.to = e.out_table == nullptr ? paged_page(a, b, to_slot)
                                 : paged_page(a, e.out_table, e.out_stride, e.out_pages, b, to_slot);
   p.to_row = r - to_slot * a.page_size;
-  if (p.to < 0) p.from = -1;
+  if (p.to < 0) p.from = kStays;
   return p;
 }
 
@@ -430,9 +433,9 @@ struct MoveBatch {
     w_to = nullptr;
     if (col == 0 && i0 == 0 && tid < m.batch) {
       const MovePlace p = places[tid];
-      if (p.from >= 0) {
+      if (p.from != kStays) {
         float *const w = a.w + h * a.ws[1];
-        wx = w[p.from * a.ws[0] + p.from_row];
+        wx = p.from >= 0 ? w[p.from * a.ws[0] + p.from_row] : 0.f;
         w_to = w + p.to * a.ws[0] + p.to_row;
       }
     }
@@ -444,10 +447,10 @@ struct MoveBatch {
       const int c = col * m.pieces + (i & (m.pieces - 1));
       const bool is_v = (i >> log_p) & 1;
       const MovePlace p = places[i >> (log_p + 1)];
-      if (p.from < 0) continue;
+      if (p.from == kStays) continue;
       const long long *st = is_v ? a.vs : a.ks;
       uint4 *const head = static_cast<uint4 *>(is_v ? a.v : a.k) + h * (st[1] / 8) + c;
-      x[u] = head[p.from * (st[0] / 8) + p.from_row * (st[2] / 8)];
+      x[u] = p.from >= 0 ? head[p.from * (st[0] / 8) + p.from_row * (st[2] / 8)] : make_uint4(0u, 0u, 0u, 0u);
       to[u] = head + p.to * (st[0] / 8) + p.to_row * (st[2] / 8);
     }
   }

@@ -8,7 +8,9 @@ import torch
 
 import llmx_b200
 from gpu_helpers import needs_cuda
-from paged_helpers import DEV, Case, check_attention, read
+from llmx_b200 import LlmxError
+from oracle import paged as opaged
+from paged_helpers import DEV, Case, check_attention, ints, place, read, table_of
 
 pytestmark = [pytest.mark.gpu, needs_cuda]
 
@@ -170,3 +172,47 @@ def test_soft_capped_bits_do_not_depend_on_what_no_row_sees(dtype, d, heads, sca
                     first = out, lse, w
                 for x, y in zip(first, (out, lse, w)):
                     assert torch.equal(x, y), (algo, kw, junk)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 256)])
+def test_evicted_tokens_of_pages_outside_the_cache_are_zeros(in_place, dtype, d):
+    """A kept token whose page lies outside the cache becomes a row of zeros with weight 0."""
+    page, lens, budget, recent, sinks = 16, [100, 40, 70], 50, 20, 18
+    gen = torch.Generator().manual_seed(d)
+    table, n_pages = table_of(lens, page, 1, gen)
+    need = -(-budget // page)
+    kc, vc = (torch.full((n_pages + 3 * need, 2, page, d), 7.0, dtype=dtype, device=DEV) for _ in range(2))
+    w = torch.full(kc.shape[:3], 7.0, device=DEV)
+    data = []
+    for b, n in enumerate(lens):
+        k, v = (torch.randn(n, 2, d, generator=gen).to(dtype) for _ in range(2))
+        x = torch.rand(n, 2, 1, generator=gen) + 1
+        place(kc, table, b, k), place(vc, table, b, v), place(w.unsqueeze(-1), table, b, x)
+        data.append((k, v, x[..., 0]))
+    # the second page of the first sequence (sinks), its fifth (recent), one of a
+    # sequence that is kept whole, and one of neither in the third
+    table[0, 1], table[0, 5], table[1, 2], table[2, 1] = n_pages + 999, -1, 2 ** 31 - 1, -2 ** 31
+    out = (n_pages + torch.randperm(3 * need, generator=gen)).view(3, need).int()
+    kept, new = llmx_b200.paged_evict(kc, vc, w, budget, kv_lens=ints(lens), block_table=table.to(DEV), recent=recent, sinks=sinks,
+                                      **({} if in_place else {"out_table": out.to(DEV)}))
+    with pytest.raises(LlmxError):
+        llmx_b200.device_status(0)
+    llmx_b200.device_status(0)
+    for b, n in enumerate(lens):
+        k, v, x = data[b]
+        outside = torch.tensor([not 0 <= int(p) < kc.shape[0] for p in table[b]])
+        gone = outside[torch.arange(n) // page]
+        ranked = torch.where(gone[:, None], torch.tensor(-math.inf), x)
+        m = min(n, budget)
+        assert int(new[b]) == m
+        for h in range(2):
+            want = opaged.kept(ranked[:, h], n, budget, recent, sinks)
+            assert kept[b, h, :m].tolist() == want
+            for r, j in enumerate(want):
+                to = int((table if in_place else out)[b, r // page])
+                if not 0 <= to < kc.shape[0]:
+                    continue  # the place itself lies outside
+                for got, src in ((kc, k), (vc, v), (w, x)):
+                    expect = torch.zeros_like(src[j, h]) if gone[j] else src[j, h]
+                    assert torch.equal(got[to, h, r % page].cpu(), expect), (b, h, r, j)
