@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const PagedAr
   const int n = min(L, e.budget);
   int *kept = e.kept + ((long long)b * a.Hkv + h) * e.budget;
   const int at = rank * kSelThreads + tid, all = ranks * kSelThreads;
-  for (int i = n + at; i < e.budget; i += all) kept[i] = -1;
+  for (unsigned i = n + at; i < (unsigned)e.budget; i += all) kept[i] = -1;  // budget may be 2^31 - 1: i does not wrap
   if (L <= e.budget) {  // the same in all CTAs of the cluster
     for (int i = at; i < n; i += all) kept[i] = i;
     return;

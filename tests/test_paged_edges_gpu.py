@@ -216,3 +216,20 @@ def test_evicted_tokens_of_pages_outside_the_cache_are_zeros(in_place, dtype, d)
                 for got, src in ((kc, k), (vc, v), (w, x)):
                     expect = torch.zeros_like(src[j, h]) if gone[j] else src[j, h]
                     assert torch.equal(got[to, h, r % page].cpu(), expect), (b, h, r, j)
+
+
+@pytest.mark.parametrize("seqs", [1, 2])
+def test_the_largest_budget_stays_inside_kept(seqs):
+    """-1 behind the kept positions up to a budget of 2^31 - 1, and nothing in front of it."""
+    page, budget, front = 16, 2 ** 31 - 1, 65536
+    kc, vc = (torch.zeros(4 * seqs, 1, page, 64, dtype=torch.float16, device=DEV) for _ in range(2))
+    w = torch.zeros(4 * seqs, 1, page, device=DEV)
+    buf = torch.full((front + seqs * budget,), 5, dtype=torch.int32, device=DEV)
+    kept = buf[front:].view(seqs, 1, budget)
+    lens = [50, 3][:seqs]
+    llmx_b200.paged_evict(kc, vc, w, budget, kv_lens=ints(lens), kept=kept)
+    assert (buf[:front] == 5).all()
+    for b, n in enumerate(lens):
+        assert kept[b, 0, :n].tolist() == list(range(n))
+        assert int(kept[b, 0, n:].max()) == -1 and int(kept[b, 0, n:].min()) == -1
+    llmx_b200.device_status(0)
