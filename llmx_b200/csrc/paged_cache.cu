@@ -69,12 +69,13 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const PagedA
   const int pieces = a.Hkv * per_head;
   for (int b = blockIdx.y; b < r.B; b += gridDim.y) {
     const int n = clamp_len(r.lens, b, r.rows);
-    const int lo = blockIdx.x * tokens, hi = min(n, lo + tokens);
-    if (lo >= hi) continue;
+    const long long from = (long long)blockIdx.x * tokens;  // rows may end at 2^31 - 1
+    if (from >= n) continue;
+    const int lo = (int)from, hi = lo + min(n - lo, tokens);
     const long long first = r.start != nullptr ? r.start[b] : 0;
     __syncthreads();  // the places of the sequence before have been read
     if (threadIdx.x < hi - lo) {
-      const long long j = first + lo + threadIdx.x;
+      const long long j = first + lo + (int)threadIdx.x;
       int2 p = make_int2(-1, 0);
       if (j >= 0 && j <= INT_MAX) {
         const int slot = (int)j / a.page_size;
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const PagedA
           if (at.x >= 0) {
             kd[u] = at.x * a.ks[0] + h * a.ks[1] + at.y * a.ks[2] + c;
             vd[u] = at.x * a.vs[0] + h * a.vs[1] + at.y * a.vs[2] + c;
-            const long long row = lo + t;
+            const long long row = (long long)lo + t;
             x[u] = *reinterpret_cast<const Piece *>(static_cast<const uint16_t *>(r.k) + b * r.ks[0] + row * r.ks[1] +
                                                     h * r.ks[2] + c);
             y[u] = *reinterpret_cast<const Piece *>(static_cast<const uint16_t *>(r.v) + b * r.vs[0] + row * r.vs[1] +
@@ -128,7 +129,7 @@ cudaError_t launch_store(const PagedArgs &a, const StoreArgs &r, bool vec, int n
   const long long pieces = (long long)a.Hkv * a.D / (vec ? 8 : 1);
   // One round of kUnroll pieces a thread, and at least one token.
   const int tokens = (int)std::max<long long>(1, std::min<long long>(std::min(r.rows, kStoreTokens), kStoreThreads * 4 / pieces));
-  const dim3 grid((r.rows + tokens - 1) / tokens, std::min(r.B, 65535));
+  const dim3 grid((unsigned)(((long long)r.rows + tokens - 1) / tokens), std::min(r.B, 65535));
   if (vec)
     paged_store_kernel<true><<<grid, kStoreThreads, 0, s>>>(a, r, tokens);
   else

@@ -8,7 +8,7 @@ import torch
 
 import llmx_b200
 from gpu_helpers import needs_cuda
-from llmx_b200 import LlmxError
+from llmx_b200 import LlmxError, paged
 from oracle import paged as opaged
 from paged_helpers import DEV, Case, check_attention, ints, place, read, table_of
 
@@ -232,4 +232,17 @@ def test_the_largest_budget_stays_inside_kept(seqs):
     for b, n in enumerate(lens):
         assert kept[b, 0, :n].tolist() == list(range(n))
         assert int(kept[b, 0, n:].max()) == -1 and int(kept[b, 0, n:].min()) == -1
+    llmx_b200.device_status(0)
+
+
+@pytest.mark.parametrize("rows", [2 ** 31 - 1, 2 ** 31 - 64, 2 ** 31 - 65])
+def test_store_of_row_counts_near_2_31(rows):
+    """Rows that are all one row (stride 0), of which lens takes a few."""
+    kc, vc = (torch.zeros(4, 1, 16, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    k = torch.randn(1, 1, 1, 64, device=DEV).bfloat16()
+    for call in (llmx_b200.paged_store, paged.paged_store_ctypes):
+        kc.zero_(), vc.zero_()
+        call(kc, vc, k.expand(1, rows, 1, 64), (-k).expand(1, rows, 1, 64), start=ints([3]), lens=ints([40]))
+        got = kc.view(64, 64)
+        assert (got[3:43] == k.view(64)).all() and not got[:3].any() and not got[43:].any() and torch.equal(vc, -kc)
     llmx_b200.device_status(0)
