@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const PagedA
     // is at most 2^31 - 1 (launch_store).
     const int total = (hi - lo) * pieces;
     int t = threadIdx.x / pieces, p = threadIdx.x - t * pieces;  // of this thread's next piece
+    const int dt = kStoreThreads / pieces, dp = kStoreThreads - dt * pieces;  // and how far the one after it is
     for (int base = threadIdx.x; base < total; base += kStoreThreads * kUnroll) {
       Piece x[kUnroll], y[kUnroll];
       long long kd[kUnroll], vd[kUnroll];
@@ -109,8 +110,9 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const PagedA
                                                     h * r.vs[2] + c);
           }
         }
-        p += kStoreThreads;
-        while (p >= pieces) {
+        t += dt;
+        p += dp;
+        if (p >= pieces) {
           p -= pieces;
           ++t;
         }
@@ -125,7 +127,7 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const PagedA
   }
 }
 
-cudaError_t launch_store(const PagedArgs &a, const StoreArgs &r, bool vec, int num_sms, cudaStream_t s) {
+cudaError_t launch_store(const PagedArgs &a, const StoreArgs &r, bool vec, cudaStream_t s) {
   const long long pieces = (long long)a.Hkv * a.D / (vec ? 8 : 1);
   // One round of kUnroll pieces a thread, and at least one token.
   const int tokens = (int)std::max<long long>(1, std::min<long long>(std::min(r.rows, kStoreTokens), kStoreThreads * 4 / pieces));
@@ -667,7 +669,7 @@ extern "C" llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv
   int sms = 0;
   st = current_device_info(&k.err, &sms);
   if (st != LLMX_OK) return st;
-  const cudaError_t e = launch_store(k, r, vec, sms, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_store(k, r, vec, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? LLMX_OK : record_error(LLMX_ERR_CUDA, cudaGetErrorString(e));
 }
 
