@@ -423,8 +423,11 @@ LLMX_API llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv4_
  * share a page leave either's weights there.
  *   A call given too little workspace for its partial results runs without
  * splitting sequences; with key_weights it is refused
- * (LLMX_ERR_WORKSPACE_TOO_SMALL).  Calls that share a workspace must not
- * overlap on the GPU. */
+ * (LLMX_ERR_WORKSPACE_TOO_SMALL).  The workspace then also holds the scores of
+ * calls with up to 32 (row, head) pairs a kv head, up to 1 GiB, and of calls
+ * with more than 128 query heads a kv head or a q of stride 0, where more than
+ * 16 GiB are refused (LLMX_ERR_UNSUPPORTED).  Calls that share a workspace must
+ * not overlap on the GPU. */
 LLMX_API llmx_status llmx_paged_attn_workspace_size(const llmx_attn_params *p, const llmx_paged_cache *c,
                                                     size_t *bytes);
 LLMX_API llmx_status llmx_paged_attn_fwd(const llmx_attn_params *p, const llmx_paged_cache *c, float decay,
@@ -434,13 +437,14 @@ LLMX_API llmx_status llmx_paged_attn_fwd(const llmx_attn_params *p, const llmx_p
  * budget) tokens are kept that are
  *   the first `sinks`, the last `recent`, and of the others those of the
  *   largest key_weights (of equal ones the earliest; a NaN counts as -inf),
- * in their order.  (A token whose page lies outside the cache ranks as -inf and, if
- * kept, becomes zeros with weight 0.)  Their rows of K, V and key_weights become tokens 0 .. n - 1
- * of the pages of out_table[b] (NULL: of the sequence's own pages, in place;
- * sequences must then share no page).  With an out_table its pages must hold
- * no token that the call reads, and share none with one another.  kept [batch, n_kv_heads,
- * budget] gets their former positions (-1 behind n), new_lens[b] = n; it may
- * be kv_lens itself.  Nothing else of the cache changes.  No workspace. */
+ * in their order.  (A token whose page lies outside the cache ranks as -inf
+ * and, if kept, becomes zeros with weight 0.)  Their rows of K, V and
+ * key_weights become tokens 0 .. n - 1 of the pages of out_table[b] (NULL: of
+ * the sequence's own pages, in place; sequences must then share no page).  With
+ * an out_table its pages must hold no token that the call reads, and share none
+ * with one another.  kept [batch, n_kv_heads, budget] gets their former
+ * positions (-1 behind n), new_lens[b] = n; it may be kv_lens itself.  Nothing
+ * else of the cache changes.  No workspace. */
 typedef struct llmx_paged_evict_params {
   int32_t batch;
   int32_t budget;            /* >= 1, >= sinks + recent                   */

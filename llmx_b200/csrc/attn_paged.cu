@@ -1161,7 +1161,10 @@ struct Plan {
 // and token (at 32 rows as much as K itself at head_dim 128), if that takes at
 // most 1 GiB; otherwise they are computed again.
 constexpr int kScoreRows = 32;
-constexpr size_t kScoreBytes = size_t(1) << 30;
+constexpr double kScoreBytes = double(1 << 30);
+// Where they cannot be (more than 128 query heads a kv head, a q that is expanded) all are
+// kept, as long as a tenth of the device's memory holds them.
+constexpr double kMostScoreBytes = 16 * kScoreBytes;
 
 llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs &k, Plan *plan) {
   const bool can = paged_tc_supports(a);
@@ -1176,9 +1179,14 @@ llmx_status choose(const llmx_attn_params *p, const AttnArgs &a, const PagedArgs
     plan->stat_at = kCounterBytes + plan->tcp.part_bytes;
     plan->bytes = plan->stat_at + (weights ? (size_t)a.B * a.Hkv * R * sizeof(float) : 0);
   } else {
-    plan->step = plan_step(a, weights, weights);
-    plan->again = weights && (R > kScoreRows || plan->step.score_bytes > kScoreBytes) && paged_weights_supports(a);
-    if (plan->again) plan->step.score_bytes = 0;
+    // (In floating point: the number of scores may pass 64 bits.)
+    const double kept = 4.0 * a.B * a.Hkv * (double)R * (((double)a.Skv + 15) / 16 * 16);
+    plan->again = weights && (R > kScoreRows || kept > kScoreBytes) && paged_weights_supports(a);
+    if (weights && !plan->again && kept > kMostScoreBytes)
+      return record_error(LLMX_ERR_UNSUPPORTED,
+                          "paged attention: key weights with more than 128 query heads a kv head, or of an expanded q, keep "
+                          "every score, and this call's would pass 16 GiB");
+    plan->step = plan_step(a, weights, weights && !plan->again);
     plan->stat_at = plan->step.part_bytes;
     plan->bytes = plan->step.part_bytes + plan->step.stat_bytes + plan->step.score_bytes;
   }
