@@ -52,6 +52,10 @@ namespace {
 // 128: this 69 / 75 / 118 / 120 / 202, tiles 84 at all; one of 32768: 48 / 48 / 58 / 56 /
 // 93, 50 / 52 / 52 / 54 / 56; 4 of 4096 at head_dim 256: 50 / 50 / 54 / 54 / 75, 51 / 53 /
 // 55 / 55 / 59; 16 of 2048 at 256: 77 / 81 / 89 / 93 / 142, 69 at all.
+//   Above that this form is taken where it is asked for and where tiles cannot be (a scale
+// that is not positive, an expanded q, more than 128 heads a kv head).  At head_dim 256 a
+// block then has 64 rows, else 32 (whose code and ring suit 64 and 128 better): one of 32768
+// tokens, 64 rows, 61 us against 70 in two blocks of 32, 16 of 2048 58 against 65.
 constexpr int kStepRows = 32;
 constexpr size_t kCounterBytes = 256;
 
@@ -75,7 +79,9 @@ struct StepWork {
 
 // Row block rb of sequence b: blocks of 128 tokens lo128 + 128 i .., tokens in
 // [lo, hi) are visible to some row.  A unit's steps are its blocks and, before
-// them, kUnitSteps that stand for what starting and ending a unit costs.
+// them, kUnitSteps that stand for what starting and ending a unit costs (us for 0 / 1 / 2 /
+// 4 of them: 128 sequences of 1-600 tokens 74 / 63 / 61 / 61, three of 9000 among 21 of 100
+// 57 / 47 / 43 / 41; sequences of equal lengths take the same time with any).
 constexpr int kUnitSteps = 2;
 struct Span {
   int ql, kl, lo, hi, all_lo, all_hi;
@@ -1093,6 +1099,8 @@ cudaError_t launch_step(const AttnArgs &a, const PagedArgs &c, const StepPlan &p
   wk.R = a.Sq * a.group;
   wk.nrb = (wk.R + p.rows - 1) / p.rows;
   wk.workers = p.workers;
+  // A share's least length: of 2 / 4 / 8 / 16 steps one sequence of 300 tokens takes 16 / 18 /
+  // 25 / 35 us, one of 8192 25 / 23 / 27 / 33; 64 of 300 and longer batches take the same time.
   wk.min_steps = 2 + kUnitSteps;
   wk.split = p.split;
   wk.reverse = a.alibi != nullptr;
@@ -1159,7 +1167,11 @@ struct Plan {
 
 // Key weights: the scores of a few rows are kept, 8 bytes written and read a row
 // and token (at 32 rows as much as K itself at head_dim 128), if that takes at
-// most 1 GiB; otherwise they are computed again.
+// most 1 GiB; otherwise they are computed again.  Kept / again, us, 32 heads on 8 of 128: 16
+// sequences of 4096 tokens, 4 rows 75 / 118, 32 rows 103 / 129, 64 rows 180 / 170; one of
+// 32768, 4 rows 51 / 76, 32 rows 72 / 78, 48 rows 97 / 87; three of 300-900, 16 rows 29 / 31,
+// 32 rows 37 / 31.  The 1 GiB is for the memory's sake: 256 of 16384, 32 rows, 4 GiB of
+// scores, take 4.42 ms kept and 5.70 again.
 constexpr int kScoreRows = 32;
 constexpr double kScoreBytes = double(1 << 30);
 // Where they cannot be (more than 128 query heads a kv head, a q that is expanded) all are

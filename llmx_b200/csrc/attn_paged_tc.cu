@@ -117,6 +117,12 @@ static_assert(sizeof(PBars) <= 1024, "barriers");
 // 1.5 for the merge, as it writes and reads 128 KB of it.  `share` is the items' mean
 // length over the longest's.  The launch ends with its last wave, or, as the pieces
 // are dealt as CTAs come free, a part of a piece after its mean.
+//   What the choice by this cost is worth, us, 32 heads on 8 of 128, against the best of 1 to
+// 64 pieces for each shape / uncut: 64 queries on each of 16 x 4,096 tokens 87, 82 / 80; 16 x
+// 8,192 151, 143 / 148; 32,768 among fifteen of 300 113, 99 / 490; 8 of 1,000-9,000 83, 75 /
+// 133; 32 of those 226, 214 / 252; one sequence of 32,768 with 10 queries 51, 51 / 476, with
+// 512 276, 276 / 493; of 131,072 with 16 130, 139 / 1,820; 400 queries on 700, 2,000 and 5,000,
+// 16 heads on 4 of 64, 74, 63 / 82; 128 on 300-4,000, 16 heads on 8 of 256, 58, 52 / 76.
 __host__ __device__ __forceinline__ float cut_cost(float nb, float s, float items, float share, float per_sm) {
   const float n = items * (1.f - share + share * s) * per_sm;  // pieces of an SM
   const float piece = ceilf(nb / s) + 3.f;
@@ -963,7 +969,10 @@ PagedTcPlan plan_paged_tc(const AttnArgs &a, bool have_ws) {
   p.piece = nb;
   if (have_ws) {
     // Of equal lengths only the items of the last, part-filled wave are cut; with
-    // lengths that only the device knows all of them, where they are few.
+    // lengths that only the device knows all of them, where they are few: below four waves.
+    // Above, us, uncut / cut: 64 queries on each of 80 sequences of 1,000-9,000 tokens 537 /
+    // 605, on 160 of 500-5,000 543 / 539, but one of 32,768 among 99 of 300 519 / 236, which
+    // a host that does not know the lengths cannot tell from the first.
     const bool ragged = a.B > 1 && (a.kv_lens != nullptr || a.q_lens != nullptr);
     const int cut = ragged ? (items < 4 * sms ? items : 0) : items % sms;
     const int most = std::min(64, std::max(1, nb / 4));

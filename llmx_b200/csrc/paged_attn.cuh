@@ -12,9 +12,6 @@
 
 namespace llmx_b200 {
 
-
-
-
 // The tokens [lo, hi) that query row i of a sequence sees (empty: lo >= hi).
 struct Visible {
   int lo, hi;

@@ -149,7 +149,9 @@ struct EvictArgs {
   int *kept, *new_lens;
 };
 
-constexpr int kSelHeld = 16384;  // weights of a CTA held in shared memory; more are read again in each round
+// Weights of a CTA held in shared memory; more are read again in each round (one sequence
+// of 131072 tokens, all held by its eight CTAs, to 16384: 57 us; of 262144, half held: 117 us).
+constexpr int kSelHeld = 16384;
 
 // The image of a weight under which unsigned order is the order of the
 // weights: the sign bit flipped, or all bits of negative ones.  -0 counts as 0
@@ -526,9 +528,11 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const PagedArg
 cudaError_t launch_evict(const PagedArgs &a, const EvictArgs &e, int num_sms, cudaStream_t s) {
   const long long units = (long long)e.B * a.Hkv;
   // CTAs of a cluster: enough that the weights stay in shared memory, and as
-  // many as keep the machine busy when there are few units.
+  // many as keep the machine busy when there are few units, with 4096 weights each or more
+  // (eight heads, with 1024 or more / 4096 or more / one CTA where it holds all, us: 4096
+  // tokens 22 / 20 / 20, 16384 29 / 27 / 37; 32 heads of 2048 25 / 20 / 20).
   int ranks = 1;
-  while (ranks < 8 && (e.max_kv > ranks * kSelHeld || (units * ranks * 2 <= num_sms && e.max_kv > ranks * 1024)))
+  while (ranks < 8 && (e.max_kv > ranks * kSelHeld || (units * ranks * 2 <= num_sms && e.max_kv > ranks * 4096)))
     ranks *= 2;
   const int per = ((e.max_kv + ranks - 1) / ranks + 3) & ~3;
   const size_t smem = (size_t)std::min(per, kSelHeld) * 4;
