@@ -246,3 +246,14 @@ def test_store_of_row_counts_near_2_31(rows):
         got = kc.view(64, 64)
         assert (got[3:43] == k.view(64)).all() and not got[:3].any() and not got[43:].any() and torch.equal(vc, -kc)
     llmx_b200.device_status(0)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("algo,q_len", [("decode", 4), ("tcgen05", 150)])
+def test_non_finite_v_with_alibi_and_padded_rows(d, algo, q_len):
+    """ALiBi takes a sequence's blocks last to first."""
+    slopes = torch.tensor([0.3, -0.1, 0.02, 0.004], device=DEV)
+    lens = [900 - 23 * i for i in range(12)]
+    c = Case(torch.bfloat16, d, 4, 2, 48, q_len, lens, q_lens=[q_len - i % 4 for i in range(12)], seed=d)
+    poison = {b: (n - 1, n - 90, n // 128 * 128 - 1, 200) for b, n in enumerate(lens) if b % 2}
+    check_spread(c, poison, math.nan, algo=algo, alibi_slopes=slopes)
