@@ -412,7 +412,9 @@ LLMX_API llmx_status llmx_paged_store(const llmx_paged_cache *c, const llmx_kv4_
  * bits far into a sequence; lse is that of slope * position.  A NaN or an
  * infinity in a cached token reaches the rows that see the token and no
  * others; one in V may make such a row of o NaN as a whole, and shows in
- * neither lse nor key weights.
+ * neither lse nor key weights.  bf16 values of V are to stay below
+ * 2^64 / kv_len: their weighted sums are kept in fp32, before the division,
+ * with weights of up to 2^64.  A soft-capped score is right to 2^-20 of itself.
  *   With c->key_weights, the weight of every token j < kv_lens[b] of every kv
  * head becomes
  *   decay * (what was there) + sum of softmax(row)[j] over the query rows and

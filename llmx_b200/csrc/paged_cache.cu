@@ -11,8 +11,9 @@
 //            image of the fp32 weights, held in shared memory after one read)
 //            and writes the kept positions in ascending order;
 //   compact  moves the kept rows of K, V and the weights to the front.
-// 32 sequences of 2500-4096 tokens to 1024, 8 heads of 128: 64 us, 0.65 of the copy
-// rate; one of 131071 to 16384: 53 us, most of it the selection's rounds.
+// 32 sequences of 2500-4096 tokens to 1024, 8 heads of 128: 65 us, 0.64 of the copy
+// rate (in place 102); one of 131071 to 16384: 53 us (in place 121), 24 of it the
+// selection's rounds.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -562,8 +563,8 @@ cudaError_t launch_evict(const PagedArgs &a, const EvictArgs &e, int num_sms, cu
     m.col_ctas = 1;
     m.chunks = (most + m.batch - 1) / m.batch;
   } else {
-    // Both ways measured, us: 256 units of 1024 rows of head_dim 128 in 32 bytes 123,
-    // in 64 bytes 109; 8 units of 16384 rows 123 and 177.
+    // Both ways measured, us, with the selection: 256 units of 1024 rows of head_dim 128 in
+    // 32 bytes 119, in 64 bytes 102; 8 units of 16384 rows 121 and 289.
     m.pieces = units * (row_pieces / 4) >= 2LL * num_sms ? 4 : 2;
     m.batch = (m.pieces == 4 ? 256 : 512) * kInPlaceItems / (2 * m.pieces);
     m.col_ctas = row_pieces / m.pieces;

@@ -224,6 +224,9 @@ def paged_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch
     call reads), or without one of the sequence's own pages (which no other
     sequence may share).
 
+    A token whose page lies outside the cache ranks last and, if kept, becomes
+    zeros with weight 0.
+
     Returns (kept, new_lens): int32 [batch, n_kv_heads, budget], the former
     positions (-1 behind the kept ones), and int32 [batch].  Both may be given;
     ``new_lens`` may be ``kv_lens``."""
